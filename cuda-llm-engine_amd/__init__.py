@@ -174,6 +174,12 @@ _SIGS = {
     "llmk_empty_launch": (_i, [_i, _i, _vp]),
     "llmk_attention_decode_fast_workspace_floats": (_sz, [_i, _i, _i]),
     "llmk_argmax_rows": (_i, [_vp, _vp, _i, _i, _vp]),
+    "llmk_kv8_append": (_i, [_vp, _i] + [_vp] * 9 + [_i] * 7 + [_vp]),
+    "llmk_kv8_gather": (_i, [_vp] * 9 + [_i] * 6 + [_vp]),
+    "llmk_kv8_attention_workspace_floats": (_sz, [_i]),
+    "llmk_kv8_attention": (_i, [_vp] * 10 + [_i] * 8 + [_vp]),
+    "llmk_verify_drafts_workspace_floats": (_sz, [_i, _i, _i]),
+    "llmk_verify_drafts": (_i, [_vp] * 10 + [_i] * 3 + [_vp]),
     "llmk_attention_decode_fast": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
     "llmk_attention_decode_fast_noalloc": (_i, [_vp] * 6 + [_i] * 7 + [_vp]),
     "llmk_decode_nongemm_pass": (_i, [ctypes.POINTER(DecodePass), _vp]),
@@ -540,6 +546,177 @@ def argmax_rows(logits, out, n_rows: int, vocab: int, stream=None) -> None:
     pl = _dev(fn, logits, torch.float16, n_rows * vocab, "logits")
     po = _dev(fn, out, torch.int32, n_rows, "out")
     _check(fn, _lib.llmk_argmax_rows(pl, po, n_rows, vocab, _stream(stream)))
+
+
+# ---------------------------------------------------------------------------------------------
+# serving from an 8-bit KV cache
+# ---------------------------------------------------------------------------------------------
+KV8_DTYPE = torch.float8_e4m3fn  # of the K and V pools
+
+
+def _here(fn: str, **tensors) -> None:
+    """Refuses tensors of another device than the current one, whose stream the call would use."""
+    at = torch.cuda.current_device()
+    for name, t in tensors.items():
+        if t is not None and t.device.index != at:
+            _fail(fn, f"{name} is on {t.device}, the current device is cuda:{at}")
+
+
+def _opt(fn: str, t, dtype, min_numel: int, name: str):
+    return None if t is None else _dev(fn, t, dtype, min_numel, name)
+
+
+def _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, seq_lens, n_rows,
+               n_seqs, max_pages, page_size, n_kv_heads, head_dim, check):
+    """The pointers of a cache and a batch; with `check`, their values on the host as well. Returns
+    also the positions [first, end) of each sequence's rows then, else None."""
+    if min(n_rows, n_seqs) < 0 or min(max_pages, page_size, n_kv_heads, head_dim) <= 0:
+        _fail(fn, "n_rows and n_seqs must be >= 0 and the other sizes > 0")
+    pools = [_dev(fn, k_pool, KV8_DTYPE, 0, "k_pool"), _dev(fn, k_scale, torch.float32, 0, "k_scale"),
+             _dev(fn, v_pool, KV8_DTYPE, 0, "v_pool"), _dev(fn, v_scale, torch.float32, 0, "v_scale")]
+    for pool, scale, name in ((k_pool, k_scale, "k"), (v_pool, v_scale, "v")):
+        if pool.numel() != scale.numel() * page_size * head_dim or scale.numel() % n_kv_heads:
+            _fail(fn, f"{name}_pool must be [num_pages, {n_kv_heads}, {page_size}, {head_dim}] and "
+                      f"{name}_scale [num_pages, {n_kv_heads}]")
+    batch = [_dev(fn, block_tables, torch.int32, n_seqs * max_pages, "block_tables"),
+             _opt(fn, row_starts, torch.int32, n_seqs + 1, "row_starts"),
+             _dev(fn, seq_lens, torch.int32, n_seqs, "seq_lens")]
+    _here(fn, k_pool=k_pool, k_scale=k_scale, v_pool=v_pool, v_scale=v_scale,
+          block_tables=block_tables, row_starts=row_starts, seq_lens=seq_lens)
+    spans = None
+    if check and n_seqs > 0:
+        lens = seq_lens[:n_seqs].long()
+        _range_check(fn, seq_lens, n_seqs, -(1 << 31), max_pages * page_size + 1, "seq_lens")
+        counts = torch.ones_like(lens)
+        if row_starts is not None:
+            starts = row_starts[:n_seqs + 1].long()
+            counts = starts[1:] - starts[:-1]
+            if int(starts[0]) != 0 or bool((counts < 0).any()) or int(starts[-1]) > n_rows:
+                _fail(fn, f"row_starts must ascend from 0 to at most {n_rows}")
+        spans = (lens - counts).clamp(min=0), lens.clamp(min=0)
+    return pools, batch, spans
+
+
+def _kv8_pages(fn, spans, block_tables, n_seqs, max_pages, page_size, num_pages):
+    """Checks the table entries of positions [first, end) and returns them, sequence by sequence."""
+    first, end = spans
+    at = torch.arange(max_pages, device=first.device)[None, :]
+    used = (at >= (first // page_size)[:, None]) & (at < ((end + page_size - 1) // page_size)[:, None])
+    used &= (end > first)[:, None]
+    pages = block_tables.reshape(-1)[:n_seqs * max_pages].view(n_seqs, max_pages)[used]
+    _range_check(fn, pages, pages.numel(), 0, num_pages, "block_tables (addressed entries)")
+    return pages
+
+
+def kv8_append(qkv, ld: int, q_out, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
+               seq_lens, inv_freq, n_rows: int, n_seqs: int, max_pages: int, page_size: int,
+               n_heads: int, n_kv_heads: int, head_dim: int, stream=None,
+               check_indices: bool | None = None) -> None:
+    """RoPE of the rows' q and k, and k and v appended to the 8-bit cache (``llmk_kv8_append``).
+
+    Pools are torch.float8_e4m3fn [num_pages, n_kv_heads, 16, head_dim], scales float32
+    [num_pages, n_kv_heads]; row_starts None: one row a sequence. ``check_indices`` also refuses a
+    page that two sequences append to."""
+    fn = "kv8_append"
+    check = _want_checks(check_indices)
+    pools, batch, spans = _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
+                                     seq_lens, n_rows, n_seqs, max_pages, page_size, n_kv_heads,
+                                     head_dim, check)
+    if n_heads <= 0 or ld < (n_heads + 2 * n_kv_heads) * head_dim:
+        _fail(fn, "n_heads must be > 0 and ld >= (n_heads + 2 n_kv_heads) head_dim")
+    width = (n_heads + 2 * n_kv_heads) * head_dim
+    px = _dev(fn, qkv, torch.float16, (n_rows - 1) * ld + width if n_rows else 0, "qkv")
+    pq = _dev(fn, q_out, torch.float16, n_rows * n_heads * head_dim, "q_out")
+    pf = _dev(fn, inv_freq, torch.float32, head_dim // 2, "inv_freq")
+    _here(fn, qkv=qkv, q_out=q_out, inv_freq=inv_freq)
+    if spans is not None:
+        pages = _kv8_pages(fn, spans, block_tables, n_seqs, max_pages, page_size,
+                           k_scale.numel() // n_kv_heads)
+        if pages.unique().numel() != pages.numel():
+            _fail(fn, "two sequences append to the same page")
+    _check(fn, _lib.llmk_kv8_append(px, ld, pq, *pools, *batch, pf, n_rows, n_seqs, max_pages,
+                                    page_size, n_heads, n_kv_heads, head_dim, _stream(stream)))
+
+
+def kv8_gather(k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, seq_lens, k_out, v_out,
+               n_rows: int, n_seqs: int, max_pages: int, page_size: int, n_kv_heads: int,
+               head_dim: int, stream=None, check_indices: bool | None = None) -> None:
+    """The last cached rows of each sequence as fp16 (``llmk_kv8_gather``; arguments as
+    kv8_append's)."""
+    fn = "kv8_gather"
+    pools, batch, spans = _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
+                                     seq_lens, n_rows, n_seqs, max_pages, page_size, n_kv_heads,
+                                     head_dim, _want_checks(check_indices))
+    pk = _dev(fn, k_out, torch.float16, n_rows * n_kv_heads * head_dim, "k_out")
+    pv = _dev(fn, v_out, torch.float16, n_rows * n_kv_heads * head_dim, "v_out")
+    _here(fn, k_out=k_out, v_out=v_out)
+    if spans is not None:
+        _kv8_pages(fn, spans, block_tables, n_seqs, max_pages, page_size,
+                   k_scale.numel() // n_kv_heads)
+    _check(fn, _lib.llmk_kv8_gather(*pools, *batch, pk, pv, n_rows, n_seqs, max_pages, page_size,
+                                    n_kv_heads, head_dim, _stream(stream)))
+
+
+def kv8_attention_workspace_floats(head_dim: int) -> int:
+    return int(_lib.llmk_kv8_attention_workspace_floats(head_dim))
+
+
+def kv8_attention(q, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, seq_lens, out,
+                  workspace, n_rows: int, n_seqs: int, max_rows: int, max_pages: int,
+                  page_size: int, n_heads: int, n_kv_heads: int, head_dim: int, stream=None,
+                  check_indices: bool | None = None) -> None:
+    """Causal attention of the rows over the 8-bit cache (``llmk_kv8_attention``; cache and batch as
+    kv8_append's). workspace None: every sequence stays whole, for short contexts."""
+    fn = "kv8_attention"
+    pools, batch, spans = _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
+                                     seq_lens, n_rows, n_seqs, max_pages, page_size, n_kv_heads,
+                                     head_dim, _want_checks(check_indices))
+    pq = _dev(fn, q, torch.float16, n_rows * n_heads * head_dim, "q")
+    po = _dev(fn, out, torch.float16, n_rows * n_heads * head_dim, "out")
+    pw = _opt(fn, workspace, torch.float32, kv8_attention_workspace_floats(head_dim), "workspace")
+    _here(fn, q=q, out=out, workspace=workspace)
+    if spans is not None:
+        _kv8_pages(fn, (torch.zeros_like(spans[0]), spans[1]), block_tables, n_seqs, max_pages,
+                   page_size, k_scale.numel() // n_kv_heads)
+    _check(fn, _lib.llmk_kv8_attention(pq, *pools, *batch, po, pw, n_rows, n_seqs, max_rows,
+                                       max_pages, page_size, n_heads, n_kv_heads, head_dim,
+                                       _stream(stream)))
+
+
+def verify_drafts_workspace_floats(n_rows: int, n_seqs: int, vocab: int) -> int:
+    return int(_lib.llmk_verify_drafts_workspace_floats(n_rows, n_seqs, vocab))
+
+
+def verify_drafts(logits, draft_logits, drafts, row_starts, temperature, accept_u, sample_u,
+                  n_accepted, tokens, workspace, n_rows: int, n_seqs: int, vocab: int,
+                  stream=None, check_indices: bool | None = None) -> None:
+    """Which drafted tokens stand against the target's probabilities, and the token behind them
+    (``llmk_verify_drafts``). draft_logits None: drafts count as certain; temperature None: 1;
+    row_starts None: one row a sequence and no drafts (drafts and accept_u may be None)."""
+    fn = "verify_drafts"
+    if min(n_rows, n_seqs) < 0 or vocab <= 0:
+        _fail(fn, "n_rows and n_seqs must be >= 0 and vocab > 0")
+    given = n_rows if row_starts is not None else 0  # of drafts and their numbers
+    ptrs = [_dev(fn, logits, torch.float16, n_rows * vocab, "logits"),
+            _opt(fn, draft_logits, torch.float16, given * vocab, "draft_logits"),
+            _opt(fn, drafts, torch.int32, given, "drafts"),
+            _opt(fn, row_starts, torch.int32, n_seqs + 1, "row_starts"),
+            _opt(fn, temperature, torch.float32, n_seqs, "temperature"),
+            _opt(fn, accept_u, torch.float32, given, "accept_u"),
+            _dev(fn, sample_u, torch.float32, n_seqs, "sample_u"),
+            _dev(fn, n_accepted, torch.int32, n_seqs, "n_accepted"),
+            _dev(fn, tokens, torch.int32, n_rows, "tokens"),
+            _dev(fn, workspace, torch.float32,
+                 verify_drafts_workspace_floats(n_rows, n_seqs, vocab), "workspace")]
+    _here(fn, logits=logits, draft_logits=draft_logits, drafts=drafts, row_starts=row_starts,
+          temperature=temperature, accept_u=accept_u, sample_u=sample_u, n_accepted=n_accepted,
+          tokens=tokens, workspace=workspace)
+    if _want_checks(check_indices) and row_starts is not None:
+        starts = row_starts[:n_seqs + 1].long()
+        if (int(starts[0]) != 0 or bool((starts[1:] < starts[:-1]).any())
+                or int(starts[-1]) > n_rows):
+            _fail(fn, f"row_starts must ascend from 0 to at most {n_rows}")
+    _check(fn, _lib.llmk_verify_drafts(*ptrs, n_rows, n_seqs, vocab, _stream(stream)))
 
 
 def copy_bytes(src, dst, nbytes: int, stream=None) -> None:

@@ -1,0 +1,319 @@
+// Writing and reading the 8-bit KV cache (layout: kv8.hpp): the append of a pass's keys and values
+// with the rotation of q and k on the way, and the read-back of cached rows as fp16.
+//
+// Append. The rotation of row at position pos, pair i < head_dim / 2 (element i with element
+// i + head_dim / 2): angle = pos * inv_freq[i] in 64 bits, c and s its cosine and sine in 32,
+// x1' = x1 c - x2 s, x2' = x2 c + x1 s in 32 bits. q is rounded once, to fp16; k and v once, to
+// e4m3 under the scale of their block. For the rows of the call that fall into one block (a page
+// and kv head, K or V):
+//   most  = the largest finite magnitude among them;
+//   e     = the least exponent in [-15, 7] with most <= 448 * 2^e, or the block's own if that is
+//           larger and the block holds tokens already (the first slot written is not its slot 0);
+//   slots in front of the first one written are rounded again where e grew.
+// So a block that is begun anew forgets its scale, and rows that are appended over others (drafted
+// tokens that were refused) only ever find it as large as those needed.
+//
+// Work split: a block of 256 threads for each row; the rows that open a page of their sequence, or
+// the call, also write K and V of all rows that follow them in the page. There a wave holds up to
+// 16 rows x head_dim / 16 pieces of one (kv head, K or V), and more heads side by side where the
+// page gets fewer rows, so that the maximum is a few lane exchanges and nothing is read twice.
+#include <math.h>
+
+#include "kv8.hpp"
+
+namespace llmk {
+namespace {
+
+using namespace kv8;
+
+// Cosine and sine of an angle in 64 bits, to 32. The quarter turns are taken off in 64 bits (the
+// angles of far positions lose their fraction in 32); what is left, at most pi / 4, goes through
+// the series of both, which end below 2^-29 there.
+__device__ __forceinline__ f32x2 cos_sin(double angle) {
+  const double k = __builtin_rint(angle * 0.63661977236758134308);
+  double rest = __builtin_fma(-k, 1.57079632679489655800, angle);
+  rest = __builtin_fma(-k, 6.12323399573676603587e-17, rest);
+  const float r = (float)rest, z = r * r;
+  float s = __builtin_fmaf(z, 2.75573192e-6f, -1.98412698e-4f);
+  s = __builtin_fmaf(z, s, 8.33333333e-3f);
+  s = __builtin_fmaf(z, s, -1.66666667e-1f);
+  s = __builtin_fmaf(r * z, s, r);
+  float c = __builtin_fmaf(z, -2.75573192e-7f, 2.48015873e-5f);
+  c = __builtin_fmaf(z, c, -1.38888889e-3f);
+  c = __builtin_fmaf(z, c, 4.16666667e-2f);
+  c = __builtin_fmaf(z, c, -0.5f);
+  c = __builtin_fmaf(z, c, 1.0f);
+  const int q = (int)k & 3;
+  const float cq = (q & 1) ? s : c, sq = (q & 1) ? c : s;
+  return f32x2{q == 1 || q == 2 ? -cq : cq, q >= 2 ? -sq : sq};
+}
+
+struct AppendArgs {
+  Batch batch;
+  const f16* qkv;
+  f16* q_out;
+  uint8_t* pool[2];  // K, V
+  float* scale[2];
+  const float* inv_freq;
+  int ld, n_heads, n_kv_heads;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a) {
+  constexpr int HALF = HD / 2, P = HD / 16;  // P pieces of a row: elements 8 p .. and HALF + 8 p ..
+  constexpr int J = P * kPage / 64;          // rows of a lane where a page gets all 16
+  __shared__ f32x2 turn[kPage][HALF];
+  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int s = __builtin_amdgcn_readfirstlane(find_seq(a.batch.starts, a.batch.n_seqs, row));
+  if (s < 0) return;
+  int i = 0, count = 1;
+  if (a.batch.starts) {
+    i = row - a.batch.starts[s];
+    count = a.batch.starts[s + 1] - a.batch.starts[s];
+  }
+  const long long pos = (long long)a.batch.lens[s] - count + i;
+  const bool in_table = pos >= 0 && pos < (long long)a.batch.max_pages * kPage;
+  const int slot = (int)(pos & (kPage - 1));
+  int n = 0;  // rows whose K and V this block writes
+  if (in_table && (i == 0 || slot == 0)) {
+    n = kPage - slot;
+    n = n < count - i ? n : count - i;
+    n = n < a.batch.n_rows - row ? n : a.batch.n_rows - row;
+  }
+  for (int t = tid; t < (n > 1 ? n : 1) * HALF; t += 256)
+    turn[t / HALF][t % HALF] =
+        cos_sin((double)(pos + t / HALF) * (double)a.inv_freq[t % HALF]);
+  __syncthreads();
+
+  // q of this row; zeros where its position lies outside the table
+  const f16* src = a.qkv + (size_t)row * a.ld;
+  for (int t = tid; t < a.n_heads * P; t += 256) {
+    const size_t at = (size_t)(t / P) * HD + (t % P) * 8;
+    const f16x8 x1 = as_h8(ld16(src + at)), x2 = as_h8(ld16(src + at + HALF));
+    f16x8 y1, y2;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const f32x2 cs = turn[0][(t % P) * 8 + e];
+      const float u = (float)x1[e], w = (float)x2[e];
+      y1[e] = in_table ? (f16)(u * cs.x - w * cs.y) : (f16)0;
+      y2[e] = in_table ? (f16)(w * cs.x + u * cs.y) : (f16)0;
+    }
+    f16* dst = a.q_out + (size_t)row * a.n_heads * HD + at;
+    st16(dst, as_u4(y1));
+    st16(dst + HALF, as_u4(y2));
+  }
+  if (n == 0) return;
+
+  const size_t page = (size_t)a.batch.tables[(size_t)s * a.batch.max_pages + pos / kPage];
+  int per = P;  // lanes of one unit, a (kv head, K or V): P for each row, rows to a power of two
+  while (per < P * n && per < 64) per *= 2;
+  const int units = 2 * a.n_kv_heads, mine = lane & (per - 1);
+  const int r0 = mine / P, p = mine % P;
+  for (int first = wave * (64 / per); first < units; first += 4 * (64 / per)) {
+    const int unit = first + lane / per;
+    const bool live = unit < units;
+    const int side = live && unit >= a.n_kv_heads, h = live ? unit - side * a.n_kv_heads : 0;
+    const f16* from =
+        a.qkv + (size_t)(a.n_heads + side * a.n_kv_heads + h) * HD + 8 * p + (size_t)row * a.ld;
+    float* const scale = a.scale[side] + page * a.n_kv_heads + h;
+    uint8_t* const block = a.pool[side] + (page * a.n_kv_heads + h) * (size_t)(kPage * HD);
+    const int before = live && slot > 0 ? exponent_of(*scale) : kMinExp;
+    float x[J][16];
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int r = r0 + j * (64 / P);
+      if (!live || r >= n) continue;
+      const f16x8 x1 = as_h8(ld16(from + (size_t)r * a.ld));
+      const f16x8 x2 = as_h8(ld16(from + (size_t)r * a.ld + HALF));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float u = (float)x1[e], w = (float)x2[e];
+        if (side == 0) {
+          const f32x2 cs = turn[r][8 * p + e];
+          x[j][e] = u * cs.x - w * cs.y;
+          x[j][8 + e] = w * cs.x + u * cs.y;
+        } else {
+          x[j][e] = u;
+          x[j][8 + e] = w;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const float m = __builtin_fabsf(x[j][e]);
+        most = m < INFINITY && m > most ? m : most;
+      }
+    }
+    for (int d = 1; d < per; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
+    int e = scale_exponent(most);
+    e = e > before ? e : before;
+    const float down = exp2_int(-e);
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int r = r0 + j * (64 / P);
+      if (!live || r >= n) continue;
+      uint8_t* dst = block + (slot + r) * HD + 8 * p;
+#pragma unroll
+      for (int g = 0; g < 2; ++g) {
+        uint2 v;
+        v.x = to_e4m3(x[j][8 * g] * down, x[j][8 * g + 1] * down, x[j][8 * g + 2] * down,
+                      x[j][8 * g + 3] * down);
+        v.y = to_e4m3(x[j][8 * g + 4] * down, x[j][8 * g + 5] * down, x[j][8 * g + 6] * down,
+                      x[j][8 * g + 7] * down);
+        *reinterpret_cast<uint2*>(dst + g * HALF) = v;
+      }
+    }
+    if (live && slot > 0 && e > before) {  // the tokens held already, under the new scale
+      const float shift = exp2_int(before - e);
+      for (int v = mine; v < slot * HD / 16; v += per) {
+        u32x4 held = ld16(block + 16 * v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t b = elem(held, k);
+          const f32x2 lo = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8(b, false));
+          const f32x2 hi = __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8(b, true));
+          held[k] = to_e4m3(lo.x * shift, lo.y * shift, hi.x * shift, hi.y * shift);
+        }
+        st16(block + 16 * v, held);
+      }
+    }
+    if (live && mine == 0) *scale = exp2_int(e);
+  }
+}
+
+// Read-back: each block takes 16 rows; a thread takes 16 values of one row at a time.
+constexpr int kGatherRows = 16;
+
+struct GatherArgs {
+  Batch batch;
+  const uint8_t* pool[2];
+  const float* scale[2];
+  f16* out[2];
+  int n_kv_heads;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv8_gather(const GatherArgs a) {
+  constexpr int P = HD / 16;
+  __shared__ long long block_of[kGatherRows];  // page, -1: no position, -2: a row of no sequence
+  __shared__ int slot_of[kGatherRows];
+  const int row0 = blockIdx.x * kGatherRows, tid = threadIdx.x;
+  const int s0 = find_seq(a.batch.starts, a.batch.n_seqs, row0);
+  if (tid < kGatherRows) {
+    const int row = row0 + tid;
+    int s = -1;
+    if (row < a.batch.n_rows && s0 >= 0)
+      s = a.batch.starts ? find_seq_from(a.batch.starts, a.batch.n_seqs, s0, row)
+                         : (row < a.batch.n_seqs ? row : -1);
+    long long page = -2;
+    if (s >= 0) {
+      const long long back = a.batch.starts ? (long long)a.batch.starts[s + 1] - row : 1;
+      const long long pos = a.batch.lens[s] - back;
+      const bool in_table = pos >= 0 && pos < (long long)a.batch.max_pages * kPage;
+      page = in_table ? a.batch.tables[(size_t)s * a.batch.max_pages + pos / kPage] : -1;
+      slot_of[tid] = (int)(pos & (kPage - 1));
+    }
+    block_of[tid] = page;
+  }
+  __syncthreads();
+  const int per_side = kGatherRows * P * a.n_kv_heads;
+  for (int t = tid; t < 2 * per_side; t += 256) {
+    const int side = t >= per_side, u = t - side * per_side;
+    const int r = u / P % kGatherRows, p = u % P, h = u / (P * kGatherRows);
+    const long long page = block_of[r];
+    if (page == -2) continue;
+    u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
+    if (page >= 0) {
+      const size_t block = (size_t)page * a.n_kv_heads + h;
+      const u32x4 b = ld16(a.pool[side] + (block * kPage + slot_of[r]) * HD + 16 * p);
+      const float scale = a.scale[side][block];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t w = elem(b, k);
+        const uint32_t x = __builtin_bit_cast(uint32_t, from_e4m3<false>(w, scale));
+        const uint32_t y = __builtin_bit_cast(uint32_t, from_e4m3<true>(w, scale));
+        if (k < 2) { lo[2 * k] = x; lo[2 * k + 1] = y; }
+        else { hi[2 * k - 4] = x; hi[2 * k - 3] = y; }
+      }
+    }
+    f16* dst = a.out[side] + ((size_t)(row0 + r) * a.n_kv_heads + h) * HD + 16 * p;
+    st16(dst, lo);
+    st16(dst + 8, hi);
+  }
+}
+
+int check_batch(int n_rows, int n_seqs, int max_pages, int page_size, int n_kv_heads, int head_dim,
+                const int32_t* row_starts) {
+  if (n_rows < 0 || n_seqs < 0 || max_pages <= 0 || n_kv_heads <= 0 || head_dim <= 0)
+    return LLMK_ERR_INVALID_VALUE;
+  if (!row_starts && n_rows != n_seqs) return LLMK_ERR_INVALID_VALUE;
+  if (page_size != kPage || (head_dim != 64 && head_dim != 128)) return LLMK_ERR_SHAPE;
+  return LLMK_OK;
+}
+
+}  // namespace
+}  // namespace llmk
+
+using namespace llmk;
+
+extern "C" int llmk_kv8_append(const uint16_t* qkv, int ld, uint16_t* q_out, uint8_t* k_pool,
+                               float* k_scale, uint8_t* v_pool, float* v_scale,
+                               const int32_t* block_tables, const int32_t* row_starts,
+                               const int32_t* seq_lens, const float* inv_freq, int n_rows,
+                               int n_seqs, int max_pages, int page_size, int n_heads,
+                               int n_kv_heads, int head_dim, void* stream) {
+  const int st = check_batch(n_rows, n_seqs, max_pages, page_size, n_kv_heads, head_dim, row_starts);
+  if (st != LLMK_OK) return st;
+  if (n_heads <= 0) return LLMK_ERR_INVALID_VALUE;
+  if ((long long)ld < ((long long)n_heads + 2LL * n_kv_heads) * head_dim || ld % 8 != 0)
+    return LLMK_ERR_SHAPE;
+  if (n_rows == 0 || n_seqs == 0) return LLMK_OK;
+  if (!qkv || !q_out || !k_pool || !k_scale || !v_pool || !v_scale || !block_tables || !seq_lens ||
+      !inv_freq)
+    return LLMK_ERR_INVALID_VALUE;
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_pool) || !aligned16(v_pool))
+    return LLMK_ERR_ALIGNMENT;
+  AppendArgs a;
+  a.batch = kv8::Batch{block_tables, row_starts, seq_lens, n_rows, n_seqs, max_pages};
+  a.qkv = reinterpret_cast<const f16*>(qkv);
+  a.q_out = reinterpret_cast<f16*>(q_out);
+  a.pool[0] = k_pool;
+  a.pool[1] = v_pool;
+  a.scale[0] = k_scale;
+  a.scale[1] = v_scale;
+  a.inv_freq = inv_freq;
+  a.ld = ld;
+  a.n_heads = n_heads;
+  a.n_kv_heads = n_kv_heads;
+  return launch(head_dim == 64 ? k_kv8_append<64> : k_kv8_append<128>, dim3((unsigned)n_rows),
+                dim3(256), 0, static_cast<hipStream_t>(stream), a);
+}
+
+extern "C" int llmk_kv8_gather(const uint8_t* k_pool, const float* k_scale, const uint8_t* v_pool,
+                               const float* v_scale, const int32_t* block_tables,
+                               const int32_t* row_starts, const int32_t* seq_lens,
+                               uint16_t* k_out, uint16_t* v_out, int n_rows, int n_seqs,
+                               int max_pages, int page_size, int n_kv_heads, int head_dim,
+                               void* stream) {
+  const int st = check_batch(n_rows, n_seqs, max_pages, page_size, n_kv_heads, head_dim, row_starts);
+  if (st != LLMK_OK) return st;
+  if (n_kv_heads > 65536) return LLMK_ERR_UNSUPPORTED;  // a block's share is counted in 32 bits
+  if (n_rows == 0 || n_seqs == 0) return LLMK_OK;
+  if (!k_pool || !k_scale || !v_pool || !v_scale || !block_tables || !seq_lens || !k_out || !v_out)
+    return LLMK_ERR_INVALID_VALUE;
+  if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned16(k_out) || !aligned16(v_out))
+    return LLMK_ERR_ALIGNMENT;
+  GatherArgs a;
+  a.batch = kv8::Batch{block_tables, row_starts, seq_lens, n_rows, n_seqs, max_pages};
+  a.pool[0] = k_pool;
+  a.pool[1] = v_pool;
+  a.scale[0] = k_scale;
+  a.scale[1] = v_scale;
+  a.out[0] = reinterpret_cast<f16*>(k_out);
+  a.out[1] = reinterpret_cast<f16*>(v_out);
+  a.n_kv_heads = n_kv_heads;
+  return launch(head_dim == 64 ? k_kv8_gather<64> : k_kv8_gather<128>,
+                dim3(ceil_div((size_t)n_rows, (size_t)kGatherRows)), dim3(256), 0,
+                static_cast<hipStream_t>(stream), a);
+}

@@ -283,6 +283,101 @@ LLMK_API int llmk_decode_nongemm_pass_layers(const llmk_decode_pass* pass, void*
 LLMK_API int llmk_decode_nongemm_pass_fused(const llmk_decode_pass* pass, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Serving from an 8-bit KV cache: append, attention, read-back, and the verification of drafted
+ * tokens. New entry points; the reference's cache is fp16 and it decodes one token at a time.
+ *
+ * The cache: K and V pools [num_pages, n_kv_heads, 16, head_dim] of e4m3 bytes (OCP: largest 448, no
+ * infinities) and their scales [num_pages, n_kv_heads], floats that are powers of two from 2^-15
+ * to 2^7: value = e4m3 * scale, which is an fp16 exactly. 1 byte a value where the fp16 pools take 2.
+ * head_dim 64 or 128, page size 16. Unwritten pages may hold anything.
+ *
+ * One description of a batch for all of them: sequence s < n_seqs owns the rows row_starts[s] ..
+ * row_starts[s + 1] - 1 of the call (row_starts: n_seqs + 1 ascending entries from 0; NULL: one row
+ * for each sequence, n_rows == n_seqs), any number from none: a decode step's one, a few drafted
+ * ones, a prompt's. seq_lens[s] is what the sequence holds once they are in, and they are its last:
+ * row i of c stands at position seq_lens[s] - c + i, in page block_tables[s * max_pages + position /
+ * 16]. Rows at row_starts[n_seqs] and behind belong to none: what they would give is left as it was.
+ * Positions below 0 or past the table are nowhere: not written, and read as nothing. Page numbers
+ * are not range-checked. Pools, q, qkv and outputs are 16-byte aligned.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Appends the rows' keys and values, the keys rotated, and rotates their queries. Row r of qkv
+ * (stride ld elements) holds q [n_heads, head_dim], k [n_kv_heads, head_dim] and v behind one
+ * another, as llmk_qkv_rope_scatter's; q_out [n_rows, n_heads, head_dim] must not overlap it.
+ * Rotation as llmk_rope_apply, but unrounded on the way: angles position * inv_freq in 64 bits,
+ * cosine, sine and products in 32, then q rounded once to fp16, k and v once to e4m3 (q of a row
+ * at a position that is nowhere is zero).
+ * The scale of a block (page and kv head): the least 2^e, e from -15 to 7, with most <= 448 * 2^e for
+ * most the largest finite magnitude of the call's rows in it. Where the first of them is not the
+ * page's token 0, the scale is not lowered, and if it grows the tokens in front are rounded again to
+ * it. Tokens behind are left as they are: appending over refused drafts is a plain append. Magnitudes
+ * past 57344 are held as 57344, infinities and NaN as NaN. No two sequences of a call may append to
+ * the same page. ld % 8 == 0, ld >= (n_heads + 2 n_kv_heads) head_dim. */
+LLMK_API int llmk_kv8_append(const uint16_t* qkv, int ld, uint16_t* q_out, uint8_t* k_pool,
+                             float* k_scale, uint8_t* v_pool, float* v_scale,
+                             const int32_t* block_tables, const int32_t* row_starts,
+                             const int32_t* seq_lens, const float* inv_freq, int n_rows,
+                             int n_seqs, int max_pages, int page_size, int n_heads,
+                             int n_kv_heads, int head_dim, void* stream);
+
+/* The cached rows as fp16 (exact), the last ones of each sequence: k_out, v_out [n_rows, n_kv_heads,
+ * head_dim]; rows that are nowhere give zeros. n_kv_heads <= 65536. */
+LLMK_API int llmk_kv8_gather(const uint8_t* k_pool, const float* k_scale, const uint8_t* v_pool,
+                             const float* v_scale, const int32_t* block_tables,
+                             const int32_t* row_starts, const int32_t* seq_lens,
+                             uint16_t* k_out, uint16_t* v_out, int n_rows, int n_seqs,
+                             int max_pages, int page_size, int n_kv_heads, int head_dim,
+                             void* stream);
+
+/* Floats of workspace llmk_kv8_attention needs, for any batch; 0 for a head_dim it does not take. */
+LLMK_API size_t llmk_kv8_attention_workspace_floats(int head_dim);
+
+/* Causal attention of the rows over the cache: out[r, h, :] = softmax_j(q[r, h, :] . K_j /
+ * sqrt(head_dim)) . V_j over the positions j <= the row's own, kv head h / (n_heads / n_kv_heads). q
+ * and out [n_rows, n_heads, head_dim], n_heads any multiple of n_kv_heads. Scores, weights and sums
+ * in fp32, the result rounded once. A row that sees no position gets zeros. A NaN that a row sees
+ * makes it NaN; what a row does not see does not touch it. max_rows: the most rows that a sequence
+ * has in this call; it only chooses kernels (more rows than that are slow, not wrong). `workspace`
+ * (llmk_kv8_attention_workspace_floats(head_dim) floats, 16-byte aligned) lets the positions of a
+ * batch be shared out evenly, with a second launch that joins their parts; NULL for contexts that are
+ * short: every sequence then stays whole. Calls that may overlap need a workspace each. */
+LLMK_API int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, const float* k_scale,
+                                const uint8_t* v_pool, const float* v_scale,
+                                const int32_t* block_tables, const int32_t* row_starts,
+                                const int32_t* seq_lens, uint16_t* out, float* workspace,
+                                int n_rows, int n_seqs, int max_rows, int max_pages,
+                                int page_size, int n_heads, int n_kv_heads, int head_dim,
+                                void* stream);
+
+/* Floats of workspace llmk_verify_drafts needs; 0 for non-positive arguments. */
+LLMK_API size_t llmk_verify_drafts_workspace_floats(int n_rows, int n_seqs, int vocab);
+
+/* Which drafted tokens stand, and the token behind them (speculative decoding; with row_starts NULL,
+ * one row a sequence and no drafts, plain sampling). Of the c rows of sequence s, row i holds in
+ * logits [n_rows, vocab] what the target gives behind the sequence's first i drafts, and drafts[row]
+ * is the draft it judges; the last row judges none (its entry is not read). draft_logits [n_rows,
+ * vocab], or NULL: what the draft model drew each draft from (last rows are not read); without them
+ * a draft counts as certain. temperature [n_seqs], or NULL for 1.
+ * With p = softmax(logits / t) and q = softmax(draft_logits / t), drafts are accepted in order while
+ * accept_u[row] * q(draft) < p(draft). The first row refused gives a token of max(p - q, 0) (of p if
+ * that is 0 everywhere), the last row one of p: the lowest v with weight_0 + .. + weight_v >
+ * sample_u[s] * total. Numbers of accept_u [n_rows] and sample_u [n_seqs] lie in [0, 1).
+ * Exponentials and sums in 64 bits. t <= 0 or NaN: greedy, a draft stands where it is its row's
+ * argmax (the lowest place), which is also the token. NaN logits count as -inf, places of +inf share
+ * all probability; a draft outside [0, vocab) is refused.
+ * n_accepted [n_seqs]: drafts that stand. tokens [n_rows]: for each sequence those, the token, then
+ * -1; -1 also for the token where a row has nothing above -inf.
+ * workspace: 16-byte aligned; calls that may overlap need one each. drafts and accept_u may be NULL
+ * with row_starts. Any vocab and alignment of logits (16-byte vectors throughout where vocab % 8 ==
+ * 0). */
+LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_logits,
+                                const int32_t* drafts, const int32_t* row_starts,
+                                const float* temperature, const float* accept_u,
+                                const float* sample_u, int32_t* n_accepted, int32_t* tokens,
+                                float* workspace, int n_rows, int n_seqs, int vocab,
+                                void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * The decode step around the kernels above: projections, the fused layouts they
  * produce, and an engine that runs a whole Llama-3 forward pass over a batch of token rows.
  * ------------------------------------------------------------------------------------------ */
