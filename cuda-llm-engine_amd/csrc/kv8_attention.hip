@@ -1,8 +1,5 @@
 // Attention over the 8-bit KV cache (layout: kv8.hpp): out = softmax_j(q . K_j / sqrt(head_dim)) V_j
 // over the positions j up to the row's own, for rows of any number a sequence.
-//
-// One wave for each (row, query head): 64 positions at a time, one to a lane for the scores, then
-// one dim to a lane for the sums. Scores, weights and sums in 32 bits.
 #include <math.h>
 
 #include "kv8.hpp"
@@ -12,7 +9,23 @@ namespace {
 
 using namespace kv8;
 
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kStep = 64;                       // positions of a step: four pages
 constexpr float kLog2e = 1.44269504088896341f;
+constexpr int kSlotColumns = 65536;             // of partial results in the workspace
+constexpr int kWorkers = 2048;                  // at most
+
+// What a worker leaves for the launch that joins parts: the unit that begins in its share and ends in
+// another's.
+struct Open {
+  int last;   // the worker that ends it; -1: there is none
+  int column, columns;  // of the tile, from the sequence's first row on
+  int seq, head;        // kv head
+  int pad[3];
+};
 
 struct AttentionArgs {
   Batch batch;
@@ -22,71 +35,536 @@ struct AttentionArgs {
   const uint8_t* v_pool;
   const float* v_scale;
   f16* out;
-  int n_heads, n_kv_heads;
+  float* parts;  // [2 workers][columns of a tile][HD], NULL: no unit is shared
+  float2* parts_ml;
+  Open* open;
+  int n_heads, n_kv_heads, group, log_workers, min_steps;
 };
 
-template <int HD>
-__global__ void __launch_bounds__(256) k_kv8_attention_rows(const AttentionArgs a) {
-  const int row = blockIdx.x, lane = threadIdx.x & 63;
-  const int head = blockIdx.y * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int s = __builtin_amdgcn_readfirstlane(find_seq(a.batch.starts, a.batch.n_seqs, row));
-  if (s < 0 || head >= a.n_heads) return;
-  const long long back = a.batch.starts ? (long long)a.batch.starts[s + 1] - row : 1;
-  long long see = a.batch.lens[s] - back + 1;  // positions that the row sees
+// A sequence's rows in this call and what they see.
+struct Seq {
+  int row0, columns;  // columns: (row, query head of the group) pairs, row by row
+  long long before;   // position of the first row
+  long long limit;    // positions that exist
+};
+__device__ __forceinline__ Seq seq_of(const AttentionArgs& a, int s) {
+  Seq q;
+  int r0 = s, r1 = s + 1;
+  if (a.batch.starts) {
+    r0 = a.batch.starts[s];
+    r1 = a.batch.starts[s + 1];
+  }
+  const int len = a.batch.lens[s];
+  q.before = (long long)len - (r1 - r0);
+  r0 = r0 < 0 ? 0 : r0;
+  r1 = r1 > a.batch.n_rows ? a.batch.n_rows : r1;
+  q.row0 = r0;
+  q.columns = r1 > r0 ? (r1 - r0) * a.group : 0;
   const long long table = (long long)a.batch.max_pages * kPage;
-  see = see < table ? see : table;
-  const int kvh = head / (a.n_heads / a.n_kv_heads);
-  const int* pages = a.batch.tables + (size_t)s * a.batch.max_pages;
-  const f16* q = a.q + ((size_t)row * a.n_heads + head) * HD;
-  const float scale = 1.0f / __builtin_sqrtf((float)HD);
+  q.limit = len < table ? len : table;
+  return q;
+}
+// Positions that the row of a column sees.
+__device__ __forceinline__ int seen(const AttentionArgs& a, const Seq& q, int column) {
+  const long long n = q.before + column / a.group + 1;
+  const long long m = n < q.limit ? n : q.limit;
+  return m < 0 ? 0 : (int)m;
+}
+// Steps of a tile: those of its last row; one for a tile that sees nothing, which writes zeros.
+template <int C>
+__device__ __forceinline__ int tile_steps(const AttentionArgs& a, const Seq& q, int tile) {
+  const int last = (tile + 1) * C < q.columns ? (tile + 1) * C - 1 : q.columns - 1;
+  const int n = (seen(a, q, last) + kStep - 1) / kStep;
+  return n > 0 ? n : 1;
+}
+template <int C>
+__device__ __forceinline__ long long seq_steps(const AttentionArgs& a, int s) {
+  const Seq q = seq_of(a, s);
+  long long n = 0;
+  for (int t = 0; t * C < q.columns; ++t) n += tile_steps<C>(a, q, t);
+  return n * a.n_kv_heads;
+}
 
-  float m = -INFINITY, l = 0.0f, acc[HD / 64];
-  for (int d = 0; d < HD / 64; ++d) acc[d] = 0.0f;
-  for (long long base = 0; base < see; base += 64) {
-    const long long pos = base + lane;
-    float x = -INFINITY;
-    if (pos < see) {
-      const size_t block = (size_t)pages[pos / kPage] * a.n_kv_heads + kvh;
-      const uint8_t* k = a.k_pool + (block * kPage + pos % kPage) * HD;
-      const float ks = a.k_scale[block];
-      float dot = 0.0f;
-      for (int v = 0; v < HD / 16; ++v) {
-        const u32x4 b = ld16(k + 16 * v);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const f16x2 lo = from_e4m3<false>(elem(b, c), ks), hi = from_e4m3<true>(elem(b, c), ks);
-          const f16* qv = q + 16 * v + 4 * c;
-          dot = __builtin_fmaf((float)qv[0], (float)lo[0], dot);
-          dot = __builtin_fmaf((float)qv[1], (float)lo[1], dot);
-          dot = __builtin_fmaf((float)qv[2], (float)hi[0], dot);
-          dot = __builtin_fmaf((float)qv[3], (float)hi[1], dot);
-        }
+// Where the share of each of a block's workers begins among the steps of all units, which are
+// ordered by sequence, tile and kv head. By all 256 threads.
+struct Share {
+  long long total;
+  int log;  // workers: 2^log
+  long long begin, end;  // of this wave
+  int seq;               // that holds begin, and begin's place in it
+  long long at;
+};
+template <int C>
+__device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, int log_workers) {
+  __shared__ long long wave_sum_[4], at_[4];
+  __shared__ int seq_[4];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = a.batch.n_seqs, per = (n + 255) / 256;
+  const int s0 = tid * per, s1 = s0 + per < n ? s0 + per : n;
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) mine += seq_steps<C>(a, s);
+  long long upto = mine;
+  for (int d = 1; d < 64; d *= 2) {
+    const long long o = __shfl_up(upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 63) wave_sum_[wave] = upto;
+  __syncthreads();
+  Share r;
+  long long base = 0;
+  r.total = 0;
+  for (int w = 0; w < 4; ++w) {
+    if (w < wave) base += wave_sum_[w];
+    r.total += wave_sum_[w];
+  }
+  r.log = log_workers;
+  while (r.log > 0 && (r.total >> r.log) < a.min_steps) --r.log;
+  const long long from = base + upto - mine;
+  const int first = worker - wave * (int)gridDim.x;  // the workers of a block are a grid apart
+  for (int w = 0; w < 4; ++w) {
+    const int id = first + w * (int)gridDim.x;
+    const long long x = (r.total * id) >> r.log;
+    if (x >= from && x < from + mine) {
+      long long left = x - from;
+      int s = s0;
+      for (; s < s1 - 1; ++s) {
+        const long long c = seq_steps<C>(a, s);
+        if (left < c) break;
+        left -= c;
       }
-      x = dot * scale;
+      seq_[w] = s;
+      at_[w] = left;
     }
-    float top = x;  // NaN scores are passed over here and come back through their weights
-    for (int d = 1; d < 64; d *= 2) top = __builtin_fmaxf(top, __shfl_xor(top, d));
-    const float next = __builtin_fmaxf(m, top);
-    const float ref = next == -INFINITY ? 0.0f : next;
-    const float corr = __builtin_amdgcn_exp2f((m - ref) * kLog2e);
-    const float p = __builtin_amdgcn_exp2f((x - ref) * kLog2e);
-    m = next;
-    l = l * corr + p;
-    for (int d = 0; d < HD / 64; ++d) acc[d] = acc[d] * corr;
-    const int n = see - base < 64 ? (int)(see - base) : 64;
-    for (int j = 0; j < n; ++j) {
-      const float w = __shfl(p, j);
-      const size_t block = (size_t)pages[(base + j) / kPage] * a.n_kv_heads + kvh;
-      const uint8_t* v = a.v_pool + (block * kPage + (base + j) % kPage) * HD;
-      for (int d = 0; d < HD / 64; ++d) {
-        const f16x2 y = from_e4m3<false>(v[64 * d + lane], a.v_scale[block]);
-        acc[d] = __builtin_fmaf(w, (float)y[0], acc[d]);
+  }
+  __syncthreads();
+  r.begin = (r.total * worker) >> r.log;
+  r.end = (r.total * (worker + 1)) >> r.log;
+  if (worker >= 1 << r.log) r.begin = r.end = r.total;
+  r.seq = __builtin_amdgcn_readfirstlane(seq_[wave]);
+  r.at = at_[wave];
+  return r;
+}
+
+__device__ __forceinline__ float max_of_quarters(float x) {
+  x = __builtin_fmaxf(x, __shfl_xor(x, 16));
+  return __builtin_fmaxf(x, __shfl_xor(x, 32));
+}
+
+// Units of few columns, a wave each. With C = 16 QT columns (rows x heads of the group) a step is
+//   S^T = K Q^T   (v_mfma_f32_16x16x32_f16; A: 16 positions of K, B: 16 columns of q)
+//   O^T += V^T P^T (.._bf16; A: 16 dims of V, B: the lane's own weights)
+// and no operand changes lanes: lane (n = l % 16, qd = l / 16) gets of S^T column n, positions 4 qd ..
+// 4 qd + 3 of each page, and those positions, of two pages, are its places in the second product's
+// contraction. K is loaded 16 bytes a lane (position n, dims 16 qd ..): the order of dims in the
+// contraction is free, and q is loaded in it too. V is loaded 4 (8) bytes for each of 4 positions;
+// dims 4 n .. become the rows n of 4 (8) products, so that a lane ends with 16 (32) dims in a row.
+// Weights enter as two bf16, high and low half: 16 significant bits at any exponent.
+template <int HD, int QT>
+__global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a) {
+  constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64;
+  const int lane = threadIdx.x & 63, n = lane & 15, qd = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int worker = wave * (int)gridDim.x + (int)blockIdx.x;
+  const bool shared_units = a.parts != nullptr;
+  const Share sh = find_share<C>(a, worker, a.log_workers);
+  int open_last = -1, open_column = 0, open_columns = 0, open_seq = 0, open_head = 0;
+
+  long long pos = sh.begin;
+  if (pos < sh.end) {
+    int s = sh.seq, tile = 0;
+    Seq q = seq_of(a, s);
+    long long at = sh.at;
+    int steps;
+    for (;;) {
+      steps = tile_steps<C>(a, q, tile);
+      if (at < (long long)steps * a.n_kv_heads) break;
+      at -= (long long)steps * a.n_kv_heads;
+      ++tile;
+    }
+    int h = (int)(at / steps), step = (int)(at % steps);
+    const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
+
+    while (pos < sh.end) {
+      if (!shared_units && step > 0) {  // begun, and done, by the worker before
+        pos += steps - step;
+      } else {
+        int stop = steps;
+        if (shared_units && sh.end - pos < steps - step) stop = step + (int)(sh.end - pos);
+        const int c0 = tile * C;
+        const int columns = q.columns - c0 < C ? q.columns - c0 : C;
+        const int see_max = seen(a, q, c0 + columns - 1), see_min = seen(a, q, c0);
+
+        int see[QT];
+        f16x8 qf[QT][2 * KU];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const int c = 16 * t + n;
+          const bool own = c < columns;
+          const int col = c0 + (own ? c : 0);
+          see[t] = own ? seen(a, q, col) : 0;
+          const size_t row = q.row0 + col / a.group;
+          const f16* src = a.q + (row * a.n_heads + h * a.group + col % a.group) * HD + 16 * qd;
+#pragma unroll
+          for (int u = 0; u < 2 * KU; ++u)
+            qf[t][u] = own ? as_h8(ld16(src + 64 * (u / 2) + 8 * (u % 2))) : (f16x8)(f16)0;
+        }
+        f32x4 acc[QT][4 * VW];
+        float m[QT], l[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          m[t] = -INFINITY;
+          l[t] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < 4 * VW; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
+        }
+
+        const int last_page = (see_max + kPage - 1) / kPage - 1;
+        const int* pages = a.batch.tables + (size_t)s * a.batch.max_pages;
+        if (see_max > 0) {
+          // 64 table entries and their scales at a time, one to a lane
+          int window = -1, ids = 0;
+          float ksc = 0, vsc = 0;
+          u32x4 kr[4][KU];
+          uint32_t vr[4][4][VW];
+          float ks[4], vs[4];
+          size_t block[4];
+          auto locate = [&](int st) {
+            const int w = (4 * st) >> 6;
+            if (w != window) {
+              window = w;
+              const int p = 64 * w + lane;
+              ids = pages[p < last_page ? p : last_page];
+              const size_t b = (size_t)ids * a.n_kv_heads + h;
+              ksc = a.k_scale[b];
+              vsc = a.v_scale[b];
+            }
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const int i = (4 * st + p) & 63;
+              block[p] = (size_t)__builtin_amdgcn_readlane(ids, i) * a.n_kv_heads + h;
+              ks[p] = readlane_f32(ksc, i);
+              vs[p] = readlane_f32(vsc, i);
+            }
+          };
+          auto load_k = [&] {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const uint8_t* src = a.k_pool + block[p] * (kPage * HD) + n * HD + 16 * qd;
+#pragma unroll
+              for (int u = 0; u < KU; ++u) kr[p][u] = ld16_stream(src + 64 * u);
+            }
+          };
+          auto load_v = [&] {
+#pragma unroll
+            for (int p = 0; p < 4; ++p) {
+              const uint8_t* src = a.v_pool + block[p] * (kPage * HD) + 4 * qd * HD + 4 * VW * n;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                if constexpr (VW == 1) {
+                  vr[p][i][0] = __builtin_nontemporal_load(
+                      reinterpret_cast<const uint32_t*>(src + i * HD));
+                } else {
+                  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+                  const u32x2 x = __builtin_nontemporal_load(
+                      reinterpret_cast<const u32x2*>(src + i * HD));
+                  vr[p][i][0] = x[0];
+                  vr[p][i][VW - 1] = x[1];
+                }
+              }
+            }
+          };
+          locate(step);
+          load_k();
+          load_v();
+          for (int st = step; st < stop; ++st) {
+            const float vs0 = vs[0], vs1 = vs[1], vs2 = vs[2], vs3 = vs[3];
+            f32x4 sc[QT][4];
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+#pragma unroll
+              for (int p = 0; p < 4; ++p) sc[t][p] = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+#pragma unroll
+              for (int u = 0; u < 2 * KU; ++u) {
+                const uint32_t lo = elem(kr[p][u / 2], 2 * (u % 2));
+                const uint32_t hi = elem(kr[p][u / 2], 2 * (u % 2) + 1);
+                u32x4 w;
+                w[0] = __builtin_bit_cast(uint32_t, from_e4m3<false>(lo, ks[p]));
+                w[1] = __builtin_bit_cast(uint32_t, from_e4m3<true>(lo, ks[p]));
+                w[2] = __builtin_bit_cast(uint32_t, from_e4m3<false>(hi, ks[p]));
+                w[3] = __builtin_bit_cast(uint32_t, from_e4m3<true>(hi, ks[p]));
+#pragma unroll
+                for (int t = 0; t < QT; ++t)
+                  sc[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), qf[t][u], sc[t][p],
+                                                                    0, 0, 0);
+              }
+            const bool more = st + 1 < stop;
+            if (more) {
+              locate(st + 1);
+              load_k();
+            }
+            const int key0 = st * kStep + 4 * qd;
+            const bool edge = (st + 1) * kStep > see_min;  // some row does not see all of it
+            uint32_t ph[QT][4][2], pl[QT][4][2];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+              float x[4][4], top = -INFINITY;
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  x[p][i] = sc[t][p][i] * to_log2;
+                  if (edge && key0 + 16 * p + i >= see[t]) x[p][i] = -INFINITY;
+                  top = __builtin_fmaxf(top, x[p][i]);
+                }
+              top = max_of_quarters(top);
+              const float next = __builtin_fmaxf(m[t], top);
+              const float ref = next == -INFINITY ? 0.0f : next;
+              if (__builtin_amdgcn_ballot_w64(next != m[t])) {
+                const float corr = __builtin_amdgcn_exp2f(m[t] - ref);
+                l[t] = l[t] * corr;
+#pragma unroll
+                for (int c = 0; c < 4 * VW; ++c) acc[t][c] = acc[t][c] * corr;
+                m[t] = next;
+              }
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                  const float w0 = __builtin_amdgcn_exp2f(x[p][i] - ref);
+                  const float w1 = __builtin_amdgcn_exp2f(x[p][i + 1] - ref);
+                  l[t] = l[t] + (w0 + w1);
+                  const uint32_t b0 = __builtin_bit_cast(uint32_t, w0);
+                  const uint32_t b1 = __builtin_bit_cast(uint32_t, w1);
+                  ph[t][p][i / 2] = __builtin_amdgcn_perm(b1, b0, 0x07060302);
+                  const float r0 = w0 - __builtin_bit_cast(float, b0 & 0xFFFF0000u);
+                  const float r1 = w1 - __builtin_bit_cast(float, b1 & 0xFFFF0000u);
+                  const bf16x2 r = {(__bf16)r0, (__bf16)r1};
+                  pl[t][p][i / 2] = __builtin_bit_cast(uint32_t, r);
+                }
+            }
+            if (edge) {
+              // What no row sees is stale: zero. A NaN of a position that only some rows see would
+              // reach the others through their zero weights: it is taken out and handed to its rows.
+              uint32_t odd = 0;
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                  for (int w = 0; w < VW; ++w) {
+                    uint32_t b = key0 + 16 * p + i < see_max ? vr[p][i][w] : 0u;
+                    const uint32_t bad = ((b & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    odd |= bad;
+                    vr[p][i][w] = b & ~((bad >> 7) * 0xFFu);
+                  }
+              if (__builtin_amdgcn_ballot_w64(odd != 0)) {
+                for (int key = st * kStep; key < (st + 1) * kStep && key < see_max; ++key) {
+                  const size_t b = (size_t)pages[key / kPage] * a.n_kv_heads + h;
+                  const uint8_t* src =
+                      a.v_pool + (b * kPage + key % kPage) * HD + 16 * VW * qd;
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int c = 0; c < 4 * VW; ++c)
+                      if ((src[4 * VW * i + c] & 0x7F) == 0x7F)
+#pragma unroll
+                        for (int t = 0; t < QT; ++t)
+                          if (key < see[t]) acc[t][c][i] = __builtin_nanf("");
+                }
+              }
+            }
+#pragma unroll
+            for (int pp = 0; pp < 4; pp += 2) {
+              const float va = pp == 0 ? vs0 : vs2, vb = pp == 0 ? vs1 : vs3;
+#pragma unroll
+              for (int w = 0; w < VW; ++w)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                  constexpr uint32_t sel[2] = {0x05010400u, 0x07030602u};
+                  const uint32_t a01 =
+                      __builtin_amdgcn_perm(vr[pp][1][w], vr[pp][0][w], sel[half]);
+                  const uint32_t a23 =
+                      __builtin_amdgcn_perm(vr[pp][3][w], vr[pp][2][w], sel[half]);
+                  const uint32_t b01 =
+                      __builtin_amdgcn_perm(vr[pp + 1][1][w], vr[pp + 1][0][w], sel[half]);
+                  const uint32_t b23 =
+                      __builtin_amdgcn_perm(vr[pp + 1][3][w], vr[pp + 1][2][w], sel[half]);
+#pragma unroll
+                  for (int c = 0; c < 2; ++c) {
+                    auto two = [&](uint32_t b, float scale) {
+                      return c ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                                                                  b, scale, true))
+                               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
+                                                                  b, scale, false));
+                    };
+                    const u32x4 v4 = {two(a01, va), two(a23, va), two(b01, vb), two(b23, vb)};
+                    const bf16x8 vf = __builtin_bit_cast(bf16x8, v4);
+#pragma unroll
+                    for (int t = 0; t < QT; ++t) {
+                      const u32x4 h4 = {ph[t][pp][0], ph[t][pp][1], ph[t][pp + 1][0],
+                                        ph[t][pp + 1][1]};
+                      const u32x4 l4 = {pl[t][pp][0], pl[t][pp][1], pl[t][pp + 1][0],
+                                        pl[t][pp + 1][1]};
+                      f32x4& o = acc[t][4 * w + 2 * half + c];
+                      o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                          vf, __builtin_bit_cast(bf16x8, h4), o, 0, 0, 0);
+                      o = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                          vf, __builtin_bit_cast(bf16x8, l4), o, 0, 0, 0);
+                    }
+                  }
+                }
+            }
+            if (more) load_v();
+          }
+        }
+
+        const bool whole = step == 0 && stop == steps;
+        if (!whole && step == 0) {  // ends in another worker's share
+          const long long end = pos + steps;
+          open_last = (int)(((end << sh.log) - 1) / sh.total);
+          open_column = c0;
+          open_columns = columns;
+          open_seq = s;
+          open_head = h;
+        }
+        const size_t slot = 2 * (size_t)worker + (step == 0 ? 1 : 0);
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          float sum = l[t] + __shfl_xor(l[t], 16);
+          sum = sum + __shfl_xor(sum, 32);
+          const int c = 16 * t + n;
+          if (c >= columns) continue;
+          if (whole) {
+            const int col = c0 + c;
+            f16* dst = a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads + h * a.group +
+                                col % a.group) * HD + 16 * VW * qd;
+#pragma unroll
+            for (int g = 0; g < 2 * VW; ++g) {
+              f16x8 o;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                const int d = 8 * g + e;  // of this lane's dims: (i, chunk)
+                const float y = acc[t][d % (4 * VW)][d / (4 * VW)];
+                o[e] = see[t] > 0 ? (f16)(y / sum) : (f16)0;
+              }
+              st16(dst + 8 * g, as_u4(o));
+            }
+          } else {
+            float* dst = a.parts + (slot * C + c) * HD + 16 * VW * qd;
+#pragma unroll
+            for (int g = 0; g < 4 * VW; ++g) {
+              f32x4 o;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int d = 4 * g + e;
+                o[e] = acc[t][d % (4 * VW)][d / (4 * VW)];
+              }
+              *reinterpret_cast<f32x4*>(dst + 4 * g) = o;
+            }
+            if (qd == 0) a.parts_ml[slot * C + c] = make_float2(m[t], sum);
+          }
+        }
+        pos += stop - step;
+      }
+      step = 0;
+      if (++h == a.n_kv_heads) {
+        h = 0;
+        ++tile;
+        while (tile * C >= q.columns && s < a.batch.n_seqs - 1) {
+          tile = 0;
+          q = seq_of(a, ++s);
+        }
+        if (tile * C >= q.columns) break;
+        steps = tile_steps<C>(a, q, tile);
       }
     }
   }
-  for (int d = 1; d < 64; d *= 2) l = l + __shfl_xor(l, d);
-  f16* out = a.out + ((size_t)row * a.n_heads + head) * HD;
-  for (int d = 0; d < HD / 64; ++d) out[64 * d + lane] = see > 0 ? (f16)(acc[d] / l) : (f16)0;
+  if (shared_units && lane == 0) {
+    Open o = {};
+    o.last = open_last;
+    o.column = open_column;
+    o.columns = open_columns;
+    o.seq = open_seq;
+    o.head = open_head;
+    a.open[worker] = o;
+  }
+}
+
+// Joins the parts of a unit: the one that its first worker left (an odd slot) and those of the
+// workers behind it (even slots). Block b looks at worker b.
+template <int HD>
+__global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs a, int C) {
+  constexpr int V = HD / 4;  // 4 dims to a thread
+  __shared__ f32x4 other[256];
+  __shared__ float2 other_ml[256];
+  const Open o = a.open[blockIdx.x];
+  if (o.last < 0) return;
+  const int tid = threadIdx.x, n = o.last - (int)blockIdx.x + 1;
+  // tasks (column, 4 dims) side by side, the parts dealt out over what threads are left
+  int lanes = V;
+  while (lanes < V * o.columns && lanes < 256) lanes *= 2;
+  const int deal = 256 / lanes, mine = tid / lanes;
+  const Seq q = seq_of(a, o.seq);
+  for (int task0 = 0; task0 < V * o.columns; task0 += lanes) {
+    const int task = task0 + tid % lanes, c = task / V, d = 4 * (task % V);
+    f32x4 acc = {0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    if (c < o.columns) {
+#pragma unroll 4
+      for (int j = mine; j < n; j += deal) {
+        const size_t slot = 2 * (size_t)(blockIdx.x + j) + (j == 0 ? 1 : 0);
+        const float2 ml = a.parts_ml[slot * C + c];
+        const f32x4 x = *reinterpret_cast<const f32x4*>(a.parts + (slot * C + c) * HD + d);
+        const float next = __builtin_fmaxf(m, ml.x), ref = next == -INFINITY ? 0.0f : next;
+        const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(ml.x - ref);
+        acc = acc * wa + x * wb;
+        l = l * wa + ml.y * wb;
+        m = next;
+      }
+    }
+    __syncthreads();
+    other[tid] = acc;
+    other_ml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (mine == 0 && c < o.columns) {
+      for (int k = 1; k < deal; ++k) {
+        const float2 ml = other_ml[tid + k * lanes];
+        const float next = __builtin_fmaxf(m, ml.x), ref = next == -INFINITY ? 0.0f : next;
+        const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(ml.x - ref);
+        acc = acc * wa + other[tid + k * lanes] * wb;
+        l = l * wa + ml.y * wb;
+        m = next;
+      }
+      const int col = o.column + c;
+      const bool any = seen(a, q, col) > 0;
+      f16x2 y[2];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e / 2][e % 2] = any ? (f16)(acc[e] / l) : (f16)0;
+      uint2 v;
+      v.x = __builtin_bit_cast(uint32_t, y[0]);
+      v.y = __builtin_bit_cast(uint32_t, y[1]);
+      *reinterpret_cast<uint2*>(a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads +
+                                         o.head * a.group + col % a.group) * HD + d) = v;
+    }
+  }
+}
+
+template <int HD, int QT>
+int few_launch(AttentionArgs a, hipStream_t stream) {
+  a.log_workers = QT == 1 ? 11 : 10;
+  const int workers = 1 << a.log_workers;
+  const int st = launch(k_kv8_attention_few<HD, QT>, dim3(workers / 4), dim3(256), 0, stream, a);
+  if (st != LLMK_OK || !a.parts) return st;
+  return launch(k_kv8_attention_join<HD>, dim3(workers), dim3(256), 0, stream, a, 16 * QT);
+}
+
+template <int HD>
+int attention_launch(const AttentionArgs& a, int max_rows, hipStream_t stream) {
+  return (long long)max_rows * a.group <= 16 ? few_launch<HD, 1>(a, stream)
+                                             : few_launch<HD, 2>(a, stream);
 }
 
 }  // namespace
@@ -95,7 +573,8 @@ __global__ void __launch_bounds__(256) k_kv8_attention_rows(const AttentionArgs 
 using namespace llmk;
 
 extern "C" size_t llmk_kv8_attention_workspace_floats(int head_dim) {
-  return head_dim == 64 || head_dim == 128 ? 4 : 0;
+  if (head_dim != 64 && head_dim != 128) return 0;
+  return (size_t)kSlotColumns * (head_dim + 2) + kWorkers * (sizeof(Open) / 4);
 }
 
 extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, const float* k_scale,
@@ -115,7 +594,10 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
   if (max_rows == 0 || !q || !k_pool || !k_scale || !v_pool || !v_scale || !block_tables ||
       !seq_lens || !out)
     return LLMK_ERR_INVALID_VALUE;
-  if (n_heads > 65535) return LLMK_ERR_UNSUPPORTED;
+  // a sequence's columns, and positions of a table, are counted in 32 bits
+  if ((long long)n_rows * (n_heads / n_kv_heads) > 0x7FFF0000LL || n_heads > 65535 ||
+      max_pages > 0x7FFF0000 / kv8::kPage)
+    return LLMK_ERR_UNSUPPORTED;
   if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) ||
       !aligned16(workspace))
     return LLMK_ERR_ALIGNMENT;
@@ -127,9 +609,15 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
   a.v_pool = v_pool;
   a.v_scale = v_scale;
   a.out = reinterpret_cast<f16*>(out);
+  a.parts = workspace;
+  a.parts_ml = reinterpret_cast<float2*>(workspace + (size_t)kSlotColumns * head_dim);
+  a.open = reinterpret_cast<Open*>(workspace + (size_t)kSlotColumns * (head_dim + 2));
   a.n_heads = n_heads;
   a.n_kv_heads = n_kv_heads;
-  return launch(head_dim == 64 ? k_kv8_attention_rows<64> : k_kv8_attention_rows<128>,
-                dim3((unsigned)n_rows, ceil_div((size_t)n_heads, 4)), dim3(256), 0,
-                static_cast<hipStream_t>(stream), a);
+  a.group = n_heads / n_kv_heads;
+  a.log_workers = 0;
+  a.min_steps = 1;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  return head_dim == 64 ? attention_launch<64>(a, max_rows, s)
+                        : attention_launch<128>(a, max_rows, s);
 }

@@ -120,8 +120,9 @@ def attention(q, k, v, tables, starts, lens):
     one rounding to fp16 may be off by: a score s is a sum of dim products, off by at most dim 2^-24
     of sum |q_i k_i| / sqrt(dim), its distance to the maximum by that again and by 2^-22 of itself
     (scale, difference and exponent are each rounded); weights, and so Σ p v, by that relative to
-    Σ p |v|, twice for the quotient, with 2^-20 for the exponentials, for weights held as two fp16
-    and for sums of up to 2^16 terms taken in parts."""
+    Σ p |v|, twice for the quotient, with 2^-20 for the exponentials and for sums of up to 2^16 terms
+    taken in parts. A weight may enter Σ p v as two bf16, its first 8 bits cut off (what is left is
+    below 2^-7 of it) and the rest rounded to 8 (2^-8 of the rest): 2^-15 of it."""
     n_rows, heads, dim = q.shape
     n_kv = k.codes.shape[1]
     out, bound = np.full(q.shape, np.inf), np.zeros(q.shape)
@@ -146,7 +147,7 @@ def attention(q, k, v, tables, starts, lens):
                     out[r, h] = p @ V[:see, g]
                     rel = 2 * off + 2.0 ** -22 * np.abs(a - a.max())
                     rel = np.expm1(np.minimum(rel, 30.0)) + 2.0 ** -20
-                    mean = (p * rel) @ np.abs(V[:see, g]) + (p * rel).sum() * (
+                    mean = (p * (rel + 2.0 ** -15)) @ np.abs(V[:see, g]) + (p * rel).sum() * (
                         p @ np.abs(V[:see, g]))
                 bound[r, h] = mean + 2.0 ** -11 * np.abs(out[r, h]) + 2.0 ** -25
     return out, bound
