@@ -2,6 +2,8 @@
 // over the positions j up to the row's own, for rows of any number a sequence.
 #include <math.h>
 
+#include <type_traits>
+
 #include "kv8.hpp"
 
 namespace llmk {
@@ -10,13 +12,24 @@ namespace {
 using namespace kv8;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr int kStep = 64;                       // positions of a step: four pages
 constexpr float kLog2e = 1.44269504088896341f;
+// Below it a rounded maximum (in log2 units) is less than 2^6 short of the exact one, which neither
+// weights nor sums mind; from there on exponents are made in two steps, and the largest weight is 1.
+constexpr float kLargeScore = 1073741824.0f;
+constexpr int kStart = 2;                       // what a unit's first loads cost, in steps
 constexpr int kSlotColumns = 65536;             // of partial results in the workspace
 constexpr int kWorkers = 2048;                  // at most
+
+template <bool HIGH>
+__device__ __forceinline__ uint32_t bf16_from_e4m3(uint32_t bytes, float scale) {
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, scale, HIGH));
+}
 
 // What a worker leaves for the launch that joins parts: the unit that begins in its share and ends in
 // another's.
@@ -38,7 +51,7 @@ struct AttentionArgs {
   float* parts;  // [2 workers][columns of a tile][HD], NULL: no unit is shared
   float2* parts_ml;
   Open* open;
-  int n_heads, n_kv_heads, group, log_workers, min_steps;
+  int n_heads, n_kv_heads, group, log_workers, min_ticks;
 };
 
 // A sequence's rows in this call and what they see.
@@ -70,7 +83,8 @@ __device__ __forceinline__ int seen(const AttentionArgs& a, const Seq& q, int co
   const long long m = n < q.limit ? n : q.limit;
   return m < 0 ? 0 : (int)m;
 }
-// Steps of a tile: those of its last row; one for a tile that sees nothing, which writes zeros.
+// Steps of a tile: those of its last row; one for a tile that sees nothing, which writes zeros. A
+// unit's share of the work is counted in ticks, its steps and kStart for its beginning.
 template <int C>
 __device__ __forceinline__ int tile_steps(const AttentionArgs& a, const Seq& q, int tile) {
   const int last = (tile + 1) * C < q.columns ? (tile + 1) * C - 1 : q.columns - 1;
@@ -78,14 +92,30 @@ __device__ __forceinline__ int tile_steps(const AttentionArgs& a, const Seq& q, 
   return n > 0 ? n : 1;
 }
 template <int C>
-__device__ __forceinline__ long long seq_steps(const AttentionArgs& a, int s) {
+__device__ __forceinline__ long long seq_ticks(const AttentionArgs& a, int s) {
   const Seq q = seq_of(a, s);
   long long n = 0;
-  for (int t = 0; t * C < q.columns; ++t) n += tile_steps<C>(a, q, t);
+  for (int t = 0; t * C < q.columns; ++t) n += kStart + tile_steps<C>(a, q, t);
   return n * a.n_kv_heads;
 }
 
-// Where the share of each of a block's workers begins among the steps of all units, which are
+// Values that are the same in every lane, as scalars.
+__device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ long long same(long long x) {
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)((uint64_t)x >> 32));
+  return (long long)(((uint64_t)hi << 32) | lo);
+}
+
+__device__ __forceinline__ Seq same(Seq q) {
+  q.row0 = same(q.row0);
+  q.columns = same(q.columns);
+  q.before = same(q.before);
+  q.limit = same(q.limit);
+  return q;
+}
+
+// Where the share of each of a block's workers begins among the ticks of all units, which are
 // ordered by sequence, tile and kv head. By all 256 threads.
 struct Share {
   long long total;
@@ -103,7 +133,7 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
   const int n = a.batch.n_seqs, per = (n + 255) / 256;
   const int s0 = tid * per, s1 = s0 + per < n ? s0 + per : n;
   long long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += seq_steps<C>(a, s);
+  for (int s = s0; s < s1; ++s) mine += seq_ticks<C>(a, s);
   long long upto = mine;
   for (int d = 1; d < 64; d *= 2) {
     const long long o = __shfl_up(upto, d);
@@ -119,7 +149,7 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
     r.total += wave_sum_[w];
   }
   r.log = log_workers;
-  while (r.log > 0 && (r.total >> r.log) < a.min_steps) --r.log;
+  while (r.log > 0 && (r.total >> r.log) < a.min_ticks) --r.log;
   const long long from = base + upto - mine;
   const int first = worker - wave * (int)gridDim.x;  // the workers of a block are a grid apart
   for (int w = 0; w < 4; ++w) {
@@ -129,7 +159,7 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
       long long left = x - from;
       int s = s0;
       for (; s < s1 - 1; ++s) {
-        const long long c = seq_steps<C>(a, s);
+        const long long c = seq_ticks<C>(a, s);
         if (left < c) break;
         left -= c;
       }
@@ -138,11 +168,13 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
     }
   }
   __syncthreads();
+  r.total = same(r.total);
+  r.log = __builtin_amdgcn_readfirstlane(r.log);
   r.begin = (r.total * worker) >> r.log;
   r.end = (r.total * (worker + 1)) >> r.log;
   if (worker >= 1 << r.log) r.begin = r.end = r.total;
   r.seq = __builtin_amdgcn_readfirstlane(seq_[wave]);
-  r.at = at_[wave];
+  r.at = same(at_[wave]);
   return r;
 }
 
@@ -161,7 +193,7 @@ __device__ __forceinline__ float max_of_quarters(float x) {
 // dims 4 n .. become the rows n of 4 (8) products, so that a lane ends with 16 (32) dims in a row.
 // Weights enter as two bf16, high and low half: 16 significant bits at any exponent.
 template <int HD, int QT>
-__global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a) {
+__global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArgs a) {
   constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64;
   const int lane = threadIdx.x & 63, n = lane & 15, qd = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -173,27 +205,33 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
   long long pos = sh.begin;
   if (pos < sh.end) {
     int s = sh.seq, tile = 0;
-    Seq q = seq_of(a, s);
+    Seq q = same(seq_of(a, s));
     long long at = sh.at;
     int steps;
     for (;;) {
-      steps = tile_steps<C>(a, q, tile);
-      if (at < (long long)steps * a.n_kv_heads) break;
-      at -= (long long)steps * a.n_kv_heads;
+      steps = same(tile_steps<C>(a, q, tile));
+      const long long ticks = (long long)(kStart + steps) * a.n_kv_heads;
+      if (at < ticks) break;
+      at -= ticks;
       ++tile;
     }
-    int h = (int)(at / steps), step = (int)(at % steps);
+    int h = same((int)at / (kStart + steps)), tick = same((int)at % (kStart + steps));
     const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
+    int ids = 0, ids_of = -1, window = -1;  // 64 entries of a sequence's table, one to a lane
 
     while (pos < sh.end) {
-      if (!shared_units && step > 0) {  // begun, and done, by the worker before
-        pos += steps - step;
-      } else {
-        int stop = steps;
-        if (shared_units && sh.end - pos < steps - step) stop = step + (int)(sh.end - pos);
+      const int ticks = kStart + steps;
+      int upto = ticks;  // this worker's end of the unit
+      if (shared_units && sh.end - pos < ticks - tick) upto = tick + (int)(sh.end - pos);
+      const int step = tick > kStart ? tick - kStart : 0;
+      int stop = upto > kStart ? upto - kStart : 0;
+      pos += upto - tick;
+      // without a workspace, a unit that began in the share before is done there
+      if (stop > step && (shared_units || tick == 0)) {
+        stop = same(stop);
         const int c0 = tile * C;
         const int columns = q.columns - c0 < C ? q.columns - c0 : C;
-        const int see_max = seen(a, q, c0 + columns - 1), see_min = seen(a, q, c0);
+        const int see_max = same(seen(a, q, c0 + columns - 1)), see_min = same(seen(a, q, c0));
 
         int see[QT];
         f16x8 qf[QT][2 * KU];
@@ -219,66 +257,64 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
           for (int c = 0; c < 4 * VW; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
         }
 
-        const int last_page = (see_max + kPage - 1) / kPage - 1;
         const int* pages = a.batch.tables + (size_t)s * a.batch.max_pages;
         if (see_max > 0) {
-          // 64 table entries and their scales at a time, one to a lane
-          int window = -1, ids = 0;
-          float ksc = 0, vsc = 0;
+          // their scales for this head
+          float ksc, vsc;
+          const int last_page = (int)((q.limit + kPage - 1) / kPage) - 1;
+          auto load_ids = [&] {
+            const int p = 64 * window + lane;
+            ids = pages[p < last_page ? p : last_page];
+          };
           u32x4 kr[4][KU];
           uint32_t vr[4][4][VW];
-          float ks[4], vs[4];
-          size_t block[4];
-          auto locate = [&](int st) {
-            const int w = (4 * st) >> 6;
-            if (w != window) {
-              window = w;
-              const int p = 64 * w + lane;
-              ids = pages[p < last_page ? p : last_page];
-              const size_t b = (size_t)ids * a.n_kv_heads + h;
-              ksc = a.k_scale[b];
-              vsc = a.v_scale[b];
-            }
+          float ks[4], vs[4], vs_next[4];
+          const uint8_t* v_next[4];
+          auto load_scales = [&] {
+            const size_t b = (size_t)ids * a.n_kv_heads + h;
+            ksc = a.k_scale[b];
+            vsc = a.v_scale[b];
+          };
+          // the pages of a step: loads of K, and where V is
+          auto load_k = [&](int st) {
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
               const int i = (4 * st + p) & 63;
-              block[p] = (size_t)__builtin_amdgcn_readlane(ids, i) * a.n_kv_heads + h;
-              ks[p] = readlane_f32(ksc, i);
-              vs[p] = readlane_f32(vsc, i);
+              const size_t at = ((size_t)__builtin_amdgcn_readlane(ids, i) * a.n_kv_heads + h) *
+                                (size_t)(kPage * HD);
+              const uint8_t* src = a.k_pool + at;
+#pragma unroll
+              for (int u = 0; u < KU; ++u)
+                kr[p][u] = ld16_stream(src + (uint32_t)(n * HD + 16 * qd + 64 * u));
+              v_next[p] = a.v_pool + at;
             }
           };
-          auto load_k = [&] {
+          auto take_scales = [&](int st) {
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-              const uint8_t* src = a.k_pool + block[p] * (kPage * HD) + n * HD + 16 * qd;
-#pragma unroll
-              for (int u = 0; u < KU; ++u) kr[p][u] = ld16_stream(src + 64 * u);
+              const int i = (4 * st + p) & 63;
+              ks[p] = readlane_f32(ksc, i);
+              vs_next[p] = readlane_f32(vsc, i);
             }
           };
           auto load_v = [&] {
 #pragma unroll
             for (int p = 0; p < 4; ++p) {
-              const uint8_t* src = a.v_pool + block[p] * (kPage * HD) + 4 * qd * HD + 4 * VW * n;
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
+                const uint8_t* src = v_next[p] + (uint32_t)((4 * qd + i) * HD + 4 * VW * n);
                 if constexpr (VW == 1) {
-                  vr[p][i][0] = __builtin_nontemporal_load(
-                      reinterpret_cast<const uint32_t*>(src + i * HD));
+                  vr[p][i][0] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(src));
                 } else {
-                  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-                  const u32x2 x = __builtin_nontemporal_load(
-                      reinterpret_cast<const u32x2*>(src + i * HD));
+                  const u32x2 x = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(src));
                   vr[p][i][0] = x[0];
                   vr[p][i][VW - 1] = x[1];
                 }
               }
             }
           };
-          locate(step);
-          load_k();
-          load_v();
-          for (int st = step; st < stop; ++st) {
-            const float vs0 = vs[0], vs1 = vs[1], vs2 = vs[2], vs3 = vs[3];
+          auto one_step = [&](int st, auto edge) {
+            constexpr bool EDGE = decltype(edge)::value;  // some row does not see all of it
             f32x4 sc[QT][4];
 #pragma unroll
             for (int t = 0; t < QT; ++t)
@@ -300,26 +336,31 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
                   sc[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), qf[t][u], sc[t][p],
                                                                     0, 0, 0);
               }
-            const bool more = st + 1 < stop;
-            if (more) {
-              locate(st + 1);
-              load_k();
+            // Past the last step it is loaded again: loads that may not happen would make the waits
+            // for those in front of them as strict as if they did not.
+            const int then = st + 1 < stop ? st + 1 : st;
+            if (then >> 4 != window) {
+              window = then >> 4;
+              load_ids();
+              load_scales();
+              // waited for here: later, the loads of K and V behind them would be, too
+              asm volatile("" : "+v"(ids), "+v"(ksc), "+v"(vsc));
             }
+            load_k(then);
+            take_scales(then);
             const int key0 = st * kStep + 4 * qd;
-            const bool edge = (st + 1) * kStep > see_min;  // some row does not see all of it
             uint32_t ph[QT][4][2], pl[QT][4][2];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
-              float x[4][4], top = -INFINITY;
+              float top = -INFINITY;
 #pragma unroll
               for (int p = 0; p < 4; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                  x[p][i] = sc[t][p][i] * to_log2;
-                  if (edge && key0 + 16 * p + i >= see[t]) x[p][i] = -INFINITY;
-                  top = __builtin_fmaxf(top, x[p][i]);
+                  if (EDGE && key0 + 16 * p + i >= see[t]) sc[t][p][i] = -INFINITY;
+                  top = __builtin_fmaxf(top, sc[t][p][i]);
                 }
-              top = max_of_quarters(top);
+              top = max_of_quarters(top) * to_log2;
               const float next = __builtin_fmaxf(m[t], top);
               const float ref = next == -INFINITY ? 0.0f : next;
               if (__builtin_amdgcn_ballot_w64(next != m[t])) {
@@ -329,12 +370,23 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
                 for (int c = 0; c < 4 * VW; ++c) acc[t][c] = acc[t][c] * corr;
                 m[t] = next;
               }
+              float x[4][4];
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[p][i] = __builtin_fmaf(sc[t][p][i], to_log2, -ref);
+              if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ref) >= kLargeScore)) {
+#pragma unroll
+                for (int p = 0; p < 4; ++p)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) x[p][i] = sc[t][p][i] * to_log2 - ref;
+              }
 #pragma unroll
               for (int p = 0; p < 4; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                  const float w0 = __builtin_amdgcn_exp2f(x[p][i] - ref);
-                  const float w1 = __builtin_amdgcn_exp2f(x[p][i + 1] - ref);
+                  const float w0 = __builtin_amdgcn_exp2f(x[p][i]);
+                  const float w1 = __builtin_amdgcn_exp2f(x[p][i + 1]);
                   l[t] = l[t] + (w0 + w1);
                   const uint32_t b0 = __builtin_bit_cast(uint32_t, w0);
                   const uint32_t b1 = __builtin_bit_cast(uint32_t, w1);
@@ -345,7 +397,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
                   pl[t][p][i / 2] = __builtin_bit_cast(uint32_t, r);
                 }
             }
-            if (edge) {
+            if constexpr (EDGE) {
               // What no row sees is stale: zero. A NaN of a position that only some rows see would
               // reach the others through their zero weights: it is taken out and handed to its rows.
               uint32_t odd = 0;
@@ -355,7 +407,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                   for (int w = 0; w < VW; ++w) {
-                    uint32_t b = key0 + 16 * p + i < see_max ? vr[p][i][w] : 0u;
+                    const uint32_t b = key0 + 16 * p + i < see_max ? vr[p][i][w] : 0u;
                     const uint32_t bad = ((b & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
                     odd |= bad;
                     vr[p][i][w] = b & ~((bad >> 7) * 0xFFu);
@@ -377,8 +429,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
               }
             }
 #pragma unroll
-            for (int pp = 0; pp < 4; pp += 2) {
-              const float va = pp == 0 ? vs0 : vs2, vb = pp == 0 ? vs1 : vs3;
+            for (int pp = 0; pp < 4; pp += 2)
 #pragma unroll
               for (int w = 0; w < VW; ++w)
 #pragma unroll
@@ -395,12 +446,10 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
 #pragma unroll
                   for (int c = 0; c < 2; ++c) {
                     auto two = [&](uint32_t b, float scale) {
-                      return c ? __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
-                                                                  b, scale, true))
-                               : __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(
-                                                                  b, scale, false));
+                      return c ? bf16_from_e4m3<true>(b, scale) : bf16_from_e4m3<false>(b, scale);
                     };
-                    const u32x4 v4 = {two(a01, va), two(a23, va), two(b01, vb), two(b23, vb)};
+                    const u32x4 v4 = {two(a01, vs[pp]), two(a23, vs[pp]), two(b01, vs[pp + 1]),
+                                      two(b23, vs[pp + 1])};
                     const bf16x8 vf = __builtin_bit_cast(bf16x8, v4);
 #pragma unroll
                     for (int t = 0; t < QT; ++t) {
@@ -416,14 +465,30 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
                     }
                   }
                 }
-            }
-            if (more) load_v();
+            load_v();
+#pragma unroll
+            for (int p = 0; p < 4; ++p) vs[p] = vs_next[p];
+          };
+          if (s != ids_of || step >> 4 != window) {
+            window = step >> 4;
+            ids_of = s;
+            load_ids();
           }
+          load_scales();
+          load_k(step);
+          load_v();
+          take_scales(step);
+#pragma unroll
+          for (int p = 0; p < 4; ++p) vs[p] = vs_next[p];
+          const int inner = see_min / kStep < stop ? see_min / kStep : stop;
+          int st = step;
+          for (; st < inner; ++st) one_step(st, std::false_type{});
+          for (; st < stop; ++st) one_step(st, std::true_type{});
         }
 
         const bool whole = step == 0 && stop == steps;
         if (!whole && step == 0) {  // ends in another worker's share
-          const long long end = pos + steps;
+          const long long end = pos + ticks - upto;
           open_last = (int)(((end << sh.log) - 1) / sh.total);
           open_column = c0;
           open_columns = columns;
@@ -467,18 +532,17 @@ __global__ void __launch_bounds__(256) k_kv8_attention_few(const AttentionArgs a
             if (qd == 0) a.parts_ml[slot * C + c] = make_float2(m[t], sum);
           }
         }
-        pos += stop - step;
       }
-      step = 0;
+      tick = 0;
       if (++h == a.n_kv_heads) {
         h = 0;
         ++tile;
         while (tile * C >= q.columns && s < a.batch.n_seqs - 1) {
           tile = 0;
-          q = seq_of(a, ++s);
+          q = same(seq_of(a, ++s));
         }
         if (tile * C >= q.columns) break;
-        steps = tile_steps<C>(a, q, tile);
+        steps = same(tile_steps<C>(a, q, tile));
       }
     }
   }
@@ -616,7 +680,7 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
   a.n_kv_heads = n_kv_heads;
   a.group = n_heads / n_kv_heads;
   a.log_workers = 0;
-  a.min_steps = 1;
+  a.min_ticks = 1;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return head_dim == 64 ? attention_launch<64>(a, max_rows, s)
                         : attention_launch<128>(a, max_rows, s);
