@@ -16,7 +16,6 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
-constexpr int kStep = 64;                       // positions of a step: four pages
 constexpr float kLog2e = 1.44269504088896341f;
 // Below it a rounded maximum (in log2 units) is less than 2^6 short of the exact one, which neither
 // weights nor sums mind; from there on exponents are made in two steps, and the largest weight is 1.
@@ -31,13 +30,13 @@ __device__ __forceinline__ uint32_t bf16_from_e4m3(uint32_t bytes, float scale) 
                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, scale, HIGH));
 }
 
-// What a worker leaves for the launch that joins parts: the unit that begins in its share and ends in
-// another's.
-struct Open {
-  int last;   // the worker that ends it; -1: there is none
+// A unit that several workers share, as each of them notes it for the launch that joins its parts: one
+// that began before the worker's share and one that ends behind it.
+struct Shared {
+  int first, last;      // the workers; first > last: there is none
   int column, columns;  // of the tile, from the sequence's first row on
   int seq, head;        // kv head
-  int pad[3];
+  int pad[2];
 };
 
 struct AttentionArgs {
@@ -50,7 +49,7 @@ struct AttentionArgs {
   f16* out;
   float* parts;  // [2 workers][columns of a tile][HD], NULL: no unit is shared
   float2* parts_ml;
-  Open* open;
+  Shared* shared;  // [2 workers]
   int n_heads, n_kv_heads, group, log_workers, min_ticks;
 };
 
@@ -83,19 +82,25 @@ __device__ __forceinline__ int seen(const AttentionArgs& a, const Seq& q, int co
   const long long m = n < q.limit ? n : q.limit;
   return m < 0 ? 0 : (int)m;
 }
+// A step: 4 KiB of K and as much of V.
+template <int HD>
+constexpr int kPages = 256 / HD;
+template <int HD>
+constexpr int kStep = kPages<HD> * kPage;
+
 // Steps of a tile: those of its last row; one for a tile that sees nothing, which writes zeros. A
 // unit's share of the work is counted in ticks, its steps and kStart for its beginning.
-template <int C>
+template <int HD, int C>
 __device__ __forceinline__ int tile_steps(const AttentionArgs& a, const Seq& q, int tile) {
   const int last = (tile + 1) * C < q.columns ? (tile + 1) * C - 1 : q.columns - 1;
-  const int n = (seen(a, q, last) + kStep - 1) / kStep;
+  const int n = (seen(a, q, last) + kStep<HD> - 1) / kStep<HD>;
   return n > 0 ? n : 1;
 }
-template <int C>
+template <int HD, int C>
 __device__ __forceinline__ long long seq_ticks(const AttentionArgs& a, int s) {
   const Seq q = seq_of(a, s);
   long long n = 0;
-  for (int t = 0; t * C < q.columns; ++t) n += kStart + tile_steps<C>(a, q, t);
+  for (int t = 0; t * C < q.columns; ++t) n += kStart + tile_steps<HD, C>(a, q, t);
   return n * a.n_kv_heads;
 }
 
@@ -124,7 +129,7 @@ struct Share {
   int seq;               // that holds begin, and begin's place in it
   long long at;
 };
-template <int C>
+template <int HD, int C>
 __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, int log_workers) {
   __shared__ long long wave_sum_[4], at_[4];
   __shared__ int seq_[4];
@@ -133,7 +138,7 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
   const int n = a.batch.n_seqs, per = (n + 255) / 256;
   const int s0 = tid * per, s1 = s0 + per < n ? s0 + per : n;
   long long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += seq_ticks<C>(a, s);
+  for (int s = s0; s < s1; ++s) mine += seq_ticks<HD, C>(a, s);
   long long upto = mine;
   for (int d = 1; d < 64; d *= 2) {
     const long long o = __shfl_up(upto, d);
@@ -159,7 +164,7 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
       long long left = x - from;
       int s = s0;
       for (; s < s1 - 1; ++s) {
-        const long long c = seq_ticks<C>(a, s);
+        const long long c = seq_ticks<HD, C>(a, s);
         if (left < c) break;
         left -= c;
       }
@@ -178,9 +183,16 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
   return r;
 }
 
+// The larger of x and what the lane 16 (32) away has.
+__device__ __forceinline__ float max_across(float x, bool halves) {
+  const uint32_t b = __builtin_bit_cast(uint32_t, x);
+  const auto r = halves ? __builtin_amdgcn_permlane32_swap(b, b, false, false)
+                        : __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  const uint32_t r0 = r[0], r1 = r[1];
+  return __builtin_fmaxf(__builtin_bit_cast(float, r0), __builtin_bit_cast(float, r1));
+}
 __device__ __forceinline__ float max_of_quarters(float x) {
-  x = __builtin_fmaxf(x, __shfl_xor(x, 16));
-  return __builtin_fmaxf(x, __shfl_xor(x, 32));
+  return max_across(max_across(x, false), true);
 }
 
 // Units of few columns, a wave each. With C = 16 QT columns (rows x heads of the group) a step is
@@ -194,13 +206,26 @@ __device__ __forceinline__ float max_of_quarters(float x) {
 // Weights enter as two bf16, high and low half: 16 significant bits at any exponent.
 template <int HD, int QT>
 __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArgs a) {
-  constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64;
+  constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64, PG = kPages<HD>, STEP = kStep<HD>;
   const int lane = threadIdx.x & 63, n = lane & 15, qd = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int worker = wave * (int)gridDim.x + (int)blockIdx.x;
   const bool shared_units = a.parts != nullptr;
-  const Share sh = find_share<C>(a, worker, a.log_workers);
-  int open_last = -1, open_column = 0, open_columns = 0, open_seq = 0, open_head = 0;
+  const Share sh = find_share<HD, C>(a, worker, a.log_workers);
+  auto note = [&](int side, int first, int last, int column, int columns, int seq, int head) {
+    Shared o = {};
+    o.first = first;
+    o.last = last;
+    o.column = column;
+    o.columns = columns;
+    o.seq = seq;
+    o.head = head;
+    if (lane == 0) a.shared[2 * worker + side] = o;
+  };
+  if (shared_units) {
+    note(0, 0, -1, 0, 0, 0, 0);
+    note(1, 0, -1, 0, 0, 0, 0);
+  }
 
   long long pos = sh.begin;
   if (pos < sh.end) {
@@ -209,7 +234,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
     long long at = sh.at;
     int steps;
     for (;;) {
-      steps = same(tile_steps<C>(a, q, tile));
+      steps = same(tile_steps<HD, C>(a, q, tile));
       const long long ticks = (long long)(kStart + steps) * a.n_kv_heads;
       if (at < ticks) break;
       at -= ticks;
@@ -266,10 +291,10 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
             const int p = 64 * window + lane;
             ids = pages[p < last_page ? p : last_page];
           };
-          u32x4 kr[4][KU];
-          uint32_t vr[4][4][VW];
-          float ks[4], vs[4], vs_next[4];
-          const uint8_t* v_next[4];
+          u32x4 kr[PG][KU];
+          uint32_t vr[PG][4][VW];
+          float ks[PG], vs[PG], vs_next[PG];
+          const uint8_t* v_next[PG];
           auto load_scales = [&] {
             const size_t b = (size_t)ids * a.n_kv_heads + h;
             ksc = a.k_scale[b];
@@ -278,8 +303,8 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
           // the pages of a step: loads of K, and where V is
           auto load_k = [&](int st) {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              const int i = (4 * st + p) & 63;
+            for (int p = 0; p < PG; ++p) {
+              const int i = (PG * st + p) & 63;
               const size_t at = ((size_t)__builtin_amdgcn_readlane(ids, i) * a.n_kv_heads + h) *
                                 (size_t)(kPage * HD);
               const uint8_t* src = a.k_pool + at;
@@ -291,15 +316,15 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
           };
           auto take_scales = [&](int st) {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
-              const int i = (4 * st + p) & 63;
+            for (int p = 0; p < PG; ++p) {
+              const int i = (PG * st + p) & 63;
               ks[p] = readlane_f32(ksc, i);
               vs_next[p] = readlane_f32(vsc, i);
             }
           };
           auto load_v = [&] {
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
+            for (int p = 0; p < PG; ++p) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
                 const uint8_t* src = v_next[p] + (uint32_t)((4 * qd + i) * HD + 4 * VW * n);
@@ -313,15 +338,18 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
               }
             }
           };
-          auto one_step = [&](int st, auto edge) {
-            constexpr bool EDGE = decltype(edge)::value;  // some row does not see all of it
-            f32x4 sc[QT][4];
+          // EDGE: some row does not see all of it. MORE: another step of the unit follows, whose K is
+          // loaded when this one's is used up, and its V likewise. (A load that may or may not happen
+          // would make the waits for those in front of it as strict as if it did not.)
+          auto one_step = [&](int st, auto edge, auto more) {
+            constexpr bool EDGE = decltype(edge)::value, MORE = decltype(more)::value;
+            f32x4 sc[QT][PG];
 #pragma unroll
             for (int t = 0; t < QT; ++t)
 #pragma unroll
-              for (int p = 0; p < 4; ++p) sc[t][p] = f32x4{0, 0, 0, 0};
+              for (int p = 0; p < PG; ++p) sc[t][p] = f32x4{0, 0, 0, 0};
 #pragma unroll
-            for (int p = 0; p < 4; ++p)
+            for (int p = 0; p < PG; ++p)
 #pragma unroll
               for (int u = 0; u < 2 * KU; ++u) {
                 const uint32_t lo = elem(kr[p][u / 2], 2 * (u % 2));
@@ -336,25 +364,24 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                   sc[t][p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(w), qf[t][u], sc[t][p],
                                                                     0, 0, 0);
               }
-            // Past the last step it is loaded again: loads that may not happen would make the waits
-            // for those in front of them as strict as if they did not.
-            const int then = st + 1 < stop ? st + 1 : st;
-            if (then >> 4 != window) {
-              window = then >> 4;
-              load_ids();
-              load_scales();
-              // waited for here: later, the loads of K and V behind them would be, too
-              asm volatile("" : "+v"(ids), "+v"(ksc), "+v"(vsc));
+            if constexpr (MORE) {
+              if ((st + 1) * PG / 64 != window) {
+                window = (st + 1) * PG / 64;
+                load_ids();
+                load_scales();
+                // waited for here: later, the loads of K and V behind them would be, too
+                asm volatile("" : "+v"(ids), "+v"(ksc), "+v"(vsc));
+              }
+              load_k(st + 1);
+              take_scales(st + 1);
             }
-            load_k(then);
-            take_scales(then);
-            const int key0 = st * kStep + 4 * qd;
-            uint32_t ph[QT][4][2], pl[QT][4][2];
+            const int key0 = st * STEP + 4 * qd;
+            uint32_t ph[QT][PG][2], pl[QT][PG][2];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
               float top = -INFINITY;
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
+              for (int p = 0; p < PG; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                   if (EDGE && key0 + 16 * p + i >= see[t]) sc[t][p][i] = -INFINITY;
@@ -370,19 +397,19 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                 for (int c = 0; c < 4 * VW; ++c) acc[t][c] = acc[t][c] * corr;
                 m[t] = next;
               }
-              float x[4][4];
+              float x[PG][4];
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
+              for (int p = 0; p < PG; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) x[p][i] = __builtin_fmaf(sc[t][p][i], to_log2, -ref);
               if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ref) >= kLargeScore)) {
 #pragma unroll
-                for (int p = 0; p < 4; ++p)
+                for (int p = 0; p < PG; ++p)
 #pragma unroll
                   for (int i = 0; i < 4; ++i) x[p][i] = sc[t][p][i] * to_log2 - ref;
               }
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
+              for (int p = 0; p < PG; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
                   const float w0 = __builtin_amdgcn_exp2f(x[p][i]);
@@ -402,7 +429,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
               // reach the others through their zero weights: it is taken out and handed to its rows.
               uint32_t odd = 0;
 #pragma unroll
-              for (int p = 0; p < 4; ++p)
+              for (int p = 0; p < PG; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -413,7 +440,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                     vr[p][i][w] = b & ~((bad >> 7) * 0xFFu);
                   }
               if (__builtin_amdgcn_ballot_w64(odd != 0)) {
-                for (int key = st * kStep; key < (st + 1) * kStep && key < see_max; ++key) {
+                for (int key = st * STEP; key < (st + 1) * STEP && key < see_max; ++key) {
                   const size_t b = (size_t)pages[key / kPage] * a.n_kv_heads + h;
                   const uint8_t* src =
                       a.v_pool + (b * kPage + key % kPage) * HD + 16 * VW * qd;
@@ -429,7 +456,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
               }
             }
 #pragma unroll
-            for (int pp = 0; pp < 4; pp += 2)
+            for (int pp = 0; pp < PG; pp += 2)
 #pragma unroll
               for (int w = 0; w < VW; ++w)
 #pragma unroll
@@ -465,12 +492,14 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                     }
                   }
                 }
-            load_v();
+            if constexpr (MORE) {
+              load_v();
 #pragma unroll
-            for (int p = 0; p < 4; ++p) vs[p] = vs_next[p];
+              for (int p = 0; p < PG; ++p) vs[p] = vs_next[p];
+            }
           };
-          if (s != ids_of || step >> 4 != window) {
-            window = step >> 4;
+          if (s != ids_of || step * PG / 64 != window) {
+            window = step * PG / 64;
             ids_of = s;
             load_ids();
           }
@@ -479,23 +508,26 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
           load_v();
           take_scales(step);
 #pragma unroll
-          for (int p = 0; p < 4; ++p) vs[p] = vs_next[p];
-          const int inner = see_min / kStep < stop ? see_min / kStep : stop;
+          for (int p = 0; p < PG; ++p) vs[p] = vs_next[p];
+          const int inner = see_min / STEP < stop ? see_min / STEP : stop;
           int st = step;
-          for (; st < inner; ++st) one_step(st, std::false_type{});
-          for (; st < stop; ++st) one_step(st, std::true_type{});
+          for (; st < inner && st < stop - 1; ++st)
+            one_step(st, std::false_type{}, std::true_type{});
+          for (; st < stop - 1; ++st) one_step(st, std::true_type{}, std::true_type{});
+          if (st < inner)
+            one_step(st, std::false_type{}, std::false_type{});
+          else
+            one_step(st, std::true_type{}, std::false_type{});
         }
 
         const bool whole = step == 0 && stop == steps;
-        if (!whole && step == 0) {  // ends in another worker's share
-          const long long end = pos + ticks - upto;
-          open_last = (int)(((end << sh.log) - 1) / sh.total);
-          open_column = c0;
-          open_columns = columns;
-          open_seq = s;
-          open_head = h;
+        const int side = step == 0 ? 1 : 0;
+        if (!whole) {  // the workers of its first and last steps
+          const long long end = pos + ticks - upto, begin = end - steps;
+          note(side, (int)((((begin + 1) << sh.log) - 1) / sh.total),
+               (int)(((end << sh.log) - 1) / sh.total), c0, columns, s, h);
         }
-        const size_t slot = 2 * (size_t)worker + (step == 0 ? 1 : 0);
+        const size_t slot = 2 * (size_t)worker + side;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           float sum = l[t] + __shfl_xor(l[t], 16);
@@ -542,76 +574,74 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
           q = same(seq_of(a, ++s));
         }
         if (tile * C >= q.columns) break;
-        steps = same(tile_steps<C>(a, q, tile));
+        steps = same(tile_steps<HD, C>(a, q, tile));
       }
     }
-  }
-  if (shared_units && lane == 0) {
-    Open o = {};
-    o.last = open_last;
-    o.column = open_column;
-    o.columns = open_columns;
-    o.seq = open_seq;
-    o.head = open_head;
-    a.open[worker] = o;
   }
 }
 
-// Joins the parts of a unit: the one that its first worker left (an odd slot) and those of the
-// workers behind it (even slots). Block b looks at worker b.
+// Joins the parts of units: the one that a unit's first worker left (an odd slot) and those of the
+// workers behind it (even slots). Block b looks at the units that worker b has a part in: the n
+// workers of a unit share its columns and dims (4 to a thread) among their blocks, in up to n / 4
+// slices, and a block deals the parts out over the threads that a slice leaves, which meet in LDS.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs a, int C) {
-  constexpr int V = HD / 4;  // 4 dims to a thread
-  __shared__ f32x4 other[256];
-  __shared__ float2 other_ml[256];
-  const Open o = a.open[blockIdx.x];
-  if (o.last < 0) return;
-  const int tid = threadIdx.x, n = o.last - (int)blockIdx.x + 1;
-  // tasks (column, 4 dims) side by side, the parts dealt out over what threads are left
-  int lanes = V;
-  while (lanes < V * o.columns && lanes < 256) lanes *= 2;
-  const int deal = 256 / lanes, mine = tid / lanes;
-  const Seq q = seq_of(a, o.seq);
-  for (int task0 = 0; task0 < V * o.columns; task0 += lanes) {
-    const int task = task0 + tid % lanes, c = task / V, d = 4 * (task % V);
-    f32x4 acc = {0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
-    if (c < o.columns) {
-#pragma unroll 4
-      for (int j = mine; j < n; j += deal) {
-        const size_t slot = 2 * (size_t)(blockIdx.x + j) + (j == 0 ? 1 : 0);
-        const float2 ml = a.parts_ml[slot * C + c];
-        const f32x4 x = *reinterpret_cast<const f32x4*>(a.parts + (slot * C + c) * HD + d);
-        const float next = __builtin_fmaxf(m, ml.x), ref = next == -INFINITY ? 0.0f : next;
-        const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(ml.x - ref);
-        acc = acc * wa + x * wb;
-        l = l * wa + ml.y * wb;
-        m = next;
-      }
+  constexpr int V = HD / 4;
+  __shared__ f32x4 others[256];
+  __shared__ float2 others_ml[256];
+  const int tid = threadIdx.x, worker = blockIdx.x;
+  struct Joint {
+    f32x4 acc;
+    float m, l;
+    __device__ __forceinline__ void add(f32x4 x, float2 ml) {
+      const float next = __builtin_fmaxf(m, ml.x), ref = next == -INFINITY ? 0.0f : next;
+      const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(ml.x - ref);
+      acc = acc * wa + x * wb;
+      l = l * wa + ml.y * wb;
+      m = next;
     }
-    __syncthreads();
-    other[tid] = acc;
-    other_ml[tid] = make_float2(m, l);
-    __syncthreads();
-    if (mine == 0 && c < o.columns) {
-      for (int k = 1; k < deal; ++k) {
-        const float2 ml = other_ml[tid + k * lanes];
-        const float next = __builtin_fmaxf(m, ml.x), ref = next == -INFINITY ? 0.0f : next;
-        const float wa = __builtin_amdgcn_exp2f(m - ref), wb = __builtin_amdgcn_exp2f(ml.x - ref);
-        acc = acc * wa + other[tid + k * lanes] * wb;
-        l = l * wa + ml.y * wb;
-        m = next;
+  };
+  for (int side = 0; side < 2; ++side) {
+    const Shared o = a.shared[2 * worker + side];
+    if (o.first > o.last) continue;
+    const int n = o.last - o.first + 1, tasks = V * o.columns;
+    int width = 16, slices = 1;  // tasks of a slice
+    while (width < tasks) width *= 2;
+    while (8 * slices <= n && width > 16) {
+      slices *= 2;
+      width /= 2;
+    }
+    const int slice = worker - o.first;
+    if (slice >= slices) continue;
+    const int lanes = width < 256 ? width : 256, deal = 256 / lanes, turn = tid / lanes;
+    const Seq q = seq_of(a, o.seq);
+    for (int task0 = slice * width; task0 < (slice + 1) * width; task0 += lanes) {
+      const int task = task0 + tid % lanes, c = task / V, d = 4 * (task % V);
+      Joint r = {f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
+      if (c < o.columns) {
+#pragma unroll 4
+        for (int j = turn; j < n; j += deal) {
+          const size_t at = (2 * (size_t)(o.first + j) + (j == 0 ? 1 : 0)) * C + c;
+          r.add(*reinterpret_cast<const f32x4*>(a.parts + at * HD + d), a.parts_ml[at]);
+        }
       }
-      const int col = o.column + c;
-      const bool any = seen(a, q, col) > 0;
-      f16x2 y[2];
+      __syncthreads();
+      others[tid] = r.acc;
+      others_ml[tid] = make_float2(r.m, r.l);
+      __syncthreads();
+      if (turn == 0 && c < o.columns) {
+        for (int k = 1; k < deal && k < n; ++k) r.add(others[tid + k * lanes], others_ml[tid + k * lanes]);
+        const int col = o.column + c;
+        const bool any = seen(a, q, col) > 0;
+        f16x2 y[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e / 2][e % 2] = any ? (f16)(acc[e] / l) : (f16)0;
-      uint2 v;
-      v.x = __builtin_bit_cast(uint32_t, y[0]);
-      v.y = __builtin_bit_cast(uint32_t, y[1]);
-      *reinterpret_cast<uint2*>(a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads +
-                                         o.head * a.group + col % a.group) * HD + d) = v;
+        for (int e = 0; e < 4; ++e) y[e / 2][e % 2] = any ? (f16)(r.acc[e] / r.l) : (f16)0;
+        uint2 v;
+        v.x = __builtin_bit_cast(uint32_t, y[0]);
+        v.y = __builtin_bit_cast(uint32_t, y[1]);
+        *reinterpret_cast<uint2*>(a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads +
+                                           o.head * a.group + col % a.group) * HD + d) = v;
+      }
     }
   }
 }
@@ -638,7 +668,7 @@ using namespace llmk;
 
 extern "C" size_t llmk_kv8_attention_workspace_floats(int head_dim) {
   if (head_dim != 64 && head_dim != 128) return 0;
-  return (size_t)kSlotColumns * (head_dim + 2) + kWorkers * (sizeof(Open) / 4);
+  return (size_t)kSlotColumns * (head_dim + 2) + 2 * kWorkers * (sizeof(Shared) / 4);
 }
 
 extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, const float* k_scale,
@@ -675,7 +705,7 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
   a.out = reinterpret_cast<f16*>(out);
   a.parts = workspace;
   a.parts_ml = reinterpret_cast<float2*>(workspace + (size_t)kSlotColumns * head_dim);
-  a.open = reinterpret_cast<Open*>(workspace + (size_t)kSlotColumns * (head_dim + 2));
+  a.shared = reinterpret_cast<Shared*>(workspace + (size_t)kSlotColumns * (head_dim + 2));
   a.n_heads = n_heads;
   a.n_kv_heads = n_kv_heads;
   a.group = n_heads / n_kv_heads;
