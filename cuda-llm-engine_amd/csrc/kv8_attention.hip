@@ -12,6 +12,7 @@ namespace {
 using namespace kv8;
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -21,13 +22,29 @@ constexpr float kLog2e = 1.44269504088896341f;
 // weights nor sums mind; from there on exponents are made in two steps, and the largest weight is 1.
 constexpr float kLargeScore = 1073741824.0f;
 constexpr int kStart = 2;                       // what a unit's first loads cost, in steps
-constexpr int kSlotColumns = 65536;             // of partial results in the workspace
+constexpr int kFewColumns = 32, kManyColumns = 128;
+// Workers of a launch, waves and blocks: what fits the 256 CUs at once.
+template <int HD, int QT>
+constexpr int kFewWorkers = QT == 1 ? 2048 : 1024;
+template <int HD>
+constexpr int kManyWorkers = 512;
 constexpr int kWorkers = 2048;                  // at most
+constexpr int kSlotColumns = 131072;            // of partial results in the workspace
 
 template <bool HIGH>
 __device__ __forceinline__ uint32_t bf16_from_e4m3(uint32_t bytes, float scale) {
   return __builtin_bit_cast(uint32_t,
                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, scale, HIGH));
+}
+
+// Two weights as packed bf16, their first 8 bits (cut off) and the rest rounded to 8.
+__device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+  hi = __builtin_amdgcn_perm(y, x, 0x07060302);
+  const float ra = a - __builtin_bit_cast(float, x & 0xFFFF0000u);
+  const float rb = b - __builtin_bit_cast(float, y & 0xFFFF0000u);
+  const bf16x2 r = {(__bf16)ra, (__bf16)rb};
+  lo = __builtin_bit_cast(uint32_t, r);
 }
 
 // A unit that several workers share, as each of them notes it for the launch that joins its parts: one
@@ -50,7 +67,8 @@ struct AttentionArgs {
   float* parts;  // [2 workers][columns of a tile][HD], NULL: no unit is shared
   float2* parts_ml;
   Shared* shared;  // [2 workers]
-  int n_heads, n_kv_heads, group, log_workers, min_ticks;
+  int n_heads, n_kv_heads, group, workers;
+  int least_columns, most_columns;  // of the sequences that a launch takes
 };
 
 // A sequence's rows in this call and what they see.
@@ -72,6 +90,7 @@ __device__ __forceinline__ Seq seq_of(const AttentionArgs& a, int s) {
   r1 = r1 > a.batch.n_rows ? a.batch.n_rows : r1;
   q.row0 = r0;
   q.columns = r1 > r0 ? (r1 - r0) * a.group : 0;
+  if (q.columns < a.least_columns || q.columns > a.most_columns) q.columns = 0;  // not this launch's
   const long long table = (long long)a.batch.max_pages * kPage;
   q.limit = len < table ? len : table;
   return q;
@@ -121,16 +140,26 @@ __device__ __forceinline__ Seq same(Seq q) {
 }
 
 // Where the share of each of a block's workers begins among the ticks of all units, which are
-// ordered by sequence, tile and kv head. By all 256 threads.
+// ordered by sequence, tile and kv head. By all 256 threads; workers are waves or blocks.
 struct Share {
-  long long total;
-  int log;  // workers: 2^log
-  long long begin, end;  // of this wave
-  int seq;               // that holds begin, and begin's place in it
-  long long at;
+  int seq;               // that holds the beginning of this worker's share, and
+  long long at;          // its place in it
+  long long begin, end;  // among all ticks
+  long long each;        // of the first `more` workers one more
+  int more;
+  __device__ __forceinline__ long long begin_of(int worker) const {
+    return each * worker + (worker < more ? worker : more);
+  }
+  __device__ __forceinline__ int worker_at(long long tick) const {
+    const long long wide = (each + 1) * more;
+    return (int)(tick < wide ? divide(tick, each + 1) : more + divide(tick - wide, each));
+  }
+  static __device__ __forceinline__ long long divide(long long a, long long b) {  // b > 0 where used
+    return (uint64_t)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+  }
 };
-template <int HD, int C>
-__device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, int log_workers) {
+template <int HD, int C, bool WAVES>
+__device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker) {
   __shared__ long long wave_sum_[4], at_[4];
   __shared__ int seq_[4];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -147,20 +176,22 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
   if (lane == 63) wave_sum_[wave] = upto;
   __syncthreads();
   Share r;
-  long long base = 0;
-  r.total = 0;
+  long long base = 0, total = 0;
   for (int w = 0; w < 4; ++w) {
     if (w < wave) base += wave_sum_[w];
-    r.total += wave_sum_[w];
+    total += wave_sum_[w];
   }
-  r.log = log_workers;
-  while (r.log > 0 && (r.total >> r.log) < a.min_ticks) --r.log;
+  total = same(total);
+  int workers = a.workers;
+  if (total < workers) workers = total > 0 ? (int)total : 1;
+  r.each = Share::divide(total, workers);
+  r.more = (int)(total - r.each * workers);
   const long long from = base + upto - mine;
-  const int first = worker - wave * (int)gridDim.x;  // the workers of a block are a grid apart
-  for (int w = 0; w < 4; ++w) {
+  const int first = blockIdx.x;  // the workers of a block are a grid apart
+  for (int w = 0; w < (WAVES ? 4 : 1); ++w) {
     const int id = first + w * (int)gridDim.x;
-    const long long x = (r.total * id) >> r.log;
-    if (x >= from && x < from + mine) {
+    const long long x = r.begin_of(id);
+    if (id < workers && x >= from && x < from + mine) {
       long long left = x - from;
       int s = s0;
       for (; s < s1 - 1; ++s) {
@@ -173,13 +204,10 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker, 
     }
   }
   __syncthreads();
-  r.total = same(r.total);
-  r.log = __builtin_amdgcn_readfirstlane(r.log);
-  r.begin = (r.total * worker) >> r.log;
-  r.end = (r.total * (worker + 1)) >> r.log;
-  if (worker >= 1 << r.log) r.begin = r.end = r.total;
-  r.seq = __builtin_amdgcn_readfirstlane(seq_[wave]);
-  r.at = same(at_[wave]);
+  r.begin = worker < workers ? r.begin_of(worker) : total;
+  r.end = worker < workers ? r.begin_of(worker + 1) : total;
+  r.seq = __builtin_amdgcn_readfirstlane(seq_[WAVES ? wave : 0]);
+  r.at = same(at_[WAVES ? wave : 0]);
   return r;
 }
 
@@ -211,7 +239,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int worker = wave * (int)gridDim.x + (int)blockIdx.x;
   const bool shared_units = a.parts != nullptr;
-  const Share sh = find_share<HD, C>(a, worker, a.log_workers);
+  const Share sh = find_share<HD, C, true>(a, worker);
   auto note = [&](int side, int first, int last, int column, int columns, int seq, int head) {
     Shared o = {};
     o.first = first;
@@ -338,11 +366,12 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
               }
             }
           };
-          // EDGE: some row does not see all of it. MORE: another step of the unit follows, whose K is
-          // loaded when this one's is used up, and its V likewise. (A load that may or may not happen
-          // would make the waits for those in front of it as strict as if it did not.)
-          auto one_step = [&](int st, auto edge, auto more) {
-            constexpr bool EDGE = decltype(edge)::value, MORE = decltype(more)::value;
+          // MORE: another step of the unit follows, whose K is loaded when this one's is used up, and its
+          // V likewise. (A load that may or may not happen would make the waits for those in front of
+          // it as strict as if it did not.)
+          auto one_step = [&](int st, auto more) {
+            constexpr bool MORE = decltype(more)::value;
+            const bool edge = (st + 1) * STEP > see_min;  // some row does not see all of it
             f32x4 sc[QT][PG];
 #pragma unroll
             for (int t = 0; t < QT; ++t)
@@ -379,14 +408,19 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
             uint32_t ph[QT][PG][2], pl[QT][PG][2];
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
+              if (edge) {
+                asm volatile("" ::: "memory");  // a branch, not selects in every step
+#pragma unroll
+                for (int p = 0; p < PG; ++p)
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    if (key0 + 16 * p + i >= see[t]) sc[t][p][i] = -INFINITY;
+              }
               float top = -INFINITY;
 #pragma unroll
               for (int p = 0; p < PG; ++p)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  if (EDGE && key0 + 16 * p + i >= see[t]) sc[t][p][i] = -INFINITY;
-                  top = __builtin_fmaxf(top, sc[t][p][i]);
-                }
+                for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, sc[t][p][i]);
               top = max_of_quarters(top) * to_log2;
               const float next = __builtin_fmaxf(m[t], top);
               const float ref = next == -INFINITY ? 0.0f : next;
@@ -397,34 +431,27 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                 for (int c = 0; c < 4 * VW; ++c) acc[t][c] = acc[t][c] * corr;
                 m[t] = next;
               }
-              float x[PG][4];
-#pragma unroll
-              for (int p = 0; p < PG; ++p)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[p][i] = __builtin_fmaf(sc[t][p][i], to_log2, -ref);
+              float scale = to_log2;
               if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ref) >= kLargeScore)) {
+                asm volatile("" ::: "memory");
+                scale = 1.0f;
 #pragma unroll
-                for (int p = 0; p < PG; ++p)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) x[p][i] = sc[t][p][i] * to_log2 - ref;
+                for (int p = 0; p < PG; ++p) sc[t][p] = sc[t][p] * to_log2;
               }
 #pragma unroll
               for (int p = 0; p < PG; ++p)
 #pragma unroll
                 for (int i = 0; i < 4; i += 2) {
-                  const float w0 = __builtin_amdgcn_exp2f(x[p][i]);
-                  const float w1 = __builtin_amdgcn_exp2f(x[p][i + 1]);
+                  const float w0 =
+                      __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][p][i], scale, -ref));
+                  const float w1 =
+                      __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][p][i + 1], scale, -ref));
                   l[t] = l[t] + (w0 + w1);
-                  const uint32_t b0 = __builtin_bit_cast(uint32_t, w0);
-                  const uint32_t b1 = __builtin_bit_cast(uint32_t, w1);
-                  ph[t][p][i / 2] = __builtin_amdgcn_perm(b1, b0, 0x07060302);
-                  const float r0 = w0 - __builtin_bit_cast(float, b0 & 0xFFFF0000u);
-                  const float r1 = w1 - __builtin_bit_cast(float, b1 & 0xFFFF0000u);
-                  const bf16x2 r = {(__bf16)r0, (__bf16)r1};
-                  pl[t][p][i / 2] = __builtin_bit_cast(uint32_t, r);
+                  split(w0, w1, ph[t][p][i / 2], pl[t][p][i / 2]);
                 }
             }
-            if constexpr (EDGE) {
+            if (edge) {
+              asm volatile("" ::: "memory");
               // What no row sees is stale: zero. A NaN of a position that only some rows see would
               // reach the others through their zero weights: it is taken out and handed to its rows.
               uint32_t odd = 0;
@@ -447,11 +474,17 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 #pragma unroll
                   for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int c = 0; c < 4 * VW; ++c)
-                      if ((src[4 * VW * i + c] & 0x7F) == 0x7F)
+                    for (int w = 0; w < VW; ++w) {
+                      const uint32_t x = reinterpret_cast<const uint32_t*>(src)[VW * i + w];
 #pragma unroll
-                        for (int t = 0; t < QT; ++t)
-                          if (key < see[t]) acc[t][c][i] = __builtin_nanf("");
+                      for (int c = 0; c < 4; ++c)
+#pragma unroll
+                        for (int t = 0; t < QT; ++t) {
+                          const bool bad = key < see[t] && ((x >> (8 * c)) & 0x7Fu) == 0x7Fu;
+                          f32x4& o = acc[t][4 * w + c];
+                          o[i] = bad ? __builtin_nanf("") : o[i];
+                        }
+                    }
                 }
               }
             }
@@ -509,23 +542,16 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
           take_scales(step);
 #pragma unroll
           for (int p = 0; p < PG; ++p) vs[p] = vs_next[p];
-          const int inner = see_min / STEP < stop ? see_min / STEP : stop;
           int st = step;
-          for (; st < inner && st < stop - 1; ++st)
-            one_step(st, std::false_type{}, std::true_type{});
-          for (; st < stop - 1; ++st) one_step(st, std::true_type{}, std::true_type{});
-          if (st < inner)
-            one_step(st, std::false_type{}, std::false_type{});
-          else
-            one_step(st, std::true_type{}, std::false_type{});
+          for (; st < stop - 1; ++st) one_step(st, std::true_type{});
+          one_step(st, std::false_type{});
         }
 
         const bool whole = step == 0 && stop == steps;
         const int side = step == 0 ? 1 : 0;
         if (!whole) {  // the workers of its first and last steps
           const long long end = pos + ticks - upto, begin = end - steps;
-          note(side, (int)((((begin + 1) << sh.log) - 1) / sh.total),
-               (int)(((end << sh.log) - 1) / sh.total), c0, columns, s, h);
+          note(side, sh.worker_at(begin), sh.worker_at(end - 1), c0, columns, s, h);
         }
         const size_t slot = 2 * (size_t)worker + side;
 #pragma unroll
@@ -581,9 +607,10 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 }
 
 // Joins the parts of units: the one that a unit's first worker left (an odd slot) and those of the
-// workers behind it (even slots). Block b looks at the units that worker b has a part in: the n
-// workers of a unit share its columns and dims (4 to a thread) among their blocks, in up to n / 4
-// slices, and a block deals the parts out over the threads that a slice leaves, which meet in LDS.
+// workers behind it (even slots). Block (b, y) looks at the units that worker b has a part in, at the
+// y-th 256 of their tasks (a column's 4 dims). The n workers of a unit share them among their blocks,
+// in up to n / 4 slices, and a block deals the parts out over the threads that a slice leaves, which
+// meet in LDS.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs a, int C) {
   constexpr int V = HD / 4;
@@ -604,61 +631,395 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
   for (int side = 0; side < 2; ++side) {
     const Shared o = a.shared[2 * worker + side];
     if (o.first > o.last) continue;
-    const int n = o.last - o.first + 1, tasks = V * o.columns;
-    int width = 16, slices = 1;  // tasks of a slice
-    while (width < tasks) width *= 2;
-    while (8 * slices <= n && width > 16) {
+    const int n = o.last - o.first + 1, base = 256 * blockIdx.y;
+    const int tasks = V * o.columns - base < 256 ? V * o.columns - base : 256;
+    if (tasks <= 0) continue;
+    int lanes = 16, slices = 1;  // tasks of a slice
+    while (lanes < tasks) lanes *= 2;
+    while (8 * slices <= n && lanes > 16) {
       slices *= 2;
-      width /= 2;
+      lanes /= 2;
     }
     const int slice = worker - o.first;
     if (slice >= slices) continue;
-    const int lanes = width < 256 ? width : 256, deal = 256 / lanes, turn = tid / lanes;
+    const int deal = 256 / lanes, turn = tid / lanes;
+    const int task = base + slice * lanes + tid % lanes, c = task / V, d = 4 * (task % V);
     const Seq q = seq_of(a, o.seq);
-    for (int task0 = slice * width; task0 < (slice + 1) * width; task0 += lanes) {
-      const int task = task0 + tid % lanes, c = task / V, d = 4 * (task % V);
-      Joint r = {f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
-      if (c < o.columns) {
+    Joint r = {f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
+    if (c < o.columns) {
 #pragma unroll 4
-        for (int j = turn; j < n; j += deal) {
-          const size_t at = (2 * (size_t)(o.first + j) + (j == 0 ? 1 : 0)) * C + c;
-          r.add(*reinterpret_cast<const f32x4*>(a.parts + at * HD + d), a.parts_ml[at]);
-        }
+      for (int j = turn; j < n; j += deal) {
+        const size_t at = (2 * (size_t)(o.first + j) + (j == 0 ? 1 : 0)) * C + c;
+        r.add(*reinterpret_cast<const f32x4*>(a.parts + at * HD + d), a.parts_ml[at]);
       }
-      __syncthreads();
-      others[tid] = r.acc;
-      others_ml[tid] = make_float2(r.m, r.l);
-      __syncthreads();
-      if (turn == 0 && c < o.columns) {
-        for (int k = 1; k < deal && k < n; ++k) r.add(others[tid + k * lanes], others_ml[tid + k * lanes]);
-        const int col = o.column + c;
-        const bool any = seen(a, q, col) > 0;
-        f16x2 y[2];
+    }
+    __syncthreads();
+    others[tid] = r.acc;
+    others_ml[tid] = make_float2(r.m, r.l);
+    __syncthreads();
+    if (turn == 0 && c < o.columns) {
+      for (int k = 1; k < deal && k < n; ++k)
+        r.add(others[tid + k * lanes], others_ml[tid + k * lanes]);
+      const int col = o.column + c;
+      const bool any = seen(a, q, col) > 0;
+      f16x2 y[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) y[e / 2][e % 2] = any ? (f16)(r.acc[e] / r.l) : (f16)0;
-        uint2 v;
-        v.x = __builtin_bit_cast(uint32_t, y[0]);
-        v.y = __builtin_bit_cast(uint32_t, y[1]);
-        *reinterpret_cast<uint2*>(a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads +
-                                           o.head * a.group + col % a.group) * HD + d) = v;
-      }
+      for (int e = 0; e < 4; ++e) y[e / 2][e % 2] = any ? (f16)(r.acc[e] / r.l) : (f16)0;
+      uint2 v;
+      v.x = __builtin_bit_cast(uint32_t, y[0]);
+      v.y = __builtin_bit_cast(uint32_t, y[1]);
+      *reinterpret_cast<uint2*>(a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads +
+                                         o.head * a.group + col % a.group) * HD + d) = v;
     }
   }
 }
 
-template <int HD, int QT>
-int few_launch(AttentionArgs a, hipStream_t stream) {
-  a.log_workers = QT == 1 ? 11 : 10;
-  const int workers = 1 << a.log_workers;
-  const int st = launch(k_kv8_attention_few<HD, QT>, dim3(workers / 4), dim3(256), 0, stream, a);
-  if (st != LLMK_OK || !a.parts) return st;
-  return launch(k_kv8_attention_join<HD>, dim3(workers), dim3(256), 0, stream, a, 16 * QT);
+// Units of many columns, a block each: 4 waves of 32 columns share the K and V of a step through LDS,
+// where they arrive as fp16 and bf16 (each wave converts a quarter). Per wave
+//   S^T = K Q^T    (v_mfma_f32_32x32x16_f16; A: 32 positions of K, B: 32 columns of q)
+//   O^T += V^T P^T (.._bf16; A: 32 dims of V, B: the lane's own weights)
+// Lane l gets of S^T column l % 32, positions 8 (i / 4) + 4 (l / 32) + i % 4; V's positions lie in LDS
+// in the order in which that makes 8 of them a lane's share of a contraction.
+template <int HD>
+__global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionArgs a) {
+  constexpr int C = kManyColumns, PG = kPages<HD>, STEP = kStep<HD>, KT = STEP / 32, DT = HD / 32;
+  constexpr int KP = HD / 16, VP = HD / 4;  // threads to a position of K, to 4 positions of V
+  // One piece of 16 bytes behind each row: 8 lanes that read a piece of as many rows meet no bank
+  // twice, and every address is a lane's base and a constant.
+  __shared__ u32x4 k_lds[2][STEP][HD / 8 + 1];  // [position][8 dims]
+  __shared__ u32x4 v_lds[2][HD][STEP / 8 + 1];  // [dim][8 positions]
+  __shared__ int odd[2];  // a NaN was taken out of V: of a unit, and of the next
+  const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
+  const int wave = same(tid >> 6), worker = blockIdx.x;
+  const bool shared_units = a.parts != nullptr;
+  int turn = 0;
+  if (tid < 2) odd[tid] = 0;
+  const Share sh = find_share<HD, C, false>(a, worker);
+  auto note = [&](int side, int first, int last, int column, int columns, int seq, int head) {
+    Shared o = {};
+    o.first = first;
+    o.last = last;
+    o.column = column;
+    o.columns = columns;
+    o.seq = seq;
+    o.head = head;
+    if (tid == 0) a.shared[2 * worker + side] = o;
+  };
+  if (shared_units) {
+    note(0, 0, -1, 0, 0, 0, 0);
+    note(1, 0, -1, 0, 0, 0, 0);
+  }
+  long long pos = sh.begin;
+  if (pos >= sh.end) return;
+  int s = sh.seq, tile = 0;
+  Seq q = same(seq_of(a, s));
+  long long at = sh.at;
+  int steps;
+  for (;;) {
+    steps = same(tile_steps<HD, C>(a, q, tile));
+    const long long ticks = (long long)(kStart + steps) * a.n_kv_heads;
+    if (at < ticks) break;
+    at -= ticks;
+    ++tile;
+  }
+  int h = same((int)at / (kStart + steps)), tick = same((int)at % (kStart + steps));
+  const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
+
+  while (pos < sh.end) {
+    const int ticks = kStart + steps;
+    int upto = ticks;  // this worker's end of the unit
+    if (shared_units && sh.end - pos < ticks - tick) upto = tick + (int)(sh.end - pos);
+    const int step = tick > kStart ? tick - kStart : 0;
+    const int stop = same(upto > kStart ? upto - kStart : 0);
+    pos += upto - tick;
+    if (stop > step && (shared_units || tick == 0)) {
+      const int c0 = tile * C;
+      const int columns = q.columns - c0 < C ? q.columns - c0 : C;
+      const int see_max = same(seen(a, q, c0 + columns - 1)), see_min = same(seen(a, q, c0));
+      const int* pages = a.batch.tables + (size_t)s * a.batch.max_pages;
+      const int last_page = (int)((q.limit + kPage - 1) / kPage) - 1;
+
+      // this wave's columns
+      const int first_own = 32 * wave, c = first_own + n;
+      const bool own = c < columns;
+      const int col = c0 + (own ? c : 0);
+      const int see = own ? seen(a, q, col) : 0;
+      const int last_own = first_own + 31 < columns ? first_own + 31 : columns - 1;
+      const int wave_max = first_own < columns ? same(seen(a, q, c0 + last_own)) : 0;
+      const int wave_min = first_own + 31 < columns ? same(seen(a, q, c0 + first_own)) : 0;
+      const f16* src = a.q + ((size_t)(q.row0 + col / a.group) * a.n_heads + h * a.group +
+                              col % a.group) * HD + 8 * half;
+      f16x8 qf[HD / 16];
+#pragma unroll
+      for (int u = 0; u < HD / 16; ++u) qf[u] = own ? as_h8(ld16(src + 16 * u)) : (f16x8)(f16)0;
+      float m = -INFINITY, l = 0.0f;
+      f32x16 acc[DT];
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) acc[d][i] = 0.0f;
+
+      if (see_max > 0) {
+        // 64 table entries, one to a lane, and their scales; the wave's page of a step on its way
+        int window = -1, ids = 0;
+        float ksc = 0, vsc = 0, ks = 0, vs = 0;
+        u32x4 kr;
+        uint32_t vr[4];
+        const int k_key = tid / KP, k_part = tid % KP, v_key = 4 * (tid / VP), v_part = tid % VP;
+        auto load = [&](int st) {
+          const int w = st * PG / 64;
+          if (w != window) {
+            window = w;
+            const int p = 64 * w + lane;
+            ids = pages[p < last_page ? p : last_page];
+            const size_t b = (size_t)ids * a.n_kv_heads + h;
+            ksc = a.k_scale[b];
+            vsc = a.v_scale[b];
+          }
+          const int i = (PG * st + wave * PG / 4) & 63;  // the page of this wave's quarter
+          const size_t block = ((size_t)__builtin_amdgcn_readlane(ids, i) * a.n_kv_heads + h) *
+                               (size_t)(kPage * HD);
+          kr = ld16(a.k_pool + block + (uint32_t)(k_key % kPage * HD + 16 * k_part));
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4)
+            vr[i4] = *reinterpret_cast<const uint32_t*>(
+                a.v_pool + block + (uint32_t)((v_key % kPage + i4) * HD + 4 * v_part));
+          ks = readlane_f32(ksc, i);
+          vs = readlane_f32(vsc, i);
+        };
+        auto store = [&](int st, int buf) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const uint32_t x = elem(kr, 2 * j), y = elem(kr, 2 * j + 1);
+            u32x4 w;
+            w[0] = __builtin_bit_cast(uint32_t, from_e4m3<false>(x, ks));
+            w[1] = __builtin_bit_cast(uint32_t, from_e4m3<true>(x, ks));
+            w[2] = __builtin_bit_cast(uint32_t, from_e4m3<false>(y, ks));
+            w[3] = __builtin_bit_cast(uint32_t, from_e4m3<true>(y, ks));
+            k_lds[buf][k_key][2 * k_part + j] = w;
+          }
+          if ((st + 1) * STEP > see_min) {
+            // What no row sees is stale: zero. A NaN of a position that only some rows see would
+            // reach the others through their zero weights: it is handed to its rows at the end.
+            uint32_t bad = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const uint32_t b = st * STEP + v_key + i < see_max ? vr[i] : 0u;
+              const uint32_t x = ((b & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+              bad |= x;
+              vr[i] = b & ~((x >> 7) * 0xFFu);
+            }
+            if (bad) odd[turn] = 1;
+          }
+          const int t = v_key / 4, piece = 2 * (t / 4) + (t & 1);
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            constexpr uint32_t sel[2] = {0x05010400u, 0x07030602u};
+            const uint32_t x01 = __builtin_amdgcn_perm(vr[1], vr[0], sel[g]);
+            const uint32_t x23 = __builtin_amdgcn_perm(vr[3], vr[2], sel[g]);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = 4 * v_part + 2 * g + e;
+              u32x2 y;
+              y[0] = e ? bf16_from_e4m3<true>(x01, vs) : bf16_from_e4m3<false>(x01, vs);
+              y[1] = e ? bf16_from_e4m3<true>(x23, vs) : bf16_from_e4m3<false>(x23, vs);
+              reinterpret_cast<u32x2*>(&v_lds[buf][d][piece])[(t >> 1) & 1] = y;
+            }
+          }
+        };
+        auto compute = [&](int st, int buf) {
+          f32x16 sc[KT];
+#pragma unroll
+          for (int t = 0; t < KT; ++t) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
+#pragma unroll
+            for (int u = 0; u < HD / 16; ++u)
+              sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                  as_h8(k_lds[buf][32 * t + n][2 * u + half]), qf[u], sc[t], 0, 0, 0);
+          }
+          if ((st + 1) * STEP > wave_min) {  // some row does not see all of it
+            asm volatile("" ::: "memory");  // a branch, not selects in every step
+            const int key0 = st * STEP + 4 * half;
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (key0 + 32 * t + 8 * (i / 4) + i % 4 >= see) sc[t][i] = -INFINITY;
+          }
+          float top = sc[0][0];
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sc[t][i]);
+          top = max_across(top, true) * to_log2;
+          const float next = __builtin_fmaxf(m, top);
+          const float ref = next == -INFINITY ? 0.0f : next;
+          if (__builtin_amdgcn_ballot_w64(next != m)) {
+            const float corr = __builtin_amdgcn_exp2f(m - ref);
+            l = l * corr;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) acc[d][i] = acc[d][i] * corr;
+            m = next;
+          }
+          float scale = to_log2;
+          if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ref) >= kLargeScore)) {
+            asm volatile("" ::: "memory");
+            scale = 1.0f;
+#pragma unroll
+            for (int t = 0; t < KT; ++t)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) sc[t][i] = sc[t][i] * to_log2;
+          }
+#pragma unroll
+          for (int cc = 0; cc < 2 * KT; ++cc) {  // 16 positions
+            uint32_t ph[4], pl[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int i = 8 * (cc % 2) + 2 * e;
+              const float w0 =
+                  __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc / 2][i], scale, -ref));
+              const float w1 =
+                  __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc / 2][i + 1], scale, -ref));
+              l = l + (w0 + w1);
+              split(w0, w1, ph[e], pl[e]);
+            }
+            const bf16x8 hi = __builtin_bit_cast(bf16x8, (u32x4{ph[0], ph[1], ph[2], ph[3]}));
+            const bf16x8 lo = __builtin_bit_cast(bf16x8, (u32x4{pl[0], pl[1], pl[2], pl[3]}));
+#pragma unroll
+            for (int d = 0; d < DT; ++d) {
+              const bf16x8 vf = __builtin_bit_cast(bf16x8, v_lds[buf][32 * d + n][2 * cc + half]);
+              acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, hi, acc[d], 0, 0, 0);
+              acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo, acc[d], 0, 0, 0);
+            }
+          }
+        };
+        load(step);
+        lds_barrier();  // the unit before is done with
+        if (tid == 0) odd[turn ^ 1] = 0;
+        store(step, 0);
+        if (step + 1 < stop) load(step + 1);
+        lds_barrier();
+        for (int st = step; st < stop; ++st) {
+          const int buf = (st - step) & 1;
+          if (st * STEP < wave_max) compute(st, buf);
+          if (st + 1 < stop) {
+            store(st + 1, buf ^ 1);
+            if (st + 2 < stop) load(st + 2);
+          }
+          lds_barrier();
+        }
+        if (odd[turn]) {
+          int key = see_min / STEP * STEP;
+          key = key > step * STEP ? key : step * STEP;
+          for (; key < stop * STEP && key < see_max; ++key) {
+            const size_t b = (size_t)pages[key / kPage] * a.n_kv_heads + h;
+            const uint8_t* v = a.v_pool + (b * kPage + key % kPage) * HD + 4 * half;
+#pragma unroll
+            for (int d = 0; d < DT; ++d)
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                const uint32_t b = *reinterpret_cast<const uint32_t*>(v + 32 * d + 8 * g);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const bool bad = key < see && ((b >> (8 * e)) & 0x7Fu) == 0x7Fu;
+                  acc[d][4 * g + e] = bad ? __builtin_nanf("") : acc[d][4 * g + e];
+                }
+              }
+          }
+        }
+        turn ^= 1;
+      }
+
+      const bool whole = step == 0 && stop == steps;
+      const int side = step == 0 ? 1 : 0;
+      if (!whole) {  // the workers of its first and last steps
+        const long long end = pos + ticks - upto, begin = end - steps;
+        note(side, sh.worker_at(begin), sh.worker_at(end - 1), c0, columns, s, h);
+      }
+      l = l + __shfl_xor(l, 32);
+      if (own && whole) {
+        f16* dst = a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads + h * a.group +
+                            col % a.group) * HD + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            f16x2 o[2];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              o[e / 2][e % 2] = see > 0 ? (f16)(acc[d][4 * g + e] / l) : (f16)0;
+            uint2 v;
+            v.x = __builtin_bit_cast(uint32_t, o[0]);
+            v.y = __builtin_bit_cast(uint32_t, o[1]);
+            *reinterpret_cast<uint2*>(dst + 32 * d + 8 * g) = v;
+          }
+      } else if (own) {
+        const size_t slot = (2 * (size_t)worker + side) * C + c;
+        float* dst = a.parts + slot * HD + 4 * half;
+#pragma unroll
+        for (int d = 0; d < DT; ++d)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * g) =
+                f32x4{acc[d][4 * g], acc[d][4 * g + 1], acc[d][4 * g + 2], acc[d][4 * g + 3]};
+        if (half == 0) a.parts_ml[slot] = make_float2(m, l);
+      }
+    }
+    tick = 0;
+    if (++h == a.n_kv_heads) {
+      h = 0;
+      ++tile;
+      while (tile * C >= q.columns && s < a.batch.n_seqs - 1) {
+        tile = 0;
+        q = same(seq_of(a, ++s));
+      }
+      if (tile * C >= q.columns) break;
+      steps = same(tile_steps<HD, C>(a, q, tile));
+    }
+  }
 }
 
 template <int HD>
-int attention_launch(const AttentionArgs& a, int max_rows, hipStream_t stream) {
-  return (long long)max_rows * a.group <= 16 ? few_launch<HD, 1>(a, stream)
-                                             : few_launch<HD, 2>(a, stream);
+int join_launch(const AttentionArgs& a, int columns, hipStream_t stream) {
+  if (!a.parts) return LLMK_OK;
+  return launch(k_kv8_attention_join<HD>, dim3(a.workers, columns * HD / 1024), dim3(256), 0,
+                stream, a, columns);
+}
+
+template <int HD, int QT>
+int few_launch(AttentionArgs a, hipStream_t stream) {
+  a.workers = kFewWorkers<HD, QT>;
+  const int st =
+      launch(k_kv8_attention_few<HD, QT>, dim3(a.workers / 4), dim3(256), 0, stream, a);
+  return st != LLMK_OK ? st : join_launch<HD>(a, 16 * QT, stream);
+}
+
+template <int HD>
+int many_launch(AttentionArgs a, hipStream_t stream) {
+  a.workers = kManyWorkers<HD>;
+  const int st = launch(k_kv8_attention_many<HD>, dim3(a.workers), dim3(256), 0, stream, a);
+  return st != LLMK_OK ? st : join_launch<HD>(a, kManyColumns, stream);
+}
+
+// Sequences of up to kFewColumns columns go by waves, longer ones by blocks. One launch serves all
+// where max_rows, or a single sequence, says that there is one kind; more columns than were announced
+// are then several tiles.
+template <int HD>
+int attention_launch(AttentionArgs a, int max_rows, hipStream_t stream) {
+  const long long columns = (long long)max_rows * a.group;
+  if (columns <= 16) return few_launch<HD, 1>(a, stream);
+  if (columns <= kFewColumns) return few_launch<HD, 2>(a, stream);
+  if (a.batch.n_seqs > 1) {
+    a.most_columns = kFewColumns;
+    const int st = few_launch<HD, 2>(a, stream);
+    if (st != LLMK_OK) return st;
+    a.most_columns = 0x7FFFFFFF;
+    a.least_columns = kFewColumns + 1;
+  }
+  return many_launch<HD>(a, stream);
 }
 
 }  // namespace
@@ -709,8 +1070,9 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
   a.n_heads = n_heads;
   a.n_kv_heads = n_kv_heads;
   a.group = n_heads / n_kv_heads;
-  a.log_workers = 0;
-  a.min_ticks = 1;
+  a.workers = 0;
+  a.least_columns = 0;
+  a.most_columns = 0x7FFFFFFF;
   hipStream_t s = static_cast<hipStream_t>(stream);
   return head_dim == 64 ? attention_launch<64>(a, max_rows, s)
                         : attention_launch<128>(a, max_rows, s);
