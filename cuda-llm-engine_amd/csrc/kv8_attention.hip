@@ -28,7 +28,7 @@ template <int HD, int QT>
 constexpr int kFewWorkers = QT == 1 ? 2048 : 1024;
 template <int HD>
 constexpr int kManyWorkers = 512;
-constexpr int kWorkers = 2048;                  // at most
+constexpr int kWorkers = 2048, kMostKvHeads = 512;  // at most
 constexpr int kSlotColumns = 131072;            // of partial results in the workspace
 
 template <bool HIGH>
@@ -50,10 +50,10 @@ __device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& 
 // A unit that several workers share, as each of them notes it for the launch that joins its parts: one
 // that began before the worker's share and one that ends behind it.
 struct Shared {
-  int first, last;      // the workers; first > last: there is none
+  int first, last;      // the teams; first > last: there is none
   int column, columns;  // of the tile, from the sequence's first row on
-  int seq, head;        // kv head
-  int pad[2];
+  int seq;
+  int pad[3];
 };
 
 struct AttentionArgs {
@@ -120,7 +120,7 @@ __device__ __forceinline__ long long seq_ticks(const AttentionArgs& a, int s) {
   const Seq q = seq_of(a, s);
   long long n = 0;
   for (int t = 0; t * C < q.columns; ++t) n += kStart + tile_steps<HD, C>(a, q, t);
-  return n * a.n_kv_heads;
+  return n;
 }
 
 // Values that are the same in every lane, as scalars.
@@ -139,18 +139,22 @@ __device__ __forceinline__ Seq same(Seq q) {
   return q;
 }
 
-// Where the share of each of a block's workers begins among the ticks of all units, which are
-// ordered by sequence, tile and kv head. By all 256 threads; workers are waves or blocks.
+// How a launch's work is shared out. A kv head's units are the tiles of all sequences, one behind the
+// other; its ticks are cut into as many equal shares as there are teams, and a team has a worker for
+// each kv head. So the heads of a page, which lie beside one another in memory, are read at about the
+// same time (256 sequences: a worker with one head's units behind the other's, 63.1 us).
+// Worker t n_kv_heads + h is head h's of team t; workers are waves or blocks. By all 256 threads.
 struct Share {
-  int seq;               // that holds the beginning of this worker's share, and
+  int team, head;
+  int seq;               // that holds the beginning of the team's share, and
   long long at;          // its place in it
-  long long begin, end;  // among all ticks
-  long long each;        // of the first `more` workers one more
+  long long begin, end;  // among the ticks of a head
+  long long each;        // of the first `more` teams one more
   int more;
-  __device__ __forceinline__ long long begin_of(int worker) const {
-    return each * worker + (worker < more ? worker : more);
+  __device__ __forceinline__ long long begin_of(int team) const {
+    return each * team + (team < more ? team : more);
   }
-  __device__ __forceinline__ int worker_at(long long tick) const {
+  __device__ __forceinline__ int team_at(long long tick) const {
     const long long wide = (each + 1) * more;
     return (int)(tick < wide ? divide(tick, each + 1) : more + divide(tick - wide, each));
   }
@@ -159,7 +163,7 @@ struct Share {
   }
 };
 template <int HD, int C, bool WAVES>
-__device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker) {
+__device__ __forceinline__ Share find_share(const AttentionArgs& a) {
   __shared__ long long wave_sum_[4], at_[4];
   __shared__ int seq_[4];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -182,16 +186,18 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker) 
     total += wave_sum_[w];
   }
   total = same(total);
-  int workers = a.workers;
-  if (total < workers) workers = total > 0 ? (int)total : 1;
-  r.each = Share::divide(total, workers);
-  r.more = (int)(total - r.each * workers);
+  const int first = WAVES ? 4 * blockIdx.x : blockIdx.x, worker = WAVES ? first + wave : first;
+  int teams = a.workers / a.n_kv_heads;
+  if (total < teams) teams = total > 0 ? (int)total : 1;
+  r.each = Share::divide(total, teams);
+  r.more = (int)(total - r.each * teams);
+  r.team = worker / a.n_kv_heads;
+  r.head = worker % a.n_kv_heads;
   const long long from = base + upto - mine;
-  const int first = blockIdx.x;  // the workers of a block are a grid apart
   for (int w = 0; w < (WAVES ? 4 : 1); ++w) {
-    const int id = first + w * (int)gridDim.x;
-    const long long x = r.begin_of(id);
-    if (id < workers && x >= from && x < from + mine) {
+    const int team = (first + w) / a.n_kv_heads;
+    const long long x = r.begin_of(team);
+    if (team < teams && x >= from && x < from + mine) {
       long long left = x - from;
       int s = s0;
       for (; s < s1 - 1; ++s) {
@@ -204,8 +210,8 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a, int worker) 
     }
   }
   __syncthreads();
-  r.begin = worker < workers ? r.begin_of(worker) : total;
-  r.end = worker < workers ? r.begin_of(worker + 1) : total;
+  r.begin = r.team < teams ? r.begin_of(r.team) : total;
+  r.end = r.team < teams ? r.begin_of(r.team + 1) : total;
   r.seq = __builtin_amdgcn_readfirstlane(seq_[WAVES ? wave : 0]);
   r.at = same(at_[WAVES ? wave : 0]);
   return r;
@@ -237,22 +243,22 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
   constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64, PG = kPages<HD>, STEP = kStep<HD>;
   const int lane = threadIdx.x & 63, n = lane & 15, qd = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int worker = wave * (int)gridDim.x + (int)blockIdx.x;
+  const int worker = 4 * (int)blockIdx.x + wave;
   const bool shared_units = a.parts != nullptr;
-  const Share sh = find_share<HD, C, true>(a, worker);
-  auto note = [&](int side, int first, int last, int column, int columns, int seq, int head) {
+  const Share sh = find_share<HD, C, true>(a);
+  const int h = sh.head;
+  auto note = [&](int side, int first, int last, int column, int columns, int seq) {
     Shared o = {};
     o.first = first;
     o.last = last;
     o.column = column;
     o.columns = columns;
     o.seq = seq;
-    o.head = head;
     if (lane == 0) a.shared[2 * worker + side] = o;
   };
   if (shared_units) {
-    note(0, 0, -1, 0, 0, 0, 0);
-    note(1, 0, -1, 0, 0, 0, 0);
+    note(0, 0, -1, 0, 0, 0);
+    note(1, 0, -1, 0, 0, 0);
   }
 
   long long pos = sh.begin;
@@ -263,12 +269,11 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
     int steps;
     for (;;) {
       steps = same(tile_steps<HD, C>(a, q, tile));
-      const long long ticks = (long long)(kStart + steps) * a.n_kv_heads;
-      if (at < ticks) break;
-      at -= ticks;
+      if (at < kStart + steps) break;
+      at -= kStart + steps;
       ++tile;
     }
-    int h = same((int)at / (kStart + steps)), tick = same((int)at % (kStart + steps));
+    int tick = same((int)at);
     const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
     int ids = 0, ids_of = -1, window = -1;  // 64 entries of a sequence's table, one to a lane
 
@@ -551,7 +556,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
         const int side = step == 0 ? 1 : 0;
         if (!whole) {  // the workers of its first and last steps
           const long long end = pos + ticks - upto, begin = end - steps;
-          note(side, sh.worker_at(begin), sh.worker_at(end - 1), c0, columns, s, h);
+          note(side, sh.team_at(begin), sh.team_at(end - 1), c0, columns, s);
         }
         const size_t slot = 2 * (size_t)worker + side;
 #pragma unroll
@@ -592,16 +597,13 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
         }
       }
       tick = 0;
-      if (++h == a.n_kv_heads) {
-        h = 0;
-        ++tile;
-        while (tile * C >= q.columns && s < a.batch.n_seqs - 1) {
-          tile = 0;
-          q = same(seq_of(a, ++s));
-        }
-        if (tile * C >= q.columns) break;
-        steps = same(tile_steps<HD, C>(a, q, tile));
+      ++tile;
+      while (tile * C >= q.columns && s < a.batch.n_seqs - 1) {
+        tile = 0;
+        q = same(seq_of(a, ++s));
       }
+      if (tile * C >= q.columns) break;
+      steps = same(tile_steps<HD, C>(a, q, tile));
     }
   }
 }
@@ -628,6 +630,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
       m = next;
     }
   };
+  const int team = worker / a.n_kv_heads, head = worker % a.n_kv_heads;
   for (int side = 0; side < 2; ++side) {
     const Shared o = a.shared[2 * worker + side];
     if (o.first > o.last) continue;
@@ -640,7 +643,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
       slices *= 2;
       lanes /= 2;
     }
-    const int slice = worker - o.first;
+    const int slice = team - o.first;
     if (slice >= slices) continue;
     const int deal = 256 / lanes, turn = tid / lanes;
     const int task = base + slice * lanes + tid % lanes, c = task / V, d = 4 * (task % V);
@@ -649,7 +652,8 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
     if (c < o.columns) {
 #pragma unroll 4
       for (int j = turn; j < n; j += deal) {
-        const size_t at = (2 * (size_t)(o.first + j) + (j == 0 ? 1 : 0)) * C + c;
+        const size_t w = (size_t)(o.first + j) * a.n_kv_heads + head;
+        const size_t at = (2 * w + (j == 0 ? 1 : 0)) * C + c;
         r.add(*reinterpret_cast<const f32x4*>(a.parts + at * HD + d), a.parts_ml[at]);
       }
     }
@@ -669,7 +673,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
       v.x = __builtin_bit_cast(uint32_t, y[0]);
       v.y = __builtin_bit_cast(uint32_t, y[1]);
       *reinterpret_cast<uint2*>(a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads +
-                                         o.head * a.group + col % a.group) * HD + d) = v;
+                                         head * a.group + col % a.group) * HD + d) = v;
     }
   }
 }
@@ -694,20 +698,20 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
   const bool shared_units = a.parts != nullptr;
   int turn = 0;
   if (tid < 2) odd[tid] = 0;
-  const Share sh = find_share<HD, C, false>(a, worker);
-  auto note = [&](int side, int first, int last, int column, int columns, int seq, int head) {
+  const Share sh = find_share<HD, C, false>(a);
+  const int h = sh.head;
+  auto note = [&](int side, int first, int last, int column, int columns, int seq) {
     Shared o = {};
     o.first = first;
     o.last = last;
     o.column = column;
     o.columns = columns;
     o.seq = seq;
-    o.head = head;
     if (tid == 0) a.shared[2 * worker + side] = o;
   };
   if (shared_units) {
-    note(0, 0, -1, 0, 0, 0, 0);
-    note(1, 0, -1, 0, 0, 0, 0);
+    note(0, 0, -1, 0, 0, 0);
+    note(1, 0, -1, 0, 0, 0);
   }
   long long pos = sh.begin;
   if (pos >= sh.end) return;
@@ -717,12 +721,11 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
   int steps;
   for (;;) {
     steps = same(tile_steps<HD, C>(a, q, tile));
-    const long long ticks = (long long)(kStart + steps) * a.n_kv_heads;
-    if (at < ticks) break;
-    at -= ticks;
+    if (at < kStart + steps) break;
+    at -= kStart + steps;
     ++tile;
   }
-  int h = same((int)at / (kStart + steps)), tick = same((int)at % (kStart + steps));
+  int tick = same((int)at);
   const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
 
   while (pos < sh.end) {
@@ -937,7 +940,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
       const int side = step == 0 ? 1 : 0;
       if (!whole) {  // the workers of its first and last steps
         const long long end = pos + ticks - upto, begin = end - steps;
-        note(side, sh.worker_at(begin), sh.worker_at(end - 1), c0, columns, s, h);
+        note(side, sh.team_at(begin), sh.team_at(end - 1), c0, columns, s);
       }
       l = l + __shfl_xor(l, 32);
       if (own && whole) {
@@ -969,16 +972,13 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
       }
     }
     tick = 0;
-    if (++h == a.n_kv_heads) {
-      h = 0;
-      ++tile;
-      while (tile * C >= q.columns && s < a.batch.n_seqs - 1) {
-        tile = 0;
-        q = same(seq_of(a, ++s));
-      }
-      if (tile * C >= q.columns) break;
-      steps = same(tile_steps<HD, C>(a, q, tile));
+    ++tile;
+    while (tile * C >= q.columns && s < a.batch.n_seqs - 1) {
+      tile = 0;
+      q = same(seq_of(a, ++s));
     }
+    if (tile * C >= q.columns) break;
+    steps = same(tile_steps<HD, C>(a, q, tile));
   }
 }
 
@@ -1051,7 +1051,7 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
     return LLMK_ERR_INVALID_VALUE;
   // a sequence's columns, and positions of a table, are counted in 32 bits
   if ((long long)n_rows * (n_heads / n_kv_heads) > 0x7FFF0000LL || n_heads > 65535 ||
-      max_pages > 0x7FFF0000 / kv8::kPage)
+      n_kv_heads > kMostKvHeads || max_pages > 0x7FFF0000 / kv8::kPage)
     return LLMK_ERR_UNSUPPORTED;
   if (!aligned16(q) || !aligned16(k_pool) || !aligned16(v_pool) || !aligned16(out) ||
       !aligned16(workspace))
