@@ -13,13 +13,16 @@
 // So a block that is begun anew forgets its scale, and rows that are appended over others (drafted
 // tokens that were refused) only ever find it as large as those needed.
 //
-// Work split: a block of 256 threads for each row; the rows that open a page of their sequence, or
-// the call, also write K and V of all rows that follow them in the page. There a wave holds up to
-// 16 rows x head_dim / 16 pieces of one (kv head, K or V), and more heads side by side where the
-// page gets fewer rows, so that the maximum is a few lane exchanges and nothing is read twice.
+// Work split: a window of 16 rows goes to a column of the grid, some blocks for its q, some for its K and
+// V. The rows of the window that open a page, of their sequence or of the call, lead the rows that
+// follow them in it. A wave holds all rows of a leader, in pieces of 16 values, and as many (kv head,
+// K or V) side by side as fit its lanes: 16 rows of one at head_dim 64, 16 of single rows. So a window
+// makes 16 to 32 such tasks whether it holds one prompt's rows or a decode step's, nothing is read
+// twice, and the maximum is a few lane exchanges.
 #include <math.h>
 
 #include "kv8.hpp"
+#include "layer_ops.hpp"
 
 namespace llmk {
 namespace {
@@ -58,64 +61,110 @@ struct AppendArgs {
   int ld, n_heads, n_kv_heads;
 };
 
+constexpr int kWindow = 16, kQuarter = 4;  // rows of a column of the grid, and of a block for q
+
 template <int HD>
-__global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a) {
+__global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a, int kv_blocks) {
   constexpr int HALF = HD / 2, P = HD / 16;  // P pieces of a row: elements 8 p .. and HALF + 8 p ..
   constexpr int J = P * kPage / 64;          // rows of a lane where a page gets all 16
-  __shared__ f32x2 turn[kPage][HALF];
-  const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  __shared__ f32x2 turn[2 * kWindow][HALF];  // of the window's rows and those that its last one leads
+  __shared__ int seq_of[kWindow], lead[kWindow], slot_of[kWindow], tasks_before[kWindow + 1];
+  __shared__ long long pos_of[kWindow];
+  __shared__ size_t page_of[kWindow];
+  const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int s = __builtin_amdgcn_readfirstlane(find_seq(a.batch.starts, a.batch.n_seqs, row));
-  if (s < 0) return;
-  int i = 0, count = 1;
-  if (a.batch.starts) {
-    i = row - a.batch.starts[s];
-    count = a.batch.starts[s + 1] - a.batch.starts[s];
+  const int window = blockIdx.x * kWindow, units = 2 * a.n_kv_heads;
+  const int s0 = find_seq(a.batch.starts, a.batch.n_seqs, window);
+  if (wave == 0) {
+    const int row = window + lane;
+    int s = -1, n = 0, slot = 0;  // n: rows that this one leads
+    long long pos = -1;
+    if (lane < kWindow && row < a.batch.n_rows && s0 >= 0)
+      s = a.batch.starts ? find_seq_from(a.batch.starts, a.batch.n_seqs, s0, row)
+                         : (row < a.batch.n_seqs ? row : -1);
+    if (s >= 0) {
+      const int r0 = a.batch.starts ? a.batch.starts[s] : row;
+      const int r1 = a.batch.starts ? a.batch.starts[s + 1] : row + 1;
+      pos = (long long)a.batch.lens[s] - (r1 - row);
+      slot = (int)(pos & (kPage - 1));
+      if (pos < 0 || pos >= (long long)a.batch.max_pages * kPage) {
+        pos = -1;
+      } else if (row == r0 || slot == 0) {
+        n = kPage - slot;
+        n = n < r1 - row ? n : r1 - row;
+        n = n < a.batch.n_rows - row ? n : a.batch.n_rows - row;
+        page_of[lane] = (size_t)a.batch.tables[(size_t)s * a.batch.max_pages + pos / kPage];
+      }
+    }
+    int per = P;
+    while (per < P * n && per < 64) per *= 2;
+    int tasks = n > 0 ? (units + 64 / per - 1) / (64 / per) : 0;
+    for (int d = 1; d < kWindow; d *= 2) {
+      const int o = __shfl_up(tasks, d);
+      if (lane >= d) tasks += o;
+    }
+    if (lane < kWindow) {
+      seq_of[lane] = s;
+      lead[lane] = n;
+      slot_of[lane] = slot;
+      pos_of[lane] = pos;
+      tasks_before[lane + 1] = tasks;
+      if (lane == 0) tasks_before[0] = 0;
+    }
   }
-  const long long pos = (long long)a.batch.lens[s] - count + i;
-  const bool in_table = pos >= 0 && pos < (long long)a.batch.max_pages * kPage;
-  const int slot = (int)(pos & (kPage - 1));
-  int n = 0;  // rows whose K and V this block writes
-  if (in_table && (i == 0 || slot == 0)) {
-    n = kPage - slot;
-    n = n < count - i ? n : count - i;
-    n = n < a.batch.n_rows - row ? n : a.batch.n_rows - row;
-  }
-  for (int t = tid; t < (n > 1 ? n : 1) * HALF; t += 256)
-    turn[t / HALF][t % HALF] =
-        cos_sin((double)(pos + t / HALF) * (double)a.inv_freq[t % HALF]);
   __syncthreads();
 
-  // q of this row; zeros where its position lies outside the table
-  const f16* src = a.qkv + (size_t)row * a.ld;
-  for (int t = tid; t < a.n_heads * P; t += 256) {
-    const size_t at = (size_t)(t / P) * HD + (t % P) * 8;
-    const f16x8 x1 = as_h8(ld16(src + at)), x2 = as_h8(ld16(src + at + HALF));
-    f16x8 y1, y2;
+  if ((int)blockIdx.y >= kv_blocks) {  // q of 4 rows; zeros where a position lies outside the table
+    const int r0 = ((int)blockIdx.y - kv_blocks) * kQuarter;
+    for (int t = tid; t < kQuarter * HALF; t += 256)
+      if (pos_of[r0 + t / HALF] >= 0)
+        turn[t / HALF][t % HALF] =
+            cos_sin((double)pos_of[r0 + t / HALF] * (double)a.inv_freq[t % HALF]);
+    __syncthreads();
+    const int per_row = a.n_heads * P;
+    for (int t = tid; t < kQuarter * per_row; t += 256) {
+      const int r = t / per_row, v = t % per_row, p = v % P;
+      if (seq_of[r0 + r] < 0) continue;
+      const bool in_table = pos_of[r0 + r] >= 0;
+      const size_t row = (size_t)window + r0 + r, at = (size_t)(v / P) * HD + p * 8;
+      const f16* src = a.qkv + row * a.ld + at;
+      const f16x8 x1 = as_h8(ld16(src)), x2 = as_h8(ld16(src + HALF));
+      f16x8 y1, y2;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const f32x2 cs = turn[0][(t % P) * 8 + e];
-      const float u = (float)x1[e], w = (float)x2[e];
-      y1[e] = in_table ? (f16)(u * cs.x - w * cs.y) : (f16)0;
-      y2[e] = in_table ? (f16)(w * cs.x + u * cs.y) : (f16)0;
+      for (int e = 0; e < 8; ++e) {
+        const f32x2 cs = turn[r][p * 8 + e];
+        const float u = (float)x1[e], w = (float)x2[e];
+        y1[e] = in_table ? (f16)(u * cs.x - w * cs.y) : (f16)0;
+        y2[e] = in_table ? (f16)(w * cs.x + u * cs.y) : (f16)0;
+      }
+      f16* dst = a.q_out + row * a.n_heads * HD + at;
+      st16(dst, as_u4(y1));
+      st16(dst + HALF, as_u4(y2));
     }
-    f16* dst = a.q_out + (size_t)row * a.n_heads * HD + at;
-    st16(dst, as_u4(y1));
-    st16(dst + HALF, as_u4(y2));
+    return;
   }
-  if (n == 0) return;
 
-  const size_t page = (size_t)a.batch.tables[(size_t)s * a.batch.max_pages + pos / kPage];
-  int per = P;  // lanes of one unit, a (kv head, K or V): P for each row, rows to a power of two
-  while (per < P * n && per < 64) per *= 2;
-  const int units = 2 * a.n_kv_heads, mine = lane & (per - 1);
-  const int r0 = mine / P, p = mine % P;
-  for (int first = wave * (64 / per); first < units; first += 4 * (64 / per)) {
-    const int unit = first + lane / per;
+  const int tasks = tasks_before[kWindow];
+  if (tasks == 0) return;
+  for (int t = tid; t < kWindow * HALF; t += 256) {  // leaders' rows, each by its leader
+    const int g = t / HALF, i = t % HALF;
+    for (int r = 0; r < lead[g]; ++r)
+      turn[g + r][i] = cos_sin((double)(pos_of[g] + r) * (double)a.inv_freq[i]);
+  }
+  __syncthreads();
+  for (int task = (int)blockIdx.y * 4 + wave; task < tasks; task += 4 * kv_blocks) {
+    int g = 0;
+    while (tasks_before[g + 1] <= task) ++g;
+    const int n = lead[g], slot = slot_of[g];
+    const size_t row = (size_t)window + g, page = page_of[g];
+    int per = P;  // lanes of one unit, a (kv head, K or V): P for each row, rows to a power of two
+    while (per < P * n && per < 64) per *= 2;
+    const int mine = lane & (per - 1), r0 = mine / P, p = mine % P;
+    const int unit = (task - tasks_before[g]) * (64 / per) + lane / per;
     const bool live = unit < units;
     const int side = live && unit >= a.n_kv_heads, h = live ? unit - side * a.n_kv_heads : 0;
     const f16* from =
-        a.qkv + (size_t)(a.n_heads + side * a.n_kv_heads + h) * HD + 8 * p + (size_t)row * a.ld;
+        a.qkv + (size_t)(a.n_heads + side * a.n_kv_heads + h) * HD + 8 * p + row * a.ld;
     float* const scale = a.scale[side] + page * a.n_kv_heads + h;
     uint8_t* const block = a.pool[side] + (page * a.n_kv_heads + h) * (size_t)(kPage * HD);
     const int before = live && slot > 0 ? exponent_of(*scale) : kMinExp;
@@ -131,7 +180,7 @@ __global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a) {
       for (int e = 0; e < 8; ++e) {
         const float u = (float)x1[e], w = (float)x2[e];
         if (side == 0) {
-          const f32x2 cs = turn[r][8 * p + e];
+          const f32x2 cs = turn[g + r][8 * p + e];
           x[j][e] = u * cs.x - w * cs.y;
           x[j][8 + e] = w * cs.x + u * cs.y;
         } else {
@@ -155,13 +204,13 @@ __global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a) {
       if (!live || r >= n) continue;
       uint8_t* dst = block + (slot + r) * HD + 8 * p;
 #pragma unroll
-      for (int g = 0; g < 2; ++g) {
+      for (int k = 0; k < 2; ++k) {
         uint2 v;
-        v.x = to_e4m3(x[j][8 * g] * down, x[j][8 * g + 1] * down, x[j][8 * g + 2] * down,
-                      x[j][8 * g + 3] * down);
-        v.y = to_e4m3(x[j][8 * g + 4] * down, x[j][8 * g + 5] * down, x[j][8 * g + 6] * down,
-                      x[j][8 * g + 7] * down);
-        *reinterpret_cast<uint2*>(dst + g * HALF) = v;
+        v.x = to_e4m3(x[j][8 * k] * down, x[j][8 * k + 1] * down, x[j][8 * k + 2] * down,
+                      x[j][8 * k + 3] * down);
+        v.y = to_e4m3(x[j][8 * k + 4] * down, x[j][8 * k + 5] * down, x[j][8 * k + 6] * down,
+                      x[j][8 * k + 7] * down);
+        *reinterpret_cast<uint2*>(dst + k * HALF) = v;
       }
     }
     if (live && slot > 0 && e > before) {  // the tokens held already, under the new scale
@@ -182,8 +231,10 @@ __global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a) {
   }
 }
 
-// Read-back: each block takes 16 rows; a thread takes 16 values of one row at a time.
-constexpr int kGatherRows = 16;
+// Read-back: a block takes 16 rows of K or of V, a thread 8 values at a time, in the order of the output
+// (a wave writes 1 KiB in a row; what it reads are 64-byte halves of lines whose other halves the
+// neighbouring rows take), four of them in flight.
+constexpr int kGatherRows = 16, kGatherFlight = 4;
 
 struct GatherArgs {
   Batch batch;
@@ -191,11 +242,12 @@ struct GatherArgs {
   const float* scale[2];
   f16* out[2];
   int n_kv_heads;
+  FastDiv per_row;  // 8-value pieces of a row
 };
 
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_gather(const GatherArgs a) {
-  constexpr int P = HD / 16;
+  constexpr int P = HD / 8;
   __shared__ long long block_of[kGatherRows];  // page, -1: no position, -2: a row of no sequence
   __shared__ int slot_of[kGatherRows];
   const int row0 = blockIdx.x * kGatherRows, tid = threadIdx.x;
@@ -217,29 +269,38 @@ __global__ void __launch_bounds__(256) k_kv8_gather(const GatherArgs a) {
     block_of[tid] = page;
   }
   __syncthreads();
-  const int per_side = kGatherRows * P * a.n_kv_heads;
-  for (int t = tid; t < 2 * per_side; t += 256) {
-    const int side = t >= per_side, u = t - side * per_side;
-    const int r = u / P % kGatherRows, p = u % P, h = u / (P * kGatherRows);
-    const long long page = block_of[r];
-    if (page == -2) continue;
-    u32x4 lo = {0, 0, 0, 0}, hi = {0, 0, 0, 0};
-    if (page >= 0) {
-      const size_t block = (size_t)page * a.n_kv_heads + h;
-      const u32x4 b = ld16(a.pool[side] + (block * kPage + slot_of[r]) * HD + 16 * p);
-      const float scale = a.scale[side][block];
+  const int side = blockIdx.y, n = kGatherRows * (int)a.per_row.d;
+  for (int t0 = tid; t0 < n; t0 += 256 * kGatherFlight) {
+    uint2 bytes[kGatherFlight];
+    float scale[kGatherFlight];
+    int row[kGatherFlight];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t w = elem(b, k);
-        const uint32_t x = __builtin_bit_cast(uint32_t, from_e4m3<false>(w, scale));
-        const uint32_t y = __builtin_bit_cast(uint32_t, from_e4m3<true>(w, scale));
-        if (k < 2) { lo[2 * k] = x; lo[2 * k + 1] = y; }
-        else { hi[2 * k - 4] = x; hi[2 * k - 3] = y; }
+    for (int k = 0; k < kGatherFlight; ++k) {
+      const int t = t0 + 256 * k;
+      const int r = t < n ? (int)fdiv((uint32_t)t, a.per_row) : 0;
+      const int v = t < n ? t - r * (int)a.per_row.d : 0;
+      const long long page = t < n ? block_of[r] : -2;
+      row[k] = page == -2 ? -1 : r;
+      bytes[k] = make_uint2(0, 0);
+      scale[k] = 1.0f;
+      if (page >= 0) {
+        const size_t block = (size_t)page * a.n_kv_heads + v / P;
+        bytes[k] = *reinterpret_cast<const uint2*>(
+            a.pool[side] + (block * kPage + slot_of[r]) * HD + 8 * (v % P));
+        scale[k] = a.scale[side][block];
       }
     }
-    f16* dst = a.out[side] + ((size_t)(row0 + r) * a.n_kv_heads + h) * HD + 16 * p;
-    st16(dst, lo);
-    st16(dst + 8, hi);
+#pragma unroll
+    for (int k = 0; k < kGatherFlight; ++k) {
+      if (row[k] < 0) continue;
+      const int v = t0 + 256 * k - row[k] * (int)a.per_row.d;
+      u32x4 y;
+      y[0] = __builtin_bit_cast(uint32_t, from_e4m3<false>(bytes[k].x, scale[k]));
+      y[1] = __builtin_bit_cast(uint32_t, from_e4m3<true>(bytes[k].x, scale[k]));
+      y[2] = __builtin_bit_cast(uint32_t, from_e4m3<false>(bytes[k].y, scale[k]));
+      y[3] = __builtin_bit_cast(uint32_t, from_e4m3<true>(bytes[k].y, scale[k]));
+      st16_stream(a.out[side] + ((size_t)(row0 + row[k]) * a.per_row.d + v) * 8, y);
+    }
   }
 }
 
@@ -286,8 +347,11 @@ extern "C" int llmk_kv8_append(const uint16_t* qkv, int ld, uint16_t* q_out, uin
   a.ld = ld;
   a.n_heads = n_heads;
   a.n_kv_heads = n_kv_heads;
-  return launch(head_dim == 64 ? k_kv8_append<64> : k_kv8_append<128>, dim3((unsigned)n_rows),
-                dim3(256), 0, static_cast<hipStream_t>(stream), a);
+  // a block for K and V takes four tasks at a time of the window's 16 to 32 at 8 kv heads
+  const int kv_blocks = (n_kv_heads + 1) / 2 < 32 ? (n_kv_heads + 1) / 2 : 32;
+  const dim3 grid(ceil_div((size_t)n_rows, (size_t)kWindow), kv_blocks + kWindow / kQuarter);
+  return launch(head_dim == 64 ? k_kv8_append<64> : k_kv8_append<128>, grid, dim3(256), 0,
+                static_cast<hipStream_t>(stream), a, kv_blocks);
 }
 
 extern "C" int llmk_kv8_gather(const uint8_t* k_pool, const float* k_scale, const uint8_t* v_pool,
@@ -313,7 +377,8 @@ extern "C" int llmk_kv8_gather(const uint8_t* k_pool, const float* k_scale, cons
   a.out[0] = reinterpret_cast<f16*>(k_out);
   a.out[1] = reinterpret_cast<f16*>(v_out);
   a.n_kv_heads = n_kv_heads;
+  a.per_row = make_fastdiv((uint32_t)n_kv_heads * (uint32_t)head_dim / 8);
   return launch(head_dim == 64 ? k_kv8_gather<64> : k_kv8_gather<128>,
-                dim3(ceil_div((size_t)n_rows, (size_t)kGatherRows)), dim3(256), 0,
+                dim3(ceil_div((size_t)n_rows, (size_t)kGatherRows), 2), dim3(256), 0,
                 static_cast<hipStream_t>(stream), a);
 }
