@@ -247,7 +247,7 @@ def _load_fast_calls():
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)
             mod.setup(torch.Tensor, torch.float16, torch.int32, torch.float32,
-                      torch.cuda.current_device, raw_stream)
+                      torch.cuda.current_device, raw_stream, torch.float8_e4m3fn)
             return mod
     return _NoFastCalls()
 
@@ -619,6 +619,12 @@ def kv8_append(qkv, ld: int, q_out, k_pool, k_scale, v_pool, v_scale, block_tabl
     page that two sequences append to."""
     fn = "kv8_append"
     check = _want_checks(check_indices)
+    if not check:
+        st = _fast.kv8_append(qkv, ld, q_out, k_pool, k_scale, v_pool, v_scale, block_tables,
+                              row_starts, seq_lens, inv_freq, n_rows, n_seqs, max_pages, page_size,
+                              n_heads, n_kv_heads, head_dim, stream)
+        if st is not None:
+            return _check(fn, st)
     pools, batch, spans = _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
                                      seq_lens, n_rows, n_seqs, max_pages, page_size, n_kv_heads,
                                      head_dim, check)
@@ -644,6 +650,12 @@ def kv8_gather(k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, seq_l
     """The last cached rows of each sequence as fp16 (``llmk_kv8_gather``; arguments as
     kv8_append's)."""
     fn = "kv8_gather"
+    if not _want_checks(check_indices):
+        st = _fast.kv8_gather(k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, seq_lens,
+                              k_out, v_out, n_rows, n_seqs, max_pages, page_size, n_kv_heads,
+                              head_dim, stream)
+        if st is not None:
+            return _check(fn, st)
     pools, batch, spans = _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
                                      seq_lens, n_rows, n_seqs, max_pages, page_size, n_kv_heads,
                                      head_dim, _want_checks(check_indices))
@@ -668,6 +680,12 @@ def kv8_attention(q, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
     """Causal attention of the rows over the 8-bit cache (``llmk_kv8_attention``; cache and batch as
     kv8_append's). workspace None: every sequence stays whole, for short contexts."""
     fn = "kv8_attention"
+    if not _want_checks(check_indices):
+        st = _fast.kv8_attention(q, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
+                                 seq_lens, out, workspace, n_rows, n_seqs, max_rows, max_pages,
+                                 page_size, n_heads, n_kv_heads, head_dim, stream)
+        if st is not None:
+            return _check(fn, st)
     pools, batch, spans = _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
                                      seq_lens, n_rows, n_seqs, max_pages, page_size, n_kv_heads,
                                      head_dim, _want_checks(check_indices))
@@ -694,6 +712,12 @@ def verify_drafts(logits, draft_logits, drafts, row_starts, temperature, accept_
     (``llmk_verify_drafts``). draft_logits None: drafts count as certain; temperature None: 1;
     row_starts None: one row a sequence and no drafts (drafts and accept_u may be None)."""
     fn = "verify_drafts"
+    if not _want_checks(check_indices):
+        st = _fast.verify_drafts(logits, draft_logits, drafts, row_starts, temperature, accept_u,
+                                 sample_u, n_accepted, tokens, workspace, n_rows, n_seqs, vocab,
+                                 stream)
+        if st is not None:
+            return _check(fn, st)
     if min(n_rows, n_seqs) < 0 or vocab <= 0:
         _fail(fn, "n_rows and n_seqs must be >= 0 and vocab > 0")
     given = n_rows if row_starts is not None else 0  # of drafts and their numbers

@@ -13,8 +13,9 @@
 
 #include "llmk.h"
 
-static PyObject *tensor_type, *half_dtype, *int_dtype, *float_dtype, *get_device, *get_stream;
-static PyObject *s_is_cuda, *s_dtype, *s_is_contiguous, *s_numel, *s_data_ptr;
+static PyObject *tensor_type, *half_dtype, *int_dtype, *float_dtype, *get_device, *get_stream,
+    *e4m3_dtype;
+static PyObject *s_is_cuda, *s_dtype, *s_is_contiguous, *s_numel, *s_data_ptr, *s_get_device;
 
 /* The device address of t when it is a contiguous CUDA torch.Tensor of this dtype with at least
  * `least` elements; 0 otherwise, with no exception set. (A tensor of no elements has no address
@@ -49,6 +50,44 @@ static void* address(PyObject* t, PyObject* dtype, long long least) {
     p = NULL;
   }
   return p;
+}
+
+/* The current device, -1 if it cannot be told. */
+static long long device_now(void) {
+  long long at = -1;
+  PyObject* v = PyObject_CallNoArgs(get_device);
+  if (v) {
+    at = PyLong_AsLongLong(v);
+    Py_DECREF(v);
+  }
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    at = -1;
+  }
+  return at;
+}
+
+/* address() of a tensor of this device, and how many elements it has. */
+static void* address_on(PyObject* t, PyObject* dtype, long long least, long long device,
+                        long long* numel) {
+  void* p = address(t, dtype, least);
+  if (!p) return NULL;
+  long long at = -1, n = -1;
+  PyObject* v = PyObject_CallMethodNoArgs(t, s_get_device);
+  if (v) {
+    at = PyLong_AsLongLong(v);
+    Py_DECREF(v);
+  }
+  if (numel && (v = PyObject_CallMethodNoArgs(t, s_numel))) {
+    n = PyLong_AsLongLong(v);
+    Py_DECREF(v);
+    *numel = n;
+  }
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return NULL;
+  }
+  return at == device ? p : NULL;
 }
 
 /* torch's current stream for None, the number itself for a number. */
@@ -229,15 +268,141 @@ FUNCTION(attention_decode_fast, 15)
                                     page_size, heads, kv_heads, head_dim, splits, stream));
 }
 
+/* Tensors of the calls below: on the current device, `here`. OPT: or None. */
+#define HERE                          \
+  const long long here = device_now(); \
+  if (here < 0) Py_RETURN_NONE
+#define TENSOR_ON(type, name, at, dtype, least)                           \
+  type* name = (type*)address_on(args[at], dtype, least, here, NULL);      \
+  if (!name) Py_RETURN_NONE
+#define OPT_ON(type, name, at, dtype, least)                                                 \
+  type* name = args[at] == Py_None ? NULL                                                    \
+                                   : (type*)address_on(args[at], dtype, least, here, NULL);  \
+  if (!name && args[at] != Py_None) Py_RETURN_NONE
+/* A cache's pool and scales, which have to fit each other, at `at` and at + 1. */
+#define POOL(name, at, kv_heads, page_size, head_dim)                                           \
+  long long name##_n = 0, name##_scales = 0;                                                    \
+  uint8_t* name##_pool = (uint8_t*)address_on(args[at], e4m3_dtype, 0, here, &name##_n);        \
+  float* name##_scale = (float*)address_on(args[at + 1], float_dtype, 0, here, &name##_scales); \
+  if (!name##_pool || !name##_scale || name##_scales % kv_heads ||                              \
+      name##_n / ((long long)page_size * head_dim) != name##_scales ||                          \
+      name##_n % ((long long)page_size * head_dim))                                             \
+  Py_RETURN_NONE
+/* The tensors of a batch, at `at` and the two behind. */
+#define BATCH(at)                                                                 \
+  TENSOR_ON(int32_t, tables, at, int_dtype, (long long)n_seqs * max_pages);       \
+  OPT_ON(int32_t, starts, (at) + 1, int_dtype, (long long)n_seqs + 1);            \
+  TENSOR_ON(int32_t, lens, (at) + 2, int_dtype, n_seqs)
+
+FUNCTION(kv8_append, 19)
+  COUNT(ld, 1);
+  COUNT(n_rows, 11);
+  COUNT(n_seqs, 12);
+  COUNT(max_pages, 13);
+  COUNT(page_size, 14);
+  COUNT(heads, 15);
+  COUNT(kv_heads, 16);
+  COUNT(head_dim, 17);
+  if (!n_rows || !page_size || !heads || !kv_heads || !head_dim || heads > 65535 ||
+      kv_heads > 65535 || head_dim > 65535 || page_size > 65535)
+    Py_RETURN_NONE;
+  const long long width = (heads + 2LL * kv_heads) * head_dim;
+  if (ld < width) Py_RETURN_NONE;
+  HERE;
+  TENSOR_ON(uint16_t, qkv, 0, half_dtype, (n_rows - 1LL) * ld + width);
+  TENSOR_ON(uint16_t, q_out, 2, half_dtype, (long long)n_rows * heads * head_dim);
+  POOL(k, 3, kv_heads, page_size, head_dim);
+  POOL(v, 5, kv_heads, page_size, head_dim);
+  BATCH(7);
+  TENSOR_ON(float, inv_freq, 10, float_dtype, head_dim / 2);
+  STREAM(18);
+  ANSWER(llmk_kv8_append(qkv, ld, q_out, k_pool, k_scale, v_pool, v_scale, tables, starts, lens,
+                         inv_freq, n_rows, n_seqs, max_pages, page_size, heads, kv_heads, head_dim,
+                         stream));
+}
+
+FUNCTION(kv8_gather, 16)
+  COUNT(n_rows, 9);
+  COUNT(n_seqs, 10);
+  COUNT(max_pages, 11);
+  COUNT(page_size, 12);
+  COUNT(kv_heads, 13);
+  COUNT(head_dim, 14);
+  if (!n_rows || !page_size || !kv_heads || !head_dim || kv_heads > 65535 || head_dim > 65535 ||
+      page_size > 65535)
+    Py_RETURN_NONE;
+  HERE;
+  POOL(k, 0, kv_heads, page_size, head_dim);
+  POOL(v, 2, kv_heads, page_size, head_dim);
+  BATCH(4);
+  TENSOR_ON(uint16_t, k_out, 7, half_dtype, (long long)n_rows * kv_heads * head_dim);
+  TENSOR_ON(uint16_t, v_out, 8, half_dtype, (long long)n_rows * kv_heads * head_dim);
+  STREAM(15);
+  ANSWER(llmk_kv8_gather(k_pool, k_scale, v_pool, v_scale, tables, starts, lens, k_out, v_out,
+                         n_rows, n_seqs, max_pages, page_size, kv_heads, head_dim, stream));
+}
+
+FUNCTION(kv8_attention, 19)
+  COUNT(n_rows, 10);
+  COUNT(n_seqs, 11);
+  COUNT(max_rows, 12);
+  COUNT(max_pages, 13);
+  COUNT(page_size, 14);
+  COUNT(heads, 15);
+  COUNT(kv_heads, 16);
+  COUNT(head_dim, 17);
+  if (!n_rows || !page_size || !heads || !kv_heads || !head_dim || heads > 65535 ||
+      kv_heads > 65535 || head_dim > 65535 || page_size > 65535)
+    Py_RETURN_NONE;
+  HERE;
+  TENSOR_ON(uint16_t, q, 0, half_dtype, (long long)n_rows * heads * head_dim);
+  POOL(k, 1, kv_heads, page_size, head_dim);
+  POOL(v, 3, kv_heads, page_size, head_dim);
+  BATCH(5);
+  TENSOR_ON(uint16_t, out, 8, half_dtype, (long long)n_rows * heads * head_dim);
+  OPT_ON(float, workspace, 9, float_dtype,
+         (long long)llmk_kv8_attention_workspace_floats(head_dim));
+  STREAM(18);
+  ANSWER(llmk_kv8_attention(q, k_pool, k_scale, v_pool, v_scale, tables, starts, lens, out,
+                            workspace, n_rows, n_seqs, max_rows, max_pages, page_size, heads,
+                            kv_heads, head_dim, stream));
+}
+
+FUNCTION(verify_drafts, 14)
+  COUNT(n_rows, 10);
+  COUNT(n_seqs, 11);
+  COUNT(vocab, 12);
+  if (!n_rows || !vocab) Py_RETURN_NONE;
+  const long long given = args[3] != Py_None ? n_rows : 0;
+  const size_t floats = llmk_verify_drafts_workspace_floats(n_rows, n_seqs, vocab);
+  if (floats > (size_t)LLONG_MAX) Py_RETURN_NONE;
+  HERE;
+  TENSOR_ON(uint16_t, logits, 0, half_dtype, (long long)n_rows * vocab);
+  OPT_ON(uint16_t, draft_logits, 1, half_dtype, given * vocab);
+  OPT_ON(int32_t, drafts, 2, int_dtype, given);
+  OPT_ON(int32_t, starts, 3, int_dtype, (long long)n_seqs + 1);
+  OPT_ON(float, temperature, 4, float_dtype, n_seqs);
+  OPT_ON(float, accept_u, 5, float_dtype, given);
+  TENSOR_ON(float, sample_u, 6, float_dtype, n_seqs);
+  TENSOR_ON(int32_t, n_accepted, 7, int_dtype, n_seqs);
+  TENSOR_ON(int32_t, tokens, 8, int_dtype, n_rows);
+  TENSOR_ON(float, workspace, 9, float_dtype, (long long)floats);
+  STREAM(13);
+  ANSWER(llmk_verify_drafts(logits, draft_logits, drafts, starts, temperature, accept_u, sample_u,
+                            n_accepted, tokens, workspace, n_rows, n_seqs, vocab, stream));
+}
+
 /* setup(torch.Tensor, torch.float16, torch.int32, torch.float32, current device, current stream
- * of a device) */
+ * of a device, torch.float8_e4m3fn) */
 static PyObject* setup(PyObject* self, PyObject* args) {
   (void)self;
-  PyObject** to[] = {&tensor_type, &half_dtype, &int_dtype, &float_dtype, &get_device, &get_stream};
-  PyObject* from[6];
-  if (!PyArg_ParseTuple(args, "OOOOOO", &from[0], &from[1], &from[2], &from[3], &from[4], &from[5]))
+  PyObject** to[] = {&tensor_type, &half_dtype, &int_dtype, &float_dtype,
+                     &get_device,  &get_stream, &e4m3_dtype};
+  PyObject* from[7];
+  if (!PyArg_ParseTuple(args, "OOOOOOO", &from[0], &from[1], &from[2], &from[3], &from[4], &from[5],
+                        &from[6]))
     return NULL;
-  for (int i = 0; i < 6; ++i) {
+  for (int i = 0; i < 7; ++i) {
     PyObject* old = *to[i];
     *to[i] = Py_NewRef(from[i]);
     Py_XDECREF(old);
@@ -255,6 +420,10 @@ static PyMethodDef methods[] = {METHOD(rmsnorm),
                                 METHOD(linear_rows_residual),
                                 METHOD(linear_rows_swiglu),
                                 METHOD(attention_decode_fast),
+                                METHOD(kv8_append),
+                                METHOD(kv8_gather),
+                                METHOD(kv8_attention),
+                                METHOD(verify_drafts),
                                 {"setup", setup, METH_VARARGS, NULL},
                                 {NULL, NULL, 0, NULL}};
 
@@ -266,7 +435,8 @@ PyMODINIT_FUNC PyInit__fast_calls(void) {
       !(s_dtype = PyUnicode_InternFromString("dtype")) ||
       !(s_is_contiguous = PyUnicode_InternFromString("is_contiguous")) ||
       !(s_numel = PyUnicode_InternFromString("numel")) ||
-      !(s_data_ptr = PyUnicode_InternFromString("data_ptr")))
+      !(s_data_ptr = PyUnicode_InternFromString("data_ptr")) ||
+      !(s_get_device = PyUnicode_InternFromString("get_device")))
     return NULL;
   return PyModule_Create(&module);
 }

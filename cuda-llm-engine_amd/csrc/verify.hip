@@ -10,15 +10,18 @@
 // greedy choice: a draft is accepted where it is the row's argmax, which is also the token. NaN
 // logits count as -inf; where +inf occurs, its places share all probability.
 //
-// Which token a random number falls on is settled at the borders of sums over 10^5 weights, so
-// exponentials, sums and comparisons are in 64 bits (their vector rate here is that of 32 bits).
+// Which token a random number falls on is settled at the borders of sums over 10^5 weights: what that
+// depends on, the row where a sequence ends, is done in 64 bits (exponentials, sums, comparisons).
+// Whether a draft stands compares two numbers: there the sums are 32-bit first, off by less than 2^-16,
+// and only a draft that is nearer than 2^-14 to the border has its rows summed again.
 //
-// Three launches, none of which needs another's order inside itself:
-//  1. every row (target and draft) in chunks of 8192 logits: maximum, its place, sum of weights
-//     relative to the chunk's maximum. A chunk is read once and kept in registers for the sum.
-//  2. with draft logits: the sums of max(p - q, 0) over each chunk of the row where a sequence ends.
-//  3. one block for each sequence: the chunk that u2 falls into, the token in it, the outputs.
-// What decides where a sequence ends is a few loads from 1; 2 and 3 each find it for themselves.
+// Launches, none of which needs an order inside itself:
+//  1. every row (target and draft) in chunks of 8192 logits: maximum, its place where the choice is
+//     greedy, sum of weights relative to the chunk's maximum. A chunk is read once and kept in registers
+//     for the sum. This is the time of a large batch: 2 bytes a logit.
+//  2. where each sequence ends, found from 1 by each of its blocks; the sums of that row's chunks.
+//  3. with draft logits: the sums of max(p - q, 0) over the row's chunks.
+//  4. one block for each sequence: the chunk that u2 falls into, the token in it, the outputs.
 #include <math.h>
 
 #include "common.hpp"
@@ -28,13 +31,24 @@ namespace {
 
 constexpr int kThreads = 256, kVectors = 4;             // 16-byte vectors per thread of a chunk
 constexpr int kChunk = kThreads * kVectors * 8;         // logits per chunk
+constexpr int kChooseThreads = kChunk / 8;              // one vector each
 constexpr double kLog2e = 1.44269504088896340736;
 
 struct Stat {
-  double sum;  // of 2^((l - max) log2e / t) over the chunk
-  float max;
-  int at;  // the lowest place of the maximum
+  float max, sum;  // sum: of 2^((l - max) log2e / t)
+  int at;          // the lowest place of the maximum, where the choice is greedy
+  int pad;
 };
+
+// Where a sequence ends.
+struct End {
+  int first, end, row;  // its rows, and the one that gives its last token
+  int last;             // that one stands behind all drafts
+  int greedy, at;       // at: the row's argmax, where the choice is greedy
+  float pm, qm;         // maxima of the target's and the draft model's row
+  double k;             // log2e / t
+};
+static_assert(sizeof(End) == 40, "workspace layout");
 
 struct VerifyArgs {
   const f16* logits;
@@ -46,8 +60,11 @@ struct VerifyArgs {
   const float* sample_u;
   int* n_accepted;
   int* tokens;
-  Stat* stats;   // [2][n_rows][chunks]: target, draft
-  double* left;  // [n_seqs][chunks]
+  Stat* stats;    // [2][n_rows][chunks]: target, draft
+  End* ends;      // [n_seqs]
+  double2* sums;  // [n_seqs][chunks]: of the target's weights (without a refused certain draft's), and
+                  // of the draft model's, or that draft's weight in its chunk
+  double* left;   // [n_seqs][chunks]: of max(p - q, 0)
   int n_rows, n_seqs, vocab, chunks;
 };
 
@@ -76,6 +93,11 @@ __device__ __forceinline__ double exp2_64(double y) {
 __device__ __forceinline__ double weight(float l, float max, double k) {
   const float d = l == max ? 0.0f : l - max;
   return exp2_64((double)d * k);
+}
+
+// The exponent of a 32-bit weight, d <= 0 times k. -inf times 0 (an infinite t) is -inf here.
+__device__ __forceinline__ float weight_exponent(float d, float k) {
+  return __builtin_fmaxf(d * k, -INFINITY);
 }
 
 __device__ __forceinline__ float logit(f16 x) {
@@ -107,12 +129,16 @@ __device__ __forceinline__ f16x8 load_vector(const Row& r, int v) {
   return x;
 }
 
+// The sum over a block of WAVES waves, in every thread. shared: WAVES numbers.
+template <int WAVES>
 __device__ __forceinline__ double block_sum(double v, double* shared) {
   for (int d = 1; d < 64; d *= 2) v = v + __shfl_xor(v, d);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
   __syncthreads();
-  return (shared[0] + shared[1]) + (shared[2] + shared[3]);
+  double sum = shared[0];
+  for (int w = 1; w < WAVES; ++w) sum = sum + shared[w];
+  return sum;
 }
 
 __device__ __forceinline__ bool is_greedy(float t) { return !(t > 0.0f); }
@@ -126,12 +152,16 @@ __device__ __forceinline__ void rows_of(const VerifyArgs& a, int s, int& first, 
 }
 
 __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
-  __shared__ double shared[4];
-  __shared__ float top[4];
-  __shared__ int top_at[4];
-  const int tid = threadIdx.x;
+  __shared__ float shared[4];
+  __shared__ int shared_at[4];
+  const int tid = threadIdx.x, wave = tid >> 6;
   const int chunk = blockIdx.x % a.chunks, which = blockIdx.x / a.chunks;
   const int draft = which >= a.n_rows, row = which - draft * a.n_rows;
+  const Row r = row_of(draft ? a.draft_logits : a.logits, row, a.vocab);
+  f16x8 x[kVectors];
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j)
+    x[j] = load_vector(r, (chunk * kVectors + j) * kThreads + tid);
   // the row's sequence, found by halves: few, and the same in every thread
   int s = row;
   if (a.starts) {
@@ -143,70 +173,84 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
     s = lo;
     if (s >= a.n_seqs || a.starts[0] > row) return;
     if (draft && row == a.starts[s + 1] - 1) return;  // no draft there
-  } else if (draft || s >= a.n_seqs) {
+  } else if (s >= a.n_seqs) {
     return;
   }
   const float t = a.temperature ? a.temperature[s] : 1.0f;
-  if (draft && is_greedy(t)) return;
-  const Row r = row_of(draft ? a.draft_logits : a.logits, row, a.vocab);
-  f16x8 x[kVectors];
+  const bool greedy = is_greedy(t);
+  if (draft && greedy) return;
+  f16x8 top = (f16x8)(f16)-INFINITY;
 #pragma unroll
-  for (int j = 0; j < kVectors; ++j)
-    x[j] = load_vector(r, (chunk * kVectors + j) * kThreads + tid);
-  float best = -INFINITY;
+  for (int j = 0; j < kVectors; ++j) {
+    x[j] = __builtin_elementwise_max(x[j], (f16x8)(f16)-INFINITY);  // NaN counts as -inf
+    top = __builtin_elementwise_max(top, x[j]);
+  }
+  float best = (float)top[0];
+#pragma unroll
+  for (int e = 1; e < 8; ++e) best = __builtin_fmaxf(best, (float)top[e]);
+  for (int d = 1; d < 64; d *= 2) best = __builtin_fmaxf(best, __shfl_xor(best, d));
+  if ((tid & 63) == 0) shared[wave] = best;
+  __syncthreads();
+  best = __builtin_fmaxf(__builtin_fmaxf(shared[0], shared[1]),
+                         __builtin_fmaxf(shared[2], shared[3]));
+  __syncthreads();
+  float sum = 0.0f;
   int at = 0x7FFFFFFF;
+  if (best > -INFINITY) {
+    if (greedy) {
 #pragma unroll
-  for (int j = 0; j < kVectors; ++j)
+      for (int j = kVectors - 1; j >= 0; --j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float l = logit(x[j][e]);
-      if (l > best) {
-        best = l;
-        at = 8 * ((chunk * kVectors + j) * kThreads + tid) - r.lead + e;
-      }
+        for (int e = 7; e >= 0; --e)
+          if ((float)x[j][e] == best)
+            at = 8 * ((chunk * kVectors + j) * kThreads + tid) - r.lead + e;
+    } else if (best == INFINITY) {
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum = sum + ((float)x[j][e] == best ? 1.0f : 0.0f);
+    } else {
+      // k and an exponent y are rounded, 2^-23 |y| in all and |y| <= 126 (smaller weights vanish), a
+      // weight by 2^-23, 32 of them and 8 parts in a sum: less than 2^-16 of the sum. k is finite, so
+      // that 0 k is 0.
+      const float k = __builtin_fminf((float)(kLog2e / (double)t), 3.0e38f);
+#pragma unroll
+      for (int j = 0; j < kVectors; ++j)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          sum = sum + __builtin_amdgcn_exp2f(weight_exponent((float)x[j][e] - best, k));
     }
+  }
   for (int d = 1; d < 64; d *= 2) {
-    const float ob = __shfl_xor(best, d);
-    const int oa = __shfl_xor(at, d);
-    const bool take = ob > best || (ob == best && oa < at);
-    best = take ? ob : best;
-    at = take ? oa : at;
+    sum = sum + __shfl_xor(sum, d);
+    const int o = __shfl_xor(at, d);
+    at = o < at ? o : at;
   }
   if ((tid & 63) == 0) {
-    top[tid >> 6] = best;
-    top_at[tid >> 6] = at;
+    shared[wave] = sum;
+    shared_at[wave] = at;
   }
   __syncthreads();
-  best = top[0];
-  at = top_at[0];
-  for (int w = 1; w < 4; ++w)
-    if (top[w] > best || (top[w] == best && top_at[w] < at)) {
-      best = top[w];
-      at = top_at[w];
-    }
-  double sum = 0.0;
-  if (!is_greedy(t) && best > -INFINITY) {
-    const double k = kLog2e / (double)t;
-#pragma unroll
-    for (int j = 0; j < kVectors; ++j)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) sum = sum + weight(logit(x[j][e]), best, k);
-  }
-  sum = block_sum(sum, shared);
   if (tid == 0) {
     Stat out;
-    out.sum = sum;
     out.max = best;
-    out.at = at;
+    out.sum = (shared[0] + shared[1]) + (shared[2] + shared[3]);
+    out.at = min(min(shared_at[0], shared_at[1]), min(shared_at[2], shared_at[3]));
+    out.pad = 0;
     a.stats[(size_t)which * a.chunks + chunk] = out;
   }
 }
 
 // A row's maximum, its place and its sum of weights, from its chunks; by one wave.
-__device__ __forceinline__ Stat row_stat(const VerifyArgs& a, size_t which, bool sums, double k) {
+struct RowStat {
+  float max;
+  int at;
+  double sum;
+};
+__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, size_t which, bool sums, double k) {
   const Stat* st = a.stats + which * a.chunks;
   const int lane = threadIdx.x & 63;
-  Stat r;
+  RowStat r;
   r.max = -INFINITY;
   r.at = 0x7FFFFFFF;
   r.sum = 0.0;
@@ -223,20 +267,22 @@ __device__ __forceinline__ Stat row_stat(const VerifyArgs& a, size_t which, bool
       r.at = oa;
     }
   }
-  if (sums)
+  if (sums) {
     for (int c = lane; c < a.chunks; c += 64)
-      if (st[c].max > -INFINITY) r.sum = r.sum + st[c].sum * weight(st[c].max, r.max, k);
-  for (int d = 1; d < 64; d *= 2) r.sum = r.sum + __shfl_xor(r.sum, d);
+      if (st[c].max > -INFINITY) r.sum = r.sum + (double)st[c].sum * weight(st[c].max, r.max, k);
+    for (int d = 1; d < 64; d *= 2) r.sum = r.sum + __shfl_xor(r.sum, d);
+  }
   return r;
 }
 
-struct End {
-  int first, end, row;  // the sequence's rows, and the one that gives its last token
-  bool last;            // it stands behind all drafts
-  bool greedy;
-  double k;
-  Stat p, q;  // q: with draft logits, and not last
-};
+// A row's sum of weights in 64 bits, by one wave.
+__device__ double exact_sum(const f16* logits, size_t row, int vocab, float max, double k) {
+  double sum = 0.0;
+  for (int v = threadIdx.x & 63; v < vocab; v += 64)
+    sum = sum + weight(logit(logits[row * vocab + v]), max, k);
+  for (int d = 1; d < 64; d *= 2) sum = sum + __shfl_xor(sum, d);
+  return sum;
+}
 
 // Where a sequence ends, in every thread of the block. Wave w looks at rows w, w + 4, ..
 __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
@@ -250,23 +296,34 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
   if (threadIdx.x == 0) stop = z.end - 1;
   __syncthreads();
   for (int row = z.first + wave; row < z.end - 1; row += 4) {
-    const Stat p = row_stat(a, row, !z.greedy, z.k);
     const int d = a.drafts[row];
+    const bool inside = d >= 0 && d < a.vocab;
+    const float u = a.accept_u[row];
+    const size_t at = (size_t)row * a.vocab + (inside ? d : 0);
+    const float ld = logit(a.logits[at]), lq = a.draft_logits ? logit(a.draft_logits[at]) : 0.0f;
+    const RowStat p = row_stat(a, row, !z.greedy, z.k);
     bool accept;
     if (z.greedy) {
-      accept = p.max > -INFINITY && d == p.at;
-    } else if (d < 0 || d >= a.vocab || !(p.max > -INFINITY)) {
+      accept = inside && p.max > -INFINITY && d == p.at;
+    } else if (!inside || !(p.max > -INFINITY)) {
       accept = false;
     } else {
-      const double pd = weight(logit(a.logits[(size_t)row * a.vocab + d]), p.max, z.k) / p.sum;
-      double qd = 1.0;
+      // u q(d) < p(d), as one side against the other with the sums multiplied out
+      const double pw = weight(ld, p.max, z.k);
+      double qw = 1.0, qs = 1.0;
+      float qm = -INFINITY;
       if (a.draft_logits) {
-        const Stat q = row_stat(a, (size_t)a.n_rows + row, true, z.k);
-        qd = q.max > -INFINITY
-                 ? weight(logit(a.draft_logits[(size_t)row * a.vocab + d]), q.max, z.k) / q.sum
-                 : 0.0;
+        const RowStat q = row_stat(a, (size_t)a.n_rows + row, true, z.k);
+        qm = q.max;
+        qw = qm > -INFINITY ? weight(lq, qm, z.k) : 0.0;
+        qs = qm > -INFINITY ? q.sum : 1.0;
       }
-      accept = (double)a.accept_u[row] * qd < pd;
+      double one = (double)u * (qw / qs), other = pw / p.sum;
+      if (__builtin_fabs(one - other) < 6.103515625e-5 * __builtin_fmax(one, other)) {
+        if (qm > -INFINITY) one = (double)u * (qw / exact_sum(a.draft_logits, row, a.vocab, qm, z.k));
+        other = pw / exact_sum(a.logits, row, a.vocab, p.max, z.k);
+      }
+      accept = one < other;
     }
     if (!accept) {
       if ((threadIdx.x & 63) == 0) atomicMin(&stop, row);
@@ -276,42 +333,24 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
   __syncthreads();
   z.row = stop;
   z.last = z.row == z.end - 1;
+  z.pm = z.qm = -INFINITY;
+  z.at = -1;
   if (z.row >= z.first) {
-    z.p = row_stat(a, z.row, !z.greedy, z.k);
-    if (a.draft_logits && !z.last && !z.greedy) z.q = row_stat(a, (size_t)a.n_rows + z.row, true, z.k);
+    const RowStat p = row_stat(a, z.row, false, z.k);
+    z.pm = p.max;
+    z.at = p.at;
+    if (a.draft_logits && !z.last && !z.greedy)
+      z.qm = row_stat(a, (size_t)a.n_rows + z.row, false, z.k).max;
   }
   return z;
 }
-
-// The weight that a place has in what the last token is drawn from.
-struct Left {
-  float pm, qm;
-  double k, ps, qs;  // 1 / sums; qs = 0: no draft model's share
-  int without;       // a certain draft that was refused, -1
-};
-__device__ __forceinline__ double left_of(const Left& w, float l, float ld, int at) {
-  const double p = weight(l, w.pm, w.k) * w.ps;
-  if (at == w.without) return 0.0;
-  if (w.qs == 0.0) return p;
-  return __builtin_fmax(p - weight(ld, w.qm, w.k) * w.qs, 0.0);
+// Whether there is a token to draw.
+__device__ __forceinline__ bool draws(const End& z) {
+  return z.row >= z.first && !z.greedy && z.pm > -INFINITY;
 }
-__device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z) {
-  Left w;
-  w.pm = z.p.max;
-  w.k = z.k;
-  w.ps = 1.0 / z.p.sum;
-  w.qm = 0.0f;
-  w.qs = 0.0;
-  w.without = -1;
-  if (!z.last) {
-    if (!a.draft_logits) {
-      w.without = a.drafts[z.row];
-    } else if (z.q.max > -INFINITY) {
-      w.qm = z.q.max;
-      w.qs = 1.0 / z.q.sum;
-    }
-  }
-  return w;
+// A certain draft that was refused, -1 if there is none.
+__device__ __forceinline__ int refused(const VerifyArgs& a, const End& z) {
+  return z.last || a.draft_logits ? -1 : a.drafts[z.row];
 }
 
 // The draft row's logit at the place of each element of the target row's vector v.
@@ -326,125 +365,176 @@ __device__ __forceinline__ f16x8 draft_vector(const VerifyArgs& a, size_t row, c
   return x;
 }
 
-__global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
+__global__ void __launch_bounds__(kThreads) k_verify_sums(const VerifyArgs a) {
   __shared__ double shared[4];
   const int chunk = blockIdx.x % a.chunks, s = blockIdx.x / a.chunks;
   const End z = find_end(a, s);
-  if (z.row < z.first || z.last || z.greedy || !(z.p.max > -INFINITY)) return;
-  const Left w = left_from(a, z);
+  if (chunk == 0 && threadIdx.x == 0) a.ends[s] = z;
+  if (!draws(z)) return;
+  const Row r = row_of(a.logits, z.row, a.vocab);
+  const int odd = refused(a, z);
+  const bool drafted = z.qm > -INFINITY;
+  double p = 0.0, q = 0.0;
+  for (int j = 0; j < kVectors; ++j) {
+    const int v = (chunk * kVectors + j) * kThreads + threadIdx.x;
+    const f16x8 x = load_vector(r, v), y = drafted ? draft_vector(a, z.row, r, v) : x;
+    for (int e = 0; e < 8; ++e) {
+      const double w = weight(logit(x[e]), z.pm, z.k);
+      if (drafted) q = q + weight(logit(y[e]), z.qm, z.k);
+      if (odd >= 0 && 8 * v - r.lead + e == odd)
+        q = q + w;
+      else
+        p = p + w;
+    }
+  }
+  p = block_sum<4>(p, shared);
+  if (drafted || odd >= 0) q = block_sum<4>(q, shared);
+  if (threadIdx.x == 0) a.sums[(size_t)s * a.chunks + chunk] = make_double2(p, q);
+}
+
+// What the last token is drawn from: a place's weight.
+struct Left {
+  float pm, qm;
+  double k, ps, qs;  // ps, qs: 1 / sums, or 1 and 0 where the draft model has no share
+  int odd;           // a certain draft that was refused, -1
+};
+__device__ __forceinline__ double left_of(const Left& w, float l, float lq, int at) {
+  const double p = weight(l, w.pm, w.k);
+  if (at == w.odd) return 0.0;
+  return w.qs == 0.0 ? p : __builtin_fmax(p * w.ps - weight(lq, w.qm, w.k) * w.qs, 0.0);
+}
+// By a block of WAVES waves.
+template <int WAVES>
+__device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int s,
+                                          double* shared) {
+  Left w = {z.pm, z.qm, z.k, 1.0, 0.0, refused(a, z)};
+  if (z.qm > -INFINITY) {
+    double p = 0.0, q = 0.0;
+    for (int c = threadIdx.x; c < a.chunks; c += 64 * WAVES) {
+      const double2 x = a.sums[(size_t)s * a.chunks + c];
+      p = p + x.x;
+      q = q + x.y;
+    }
+    w.ps = 1.0 / block_sum<WAVES>(p, shared);
+    w.qs = 1.0 / block_sum<WAVES>(q, shared);
+  }
+  return w;
+}
+
+__global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
+  __shared__ double shared[4];
+  const int chunk = blockIdx.x % a.chunks, s = blockIdx.x / a.chunks;
+  const End z = a.ends[s];
+  if (!draws(z) || !(z.qm > -INFINITY)) return;
+  const Left w = left_from<4>(a, z, s, shared);
   const Row r = row_of(a.logits, z.row, a.vocab);
   double sum = 0.0;
   for (int j = 0; j < kVectors; ++j) {
     const int v = (chunk * kVectors + j) * kThreads + threadIdx.x;
     const f16x8 x = load_vector(r, v), y = draft_vector(a, z.row, r, v);
-    for (int e = 0; e < 8; ++e) {
-      const int at = 8 * v - r.lead + e;
-      if (at >= 0 && at < a.vocab) sum = sum + left_of(w, logit(x[e]), logit(y[e]), at);
-    }
+    for (int e = 0; e < 8; ++e) sum = sum + left_of(w, logit(x[e]), logit(y[e]), -2);
   }
-  sum = block_sum(sum, shared);
+  sum = block_sum<4>(sum, shared);
   if (threadIdx.x == 0) a.left[(size_t)s * a.chunks + chunk] = sum;
 }
 
-__global__ void __launch_bounds__(kThreads) k_verify_choose(const VerifyArgs a) {
-  __shared__ double shared[4], before[kThreads];
+__global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyArgs a) {
+  constexpr int WAVES = kChooseThreads / 64;
+  __shared__ double shared[WAVES];
+  __shared__ double parts[kChooseThreads];
   __shared__ int first_past, last_any;
-  const int s = blockIdx.x, tid = threadIdx.x;
-  const End z = find_end(a, s);
-  for (int row = z.first + tid; row < z.end; row += kThreads)
-    a.tokens[row] = row < z.row ? a.drafts[row] : -1;
-  if (z.end <= z.first) {
-    if (tid == 0) a.n_accepted[s] = 0;
-    return;
-  }
-  __syncthreads();  // the row's own -1 is in place before its token
-  if (tid == 0) a.n_accepted[s] = z.row - z.first;
-  if (!(z.p.max > -INFINITY)) return;  // nothing to draw from
-  if (z.greedy) {
-    if (tid == 0) a.tokens[z.row] = z.p.at;
-    return;
-  }
-  Left w = left_from(a, z);
-  const Row r = row_of(a.logits, z.row, a.vocab);
-  // the sum over this thread's own 32 places of a chunk, which follow one another
-  auto mine = [&](int chunk, double* each) {
-    double sum = 0.0;
-    for (int j = 0; j < kVectors; ++j) {
-      const int v = (chunk * kThreads + tid) * kVectors + j;
-      const f16x8 x = load_vector(r, v);
-      const f16x8 y = w.qs != 0.0 ? draft_vector(a, z.row, r, v) : x;
-      for (int e = 0; e < 8; ++e) {
-        const int at = 8 * v - r.lead + e;
-        const double l =
-            at >= 0 && at < a.vocab ? left_of(w, logit(x[e]), logit(y[e]), at) : 0.0;
-        if (each) each[8 * j + e] = l;
-        sum = sum + l;
-      }
-    }
-    return sum;
-  };
-  const Stat* st = a.stats + (size_t)z.row * a.chunks;
-  auto p_sum = [&](int c) {
-    return st[c].max > -INFINITY ? st[c].sum * weight(st[c].max, z.p.max, z.k) * w.ps : 0.0;
-  };
-  // The sum without a refused draft is taken again, not subtracted: it may be all there was.
-  const int odd = w.without >= 0 && w.without < a.vocab ? (w.without + r.lead) / kChunk : -1;
-  const double odd_sum = odd >= 0 ? block_sum(mine(odd, nullptr), shared) : 0.0;
-  bool only_p = false;
-  auto chunk_sum = [&](int c) {
-    if (only_p) return p_sum(c);
-    if (w.qs != 0.0) return a.left[(size_t)s * a.chunks + c];
-    return c == odd ? odd_sum : p_sum(c);
-  };
-  double total = 0.0;
-  for (int c = 0; c < a.chunks; ++c) total = total + chunk_sum(c);
-  if (!(total > 0.0)) {  // p is nowhere above q
-    only_p = true;
-    w.without = -1;
-    w.qs = 0.0;
-    for (int c = 0; c < a.chunks; ++c) total = total + p_sum(c);
-  }
-  const double aim = (double)a.sample_u[s] * total;
-  int chunk = 0;
-  double base = 0.0, sum = 0.0;
-  for (int c = 0; c < a.chunks; ++c) {
-    const double one = chunk_sum(c);
-    if (one > 0.0) {  // where rounding leaves the aim behind all: the last chunk with any weight
-      chunk = c;
-      base = sum;
-    }
-    sum = sum + one;
-    if (sum > aim) break;
-  }
-  double each[kVectors * 8];
-  const double own = mine(chunk, each);
-  before[tid] = own;
+  int chosen = 0;
+  double chosen_base = 0.0;
+  const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const End z = a.ends[s];
+  for (int row = z.first + tid; row < z.end; row += kChooseThreads)
+    if (row != z.row) a.tokens[row] = row < z.row ? a.drafts[row] : -1;
   if (tid == 0) {
+    a.n_accepted[s] = z.end > z.first ? z.row - z.first : 0;
+    if (z.end > z.first && !draws(z)) a.tokens[z.row] = z.greedy && z.pm > -INFINITY ? z.at : -1;
     first_past = 0x7FFFFFFF;
     last_any = -1;
   }
-  __syncthreads();
-  for (int d = 1; d < kThreads; d *= 2) {
-    const double add = tid >= d ? before[tid - d] : 0.0;
-    __syncthreads();
-    before[tid] = before[tid] + add;
-    __syncthreads();
+  if (!draws(z)) return;
+  Left w = left_from<WAVES>(a, z, s, shared);
+  const double2* sums = a.sums + (size_t)s * a.chunks;
+  // chunk c's sum; with only_p of p alone, where p is nowhere above q
+  const bool drafted = w.qs != 0.0, certain = w.odd >= 0;
+  bool only_p = false;
+  auto chunk_sum = [&](int c) {
+    if (only_p) return certain ? sums[c].x + sums[c].y : sums[c].x;
+    return drafted ? a.left[(size_t)s * a.chunks + c] : sums[c].x;
+  };
+  auto total_of = [&] {
+    double sum = 0.0;
+    for (int c = tid; c < a.chunks; c += kChooseThreads) sum = sum + chunk_sum(c);
+    return block_sum<WAVES>(sum, shared);
+  };
+  double total = total_of();
+  if (!(total > 0.0)) {
+    only_p = true;
+    w.odd = -1;
+    w.qs = 0.0;
+    total = total_of();
   }
-  // every thread's candidate: its first place past the aim, or behind it its last with any weight
-  double c = base + (tid > 0 ? before[tid - 1] : 0.0);
-  int token = -1, last = -1;
-  for (int e = 0; e < kVectors * 8; ++e) {
-    c = c + each[e];
-    const int at = (chunk * kThreads + tid) * kVectors * 8 + e - r.lead;
-    if (each[e] > 0.0) {
-      last = at;
-      if (token < 0 && c > aim) token = at;
+  const double aim = (double)a.sample_u[s] * total;
+  // the first chunk that ends past the aim, or behind them all, by rounding, the last with any weight
+  double before = 0.0;
+  bool past = false;
+  for (int c0 = 0; c0 < a.chunks && !past; c0 += kChooseThreads) {
+    const int n = a.chunks - c0 < kChooseThreads ? a.chunks - c0 : kChooseThreads;
+    __syncthreads();
+    if (tid < n) parts[tid] = chunk_sum(c0 + tid);
+    __syncthreads();
+    for (int c = 0; c < n && !past; ++c) {
+      const double one = parts[c];
+      if (one > 0.0) {
+        chosen = c0 + c;
+        chosen_base = before;
+      }
+      before = before + one;
+      past = before > aim;
     }
   }
-  if (token >= 0) atomicMin(&first_past, token);
+  __syncthreads();  // `shared` is free
+  const Row r = row_of(a.logits, z.row, a.vocab);
+  const int v = chosen * kChooseThreads + tid;
+  const f16x8 x = load_vector(r, v), y = w.qs != 0.0 ? draft_vector(a, z.row, r, v) : x;
+  double each[8], own = 0.0;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    each[e] = left_of(w, logit(x[e]), logit(y[e]), 8 * v - r.lead + e);
+    own = own + each[e];
+  }
+  double upto = own;
+  for (int d = 1; d < 64; d *= 2) {
+    const double o = __shfl_up(upto, d);
+    if (lane >= d) upto = upto + o;
+  }
+  if (lane == 63) shared[tid >> 6] = upto;
+  __syncthreads();
+  double c = chosen_base + (upto - own);
+  for (int k = 0; k < (tid >> 6); ++k) c = c + shared[k];
+  // every thread's candidate: its first place past the aim; and its last with any weight
+  int token = 0x7FFFFFFF, last = -1;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    c = c + each[e];
+    if (each[e] > 0.0) {
+      last = 8 * v - r.lead + e;
+      if (c > aim && token == 0x7FFFFFFF) token = last;
+    }
+  }
+  if (token != 0x7FFFFFFF) atomicMin(&first_past, token);
   if (last >= 0) atomicMax(&last_any, last);
   __syncthreads();
   if (tid == 0) a.tokens[z.row] = first_past != 0x7FFFFFFF ? first_past : last_any;
+}
+
+// No rows at all: no draft stands.
+__global__ void __launch_bounds__(kThreads) k_verify_none(int* n_accepted, int n_seqs) {
+  const int s = blockIdx.x * kThreads + threadIdx.x;
+  if (s < n_seqs) n_accepted[s] = 0;
 }
 
 int chunks_of(int vocab) { return (int)(((long long)vocab + 7 + kChunk - 1) / kChunk); }
@@ -457,7 +547,8 @@ using namespace llmk;
 extern "C" size_t llmk_verify_drafts_workspace_floats(int n_rows, int n_seqs, int vocab) {
   if (n_rows <= 0 || n_seqs <= 0 || vocab <= 0) return 0;
   const size_t chunks = (size_t)chunks_of(vocab);
-  return chunks * (2 * (size_t)n_rows * (sizeof(Stat) / 4) + 2 * (size_t)n_seqs);
+  return 4 * ((size_t)n_seqs * 3) +  // ends of 40 bytes, to 16
+         chunks * (2 * (size_t)n_rows * (sizeof(Stat) / 4) + (size_t)n_seqs * 8);
 }
 
 extern "C" int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_logits,
@@ -489,20 +580,23 @@ extern "C" int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_
   a.n_accepted = n_accepted;
   a.tokens = tokens;
   a.stats = reinterpret_cast<Stat*>(workspace);
-  a.left = reinterpret_cast<double*>(a.stats + (size_t)2 * n_rows * chunks);
+  a.sums = reinterpret_cast<double2*>(a.stats + (size_t)2 * n_rows * chunks);
+  a.left = reinterpret_cast<double*>(a.sums + (size_t)n_seqs * chunks);
+  a.ends = reinterpret_cast<End*>(a.left + (size_t)2 * n_seqs * chunks);
   a.n_rows = n_rows;
   a.n_seqs = n_seqs;
   a.vocab = vocab;
   a.chunks = chunks;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  int rc = LLMK_OK;
-  if (n_rows > 0) {
-    const unsigned rows = (unsigned)n_rows * (a.draft_logits ? 2u : 1u);
-    rc = launch(k_verify_stats, dim3((unsigned)chunks * rows), dim3(kThreads), 0, st, a);
-    if (rc == LLMK_OK && a.draft_logits)
-      rc = launch(k_verify_left, dim3((unsigned)chunks * (unsigned)n_seqs), dim3(kThreads), 0, st,
-                  a);
-  }
+  if (n_rows == 0)
+    return launch(k_verify_none, dim3(ceil_div((size_t)n_seqs, kThreads)), dim3(kThreads), 0, st,
+                  n_accepted, n_seqs);
+  const unsigned rows = (unsigned)n_rows * (a.draft_logits ? 2u : 1u);
+  int rc = launch(k_verify_stats, dim3((unsigned)chunks * rows), dim3(kThreads), 0, st, a);
+  const dim3 per_chunk((unsigned)chunks * (unsigned)n_seqs);
+  if (rc == LLMK_OK) rc = launch(k_verify_sums, per_chunk, dim3(kThreads), 0, st, a);
+  if (rc == LLMK_OK && a.draft_logits)
+    rc = launch(k_verify_left, per_chunk, dim3(kThreads), 0, st, a);
   if (rc != LLMK_OK) return rc;
-  return launch(k_verify_choose, dim3((unsigned)n_seqs), dim3(kThreads), 0, st, a);
+  return launch(k_verify_choose, dim3((unsigned)n_seqs), dim3(kChooseThreads), 0, st, a);
 }

@@ -188,6 +188,41 @@ def test_many_rows_of_one_sequence_and_many_sequences(llmk):
     check(llmk, case(14, rng.integers(0, 4, 700), 33, True))
 
 
+def test_no_rows(llmk):
+    """Sequences without a row in the call: nothing but zeros, and no workspace needed."""
+    n_accepted = torch.full((5,), -9, dtype=torch.int32, device=DEV)
+    none = torch.empty(0, dtype=torch.float16, device=DEV)
+    llmk.verify_drafts(none, None, none.int(), torch.zeros(6, dtype=torch.int32, device=DEV), None,
+                       none.float(), torch.zeros(5, device=DEV), n_accepted, none.int(),
+                       none.float(), 0, 5, 100)
+    torch.cuda.synchronize()
+    assert not n_accepted.any()
+
+
+def test_drafts_next_to_the_border(llmk):
+    """Random numbers a few roundings of fp32 from p / q, on either side, over long rows: the
+    comparison is that of 64 bits."""
+    n, vocab = 12, 70001
+    c = list(case(21, [2] * n, vocab, True, std=1.0))
+    for drafted in (True, False):
+        if not drafted:
+            c[1] = None
+        for s in range(n):
+            r, d = 2 * s, int(c[2][2 * s])
+            p = ref.softmax(c[0][r], float(c[4][s]))[d]
+            q = ref.softmax(c[1][r], float(c[4][s]))[d] if drafted else 1.0
+            if p >= q:  # the draft's probability is to be the smaller one
+                c[2][r] = d = int((ref.softmax(c[0][r], 1.0) - (
+                    ref.softmax(c[1][r], 1.0) if drafted else 1.0)).argmin())
+                p = ref.softmax(c[0][r], float(c[4][s]))[d]
+                q = ref.softmax(c[1][r], float(c[4][s]))[d] if drafted else 1.0
+            u = np.float32(min(p / q, 0.999))
+            for _ in range(abs(s - 6)):
+                u = np.nextafter(u, np.float32(s > 6))
+            c[5][r] = u
+        check(llmk, c)
+
+
 def test_graph_replays_with_other_numbers(llmk):
     """Captured once, replayed with other logits, numbers and rows, eager work in between."""
     a = case(15, [3, 1, 4, 2], 9000, True)

@@ -92,6 +92,8 @@ def test_attention(llmk):
     for bad in (dict(q=MIS), dict(out=MIS), dict(ws=MIS)):
         assert attention(L, **bad) == E.LLMK_ERR_ALIGNMENT, bad
     assert attention(L, heads=65536) == E.LLMK_ERR_UNSUPPORTED
+    assert attention(L, heads=513, kv=513) == E.LLMK_ERR_UNSUPPORTED
+    assert attention(L, max_pages=2 ** 27) == E.LLMK_ERR_UNSUPPORTED
     assert E.kv8_attention_workspace_floats(96) == 0
     assert 0 < E.kv8_attention_workspace_floats(64) < E.kv8_attention_workspace_floats(128) or (
         E.kv8_attention_workspace_floats(64) > 0)
@@ -109,7 +111,7 @@ def test_verify(llmk):
     assert verify(L, n_rows=2 ** 30, vocab=128256) == E.LLMK_ERR_UNSUPPORTED
     assert verify(L, vocab=2 ** 31 - 1) == E.LLMK_ERR_UNSUPPORTED
     assert E.verify_drafts_workspace_floats(0, 1, 8) == 0
-    assert E.verify_drafts_workspace_floats(5, 1, 128256) == 16 * (2 * 5 * 4 + 2)
+    assert E.verify_drafts_workspace_floats(5, 1, 128256) == 12 + 16 * (2 * 5 * 4 + 8)
 
 
 def test_python_face_refuses_host_tensors(llmk):
