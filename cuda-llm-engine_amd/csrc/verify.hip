@@ -68,42 +68,32 @@ struct VerifyArgs {
   int n_rows, n_seqs, vocab, chunks;
 };
 
-// 2^y for y <= 0, to the last bits of 64: the series of e^z, |z| <= ln 2 / 2, behind the whole part.
+// 2^y for y <= 0: the series of 2^f, |f| <= 1/2, behind the whole part, to 2^-42 of it. NaN gives 0.
 __device__ __forceinline__ double exp2_64(double y) {
   y = __builtin_fmax(y, -1100.0);
-  const double n = __builtin_rint(y);
-  const double z = (y - n) * 0.69314718055994530942;
-  double p = 1.0 / 479001600.0;
-  p = __builtin_fma(p, z, 1.0 / 39916800.0);
-  p = __builtin_fma(p, z, 1.0 / 3628800.0);
-  p = __builtin_fma(p, z, 1.0 / 362880.0);
-  p = __builtin_fma(p, z, 1.0 / 40320.0);
-  p = __builtin_fma(p, z, 1.0 / 5040.0);
-  p = __builtin_fma(p, z, 1.0 / 720.0);
-  p = __builtin_fma(p, z, 1.0 / 120.0);
-  p = __builtin_fma(p, z, 1.0 / 24.0);
-  p = __builtin_fma(p, z, 1.0 / 6.0);
-  p = __builtin_fma(p, z, 0.5);
-  p = __builtin_fma(p, z, 1.0);
-  p = __builtin_fma(p, z, 1.0);
+  const double n = __builtin_rint(y), f = y - n;
+  double p = 7.0549116208011233e-09;  // ln(2)^i / i!
+  p = __builtin_fma(p, f, 1.0178086009239699e-07);
+  p = __builtin_fma(p, f, 1.3215486790144309e-06);
+  p = __builtin_fma(p, f, 1.5252733804059840e-05);
+  p = __builtin_fma(p, f, 1.5403530393381609e-04);
+  p = __builtin_fma(p, f, 1.3333558146428443e-03);
+  p = __builtin_fma(p, f, 9.6181291076284772e-03);
+  p = __builtin_fma(p, f, 5.5504108664821580e-02);
+  p = __builtin_fma(p, f, 2.4022650695910071e-01);
+  p = __builtin_fma(p, f, 6.9314718055994531e-01);
+  p = __builtin_fma(p, f, 1.0);
   return __builtin_ldexp(p, (int)n);
 }
 
-// The weight of a logit under a maximum; k = log2e / t. Equal infinities weigh 1.
+// The weight of a logit under a maximum; k = log2e / t. Equal infinities weigh 1: what their
+// difference is not, a minimum with 0 makes 0.
 __device__ __forceinline__ double weight(float l, float max, double k) {
-  const float d = l == max ? 0.0f : l - max;
-  return exp2_64((double)d * k);
+  return exp2_64((double)__builtin_fminf(l - max, 0.0f) * k);
 }
 
-// The exponent of a 32-bit weight, d <= 0 times k. -inf times 0 (an infinite t) is -inf here.
-__device__ __forceinline__ float weight_exponent(float d, float k) {
-  return __builtin_fmaxf(d * k, -INFINITY);
-}
-
-__device__ __forceinline__ float logit(f16 x) {
-  const float l = (float)x;
-  return l != l ? -INFINITY : l;
-}
+// NaN counts as -inf.
+__device__ __forceinline__ float logit(f16 x) { return __builtin_fmaxf((float)x, -INFINITY); }
 
 // The vectors of a row: element e of the row is element e + lead of the 16-byte aligned memory that
 // holds it; vector v of it is the row's elements 8 v - lead .. + 7. Those that the row does not fill
@@ -129,16 +119,72 @@ __device__ __forceinline__ f16x8 load_vector(const Row& r, int v) {
   return x;
 }
 
-// The sum over a block of WAVES waves, in every thread. shared: WAVES numbers.
+// Sums in 64 bits by lane moves (as wave_sum): over each 16 lanes, over the wave, and over a block of
+// WAVES waves; the same in every thread. shared: WAVES numbers.
+template <int CTRL, int ROWS = 0xF>  // 0 where there is no source lane, and in rows not named
+__device__ __forceinline__ double dpp_f64(double v) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo =
+      __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, ROWS == 0xF);
+  const uint32_t hi =
+      __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xF, ROWS == 0xF);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double readlane_f64(double v, int lane) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+  return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+// The sum of the lanes up to each: within 16 lanes, then the rows in front (their last lanes', by
+// row_bcast).
+__device__ __forceinline__ double wave_prefix(double v) {
+  v = v + dpp_f64<0x111>(v);
+  v = v + dpp_f64<0x112>(v);
+  v = v + dpp_f64<0x114>(v);
+  v = v + dpp_f64<0x118>(v);
+  v = v + dpp_f64<0x142, 0xA>(v);
+  return v + dpp_f64<0x143, 0xC>(v);
+}
+template <int LANES>
+__device__ __forceinline__ double row_sum(double v) {
+  v = v + dpp_f64<0xB1>(v);
+  v = v + dpp_f64<0x4E>(v);
+  if constexpr (LANES == 16) {
+    v = v + dpp_f64<0x141>(v);
+    v = v + dpp_f64<0x140>(v);
+  }
+  return v;
+}
+__device__ __forceinline__ double wave_sum(double v) {
+  v = row_sum<16>(v);
+  return (readlane_f64(v, 0) + readlane_f64(v, 16)) + (readlane_f64(v, 32) + readlane_f64(v, 48));
+}
 template <int WAVES>
 __device__ __forceinline__ double block_sum(double v, double* shared) {
-  for (int d = 1; d < 64; d *= 2) v = v + __shfl_xor(v, d);
+  static_assert(WAVES == 4 || WAVES == 16, "a quad or a row of lanes takes the waves' sums");
+  v = wave_sum(v);
   __syncthreads();
   if ((threadIdx.x & 63) == 0) shared[threadIdx.x >> 6] = v;
   __syncthreads();
-  double sum = shared[0];
-  for (int w = 1; w < WAVES; ++w) sum = sum + shared[w];
-  return sum;
+  return row_sum<WAVES>(shared[threadIdx.x & (WAVES - 1)]);
+}
+__device__ __forceinline__ float wave_max(float v) {
+  v = __builtin_fmaxf(v, dpp_f32<0xB1>(v));
+  v = __builtin_fmaxf(v, dpp_f32<0x4E>(v));
+  v = __builtin_fmaxf(v, dpp_f32<0x141>(v));
+  v = __builtin_fmaxf(v, dpp_f32<0x140>(v));
+  return __builtin_fmaxf(__builtin_fmaxf(readlane_f32(v, 0), readlane_f32(v, 16)),
+                         __builtin_fmaxf(readlane_f32(v, 32), readlane_f32(v, 48)));
+}
+template <int CTRL>
+__device__ __forceinline__ int lower_dpp(int v) {
+  return min(v, __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ int wave_min(int v) {
+  v = lower_dpp<0x140>(lower_dpp<0x141>(lower_dpp<0x4E>(lower_dpp<0xB1>(v))));
+  return min(min(__builtin_amdgcn_readlane(v, 0), __builtin_amdgcn_readlane(v, 16)),
+             min(__builtin_amdgcn_readlane(v, 32), __builtin_amdgcn_readlane(v, 48)));
 }
 
 __device__ __forceinline__ bool is_greedy(float t) { return !(t > 0.0f); }
@@ -188,7 +234,7 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
   float best = (float)top[0];
 #pragma unroll
   for (int e = 1; e < 8; ++e) best = __builtin_fmaxf(best, (float)top[e]);
-  for (int d = 1; d < 64; d *= 2) best = __builtin_fmaxf(best, __shfl_xor(best, d));
+  best = wave_max(best);
   if ((tid & 63) == 0) shared[wave] = best;
   __syncthreads();
   best = __builtin_fmaxf(__builtin_fmaxf(shared[0], shared[1]),
@@ -211,21 +257,19 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
         for (int e = 0; e < 8; ++e) sum = sum + ((float)x[j][e] == best ? 1.0f : 0.0f);
     } else {
       // k and an exponent y are rounded, 2^-23 |y| in all and |y| <= 126 (smaller weights vanish), a
-      // weight by 2^-23, 32 of them and 8 parts in a sum: less than 2^-16 of the sum. k is finite, so
-      // that 0 k is 0.
-      const float k = __builtin_fminf((float)(kLog2e / (double)t), 3.0e38f);
+      // weight by 2^-23, 32 of them and 8 parts in a sum: less than 2^-16 of the sum. k is neither 0
+      // nor infinite, so that 0 k is 0 and -inf k is -inf.
+      const float k =
+          __builtin_fminf(__builtin_fmaxf((float)(kLog2e / (double)t), 1.0e-37f), 3.0e38f);
 #pragma unroll
       for (int j = 0; j < kVectors; ++j)
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-          sum = sum + __builtin_amdgcn_exp2f(weight_exponent((float)x[j][e] - best, k));
+          sum = sum + __builtin_amdgcn_exp2f(((float)x[j][e] - best) * k);
     }
   }
-  for (int d = 1; d < 64; d *= 2) {
-    sum = sum + __shfl_xor(sum, d);
-    const int o = __shfl_xor(at, d);
-    at = o < at ? o : at;
-  }
+  sum = llmk::wave_sum(sum);
+  at = wave_min(at);
   if ((tid & 63) == 0) {
     shared[wave] = sum;
     shared_at[wave] = at;
@@ -250,28 +294,19 @@ struct RowStat {
 __device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, size_t which, bool sums, double k) {
   const Stat* st = a.stats + which * a.chunks;
   const int lane = threadIdx.x & 63;
+  float max = -INFINITY, own = -INFINITY;
+  int at = 0x7FFFFFFF;
+  double sum = 0.0;
+  for (int c = lane; c < a.chunks; c += 64) own = __builtin_fmaxf(own, st[c].max);
   RowStat r;
-  r.max = -INFINITY;
-  r.at = 0x7FFFFFFF;
-  r.sum = 0.0;
-  for (int c = lane; c < a.chunks; c += 64)
-    if (st[c].max > r.max) {
-      r.max = st[c].max;
-      r.at = st[c].at;
-    }
-  for (int d = 1; d < 64; d *= 2) {
-    const float om = __shfl_xor(r.max, d);
-    const int oa = __shfl_xor(r.at, d);
-    if (om > r.max || (om == r.max && oa < r.at)) {
-      r.max = om;
-      r.at = oa;
-    }
+  r.max = max = wave_max(own);
+  for (int c = lane; c < a.chunks; c += 64) {
+    const Stat x = st[c];
+    if (x.max == max) at = min(at, x.at);
+    if (sums && x.max > -INFINITY) sum = sum + (double)x.sum * weight(x.max, max, k);
   }
-  if (sums) {
-    for (int c = lane; c < a.chunks; c += 64)
-      if (st[c].max > -INFINITY) r.sum = r.sum + (double)st[c].sum * weight(st[c].max, r.max, k);
-    for (int d = 1; d < 64; d *= 2) r.sum = r.sum + __shfl_xor(r.sum, d);
-  }
+  r.at = wave_min(at);
+  r.sum = sums ? wave_sum(sum) : 0.0;
   return r;
 }
 
@@ -280,8 +315,7 @@ __device__ double exact_sum(const f16* logits, size_t row, int vocab, float max,
   double sum = 0.0;
   for (int v = threadIdx.x & 63; v < vocab; v += 64)
     sum = sum + weight(logit(logits[row * vocab + v]), max, k);
-  for (int d = 1; d < 64; d *= 2) sum = sum + __shfl_xor(sum, d);
-  return sum;
+  return wave_sum(sum);
 }
 
 // Where a sequence ends, in every thread of the block. Wave w looks at rows w, w + 4, ..
@@ -374,18 +408,30 @@ __global__ void __launch_bounds__(kThreads) k_verify_sums(const VerifyArgs a) {
   const Row r = row_of(a.logits, z.row, a.vocab);
   const int odd = refused(a, z);
   const bool drafted = z.qm > -INFINITY;
+  const int v0 = chunk * kVectors * kThreads + threadIdx.x;
+  f16x8 x[kVectors], y[kVectors];
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j) x[j] = load_vector(r, v0 + j * kThreads);
+  if (drafted) {
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j) y[j] = draft_vector(a, z.row, r, v0 + j * kThreads);
+  }
   double p = 0.0, q = 0.0;
-  for (int j = 0; j < kVectors; ++j) {
-    const int v = (chunk * kVectors + j) * kThreads + threadIdx.x;
-    const f16x8 x = load_vector(r, v), y = drafted ? draft_vector(a, z.row, r, v) : x;
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j)
+#pragma unroll 2
     for (int e = 0; e < 8; ++e) {
-      const double w = weight(logit(x[e]), z.pm, z.k);
-      if (drafted) q = q + weight(logit(y[e]), z.qm, z.k);
-      if (odd >= 0 && 8 * v - r.lead + e == odd)
+      const double w = weight(logit(x[j][e]), z.pm, z.k);
+      if (odd >= 0 && 8 * (v0 + j * kThreads) - r.lead + e == odd)
         q = q + w;
       else
         p = p + w;
     }
+  if (drafted) {
+#pragma unroll
+    for (int j = 0; j < kVectors; ++j)
+#pragma unroll 2
+      for (int e = 0; e < 8; ++e) q = q + weight(logit(y[j][e]), z.qm, z.k);
   }
   p = block_sum<4>(p, shared);
   if (drafted || odd >= 0) q = block_sum<4>(q, shared);
@@ -403,14 +449,14 @@ __device__ __forceinline__ double left_of(const Left& w, float l, float lq, int 
   if (at == w.odd) return 0.0;
   return w.qs == 0.0 ? p : __builtin_fmax(p * w.ps - weight(lq, w.qm, w.k) * w.qs, 0.0);
 }
-// By a block of WAVES waves.
+// By a block of WAVES waves; first: the sums of chunk threadIdx.x, 0 where there is none.
 template <int WAVES>
-__device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int s,
+__device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int s, double2 first,
                                           double* shared) {
   Left w = {z.pm, z.qm, z.k, 1.0, 0.0, refused(a, z)};
   if (z.qm > -INFINITY) {
-    double p = 0.0, q = 0.0;
-    for (int c = threadIdx.x; c < a.chunks; c += 64 * WAVES) {
+    double p = first.x, q = first.y;
+    for (int c = threadIdx.x + 64 * WAVES; c < a.chunks; c += 64 * WAVES) {
       const double2 x = a.sums[(size_t)s * a.chunks + c];
       p = p + x.x;
       q = q + x.y;
@@ -425,15 +471,23 @@ __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
   __shared__ double shared[4];
   const int chunk = blockIdx.x % a.chunks, s = blockIdx.x / a.chunks;
   const End z = a.ends[s];
+  const double2 first = (int)threadIdx.x < a.chunks ? a.sums[(size_t)s * a.chunks + threadIdx.x]
+                                                    : make_double2(0.0, 0.0);
   if (!draws(z) || !(z.qm > -INFINITY)) return;
-  const Left w = left_from<4>(a, z, s, shared);
   const Row r = row_of(a.logits, z.row, a.vocab);
-  double sum = 0.0;
+  const int v0 = chunk * kVectors * kThreads + threadIdx.x;
+  f16x8 x[kVectors], y[kVectors];
+#pragma unroll
   for (int j = 0; j < kVectors; ++j) {
-    const int v = (chunk * kVectors + j) * kThreads + threadIdx.x;
-    const f16x8 x = load_vector(r, v), y = draft_vector(a, z.row, r, v);
-    for (int e = 0; e < 8; ++e) sum = sum + left_of(w, logit(x[e]), logit(y[e]), -2);
+    x[j] = load_vector(r, v0 + j * kThreads);
+    y[j] = draft_vector(a, z.row, r, v0 + j * kThreads);
   }
+  const Left w = left_from<4>(a, z, s, first, shared);
+  double sum = 0.0;
+#pragma unroll
+  for (int j = 0; j < kVectors; ++j)
+#pragma unroll 2
+    for (int e = 0; e < 8; ++e) sum = sum + left_of(w, logit(x[j][e]), logit(y[j][e]), -2);
   sum = block_sum<4>(sum, shared);
   if (threadIdx.x == 0) a.left[(size_t)s * a.chunks + chunk] = sum;
 }
@@ -447,6 +501,12 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
   double chosen_base = 0.0;
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const End z = a.ends[s];
+  const double2* sums = a.sums + (size_t)s * a.chunks;
+  // what all this waits for, in one go
+  const double2 first = tid < a.chunks ? sums[tid] : make_double2(0.0, 0.0);
+  const double first_left =
+      a.draft_logits && tid < a.chunks ? a.left[(size_t)s * a.chunks + tid] : 0.0;
+  const float u = a.sample_u[s];
   for (int row = z.first + tid; row < z.end; row += kChooseThreads)
     if (row != z.row) a.tokens[row] = row < z.row ? a.drafts[row] : -1;
   if (tid == 0) {
@@ -456,14 +516,14 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
     last_any = -1;
   }
   if (!draws(z)) return;
-  Left w = left_from<WAVES>(a, z, s, shared);
-  const double2* sums = a.sums + (size_t)s * a.chunks;
+  Left w = left_from<WAVES>(a, z, s, first, shared);
   // chunk c's sum; with only_p of p alone, where p is nowhere above q
   const bool drafted = w.qs != 0.0, certain = w.odd >= 0;
   bool only_p = false;
   auto chunk_sum = [&](int c) {
-    if (only_p) return certain ? sums[c].x + sums[c].y : sums[c].x;
-    return drafted ? a.left[(size_t)s * a.chunks + c] : sums[c].x;
+    if (drafted && !only_p) return c == tid ? first_left : a.left[(size_t)s * a.chunks + c];
+    const double2 x = c == tid ? first : sums[c];
+    return only_p && certain ? x.x + x.y : x.x;
   };
   auto total_of = [&] {
     double sum = 0.0;
@@ -477,7 +537,7 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
     w.qs = 0.0;
     total = total_of();
   }
-  const double aim = (double)a.sample_u[s] * total;
+  const double aim = (double)u * total;
   // the first chunk that ends past the aim, or behind them all, by rounding, the last with any weight
   double before = 0.0;
   bool past = false;
@@ -506,11 +566,7 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
     each[e] = left_of(w, logit(x[e]), logit(y[e]), 8 * v - r.lead + e);
     own = own + each[e];
   }
-  double upto = own;
-  for (int d = 1; d < 64; d *= 2) {
-    const double o = __shfl_up(upto, d);
-    if (lane >= d) upto = upto + o;
-  }
+  const double upto = wave_prefix(own);
   if (lane == 63) shared[tid >> 6] = upto;
   __syncthreads();
   double c = chosen_base + (upto - own);
