@@ -581,8 +581,13 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
       if (c > aim && token == 0x7FFFFFFF) token = last;
     }
   }
-  if (token != 0x7FFFFFFF) atomicMin(&first_past, token);
-  if (last >= 0) atomicMax(&last_any, last);
+  // one lane of a wave: all 1024 threads at one address take 6 us
+  token = wave_min(token);
+  last = -wave_min(-last);
+  if (lane == 0) {
+    atomicMin(&first_past, token);
+    atomicMax(&last_any, last);
+  }
   __syncthreads();
   if (tid == 0) a.tokens[z.row] = first_past != 0x7FFFFFFF ? first_past : last_any;
 }
