@@ -414,12 +414,14 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 #pragma unroll
             for (int t = 0; t < QT; ++t) {
               if (edge) {
-                asm volatile("" ::: "memory");  // a branch, not selects in every step
+                const int left = see[t] - key0;
 #pragma unroll
-                for (int p = 0; p < PG; ++p)
+                for (int p = 0; p < PG; ++p) {
 #pragma unroll
                   for (int i = 0; i < 4; ++i)
-                    if (key0 + 16 * p + i >= see[t]) sc[t][p][i] = -INFINITY;
+                    if (16 * p + i >= left) sc[t][p][i] = -INFINITY;
+                  asm volatile("" : "+v"(sc[t][p]));  // here: a branch, not selects in every step
+                }
               }
               float top = -INFINITY;
 #pragma unroll
@@ -438,10 +440,12 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
               }
               float scale = to_log2;
               if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ref) >= kLargeScore)) {
-                asm volatile("" ::: "memory");
                 scale = 1.0f;
 #pragma unroll
-                for (int p = 0; p < PG; ++p) sc[t][p] = sc[t][p] * to_log2;
+                for (int p = 0; p < PG; ++p) {
+                  sc[t][p] = sc[t][p] * to_log2;
+                  asm volatile("" : "+v"(sc[t][p]));
+                }
               }
 #pragma unroll
               for (int p = 0; p < PG; ++p)
@@ -456,7 +460,6 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                 }
             }
             if (edge) {
-              asm volatile("" ::: "memory");
               // What no row sees is stale: zero. A NaN of a position that only some rows see would
               // reach the others through their zero weights: it is taken out and handed to its rows.
               uint32_t odd = 0;
@@ -842,13 +845,14 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
                   as_h8(k_lds[buf][32 * t + n][2 * u + half]), qf[u], sc[t], 0, 0, 0);
           }
           if ((st + 1) * STEP > wave_min) {  // some row does not see all of it
-            asm volatile("" ::: "memory");  // a branch, not selects in every step
-            const int key0 = st * STEP + 4 * half;
+            const int left = see - st * STEP - 4 * half;
 #pragma unroll
-            for (int t = 0; t < KT; ++t)
+            for (int t = 0; t < KT; ++t) {
 #pragma unroll
               for (int i = 0; i < 16; ++i)
-                if (key0 + 32 * t + 8 * (i / 4) + i % 4 >= see) sc[t][i] = -INFINITY;
+                if (32 * t + 8 * (i / 4) + i % 4 >= left) sc[t][i] = -INFINITY;
+              asm volatile("" : "+v"(sc[t]));  // here: a branch, not selects in every step
+            }
           }
           float top = sc[0][0];
 #pragma unroll
@@ -869,12 +873,13 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
           }
           float scale = to_log2;
           if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ref) >= kLargeScore)) {
-            asm volatile("" ::: "memory");
             scale = 1.0f;
 #pragma unroll
-            for (int t = 0; t < KT; ++t)
+            for (int t = 0; t < KT; ++t) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) sc[t][i] = sc[t][i] * to_log2;
+              asm volatile("" : "+v"(sc[t]));
+            }
           }
 #pragma unroll
           for (int cc = 0; cc < 2 * KT; ++cc) {  // 16 positions
