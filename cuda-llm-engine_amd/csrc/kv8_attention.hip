@@ -21,6 +21,9 @@ constexpr float kLog2e = 1.44269504088896341f;
 // Below it a rounded maximum (in log2 units) is less than 2^6 short of the exact one, which neither
 // weights nor sums mind; from there on exponents are made in two steps, and the largest weight is 1.
 constexpr float kLargeScore = 1073741824.0f;
+// A row's weights are relative to a maximum that gives way only to one larger by more than this (in
+// log2 units): they reach 2^kSlack, and sums are seldom rescaled.
+constexpr float kSlack = 8.0f;
 constexpr int kStart = 2;                       // what a unit's first loads cost, in steps
 constexpr int kFewColumns = 32, kManyColumns = 128;
 // Workers of a launch, waves and blocks: what fits the 256 CUs at once.
@@ -215,6 +218,13 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a) {
   r.seq = __builtin_amdgcn_readfirstlane(seq_[WAVES ? wave : 0]);
   r.at = same(at_[WAVES ? wave : 0]);
   return r;
+}
+
+// x, or -inf where bit i is set: without a comparison's scalar registers, which a step has none to spare
+// of.
+__device__ __forceinline__ float hide(float x, uint32_t bits, int i) {
+  const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
+  return __builtin_bit_cast(float, (m & 0xFF800000u) | (~m & __builtin_bit_cast(uint32_t, x)));
 }
 
 // The larger of x and what the lane 16 (32) away has.
@@ -429,7 +439,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 #pragma unroll
                 for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, sc[t][p][i]);
               top = max_of_quarters(top) * to_log2;
-              const float next = __builtin_fmaxf(m[t], top);
+              const float next = top > m[t] + kSlack ? top : m[t];
               const float ref = next == -INFINITY ? 0.0f : next;
               if (__builtin_amdgcn_ballot_w64(next != m[t])) {
                 const float corr = __builtin_amdgcn_exp2f(m[t] - ref);
@@ -845,12 +855,14 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
                   as_h8(k_lds[buf][32 * t + n][2 * u + half]), qf[u], sc[t], 0, 0, 0);
           }
           if ((st + 1) * STEP > wave_min) {  // some row does not see all of it
-            const int left = see - st * STEP - 4 * half;
 #pragma unroll
             for (int t = 0; t < KT; ++t) {
+              // of 8 positions in a row a lane has 4: the number of those that its row sees
+              int left = see - (st * STEP + 32 * t + 4 * half);
+              left = left < 0 ? 0 : left > 32 ? 32 : left;
+              const uint32_t beyond = 0xFFFFu << (4 * (left / 8) + (left % 8 < 4 ? left % 8 : 4));
 #pragma unroll
-              for (int i = 0; i < 16; ++i)
-                if (32 * t + 8 * (i / 4) + i % 4 >= left) sc[t][i] = -INFINITY;
+              for (int i = 0; i < 16; ++i) sc[t][i] = hide(sc[t][i], beyond, i);
               asm volatile("" : "+v"(sc[t]));  // here: a branch, not selects in every step
             }
           }
@@ -860,7 +872,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
 #pragma unroll
             for (int i = 0; i < 16; ++i) top = __builtin_fmaxf(top, sc[t][i]);
           top = max_across(top, true) * to_log2;
-          const float next = __builtin_fmaxf(m, top);
+          const float next = top > m + kSlack ? top : m;
           const float ref = next == -INFINITY ? 0.0f : next;
           if (__builtin_amdgcn_ballot_w64(next != m)) {
             const float corr = __builtin_amdgcn_exp2f(m - ref);
