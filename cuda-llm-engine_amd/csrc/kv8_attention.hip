@@ -40,13 +40,31 @@ __device__ __forceinline__ uint32_t bf16_from_e4m3(uint32_t bytes, float scale) 
                             __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(bytes, scale, HIGH));
 }
 
-// Two weights as packed bf16, their first 8 bits (cut off) and the rest rounded to 8.
-__device__ __forceinline__ void split(float a, float b, uint32_t& hi, uint32_t& lo) {
+// Two weights as packed bf16: their first 8 bits, and what that leaves rounded to 8 more, so that a
+// weight keeps 16 bits or nearly so at any size. In one way the first are cut off.
+__device__ __forceinline__ void split_cut(float a, float b, uint32_t& hi, uint32_t& lo) {
   const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
   hi = __builtin_amdgcn_perm(y, x, 0x07060302);
   const float ra = a - __builtin_bit_cast(float, x & 0xFFFF0000u);
   const float rb = b - __builtin_bit_cast(float, y & 0xFFFF0000u);
   const bf16x2 r = {(__bf16)ra, (__bf16)rb};
+  lo = __builtin_bit_cast(uint32_t, r);
+}
+// In the other they are rounded, and what is left is a product of the packed halves with (-1, 0) or
+// (0, -1) added to the weight: exact, and 4 instructions where the first way takes 6. Units of few
+// columns gain by it (48 sequences of up to 5 rows: 36.2 -> 35.3 us); those of many, whose matrix
+// instructions run beside it, lose (1507 rows: 84.6 -> 86.2 us).
+__device__ __forceinline__ void split_rounded(float a, float b, uint32_t& hi, uint32_t& lo) {
+  const bf16x2 h = {(__bf16)a, (__bf16)b};
+  // from registers: as an operand in the instruction, -1 in the low half is taken for the high one
+  uint32_t first = 0x0000BF80u, second = 0xBF800000u;
+  asm("" : "+s"(first), "+s"(second));
+  const float ra =
+      __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, first), a, false);
+  const float rb =
+      __builtin_amdgcn_fdot2_f32_bf16(h, __builtin_bit_cast(bf16x2, second), b, false);
+  const bf16x2 r = {(__bf16)ra, (__bf16)rb};
+  hi = __builtin_bit_cast(uint32_t, h);
   lo = __builtin_bit_cast(uint32_t, r);
 }
 
@@ -466,7 +484,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                   const float w1 =
                       __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][p][i + 1], scale, -ref));
                   l[t] = l[t] + (w0 + w1);
-                  split(w0, w1, ph[t][p][i / 2], pl[t][p][i / 2]);
+                  split_rounded(w0, w1, ph[t][p][i / 2], pl[t][p][i / 2]);
                 }
             }
             if (edge) {
@@ -904,7 +922,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
               const float w1 =
                   __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc / 2][i + 1], scale, -ref));
               l = l + (w0 + w1);
-              split(w0, w1, ph[e], pl[e]);
+              split_cut(w0, w1, ph[e], pl[e]);
             }
             const bf16x8 hi = __builtin_bit_cast(bf16x8, (u32x4{ph[0], ph[1], ph[2], ph[3]}));
             const bf16x8 lo = __builtin_bit_cast(bf16x8, (u32x4{pl[0], pl[1], pl[2], pl[3]}));
