@@ -25,12 +25,17 @@ constexpr float kLargeScore = 1073741824.0f;
 // log2 units): they reach 2^kSlack, and sums are seldom rescaled.
 constexpr float kSlack = 8.0f;
 constexpr int kStart = 2;                       // what a unit's first loads cost, in steps
-constexpr int kFewColumns = 32, kManyColumns = 128;
+constexpr int kFewColumns = 32;
+// From here on blocks of 8 waves and 256 columns: 1507 rows at 64 dims 74.0 -> 69.5 us, 500 rows at 128
+// dims 60.0 -> 53.8, 5 x 500 rows at 8000 positions 234 -> 206. Below, tiles of 128 columns leave fewer
+// waves without work (32 query heads on 8, us, both at 2000 positions: 250 rows 27.9 and 29.3, 100 rows
+// 21.7 and 25.4, 20 x up to 100 rows 46.0 and 54.2).
+constexpr int kWideColumns = 1024;
 // Workers of a launch, waves and blocks: what fits the 256 CUs at once.
 template <int HD, int QT>
 constexpr int kFewWorkers = QT == 1 ? 2048 : 1024;
-template <int HD>
-constexpr int kManyWorkers = 512;
+template <int W>
+constexpr int kManyWorkers = 2048 / W;
 constexpr int kWorkers = 2048, kMostKvHeads = 512;  // at most
 constexpr int kSlotColumns = 131072;            // of partial results in the workspace
 
@@ -122,28 +127,21 @@ __device__ __forceinline__ int seen(const AttentionArgs& a, const Seq& q, int co
   const long long m = n < q.limit ? n : q.limit;
   return m < 0 ? 0 : (int)m;
 }
-// A step: 4 KiB of K and as much of V.
-template <int HD>
-constexpr int kPages = 256 / HD;
-template <int HD>
-constexpr int kStep = kPages<HD> * kPage;
+// A step of units of C columns: 16 bytes of K and as many of V for each of a block's threads, or, of
+// the 64 of a wave, for each of 4 times.
+template <int HD, int C>
+constexpr int kPages = (C > 128 ? 512 : 256) / HD;
+template <int HD, int C>
+constexpr int kStep = kPages<HD, C> * kPage;
 
 // Steps of a tile: those of its last row; one for a tile that sees nothing, which writes zeros. A
 // unit's share of the work is counted in ticks, its steps and kStart for its beginning.
 template <int HD, int C>
 __device__ __forceinline__ int tile_steps(const AttentionArgs& a, const Seq& q, int tile) {
   const int last = (tile + 1) * C < q.columns ? (tile + 1) * C - 1 : q.columns - 1;
-  const int n = (seen(a, q, last) + kStep<HD> - 1) / kStep<HD>;
+  const int n = (seen(a, q, last) + kStep<HD, C> - 1) / kStep<HD, C>;
   return n > 0 ? n : 1;
 }
-template <int HD, int C>
-__device__ __forceinline__ long long seq_ticks(const AttentionArgs& a, int s) {
-  const Seq q = seq_of(a, s);
-  long long n = 0;
-  for (int t = 0; t * C < q.columns; ++t) n += kStart + tile_steps<HD, C>(a, q, t);
-  return n;
-}
-
 // Values that are the same in every lane, as scalars.
 __device__ __forceinline__ int same(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ long long same(long long x) {
@@ -166,9 +164,9 @@ __device__ __forceinline__ Seq same(Seq q) {
 // same time (256 sequences: a worker with one head's units behind the other's, 63.1 us).
 // Worker t n_kv_heads + h is head h's of team t; workers are waves or blocks. By all 256 threads.
 struct Share {
-  int team, head;
-  int seq;               // that holds the beginning of the team's share, and
-  long long at;          // its place in it
+  int team, head, teams;
+  int seq, tile;         // that hold the beginning of the team's share, and
+  int at;                // its place in them, in ticks
   long long begin, end;  // among the ticks of a head
   long long each;        // of the first `more` teams one more
   int more;
@@ -182,17 +180,29 @@ struct Share {
   static __device__ __forceinline__ long long divide(long long a, long long b) {  // b > 0 where used
     return (uint64_t)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
   }
+  // all but the place of the beginning
+  static __device__ __forceinline__ Share of(const AttentionArgs& a, long long total, int worker) {
+    Share r = {};
+    r.teams = a.workers / a.n_kv_heads;
+    if (total < r.teams) r.teams = total > 0 ? (int)total : 1;
+    r.each = divide(total, r.teams);
+    r.more = (int)(total - r.each * r.teams);
+    r.team = worker / a.n_kv_heads;
+    r.head = worker % a.n_kv_heads;
+    r.begin = r.team < r.teams ? r.begin_of(r.team) : total;
+    r.end = r.team < r.teams ? r.begin_of(r.team + 1) : total;
+    return r;
+  }
 };
-template <int HD, int C, bool WAVES>
-__device__ __forceinline__ Share find_share(const AttentionArgs& a) {
-  __shared__ long long wave_sum_[4], at_[4];
-  __shared__ int seq_[4];
-  const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int n = a.batch.n_seqs, per = (n + 255) / 256;
-  const int s0 = tid * per, s1 = s0 + per < n ? s0 + per : n;
-  long long mine = 0;
-  for (int s = s0; s < s1; ++s) mine += seq_ticks<HD, C>(a, s);
+
+// A thread's place in a sum over the block's W waves: what those in front of it have, and all.
+struct Place {
+  long long before, total;
+};
+template <int W>
+__device__ __forceinline__ Place place_of(long long mine) {
+  __shared__ long long wave_sum_[W];
+  const int lane = threadIdx.x & 63, wave = same((int)threadIdx.x >> 6);
   long long upto = mine;
   for (int d = 1; d < 64; d *= 2) {
     const long long o = __shfl_up(upto, d);
@@ -200,41 +210,123 @@ __device__ __forceinline__ Share find_share(const AttentionArgs& a) {
   }
   if (lane == 63) wave_sum_[wave] = upto;
   __syncthreads();
-  Share r;
-  long long base = 0, total = 0;
-  for (int w = 0; w < 4; ++w) {
-    if (w < wave) base += wave_sum_[w];
-    total += wave_sum_[w];
+  Place r = {upto - mine, 0};
+  for (int w = 0; w < W; ++w) {
+    if (w < wave) r.before += wave_sum_[w];
+    r.total += wave_sum_[w];
   }
-  total = same(total);
-  const int first = WAVES ? 4 * blockIdx.x : blockIdx.x, worker = WAVES ? first + wave : first;
-  int teams = a.workers / a.n_kv_heads;
-  if (total < teams) teams = total > 0 ? (int)total : 1;
-  r.each = Share::divide(total, teams);
-  r.more = (int)(total - r.each * teams);
-  r.team = worker / a.n_kv_heads;
-  r.head = worker % a.n_kv_heads;
-  const long long from = base + upto - mine;
-  for (int w = 0; w < (WAVES ? 4 : 1); ++w) {
+  r.total = same(r.total);
+  return r;
+}
+
+// Tiles of a sequence: none where it has no rows here.
+template <int C>
+__device__ __forceinline__ int tiles_of(const AttentionArgs& a, int s) {
+  return (seq_of(a, s).columns + C - 1) / C;
+}
+
+// The beginnings of the shares of a block's WORKERS workers (4 waves, or the block): a thread sums the
+// ticks of a run of tiles, and the one whose run holds the beginning finds its place. Sequences of few
+// tiles are dealt out to the threads.
+template <int HD, int C, int WORKERS>
+__device__ __forceinline__ Share find_share_by_sequence(const AttentionArgs& a) {
+  __shared__ int seq_[WORKERS], at_[WORKERS];
+  const int tid = threadIdx.x, n = a.batch.n_seqs, per = (n + 255) / 256;
+  const int first = WORKERS * (int)blockIdx.x, own = WORKERS > 1 ? same(tid >> 6) : 0;
+  const int s0 = tid * per, s1 = s0 + per < n ? s0 + per : n;
+  auto ticks_of = [&](int s) {
+    const Seq q = seq_of(a, s);
+    long long n = 0;
+    for (int t = 0; t * C < q.columns; ++t) n += kStart + tile_steps<HD, C>(a, q, t);
+    return n;
+  };
+  long long mine = 0;
+  for (int s = s0; s < s1; ++s) mine += ticks_of(s);
+  const Place p = place_of<4>(mine);
+  Share r = Share::of(a, p.total, first + own);
+  for (int w = 0; w < WORKERS; ++w) {
     const int team = (first + w) / a.n_kv_heads;
-    const long long x = r.begin_of(team);
-    if (team < teams && x >= from && x < from + mine) {
-      long long left = x - from;
+    long long left = r.begin_of(team) - p.before;
+    if (team < r.teams && left >= 0 && left < mine) {
       int s = s0;
       for (; s < s1 - 1; ++s) {
-        const long long c = seq_ticks<HD, C>(a, s);
-        if (left < c) break;
-        left -= c;
+        const long long ticks = ticks_of(s);
+        if (left < ticks) break;
+        left -= ticks;
       }
       seq_[w] = s;
-      at_[w] = left;
+      at_[w] = (int)left;
     }
   }
   __syncthreads();
-  r.begin = r.team < teams ? r.begin_of(r.team) : total;
-  r.end = r.team < teams ? r.begin_of(r.team + 1) : total;
-  r.seq = __builtin_amdgcn_readfirstlane(seq_[WAVES ? wave : 0]);
-  r.at = same(at_[WAVES ? wave : 0]);
+  r.seq = same(seq_[own]);
+  r.at = same(at_[own]);
+  r.tile = 0;
+  if (r.begin < r.end) {
+    const Seq q = same(seq_of(a, r.seq));
+    for (;; ++r.tile) {
+      const int ticks = kStart + same(tile_steps<HD, C>(a, q, r.tile));
+      if (r.at < ticks) break;
+      r.at -= ticks;
+    }
+  }
+  return r;
+}
+
+// Of those that have many each thread takes an equal part, whose beginning is looked up among the
+// threads' sums of tiles (by sequence, where there is one of 1507 rows: 12.3 us, and 4.2 so).
+template <int HD, int C, int W>
+__device__ __forceinline__ Share find_share_by_tile(const AttentionArgs& a) {
+  constexpr int T = 64 * W;
+  __shared__ int upto_[T], found_[3];
+  const int tid = threadIdx.x, n = a.batch.n_seqs, per = (n + T - 1) / T;
+  int s0 = tid * per < n ? tid * per : n;
+  int tiles_here = 0;
+  for (int s = s0; s < s0 + per && s < n; ++s) tiles_here += (seq_of(a, s).columns + C - 1) / C;
+  const Place q = place_of<W>(tiles_here);
+  upto_[tid] = (int)q.before + tiles_here;
+  __syncthreads();
+  const int all = (int)q.total, each = all / T, more = all % T;
+  const int tiles = each + (tid < more ? 1 : 0);
+  int tile0 = each * tid + (tid < more ? tid : more);
+  int lo = 0;  // the thread whose sequences have tile0
+  for (int d = T / 2; d > 0; d /= 2)
+    if (upto_[lo + d - 1] <= tile0) lo += d;
+  if (lo > 0) tile0 -= upto_[lo - 1];
+  s0 = lo * per;
+  // each tile of the run in turn, until `what` says that it is enough
+  auto run = [&](auto what) {
+    int left = tiles, t = tile0;
+    for (int s = s0; s < n && left > 0; ++s) {
+      const Seq q = seq_of(a, s);
+      for (; t * C < q.columns && left > 0; ++t, --left)
+        if (what(s, t, kStart + tile_steps<HD, C>(a, q, t))) return;
+      t -= (q.columns + C - 1) / C;
+    }
+  };
+  long long mine = 0;
+  run([&](int, int, int ticks) {
+    mine += ticks;
+    return false;
+  });
+  const Place p = place_of<W>(mine);
+  Share r = Share::of(a, p.total, blockIdx.x);
+  long long left = r.begin - p.before;
+  if (r.begin < r.end && left >= 0 && left < mine)
+    run([&](int s, int t, int ticks) {
+      if (left >= ticks) {
+        left -= ticks;
+        return false;
+      }
+      found_[0] = s;
+      found_[1] = t;
+      found_[2] = (int)left;
+      return true;
+    });
+  __syncthreads();
+  r.seq = same(found_[0]);
+  r.tile = same(found_[1]);
+  r.at = same(found_[2]);
   return r;
 }
 
@@ -268,12 +360,12 @@ __device__ __forceinline__ float max_of_quarters(float x) {
 // Weights enter as two bf16, high and low half: 16 significant bits at any exponent.
 template <int HD, int QT>
 __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArgs a) {
-  constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64, PG = kPages<HD>, STEP = kStep<HD>;
+  constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64, PG = kPages<HD, C>, STEP = kStep<HD, C>;
   const int lane = threadIdx.x & 63, n = lane & 15, qd = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int worker = 4 * (int)blockIdx.x + wave;
   const bool shared_units = a.parts != nullptr;
-  const Share sh = find_share<HD, C, true>(a);
+  const Share sh = find_share_by_sequence<HD, C, 4>(a);
   const int h = sh.head;
   auto note = [&](int side, int first, int last, int column, int columns, int seq) {
     Shared o = {};
@@ -291,17 +383,9 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 
   long long pos = sh.begin;
   if (pos < sh.end) {
-    int s = sh.seq, tile = 0;
+    int s = sh.seq, tile = sh.tile, tick = sh.at;
     Seq q = same(seq_of(a, s));
-    long long at = sh.at;
-    int steps;
-    for (;;) {
-      steps = same(tile_steps<HD, C>(a, q, tile));
-      if (at < kStart + steps) break;
-      at -= kStart + steps;
-      ++tile;
-    }
-    int tick = same((int)at);
+    int steps = same(tile_steps<HD, C>(a, q, tile));
     const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
     int ids = 0, ids_of = -1, window = -1;  // 64 entries of a sequence's table, one to a lane
 
@@ -715,9 +799,9 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
 //   O^T += V^T P^T (.._bf16; A: 32 dims of V, B: the lane's own weights)
 // Lane l gets of S^T column l % 32, positions 8 (i / 4) + 4 (l / 32) + i % 4; V's positions lie in LDS
 // in the order in which that makes 8 of them a lane's share of a contraction.
-template <int HD>
-__global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionArgs a) {
-  constexpr int C = kManyColumns, PG = kPages<HD>, STEP = kStep<HD>, KT = STEP / 32, DT = HD / 32;
+template <int HD, int W>
+__global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const AttentionArgs a) {
+  constexpr int C = 32 * W, PG = kPages<HD, C>, STEP = kStep<HD, C>, KT = STEP / 32, DT = HD / 32;
   constexpr int KP = HD / 16, VP = HD / 4;  // threads to a position of K, to 4 positions of V
   // One piece of 16 bytes behind each row: 8 lanes that read a piece of as many rows meet no bank
   // twice, and every address is a lane's base and a constant.
@@ -729,7 +813,11 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
   const bool shared_units = a.parts != nullptr;
   int turn = 0;
   if (tid < 2) odd[tid] = 0;
-  const Share sh = find_share<HD, C, false>(a);
+  Share sh;
+  if constexpr (W == 4)
+    sh = find_share_by_sequence<HD, C, 1>(a);
+  else
+    sh = find_share_by_tile<HD, C, W>(a);
   const int h = sh.head;
   auto note = [&](int side, int first, int last, int column, int columns, int seq) {
     Shared o = {};
@@ -746,17 +834,9 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
   }
   long long pos = sh.begin;
   if (pos >= sh.end) return;
-  int s = sh.seq, tile = 0;
+  int s = sh.seq, tile = sh.tile, tick = sh.at;
   Seq q = same(seq_of(a, s));
-  long long at = sh.at;
-  int steps;
-  for (;;) {
-    steps = same(tile_steps<HD, C>(a, q, tile));
-    if (at < kStart + steps) break;
-    at -= kStart + steps;
-    ++tile;
-  }
-  int tick = same((int)at);
+  int steps = same(tile_steps<HD, C>(a, q, tile));
   const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
 
   while (pos < sh.end) {
@@ -810,7 +890,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_many(const AttentionAr
             ksc = a.k_scale[b];
             vsc = a.v_scale[b];
           }
-          const int i = (PG * st + wave * PG / 4) & 63;  // the page of this wave's quarter
+          const int i = (PG * st + wave * PG / W) & 63;  // the page of this wave's part
           const size_t block = ((size_t)__builtin_amdgcn_readlane(ids, i) * a.n_kv_heads + h) *
                                (size_t)(kPage * HD);
           kr = ld16(a.k_pool + block + (uint32_t)(k_key % kPage * HD + 16 * k_part));
@@ -1032,11 +1112,12 @@ int few_launch(AttentionArgs a, hipStream_t stream) {
   return st != LLMK_OK ? st : join_launch<HD>(a, 16 * QT, stream);
 }
 
-template <int HD>
+template <int HD, int W>
 int many_launch(AttentionArgs a, hipStream_t stream) {
-  a.workers = kManyWorkers<HD>;
-  const int st = launch(k_kv8_attention_many<HD>, dim3(a.workers), dim3(256), 0, stream, a);
-  return st != LLMK_OK ? st : join_launch<HD>(a, kManyColumns, stream);
+  a.workers = kManyWorkers<W>;
+  const int st =
+      launch(k_kv8_attention_many<HD, W>, dim3(a.workers), dim3(64 * W), 0, stream, a);
+  return st != LLMK_OK ? st : join_launch<HD>(a, 32 * W, stream);
 }
 
 // Sequences of up to kFewColumns columns go by waves, longer ones by blocks. One launch serves all
@@ -1054,7 +1135,8 @@ int attention_launch(AttentionArgs a, int max_rows, hipStream_t stream) {
     a.most_columns = 0x7FFFFFFF;
     a.least_columns = kFewColumns + 1;
   }
-  return many_launch<HD>(a, stream);
+  return columns <= kWideColumns || a.n_kv_heads > kManyWorkers<8> ? many_launch<HD, 4>(a, stream)
+                                                                   : many_launch<HD, 8>(a, stream);
 }
 
 }  // namespace
