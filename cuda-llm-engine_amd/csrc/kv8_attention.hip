@@ -942,15 +942,32 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
           }
         };
         auto compute = [&](int st, int buf) {
+          // 4 pieces of K are on their way while 4 are multiplied: the compiler, left to itself, waits for
+          // each (ATIME)
+          constexpr int G = 4, GROUPS = KT * (HD / 16) / G;
           f32x16 sc[KT];
+          u32x4 kf[2][G];
+          auto fetch = [&](int g) {
 #pragma unroll
-          for (int t = 0; t < KT; ++t) {
+            for (int j = 0; j < G; ++j) {
+              const int u = (G * g + j) / KT, t = (G * g + j) % KT;
+              kf[g & 1][j] = k_lds[buf][32 * t + n][2 * u + half];
+            }
+          };
+#pragma unroll
+          for (int t = 0; t < KT; ++t)
 #pragma unroll
             for (int i = 0; i < 16; ++i) sc[t][i] = 0.0f;
+          fetch(0);
 #pragma unroll
-            for (int u = 0; u < HD / 16; ++u)
-              sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                  as_h8(k_lds[buf][32 * t + n][2 * u + half]), qf[u], sc[t], 0, 0, 0);
+          for (int g = 0; g < GROUPS; ++g) {
+            if (g + 1 < GROUPS) fetch(g + 1);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+              const int u = (G * g + j) / KT, t = (G * g + j) % KT;
+              sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[g & 1][j]), qf[u], sc[t], 0, 0, 0);
+            }
           }
           if ((st + 1) * STEP > wave_min) {  // some row does not see all of it
 #pragma unroll
