@@ -162,3 +162,60 @@ inline void argmax_rows(const __half* logits, int* out, int n_rows, int vocab,
   llmk_shim::check(llmk_argmax_rows(llmk_shim::h(logits), out, n_rows, vocab, stream),
                    "argmax_rows");
 }
+
+// Serving from an 8-bit KV cache (new entry points, documented in llmk.h): pools and scales as there,
+// a violated precondition is a fatal host error.
+inline void kv8_append(const __half* qkv, int ld, __half* q_out, uint8_t* k_pool, float* k_scale,
+                       uint8_t* v_pool, float* v_scale, const int* block_tables,
+                       const int* row_starts, const int* seq_lens, const float* inv_freq, int n_rows,
+                       int n_seqs, int max_pages, int page_size, int n_heads, int n_kv_heads,
+                       int head_dim, hipStream_t stream = 0) {
+  llmk_shim::check(
+      llmk_kv8_append(llmk_shim::h(qkv), ld, llmk_shim::h(q_out), k_pool, k_scale, v_pool, v_scale,
+                      block_tables, row_starts, seq_lens, inv_freq, n_rows, n_seqs, max_pages,
+                      page_size, n_heads, n_kv_heads, head_dim, stream),
+      "kv8_append");
+}
+
+inline void kv8_gather(const uint8_t* k_pool, const float* k_scale, const uint8_t* v_pool,
+                       const float* v_scale, const int* block_tables, const int* row_starts,
+                       const int* seq_lens, __half* k_out, __half* v_out, int n_rows, int n_seqs,
+                       int max_pages, int page_size, int n_kv_heads, int head_dim,
+                       hipStream_t stream = 0) {
+  llmk_shim::check(
+      llmk_kv8_gather(k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, seq_lens,
+                      llmk_shim::h(k_out), llmk_shim::h(v_out), n_rows, n_seqs, max_pages, page_size,
+                      n_kv_heads, head_dim, stream),
+      "kv8_gather");
+}
+
+inline size_t kv8_attention_workspace_floats(int head_dim) {
+  return llmk_kv8_attention_workspace_floats(head_dim);
+}
+
+inline void kv8_attention(const __half* q, const uint8_t* k_pool, const float* k_scale,
+                          const uint8_t* v_pool, const float* v_scale, const int* block_tables,
+                          const int* row_starts, const int* seq_lens, __half* out, float* workspace,
+                          int n_rows, int n_seqs, int max_rows, int max_pages, int page_size,
+                          int n_heads, int n_kv_heads, int head_dim, hipStream_t stream = 0) {
+  llmk_shim::check(
+      llmk_kv8_attention(llmk_shim::h(q), k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
+                         seq_lens, llmk_shim::h(out), workspace, n_rows, n_seqs, max_rows, max_pages,
+                         page_size, n_heads, n_kv_heads, head_dim, stream),
+      "kv8_attention");
+}
+
+inline size_t verify_drafts_workspace_floats(int n_rows, int n_seqs, int vocab) {
+  return llmk_verify_drafts_workspace_floats(n_rows, n_seqs, vocab);
+}
+
+inline void verify_drafts(const __half* logits, const __half* draft_logits, const int* drafts,
+                          const int* row_starts, const float* temperature, const float* accept_u,
+                          const float* sample_u, int* n_accepted, int* tokens, float* workspace,
+                          int n_rows, int n_seqs, int vocab, hipStream_t stream = 0) {
+  llmk_shim::check(
+      llmk_verify_drafts(llmk_shim::h(logits), llmk_shim::h(draft_logits), drafts, row_starts,
+                         temperature, accept_u, sample_u, n_accepted, tokens, workspace, n_rows,
+                         n_seqs, vocab, stream),
+      "verify_drafts");
+}
