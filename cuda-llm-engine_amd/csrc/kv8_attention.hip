@@ -24,20 +24,24 @@ constexpr float kLargeScore = 1073741824.0f;
 // A row's weights are relative to a maximum that gives way only to one larger by more than this (in
 // log2 units): they reach 2^kSlack, and sums are seldom rescaled.
 constexpr float kSlack = 8.0f;
-constexpr int kStart = 2;                       // what a unit's first loads cost, in steps
-constexpr int kFewColumns = 32;
+// What a unit's beginning costs, in steps. With 0 / 1 / 2 / 4, us: 48 sequences of up to 5 rows 41.1 /
+// 37.5 / 35.8 / 36.1, 1507 rows of one 68.2 / 68.5 / 67.5 / 72.0.
+constexpr int kStart = 2;
+// Sequences of up to this many columns go by waves, in tiles of 32; us by waves and by blocks: 48 x 16
+// rows (64 columns) 58.5 and 67.5, 4 x 16 19.9 and 23.4, 48 x 24 rows (96 columns) 82.7 and 74.0.
+constexpr int kFewColumns = 64;
 // From here on blocks of 8 waves and 256 columns: 1507 rows at 64 dims 74.0 -> 69.5 us, 500 rows at 128
 // dims 60.0 -> 53.8, 5 x 500 rows at 8000 positions 234 -> 206. Below, tiles of 128 columns leave fewer
 // waves without work (32 query heads on 8, us, both at 2000 positions: 250 rows 27.9 and 29.3, 100 rows
 // 21.7 and 25.4, 20 x up to 100 rows 46.0 and 54.2).
 constexpr int kWideColumns = 1024;
-// Workers of a launch, waves and blocks: what fits the 256 CUs at once.
-template <int HD, int QT>
-constexpr int kFewWorkers = QT == 1 ? 2048 : 1024;
+// Workers of a launch: a wave for each SIMD (256 sequences, us: 512 waves 92.1, 768 69.7, 1024 59.9, 1280
+// 77.0, 2048 62.0 with twice the parts to join), or as many blocks as give it two.
+constexpr int kFewWorkers = 1024;
 template <int W>
 constexpr int kManyWorkers = 2048 / W;
-constexpr int kWorkers = 2048, kMostKvHeads = 512;  // at most
-constexpr int kSlotColumns = 131072;            // of partial results in the workspace
+constexpr int kWorkers = 1024, kMostKvHeads = 512;  // at most
+constexpr int kSlotColumns = 131072;                // of partial results in the workspace
 
 template <bool HIGH>
 __device__ __forceinline__ uint32_t bf16_from_e4m3(uint32_t bytes, float scale) {
@@ -230,7 +234,8 @@ __device__ __forceinline__ int tiles_of(const AttentionArgs& a, int s) {
 // tiles are dealt out to the threads.
 template <int HD, int C, int WORKERS>
 __device__ __forceinline__ Share find_share_by_sequence(const AttentionArgs& a) {
-  __shared__ int seq_[WORKERS], at_[WORKERS];
+  __shared__ int seq_[WORKERS];
+  __shared__ long long at_[WORKERS];
   const int tid = threadIdx.x, n = a.batch.n_seqs, per = (n + 255) / 256;
   const int first = WORKERS * (int)blockIdx.x, own = WORKERS > 1 ? same(tid >> 6) : 0;
   const int s0 = tid * per, s1 = s0 + per < n ? s0 + per : n;
@@ -255,21 +260,22 @@ __device__ __forceinline__ Share find_share_by_sequence(const AttentionArgs& a) 
         left -= ticks;
       }
       seq_[w] = s;
-      at_[w] = (int)left;
+      at_[w] = left;
     }
   }
   __syncthreads();
   r.seq = same(seq_[own]);
-  r.at = same(at_[own]);
+  long long at = same(at_[own]);
   r.tile = 0;
   if (r.begin < r.end) {
     const Seq q = same(seq_of(a, r.seq));
     for (;; ++r.tile) {
       const int ticks = kStart + same(tile_steps<HD, C>(a, q, r.tile));
-      if (r.at < ticks) break;
-      r.at -= ticks;
+      if (at < ticks) break;
+      at -= ticks;
     }
   }
+  r.at = (int)at;
   return r;
 }
 
@@ -1123,7 +1129,7 @@ int join_launch(const AttentionArgs& a, int columns, hipStream_t stream) {
 
 template <int HD, int QT>
 int few_launch(AttentionArgs a, hipStream_t stream) {
-  a.workers = kFewWorkers<HD, QT>;
+  a.workers = kFewWorkers;
   const int st =
       launch(k_kv8_attention_few<HD, QT>, dim3(a.workers / 4), dim3(256), 0, stream, a);
   return st != LLMK_OK ? st : join_launch<HD>(a, 16 * QT, stream);
