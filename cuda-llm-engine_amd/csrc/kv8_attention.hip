@@ -82,8 +82,8 @@ __device__ __forceinline__ void split_rounded(float a, float b, uint32_t& hi, ui
 struct Shared {
   int first, last;      // the teams; first > last: there is none
   int column, columns;  // of the tile, from the sequence's first row on
-  int seq;
-  int pad[3];
+  int row0, blind;      // the sequence's first row; columns in front of `blind` see nothing
+  int pad[2];
 };
 
 struct AttentionArgs {
@@ -130,6 +130,11 @@ __device__ __forceinline__ int seen(const AttentionArgs& a, const Seq& q, int co
   const long long n = q.before + column / a.group + 1;
   const long long m = n < q.limit ? n : q.limit;
   return m < 0 ? 0 : (int)m;
+}
+// Columns in front of the first that sees something.
+__device__ __forceinline__ int blind_of(const AttentionArgs& a, const Seq& q) {
+  const long long n = q.limit <= 0 ? q.columns : -q.before * a.group;
+  return n <= 0 ? 0 : n < q.columns ? (int)n : q.columns;
 }
 // A step of units of C columns: 16 bytes of K and as many of V for each of a block's threads, or, of
 // the 64 of a wave, for each of 4 times.
@@ -373,18 +378,19 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
   const bool shared_units = a.parts != nullptr;
   const Share sh = find_share_by_sequence<HD, C, 4>(a);
   const int h = sh.head;
-  auto note = [&](int side, int first, int last, int column, int columns, int seq) {
+  auto note = [&](int side, int first, int last, int column, int columns, const Seq& q) {
     Shared o = {};
     o.first = first;
     o.last = last;
     o.column = column;
     o.columns = columns;
-    o.seq = seq;
+    o.row0 = q.row0;
+    o.blind = blind_of(a, q);
     if (lane == 0) a.shared[2 * worker + side] = o;
   };
   if (shared_units) {
-    note(0, 0, -1, 0, 0, 0);
-    note(1, 0, -1, 0, 0, 0);
+    note(0, 0, -1, 0, 0, Seq{});
+    note(1, 0, -1, 0, 0, Seq{});
   }
 
   long long pos = sh.begin;
@@ -677,7 +683,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
         const int side = step == 0 ? 1 : 0;
         if (!whole) {  // the workers of its first and last steps
           const long long end = pos + ticks - upto, begin = end - steps;
-          note(side, sh.team_at(begin), sh.team_at(end - 1), c0, columns, s);
+          note(side, sh.team_at(begin), sh.team_at(end - 1), c0, columns, q);
         }
         const size_t slot = 2 * (size_t)worker + side;
 #pragma unroll
@@ -752,8 +758,10 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
     }
   };
   const int team = worker / a.n_kv_heads, head = worker % a.n_kv_heads;
+  const Shared both[2] = {a.shared[2 * worker], a.shared[2 * worker + 1]};
+#pragma unroll
   for (int side = 0; side < 2; ++side) {
-    const Shared o = a.shared[2 * worker + side];
+    const Shared o = both[side];
     if (o.first > o.last) continue;
     const int n = o.last - o.first + 1, base = 256 * blockIdx.y;
     const int tasks = V * o.columns - base < 256 ? V * o.columns - base : 256;
@@ -768,7 +776,6 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
     if (slice >= slices) continue;
     const int deal = 256 / lanes, turn = tid / lanes;
     const int task = base + slice * lanes + tid % lanes, c = task / V, d = 4 * (task % V);
-    const Seq q = seq_of(a, o.seq);
     Joint r = {f32x4{0, 0, 0, 0}, -INFINITY, 0.0f};
     if (c < o.columns) {
 #pragma unroll 4
@@ -786,14 +793,14 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
       for (int k = 1; k < deal && k < n; ++k)
         r.add(others[tid + k * lanes], others_ml[tid + k * lanes]);
       const int col = o.column + c;
-      const bool any = seen(a, q, col) > 0;
+      const bool any = col >= o.blind;
       f16x2 y[2];
 #pragma unroll
       for (int e = 0; e < 4; ++e) y[e / 2][e % 2] = any ? (f16)(r.acc[e] / r.l) : (f16)0;
       uint2 v;
       v.x = __builtin_bit_cast(uint32_t, y[0]);
       v.y = __builtin_bit_cast(uint32_t, y[1]);
-      *reinterpret_cast<uint2*>(a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads +
+      *reinterpret_cast<uint2*>(a.out + ((size_t)(o.row0 + col / a.group) * a.n_heads +
                                          head * a.group + col % a.group) * HD + d) = v;
     }
   }
@@ -825,18 +832,19 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
   else
     sh = find_share_by_tile<HD, C, W>(a);
   const int h = sh.head;
-  auto note = [&](int side, int first, int last, int column, int columns, int seq) {
+  auto note = [&](int side, int first, int last, int column, int columns, const Seq& q) {
     Shared o = {};
     o.first = first;
     o.last = last;
     o.column = column;
     o.columns = columns;
-    o.seq = seq;
+    o.row0 = q.row0;
+    o.blind = blind_of(a, q);
     if (tid == 0) a.shared[2 * worker + side] = o;
   };
   if (shared_units) {
-    note(0, 0, -1, 0, 0, 0);
-    note(1, 0, -1, 0, 0, 0);
+    note(0, 0, -1, 0, 0, Seq{});
+    note(1, 0, -1, 0, 0, Seq{});
   }
   long long pos = sh.begin;
   if (pos >= sh.end) return;
@@ -1078,7 +1086,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
       const int side = step == 0 ? 1 : 0;
       if (!whole) {  // the workers of its first and last steps
         const long long end = pos + ticks - upto, begin = end - steps;
-        note(side, sh.team_at(begin), sh.team_at(end - 1), c0, columns, s);
+        note(side, sh.team_at(begin), sh.team_at(end - 1), c0, columns, q);
       }
       l = l + __shfl_xor(l, 32);
       if (own && whole) {
