@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(kThreads) k_verify_sums(const VerifyArgs a) {
   double sum = 0.0, of_odd = 0.0;
 #pragma unroll
   for (int j = 0; j < kPieceVectors; ++j)
-#pragma unroll 4
+#pragma unroll
     for (int e = 0; e < 8; ++e) {
       const double w = weight(logit(x[j][e]), max, z.k);
       const bool is_odd = odd >= 0 && 8 * (v0 + j * kThreads) - r.lead + e == odd;
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
   double sum = 0.0;
 #pragma unroll
   for (int j = 0; j < kPieceVectors; ++j)
-#pragma unroll 4
+#pragma unroll
     for (int e = 0; e < 8; ++e) sum = sum + left_of(w, logit(x[j][e]), logit(y[j][e]), -2);
   sum = block_sum<4>(sum, shared);
   if (threadIdx.x == 0) a.left[(size_t)s * a.pieces + piece] = sum;
