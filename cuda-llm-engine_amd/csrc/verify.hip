@@ -497,7 +497,10 @@ __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
 #pragma unroll
   for (int j = 0; j < kPieceVectors; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sum = sum + left_of(w, logit(x[j][e]), logit(y[j][e]), -2);
+    for (int e = 0; e < 8; ++e)  // as left_of where the draft model has a share, without its branches
+      sum = sum + __builtin_fmax(weight(logit(x[j][e]), w.pm, w.k) * w.ps -
+                                     weight(logit(y[j][e]), w.qm, w.k) * w.qs,
+                                 0.0);
   sum = block_sum<4>(sum, shared);
   if (threadIdx.x == 0) a.left[(size_t)s * a.pieces + piece] = sum;
 }
