@@ -44,15 +44,23 @@ struct Stat {
   int pad;
 };
 
+// Logits over a temperature t, in log2 units.
+struct Scale {
+  double k;   // log2e / t
+  float far;  // at a distance of -far and beyond weights are 0: about 10^9 / k
+  int pad;
+};
+constexpr float kFar = 3.0e38f;  // at most
+
 // Where a sequence ends.
 struct End {
   int first, end, row;  // its rows, and the one that gives its last token
   int last;             // that one stands behind all drafts
   int greedy, at;       // at: the row's argmax, where the choice is greedy
   float pm, qm;         // maxima of the target's and the draft model's row
-  double k;             // log2e / t
+  Scale by;
 };
-static_assert(sizeof(End) == 40, "workspace layout");
+static_assert(sizeof(End) == 48, "workspace layout");
 
 struct VerifyArgs {
   const f16* logits;
@@ -72,32 +80,34 @@ struct VerifyArgs {
   int n_rows, n_seqs, vocab, chunks, pieces;
 };
 
-// 2^y for y <= 0: the series of 2^f, |f| <= 1/2, behind the whole part, to 2^-42 of it. NaN gives 0.
+// 2^y for y from -2^31 to 0, to 2^-40 of it: the whole part by the exponent, f of at most 1/2 by 1 + f g(f),
+// with the g of degree 7 whose largest error there is the least. 2^0 is 1 exactly.
 __device__ __forceinline__ double exp2_64(double y) {
-  y = __builtin_fmax(y, -1100.0);
   const double n = __builtin_rint(y), f = y - n;
-  double p = 7.0549116208011233e-09;  // ln(2)^i / i!
-  p = __builtin_fma(p, f, 1.0178086009239699e-07);
-  p = __builtin_fma(p, f, 1.3215486790144309e-06);
-  p = __builtin_fma(p, f, 1.5252733804059840e-05);
-  p = __builtin_fma(p, f, 1.5403530393381609e-04);
-  p = __builtin_fma(p, f, 1.3333558146428443e-03);
-  p = __builtin_fma(p, f, 9.6181291076284772e-03);
-  p = __builtin_fma(p, f, 5.5504108664821580e-02);
-  p = __builtin_fma(p, f, 2.4022650695910071e-01);
-  p = __builtin_fma(p, f, 6.9314718055994531e-01);
+  double p = 1.31789487561122369e-06;
+  p = __builtin_fma(p, f, 1.53091560970623410e-05);
+  p = __builtin_fma(p, f, 1.54038254120923311e-04);
+  p = __builtin_fma(p, f, 1.33334548606907984e-03);
+  p = __builtin_fma(p, f, 9.61812861616447544e-03);
+  p = __builtin_fma(p, f, 5.55041093526646920e-02);
+  p = __builtin_fma(p, f, 2.40226506981104870e-01);
+  p = __builtin_fma(p, f, 6.93147180548211450e-01);
   p = __builtin_fma(p, f, 1.0);
   return __builtin_ldexp(p, (int)n);
 }
 
-// The weight of a logit under a maximum; k = log2e / t. Equal infinities weigh 1: what their
-// difference is not, a minimum with 0 makes 0.
-__device__ __forceinline__ double weight(float l, float max, double k) {
-  return exp2_64((double)__builtin_fminf(l - max, 0.0f) * k);
+// The weight of a logit under a maximum above -inf. The distance goes to [-far, 0]: at -far it weighs
+// nothing, and a NaN logit, which counts as -inf, has it (the median of a NaN and two numbers is the
+// lower one). Under an infinite maximum, which stands as kFar, only its equals weigh, 1.
+__device__ __forceinline__ double weight(float l, float max, const Scale& by) {
+  const float d = l - __builtin_fminf(max, kFar);
+  return exp2_64((double)__builtin_amdgcn_fmed3f(d, -by.far, 0.0f) * by.k);
 }
-
-// NaN counts as -inf.
-__device__ __forceinline__ float logit(f16 x) { return __builtin_fmaxf((float)x, -INFINITY); }
+// Below 4e-36 finite logits weigh 1 to the last bit, and -kFar still 0.
+__device__ __forceinline__ Scale scale_of(float t) {
+  const double k = __builtin_fmax(kLog2e / (double)t, 4.0e-36);
+  return Scale{k, (float)__builtin_fmin(1.0e9 / k, (double)kFar), 0};
+}
 
 // The vectors of a row: element e of the row is element e + lead of the 16-byte aligned memory that
 // holds it; vector v of it is the row's elements 8 v - lead .. + 7. Those that the row does not fill
@@ -293,7 +303,8 @@ struct RowStat {
   int at;
   double sum;
 };
-__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, size_t which, bool sums, double k) {
+__device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, size_t which, bool sums,
+                                            const Scale& by) {
   const Stat* st = a.stats + which * a.chunks;
   const int lane = threadIdx.x & 63;
   float max = -INFINITY, own = -INFINITY;
@@ -305,7 +316,7 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, size_t which, b
   for (int c = lane; c < a.chunks; c += 64) {
     const Stat x = st[c];
     if (x.max == max) at = min(at, x.at);
-    if (sums && x.max > -INFINITY) sum = sum + (double)x.sum * weight(x.max, max, k);
+    if (sums && x.max > -INFINITY) sum = sum + (double)x.sum * weight(x.max, max, by);
   }
   r.at = wave_min(at);
   r.sum = sums ? wave_sum(sum) : 0.0;
@@ -313,10 +324,11 @@ __device__ __forceinline__ RowStat row_stat(const VerifyArgs& a, size_t which, b
 }
 
 // A row's sum of weights in 64 bits, by one wave.
-__device__ double exact_sum(const f16* logits, size_t row, int vocab, float max, double k) {
+__device__ double exact_sum(const f16* logits, size_t row, int vocab, float max,
+                            const Scale& by) {
   double sum = 0.0;
   for (int v = threadIdx.x & 63; v < vocab; v += 64)
-    sum = sum + weight(logit(logits[row * vocab + v]), max, k);
+    sum = sum + weight((float)logits[row * vocab + v], max, by);
   return wave_sum(sum);
 }
 
@@ -328,7 +340,7 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
   rows_of(a, s, z.first, z.end);
   const float t = a.temperature ? a.temperature[s] : 1.0f;
   z.greedy = is_greedy(t);
-  z.k = z.greedy ? 0.0 : kLog2e / (double)t;
+  z.by = z.greedy ? Scale{} : scale_of(t);
   if (threadIdx.x == 0) stop = z.end - 1;
   __syncthreads();
   for (int row = z.first + wave; row < z.end - 1; row += 4) {
@@ -336,8 +348,8 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
     const bool inside = d >= 0 && d < a.vocab;
     const float u = a.accept_u[row];
     const size_t at = (size_t)row * a.vocab + (inside ? d : 0);
-    const float ld = logit(a.logits[at]), lq = a.draft_logits ? logit(a.draft_logits[at]) : 0.0f;
-    const RowStat p = row_stat(a, row, !z.greedy, z.k);
+    const float ld = (float)a.logits[at], lq = a.draft_logits ? (float)a.draft_logits[at] : 0.0f;
+    const RowStat p = row_stat(a, row, !z.greedy, z.by);
     bool accept;
     if (z.greedy) {
       accept = inside && p.max > -INFINITY && d == p.at;
@@ -345,19 +357,19 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
       accept = false;
     } else {
       // u q(d) < p(d), as one side against the other with the sums multiplied out
-      const double pw = weight(ld, p.max, z.k);
+      const double pw = weight(ld, p.max, z.by);
       double qw = 1.0, qs = 1.0;
       float qm = -INFINITY;
       if (a.draft_logits) {
-        const RowStat q = row_stat(a, (size_t)a.n_rows + row, true, z.k);
+        const RowStat q = row_stat(a, (size_t)a.n_rows + row, true, z.by);
         qm = q.max;
-        qw = qm > -INFINITY ? weight(lq, qm, z.k) : 0.0;
+        qw = qm > -INFINITY ? weight(lq, qm, z.by) : 0.0;
         qs = qm > -INFINITY ? q.sum : 1.0;
       }
       double one = (double)u * (qw / qs), other = pw / p.sum;
       if (__builtin_fabs(one - other) < 6.103515625e-5 * __builtin_fmax(one, other)) {
-        if (qm > -INFINITY) one = (double)u * (qw / exact_sum(a.draft_logits, row, a.vocab, qm, z.k));
-        other = pw / exact_sum(a.logits, row, a.vocab, p.max, z.k);
+        if (qm > -INFINITY) one = (double)u * (qw / exact_sum(a.draft_logits, row, a.vocab, qm, z.by));
+        other = pw / exact_sum(a.logits, row, a.vocab, p.max, z.by);
       }
       accept = one < other;
     }
@@ -372,11 +384,11 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
   z.pm = z.qm = -INFINITY;
   z.at = -1;
   if (z.row >= z.first) {
-    const RowStat p = row_stat(a, z.row, false, z.k);
+    const RowStat p = row_stat(a, z.row, false, z.by);
     z.pm = p.max;
     z.at = p.at;
     if (a.draft_logits && !z.last && !z.greedy)
-      z.qm = row_stat(a, (size_t)a.n_rows + z.row, false, z.k).max;
+      z.qm = row_stat(a, (size_t)a.n_rows + z.row, false, z.by).max;
   }
   return z;
 }
@@ -425,15 +437,22 @@ __global__ void __launch_bounds__(kThreads) k_verify_sums(const VerifyArgs a) {
                       : draft_vector(a, z.row, r, v0 + j * kThreads);
   const float max = share == 0 ? z.pm : z.qm;
   double sum = 0.0, of_odd = 0.0;
+  if (odd < 0) {
 #pragma unroll
-  for (int j = 0; j < kPieceVectors; ++j)
+    for (int j = 0; j < kPieceVectors; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const double w = weight(logit(x[j][e]), max, z.k);
-      const bool is_odd = odd >= 0 && 8 * (v0 + j * kThreads) - r.lead + e == odd;
-      of_odd = is_odd ? w : of_odd;
-      sum = sum + (is_odd ? 0.0 : w);
-    }
+      for (int e = 0; e < 8; ++e) sum = sum + weight((float)x[j][e], max, z.by);
+  } else {
+#pragma unroll
+    for (int j = 0; j < kPieceVectors; ++j)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const double w = weight((float)x[j][e], max, z.by);
+        const bool is_odd = 8 * (v0 + j * kThreads) - r.lead + e == odd;
+        of_odd = is_odd ? w : of_odd;
+        sum = sum + (is_odd ? 0.0 : w);
+      }
+  }
   sum = block_sum<4>(sum, shared);
   if (odd >= 0) of_odd = block_sum<4>(of_odd, shared);
   if (threadIdx.x == 0) {
@@ -451,19 +470,20 @@ __global__ void __launch_bounds__(kThreads) k_verify_sums(const VerifyArgs a) {
 // What the last token is drawn from: a place's weight.
 struct Left {
   float pm, qm;
-  double k, ps, qs;  // ps, qs: 1 / sums, or 1 and 0 where the draft model has no share
+  Scale by;
+  double ps, qs;  // ps, qs: 1 / sums, or 1 and 0 where the draft model has no share
   int odd;           // a certain draft that was refused, -1
 };
 __device__ __forceinline__ double left_of(const Left& w, float l, float lq, int at) {
-  const double p = weight(l, w.pm, w.k);
+  const double p = weight(l, w.pm, w.by);
   if (at == w.odd) return 0.0;
-  return w.qs == 0.0 ? p : __builtin_fmax(p * w.ps - weight(lq, w.qm, w.k) * w.qs, 0.0);
+  return w.qs == 0.0 ? p : __builtin_fmax(p * w.ps - weight(lq, w.qm, w.by) * w.qs, 0.0);
 }
 // By a block of WAVES waves; first: the sums of piece threadIdx.x, 0 where there is none.
 template <int WAVES>
 __device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int s, double2 first,
                                           double* shared) {
-  Left w = {z.pm, z.qm, z.k, 1.0, 0.0, refused(a, z)};
+  Left w = {z.pm, z.qm, z.by, 1.0, 0.0, refused(a, z)};
   if (z.qm > -INFINITY) {
     double p = first.x, q = first.y;
     for (int c = threadIdx.x + 64 * WAVES; c < a.pieces; c += 64 * WAVES) {
@@ -498,8 +518,8 @@ __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
   for (int j = 0; j < kPieceVectors; ++j)
 #pragma unroll
     for (int e = 0; e < 8; ++e)  // as left_of where the draft model has a share, without its branches
-      sum = sum + __builtin_fmax(weight(logit(x[j][e]), w.pm, w.k) * w.ps -
-                                     weight(logit(y[j][e]), w.qm, w.k) * w.qs,
+      sum = sum + __builtin_fmax(weight((float)x[j][e], w.pm, w.by) * w.ps -
+                                     weight((float)y[j][e], w.qm, w.by) * w.qs,
                                  0.0);
   sum = block_sum<4>(sum, shared);
   if (threadIdx.x == 0) a.left[(size_t)s * a.pieces + piece] = sum;
@@ -576,7 +596,7 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
   double each[8], own = 0.0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    each[e] = left_of(w, logit(x[e]), logit(y[e]), 8 * v - r.lead + e);
+    each[e] = left_of(w, (float)x[e], (float)y[e], 8 * v - r.lead + e);
     own = own + each[e];
   }
   const double upto = wave_prefix(own);
@@ -622,7 +642,7 @@ using namespace llmk;
 
 extern "C" size_t llmk_verify_drafts_workspace_floats(int n_rows, int n_seqs, int vocab) {
   if (n_rows <= 0 || n_seqs <= 0 || vocab <= 0) return 0;
-  return (size_t)n_seqs * 12 +  // ends of 40 bytes, to 16
+  return (size_t)n_seqs * (sizeof(End) / 4) +
          (size_t)chunks_of(vocab) * 2 * (size_t)n_rows * (sizeof(Stat) / 4) +
          (size_t)pieces_of(vocab) * (size_t)n_seqs * 6;
 }
