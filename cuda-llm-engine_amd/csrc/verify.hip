@@ -481,30 +481,29 @@ __device__ __forceinline__ double left_of(const Left& w, float l, float lq, int 
   if (at == w.odd) return 0.0;
   return w.qs == 0.0 ? p : __builtin_fmax(p * w.ps - weight(lq, w.qm, w.by) * w.qs, 0.0);
 }
-// By a block of WAVES waves; first: the sums of piece threadIdx.x, 0 where there is none.
-template <int WAVES>
-__device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int s, double2 first,
-                                          double* shared) {
+// By each wave for itself, 64 pieces at a time, without a barrier; first: the sums of piece `lane`, 0
+// where there is none.
+__device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int s, double2 first) {
   Left w = {z.pm, z.qm, z.by, 1.0, 0.0, refused(a, z)};
   if (z.qm > -INFINITY) {
     double p = first.x, q = first.y;
-    for (int c = threadIdx.x + 64 * WAVES; c < a.pieces; c += 64 * WAVES) {
+    for (int c = (threadIdx.x & 63) + 64; c < a.pieces; c += 64) {
       const double2 x = a.sums[(size_t)s * a.pieces + c];
       p = p + x.x;
       q = q + x.y;
     }
-    w.ps = 1.0 / block_sum<WAVES>(p, shared);
-    w.qs = 1.0 / block_sum<WAVES>(q, shared);
+    w.ps = 1.0 / wave_sum(p);
+    w.qs = 1.0 / wave_sum(q);
   }
   return w;
 }
 
 __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
   __shared__ double shared[4];
-  const int piece = blockIdx.x % a.pieces, s = blockIdx.x / a.pieces;
+  const int piece = blockIdx.x % a.pieces, s = blockIdx.x / a.pieces, lane = threadIdx.x & 63;
   const End z = a.ends[s];
-  const double2 first = (int)threadIdx.x < a.pieces ? a.sums[(size_t)s * a.pieces + threadIdx.x]
-                                                    : make_double2(0.0, 0.0);
+  const double2 first =
+      lane < a.pieces ? a.sums[(size_t)s * a.pieces + lane] : make_double2(0.0, 0.0);
   if (!draws(z) || !(z.qm > -INFINITY)) return;
   const Row r = row_of(a.logits, z.row, a.vocab);
   const int v0 = piece * kPieceVectors * kThreads + threadIdx.x;
@@ -514,7 +513,7 @@ __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
     x[j] = load_vector(r, v0 + j * kThreads);
     y[j] = draft_vector(a, z.row, r, v0 + j * kThreads);
   }
-  const Left w = left_from<4>(a, z, s, first, shared);
+  const Left w = left_from(a, z, s, first);
   double sum = 0.0;
 #pragma unroll
   for (int j = 0; j < kPieceVectors; ++j)
@@ -530,40 +529,41 @@ __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
 __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyArgs a) {
   constexpr int WAVES = kChooseThreads / 64;
   __shared__ double shared[WAVES];
-  __shared__ double parts[kChooseThreads];
   __shared__ int first_past, last_any;
-  int chosen = 0;
-  double chosen_base = 0.0;
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const End z = a.ends[s];
   const double2* sums = a.sums + (size_t)s * a.pieces;
   // what all this waits for, in one go
-  const double2 first = tid < a.pieces ? sums[tid] : make_double2(0.0, 0.0);
-  const double first_left =
-      a.draft_logits && tid < a.pieces ? a.left[(size_t)s * a.pieces + tid] : 0.0;
+  const double2 first = lane < a.pieces ? sums[lane] : make_double2(0.0, 0.0);
+  const double first_left =  // nobody's where the draft model has no share
+      a.draft_logits && lane < a.pieces ? a.left[(size_t)s * a.pieces + lane] : 0.0;
   const float u = a.sample_u[s];
   for (int row = z.first + tid; row < z.end; row += kChooseThreads)
     if (row != z.row) a.tokens[row] = row < z.row ? a.drafts[row] : -1;
   if (tid == 0) {
     a.n_accepted[s] = z.end > z.first ? z.row - z.first : 0;
     if (z.end > z.first && !draws(z)) a.tokens[z.row] = z.greedy && z.pm > -INFINITY ? z.at : -1;
+  }
+  if (!draws(z)) return;
+  if (tid == 0) {
     first_past = 0x7FFFFFFF;
     last_any = -1;
   }
-  if (!draws(z)) return;
-  Left w = left_from<WAVES>(a, z, s, first, shared);
-  // piece c's sum; with only_p of p alone, where p is nowhere above q
+  Left w = left_from(a, z, s, first);
+  // Each wave looks for the piece by itself, a lane for each. Piece c's sum; with only_p of p alone, where
+  // p is nowhere above q.
   const bool drafted = w.qs != 0.0, certain = w.odd >= 0;
   bool only_p = false;
   auto piece_sum = [&](int c) {
-    if (drafted && !only_p) return c == tid ? first_left : a.left[(size_t)s * a.pieces + c];
-    const double2 x = c == tid ? first : sums[c];
+    if (c >= a.pieces) return 0.0;
+    if (drafted && !only_p) return c == lane ? first_left : a.left[(size_t)s * a.pieces + c];
+    const double2 x = c == lane ? first : sums[c];
     return only_p && certain ? x.x + x.y : x.x;
   };
   auto total_of = [&] {
-    double sum = 0.0;
-    for (int c = tid; c < a.pieces; c += kChooseThreads) sum = sum + piece_sum(c);
-    return block_sum<WAVES>(sum, shared);
+    double sum = piece_sum(lane);
+    for (int c = lane + 64; c < a.pieces; c += 64) sum = sum + piece_sum(c);
+    return wave_sum(sum);
   };
   double total = total_of();
   if (!(total > 0.0)) {
@@ -574,24 +574,20 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
   }
   const double aim = (double)u * total;
   // the first piece that ends past the aim, or behind them all, by rounding, the last with any weight
-  double before = 0.0;
-  bool past = false;
-  for (int c0 = 0; c0 < a.pieces && !past; c0 += kChooseThreads) {
-    const int n = a.pieces - c0 < kChooseThreads ? a.pieces - c0 : kChooseThreads;
-    __syncthreads();
-    if (tid < n) parts[tid] = piece_sum(c0 + tid);
-    __syncthreads();
-    for (int c = 0; c < n && !past; ++c) {
-      const double one = parts[c];
-      if (one > 0.0) {
-        chosen = c0 + c;
-        chosen_base = before;
-      }
-      before = before + one;
-      past = before > aim;
+  int chosen = 0;
+  double chosen_base = 0.0, before = 0.0;
+  for (int c0 = 0; c0 < a.pieces; c0 += 64) {
+    const double one = piece_sum(c0 + lane), upto = wave_prefix(one), end = before + upto;
+    const uint64_t any = __builtin_amdgcn_ballot_w64(one > 0.0);
+    const uint64_t past = __builtin_amdgcn_ballot_w64(one > 0.0 && end > aim);
+    if (any) {
+      const int at = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(any);
+      chosen = c0 + at;
+      chosen_base = readlane_f64(end - one, at);
     }
+    if (past) break;
+    before = before + readlane_f64(upto, 63);
   }
-  __syncthreads();  // `shared` is free
   const Row r = row_of(a.logits, z.row, a.vocab);
   const int v = chosen * kChooseThreads + tid;
   const f16x8 x = load_vector(r, v), y = w.qs != 0.0 ? draft_vector(a, z.row, r, v) : x;
@@ -616,7 +612,7 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
       if (c > aim && token == 0x7FFFFFFF) token = last;
     }
   }
-  // one lane of a wave: all 1024 threads at one address take 6 us
+  // one lane of a wave: all threads at one address take 6 us
   token = wave_min(token);
   last = -wave_min(-last);
   if (lane == 0) {

@@ -188,6 +188,23 @@ def test_many_rows_of_one_sequence_and_many_sequences(llmk):
     check(llmk, case(14, rng.integers(0, 4, 700), 33, True))
 
 
+@pytest.mark.parametrize("drafted", [True, False])
+def test_vocabularies_of_more_pieces_than_a_wave_has_lanes(llmk, drafted):
+    """Tokens in the first pieces, behind the 64th, and the row's last; weights in a few places only."""
+    vocab = 300001
+    c = list(case(22, [2, 1, 3, 2, 1], vocab, drafted, std=1.0))
+    for u in (0.0, 0.5, 0.97, np.nextafter(np.float32(1.0), np.float32(0.0))):
+        c[6] = np.full(5, u, np.float32)
+        check(llmk, c)
+    c[0][:] = -np.inf
+    c[0][:, [70000, 290000, 300000]] = np.array([1.0, 0.5, 2.0], np.float16)
+    if drafted:
+        c[1][:, [70000, 290000, 300000]] = np.array([9.0, 9.0, 8.0], np.float16)
+    for u in (0.0, 0.4, 0.999):
+        c[6] = np.full(5, u, np.float32)
+        check(llmk, c)
+
+
 def test_no_rows(llmk):
     """Sequences without a row in the call: nothing but zeros, and no workspace needed."""
     n_accepted = torch.full((5,), -9, dtype=torch.int32, device=DEV)
