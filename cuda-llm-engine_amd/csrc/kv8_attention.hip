@@ -27,9 +27,11 @@ constexpr float kSlack = 8.0f;
 // What a unit's beginning costs, in steps. With 0 / 1 / 2 / 4, us: 48 sequences of up to 5 rows 41.1 /
 // 37.5 / 35.8 / 36.1, 1507 rows of one 68.2 / 68.5 / 67.5 / 72.0.
 constexpr int kStart = 2;
-// Sequences of up to this many columns go by waves, in tiles of 32; us by waves and by blocks: 48 x 16
-// rows (64 columns) 58.5 and 67.5, 4 x 16 19.9 and 23.4, 48 x 24 rows (96 columns) 82.7 and 74.0.
-constexpr int kFewColumns = 64;
+// Sequences of up to this many columns go by waves, in tiles of 32, where no sequence of the call has more;
+// us by waves and by blocks: 48 x 16 rows (64 columns) 58.5 and 67.5, 4 x 16 19.9 and 23.4, 48 x 24 rows
+// (96 columns) 82.7 and 74.0. Beside longer ones, up to kMixedColumns: blocks run anyhow, and the waves'
+// launch stands in front of theirs (20 x up to 100 rows, 46.7 us with 32 and 56.7 with 64).
+constexpr int kFewColumns = 64, kMixedColumns = 32;
 // From here on blocks of 8 waves and 256 columns: 1507 rows at 64 dims 74.0 -> 69.5 us, 500 rows at 128
 // dims 60.0 -> 53.8, 5 x 500 rows at 8000 positions 234 -> 206. Below, tiles of 128 columns leave fewer
 // waves without work (32 query heads on 8, us, both at 2000 positions: 250 rows 27.9 and 29.3, 100 rows
@@ -176,6 +178,7 @@ struct Share {
   int team, head, teams;
   int seq, tile;         // that hold the beginning of the team's share, and
   int at;                // its place in them, in ticks
+  Seq rows;              // the sequence's
   long long begin, end;  // among the ticks of a head
   long long each;        // of the first `more` teams one more
   int more;
@@ -204,6 +207,30 @@ struct Share {
   }
 };
 
+// The sum of the lanes up to each, by lane moves: within 16 lanes, then the rows in front (their last
+// lanes').
+template <int CTRL, int ROWS = 0xF>  // 0 where there is no source lane, and in rows not named
+__device__ __forceinline__ long long dpp_i64(long long v) {
+  const uint32_t lo =
+      __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xF, ROWS == 0xF);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)((uint64_t)v >> 32), CTRL, ROWS,
+                                                  0xF, ROWS == 0xF);
+  return (long long)(((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ long long wave_prefix(long long v) {
+  v = v + dpp_i64<0x111>(v);
+  v = v + dpp_i64<0x112>(v);
+  v = v + dpp_i64<0x114>(v);
+  v = v + dpp_i64<0x118>(v);
+  v = v + dpp_i64<0x142, 0xA>(v);
+  return v + dpp_i64<0x143, 0xC>(v);
+}
+__device__ __forceinline__ long long readlane_i64(long long v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)v >> 32), lane);
+  return (long long)(((uint64_t)hi << 32) | lo);
+}
+
 // A thread's place in a sum over the block's W waves: what those in front of it have, and all.
 struct Place {
   long long before, total;
@@ -212,11 +239,7 @@ template <int W>
 __device__ __forceinline__ Place place_of(long long mine) {
   __shared__ long long wave_sum_[W];
   const int lane = threadIdx.x & 63, wave = same((int)threadIdx.x >> 6);
-  long long upto = mine;
-  for (int d = 1; d < 64; d *= 2) {
-    const long long o = __shfl_up(upto, d);
-    if (lane >= d) upto += o;
-  }
+  const long long upto = wave_prefix(mine);
   if (lane == 63) wave_sum_[wave] = upto;
   __syncthreads();
   Place r = {upto - mine, 0};
@@ -232,6 +255,17 @@ __device__ __forceinline__ Place place_of(long long mine) {
 template <int C>
 __device__ __forceinline__ int tiles_of(const AttentionArgs& a, int s) {
   return (seq_of(a, s).columns + C - 1) / C;
+}
+
+// The tile of the share's sequence that holds a place in its ticks.
+template <int HD, int C>
+__device__ __forceinline__ void find_tile(const AttentionArgs& a, Share& r, long long at) {
+  for (r.tile = 0;; ++r.tile) {
+    const int ticks = kStart + same(tile_steps<HD, C>(a, r.rows, r.tile));
+    if (at < ticks) break;
+    at -= ticks;
+  }
+  r.at = (int)at;
 }
 
 // The beginnings of the shares of a block's WORKERS workers (4 waves, or the block): a thread sums the
@@ -270,17 +304,55 @@ __device__ __forceinline__ Share find_share_by_sequence(const AttentionArgs& a) 
   }
   __syncthreads();
   r.seq = same(seq_[own]);
-  long long at = same(at_[own]);
-  r.tile = 0;
   if (r.begin < r.end) {
-    const Seq q = same(seq_of(a, r.seq));
-    for (;; ++r.tile) {
-      const int ticks = kStart + same(tile_steps<HD, C>(a, q, r.tile));
-      if (at < ticks) break;
-      at -= ticks;
+    r.rows = same(seq_of(a, r.seq));
+    find_tile<HD, C>(a, r, same(at_[own]));
+  }
+  return r;
+}
+
+// The same by each wave for itself, with up to 256 sequences in its lanes: no barrier, and the found
+// one's rows come from its lane (one sequence 10.4 -> 9.4 us, 48 of up to 5 rows 35.3 -> 34.1).
+template <int HD, int C>
+__device__ __forceinline__ Share find_share_by_lane(const AttentionArgs& a, int worker) {
+  constexpr int N = 4;
+  const int lane = threadIdx.x & 63;
+  Seq q[N];
+  long long mine[N], upto[N], total = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int s = 64 * i + lane;
+    mine[i] = 0;
+    q[i] = Seq{};
+    if (64 * i >= a.batch.n_seqs) continue;
+    if (s < a.batch.n_seqs) {
+      q[i] = seq_of(a, s);
+      for (int t = 0; t * C < q[i].columns; ++t) mine[i] += kStart + tile_steps<HD, C>(a, q[i], t);
     }
   }
-  r.at = (int)at;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    upto[i] = 0;
+    if (64 * i >= a.batch.n_seqs) continue;
+    upto[i] = total + wave_prefix(mine[i]);
+    total = readlane_i64(upto[i], 63);
+  }
+  Share r = Share::of(a, total, worker);
+  if (r.begin >= r.end) return r;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const long long from = upto[i] - mine[i];
+    const uint64_t at = __builtin_amdgcn_ballot_w64(r.begin >= from && r.begin < upto[i]);
+    if (at) {
+      const int l = __builtin_ctzll(at);
+      r.seq = 64 * i + l;
+      r.rows.row0 = __builtin_amdgcn_readlane(q[i].row0, l);
+      r.rows.columns = __builtin_amdgcn_readlane(q[i].columns, l);
+      r.rows.before = readlane_i64(q[i].before, l);
+      r.rows.limit = readlane_i64(q[i].limit, l);
+      find_tile<HD, C>(a, r, r.begin - readlane_i64(from, l));
+    }
+  }
   return r;
 }
 
@@ -338,6 +410,7 @@ __device__ __forceinline__ Share find_share_by_tile(const AttentionArgs& a) {
   r.seq = same(found_[0]);
   r.tile = same(found_[1]);
   r.at = same(found_[2]);
+  if (r.begin < r.end) r.rows = same(seq_of(a, r.seq));
   return r;
 }
 
@@ -376,7 +449,8 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int worker = 4 * (int)blockIdx.x + wave;
   const bool shared_units = a.parts != nullptr;
-  const Share sh = find_share_by_sequence<HD, C, 4>(a);
+  const Share sh = a.batch.n_seqs <= 256 ? find_share_by_lane<HD, C>(a, worker)
+                                         : find_share_by_sequence<HD, C, 4>(a);
   const int h = sh.head;
   auto note = [&](int side, int first, int last, int column, int columns, const Seq& q) {
     Shared o = {};
@@ -396,7 +470,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
   long long pos = sh.begin;
   if (pos < sh.end) {
     int s = sh.seq, tile = sh.tile, tick = sh.at;
-    Seq q = same(seq_of(a, s));
+    Seq q = sh.rows;
     int steps = same(tile_steps<HD, C>(a, q, tile));
     const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
     int ids = 0, ids_of = -1, window = -1;  // 64 entries of a sequence's table, one to a lane
@@ -828,7 +902,8 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
   if (tid < 2) odd[tid] = 0;
   Share sh;
   if constexpr (W == 4)
-    sh = find_share_by_sequence<HD, C, 1>(a);
+    sh = a.batch.n_seqs <= 256 ? find_share_by_lane<HD, C>(a, worker)
+                               : find_share_by_sequence<HD, C, 1>(a);
   else
     sh = find_share_by_tile<HD, C, W>(a);
   const int h = sh.head;
@@ -849,7 +924,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
   long long pos = sh.begin;
   if (pos >= sh.end) return;
   int s = sh.seq, tile = sh.tile, tick = sh.at;
-  Seq q = same(seq_of(a, s));
+  Seq q = sh.rows;
   int steps = same(tile_steps<HD, C>(a, q, tile));
   const float to_log2 = kLog2e / __builtin_sqrtf((float)HD);
 
@@ -1160,11 +1235,11 @@ int attention_launch(AttentionArgs a, int max_rows, hipStream_t stream) {
   if (columns <= 16) return few_launch<HD, 1>(a, stream);
   if (columns <= kFewColumns) return few_launch<HD, 2>(a, stream);
   if (a.batch.n_seqs > 1) {
-    a.most_columns = kFewColumns;
+    a.most_columns = kMixedColumns;
     const int st = few_launch<HD, 2>(a, stream);
     if (st != LLMK_OK) return st;
     a.most_columns = 0x7FFFFFFF;
-    a.least_columns = kFewColumns + 1;
+    a.least_columns = kMixedColumns + 1;
   }
   return columns <= kWideColumns || a.n_kv_heads > kManyWorkers<8> ? many_launch<HD, 4>(a, stream)
                                                                    : many_launch<HD, 8>(a, stream);
