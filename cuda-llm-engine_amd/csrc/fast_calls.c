@@ -52,42 +52,43 @@ static void* address(PyObject* t, PyObject* dtype, long long least) {
   return p;
 }
 
-/* The current device, -1 if it cannot be told. */
-static long long device_now(void) {
-  long long at = -1;
-  PyObject* v = PyObject_CallNoArgs(get_device);
-  if (v) {
-    at = PyLong_AsLongLong(v);
-    Py_DECREF(v);
-  }
-  if (PyErr_Occurred()) {
-    PyErr_Clear();
-    at = -1;
-  }
-  return at;
-}
-
-/* address() of a tensor of this device, and how many elements it has. */
+/* address() of a tensor of this device, and how many elements it has. The device number of a tensor that
+ * is not on a GPU is -1. */
 static void* address_on(PyObject* t, PyObject* dtype, long long least, long long device,
                         long long* numel) {
-  void* p = address(t, dtype, least);
-  if (!p) return NULL;
-  long long at = -1, n = -1;
+  if ((PyObject*)Py_TYPE(t) != tensor_type) return NULL;
+  long long n = -1, at = -1;
+  void* p = NULL;
   PyObject* v = PyObject_CallMethodNoArgs(t, s_get_device);
   if (v) {
     at = PyLong_AsLongLong(v);
     Py_DECREF(v);
   }
-  if (numel && (v = PyObject_CallMethodNoArgs(t, s_numel))) {
+  int ok = at == device && at >= 0;
+  if (ok) {
+    v = PyObject_GetAttr(t, s_dtype);
+    ok = v == dtype;
+    Py_XDECREF(v);
+  }
+  if (ok) {
+    v = PyObject_CallMethodNoArgs(t, s_is_contiguous);
+    ok = v == Py_True;
+    Py_XDECREF(v);
+  }
+  if (ok && (v = PyObject_CallMethodNoArgs(t, s_numel))) {
     n = PyLong_AsLongLong(v);
     Py_DECREF(v);
-    *numel = n;
+  }
+  if (ok && n >= least && n > 0 && (v = PyObject_CallMethodNoArgs(t, s_data_ptr))) {
+    p = PyLong_AsVoidPtr(v);
+    Py_DECREF(v);
   }
   if (PyErr_Occurred()) {
     PyErr_Clear();
-    return NULL;
+    p = NULL;
   }
-  return at == device ? p : NULL;
+  if (numel) *numel = n;
+  return p;
 }
 
 /* torch's current stream for None, the number itself for a number. */
@@ -107,6 +108,25 @@ static int stream_of(PyObject* o, void** stream) {
   const int ok = v && !PyErr_Occurred();
   if (!ok) PyErr_Clear();
   return ok;
+}
+
+/* The current device, -1 if it cannot be told, and the stream as stream_of() gives it. */
+static long long device_and_stream(PyObject* o, void** stream) {
+  long long at = -1;
+  PyObject *dev = PyObject_CallNoArgs(get_device), *v = NULL;
+  if (dev) {
+    at = PyLong_AsLongLong(dev);
+    v = o == Py_None ? PyObject_CallOneArg(get_stream, dev)
+                     : PyLong_CheckExact(o) ? Py_NewRef(o) : NULL;
+    Py_DECREF(dev);
+  }
+  if (v) {
+    *stream = PyLong_AsVoidPtr(v);
+    Py_DECREF(v);
+  }
+  const int ok = v && !PyErr_Occurred();
+  if (!ok) PyErr_Clear();
+  return ok ? at : -1;
 }
 
 /* A Python int from 0 to INT_MAX, the products of two of which fit a long long. */
@@ -268,9 +288,10 @@ FUNCTION(attention_decode_fast, 15)
                                     page_size, heads, kv_heads, head_dim, splits, stream));
 }
 
-/* Tensors of the calls below: on the current device, `here`. OPT: or None. */
-#define HERE                          \
-  const long long here = device_now(); \
+/* Tensors of the calls below: on the current device, `here`. OPT: or None. The stream is argument `at`. */
+#define HERE(at)                                               \
+  void* stream;                                                \
+  const long long here = device_and_stream(args[at], &stream); \
   if (here < 0) Py_RETURN_NONE
 #define TENSOR_ON(type, name, at, dtype, least)                           \
   type* name = (type*)address_on(args[at], dtype, least, here, NULL);      \
@@ -308,14 +329,13 @@ FUNCTION(kv8_append, 19)
     Py_RETURN_NONE;
   const long long width = (heads + 2LL * kv_heads) * head_dim;
   if (ld < width) Py_RETURN_NONE;
-  HERE;
+  HERE(18);
   TENSOR_ON(uint16_t, qkv, 0, half_dtype, (n_rows - 1LL) * ld + width);
   TENSOR_ON(uint16_t, q_out, 2, half_dtype, (long long)n_rows * heads * head_dim);
   POOL(k, 3, kv_heads, page_size, head_dim);
   POOL(v, 5, kv_heads, page_size, head_dim);
   BATCH(7);
   TENSOR_ON(float, inv_freq, 10, float_dtype, head_dim / 2);
-  STREAM(18);
   ANSWER(llmk_kv8_append(qkv, ld, q_out, k_pool, k_scale, v_pool, v_scale, tables, starts, lens,
                          inv_freq, n_rows, n_seqs, max_pages, page_size, heads, kv_heads, head_dim,
                          stream));
@@ -331,13 +351,12 @@ FUNCTION(kv8_gather, 16)
   if (!n_rows || !page_size || !kv_heads || !head_dim || kv_heads > 65535 || head_dim > 65535 ||
       page_size > 65535)
     Py_RETURN_NONE;
-  HERE;
+  HERE(15);
   POOL(k, 0, kv_heads, page_size, head_dim);
   POOL(v, 2, kv_heads, page_size, head_dim);
   BATCH(4);
   TENSOR_ON(uint16_t, k_out, 7, half_dtype, (long long)n_rows * kv_heads * head_dim);
   TENSOR_ON(uint16_t, v_out, 8, half_dtype, (long long)n_rows * kv_heads * head_dim);
-  STREAM(15);
   ANSWER(llmk_kv8_gather(k_pool, k_scale, v_pool, v_scale, tables, starts, lens, k_out, v_out,
                          n_rows, n_seqs, max_pages, page_size, kv_heads, head_dim, stream));
 }
@@ -354,7 +373,7 @@ FUNCTION(kv8_attention, 19)
   if (!n_rows || !page_size || !heads || !kv_heads || !head_dim || heads > 65535 ||
       kv_heads > 65535 || head_dim > 65535 || page_size > 65535)
     Py_RETURN_NONE;
-  HERE;
+  HERE(18);
   TENSOR_ON(uint16_t, q, 0, half_dtype, (long long)n_rows * heads * head_dim);
   POOL(k, 1, kv_heads, page_size, head_dim);
   POOL(v, 3, kv_heads, page_size, head_dim);
@@ -362,7 +381,6 @@ FUNCTION(kv8_attention, 19)
   TENSOR_ON(uint16_t, out, 8, half_dtype, (long long)n_rows * heads * head_dim);
   OPT_ON(float, workspace, 9, float_dtype,
          (long long)llmk_kv8_attention_workspace_floats(head_dim));
-  STREAM(18);
   ANSWER(llmk_kv8_attention(q, k_pool, k_scale, v_pool, v_scale, tables, starts, lens, out,
                             workspace, n_rows, n_seqs, max_rows, max_pages, page_size, heads,
                             kv_heads, head_dim, stream));
@@ -376,7 +394,7 @@ FUNCTION(verify_drafts, 14)
   const long long given = args[3] != Py_None ? n_rows : 0;
   const size_t floats = llmk_verify_drafts_workspace_floats(n_rows, n_seqs, vocab);
   if (floats > (size_t)LLONG_MAX) Py_RETURN_NONE;
-  HERE;
+  HERE(13);
   TENSOR_ON(uint16_t, logits, 0, half_dtype, (long long)n_rows * vocab);
   OPT_ON(uint16_t, draft_logits, 1, half_dtype, given * vocab);
   OPT_ON(int32_t, drafts, 2, int_dtype, given);
@@ -387,7 +405,6 @@ FUNCTION(verify_drafts, 14)
   TENSOR_ON(int32_t, n_accepted, 7, int_dtype, n_seqs);
   TENSOR_ON(int32_t, tokens, 8, int_dtype, n_rows);
   TENSOR_ON(float, workspace, 9, float_dtype, (long long)floats);
-  STREAM(13);
   ANSWER(llmk_verify_drafts(logits, draft_logits, drafts, starts, temperature, accept_u, sample_u,
                             n_accepted, tokens, workspace, n_rows, n_seqs, vocab, stream));
 }
