@@ -1,5 +1,28 @@
-// Attention over the 8-bit KV cache (layout: kv8.hpp): out = softmax_j(q . K_j / sqrt(head_dim)) V_j
-// over the positions j up to the row's own, for rows of any number a sequence.
+// Attention over the 8-bit KV cache (layout: kv8.hpp): out = softmax_j(q . K_j / sqrt(head_dim))
+// V_j over the positions j up to the row's own, for rows of any number a sequence.
+//
+// One pass with a running maximum m and sum l in 32 bits: of a step's scores s, in log2 units,
+//   m' = max(m, s), l' = 2^(m - m') l + sum 2^(s - m'), O' = 2^(m - m') O + sum 2^(s - m') V,
+// and O / l at the end, rounded once. Both products run on the matrix cores, transposed, so that a
+// row of q (a column here) stays in its lanes from the scores to the weights. K and V become fp16
+// and bf16 on the way, exactly: v_cvt_scalef32_pk takes a block's scale along, and 4 significant
+// bits fit both. Weights enter as two bf16, whatever their size: single ones of 8 or 11 bits would
+// be the largest error of the result, and fp16 would lose those below 2^-24 of the maximum, of
+// which a long context has many. That doubles the second product.
+//
+// What bounds it. A decode step reads 2 n_kv_heads head_dim bytes a position and uses each 4 times
+// for each query head of a group: HBM, and the matrix cores only because the vector units, with
+// e4m3 to convert and weights to make, would be slower than it (256 sequences of up to 2048
+// positions 1494 us there). 256 sequences 59 us for 283 MB, 54.5 at a large copy's rate; 3 of up to
+// 65001 positions 49 us for 242 MB. Prompts are bound by the vector units: a weight takes about 7
+// instructions (scale and subtract, exponential, sum, split), as many cycles as its 3 products, and
+// in the counters the vector and the matrix instructions together are some 90% of the steps'
+// cycles: 1507 rows behind 1494 positions, 32 heads of 64 dims, 65.7 us, 422 TFLOP/s of the
+// definition's two products.
+//
+// Two kernels: waves on their own for few columns (k_kv8_attention_few) and blocks that share K and
+// V through LDS for many. In both the work is cut into equal shares across the ends of sequences,
+// and a second launch joins what several workers have of one unit.
 #include <math.h>
 
 #include <type_traits>
@@ -19,26 +42,28 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 constexpr float kLog2e = 1.44269504088896341f;
 // Below it a rounded maximum (in log2 units) is less than 2^6 short of the exact one, which neither
-// weights nor sums mind; from there on exponents are made in two steps, and the largest weight is 1.
+// weights nor sums mind; from there on exponents are made in two steps, and the largest weight is
+// 1.
 constexpr float kLargeScore = 1073741824.0f;
 // A row's weights are relative to a maximum that gives way only to one larger by more than this (in
 // log2 units): they reach 2^kSlack, and sums are seldom rescaled.
 constexpr float kSlack = 8.0f;
-// What a unit's beginning costs, in steps. With 0 / 1 / 2 / 4, us: 48 sequences of up to 5 rows 41.1 /
-// 37.5 / 35.8 / 36.1, 1507 rows of one 68.2 / 68.5 / 67.5 / 72.0.
+// What a unit's beginning costs, in steps. With 0 / 1 / 2 / 4, us: 48 sequences of up to 5 rows
+// 41.1 / 37.5 / 35.8 / 36.1, 1507 rows of one 68.2 / 68.5 / 67.5 / 72.0.
 constexpr int kStart = 2;
-// Sequences of up to this many columns go by waves, in tiles of 32, where no sequence of the call has more;
-// us by waves and by blocks: 48 x 16 rows (64 columns) 58.5 and 67.5, 4 x 16 19.9 and 23.4, 48 x 24 rows
-// (96 columns) 82.7 and 74.0. Beside longer ones, up to kMixedColumns: blocks run anyhow, and the waves'
-// launch stands in front of theirs (20 x up to 100 rows, 46.7 us with 32 and 56.7 with 64).
+// Sequences of up to this many columns go by waves, in tiles of 32, where no sequence of the call
+// has more; us by waves and by blocks: 48 x 16 rows (64 columns) 58.5 and 67.5, 4 x 16 19.9 and
+// 23.4, 48 x 24 rows (96 columns) 82.7 and 74.0. Beside longer ones, up to kMixedColumns: blocks
+// run anyhow, and the waves' launch stands in front of theirs (20 x up to 100 rows, 46.7 us with 32
+// and 56.7 with 64).
 constexpr int kFewColumns = 64, kMixedColumns = 32;
-// From here on blocks of 8 waves and 256 columns: 1507 rows at 64 dims 74.0 -> 69.5 us, 500 rows at 128
-// dims 60.0 -> 53.8, 5 x 500 rows at 8000 positions 234 -> 206. Below, tiles of 128 columns leave fewer
-// waves without work (32 query heads on 8, us, both at 2000 positions: 250 rows 27.9 and 29.3, 100 rows
-// 21.7 and 25.4, 20 x up to 100 rows 46.0 and 54.2).
+// From here on blocks of 8 waves and 256 columns: 1507 rows at 64 dims 74.0 -> 69.5 us, 500 rows at
+// 128 dims 60.0 -> 53.8, 5 x 500 rows at 8000 positions 234 -> 206. Below, tiles of 128 columns
+// leave fewer waves without work (32 query heads on 8, us, both at 2000 positions: 250 rows 27.9
+// and 29.3, 100 rows 21.7 and 25.4, 20 x up to 100 rows 46.0 and 54.2).
 constexpr int kWideColumns = 1024;
-// Workers of a launch: a wave for each SIMD (256 sequences, us: 512 waves 92.1, 768 69.7, 1024 59.9, 1280
-// 77.0, 2048 62.0 with twice the parts to join), or as many blocks as give it two.
+// Workers of a launch: a wave for each SIMD (256 sequences, us: 512 waves 92.1, 768 69.7, 1024
+// 59.9, 1280 77.0, 2048 62.0 with twice the parts to join), or as many blocks as give it two.
 constexpr int kFewWorkers = 1024;
 template <int W>
 constexpr int kManyWorkers = 2048 / W;
@@ -79,8 +104,8 @@ __device__ __forceinline__ void split_rounded(float a, float b, uint32_t& hi, ui
   lo = __builtin_bit_cast(uint32_t, r);
 }
 
-// A unit that several workers share, as each of them notes it for the launch that joins its parts: one
-// that began before the worker's share and one that ends behind it.
+// A unit that several workers share, as each of them notes it for the launch that joins its parts:
+// one that began before the worker's share and one that ends behind it.
 struct Shared {
   int first, last;      // the teams; first > last: there is none
   int column, columns;  // of the tile, from the sequence's first row on
@@ -122,7 +147,8 @@ __device__ __forceinline__ Seq seq_of(const AttentionArgs& a, int s) {
   r1 = r1 > a.batch.n_rows ? a.batch.n_rows : r1;
   q.row0 = r0;
   q.columns = r1 > r0 ? (r1 - r0) * a.group : 0;
-  if (q.columns < a.least_columns || q.columns > a.most_columns) q.columns = 0;  // not this launch's
+  // none of another launch's
+  if (q.columns < a.least_columns || q.columns > a.most_columns) q.columns = 0;
   const long long table = (long long)a.batch.max_pages * kPage;
   q.limit = len < table ? len : table;
   return q;
@@ -138,8 +164,8 @@ __device__ __forceinline__ int blind_of(const AttentionArgs& a, const Seq& q) {
   const long long n = q.limit <= 0 ? q.columns : -q.before * a.group;
   return n <= 0 ? 0 : n < q.columns ? (int)n : q.columns;
 }
-// A step of units of C columns: 16 bytes of K and as many of V for each of a block's threads, or, of
-// the 64 of a wave, for each of 4 times.
+// A step of units of C columns: 16 bytes of K and as many of V for each of a block's threads, or,
+// of the 64 of a wave, for each of 4 times.
 template <int HD, int C>
 constexpr int kPages = (C > 128 ? 512 : 256) / HD;
 template <int HD, int C>
@@ -169,11 +195,12 @@ __device__ __forceinline__ Seq same(Seq q) {
   return q;
 }
 
-// How a launch's work is shared out. A kv head's units are the tiles of all sequences, one behind the
-// other; its ticks are cut into as many equal shares as there are teams, and a team has a worker for
-// each kv head. So the heads of a page, which lie beside one another in memory, are read at about the
-// same time (256 sequences: a worker with one head's units behind the other's, 63.1 us).
-// Worker t n_kv_heads + h is head h's of team t; workers are waves or blocks. By all 256 threads.
+// How a launch's work is shared out. A kv head's units are the tiles of all sequences, one behind
+// the other; its ticks are cut into as many equal shares as there are teams, and a team has a
+// worker for each kv head. So the heads of a page, which lie beside one another in memory, are read
+// at about the same time (256 sequences 63.1 -> 61.8 us). Worker t n_kv_heads + h is head h's of
+// team t; workers are waves or blocks. Who finds a share depends on how many sequences and tiles
+// there are: a wave's lanes for up to 256, else the block's threads.
 struct Share {
   int team, head, teams;
   int seq, tile;         // that hold the beginning of the team's share, and
@@ -189,7 +216,7 @@ struct Share {
     const long long wide = (each + 1) * more;
     return (int)(tick < wide ? divide(tick, each + 1) : more + divide(tick - wide, each));
   }
-  static __device__ __forceinline__ long long divide(long long a, long long b) {  // b > 0 where used
+  static __device__ __forceinline__ long long divide(long long a, long long b) {  // b > 0
     return (uint64_t)(a | b) >> 32 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
   }
   // all but the place of the beginning
@@ -207,8 +234,8 @@ struct Share {
   }
 };
 
-// The sum of the lanes up to each, by lane moves: within 16 lanes, then the rows in front (their last
-// lanes').
+// The sum of the lanes up to each, by lane moves: within 16 lanes, then the rows in front (their
+// last lanes').
 template <int CTRL, int ROWS = 0xF>  // 0 where there is no source lane, and in rows not named
 __device__ __forceinline__ long long dpp_i64(long long v) {
   const uint32_t lo =
@@ -268,9 +295,9 @@ __device__ __forceinline__ void find_tile(const AttentionArgs& a, Share& r, long
   r.at = (int)at;
 }
 
-// The beginnings of the shares of a block's WORKERS workers (4 waves, or the block): a thread sums the
-// ticks of a run of tiles, and the one whose run holds the beginning finds its place. Sequences of few
-// tiles are dealt out to the threads.
+// The beginnings of the shares of a block's WORKERS workers (4 waves, or the block): a thread sums
+// the ticks of a run of tiles, and the one whose run holds the beginning finds its place. Sequences
+// of few tiles are dealt out to the threads.
 template <int HD, int C, int WORKERS>
 __device__ __forceinline__ Share find_share_by_sequence(const AttentionArgs& a) {
   __shared__ int seq_[WORKERS];
@@ -311,8 +338,9 @@ __device__ __forceinline__ Share find_share_by_sequence(const AttentionArgs& a) 
   return r;
 }
 
-// The same by each wave for itself, with up to 256 sequences in its lanes: no barrier, and the found
-// one's rows come from its lane (one sequence 10.4 -> 9.4 us, 48 of up to 5 rows 35.3 -> 34.1).
+// The same by each wave for itself, with up to 256 sequences in its lanes: no barrier, and the
+// found one's rows come from its lane (one sequence 10.4 -> 9.4 us, 48 of up to 5 rows 35.3 ->
+// 34.1).
 template <int HD, int C>
 __device__ __forceinline__ Share find_share_by_lane(const AttentionArgs& a, int worker) {
   constexpr int N = 4;
@@ -358,7 +386,8 @@ __device__ __forceinline__ Share find_share_by_lane(const AttentionArgs& a, int 
 
 // One sequence of up to 256 tiles: a lane for each, 4 times (1507 rows 67.5 -> 65.7 us).
 template <int HD, int C>
-__device__ __forceinline__ Share find_share_of_one(const AttentionArgs& a, const Seq& q, int worker) {
+__device__ __forceinline__ Share find_share_of_one(const AttentionArgs& a, const Seq& q,
+                                                   int worker) {
   constexpr int N = 4;
   const int lane = threadIdx.x & 63, tiles = (q.columns + C - 1) / C;
   long long mine[N], upto[N], total = 0;
@@ -445,8 +474,8 @@ __device__ __forceinline__ Share find_share_by_tile(const AttentionArgs& a) {
   return r;
 }
 
-// x, or -inf where bit i is set: without a comparison's scalar registers, which a step has none to spare
-// of.
+// x, or -inf where bit i is set: without a comparison's scalar registers, which a step has none to
+// spare of.
 __device__ __forceinline__ float hide(float x, uint32_t bits, int i) {
   const uint32_t m = (uint32_t)__builtin_amdgcn_sbfe((int)bits, i, 1);
   return __builtin_bit_cast(float, (m & 0xFF800000u) | (~m & __builtin_bit_cast(uint32_t, x)));
@@ -467,12 +496,16 @@ __device__ __forceinline__ float max_of_quarters(float x) {
 // Units of few columns, a wave each. With C = 16 QT columns (rows x heads of the group) a step is
 //   S^T = K Q^T   (v_mfma_f32_16x16x32_f16; A: 16 positions of K, B: 16 columns of q)
 //   O^T += V^T P^T (.._bf16; A: 16 dims of V, B: the lane's own weights)
-// and no operand changes lanes: lane (n = l % 16, qd = l / 16) gets of S^T column n, positions 4 qd ..
-// 4 qd + 3 of each page, and those positions, of two pages, are its places in the second product's
-// contraction. K is loaded 16 bytes a lane (position n, dims 16 qd ..): the order of dims in the
-// contraction is free, and q is loaded in it too. V is loaded 4 (8) bytes for each of 4 positions;
-// dims 4 n .. become the rows n of 4 (8) products, so that a lane ends with 16 (32) dims in a row.
-// Weights enter as two bf16, high and low half: 16 significant bits at any exponent.
+// and no operand changes lanes: lane (n = l % 16, qd = l / 16) gets of S^T column n, positions 4 qd
+// .. 4 qd + 3 of each page, and those positions, of two pages, are its places in the second
+// product's contraction. K is loaded 16 bytes a lane (position n, dims 16 qd ..): the order of dims
+// in the contraction is free, and q is loaded in it too. V is loaded 4 (8) bytes for each of 4
+// positions; dims 4 n .. become the rows n of 4 (8) products, so that a lane ends with 16 (32) dims
+// in a row. Nothing goes through LDS and no wave waits for another. A step's K is loaded when the
+// last one's is used up and its V likewise, 8 KiB on the way for each SIMD; steps of twice the size
+// 59.8 -> 65.1 us (256 sequences), 50.5 -> 53.1 (3 long ones). Bound by HBM: 55 us of 256
+// sequences' 59 for 283 MB, the rest is the joining launch; of a single short sequence's 9.4 us 6.7
+// are the way from the lengths over the table and the scales to K and V, one load behind the other.
 template <int HD, int QT>
 __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArgs a) {
   constexpr int C = 16 * QT, KU = HD / 64, VW = HD / 64, PG = kPages<HD, C>, STEP = kStep<HD, C>;
@@ -600,9 +633,9 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
               }
             }
           };
-          // MORE: another step of the unit follows, whose K is loaded when this one's is used up, and its
-          // V likewise. (A load that may or may not happen would make the waits for those in front of
-          // it as strict as if it did not.)
+          // MORE: another step of the unit follows, whose K is loaded when this one's is used up,
+          // and its V likewise. (A load that may or may not happen would make the waits for those
+          // in front of it as strict as if it did not.)
           auto one_step = [&](int st, auto more) {
             constexpr bool MORE = decltype(more)::value;
             const bool edge = (st + 1) * STEP > see_min;  // some row does not see all of it
@@ -690,7 +723,8 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
             }
             if (edge) {
               // What no row sees is stale: zero. A NaN of a position that only some rows see would
-              // reach the others through their zero weights: it is taken out and handed to its rows.
+              // reach the others through their zero weights: it is taken out and handed to its
+              // rows.
               uint32_t odd = 0;
 #pragma unroll
               for (int p = 0; p < PG; ++p)
@@ -841,10 +875,11 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 }
 
 // Joins the parts of units: the one that a unit's first worker left (an odd slot) and those of the
-// workers behind it (even slots). Block (b, y) looks at the units that worker b has a part in, at the
-// y-th 256 of their tasks (a column's 4 dims). The n workers of a unit share them among their blocks,
-// in up to n / 4 slices, and a block deals the parts out over the threads that a slice leaves, which
-// meet in LDS.
+// workers behind it (even slots). Block (b, y) looks at the units that worker b has a part in, at
+// the y-th 256 of their tasks (a column's 4 dims). The n workers of a unit share them among their
+// blocks, in up to n / 4 slices, and a block deals the parts out over the threads that a slice
+// leaves, which meet in LDS. Bound by latency where rows are few, 2.7 us for one sequence and 4.6
+// for 256, and by the parts' bytes for prompts: 8 us for the 15 MB, written and read, of 1507 rows.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs a, int C) {
   constexpr int V = HD / 4;
@@ -911,12 +946,15 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
   }
 }
 
-// Units of many columns, a block each: 4 waves of 32 columns share the K and V of a step through LDS,
-// where they arrive as fp16 and bf16 (each wave converts a quarter). Per wave
+// Units of many columns, a block each: W = 4 or 8 waves of 32 columns share the K and V of a step
+// through LDS, where they arrive as fp16 and bf16 (each wave converts its part). Per wave
 //   S^T = K Q^T    (v_mfma_f32_32x32x16_f16; A: 32 positions of K, B: 32 columns of q)
 //   O^T += V^T P^T (.._bf16; A: 32 dims of V, B: the lane's own weights)
-// Lane l gets of S^T column l % 32, positions 8 (i / 4) + 4 (l / 32) + i % 4; V's positions lie in LDS
-// in the order in which that makes 8 of them a lane's share of a contraction.
+// Lane l gets of S^T column l % 32, positions 8 (i / 4) + 4 (l / 32) + i % 4; V's positions lie in
+// LDS in the order in which that makes 8 of them a lane's share of a contraction. Two buffers and a
+// barrier a step; the next but one's loads are on their way meanwhile. 1507 rows: 65.7 us, of which
+// a block is 2 on the way to its share, 3 on that to its first step's data, 47 in its 14 steps and
+// 2 writing parts; the joining launch and the gap in front of it take the rest.
 template <int HD, int W>
 __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const AttentionArgs a) {
   constexpr int C = 32 * W, PG = kPages<HD, C>, STEP = kStep<HD, C>, KT = STEP / 32, DT = HD / 32;
@@ -1065,8 +1103,8 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
           }
         };
         auto compute = [&](int st, int buf) {
-          // 4 pieces of K are on their way while 4 are multiplied: the compiler, left to itself, waits for
-          // each (1507 rows: 69.6 us, and 67.0 so)
+          // 4 pieces of K are on their way while 4 are multiplied: the compiler, left to itself,
+          // waits for each (1507 rows: 69.6 us, and 67.0 so)
           constexpr int G = 4, GROUPS = KT * (HD / 16) / G;
           f32x16 sc[KT];
           u32x4 kf[2][G];
@@ -1089,7 +1127,8 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
 #pragma unroll
             for (int j = 0; j < G; ++j) {
               const int u = (G * g + j) / KT, t = (G * g + j) % KT;
-              sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[g & 1][j]), qf[u], sc[t], 0, 0, 0);
+              sc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(as_h8(kf[g & 1][j]), qf[u], sc[t], 0,
+                                                             0, 0);
             }
           }
           if ((st + 1) * STEP > wave_min) {  // some row does not see all of it
@@ -1261,8 +1300,8 @@ int many_launch(AttentionArgs a, hipStream_t stream) {
 }
 
 // Sequences of up to kFewColumns columns go by waves, longer ones by blocks. One launch serves all
-// where max_rows, or a single sequence, says that there is one kind; more columns than were announced
-// are then several tiles.
+// where max_rows, or a single sequence, says that there is one kind; more columns than were
+// announced are then several tiles.
 template <int HD>
 int attention_launch(AttentionArgs a, int max_rows, hipStream_t stream) {
   const long long columns = (long long)max_rows * a.group;

@@ -10,19 +10,26 @@
 // greedy choice: a draft is accepted where it is the row's argmax, which is also the token. NaN
 // logits count as -inf; where +inf occurs, its places share all probability.
 //
-// Which token a random number falls on is settled at the borders of sums over 10^5 weights: what that
-// depends on, the row where a sequence ends, is done in 64 bits (exponentials, sums, comparisons).
-// Whether a draft stands compares two numbers: there the sums are 32-bit first, off by less than 2^-16,
-// and only a draft that is nearer than 2^-14 to the border has its rows summed again.
+// Which token a random number falls on is settled at the borders of sums over 10^5 weights: what
+// that depends on, the row where a sequence ends, is done in 64 bits (exponentials, sums,
+// comparisons). Whether a draft stands compares two numbers: there the sums are 32-bit first, off
+// by less than 2^-16, and only a draft that is nearer than 2^-14 to the border has its rows summed
+// again.
 //
 // Launches, none of which needs an order inside itself:
 //  1. every row (target and draft) in chunks of 8192 logits: maximum, its place where the choice is
-//     greedy, sum of weights relative to the chunk's maximum. A chunk is read once and kept in registers
-//     for the sum. This is the time of a large batch: 2 bytes a logit.
-//  2. where each sequence ends, found from 1 by each of its blocks; the sums of that row,
-//     in pieces of 4096.
+//     greedy, sum of weights relative to the chunk's maximum. A chunk is read once and kept in
+//     registers for the sum.
+//  2. where each sequence ends, found from 1 by each of its blocks, or in a launch of its own; the
+//     sums of that row, in pieces of 4096.
 //  3. with draft logits: the sums of max(p - q, 0) over the row's pieces.
 //  4. one block for each sequence: the piece that u2 falls into, the token in it, the outputs.
+//
+// What bounds it: 1 reads 2 bytes a logit (64 sequences of 5 rows, 128256 logits and a draft
+// model's: 31 us for 148 MB), 2 and 3 are 64-bit exponentials, some 19 instructions each, two for
+// each logit of 64 rows and twice (14 and 12 us), where sequences end takes 5 and 4 another 5.5;
+// 62.5 us in all. A single sequence is launches in a row: 5 rows of 32000 logits 12.5 us, of which
+// 3.3, 5.6 and 3.5 in the kernels.
 #include <math.h>
 
 #include "common.hpp"
@@ -32,8 +39,8 @@ namespace {
 
 constexpr int kThreads = 256, kVectors = 4;             // 16-byte vectors per thread of a chunk
 constexpr int kChunk = kThreads * kVectors * 8;         // logits per chunk
-// The drawn row goes in pieces of half a chunk: a few sequences give each SIMD more than one wave, and
-// pieces with a draft model's share, twice the work, spread over the CUs.
+// The drawn row goes in pieces of half a chunk: a few sequences give each SIMD more than one wave,
+// and pieces with a draft model's share, twice the work, spread over the CUs.
 constexpr int kPieceVectors = 2, kPiece = kThreads * kPieceVectors * 8;
 constexpr int kChooseThreads = kPiece / 8;              // one vector each
 constexpr double kLog2e = 1.44269504088896340736;
@@ -74,14 +81,14 @@ struct VerifyArgs {
   int* tokens;
   Stat* stats;    // [2][n_rows][chunks]: target, draft
   End* ends;      // [n_seqs]
-  double2* sums;  // [n_seqs][pieces]: of the target's weights (without a refused certain draft's), and
-                  // of the draft model's, or that draft's weight in its piece
+  double2* sums;  // [n_seqs][pieces]: of the target's weights (without a refused certain draft's),
+                  // and of the draft model's, or that draft's weight in its piece
   double* left;   // [n_seqs][pieces]: of max(p - q, 0)
   int n_rows, n_seqs, vocab, chunks, pieces;
 };
 
-// 2^y for y from -2^31 to 0, to 2^-40 of it: the whole part by the exponent, f of at most 1/2 by 1 + f g(f),
-// with the g of degree 7 whose largest error there is the least. 2^0 is 1 exactly.
+// 2^y for y from -2^31 to 0, to 2^-40 of it: the whole part by the exponent, f of at most 1/2 by 1
+// + f g(f), with the g of degree 7 whose largest error there is the least. 2^0 is 1 exactly.
 __device__ __forceinline__ double exp2_64(double y) {
   const double n = __builtin_rint(y), f = y - n;
   double p = 1.31789487561122369e-06;
@@ -96,9 +103,10 @@ __device__ __forceinline__ double exp2_64(double y) {
   return __builtin_ldexp(p, (int)n);
 }
 
-// The weight of a logit under a maximum above -inf. The distance goes to [-far, 0]: at -far it weighs
-// nothing, and a NaN logit, which counts as -inf, has it (the median of a NaN and two numbers is the
-// lower one). Under an infinite maximum, which stands as kFar, only its equals weigh, 1.
+// The weight of a logit under a maximum above -inf. The distance goes to [-far, 0]: at -far it
+// weighs nothing, and a NaN logit, which counts as -inf, has it (the median of a NaN and two
+// numbers is the lower one). Under an infinite maximum, which stands as kFar, only its equals
+// weigh, 1.
 __device__ __forceinline__ double weight(float l, float max, const Scale& by) {
   const float d = l - __builtin_fminf(max, kFar);
   return exp2_64((double)__builtin_amdgcn_fmed3f(d, -by.far, 0.0f) * by.k);
@@ -110,9 +118,9 @@ __device__ __forceinline__ Scale scale_of(float t) {
 }
 
 // The vectors of a row: element e of the row is element e + lead of the 16-byte aligned memory that
-// holds it; vector v of it is the row's elements 8 v - lead .. + 7. Those that the row does not fill
-// are read one by one; places outside the row count as -inf. Streamed loads: 64 x 5 rows with draft
-// logits 67.6 -> 65.8 us, 4 x 5 rows 22.8 -> 23.5.
+// holds it; vector v of it is the row's elements 8 v - lead .. + 7. Those that the row does not
+// fill are read one by one; places outside the row count as -inf. Streamed loads: 64 x 5 rows with
+// draft logits 67.6 -> 65.8 us, 4 x 5 rows 22.8 -> 23.5.
 struct Row {
   const f16* base;
   int lead, vocab;
@@ -134,8 +142,8 @@ __device__ __forceinline__ f16x8 load_vector(const Row& r, int v) {
   return x;
 }
 
-// Sums in 64 bits by lane moves (as wave_sum): over each 16 lanes, over the wave, and over a block of
-// WAVES waves; the same in every thread. shared: WAVES numbers.
+// Sums in 64 bits by lane moves (as wave_sum): over each 16 lanes, over the wave, and over a block
+// of WAVES waves; the same in every thread. shared: WAVES numbers.
 template <int CTRL, int ROWS = 0xF>  // 0 where there is no source lane, and in rows not named
 __device__ __forceinline__ double dpp_f64(double v) {
   const uint64_t b = __builtin_bit_cast(uint64_t, v);
@@ -217,8 +225,8 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
   const int chunk = blockIdx.x % a.chunks, which = blockIdx.x / a.chunks;
   const int draft = which >= a.n_rows, row = which - draft * a.n_rows;
   const Row r = row_of(draft ? a.draft_logits : a.logits, row, a.vocab);
-  // the row's sequence, found by halves: few loads, the same in every thread, in front of the logits'
-  // (behind them 64 x 5 rows took 69.4 us and not 67.6)
+  // the row's sequence, found by halves: few loads, the same in every thread, in front of the
+  // logits' (behind them 64 x 5 rows took 69.4 us and not 67.6)
   int s = row;
   if (a.starts) {
     int lo = 0, hi = a.n_seqs + 1;
@@ -270,9 +278,9 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sum = sum + ((float)x[j][e] == best ? 1.0f : 0.0f);
     } else {
-      // k and an exponent y are rounded, 2^-23 |y| in all and |y| <= 126 (smaller weights vanish), a
-      // weight by 2^-23, 32 of them and 8 parts in a sum: less than 2^-16 of the sum. k is neither 0
-      // nor infinite, so that 0 k is 0 and -inf k is -inf.
+      // k and an exponent y are rounded, 2^-23 |y| in all and |y| <= 126 (smaller weights vanish),
+      // a weight by 2^-23, 32 of them and 8 parts in a sum: less than 2^-16 of the sum. k is
+      // neither 0 nor infinite, so that 0 k is 0 and -inf k is -inf.
       const float k =
           __builtin_fminf(__builtin_fmaxf((float)(kLog2e / (double)t), 1.0e-37f), 3.0e38f);
 #pragma unroll
@@ -370,7 +378,8 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
       }
       double one = (double)u * (qw / qs), other = pw / p.sum;
       if (__builtin_fabs(one - other) < 6.103515625e-5 * __builtin_fmax(one, other)) {
-        if (qm > -INFINITY) one = (double)u * (qw / exact_sum(a.draft_logits, row, a.vocab, qm, z.by));
+        if (qm > -INFINITY)
+          one = (double)u * (qw / exact_sum(a.draft_logits, row, a.vocab, qm, z.by));
         other = pw / exact_sum(a.logits, row, a.vocab, p.max, z.by);
       }
       accept = one < other;
@@ -404,7 +413,8 @@ __device__ __forceinline__ int refused(const VerifyArgs& a, const End& z) {
 }
 
 // The draft row's logit at the place of each element of the target row's vector v.
-__device__ __forceinline__ f16x8 draft_vector(const VerifyArgs& a, size_t row, const Row& r, int v) {
+__device__ __forceinline__ f16x8 draft_vector(const VerifyArgs& a, size_t row, const Row& r,
+                                              int v) {
   const Row d = row_of(a.draft_logits, row, a.vocab);
   if (d.lead == r.lead) return load_vector(d, v);
   f16x8 x;
@@ -421,8 +431,8 @@ __global__ void __launch_bounds__(kThreads) k_verify_ends(const VerifyArgs a) {
 }
 
 // Block (piece and sequence, share): share 0 sums the target's weights, share 1 the draft model's.
-// FIND: where the sequence ends is found here, 4 us that few blocks spend at the same time; many would
-// spend them one behind the other.
+// FIND: where the sequence ends is found here, 4 us that few blocks spend at the same time; many
+// would spend them one behind the other.
 template <bool FIND>
 __global__ void __launch_bounds__(kThreads) k_verify_sums(const VerifyArgs a) {
   __shared__ double shared[4];
@@ -481,8 +491,8 @@ __device__ __forceinline__ double left_of(const Left& w, float l, float lq, int 
   if (at == w.odd) return 0.0;
   return w.qs == 0.0 ? p : __builtin_fmax(p * w.ps - weight(lq, w.qm, w.by) * w.qs, 0.0);
 }
-// By each wave for itself, 64 pieces at a time, without a barrier; first: the sums of piece `lane`, 0
-// where there is none.
+// By each wave for itself, 64 pieces at a time, without a barrier; first: the sums of piece `lane`,
+// 0 where there is none.
 __device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int s, double2 first) {
   Left w = {z.pm, z.qm, z.by, 1.0, 0.0, refused(a, z)};
   if (z.qm > -INFINITY) {
@@ -518,7 +528,7 @@ __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
 #pragma unroll
   for (int j = 0; j < kPieceVectors; ++j)
 #pragma unroll
-    for (int e = 0; e < 8; ++e)  // as left_of where the draft model has a share, without its branches
+    for (int e = 0; e < 8; ++e)  // as left_of where the draft model has a share, no branches
       sum = sum + __builtin_fmax(weight((float)x[j][e], w.pm, w.by) * w.ps -
                                      weight((float)y[j][e], w.qm, w.by) * w.qs,
                                  0.0);
@@ -550,8 +560,8 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
     last_any = -1;
   }
   Left w = left_from(a, z, s, first);
-  // Each wave looks for the piece by itself, a lane for each. Piece c's sum; with only_p of p alone, where
-  // p is nowhere above q.
+  // Each wave looks for the piece by itself, a lane for each. Piece c's sum; with only_p of p
+  // alone, where p is nowhere above q.
   const bool drafted = w.qs != 0.0, certain = w.odd >= 0;
   bool only_p = false;
   auto piece_sum = [&](int c) {
@@ -573,7 +583,8 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
     total = total_of();
   }
   const double aim = (double)u * total;
-  // the first piece that ends past the aim, or behind them all, by rounding, the last with any weight
+  // the first piece that ends past the aim, or behind them all, by rounding, the last with any
+  // weight
   int chosen = 0;
   double chosen_base = 0.0, before = 0.0;
   for (int c0 = 0; c0 < a.pieces; c0 += 64) {

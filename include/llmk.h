@@ -2,7 +2,7 @@
  * llmk.h - C-ABI of libllmk, the MI355X (gfx950) implementation of the non-GEMM layer kernels
  * of a Llama-style fp16 decoder: embedding gather, residual add, RMSNorm, fused residual add +
  * RMSNorm, RoPE with Llama-3 frequency scaling, SwiGLU, and the paged KV scatter (plain and
- * fused with RoPE).
+ * fused with RoPE); and of what stands around them, section by section below.
  *
  * Conventions shared by every entry point:
  *  - Tensors are device pointers owned by the caller; fp16 values travel as uint16_t bit
@@ -284,7 +284,8 @@ LLMK_API int llmk_decode_nongemm_pass_fused(const llmk_decode_pass* pass, void* 
 
 /* ------------------------------------------------------------------------------------------
  * Serving from an 8-bit KV cache: append, attention, read-back, and the verification of drafted
- * tokens. New entry points; the reference's cache is fp16 and it decodes one token at a time.
+ * tokens. New entry points; the reference's cache is fp16 and it decodes one token at a time. Their
+ * C++ names in llmk.hpp are these without the prefix.
  *
  * The cache: K and V pools [num_pages, n_kv_heads, 16, head_dim] of e4m3 bytes (OCP: largest 448, no
  * infinities) and their scales [num_pages, n_kv_heads], floats that are powers of two from 2^-15
@@ -340,7 +341,9 @@ LLMK_API size_t llmk_kv8_attention_workspace_floats(int head_dim);
  * has in this call; it only chooses kernels (more rows than that are slow, not wrong). `workspace`
  * (llmk_kv8_attention_workspace_floats(head_dim) floats, 16-byte aligned) lets the positions of a
  * batch be shared out evenly, with a second launch that joins their parts; NULL for contexts that are
- * short: every sequence then stays whole. Calls that may overlap need a workspace each. */
+ * short: every sequence then stays whole. Calls that may overlap need a workspace each; graphs that
+ * are replayed one behind the other may share one. n_kv_heads <= 512, n_heads <= 65535, rows times
+ * query heads of a group and table positions below 2^31 - 65536: LLMK_ERR_UNSUPPORTED past them. */
 LLMK_API int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, const float* k_scale,
                                 const uint8_t* v_pool, const float* v_scale,
                                 const int32_t* block_tables, const int32_t* row_starts,
@@ -368,8 +371,9 @@ LLMK_API size_t llmk_verify_drafts_workspace_floats(int n_rows, int n_seqs, int 
  * n_accepted [n_seqs]: drafts that stand. tokens [n_rows]: for each sequence those, the token, then
  * -1; -1 also for the token where a row has nothing above -inf.
  * workspace: 16-byte aligned; calls that may overlap need one each. drafts and accept_u may be NULL
- * with row_starts. Any vocab and alignment of logits (16-byte vectors throughout where vocab % 8 ==
- * 0). */
+ * with row_starts NULL. Any vocab and alignment of logits (16-byte vectors throughout where vocab %
+ * 8 == 0). LLMK_ERR_UNSUPPORTED where rows times 8192-logit chunks, twice, or sequences times
+ * 4096-logit pieces pass 2^31 - 1. */
 LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_logits,
                                 const int32_t* drafts, const int32_t* row_starts,
                                 const float* temperature, const float* accept_u,
