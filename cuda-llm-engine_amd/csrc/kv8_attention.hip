@@ -278,12 +278,6 @@ __device__ __forceinline__ Place place_of(long long mine) {
   return r;
 }
 
-// Tiles of a sequence: none where it has no rows here.
-template <int C>
-__device__ __forceinline__ int tiles_of(const AttentionArgs& a, int s) {
-  return (seq_of(a, s).columns + C - 1) / C;
-}
-
 // The tile of the share's sequence that holds a place in its ticks.
 template <int HD, int C>
 __device__ __forceinline__ void find_tile(const AttentionArgs& a, Share& r, long long at) {
@@ -879,7 +873,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 // the y-th 256 of their tasks (a column's 4 dims). The n workers of a unit share them among their
 // blocks, in up to n / 4 slices, and a block deals the parts out over the threads that a slice
 // leaves, which meet in LDS. Bound by latency where rows are few, 2.7 us for one sequence and 4.6
-// for 256, and by the parts' bytes for prompts: 8 us for the 15 MB, written and read, of 1507 rows.
+// for 256, and by the parts' bytes for prompts: 8 us for the 20 MB, written and read, of 1507 rows.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs a, int C) {
   constexpr int V = HD / 4;

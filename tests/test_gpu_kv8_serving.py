@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import _kv8 as ref
-from test_gpu_kv8 import (DEV, PAGE, Pools, attention_case, check_append, check_attention, dev, i32,
+from test_gpu_kv8 import (DEV, PAGE, Pools, attention_case, check_attention, dev, do_attention, i32,
                           inv_freq)
 
 pytestmark = pytest.mark.gpu
@@ -46,6 +46,31 @@ def test_long_prompts_among_hundreds_of_sequences(llmk):
     lens = counts + rng.integers(0, 30, 700)
     case = attention_case(74, (4, 1, 64), lens, counts, slack=1)
     check_attention(llmk, *case)
+
+
+@pytest.mark.parametrize("n", [64, 65, 200, 256, 257, 600])
+def test_batches_of_many_sequences(llmk, n):
+    """Shares are found by lanes up to 256 sequences and by threads past them: single rows, a few, and
+    a few beside more."""
+    rng = np.random.default_rng(n)
+    lens = rng.integers(0, 150, n)
+    check_attention(llmk, *attention_case(77, (4, 1, 64), lens))
+    counts = np.minimum(rng.integers(0, 5, n), lens)
+    check_attention(llmk, *attention_case(78, (4, 1, 128), lens, counts, slack=1))
+    counts[rng.integers(0, n, 5)] = 20
+    check_attention(llmk, *attention_case(79, (4, 1, 64), lens, counts))
+
+
+def test_a_prompt_of_more_tiles_than_a_wave_counts(llmk):
+    """One sequence of 67200 columns; some of its rows against the definition."""
+    heads, rows = 32, 2100
+    q, pools, tables, starts, lens = attention_case(80, (heads, 1, 64), [rows], [rows])
+    got = do_attention(llmk, q, pools, tables, starts, lens).astype(np.float64)
+    some = np.array([0, 1, 7, 8, 1000, 2040, 2047, 2048, 2098, 2099])
+    want, bound = ref.attention(q[some], pools.k, pools.v, np.repeat(tables, some.size, 0), None,
+                                some + 1)
+    assert (np.abs(got[some] - want) <= np.maximum(bound, 2.0 ** -60)).all()
+    assert np.isfinite(got).all()
 
 
 def test_long_prompts_with_scores_of_any_size(llmk):
