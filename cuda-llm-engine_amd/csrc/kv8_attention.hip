@@ -953,13 +953,18 @@ template <int HD, int W>
 __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const AttentionArgs a) {
   constexpr int C = 32 * W, PG = kPages<HD, C>, STEP = kStep<HD, C>, KT = STEP / 32, DT = HD / 32;
   constexpr int KP = HD / 16, VP = HD / 4;  // threads to a position of K, to 4 positions of V
-  // One piece of 16 bytes behind each row: 8 lanes that read a piece of as many rows meet no bank
-  // twice, and every address is a lane's base and a constant.
+  // One piece of 16 bytes behind each row: 16 lanes that read a piece of as many rows meet no bank
+  // twice, and every address is a lane's base and a constant. Rows change places within 16 so that
+  // neither do lanes that write: K's come 4 (2) at a time, and V's are 4 apart.
   __shared__ u32x4 k_lds[2][STEP][HD / 8 + 1];  // [position][8 dims]
   __shared__ u32x4 v_lds[2][HD][STEP / 8 + 1];  // [dim][8 positions]
   __shared__ int odd[2];  // a NaN was taken out of V: of a unit, and of the next
   const int tid = threadIdx.x, lane = tid & 63, n = lane & 31, half = lane >> 5;
   const int wave = same(tid >> 6), worker = blockIdx.x;
+  auto k_row = [](int key) {
+    return (key & ~15) | ((key & 2) << 2) | ((key & 12) >> 1) | (key & 1);
+  };
+  auto v_row = [](int d) { return (d & ~15) | ((d + (d >> 4)) & 15); };
   const bool shared_units = a.parts != nullptr;
   int turn = 0;
   if (tid < 2) odd[tid] = 0;
@@ -1034,7 +1039,10 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
         float ksc = 0, vsc = 0, ks = 0, vs = 0;
         u32x4 kr;
         uint32_t vr[4];
-        const int k_key = tid / KP, k_part = tid % KP, v_key = 4 * (tid / VP), v_part = tid % VP;
+        const int k_key = tid / KP, k_part = tid % KP, v_part = tid % VP;
+        // 4 positions of V; those of a wave fill both halves of a piece
+        const int vt = VP == 16 ? tid / VP : 4 * (wave / 2) + (wave & 1) + 2 * (lane / VP);
+        const int v_key = 4 * vt;
         auto load = [&](int st) {
           const int w = st * PG / 64;
           if (w != window) {
@@ -1065,7 +1073,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
             w[1] = __builtin_bit_cast(uint32_t, from_e4m3<true>(x, ks));
             w[2] = __builtin_bit_cast(uint32_t, from_e4m3<false>(y, ks));
             w[3] = __builtin_bit_cast(uint32_t, from_e4m3<true>(y, ks));
-            k_lds[buf][k_key][2 * k_part + j] = w;
+            k_lds[buf][k_row(k_key)][2 * k_part + j] = w;
           }
           if ((st + 1) * STEP > see_min) {
             // What no row sees is stale: zero. A NaN of a position that only some rows see would
@@ -1080,7 +1088,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
             }
             if (bad) odd[turn] = 1;
           }
-          const int t = v_key / 4, piece = 2 * (t / 4) + (t & 1);
+          const int piece = 2 * (vt / 4) + (vt & 1);
 #pragma unroll
           for (int g = 0; g < 2; ++g) {
             constexpr uint32_t sel[2] = {0x05010400u, 0x07030602u};
@@ -1092,7 +1100,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
               u32x2 y;
               y[0] = e ? bf16_from_e4m3<true>(x01, vs) : bf16_from_e4m3<false>(x01, vs);
               y[1] = e ? bf16_from_e4m3<true>(x23, vs) : bf16_from_e4m3<false>(x23, vs);
-              reinterpret_cast<u32x2*>(&v_lds[buf][d][piece])[(t >> 1) & 1] = y;
+              reinterpret_cast<u32x2*>(&v_lds[buf][v_row(d)][piece])[(vt >> 1) & 1] = y;
             }
           }
         };
@@ -1106,7 +1114,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
 #pragma unroll
             for (int j = 0; j < G; ++j) {
               const int u = (G * g + j) / KT, t = (G * g + j) % KT;
-              kf[g & 1][j] = k_lds[buf][32 * t + n][2 * u + half];
+              kf[g & 1][j] = k_lds[buf][32 * t + k_row(n)][2 * u + half];
             }
           };
 #pragma unroll
@@ -1181,7 +1189,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
             const bf16x8 lo = __builtin_bit_cast(bf16x8, (u32x4{pl[0], pl[1], pl[2], pl[3]}));
 #pragma unroll
             for (int d = 0; d < DT; ++d) {
-              const bf16x8 vf = __builtin_bit_cast(bf16x8, v_lds[buf][32 * d + n][2 * cc + half]);
+              const bf16x8 vf = __builtin_bit_cast(bf16x8, v_lds[buf][v_row(32 * d + n)][2 * cc + half]);
               acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, hi, acc[d], 0, 0, 0);
               acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo, acc[d], 0, 0, 0);
             }
