@@ -38,7 +38,7 @@ namespace llmk {
 namespace {
 
 constexpr int kThreads = 256, kVectors = 4;             // 16-byte vectors per thread of a chunk
-constexpr int kChunk = kThreads * kVectors * 8;         // logits per chunk
+constexpr int kChunk = 64 * kVectors * 8;               // logits per chunk, a wave's
 // The drawn row goes in pieces of half a chunk: a few sequences give each SIMD more than one wave,
 // and pieces with a draft model's share, twice the work, spread over the CUs.
 constexpr int kPieceVectors = 2, kPiece = kThreads * kPieceVectors * 8;
@@ -219,10 +219,11 @@ __device__ __forceinline__ void rows_of(const VerifyArgs& a, int s, int& first, 
 }
 
 __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
-  __shared__ float shared[4];
-  __shared__ int shared_at[4];
-  const int tid = threadIdx.x, wave = tid >> 6;
-  const int chunk = blockIdx.x % a.chunks, which = blockIdx.x / a.chunks;
+  const int lane = threadIdx.x & 63;
+  const unsigned unit =
+      kThreads / 64 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunk = unit % a.chunks, which = unit / a.chunks;
+  if (which >= (a.draft_logits ? 2 : 1) * a.n_rows) return;
   const int draft = which >= a.n_rows, row = which - draft * a.n_rows;
   const Row r = row_of(draft ? a.draft_logits : a.logits, row, a.vocab);
   // the row's sequence, found by halves: few loads, the same in every thread, in front of the
@@ -243,7 +244,7 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
   f16x8 x[kVectors];
 #pragma unroll
   for (int j = 0; j < kVectors; ++j)
-    x[j] = load_vector(r, (chunk * kVectors + j) * kThreads + tid);
+    x[j] = load_vector(r, (chunk * kVectors + j) * 64 + lane);
   const float t = a.temperature ? a.temperature[s] : 1.0f;
   const bool greedy = is_greedy(t);
   if (draft && greedy) return;
@@ -257,11 +258,6 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
 #pragma unroll
   for (int e = 1; e < 8; ++e) best = __builtin_fmaxf(best, (float)top[e]);
   best = wave_max(best);
-  if ((tid & 63) == 0) shared[wave] = best;
-  __syncthreads();
-  best = __builtin_fmaxf(__builtin_fmaxf(shared[0], shared[1]),
-                         __builtin_fmaxf(shared[2], shared[3]));
-  __syncthreads();
   float sum = 0.0f;
   int at = 0x7FFFFFFF;
   if (best > -INFINITY) {
@@ -271,7 +267,7 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
 #pragma unroll
         for (int e = 7; e >= 0; --e)
           if ((float)x[j][e] == best)
-            at = 8 * ((chunk * kVectors + j) * kThreads + tid) - r.lead + e;
+            at = 8 * ((chunk * kVectors + j) * 64 + lane) - r.lead + e;
     } else if (best == INFINITY) {
 #pragma unroll
       for (int j = 0; j < kVectors; ++j)
@@ -290,21 +286,12 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
           sum = sum + __builtin_amdgcn_exp2f(((float)x[j][e] - best) * k);
     }
   }
-  sum = llmk::wave_sum(sum);
-  at = wave_min(at);
-  if ((tid & 63) == 0) {
-    shared[wave] = sum;
-    shared_at[wave] = at;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    Stat out;
-    out.max = best;
-    out.sum = (shared[0] + shared[1]) + (shared[2] + shared[3]);
-    out.at = min(min(shared_at[0], shared_at[1]), min(shared_at[2], shared_at[3]));
-    out.pad = 0;
-    a.stats[(size_t)which * a.chunks + chunk] = out;
-  }
+  Stat out;
+  out.max = best;
+  out.sum = llmk::wave_sum(sum);
+  out.at = greedy ? wave_min(at) : at;
+  out.pad = 0;
+  if (lane == 0) a.stats[(size_t)which * a.chunks + chunk] = out;
 }
 
 // A row's maximum, its place and its sum of weights, from its chunks; by one wave.
@@ -698,7 +685,8 @@ extern "C" int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_
     return launch(k_verify_none, dim3(ceil_div((size_t)n_seqs, kThreads)), dim3(kThreads), 0, st,
                   n_accepted, n_seqs);
   const unsigned rows = (unsigned)n_rows * (a.draft_logits ? 2u : 1u);
-  int rc = launch(k_verify_stats, dim3((unsigned)chunks * rows), dim3(kThreads), 0, st, a);
+  int rc = launch(k_verify_stats, dim3(ceil_div((size_t)chunks * rows, kThreads / 64)),
+                  dim3(kThreads), 0, st, a);
   const unsigned per_piece = (unsigned)pieces * (unsigned)n_seqs;
   const dim3 shares(per_piece, a.draft_logits ? 2 : 1);
   // Blocks of the drawn rows' sums up to which they find the ends themselves. 5 rows a sequence,
