@@ -17,18 +17,19 @@
 // again.
 //
 // Launches, none of which needs an order inside itself:
-//  1. every row (target and draft) in chunks of 8192 logits: maximum, its place where the choice is
-//     greedy, sum of weights relative to the chunk's maximum. A chunk is read once and kept in
-//     registers for the sum.
+//  1. every row (target and draft) in chunks of 2048 logits, a wave each: maximum, its place where
+//     the choice is greedy, sum of weights relative to the chunk's maximum. A chunk is read once and
+//     kept in registers for the sum. (Chunks of a block, with barriers: 62.4 us in all below, not
+//     61.0; 2 or 4 chunks of a wave one behind the other, the next one's loads ahead, 65.)
 //  2. where each sequence ends, found from 1 by each of its blocks, or in a launch of its own; the
 //     sums of that row, in pieces of 4096.
 //  3. with draft logits: the sums of max(p - q, 0) over the row's pieces.
 //  4. one block for each sequence: the piece that u2 falls into, the token in it, the outputs.
 //
 // What bounds it: 1 reads 2 bytes a logit (64 sequences of 5 rows, 128256 logits and a draft
-// model's: 31 us for 148 MB), 2 and 3 are 64-bit exponentials, some 19 instructions each, two for
+// model's: 29.6 us for 148 MB), 2 and 3 are 64-bit exponentials, some 19 instructions each, two for
 // each logit of 64 rows and twice (14 and 12 us), where sequences end takes 5 and 4 another 5.5;
-// 62.5 us in all. A single sequence is launches in a row: 5 rows of 32000 logits 12.5 us, of which
+// 61.0 us in all. A single sequence is launches in a row: 5 rows of 32000 logits 12.5 us, of which
 // 3.3, 5.6 and 3.5 in the kernels.
 #include <math.h>
 
@@ -39,7 +40,7 @@ namespace {
 
 constexpr int kThreads = 256, kVectors = 4;             // 16-byte vectors per thread of a chunk
 constexpr int kChunk = 64 * kVectors * 8;               // logits per chunk, a wave's
-// The drawn row goes in pieces of half a chunk: a few sequences give each SIMD more than one wave,
+// The drawn row goes in pieces of 4096 logits: a few sequences give each SIMD more than one wave,
 // and pieces with a draft model's share, twice the work, spread over the CUs.
 constexpr int kPieceVectors = 2, kPiece = kThreads * kPieceVectors * 8;
 constexpr int kChooseThreads = kPiece / 8;              // one vector each
@@ -275,8 +276,8 @@ __global__ void __launch_bounds__(kThreads) k_verify_stats(const VerifyArgs a) {
         for (int e = 0; e < 8; ++e) sum = sum + ((float)x[j][e] == best ? 1.0f : 0.0f);
     } else {
       // k and an exponent y are rounded, 2^-23 |y| in all and |y| <= 126 (smaller weights vanish),
-      // a weight by 2^-23, 32 of them and 8 parts in a sum: less than 2^-16 of the sum. k is
-      // neither 0 nor infinite, so that 0 k is 0 and -inf k is -inf.
+      // a weight by 2^-23, 32 of them and 6 steps over lanes in a sum: less than 2^-16 of the sum.
+      // k is neither 0 nor infinite, so that 0 k is 0 and -inf k is -inf.
       const float k =
           __builtin_fminf(__builtin_fmaxf((float)(kLog2e / (double)t), 1.0e-37f), 3.0e38f);
 #pragma unroll

@@ -372,7 +372,7 @@ LLMK_API size_t llmk_verify_drafts_workspace_floats(int n_rows, int n_seqs, int 
  * -1; -1 also for the token where a row has nothing above -inf.
  * workspace: 16-byte aligned; calls that may overlap need one each. drafts and accept_u may be NULL
  * with row_starts NULL. Any vocab and alignment of logits (16-byte vectors throughout where vocab %
- * 8 == 0). LLMK_ERR_UNSUPPORTED where rows times 8192-logit chunks, twice, or sequences times
+ * 8 == 0). LLMK_ERR_UNSUPPORTED where rows times 2048-logit chunks, twice, or sequences times
  * 4096-logit pieces pass 2^31 - 1. */
 LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_logits,
                                 const int32_t* drafts, const int32_t* row_starts,
