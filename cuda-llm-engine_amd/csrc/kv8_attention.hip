@@ -69,6 +69,11 @@ template <int W>
 constexpr int kManyWorkers = 2048 / W;
 constexpr int kWorkers = 1024, kMostKvHeads = 512;  // at most
 constexpr int kSlotColumns = 131072;                // of partial results in the workspace
+// With tables of up to this many pages units stay whole, and nothing is joined. Us with units shared
+// and whole, one sequence, 64 of them and one of 5 rows: 192 positions of 64 dims 8.7 and 7.4, 11.5
+// and 9.0, 10.9 and 10.4 (256: 9.5 and 9.6, 11.6 and 9.8, 11.3 and 13.5); 128 of 128 dims 9.5 and
+// 8.7, 13.0 and 10.6, 12.0 and 12.1.
+constexpr int whole_pages(int head_dim) { return head_dim == 64 ? 12 : 8; }
 
 template <bool HIGH>
 __device__ __forceinline__ uint32_t bf16_from_e4m3(uint32_t bytes, float scale) {
@@ -1362,7 +1367,7 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
   a.v_pool = v_pool;
   a.v_scale = v_scale;
   a.out = reinterpret_cast<f16*>(out);
-  a.parts = workspace;
+  a.parts = max_pages > whole_pages(head_dim) ? workspace : nullptr;
   a.parts_ml = reinterpret_cast<float2*>(workspace + (size_t)kSlotColumns * head_dim);
   a.shared = reinterpret_cast<Shared*>(workspace + (size_t)kSlotColumns * (head_dim + 2));
   a.n_heads = n_heads;
