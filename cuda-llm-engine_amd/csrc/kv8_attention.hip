@@ -17,7 +17,7 @@
 // 65001 positions 49 us for 242 MB. Prompts are bound by the vector units: a weight takes about 7
 // instructions (scale and subtract, exponential, sum, split), as many cycles as its 3 products, and
 // in the counters the vector and the matrix instructions together are some 90% of the steps'
-// cycles: 1507 rows behind 1494 positions, 32 heads of 64 dims, 65.7 us, 422 TFLOP/s of the
+// cycles: 1507 rows behind 1494 positions, 32 heads of 64 dims, 65 us, 427 TFLOP/s of the
 // definition's two products.
 //
 // Two kernels: waves on their own for few columns (k_kv8_attention_few) and blocks that share K and
@@ -951,7 +951,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
 //   O^T += V^T P^T (.._bf16; A: 32 dims of V, B: the lane's own weights)
 // Lane l gets of S^T column l % 32, positions 8 (i / 4) + 4 (l / 32) + i % 4; V's positions lie in
 // LDS in the order in which that makes 8 of them a lane's share of a contraction. Two buffers and a
-// barrier a step; the next but one's loads are on their way meanwhile. 1507 rows: 65.7 us, of which
+// barrier a step; the next but one's loads are on their way meanwhile. 1507 rows: 65 us, of which
 // a block is 2 on the way to its share, 3 on that to its first step's data, 47 in its 14 steps and
 // 2 writing parts; the joining launch and the gap in front of it take the rest.
 template <int HD, int W>
