@@ -63,16 +63,19 @@ constexpr int kFewColumns = 64, kMixedColumns = 32;
 // and 29.3, 100 rows 21.7 and 25.4, 20 x up to 100 rows 46.0 and 54.2).
 constexpr int kWideColumns = 1024;
 // Workers of a launch: a wave for each SIMD (256 sequences, us: 512 waves 92.1, 768 69.7, 1024
-// 59.9, 1280 77.0, 2048 62.0 with twice the parts to join), or as many blocks as give it two.
-constexpr int kFewWorkers = 1024;
+// 59.9, 1280 77.0, 2048 62.0 with twice the parts to join), or as many blocks as give it two. Two
+// waves where each finds a unit of 16 columns or more of them and tables are of up to kShortPages
+// pages, so that units are many and their beginnings the most of it: 256 sequences of up to 180,
+// 300, 600 and 1000 positions 18.4 -> 16.8, 22.9 -> 21.7, 28.8 -> 27.7 and 36.4 -> 36.6 us.
+constexpr int kFewWorkers = 1024, kShortPages = 40;
 template <int W>
 constexpr int kManyWorkers = 2048 / W;
-constexpr int kWorkers = 1024, kMostKvHeads = 512;  // at most
+constexpr int kWorkers = 2048, kMostKvHeads = 512;  // at most
 constexpr int kSlotColumns = 131072;                // of partial results in the workspace
-// With tables of up to this many pages units stay whole, and nothing is joined. Us with units shared
-// and whole, one sequence, 64 of them and one of 5 rows: 192 positions of 64 dims 8.7 and 7.4, 11.5
-// and 9.0, 10.9 and 10.4 (256: 9.5 and 9.6, 11.6 and 9.8, 11.3 and 13.5); 128 of 128 dims 9.5 and
-// 8.7, 13.0 and 10.6, 12.0 and 12.1.
+// With tables of up to this many pages units stay whole, and nothing is joined. Us with units
+// shared and whole, one sequence, 64 of them and one of 5 rows: 192 positions of 64 dims 8.7 and
+// 7.4, 11.5 and 9.0, 10.9 and 10.4 (256: 9.5 and 9.6, 11.6 and 9.8, 11.3 and 13.5); 128 of 128 dims
+// 9.5 and 8.7, 13.0 and 10.6, 12.0 and 12.1.
 constexpr int whole_pages(int head_dim) { return head_dim == 64 ? 12 : 8; }
 
 template <bool HIGH>
@@ -1292,7 +1295,9 @@ int join_launch(const AttentionArgs& a, int columns, hipStream_t stream) {
 
 template <int HD, int QT>
 int few_launch(AttentionArgs a, hipStream_t stream) {
-  a.workers = kFewWorkers;
+  const bool two = QT == 1 && a.batch.max_pages <= kShortPages &&
+                   (long long)a.batch.n_seqs * a.n_kv_heads >= 2 * kFewWorkers;
+  a.workers = two ? 2 * kFewWorkers : kFewWorkers;
   const int st =
       launch(k_kv8_attention_few<HD, QT>, dim3(a.workers / 4), dim3(256), 0, stream, a);
   return st != LLMK_OK ? st : join_launch<HD>(a, 16 * QT, stream);

@@ -61,6 +61,14 @@ def test_batches_of_many_sequences(llmk, n):
     check_attention(llmk, *attention_case(79, (4, 1, 64), lens, counts))
 
 
+@pytest.mark.parametrize("longest", [90, 250, 640])
+def test_more_units_than_simds_under_narrow_tables(llmk, longest):
+    """2400 pairs of a sequence and a kv head: whole, shared among two waves a SIMD, among one."""
+    lens = np.random.default_rng(longest).integers(0, 60, 300)
+    lens[7] = longest
+    check_attention(llmk, *attention_case(81, (8, 8, 64), lens))
+
+
 def test_a_prompt_of_more_tiles_than_a_wave_counts(llmk):
     """One sequence of 67200 columns; some of its rows against the definition."""
     heads, rows = 32, 2100
