@@ -239,15 +239,17 @@ def _load_fast_calls():
     the checks below have to decide."""
     import importlib.machinery
     import importlib.util
-    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # torch without a GPU: none
+    # torch without a GPU has neither; of a torch that is not initialised yet no tensor is on a GPU
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    device = getattr(torch._C, "_cuda_getDevice", None)
     for suffix in importlib.machinery.EXTENSION_SUFFIXES:
         path = os.path.join(_HERE, "_fast_calls" + suffix)
-        if os.path.exists(path) and raw_stream is not None:
+        if os.path.exists(path) and raw_stream is not None and device is not None:
             spec = importlib.util.spec_from_file_location("_fast_calls", path)
             mod = importlib.util.module_from_spec(spec)
             spec.loader.exec_module(mod)
             mod.setup(torch.Tensor, torch.float16, torch.int32, torch.float32,
-                      torch.cuda.current_device, raw_stream, torch.float8_e4m3fn)
+                      device, raw_stream, torch.float8_e4m3fn)
             return mod
     return _NoFastCalls()
 

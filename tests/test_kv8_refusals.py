@@ -111,7 +111,9 @@ def test_verify(llmk):
     assert verify(L, n_rows=2 ** 30, vocab=128256) == E.LLMK_ERR_UNSUPPORTED
     assert verify(L, vocab=2 ** 31 - 1) == E.LLMK_ERR_UNSUPPORTED
     assert E.verify_drafts_workspace_floats(0, 1, 8) == 0
-    assert E.verify_drafts_workspace_floats(5, 1, 128256) == 12 + 16 * 2 * 5 * 4 + 32 * 6
+    # 63 chunks of 2048 logits and 32 pieces of 4096: where a sequence ends, chunks of both models' rows
+    # (16 bytes), sums of pieces (24 bytes)
+    assert E.verify_drafts_workspace_floats(5, 1, 128256) == 12 + 63 * 2 * 5 * 4 + 32 * 6
 
 
 def test_python_face_refuses_host_tensors(llmk):
