@@ -1,11 +1,13 @@
 // Writing and reading the 8-bit KV cache (layout: kv8.hpp): the append of a pass's keys and values
 // with the rotation of q and k on the way, and the read-back of cached rows as fp16.
 //
-// Append. The rotation of row at position pos, pair i < head_dim / 2 (element i with element
-// i + head_dim / 2): angle = pos * inv_freq[i] in 64 bits, c and s its cosine and sine in 32,
-// x1' = x1 c - x2 s, x2' = x2 c + x1 s in 32 bits. q is rounded once, to fp16; k and v once, to
-// e4m3 under the scale of their block. For the rows of the call that fall into one block (a page
-// and kv head, K or V):
+// Append. The rotation of row at position pos, pair i < head_dim / 2 (element i with element i +
+// head_dim / 2): angle = pos * inv_freq[i], c and s its cosine and sine, x1' = x1 c - x2 s, x2' =
+// x2 c + x1 s. For k all of it is in 64 bits, so that its e4m3 codes, of which ties are close, are
+// those of the definition (in 32 bits single ones are their neighbours: 28.6 and not 29.6 us for
+// the prompts below, with read-back); for q c and s are rounded to 32 bits, the rest is done in
+// them and rounded to fp16. k and v are rounded once, to e4m3 under the scale of their block. For
+// the rows of the call that fall into one block (a page and kv head, K or V):
 //   most  = the largest finite magnitude among them;
 //   e     = the least exponent in [-15, 7] with most <= 448 * 2^e, or the block's own if that is
 //           larger and the block holds tokens already (the first slot written is not its slot 0);
@@ -20,10 +22,10 @@
 // rows. So a window makes 16 to 32 such tasks whether it holds one prompt's rows or a decode
 // step's, nothing is read twice, and the maximum is a few lane exchanges.
 //
-// What bounds it: HBM for prompts, where 5 of up to 2001 rows take 21.7 us for 81 MB, 15.6 at a
+// What bounds it: HBM for prompts, where 5 of up to 2001 rows take 22.4 us for 81 MB, 15.6 at a
 // large copy's rate (a block's leaders, angles and maxima stand in front of its writes); for a
-// decode step the way from the row starts over the lengths and tables to the scales, 4.1 us for one
-// row and 6.5 for 256 of them (2.6 MB). A grid of one block for each row and head took 21.7 us
+// decode step the way from the row starts over the lengths and tables to the scales, 4.2 us for one
+// row and 6.3 for 256 of them (2.6 MB). A grid of one block for each row and head took 21.7 us
 // there, with read-back, and not 10.3.
 #include <math.h>
 
@@ -35,26 +37,44 @@ namespace {
 
 using namespace kv8;
 
-// Cosine and sine of an angle in 64 bits, to 32. The quarter turns are taken off in 64 bits (the
-// angles of far positions lose their fraction in 32); what is left, at most pi / 4, goes through
-// the series of both, which end below 2^-29 there.
-__device__ __forceinline__ f32x2 cos_sin(double angle) {
+// Cosine and sine of an angle, in 64 bits: the quarter turns are taken off in two parts (the angles
+// of far positions lose their fraction in 32 bits), and what is left, at most pi / 4, goes through
+// the series of both, which end below 2^-48 there.
+__device__ __forceinline__ double2 cos_sin(double angle) {
   const double k = __builtin_rint(angle * 0.63661977236758134308);
-  double rest = __builtin_fma(-k, 1.57079632679489655800, angle);
-  rest = __builtin_fma(-k, 6.12323399573676603587e-17, rest);
-  const float r = (float)rest, z = r * r;
-  float s = __builtin_fmaf(z, 2.75573192e-6f, -1.98412698e-4f);
-  s = __builtin_fmaf(z, s, 8.33333333e-3f);
-  s = __builtin_fmaf(z, s, -1.66666667e-1f);
-  s = __builtin_fmaf(r * z, s, r);
-  float c = __builtin_fmaf(z, -2.75573192e-7f, 2.48015873e-5f);
-  c = __builtin_fmaf(z, c, -1.38888889e-3f);
-  c = __builtin_fmaf(z, c, 4.16666667e-2f);
-  c = __builtin_fmaf(z, c, -0.5f);
-  c = __builtin_fmaf(z, c, 1.0f);
+  double r = __builtin_fma(-k, 1.57079632679489655800, angle);
+  r = __builtin_fma(-k, 6.12323399573676603587e-17, r);
+  const double z = r * r;
+  double s = -7.6471637318198164759e-13;  // (-1)^i / (2 i + 1)!, from i = 7 on down
+  s = __builtin_fma(s, z, 1.6059043836821614599e-10);
+  s = __builtin_fma(s, z, -2.5052108385441718775e-08);
+  s = __builtin_fma(s, z, 2.7557319223985890653e-06);
+  s = __builtin_fma(s, z, -1.9841269841269841270e-04);
+  s = __builtin_fma(s, z, 8.3333333333333333333e-03);
+  s = __builtin_fma(s, z, -1.6666666666666666667e-01);
+  s = __builtin_fma(r * z, s, r);
+  double c = -1.1470745597729724714e-11;  // (-1)^i / (2 i)!
+  c = __builtin_fma(c, z, 2.0876756987868098979e-09);
+  c = __builtin_fma(c, z, -2.7557319223985890653e-07);
+  c = __builtin_fma(c, z, 2.4801587301587301587e-05);
+  c = __builtin_fma(c, z, -1.3888888888888888889e-03);
+  c = __builtin_fma(c, z, 4.1666666666666666667e-02);
+  c = __builtin_fma(c, z, -0.5);
+  c = __builtin_fma(c, z, 1.0);
   const int q = (int)k & 3;
-  const float cq = (q & 1) ? s : c, sq = (q & 1) ? c : s;
-  return f32x2{q == 1 || q == 2 ? -cq : cq, q >= 2 ? -sq : sq};
+  const double cq = (q & 1) ? s : c, sq = (q & 1) ? c : s;
+  return make_double2(q == 1 || q == 2 ? -cq : cq, q >= 2 ? -sq : sq);
+}
+
+// x to 32 bits such that a later rounding to fewer than 23 is that of x itself, and so are
+// comparisons with numbers of as few: the bits that do not fit are cut off, and where any was set
+// the last one that does is set, too. They are the low 29 of the low half; infinities have none,
+// and NaN stays NaN.
+__device__ __forceinline__ float to_odd(double x) {
+  const uint64_t b = __builtin_bit_cast(uint64_t, x);
+  const uint32_t lo = (uint32_t)b;
+  const uint32_t cut = (((lo & 0x1FFFFFFFu) + 0x1FFFFFFFu) | lo) & 0xE0000000u;
+  return (float)__builtin_bit_cast(double, (b & 0xFFFFFFFF00000000ull) | cut);
 }
 
 struct AppendArgs {
@@ -73,7 +93,7 @@ template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a, int kv_blocks) {
   constexpr int HALF = HD / 2, P = HD / 16;  // P pieces of a row: elements 8 p .. and HALF + 8 p ..
   constexpr int J = P * kPage / 64;          // rows of a lane where a page gets all 16
-  __shared__ f32x2 turn[2 * kWindow][HALF];  // of the window's rows and what its last one leads
+  __shared__ double2 turn[2 * kWindow][HALF];  // of the window's rows and what its last one leads
   __shared__ int seq_of[kWindow], lead[kWindow], slot_of[kWindow], tasks_before[kWindow + 1];
   __shared__ long long pos_of[kWindow];
   __shared__ size_t page_of[kWindow];
@@ -138,10 +158,10 @@ __global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a, int kv_b
       f16x8 y1, y2;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const f32x2 cs = turn[r][p * 8 + e];
-        const float u = (float)x1[e], w = (float)x2[e];
-        y1[e] = in_table ? (f16)(u * cs.x - w * cs.y) : (f16)0;
-        y2[e] = in_table ? (f16)(w * cs.x + u * cs.y) : (f16)0;
+        const double2 cs = turn[r][p * 8 + e];
+        const float u = (float)x1[e], w = (float)x2[e], c = (float)cs.x, s = (float)cs.y;
+        y1[e] = in_table ? (f16)(u * c - w * s) : (f16)0;
+        y2[e] = in_table ? (f16)(w * c + u * s) : (f16)0;
       }
       f16* dst = a.q_out + row * a.n_heads * HD + at;
       st16(dst, as_u4(y1));
@@ -186,9 +206,9 @@ __global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a, int kv_b
       for (int e = 0; e < 8; ++e) {
         const float u = (float)x1[e], w = (float)x2[e];
         if (side == 0) {
-          const f32x2 cs = turn[g + r][8 * p + e];
-          x[j][e] = u * cs.x - w * cs.y;
-          x[j][8 + e] = w * cs.x + u * cs.y;
+          const double2 cs = turn[g + r][8 * p + e];
+          x[j][e] = to_odd(__builtin_fma((double)u, cs.x, -((double)w * cs.y)));
+          x[j][8 + e] = to_odd(__builtin_fma((double)w, cs.x, (double)u * cs.y));
         } else {
           x[j][e] = u;
           x[j][8 + e] = w;

@@ -305,9 +305,9 @@ LLMK_API int llmk_decode_nongemm_pass_fused(const llmk_decode_pass* pass, void* 
 /* Appends the rows' keys and values, the keys rotated, and rotates their queries. Row r of qkv
  * (stride ld elements) holds q [n_heads, head_dim], k [n_kv_heads, head_dim] and v behind one
  * another, as llmk_qkv_rope_scatter's; q_out [n_rows, n_heads, head_dim] must not overlap it.
- * Rotation as llmk_rope_apply, but unrounded on the way: angles position * inv_freq in 64 bits,
- * cosine, sine and products in 32, then q rounded once to fp16, k and v once to e4m3 (q of a row
- * at a position that is nowhere is zero).
+ * Rotation as llmk_rope_apply, but unrounded on the way: angles position * inv_freq, cosine and sine in
+ * 64 bits; k's products in them, too, and one rounding to e4m3; q's in 32 and one rounding to fp16; v is
+ * rounded once to e4m3 (q of a row at a position that is nowhere is zero).
  * The scale of a block (page and kv head): the least 2^e, e from -15 to 7, with most <= 448 * 2^e for
  * most the largest finite magnitude of the call's rows in it. Where the first of them is not the
  * page's token 0, the scale is not lowered, and if it grows the tokens in front are rounded again to

@@ -5,8 +5,8 @@ import pytest
 import torch
 
 import _kv8 as ref
-from test_gpu_kv8 import (DEV, PAGE, Pools, attention_case, check_attention, dev, do_attention, i32,
-                          inv_freq)
+from test_gpu_kv8 import (DEV, PAGE, Pools, attention_case, check_attention, dev, do_append, do_attention,
+                          i32, inv_freq)
 
 pytestmark = pytest.mark.gpu
 
@@ -108,6 +108,27 @@ def test_more_kv_heads_than_wide_blocks(llmk, n_kv):
     """max_rows announces a long prompt where a launch has fewer such blocks than kv heads."""
     case = attention_case(76, (n_kv, n_kv, 64), [37, 20], [3, 2])
     check_attention(llmk, *case, max_rows=2000)
+
+
+@pytest.mark.parametrize("n_kv,dim", [(8, 64), (4, 128)])
+def test_keys_are_the_nearest_to_the_definition(llmk, n_kv, dim):
+    """Two million rotated keys, at near and far positions: every code that of the 64-bit value."""
+    rng = np.random.default_rng(82)
+    for first in (0, 120000):
+        rows = 4000
+        lens = np.array([first + rows])
+        tables = np.zeros((1, (first + rows + 15) // 16), np.int32)
+        tables[0, first // 16:] = rng.permutation(rows // 16)
+        pools = Pools(rows // 16, n_kv, dim)
+        qkv = (rng.standard_normal((rows, (1 + 2 * n_kv) * dim))
+               * np.exp(rng.standard_normal((rows, 1)))).astype(np.float16)
+        inv = inv_freq(llmk, dim)
+        starts = np.array([0, rows])
+        do_append(llmk, pools, qkv, tables, starts, lens, inv, (1, n_kv, dim))
+        ref.append(pools.k, pools.v, qkv, tables, starts, lens, inv, 1, n_kv, dim)
+        for side, c in enumerate((pools.k, pools.v)):
+            assert np.array_equal(pools.scale(side), c.scale)
+            assert np.array_equal(pools.codes(side), c.codes)
 
 
 # ---------------------------------------------------------------------------------------------
