@@ -112,6 +112,26 @@ __device__ __forceinline__ void split_rounded(float a, float b, uint32_t& hi, ui
   lo = __builtin_bit_cast(uint32_t, r);
 }
 
+// A running sum of the steps' sums of weights that takes along what each addition lost. A worker may
+// walk a unit of 10^5 positions by itself, and equal weights added pair by pair lose the same way
+// each time: 2^-11 of the sum at 131072 positions, as much as the result's own rounding. So it is
+// the 32 additions of a step at most that count, less than 2^-20. O has no such help: a position's
+// value is one of 32 (16) in a sum that the matrix cores add twice, so it may be off by 2^-28
+// (2^-27) of itself for each position, where weights and values are all equal: past 2^-11.5 there at
+// 131072 positions, and 2^-18 with weights that differ.
+struct Sum {
+  float of, lost;
+  __device__ __forceinline__ void add(float x) {
+    const float y = x - lost, next = of + y;
+    lost = (next - of) - y;
+    of = next;
+  }
+  __device__ __forceinline__ void scale(float by) {
+    of = of * by;
+    lost = lost * by;
+  }
+};
+
 // A unit that several workers share, as each of them notes it for the launch that joins its parts:
 // one that began before the worker's share and one that ends behind it.
 struct Shared {
@@ -570,11 +590,12 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
             qf[t][u] = own ? as_h8(ld16(src + 64 * (u / 2) + 8 * (u % 2))) : (f16x8)(f16)0;
         }
         f32x4 acc[QT][4 * VW];
-        float m[QT], l[QT];
+        float m[QT];
+        Sum l[QT];
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           m[t] = -INFINITY;
-          l[t] = 0.0f;
+          l[t] = Sum{0.0f, 0.0f};
 #pragma unroll
           for (int c = 0; c < 4 * VW; ++c) acc[t][c] = f32x4{0, 0, 0, 0};
         }
@@ -697,7 +718,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
               const float ref = next == -INFINITY ? 0.0f : next;
               if (__builtin_amdgcn_ballot_w64(next != m[t])) {
                 const float corr = __builtin_amdgcn_exp2f(m[t] - ref);
-                l[t] = l[t] * corr;
+                l[t].scale(corr);
 #pragma unroll
                 for (int c = 0; c < 4 * VW; ++c) acc[t][c] = acc[t][c] * corr;
                 m[t] = next;
@@ -711,6 +732,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                   asm volatile("" : "+v"(sc[t][p]));
                 }
               }
+              float sum = 0.0f;
 #pragma unroll
               for (int p = 0; p < PG; ++p)
 #pragma unroll
@@ -719,9 +741,10 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
                       __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][p][i], scale, -ref));
                   const float w1 =
                       __builtin_amdgcn_exp2f(__builtin_fmaf(sc[t][p][i + 1], scale, -ref));
-                  l[t] = l[t] + (w0 + w1);
+                  sum = sum + (w0 + w1);
                   split_rounded(w0, w1, ph[t][p][i / 2], pl[t][p][i / 2]);
                 }
+              l[t].add(sum);
             }
             if (edge) {
               // What no row sees is stale: zero. A NaN of a position that only some rows see would
@@ -829,7 +852,7 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
         const size_t slot = 2 * (size_t)worker + side;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-          float sum = l[t] + __shfl_xor(l[t], 16);
+          float sum = l[t].of + __shfl_xor(l[t].of, 16);
           sum = sum + __shfl_xor(sum, 32);
           const int c = 16 * t + n;
           if (c >= columns) continue;
@@ -1034,7 +1057,8 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
       f16x8 qf[HD / 16];
 #pragma unroll
       for (int u = 0; u < HD / 16; ++u) qf[u] = own ? as_h8(ld16(src + 16 * u)) : (f16x8)(f16)0;
-      float m = -INFINITY, l = 0.0f;
+      float m = -INFINITY;
+      Sum sum = {0.0f, 0.0f};
       f32x16 acc[DT];
 #pragma unroll
       for (int d = 0; d < DT; ++d)
@@ -1163,7 +1187,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
           const float ref = next == -INFINITY ? 0.0f : next;
           if (__builtin_amdgcn_ballot_w64(next != m)) {
             const float corr = __builtin_amdgcn_exp2f(m - ref);
-            l = l * corr;
+            sum.scale(corr);
 #pragma unroll
             for (int d = 0; d < DT; ++d)
 #pragma unroll
@@ -1180,6 +1204,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
               asm volatile("" : "+v"(sc[t]));
             }
           }
+          float of_step = 0.0f;
 #pragma unroll
           for (int cc = 0; cc < 2 * KT; ++cc) {  // 16 positions
             uint32_t ph[4], pl[4];
@@ -1190,7 +1215,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
                   __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc / 2][i], scale, -ref));
               const float w1 =
                   __builtin_amdgcn_exp2f(__builtin_fmaf(sc[cc / 2][i + 1], scale, -ref));
-              l = l + (w0 + w1);
+              of_step = of_step + (w0 + w1);
               split_cut(w0, w1, ph[e], pl[e]);
             }
             const bf16x8 hi = __builtin_bit_cast(bf16x8, (u32x4{ph[0], ph[1], ph[2], ph[3]}));
@@ -1202,6 +1227,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
               acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf, lo, acc[d], 0, 0, 0);
             }
           }
+          sum.add(of_step);
         };
         load(step);
         lds_barrier();  // the unit before is done with
@@ -1246,7 +1272,7 @@ __global__ void __launch_bounds__(64 * W, 2) k_kv8_attention_many(const Attentio
         const long long end = pos + ticks - upto, begin = end - steps;
         note(side, sh.team_at(begin), sh.team_at(end - 1), c0, columns, q);
       }
-      l = l + __shfl_xor(l, 32);
+      const float l = sum.of + __shfl_xor(sum.of, 32);
       if (own && whole) {
         f16* dst = a.out + ((size_t)(q.row0 + col / a.group) * a.n_heads + h * a.group +
                             col % a.group) * HD + 4 * half;
