@@ -28,6 +28,7 @@
 #include <type_traits>
 
 #include "kv8.hpp"
+#include "kv8_shared.hpp"
 
 namespace llmk {
 namespace {
@@ -130,15 +131,6 @@ struct Sum {
     of = of * by;
     lost = lost * by;
   }
-};
-
-// A unit that several workers share, as each of them notes it for the launch that joins its parts:
-// one that began before the worker's share and one that ends behind it.
-struct Shared {
-  int first, last;      // the teams; first > last: there is none
-  int column, columns;  // of the tile, from the sequence's first row on
-  int row0, blind;      // the sequence's first row; columns in front of `blind` see nothing
-  int pad[2];
 };
 
 struct AttentionArgs {
@@ -927,7 +919,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const Shared o = both[side];
-    if (o.first > o.last) continue;
+    if (!is_unit(o, team, a.workers / a.n_kv_heads, C, a.batch.n_rows, a.group)) continue;
     const int n = o.last - o.first + 1, base = 256 * blockIdx.y;
     const int tasks = V * o.columns - base < 256 ? V * o.columns - base : 256;
     if (tasks <= 0) continue;
