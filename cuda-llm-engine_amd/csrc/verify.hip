@@ -34,9 +34,12 @@
 #include <math.h>
 
 #include "common.hpp"
+#include "verify_end.hpp"
 
 namespace llmk {
 namespace {
+
+using namespace verify;
 
 constexpr int kThreads = 256, kVectors = 4;             // 16-byte vectors per thread of a chunk
 constexpr int kChunk = 64 * kVectors * 8;               // logits per chunk, a wave's
@@ -52,23 +55,7 @@ struct Stat {
   int pad;
 };
 
-// Logits over a temperature t, in log2 units.
-struct Scale {
-  double k;   // log2e / t
-  float far;  // at a distance of -far and beyond weights are 0: about 10^9 / k
-  int pad;
-};
 constexpr float kFar = 3.0e38f;  // at most
-
-// Where a sequence ends.
-struct End {
-  int first, end, row;  // its rows, and the one that gives its last token
-  int last;             // that one stands behind all drafts
-  int greedy, at;       // at: the row's argmax, where the choice is greedy
-  float pm, qm;         // maxima of the target's and the draft model's row
-  Scale by;
-};
-static_assert(sizeof(End) == 48, "workspace layout");
 
 struct VerifyArgs {
   const f16* logits;
@@ -391,6 +378,10 @@ __device__ __forceinline__ End find_end(const VerifyArgs& a, int s) {
   }
   return z;
 }
+// As an earlier launch found it.
+__device__ __forceinline__ End end_of(const VerifyArgs& a, int s) {
+  return checked(a.ends[s], s, a.starts != nullptr, a.n_rows);
+}
 // Whether there is a token to draw.
 __device__ __forceinline__ bool draws(const End& z) {
   return z.row >= z.first && !z.greedy && z.pm > -INFINITY;
@@ -425,7 +416,7 @@ template <bool FIND>
 __global__ void __launch_bounds__(kThreads) k_verify_sums(const VerifyArgs a) {
   __shared__ double shared[4];
   const int piece = blockIdx.x % a.pieces, s = blockIdx.x / a.pieces, share = blockIdx.y;
-  const End z = FIND ? find_end(a, s) : a.ends[s];
+  const End z = FIND ? find_end(a, s) : end_of(a, s);
   if (FIND && piece == 0 && share == 0 && threadIdx.x == 0) a.ends[s] = z;
   if (!draws(z) || (share == 1 && !(z.qm > -INFINITY))) return;
   const Row r = row_of(a.logits, z.row, a.vocab);
@@ -499,7 +490,7 @@ __device__ __forceinline__ Left left_from(const VerifyArgs& a, const End& z, int
 __global__ void __launch_bounds__(kThreads) k_verify_left(const VerifyArgs a) {
   __shared__ double shared[4];
   const int piece = blockIdx.x % a.pieces, s = blockIdx.x / a.pieces, lane = threadIdx.x & 63;
-  const End z = a.ends[s];
+  const End z = end_of(a, s);
   const double2 first =
       lane < a.pieces ? a.sums[(size_t)s * a.pieces + lane] : make_double2(0.0, 0.0);
   if (!draws(z) || !(z.qm > -INFINITY)) return;
@@ -529,7 +520,7 @@ __global__ void __launch_bounds__(kChooseThreads) k_verify_choose(const VerifyAr
   __shared__ double shared[WAVES];
   __shared__ int first_past, last_any;
   const int s = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const End z = a.ends[s];
+  const End z = end_of(a, s);
   const double2* sums = a.sums + (size_t)s * a.pieces;
   // what all this waits for, in one go
   const double2 first = lane < a.pieces ? sums[lane] : make_double2(0.0, 0.0);
