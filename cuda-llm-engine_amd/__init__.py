@@ -599,9 +599,12 @@ def _kv8_batch(fn, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, s
     return pools, batch, spans
 
 
-def _kv8_pages(fn, spans, block_tables, n_seqs, max_pages, page_size, num_pages):
-    """Checks the table entries of positions [first, end) and returns them, sequence by sequence."""
+def _kv8_pages(fn, spans, block_tables, n_seqs, max_pages, page_size, k_scale, v_scale,
+               n_kv_heads):
+    """Checks the table entries of positions [first, end), which are pages of both pools, and returns
+    them, sequence by sequence."""
     first, end = spans
+    num_pages = min(k_scale.numel(), v_scale.numel()) // n_kv_heads
     at = torch.arange(max_pages, device=first.device)[None, :]
     used = (at >= (first // page_size)[:, None]) & (at < ((end + page_size - 1) // page_size)[:, None])
     used &= (end > first)[:, None]
@@ -639,7 +642,7 @@ def kv8_append(qkv, ld: int, q_out, k_pool, k_scale, v_pool, v_scale, block_tabl
     _here(fn, qkv=qkv, q_out=q_out, inv_freq=inv_freq)
     if spans is not None:
         pages = _kv8_pages(fn, spans, block_tables, n_seqs, max_pages, page_size,
-                           k_scale.numel() // n_kv_heads)
+                           k_scale, v_scale, n_kv_heads)
         if pages.unique().numel() != pages.numel():
             _fail(fn, "two sequences append to the same page")
     _check(fn, _lib.llmk_kv8_append(px, ld, pq, *pools, *batch, pf, n_rows, n_seqs, max_pages,
@@ -666,7 +669,7 @@ def kv8_gather(k_pool, k_scale, v_pool, v_scale, block_tables, row_starts, seq_l
     _here(fn, k_out=k_out, v_out=v_out)
     if spans is not None:
         _kv8_pages(fn, spans, block_tables, n_seqs, max_pages, page_size,
-                   k_scale.numel() // n_kv_heads)
+                   k_scale, v_scale, n_kv_heads)
     _check(fn, _lib.llmk_kv8_gather(*pools, *batch, pk, pv, n_rows, n_seqs, max_pages, page_size,
                                     n_kv_heads, head_dim, _stream(stream)))
 
@@ -697,7 +700,7 @@ def kv8_attention(q, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
     _here(fn, q=q, out=out, workspace=workspace)
     if spans is not None:
         _kv8_pages(fn, (torch.zeros_like(spans[0]), spans[1]), block_tables, n_seqs, max_pages,
-                   page_size, k_scale.numel() // n_kv_heads)
+                   page_size, k_scale, v_scale, n_kv_heads)
     _check(fn, _lib.llmk_kv8_attention(pq, *pools, *batch, po, pw, n_rows, n_seqs, max_rows,
                                        max_pages, page_size, n_heads, n_kv_heads, head_dim,
                                        _stream(stream)))
