@@ -698,9 +698,11 @@ def kv8_attention(q, k_pool, k_scale, v_pool, v_scale, block_tables, row_starts,
     po = _dev(fn, out, torch.float16, n_rows * n_heads * head_dim, "out")
     pw = _opt(fn, workspace, torch.float32, kv8_attention_workspace_floats(head_dim), "workspace")
     _here(fn, q=q, out=out, workspace=workspace)
-    if spans is not None:
-        _kv8_pages(fn, (torch.zeros_like(spans[0]), spans[1]), block_tables, n_seqs, max_pages,
-                   page_size, k_scale, v_scale, n_kv_heads)
+    if spans is not None:  # from position 0 on, of sequences that have rows
+        first, end = spans
+        whole = torch.zeros_like(first), torch.where(first < end, end, torch.zeros_like(end))
+        _kv8_pages(fn, whole, block_tables, n_seqs, max_pages, page_size, k_scale, v_scale,
+                   n_kv_heads)
     _check(fn, _lib.llmk_kv8_attention(pq, *pools, *batch, po, pw, n_rows, n_seqs, max_rows,
                                        max_pages, page_size, n_heads, n_kv_heads, head_dim,
                                        _stream(stream)))

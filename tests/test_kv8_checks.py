@@ -62,3 +62,12 @@ def test_a_page_is_one_of_both_pools(llmk, calls, name):
     for k_pages, v_pages in ((4, 9), (9, 4), (9, 1)):
         with pytest.raises(llmk.LlmkError, match="block_tables"):
             calls(name, k_pages, v_pages, ints(4, 4, 1, 3), ints(0, 20, 21), ints(20, 30), 21)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_sequence_without_rows_names_no_page(llmk, calls, name):
+    """Its table is not read: it may hold anything. With a row its pages are looked at."""
+    tables, lens = ints(0, 1, 99, -7, 2, 3), ints(20, 30, 32)
+    assert calls(name, 4, 4, tables, ints(0, 2, 2, 5), lens, 5)
+    with pytest.raises(llmk.LlmkError, match="block_tables"):
+        calls(name, 4, 4, tables, ints(0, 2, 3, 5), lens, 5)
