@@ -111,6 +111,9 @@ __device__ __forceinline__ void lds_barrier() {
 
 inline unsigned ceil_div(size_t a, size_t b) { return (unsigned)((a + b - 1) / b); }
 
+// Whether a launch takes so many blocks in a dimension, whose threads HIP counts in 32 bits.
+inline bool grid_takes(size_t blocks, size_t threads) { return blocks < (1ull << 32) / threads; }
+
 // The current device's CU count, read once per device (0 if it cannot be read). Launch shapes
 // that size a grid to one resident round of blocks use it.
 inline int device_cus() {

@@ -360,6 +360,8 @@ extern "C" int llmk_kv8_append(const uint16_t* qkv, int ld, uint16_t* q_out, uin
   if ((long long)ld < ((long long)n_heads + 2LL * n_kv_heads) * head_dim || ld % 8 != 0)
     return LLMK_ERR_SHAPE;
   if (n_rows == 0 || n_seqs == 0) return LLMK_OK;
+  const size_t windows = ceil_div((size_t)n_rows, (size_t)kWindow);
+  if (!grid_takes(windows, 256)) return LLMK_ERR_UNSUPPORTED;
   if (!qkv || !q_out || !k_pool || !k_scale || !v_pool || !v_scale || !block_tables || !seq_lens ||
       !inv_freq)
     return LLMK_ERR_INVALID_VALUE;
@@ -379,7 +381,7 @@ extern "C" int llmk_kv8_append(const uint16_t* qkv, int ld, uint16_t* q_out, uin
   a.n_kv_heads = n_kv_heads;
   // a block for K and V takes four tasks at a time of the window's 16 to 32 at 8 kv heads
   const int kv_blocks = (n_kv_heads + 1) / 2 < 32 ? (n_kv_heads + 1) / 2 : 32;
-  const dim3 grid(ceil_div((size_t)n_rows, (size_t)kWindow), kv_blocks + kWindow / kQuarter);
+  const dim3 grid((unsigned)windows, kv_blocks + kWindow / kQuarter);
   return launch(head_dim == 64 ? k_kv8_append<64> : k_kv8_append<128>, grid, dim3(256), 0,
                 static_cast<hipStream_t>(stream), a, kv_blocks);
 }
@@ -395,6 +397,8 @@ extern "C" int llmk_kv8_gather(const uint8_t* k_pool, const float* k_scale, cons
   if (st != LLMK_OK) return st;
   if (n_kv_heads > 65536) return LLMK_ERR_UNSUPPORTED;  // a block's share is counted in 32 bits
   if (n_rows == 0 || n_seqs == 0) return LLMK_OK;
+  const size_t blocks = ceil_div((size_t)n_rows, (size_t)kGatherRows);
+  if (!grid_takes(blocks, 256)) return LLMK_ERR_UNSUPPORTED;
   if (!k_pool || !k_scale || !v_pool || !v_scale || !block_tables || !seq_lens || !k_out || !v_out)
     return LLMK_ERR_INVALID_VALUE;
   if (!aligned16(k_pool) || !aligned16(v_pool) || !aligned16(k_out) || !aligned16(v_out))
@@ -410,6 +414,5 @@ extern "C" int llmk_kv8_gather(const uint8_t* k_pool, const float* k_scale, cons
   a.n_kv_heads = n_kv_heads;
   a.per_row = make_fastdiv((uint32_t)n_kv_heads * (uint32_t)head_dim / 8);
   return launch(head_dim == 64 ? k_kv8_gather<64> : k_kv8_gather<128>,
-                dim3(ceil_div((size_t)n_rows, (size_t)kGatherRows), 2), dim3(256), 0,
-                static_cast<hipStream_t>(stream), a);
+                dim3((unsigned)blocks, 2), dim3(256), 0, static_cast<hipStream_t>(stream), a);
 }

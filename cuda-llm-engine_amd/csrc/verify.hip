@@ -653,9 +653,15 @@ extern "C" int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_
   if ((long long)chunks * 2 * n_rows > 0x7FFFFFFFLL || (long long)pieces * n_seqs > 0x7FFFFFFFLL ||
       vocab > 0x7FFFFFFF - 2 * kChunk)
     return LLMK_ERR_UNSUPPORTED;
+  const bool drafted = row_starts && draft_logits;
+  const size_t units = (size_t)chunks * (size_t)n_rows * (drafted ? 2 : 1);
+  if (n_rows > 0 && (!grid_takes((units + kThreads / 64 - 1) / (kThreads / 64), kThreads) ||
+                     !grid_takes((size_t)pieces * (size_t)n_seqs, kThreads) ||
+                     !grid_takes((size_t)n_seqs, kChooseThreads)))
+    return LLMK_ERR_UNSUPPORTED;
   VerifyArgs a;
   a.logits = reinterpret_cast<const f16*>(logits);
-  a.draft_logits = row_starts ? reinterpret_cast<const f16*>(draft_logits) : nullptr;
+  a.draft_logits = drafted ? reinterpret_cast<const f16*>(draft_logits) : nullptr;
   a.drafts = drafts;
   a.starts = row_starts;
   a.temperature = temperature;
@@ -676,9 +682,7 @@ extern "C" int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_
   if (n_rows == 0)
     return launch(k_verify_none, dim3(ceil_div((size_t)n_seqs, kThreads)), dim3(kThreads), 0, st,
                   n_accepted, n_seqs);
-  const unsigned rows = (unsigned)n_rows * (a.draft_logits ? 2u : 1u);
-  int rc = launch(k_verify_stats, dim3(ceil_div((size_t)chunks * rows, kThreads / 64)),
-                  dim3(kThreads), 0, st, a);
+  int rc = launch(k_verify_stats, dim3(ceil_div(units, kThreads / 64)), dim3(kThreads), 0, st, a);
   const unsigned per_piece = (unsigned)pieces * (unsigned)n_seqs;
   const dim3 shares(per_piece, a.draft_logits ? 2 : 1);
   // Blocks of the drawn rows' sums up to which they find the ends themselves. 5 rows a sequence,

@@ -299,7 +299,8 @@ LLMK_API int llmk_decode_nongemm_pass_fused(const llmk_decode_pass* pass, void* 
  * row i of c stands at position seq_lens[s] - c + i, in page block_tables[s * max_pages + position /
  * 16]. Rows at row_starts[n_seqs] and behind belong to none: what they would give is left as it was.
  * Positions below 0 or past the table are nowhere: not written, and read as nothing. Page numbers
- * are not range-checked. Pools, q, qkv and outputs are 16-byte aligned.
+ * are not range-checked. Pools, q, qkv and outputs are 16-byte aligned. Append and read-back take up to
+ * 2^28 - 16 rows, LLMK_ERR_UNSUPPORTED past them.
  * ------------------------------------------------------------------------------------------ */
 
 /* Appends the rows' keys and values, the keys rotated, and rotates their queries. Row r of qkv
@@ -372,8 +373,9 @@ LLMK_API size_t llmk_verify_drafts_workspace_floats(int n_rows, int n_seqs, int 
  * -1; -1 also for the token where a row has nothing above -inf.
  * workspace: 16-byte aligned; calls that may overlap need one each. drafts and accept_u may be NULL
  * with row_starts NULL. Any vocab and alignment of logits (16-byte vectors throughout where vocab %
- * 8 == 0). LLMK_ERR_UNSUPPORTED where rows times 2048-logit chunks, twice, or sequences times
- * 4096-logit pieces pass 2^31 - 1. */
+ * 8 == 0). LLMK_ERR_UNSUPPORTED, before any launch, where rows times 2048-logit chunks, twice with draft
+ * logits, pass 2^26 - 4, sequences times 4096-logit pieces 2^24 - 1, sequences 2^23 - 1, or vocab
+ * 2^31 - 4097. */
 LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_logits,
                                 const int32_t* drafts, const int32_t* row_starts,
                                 const float* temperature, const float* accept_u,
