@@ -39,9 +39,11 @@ using namespace kv8;
 
 // Cosine and sine of an angle, in 64 bits: the quarter turns are taken off in two parts (the angles
 // of far positions lose their fraction in 32 bits), and what is left, at most pi / 4, goes through
-// the series of both, which end below 2^-48 there.
+// the series of both, which end below 2^-48 there. Their number, of up to 2^51, is the low bits of a
+// sum with 1.5 * 2^52, whose last one is 1: a conversion to 32 bits would end at 2^31.
 __device__ __forceinline__ double2 cos_sin(double angle) {
-  const double k = __builtin_rint(angle * 0.63661977236758134308);
+  constexpr double kWhole = 6755399441055744.0;
+  const double turns = __builtin_fma(angle, 0.63661977236758134308, kWhole), k = turns - kWhole;
   double r = __builtin_fma(-k, 1.57079632679489655800, angle);
   r = __builtin_fma(-k, 6.12323399573676603587e-17, r);
   const double z = r * r;
@@ -61,7 +63,7 @@ __device__ __forceinline__ double2 cos_sin(double angle) {
   c = __builtin_fma(c, z, 4.1666666666666666667e-02);
   c = __builtin_fma(c, z, -0.5);
   c = __builtin_fma(c, z, 1.0);
-  const int q = (int)k & 3;
+  const int q = (int)(uint32_t)__builtin_bit_cast(uint64_t, turns) & 3;
   const double cq = (q & 1) ? s : c, sq = (q & 1) ? c : s;
   return make_double2(q == 1 || q == 2 ? -cq : cq, q >= 2 ? -sq : sq);
 }
