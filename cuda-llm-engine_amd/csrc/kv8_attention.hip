@@ -144,7 +144,7 @@ struct AttentionArgs {
   float* parts;  // [2 workers][columns of a tile][HD], NULL: no unit is shared
   float2* parts_ml;
   Shared* shared;  // [2 workers]
-  int n_heads, n_kv_heads, group, workers;
+  int n_heads, n_kv_heads, group, workers, teams;  // teams: workers / n_kv_heads
   int least_columns, most_columns;  // of the sequences that a launch takes
 };
 
@@ -242,7 +242,7 @@ struct Share {
   // all but the place of the beginning
   static __device__ __forceinline__ Share of(const AttentionArgs& a, long long total, int worker) {
     Share r = {};
-    r.teams = a.workers / a.n_kv_heads;
+    r.teams = a.teams;
     if (total < r.teams) r.teams = total > 0 ? (int)total : 1;
     r.each = divide(total, r.teams);
     r.more = (int)(total - r.each * r.teams);
@@ -919,7 +919,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
 #pragma unroll
   for (int side = 0; side < 2; ++side) {
     const Shared o = both[side];
-    if (!is_unit(o, team, a.workers / a.n_kv_heads, C, a.batch.n_rows, a.group)) continue;
+    if (!is_unit(o, team, a.teams, C)) continue;
     const int n = o.last - o.first + 1, base = 256 * blockIdx.y;
     const int tasks = V * o.columns - base < 256 ? V * o.columns - base : 256;
     if (tasks <= 0) continue;
@@ -949,7 +949,7 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
     if (turn == 0 && c < o.columns) {
       for (int k = 1; k < deal && k < n; ++k)
         r.add(others[tid + k * lanes], others_ml[tid + k * lanes]);
-      const int col = o.column + c;
+      const int col = o.column + c, row = row_of(o, c, a.batch.n_rows, a.group);
       const bool any = col >= o.blind;
       f16x2 y[2];
 #pragma unroll
@@ -957,8 +957,9 @@ __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs 
       uint2 v;
       v.x = __builtin_bit_cast(uint32_t, y[0]);
       v.y = __builtin_bit_cast(uint32_t, y[1]);
-      *reinterpret_cast<uint2*>(a.out + ((size_t)(o.row0 + col / a.group) * a.n_heads +
-                                         head * a.group + col % a.group) * HD + d) = v;
+      if (row >= 0)
+        *reinterpret_cast<uint2*>(
+            a.out + ((size_t)row * a.n_heads + head * a.group + col % a.group) * HD + d) = v;
     }
   }
 }
@@ -1316,6 +1317,7 @@ int few_launch(AttentionArgs a, hipStream_t stream) {
   const bool two = QT == 1 && a.batch.max_pages <= kShortPages &&
                    (long long)a.batch.n_seqs * a.n_kv_heads >= 2 * kFewWorkers;
   a.workers = two ? 2 * kFewWorkers : kFewWorkers;
+  a.teams = a.workers / a.n_kv_heads;
   const int st =
       launch(k_kv8_attention_few<HD, QT>, dim3(a.workers / 4), dim3(256), 0, stream, a);
   return st != LLMK_OK ? st : join_launch<HD>(a, 16 * QT, stream);
@@ -1324,6 +1326,7 @@ int few_launch(AttentionArgs a, hipStream_t stream) {
 template <int HD, int W>
 int many_launch(AttentionArgs a, hipStream_t stream) {
   a.workers = kManyWorkers<W>;
+  a.teams = a.workers / a.n_kv_heads;
   const int st =
       launch(k_kv8_attention_many<HD, W>, dim3(a.workers), dim3(64 * W), 0, stream, a);
   return st != LLMK_OK ? st : join_launch<HD>(a, 32 * W, stream);
@@ -1396,7 +1399,7 @@ extern "C" int llmk_kv8_attention(const uint16_t* q, const uint8_t* k_pool, cons
   a.n_heads = n_heads;
   a.n_kv_heads = n_kv_heads;
   a.group = n_heads / n_kv_heads;
-  a.workers = 0;
+  a.workers = a.teams = 0;
   a.least_columns = 0;
   a.most_columns = 0x7FFFFFFF;
   hipStream_t s = static_cast<hipStream_t>(stream);
