@@ -620,8 +620,9 @@ def kv8_append(qkv, ld: int, q_out, k_pool, k_scale, v_pool, v_scale, block_tabl
     """RoPE of the rows' q and k, and k and v appended to the 8-bit cache (``llmk_kv8_append``).
 
     Pools are torch.float8_e4m3fn [num_pages, n_kv_heads, 16, head_dim], scales float32
-    [num_pages, n_kv_heads]; row_starts None: one row a sequence. ``check_indices`` also refuses a
-    page that two sequences append to."""
+    [num_pages, n_kv_heads]; row_starts None: one row a sequence. ``check_indices`` refuses, here and
+    in the calls below, pages that are not of both pools and lengths past the table (whose rows are
+    nowhere for the call itself), here also a page that two sequences append to."""
     fn = "kv8_append"
     check = _want_checks(check_indices)
     if not check:

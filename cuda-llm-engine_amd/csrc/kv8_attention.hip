@@ -13,12 +13,13 @@
 // What bounds it. A decode step reads 2 n_kv_heads head_dim bytes a position and uses each 4 times
 // for each query head of a group: HBM, and the matrix cores only because the vector units, with
 // e4m3 to convert and weights to make, would be slower than it (256 sequences of up to 2048
-// positions 1494 us there). 256 sequences 59 us for 283 MB, 54.5 at a large copy's rate; 3 of up to
-// 65001 positions 49 us for 242 MB. Prompts are bound by the vector units: a weight takes about 7
-// instructions (scale and subtract, exponential, sum, split), as many cycles as its 3 products, and
-// in the counters the vector and the matrix instructions together are some 90% of the steps'
-// cycles: 1507 rows behind 1494 positions, 32 heads of 64 dims, 65 us, 427 TFLOP/s of the
-// definition's two products.
+// positions 1494 us there). 256 sequences 59 us for 283 MB, 43.6 at a large copy's 6.5 TB/s; 3 of
+// up to 65001 positions 48.5 us for 242 MB (37.2). Prompts are bound by the vector and the matrix
+// units one after the other: a weight takes about 7 vector instructions (scale and subtract,
+// exponential, sum, split) and 3 products, and by the counters a SIMD has vector instructions at
+// work for 71 thousand cycles and products for 41 of the 115 thousand that its two waves live. They
+// meet at a barrier every step, so neither hides the other. 1507 rows behind 1494 positions, 32
+// heads of 64 dims, 65 us, 427 TFLOP/s of the definition's two products.
 //
 // Two kernels: waves on their own for few columns (k_kv8_attention_few) and blocks that share K and
 // V through LDS for many. In both the work is cut into equal shares across the ends of sequences,
@@ -895,8 +896,9 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 // workers behind it (even slots). Block (b, y) looks at the units that worker b has a part in, at
 // the y-th 256 of their tasks (a column's 4 dims). The n workers of a unit share them among their
 // blocks, in up to n / 4 slices, and a block deals the parts out over the threads that a slice
-// leaves, which meet in LDS. Bound by latency where rows are few, 2.7 us for one sequence and 4.6
-// for 256, and by the parts' bytes for prompts: 8 us for the 20 MB, written and read, of 1507 rows.
+// leaves, which meet in LDS. Bound by latency where rows are few, 3.7 us of a trace for one sequence
+// and 4.7 for 256, and by the parts' bytes for prompts: 8.6 us for the 20 MB, written and read, of
+// 1507 rows.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs a, int C) {
   constexpr int V = HD / 4;

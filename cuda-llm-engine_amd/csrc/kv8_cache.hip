@@ -22,11 +22,13 @@
 // rows. So a window makes 16 to 32 such tasks whether it holds one prompt's rows or a decode
 // step's, nothing is read twice, and the maximum is a few lane exchanges.
 //
-// What bounds it: HBM for prompts, where 5 of up to 2001 rows take 22.4 us for 81 MB, 15.6 at a
-// large copy's rate (a block's leaders, angles and maxima stand in front of its writes); for a
-// decode step the way from the row starts over the lengths and tables to the scales, 4.2 us for one
-// row and 6.3 for 256 of them (2.6 MB). A grid of one block for each row and head took 21.7 us
-// there, with read-back, and not 10.3.
+// What bounds it: for prompts HBM and what stands in front of a block's writes, its leaders, angles
+// and maxima: 5 of up to 2001 rows take 25.5 us for 81 MB (22 where half of that is in the
+// last-level cache), 12.5 at a large copy's 6.5 TB/s. Angles go by leader: where one leads 16 rows,
+// 32 of the block's threads (64 at 128 dims) make all of them, and K and V are loaded behind that.
+// For a decode step the way from the row starts over the lengths and tables to the scales, 4.7 us
+// for one row and 6.0 for 256 of them (2.6 MB). A grid of one block for each row and head took 21.7
+// us there, with read-back, and not 10.3.
 #include <math.h>
 
 #include "kv8.hpp"
@@ -262,9 +264,10 @@ __global__ void __launch_bounds__(256) k_kv8_append(const AppendArgs a, int kv_b
 // Read-back: a block takes 16 rows of K or of V, a thread 8 values at a time, in the order of the
 // output (a wave writes 1 KiB in a row; what it reads are 64-byte halves of lines whose other
 // halves the neighbouring rows take), four of them in flight. Bound by HBM, two thirds of it
-// writes: 64 sequences of up to 3001 rows, 314 MB, 59.7 us, 5.3 TB/s; in the order of the cache,
-// which leaves lines half written, 82.4. 77 rows of one sequence 3.6 us, the way over starts,
-// lengths, table and scale.
+// writes: 64 sequences of up to 3001 rows, 314 MB, 59.7 us, 5.3 TB/s (48.5 where two such batches
+// take turns and what is read stays in the last-level cache); in the order of the cache, which
+// leaves lines half written, 82.4. 77 rows of one sequence 3.6 us, the way over starts, lengths,
+// table and scale.
 constexpr int kGatherRows = 16, kGatherFlight = 4;
 
 struct GatherArgs {

@@ -339,7 +339,9 @@ LLMK_API size_t llmk_kv8_attention_workspace_floats(int head_dim);
  * and out [n_rows, n_heads, head_dim], n_heads any multiple of n_kv_heads. Scores, weights and sums
  * in fp32, the result rounded once. A row that sees no position gets zeros. A NaN that a row sees
  * makes it NaN; what a row does not see does not touch it. max_rows: the most rows that a sequence
- * has in this call; it only chooses kernels (more rows than that are slow, not wrong). `workspace`
+ * has in this call; it only chooses kernels (more rows than that are slow, not wrong). Over n positions
+ * that stay whole (below) the sum of weights is off by less than 2^-20 and that of a dim's values by at
+ * most n 2^-27 of their magnitudes', which equal weights of equal values come near. `workspace`
  * (llmk_kv8_attention_workspace_floats(head_dim) floats, 16-byte aligned) lets the positions of a
  * batch be shared out evenly, with a second launch that joins their parts; NULL for contexts that are
  * short: every sequence then stays whole. Calls that may overlap need a workspace each; graphs that
@@ -366,9 +368,11 @@ LLMK_API size_t llmk_verify_drafts_workspace_floats(int n_rows, int n_seqs, int 
  * accept_u[row] * q(draft) < p(draft). The first row refused gives a token of max(p - q, 0) (of p if
  * that is 0 everywhere), the last row one of p: the lowest v with weight_0 + .. + weight_v >
  * sample_u[s] * total. Numbers of accept_u [n_rows] and sample_u [n_seqs] lie in [0, 1).
- * Exponentials and sums in 64 bits. t <= 0 or NaN: greedy, a draft stands where it is its row's
- * argmax (the lowest place), which is also the token. NaN logits count as -inf, places of +inf share
- * all probability; a draft outside [0, vocab) is refused.
+ * Exponentials and sums in 64 bits. (A draft within 2^-14 of its border has its rows summed once more: a
+ * call that holds one, one in a hundred of 64 sequences of 5 rows, takes 0.5 ms longer at 128256 logits.)
+ * t <= 0 or NaN: greedy, a draft stands where it is its row's argmax (the lowest place), which is also the
+ * token. NaN logits count as -inf, places of +inf share all probability; a draft outside [0, vocab) is
+ * refused.
  * n_accepted [n_seqs]: drafts that stand. tokens [n_rows]: for each sequence those, the token, then
  * -1; -1 also for the token where a row has nothing above -inf.
  * workspace: 16-byte aligned; calls that may overlap need one each. drafts and accept_u may be NULL
