@@ -114,13 +114,13 @@ __device__ __forceinline__ void split_rounded(float a, float b, uint32_t& hi, ui
   lo = __builtin_bit_cast(uint32_t, r);
 }
 
-// A running sum of the steps' sums of weights that takes along what each addition lost. A worker may
-// walk a unit of 10^5 positions by itself, and equal weights added pair by pair lose the same way
-// each time: 2^-11 of the sum at 131072 positions, as much as the result's own rounding. So it is
-// the 32 additions of a step at most that count, less than 2^-20. O has no such help: a position's
-// value is one of 32 (16) in a sum that the matrix cores add twice, so it may be off by 2^-28
-// (2^-27) of itself for each position, where weights and values are all equal: past 2^-11.5 there at
-// 131072 positions, and 2^-18 with weights that differ.
+// A running sum of the steps' sums of weights that takes along what each addition lost. A worker
+// may walk a unit of 10^5 positions by itself, and equal weights added pair by pair lose the same
+// way each time: 2^-11 of the sum at 131072 positions, as much as the result's own rounding. So it
+// is the 32 additions of a step at most that count, less than 2^-20. O has no such help: a
+// position's value is one of 32 (16) in a sum that the matrix cores add twice, so it may be off by
+// 2^-28 (2^-27) of itself for each position, where weights and values are all equal: past 2^-11.5
+// there at 131072 positions, and 2^-18 with weights that differ.
 struct Sum {
   float of, lost;
   __device__ __forceinline__ void add(float x) {
@@ -896,9 +896,9 @@ __global__ void __launch_bounds__(256, 2) k_kv8_attention_few(const AttentionArg
 // workers behind it (even slots). Block (b, y) looks at the units that worker b has a part in, at
 // the y-th 256 of their tasks (a column's 4 dims). The n workers of a unit share them among their
 // blocks, in up to n / 4 slices, and a block deals the parts out over the threads that a slice
-// leaves, which meet in LDS. Bound by latency where rows are few, 3.7 us of a trace for one sequence
-// and 4.7 for 256, and by the parts' bytes for prompts: 8.6 us for the 20 MB, written and read, of
-// 1507 rows.
+// leaves, which meet in LDS. Bound by latency where rows are few, 3.7 us of a trace for one
+// sequence and 4.7 for 256, and by the parts' bytes for prompts: 8.6 us for the 20 MB, written and
+// read, of 1507 rows.
 template <int HD>
 __global__ void __launch_bounds__(256) k_kv8_attention_join(const AttentionArgs a, int C) {
   constexpr int V = HD / 4;

@@ -41,8 +41,8 @@ using namespace kv8;
 
 // Cosine and sine of an angle, in 64 bits: the quarter turns are taken off in two parts (the angles
 // of far positions lose their fraction in 32 bits), and what is left, at most pi / 4, goes through
-// the series of both, which end below 2^-48 there. Their number, of up to 2^51, is the low bits of a
-// sum with 1.5 * 2^52, whose last one is 1: a conversion to 32 bits would end at 2^31.
+// the series of both, which end below 2^-48 there. Their number, of up to 2^51, is the low bits of
+// a sum with 1.5 * 2^52, whose last one is 1: a conversion to 32 bits would end at 2^31.
 __device__ __forceinline__ double2 cos_sin(double angle) {
   constexpr double kWhole = 6755399441055744.0;
   const double turns = __builtin_fma(angle, 0.63661977236758134308, kWhole), k = turns - kWhole;

@@ -32,8 +32,8 @@
 // What bounds it: 1 reads 2 bytes a logit (64 sequences of 5 rows, 128256 logits and a draft
 // model's: 30 us for 148 MB), 2 and 3 are 64-bit exponentials, some 19 instructions each, two for
 // each logit of 64 rows and twice (14 and 12 us), where sequences end takes 5 and 4 another 5.5;
-// 61.4 us in all. Greedy, where 2 and 3 leave at once, 32.4. Sampling without drafts reads every row
-// twice and sums it in 64 bits: 256 rows 48.6 us, 64 rows 21.1, one 10.6. A single sequence is
+// 61.4 us in all. Greedy, where 2 and 3 leave at once, 32.4. Sampling without drafts reads every
+// row twice and sums it in 64 bits: 256 rows 48.6 us, 64 rows 21.1, one 10.6. A single sequence is
 // launches in a row: 5 rows of 32000 logits 12.6 us, of which 3.5, 6 and 3.5 in the kernels.
 #include <math.h>
 
