@@ -180,6 +180,16 @@ _SIGS = {
     "llmk_kv8_attention": (_i, [_vp] * 10 + [_i] * 8 + [_vp]),
     "llmk_verify_drafts_workspace_floats": (_sz, [_i, _i, _i]),
     "llmk_verify_drafts": (_i, [_vp] * 10 + [_i] * 3 + [_vp]),
+    "llmk_lora_add_workspace_floats": (_sz, [_i] * 6),
+    "llmk_lora_add": (_i, [_vp, _i] + [_vp] * 7 + [_i, _i32p, _i, _vp] + [_i] * 5 + [_vp]),
+    "llmk_rotary_apply": (_i, [_vp, _i, _vp, _i] + [_vp] * 4 + [_i] * 7 + [_vp]),
+    "llmk_qkv_rotary_scatter": (_i, [_vp, _i] + [_vp] * 8 + [_i] * 9 + [_vp]),
+    "llmk_compute_rotary_inv_freq": (_i, [_i, _i] + [_d] * 5 + [ctypes.POINTER(_f)] * 2),
+    "llmk_kv_copy_pages": (_i, [ctypes.POINTER(_vp), ctypes.POINTER(_sz), _i, _vp, _vp, _i, _i, _vp]),
+    "llmk_kv_fork_workspace_ints": (_sz, [_i] * 4),
+    "llmk_kv_fork": (_i, [_vp] * 10 + [_i] * 5 + [_vp]),
+    "llmk_kv_compact_workspace_ints": (_sz, [_i]),
+    "llmk_kv_compact": (_i, [_vp] * 7 + [_i] * 3 + [_vp]),
     "llmk_attention_decode_fast": (_i, [_vp] * 7 + [_i] * 7 + [_vp]),
     "llmk_attention_decode_fast_noalloc": (_i, [_vp] * 6 + [_i] * 7 + [_vp]),
     "llmk_decode_nongemm_pass": (_i, [ctypes.POINTER(DecodePass), _vp]),
@@ -749,6 +759,252 @@ def verify_drafts(logits, draft_logits, drafts, row_starts, temperature, accept_
                 or int(starts[-1]) > n_rows):
             _fail(fn, f"row_starts must ascend from 0 to at most {n_rows}")
     _check(fn, _lib.llmk_verify_drafts(*ptrs, n_rows, n_seqs, vocab, _stream(stream)))
+
+
+# ---------------------------------------------------------------------------------------------
+# serving requests that are not alike: adapters, rotary layouts and scalings, shared cache pages
+# ---------------------------------------------------------------------------------------------
+def _rows(fn: str, t, n: int, ld: int, width: int, name: str) -> int:
+    """The address of n rows of `width` values, `ld` apart, that begin where t does. t may be a view of
+    a wider tensor's columns: its storage has to hold the rows, its last dimension to be unbroken."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float16:
+        _fail(fn, f"{name} must be a CUDA tensor of {torch.float16}")
+    if n == 0 or width == 0:
+        return t.data_ptr()
+    if t.dim() == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        _fail(fn, f"{name}'s last dimension must be contiguous")
+    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) != ld:
+        _fail(fn, f"{name}'s rows are {t.stride(0)} apart, not {ld}")
+    if t.dim() != 2 and not t.is_contiguous():
+        _fail(fn, f"{name} must be contiguous or a matrix")
+    held = t.untyped_storage().nbytes() // 2 - t.storage_offset()
+    if t.numel() == 0 or held < (n - 1) * ld + width:
+        _fail(fn, f"{name} holds {held} elements, the call touches {(n - 1) * ld + width}")
+    if t.dim() == 2 and (t.shape[0] < n or t.shape[1] < width):
+        _fail(fn, f"{name} is {list(t.shape)}, the call touches [{n}, {width}]")
+    return t.data_ptr()
+
+
+def lora_add_workspace_floats(n_rows: int, n_seqs: int, n_adapters: int, max_rank: int,
+                              in_features: int, n_parts: int) -> int:
+    return int(_lib.llmk_lora_add_workspace_floats(n_rows, n_seqs, n_adapters, max_rank, in_features,
+                                                   n_parts))
+
+
+def lora_add(x, ldx: int, a, b, ranks, scales, adapter_ids, row_starts, y, ldy: int, part_ends,
+             workspace, n_rows: int, n_seqs: int, n_adapters: int, max_rank: int, in_features: int,
+             stream=None, check_indices: bool | None = None) -> None:
+    """Adds each sequence's low-rank adapter to a shared projection's output y (``llmk_lora_add``).
+
+    ``part_ends``: where the parts of a fused projection end, e.g. (hidden,), or (q, q + kv, q + 2 kv);
+    a [n_adapters, parts, max_rank, in_features], b [n_adapters, part_ends[-1], max_rank]; ranks, scales
+    and row_starts may be None. adapter_ids outside [0, n_adapters): no adapter.
+    ``check_indices`` refuses row_starts that do not ascend from 0 to at most n_rows and ranks past
+    max_rank."""
+    fn = "lora_add"
+    if min(n_rows, n_seqs, n_adapters) < 0 or min(max_rank, in_features) <= 0:
+        _fail(fn, "n_rows, n_seqs and n_adapters must be >= 0 and the other sizes > 0")
+    ends = (ctypes.c_int32 * max(1, len(part_ends)))(*part_ends)
+    if not 1 <= len(part_ends) <= 8 or min(part_ends) <= 0:
+        _fail(fn, "part_ends must be 1 to 8 ascending columns")
+    out = part_ends[-1]
+    px = _rows(fn, x, n_rows, ldx, in_features, "x")
+    py = _rows(fn, y, n_rows, ldy, out, "y")
+    pa = _dev(fn, a, torch.float16, n_adapters * len(part_ends) * max_rank * in_features, "a")
+    pb = _dev(fn, b, torch.float16, n_adapters * out * max_rank, "b")
+    pr = _opt(fn, ranks, torch.int32, n_adapters, "ranks")
+    ps = _opt(fn, scales, torch.float32, n_adapters, "scales")
+    pi = _dev(fn, adapter_ids, torch.int32, n_seqs, "adapter_ids")
+    pst = _opt(fn, row_starts, torch.int32, n_seqs + 1, "row_starts")
+    pw = _dev(fn, workspace, torch.float32, lora_add_workspace_floats(
+        n_rows, n_seqs, n_adapters, max_rank, in_features, len(part_ends)), "workspace")
+    _here(fn, x=x, y=y, a=a, b=b, ranks=ranks, scales=scales, adapter_ids=adapter_ids,
+          row_starts=row_starts, workspace=workspace)
+    if _want_checks(check_indices):
+        if row_starts is not None and n_seqs > 0:
+            starts = row_starts[:n_seqs + 1].long()
+            if int(starts[0]) != 0 or bool((starts[1:] < starts[:-1]).any()) or int(starts[-1]) > n_rows:
+                _fail(fn, f"row_starts must ascend from 0 to at most {n_rows}")
+        if ranks is not None:
+            _range_check(fn, ranks, n_adapters, -(1 << 31), max_rank + 1, "ranks")
+    _check(fn, _lib.llmk_lora_add(px, ldx, pa, pb, pr, ps, pi, pst, py, ldy, ends, len(part_ends), pw,
+                                  n_rows, n_seqs, n_adapters, max_rank, in_features,
+                                  _stream(stream)))
+
+
+ROTARY_HALVES, ROTARY_PAIRS = 0, 1
+ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_NTK, ROTARY_YARN = range(4)
+
+
+def _tables(fn, positions, inv_freq, table_ids, scales, n, rotary_dim, check):
+    """The pointers of a rotation and the number of frequency tables."""
+    if n < 0 or rotary_dim <= 0 or rotary_dim % 2:
+        _fail(fn, "the number of rows must be >= 0 and rotary_dim even and > 0")
+    pp = _dev(fn, positions, torch.int32, n, "positions")
+    pf = _dev(fn, inv_freq, torch.float32, rotary_dim // 2, "inv_freq")
+    n_tables = inv_freq.numel() // (rotary_dim // 2)
+    pt = _opt(fn, table_ids, torch.int32, n, "table_ids")
+    ps = _opt(fn, scales, torch.float32, n_tables, "scales")
+    _here(fn, positions=positions, inv_freq=inv_freq, table_ids=table_ids, scales=scales)
+    if check and table_ids is not None:
+        _range_check(fn, table_ids, n, 0, n_tables, "table_ids")
+    return pp, pf, pt, ps, n_tables
+
+
+def rotary_apply(q, ldq: int, k, ldk: int, positions, inv_freq, table_ids, scales, n_rows: int,
+                 n_heads: int, n_kv_heads: int, head_dim: int, rotary_dim: int, layout: int = 0,
+                 stream=None, check_indices: bool | None = None) -> None:
+    """Rotates the first rotary_dim elements of q's and k's heads where they lie
+    (``llmk_rotary_apply``). q and k may be columns of one fused projection (rows ldq, ldk apart);
+    inv_freq [tables, rotary_dim / 2], table_ids and scales may be None; ``layout``: ROTARY_HALVES or
+    ROTARY_PAIRS. ``check_indices`` refuses table_ids that name no table."""
+    fn = "rotary_apply"
+    pq = _rows(fn, q, n_rows, ldq, n_heads * head_dim, "q") if n_heads else None
+    pk = _rows(fn, k, n_rows, ldk, n_kv_heads * head_dim, "k") if n_kv_heads else None
+    pp, pf, pt, ps, n_tables = _tables(fn, positions, inv_freq, table_ids, scales, n_rows, rotary_dim,
+                                       _want_checks(check_indices))
+    _here(fn, q=q if n_heads else None, k=k if n_kv_heads else None)
+    _check(fn, _lib.llmk_rotary_apply(pq, ldq, pk, ldk, pp, pf, pt, ps, n_rows, n_heads, n_kv_heads,
+                                      head_dim, rotary_dim, n_tables, layout, _stream(stream)))
+
+
+def qkv_rotary_scatter(qkv, ld: int, q_out, k_pool, v_pool, block_tables, positions, inv_freq,
+                       table_ids, scales, n: int, max_pages: int, page_size: int, n_heads: int,
+                       n_kv_heads: int, head_dim: int, rotary_dim: int, layout: int = 0, stream=None,
+                       check_indices: bool | None = None) -> None:
+    """The rotation of rotary_apply on the way from a fused projection's rows into the paged fp16 cache
+    (``llmk_qkv_rotary_scatter``). ``check_indices`` refuses rows that have no page of the pools."""
+    fn = "qkv_rotary_scatter"
+    if min(max_pages, page_size, n_heads, n_kv_heads, head_dim) <= 0:
+        _fail(fn, "max_pages, page_size, the head counts and head_dim must be > 0")
+    check = _want_checks(check_indices)
+    pp, pf, pt, ps, n_tables = _tables(fn, positions, inv_freq, table_ids, scales, n, rotary_dim, check)
+    px = _rows(fn, qkv, n, ld, (n_heads + 2 * n_kv_heads) * head_dim, "qkv")
+    pq = _dev(fn, q_out, torch.float16, n * n_heads * head_dim, "q_out")
+    pk = _dev(fn, k_pool, torch.float16, 0, "k_pool")
+    pv = _dev(fn, v_pool, torch.float16, 0, "v_pool")
+    pb = _dev(fn, block_tables, torch.int32, n * max_pages, "block_tables")
+    _here(fn, qkv=qkv, q_out=q_out, k_pool=k_pool, v_pool=v_pool, block_tables=block_tables)
+    if check:
+        _check_batch_tables(fn, block_tables, positions, [k_pool, v_pool], n, max_pages, page_size,
+                            n_kv_heads * head_dim)
+    _check(fn, _lib.llmk_qkv_rotary_scatter(px, ld, pq, pk, pv, pb, pp, pf, pt, ps, n, max_pages,
+                                            page_size, n_heads, n_kv_heads, head_dim, rotary_dim,
+                                            n_tables, layout, _stream(stream)))
+
+
+def compute_rotary_inv_freq(scaling: int, rotary_dim: int, theta: float, factor: float = 1.0,
+                            original_max_pos: float = 0.0, beta_fast: float = 32.0,
+                            beta_slow: float = 1.0) -> tuple[list[float], float]:
+    """Host function: one frequency table and its scale, for ROTARY_PLAIN, ROTARY_LINEAR, ROTARY_NTK or
+    ROTARY_YARN (``llmk_compute_rotary_inv_freq``)."""
+    fn = "compute_rotary_inv_freq"
+    if rotary_dim <= 0 or rotary_dim % 2:
+        _fail(fn, "rotary_dim must be even and positive")
+    buf, scale = (_f * (rotary_dim // 2))(), _f()
+    _check(fn, _lib.llmk_compute_rotary_inv_freq(scaling, rotary_dim, theta, factor, original_max_pos,
+                                                 beta_fast, beta_slow, buf, ctypes.byref(scale)))
+    return list(buf), scale.value
+
+
+def kv_copy_pages(pools, copies, count, n_copies: int, num_pages: int, stream=None,
+                  check_indices: bool | None = None) -> None:
+    """Copies pages within every pool of ``pools``, by the pairs (from, to) of copies
+    (``llmk_kv_copy_pages``). A pool is a contiguous tensor of num_pages equal pages, of any dtype;
+    count: None, or kv_compact's counts. ``check_indices`` refuses a page that two pairs write, and one
+    that is written and read."""
+    fn = "kv_copy_pages"
+    if n_copies < 0 or num_pages <= 0:
+        _fail(fn, "n_copies must be >= 0 and num_pages > 0")
+    pc = _dev(fn, copies, torch.int32, 2 * n_copies, "copies")
+    pn = _opt(fn, count, torch.int32, 1, "count")
+    ptrs, sizes = (_vp * max(1, len(pools)))(), (_sz * max(1, len(pools)))()
+    for i, pool in enumerate(pools):
+        ptrs[i] = _dev(fn, pool, pool.dtype, 1, f"pools[{i}]")
+        nbytes = pool.numel() * pool.element_size()
+        if nbytes % num_pages:
+            _fail(fn, f"pools[{i}] is not {num_pages} equal pages")
+        sizes[i] = nbytes // num_pages
+        _here(fn, **{f"pools[{i}]": pool})
+    _here(fn, copies=copies, count=count)
+    if _want_checks(check_indices) and n_copies > 0:
+        n = n_copies if count is None else max(0, min(n_copies, int(count.reshape(-1)[0])))
+        pairs = copies.reshape(-1)[:2 * n].view(n, 2)
+        pairs = pairs[((pairs >= 0) & (pairs < num_pages)).all(1) & (pairs[:, 0] != pairs[:, 1])]
+        to = pairs[:, 1]
+        if to.unique().numel() != to.numel() or bool(torch.isin(to, pairs[:, 0]).any()):
+            _fail(fn, "a page is written twice, or written and read")
+    _check(fn, _lib.llmk_kv_copy_pages(ptrs, sizes, len(pools), pc, pn, n_copies, num_pages,
+                                       _stream(stream)))
+
+
+def kv_fork_workspace_ints(n_old: int, n_new: int, max_pages: int, num_pages: int) -> int:
+    return int(_lib.llmk_kv_fork_workspace_ints(n_old, n_new, max_pages, num_pages))
+
+
+def _overlap(fn, **tensors) -> None:
+    """Refuses two tensors of one storage whose elements overlap."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), name)
+             for name, t in tensors.items() if t is not None and t.numel()]
+    for (at, end, name), (at2, _, name2) in zip(sorted(spans), sorted(spans)[1:]):
+        if at2 < end:
+            _fail(fn, f"{name} and {name2} overlap")
+
+
+def kv_fork(block_tables, seq_lens, parents, reserve, refs, new_tables, new_lens, copies, counts,
+            workspace, n_old: int, n_new: int, max_pages: int, page_size: int, num_pages: int,
+            stream=None, check_indices: bool | None = None) -> None:
+    """The step from one batch to the next: children share their parents' whole pages, and pages that
+    nobody holds any more are free (``llmk_kv_fork``; kv_copy_pages then makes the copies that it
+    names). ``check_indices`` refuses counts in refs that are not the block tables' holders."""
+    fn = "kv_fork"
+    if min(n_old, n_new) < 0 or min(max_pages, page_size, num_pages) <= 0:
+        _fail(fn, "n_old and n_new must be >= 0 and the other sizes > 0")
+    i32 = torch.int32
+    ptrs = [_dev(fn, block_tables, i32, n_old * max_pages, "block_tables"),
+            _dev(fn, seq_lens, i32, n_old, "seq_lens"), _dev(fn, parents, i32, n_new, "parents"),
+            _opt(fn, reserve, i32, n_new, "reserve"), _dev(fn, refs, i32, num_pages, "refs"),
+            _dev(fn, new_tables, i32, n_new * max_pages, "new_tables"),
+            _dev(fn, new_lens, i32, n_new, "new_lens"), _dev(fn, copies, i32, 2 * n_new, "copies"),
+            _dev(fn, counts, i32, 2, "counts"),
+            _dev(fn, workspace, i32, kv_fork_workspace_ints(n_old, n_new, max_pages, num_pages),
+                 "workspace")]
+    named = dict(block_tables=block_tables, seq_lens=seq_lens, parents=parents, reserve=reserve,
+                 refs=refs, new_tables=new_tables, new_lens=new_lens, copies=copies, counts=counts,
+                 workspace=workspace)
+    _here(fn, **named)
+    if _want_checks(check_indices):
+        _overlap(fn, **named)
+        old = block_tables.reshape(-1)[:n_old * max_pages].view(n_old, max_pages).long()
+        held = ((old >= 0) & (old < num_pages)).long().cumprod(1).bool()
+        holders = torch.bincount(old[held], minlength=num_pages)
+        if bool((holders > refs[:num_pages]).any()):
+            _fail(fn, "refs counts fewer holders of a page than block_tables has")
+    _check(fn, _lib.llmk_kv_fork(*ptrs, n_old, n_new, max_pages, page_size, num_pages,
+                                 _stream(stream)))
+
+
+def kv_compact_workspace_ints(num_pages: int) -> int:
+    return int(_lib.llmk_kv_compact_workspace_ints(num_pages))
+
+
+def kv_compact(block_tables, refs, new_tables, new_refs, copies, counts, workspace, n_seqs: int,
+               max_pages: int, num_pages: int, stream=None) -> None:
+    """Renumbers the pages that are held to the pool's front (``llmk_kv_compact``; kv_copy_pages with its
+    copies and counts then moves them). In place where new_tables is block_tables, new_refs refs."""
+    fn = "kv_compact"
+    if n_seqs < 0 or min(max_pages, num_pages) <= 0:
+        _fail(fn, "n_seqs must be >= 0 and the other sizes > 0")
+    i32 = torch.int32
+    ptrs = [_dev(fn, block_tables, i32, n_seqs * max_pages, "block_tables"),
+            _dev(fn, refs, i32, num_pages, "refs"),
+            _dev(fn, new_tables, i32, n_seqs * max_pages, "new_tables"),
+            _dev(fn, new_refs, i32, num_pages, "new_refs"),
+            _dev(fn, copies, i32, 2 * (num_pages // 2), "copies"), _dev(fn, counts, i32, 2, "counts"),
+            _dev(fn, workspace, i32, kv_compact_workspace_ints(num_pages), "workspace")]
+    _here(fn, block_tables=block_tables, refs=refs, new_tables=new_tables, new_refs=new_refs,
+          copies=copies, counts=counts, workspace=workspace)
+    _check(fn, _lib.llmk_kv_compact(*ptrs, n_seqs, max_pages, num_pages, _stream(stream)))
 
 
 def copy_bytes(src, dst, nbytes: int, stream=None) -> None:

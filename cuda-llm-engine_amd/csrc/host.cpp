@@ -57,6 +57,41 @@ extern "C" int llmk_compute_rope_inv_freq(int head_dim, double theta, double fac
   return LLMK_OK;
 }
 
+// One frequency table of the scalings that the reference does not have (llmk.h states the formulas), in
+// 64 bits until the last rounding.
+extern "C" int llmk_compute_rotary_inv_freq(int scaling, int rotary_dim, double theta, double factor,
+                                            double original_max_pos, double beta_fast,
+                                            double beta_slow, float* out, float* scale) {
+  if (rotary_dim <= 0 || rotary_dim % 2 != 0 || !out || scaling < LLMK_ROTARY_PLAIN ||
+      scaling > LLMK_ROTARY_YARN || !(theta > 0) || !isfinite(theta))
+    return LLMK_ERR_INVALID_VALUE;
+  if (scaling != LLMK_ROTARY_PLAIN && (!(factor > 0) || !isfinite(factor)))
+    return LLMK_ERR_INVALID_VALUE;
+  double low = 0, high = 0;
+  if (scaling == LLMK_ROTARY_YARN) {
+    if (!(original_max_pos > 0) || !(beta_slow > 0) || !(beta_fast >= beta_slow) || !(theta > 1) ||
+        !isfinite(original_max_pos) || !isfinite(beta_fast))
+      return LLMK_ERR_INVALID_VALUE;
+    const auto pair_of = [&](double turns) {  // the pair that turns so often within the trained positions
+      return rotary_dim * log(original_max_pos / (turns * 2.0 * M_PI)) / (2.0 * log(theta));
+    };
+    low = fmax(floor(pair_of(beta_fast)), 0.0);
+    high = fmin(ceil(pair_of(beta_slow)), (double)(rotary_dim - 1));
+    high = fmax(high, low + 0.001);
+  }
+  const double base = scaling == LLMK_ROTARY_NTK && rotary_dim > 2
+                          ? theta * pow(factor, (double)rotary_dim / (rotary_dim - 2))
+                          : theta;
+  for (int i = 0; i < rotary_dim / 2; ++i) {
+    const double f = pow(base, -2.0 * i / rotary_dim);
+    double part = scaling == LLMK_ROTARY_LINEAR ? 1.0 : 0.0;  // of it that is interpolated
+    if (scaling == LLMK_ROTARY_YARN) part = fmin(fmax((i - low) / (high - low), 0.0), 1.0);
+    out[i] = (float)(f * (1.0 - part) + f / (part > 0.0 ? factor : 1.0) * part);
+  }
+  if (scale) *scale = scaling == LLMK_ROTARY_YARN && factor > 1.0 ? (float)(0.1 * log(factor) + 1.0) : 1.f;
+  return LLMK_OK;
+}
+
 // One non-GEMM decode pass, launched op by op on one stream (capturable into a HIP graph).
 // Mirrors the per-layer order of ref: engine/batched.cu:112-115 with the layer body of
 // engine/batched.cu:51-71 reduced to its non-GEMM operations: one add + RMSNorm per layer, or

@@ -1,0 +1,256 @@
+// Rotary positions of either layout, of part of a head, with a frequency table and a scale for each
+// row; where the rows lie, or on their way into the paged cache.
+//
+// x1' = s (x1 cos t - x2 sin t), x2' = s (x2 cos t + x1 sin t) for the elements that turn together, t =
+// position * inv_freq in 64 bits: an angle of a far position has lost its fraction in 32. The cosine and
+// sine, times s, are rounded to fp32 once for all heads of the row, the products and their sum are fp32
+// and the result is rounded to fp16: off by 2^-11 of itself and 2^-22 of |x1| + |x2|.
+//
+// A head's rotated part is cut into units of 16 elements, two 16-byte vectors that a thread turns by
+// itself, without its neighbours: vectors u and u + rotary_dim / 16. As halves they are each other's
+// partners; as pairs each holds four pairs. Either way a wave's loads cover whole lines.
+#include "angles.hpp"
+#include "layer_ops.hpp"
+
+namespace llmk {
+namespace {
+
+struct RotaryArgs {
+  const f16 *q, *k, *v;  // row r at r * ld of each
+  f16 *q_out, *k_out, *v_out;
+  const int *positions, *table_ids, *tables;
+  const float *inv_freq, *scales;
+  int ldq, ldk, ldq_out, ldk_out;  // ldk_out: of a row of the pool (in place: ldk)
+  int n_rows, n_heads, n_kv_heads, head_dim, rotary_dim, n_tables;
+  int max_pages, page_size;
+  int rows_per_block;
+};
+
+// (scale cos, scale sin) of pair i of a row.
+__device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int row, int i) {
+  int t = a.table_ids ? a.table_ids[row] : 0;
+  t = (unsigned)t < (unsigned)a.n_tables ? t : 0;
+  const double f = (double)a.inv_freq[(size_t)t * (a.rotary_dim / 2) + i];
+  const double2 cs = cos_sin((double)a.positions[row] * f);
+  const double s = a.scales ? (double)a.scales[t] : 1.0;
+  return make_float2((float)(cs.x * s), (float)(cs.y * s));
+}
+
+// The pool row (page * page_size + token) of a row, -1 where it has none.
+__device__ __forceinline__ long long pool_row_of(const RotaryArgs& a, int row) {
+  const int pos = a.positions[row];
+  if (pos < 0 || pos / a.page_size >= a.max_pages) return -1;
+  const int page = a.tables[(size_t)row * a.max_pages + pos / a.page_size];
+  return page < 0 ? -1 : (long long)page * a.page_size + pos % a.page_size;
+}
+
+template <bool PAIRS>
+__device__ __forceinline__ void turn(f16x8& x, f16x8& y, const float2* lo, const float2* hi) {
+  if (PAIRS) {  // lo, hi: the four turns of x's pairs and of y's
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float2 c = lo[e / 2], d = hi[e / 2];
+      const float x1 = (float)x[e], x2 = (float)x[e + 1], y1 = (float)y[e], y2 = (float)y[e + 1];
+      x[e] = (f16)(x1 * c.x - x2 * c.y);
+      x[e + 1] = (f16)(x2 * c.x + x1 * c.y);
+      y[e] = (f16)(y1 * d.x - y2 * d.y);
+      y[e + 1] = (f16)(y2 * d.x + y1 * d.y);
+    }
+  } else {  // lo: the eight turns of x's elements with y's
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 c = lo[e];
+      const float x1 = (float)x[e], x2 = (float)y[e];
+      x[e] = (f16)(x1 * c.x - x2 * c.y);
+      y[e] = (f16)(x2 * c.x + x1 * c.y);
+    }
+  }
+}
+
+template <bool PAIRS, bool SCATTER>
+__global__ void __launch_bounds__(256) k_rotary(const RotaryArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  float2* turns = reinterpret_cast<float2*>(smem);  // [row][pair]
+  const int half = a.rotary_dim / 2, R = a.rotary_dim / 16;
+  const int row0 = blockIdx.x * a.rows_per_block;
+  const int rows = min(a.rows_per_block, a.n_rows - row0);
+  long long* pool_row = reinterpret_cast<long long*>(turns + (size_t)a.rows_per_block * half);
+  for (int e = threadIdx.x; e < rows * half; e += 256)
+    turns[e] = turn_of(a, row0 + e / half, e % half);
+  if (SCATTER)
+    for (int e = threadIdx.x; e < rows; e += 256) pool_row[e] = pool_row_of(a, row0 + e);
+  __syncthreads();
+  // a head's units: R that turn and, where rows move, those behind them; v's heads move whole
+  const int units = SCATTER ? a.head_dim / 16 : R;
+  const int heads = a.n_heads + (SCATTER ? 2 : 1) * a.n_kv_heads;
+  const int per_row = heads * units;
+  for (int e = threadIdx.x; e < rows * per_row; e += 256) {
+    const int r = e / per_row, head = e % per_row / units, u = e % units;
+    const size_t row = row0 + r;
+    const int kv = head - a.n_heads, vv = kv - a.n_kv_heads;
+    const f16* src;
+    f16* dst;
+    if (kv < 0) {
+      src = a.q + row * a.ldq + (size_t)head * a.head_dim;
+      dst = a.q_out + row * a.ldq_out + (size_t)head * a.head_dim;
+    } else {
+      const long long to = SCATTER ? pool_row[r] : (long long)row;
+      if (to < 0) continue;
+      const bool is_v = SCATTER && vv >= 0;
+      const int h = is_v ? vv : kv;
+      src = (is_v ? a.v : a.k) + row * a.ldk + (size_t)h * a.head_dim;
+      dst = (is_v ? a.v_out : a.k_out) + to * a.ldk_out + (size_t)h * a.head_dim;
+    }
+    const bool moves = SCATTER && (u >= R || vv >= 0);
+    const int i = moves ? 2 * u : u, j = moves ? 2 * u + 1 : u + R;
+    f16x8 x = as_h8(ld16_stream(src + 8 * i)), y = as_h8(ld16_stream(src + 8 * j));
+    if (!moves) {
+      const float2* t = turns + (size_t)r * half;
+      if (PAIRS) turn<true>(x, y, t + 4 * i, t + 4 * j);
+      else turn<false>(x, y, t + 8 * i, nullptr);
+    }
+    st16_stream(dst + 8 * i, as_u4(x));
+    st16_stream(dst + 8 * j, as_u4(y));
+  }
+}
+
+// Any sizes, strides and alignment, in place: a pair for each thread and step.
+template <bool PAIRS>
+__global__ void __launch_bounds__(256) k_rotary_scalar(const RotaryArgs a) {
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  float2* turns = reinterpret_cast<float2*>(smem);
+  const int half = a.rotary_dim / 2;
+  const int row0 = blockIdx.x * a.rows_per_block;
+  const int rows = min(a.rows_per_block, a.n_rows - row0);
+  for (int e = threadIdx.x; e < rows * half; e += 256)
+    turns[e] = turn_of(a, row0 + e / half, e % half);
+  __syncthreads();
+  const int per_row = (a.n_heads + a.n_kv_heads) * half;
+  for (int e = threadIdx.x; e < rows * per_row; e += 256) {
+    const int r = e / per_row, head = e % per_row / half, i = e % half;
+    const size_t row = row0 + r;
+    f16* x = head < a.n_heads ? a.q_out + row * a.ldq + (size_t)head * a.head_dim
+                              : a.k_out + row * a.ldk + (size_t)(head - a.n_heads) * a.head_dim;
+    f16 *p1 = x + (PAIRS ? 2 * i : i), *p2 = PAIRS ? p1 + 1 : p1 + half;
+    const float2 c = turns[(size_t)r * half + i];
+    const float x1 = (float)*p1, x2 = (float)*p2;
+    *p1 = (f16)(x1 * c.x - x2 * c.y);
+    *p2 = (f16)(x2 * c.x + x1 * c.y);
+  }
+}
+
+// Rows of a block: its cosines and sines fill at most 32 KiB.
+int rows_of_block(int n_rows, int half, int most) {
+  int rows = 1;
+  while (rows < most && (size_t)2 * rows * half * 8 <= 32768 && n_rows / (2 * rows) >= 512) rows *= 2;
+  return rows;
+}
+
+int check_turn(const float* inv_freq, const int32_t* positions, int rotary_dim, int n_tables, int layout) {
+  if (!inv_freq || !positions || n_tables <= 0 ||
+      (layout != LLMK_ROTARY_HALVES && layout != LLMK_ROTARY_PAIRS))
+    return LLMK_ERR_INVALID_VALUE;
+  return rotary_dim % 2 ? LLMK_ERR_SHAPE : LLMK_OK;
+}
+
+}  // namespace
+}  // namespace llmk
+
+using namespace llmk;
+
+extern "C" int llmk_rotary_apply(uint16_t* q, int ldq, uint16_t* k, int ldk, const int32_t* positions,
+                                 const float* inv_freq, const int32_t* table_ids, const float* scales,
+                                 int n_rows, int n_heads, int n_kv_heads, int head_dim, int rotary_dim,
+                                 int n_tables, int layout, void* stream) {
+  if (n_rows < 0 || n_heads < 0 || n_kv_heads < 0 || head_dim <= 0 || rotary_dim <= 0)
+    return LLMK_ERR_INVALID_VALUE;
+  if (rotary_dim > head_dim || (long long)ldq < (long long)n_heads * head_dim ||
+      (long long)ldk < (long long)n_kv_heads * head_dim)
+    return LLMK_ERR_SHAPE;
+  if (n_rows == 0 || (n_heads == 0 && n_kv_heads == 0)) return LLMK_OK;
+  if ((n_heads > 0 && !q) || (n_kv_heads > 0 && !k)) return LLMK_ERR_INVALID_VALUE;
+  const int st = check_turn(inv_freq, positions, rotary_dim, n_tables, layout);
+  if (st != LLMK_OK) return st;
+  if (head_dim > 4096) return LLMK_ERR_UNSUPPORTED;
+  RotaryArgs a{};
+  a.q = a.q_out = reinterpret_cast<f16*>(q);
+  a.k = a.k_out = reinterpret_cast<f16*>(k);
+  a.positions = positions;
+  a.table_ids = table_ids;
+  a.inv_freq = inv_freq;
+  a.scales = scales;
+  a.ldq = a.ldq_out = ldq;
+  a.ldk = a.ldk_out = ldk;
+  a.n_rows = n_rows;
+  a.n_heads = n_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.head_dim = head_dim;
+  a.rotary_dim = rotary_dim;
+  a.n_tables = n_tables;
+  a.rows_per_block = rows_of_block(n_rows, rotary_dim / 2, 16);
+  const unsigned blocks = ceil_div((size_t)n_rows, (size_t)a.rows_per_block);
+  const size_t lds = (size_t)a.rows_per_block * (rotary_dim / 2) * 8;
+  if (!grid_takes(blocks, 256) ||
+      (long long)a.rows_per_block * (n_heads + n_kv_heads) * head_dim > 0x7FFFFFFF - 4096)
+    return LLMK_ERR_UNSUPPORTED;
+  const bool vectors = head_dim % 8 == 0 && rotary_dim % 16 == 0 &&
+                       (n_heads == 0 || (aligned16(q) && ldq % 8 == 0)) &&
+                       (n_kv_heads == 0 || (aligned16(k) && ldk % 8 == 0));
+  const bool pairs = layout == LLMK_ROTARY_PAIRS;
+  return launch(vectors ? (pairs ? k_rotary<true, false> : k_rotary<false, false>)
+                        : (pairs ? k_rotary_scalar<true> : k_rotary_scalar<false>),
+                dim3(blocks), dim3(256), lds, static_cast<hipStream_t>(stream), a);
+}
+
+extern "C" int llmk_qkv_rotary_scatter(const uint16_t* qkv, int ld, uint16_t* q_out, uint16_t* k_pool,
+                                       uint16_t* v_pool, const int32_t* block_tables,
+                                       const int32_t* positions, const float* inv_freq,
+                                       const int32_t* table_ids, const float* scales, int n,
+                                       int max_pages, int page_size, int n_heads, int n_kv_heads,
+                                       int head_dim, int rotary_dim, int n_tables, int layout,
+                                       void* stream) {
+  if (n < 0 || max_pages <= 0 || page_size <= 0 || n_heads <= 0 || n_kv_heads <= 0 || head_dim <= 0 ||
+      rotary_dim <= 0)
+    return LLMK_ERR_INVALID_VALUE;
+  if (head_dim % 16 || rotary_dim % 16 || rotary_dim > head_dim || ld % 8 ||
+      (long long)ld < (n_heads + 2LL * n_kv_heads) * head_dim)
+    return LLMK_ERR_SHAPE;
+  if (n == 0) return LLMK_OK;
+  if (!qkv || !q_out || !k_pool || !v_pool || !block_tables) return LLMK_ERR_INVALID_VALUE;
+  const int st = check_turn(inv_freq, positions, rotary_dim, n_tables, layout);
+  if (st != LLMK_OK) return st;
+  if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_pool) || !aligned16(v_pool))
+    return LLMK_ERR_ALIGNMENT;
+  if (head_dim > 512) return LLMK_ERR_UNSUPPORTED;
+  RotaryArgs a{};
+  a.q = reinterpret_cast<const f16*>(qkv);
+  a.k = a.q + (size_t)n_heads * head_dim;
+  a.v = a.k + (size_t)n_kv_heads * head_dim;
+  a.q_out = reinterpret_cast<f16*>(q_out);
+  a.k_out = reinterpret_cast<f16*>(k_pool);
+  a.v_out = reinterpret_cast<f16*>(v_pool);
+  a.positions = positions;
+  a.table_ids = table_ids;
+  a.tables = block_tables;
+  a.inv_freq = inv_freq;
+  a.scales = scales;
+  a.ldq = a.ldk = ld;
+  a.ldq_out = n_heads * head_dim;
+  a.ldk_out = n_kv_heads * head_dim;
+  a.n_rows = n;
+  a.n_heads = n_heads;
+  a.n_kv_heads = n_kv_heads;
+  a.head_dim = head_dim;
+  a.rotary_dim = rotary_dim;
+  a.n_tables = n_tables;
+  a.max_pages = max_pages;
+  a.page_size = page_size;
+  a.rows_per_block = rows_of_block(n, rotary_dim / 2, 16);
+  const unsigned blocks = ceil_div((size_t)n, (size_t)a.rows_per_block);
+  const size_t lds = (size_t)a.rows_per_block * ((rotary_dim / 2) * 8 + 8);
+  if (!grid_takes(blocks, 256) ||
+      (long long)a.rows_per_block * (n_heads + 2LL * n_kv_heads) * head_dim > 0x7FFFFFFF - 4096)
+    return LLMK_ERR_UNSUPPORTED;
+  return launch(layout == LLMK_ROTARY_PAIRS ? k_rotary<true, true> : k_rotary<false, true>,
+                dim3(blocks), dim3(256), lds, static_cast<hipStream_t>(stream), a);
+}

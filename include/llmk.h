@@ -388,6 +388,141 @@ LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_lo
                                 void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Serving requests that are not alike: adapters of their own beside a shared projection, rotary
+ * positions of other layouts and scalings, and cache pages that sequences share. New entry points;
+ * the reference has one set of weights, one rotation and one holder for each page. Their C++ names in
+ * llmk.hpp are these without the prefix.
+ * ------------------------------------------------------------------------------------------ */
+
+/* Adds each sequence's low-rank adapter to the rows of a shared projection's output, in place:
+ *   y[r, n] = fp16(y[r, n] + scales[a] * sum_{j < ranks[a]} B_a[n, j] * (A_{a, p}[j, :] . x[r, :]))
+ * for a = adapter_ids[s] of row r's sequence s and the part p that column n lies in. The projection
+ * may be a fused one: its n_parts (1 to 8) parts end at columns part_ends[0] < part_ends[1] < .. (a
+ * HOST array; q|k|v, gate|up; one part: its width), and an adapter has an A for each of them.
+ * a [n_adapters, n_parts, max_rank, in_features], b [n_adapters, part_ends[n_parts - 1], max_rank];
+ * ranks [n_adapters], or NULL for max_rank: what lies past an adapter's rank is not read as numbers.
+ * scales [n_adapters], or NULL for 1. Sequence s owns the rows row_starts[s] .. row_starts[s + 1] - 1
+ * (NULL: one row each, n_rows == n_seqs), as the batches of the 8-bit cache do. Rows of no
+ * sequence, of an adapter outside [0, n_adapters) and of one of rank <= 0 are left as they are, bit
+ * for bit; a row depends on its own x, y and adapter alone. Sums in fp32; between the two products 22
+ * bits of a row's values relative to its largest one of the part; one rounding.
+ * x rows have stride ldx and y rows ldy (elements, multiples of 8); in_features, max_rank (at most
+ * 256) and the part ends are multiples of 8; x, a, b and y are 16-byte aligned. x and y may not overlap.
+ * workspace: llmk_lora_add_workspace_floats(..) floats, 16-byte aligned; calls that may overlap need
+ * one each, graphs replayed one behind the other may share one. LLMK_ERR_UNSUPPORTED for more than
+ * 2^20 rows or sequences. */
+LLMK_API size_t llmk_lora_add_workspace_floats(int n_rows, int n_seqs, int n_adapters, int max_rank,
+                                               int in_features, int n_parts);
+LLMK_API int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, const uint16_t* b,
+                           const int32_t* ranks, const float* scales, const int32_t* adapter_ids,
+                           const int32_t* row_starts, uint16_t* y, int ldy,
+                           const int32_t* part_ends, int n_parts, float* workspace, int n_rows,
+                           int n_seqs, int n_adapters, int max_rank, int in_features,
+                           void* stream);
+
+/* Which elements of a head's first rotary_dim turn together: i and i + rotary_dim / 2, or 2 i and
+ * 2 i + 1. */
+#define LLMK_ROTARY_HALVES 0
+#define LLMK_ROTARY_PAIRS 1
+
+/* Rotates the first rotary_dim elements of every head of q and k where they lie; the rest of a head is
+ * neither read nor written. Row r of q (stride ldq elements) holds n_heads heads of head_dim, row r of k
+ * (stride ldk) n_kv_heads; they may be columns of one fused projection. With t = table_ids[r], the angle
+ * of pair i is positions[r] * inv_freq[t, i] and
+ *   x1' = fp16(scales[t] (x1 cos - x2 sin)), x2' = fp16(scales[t] (x2 cos + x1 sin)):
+ * angles, cosines and sines in 64 bits, products in 32, one rounding. inv_freq [n_tables, rotary_dim / 2],
+ * scales [n_tables] or NULL for 1, table_ids [n_rows] or NULL for 0 (values outside [0, n_tables) count as
+ * 0). Positions may be any. rotary_dim is even, from 2 to head_dim <= 4096. Any alignment and strides; 16-byte
+ * vectors where q, k and their strides are whole ones, head_dim % 8 == 0 and rotary_dim % 16 == 0.
+ * Beside llmk_rope_apply, which has one table, whole heads and the reference's fp16 steps. */
+LLMK_API int llmk_rotary_apply(uint16_t* q, int ldq, uint16_t* k, int ldk, const int32_t* positions,
+                               const float* inv_freq, const int32_t* table_ids, const float* scales,
+                               int n_rows, int n_heads, int n_kv_heads, int head_dim, int rotary_dim,
+                               int n_tables, int layout, void* stream);
+
+/* The same rotation on the way from a fused projection into the paged cache: row r of qkv (stride ld) holds
+ * q, k and v as for llmk_qkv_rope_scatter; q goes to q_out [n, n_heads, head_dim], k (rotated) and v to the
+ * pools [num_pages, page_size, n_kv_heads, head_dim] at positions[r] by block_tables[r, :] [n, max_pages].
+ * Rows whose position is below 0 or past the table, or whose table entry is negative, write no k and v.
+ * head_dim % 16 == 0, up to 512; rotary_dim % 16 == 0; ld % 8 == 0; qkv, q_out and the pools 16-byte aligned and
+ * not overlapping. */
+LLMK_API int llmk_qkv_rotary_scatter(const uint16_t* qkv, int ld, uint16_t* q_out, uint16_t* k_pool,
+                                     uint16_t* v_pool, const int32_t* block_tables,
+                                     const int32_t* positions, const float* inv_freq,
+                                     const int32_t* table_ids, const float* scales, int n, int max_pages,
+                                     int page_size, int n_heads, int n_kv_heads, int head_dim,
+                                     int rotary_dim, int n_tables, int layout, void* stream);
+
+/* Host function: one frequency table (rotary_dim / 2 values, in 64 bits until the last rounding) and the
+ * scale that goes with it. f_i = theta^(-2 i / rotary_dim);
+ *   _PLAIN: f_i.  _LINEAR: f_i / factor (positions interpolated).
+ *   _NTK: theta grown to theta * factor^(rotary_dim / (rotary_dim - 2)): the fastest pair turns as before, the
+ *     slowest factor times slower (rotary_dim 2: as _PLAIN).
+ *   _YARN: f_i / factor for pairs that turn fewer than beta_slow times within original_max_pos positions, f_i
+ *     for those that turn more than beta_fast times, mixed in between linearly in i:
+ *     d(b) = rotary_dim ln(original_max_pos / (2 pi b)) / (2 ln theta), low = max(floor d(beta_fast), 0), high =
+ *     max(min(ceil d(beta_slow), rotary_dim - 1), low + 0.001), m = clamp((i - low) / (high - low), 0, 1),
+ *     out = f_i (1 - m) + f_i / factor * m; *scale = 0.1 ln(factor) + 1 for factor > 1.
+ * *scale (may be NULL) is 1 for the others. original_max_pos, beta_fast and beta_slow are read for _YARN alone.
+ * The Llama-3 scaling is llmk_compute_rope_inv_freq. */
+#define LLMK_ROTARY_PLAIN 0
+#define LLMK_ROTARY_LINEAR 1
+#define LLMK_ROTARY_NTK 2
+#define LLMK_ROTARY_YARN 3
+LLMK_API int llmk_compute_rotary_inv_freq(int scaling, int rotary_dim, double theta, double factor,
+                                          double original_max_pos, double beta_fast,
+                                          double beta_slow, float* out, float* scale);
+
+/* Cache pages that sequences share, on the GPU. refs [num_pages] counts the holders of each page (0: free). A
+ * sequence holds the pages that its row of a block table names, up to the first entry that is no page (negative or
+ * past the pool), and its tokens fill them in order, page_size a page. Only whole pages are shared. */
+
+/* Copies pages within pools: pair i of copies [n_copies, 2] is (from, to); the same pairs for all n_pools pools.
+ * pools and page_bytes are HOST arrays: the pools' device pointers and the bytes of a page in each (K and V of
+ * every layer, the scales of an 8-bit cache: any layout whose pages are page_bytes apart; pointers and sizes
+ * multiples of 4). Pairs with an entry outside [0, num_pages) or two equal ones copy nothing. No page may be
+ * written twice, nor read and written. count: NULL, or the device address of the number of pairs (n_copies at
+ * most), as llmk_kv_compact leaves it. n_pools any number from 0. */
+LLMK_API int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, int n_pools,
+                                const int32_t* copies, const int32_t* count, int n_copies,
+                                int num_pages, void* stream);
+
+/* The step from one batch to the next: child c continues sequence parents[c] of the old batch (outside
+ * [0, n_old): begins empty), sharing its whole pages, with room for reserve[c] more tokens (reserve NULL: none;
+ * negative counts as 0). Sequences without children let go of their pages: beam search, several samples of one
+ * prompt, requests that join and leave. Old: block_tables [n_old, max_pages], seq_lens [n_old] (cut to what the
+ * pages held can hold, and to 0 from below). With L the parent's length, whole = L / page_size and need =
+ * ceil((L + reserve) / page_size), at most max_pages, entry j of new_tables [n_new, max_pages] is
+ *   j < whole: the parent's page;
+ *   whole <= j < need: the parent's page if c is its first child and nobody else held the page before the call,
+ *     else a fresh one; if it replaces the page that L ends inside, copies[c] = (parent's page, fresh page);
+ *   j >= need: -1.
+ * Fresh pages are the lowest-numbered ones that nobody holds once the old batch has let go and the new one has
+ * taken over, in the order of (c, j); where they run out the entry is -1. new_lens [n_new] = L; copies
+ * [n_new, 2] is (-1, -1) where nothing is to be copied (llmk_kv_copy_pages does that); counts [2] = fresh pages
+ * given, and lacking (the table's row of a child that lacks some is then too short for L + reserve). refs is
+ * brought up to date. n_new == 0 frees the old batch. New and old arrays may not overlap.
+ * workspace: llmk_kv_fork_workspace_ints(..) int32. Batches up to 65535 sequences. */
+LLMK_API size_t llmk_kv_fork_workspace_ints(int n_old, int n_new, int max_pages, int num_pages);
+LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
+                          const int32_t* parents, const int32_t* reserve, int32_t* refs,
+                          int32_t* new_tables, int32_t* new_lens, int32_t* copies,
+                          int32_t* counts, int32_t* workspace, int n_old, int n_new,
+                          int max_pages, int page_size, int num_pages, void* stream);
+
+/* Moves the pages that are held (refs > 0) to the pool's front: with n of them, the k-th held page at or past n
+ * goes to the k-th free page below n. new_tables [n_seqs, max_pages] names pages by their new numbers (entries
+ * that are no held page stay as they are), new_refs [num_pages] counts their holders; copies [num_pages / 2, 2]
+ * gets the pairs (from, to), whose number is counts[0] (counts[1] = n), for llmk_kv_copy_pages. new_tables may be
+ * block_tables, new_refs may be refs. workspace: llmk_kv_compact_workspace_ints(num_pages) int32. num_pages up to
+ * 2^24. */
+LLMK_API size_t llmk_kv_compact_workspace_ints(int num_pages);
+LLMK_API int llmk_kv_compact(const int32_t* block_tables, const int32_t* refs, int32_t* new_tables,
+                             int32_t* new_refs, int32_t* copies, int32_t* counts,
+                             int32_t* workspace, int n_seqs, int max_pages, int num_pages,
+                             void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * The decode step around the kernels above: projections, the fused layouts they
  * produce, and an engine that runs a whole Llama-3 forward pass over a batch of token rows.
  * ------------------------------------------------------------------------------------------ */

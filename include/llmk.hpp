@@ -219,3 +219,91 @@ inline void verify_drafts(const __half* logits, const __half* draft_logits, cons
                          n_seqs, vocab, stream),
       "verify_drafts");
 }
+
+// Serving requests that are not alike (new entry points, documented in llmk.h): a violated precondition is a
+// fatal host error, as above.
+inline size_t lora_add_workspace_floats(int n_rows, int n_seqs, int n_adapters, int max_rank,
+                                        int in_features, int n_parts) {
+  return llmk_lora_add_workspace_floats(n_rows, n_seqs, n_adapters, max_rank, in_features, n_parts);
+}
+
+inline void lora_add(const __half* x, int ldx, const __half* a, const __half* b, const int* ranks,
+                     const float* scales, const int* adapter_ids, const int* row_starts, __half* y,
+                     int ldy, const int* part_ends, int n_parts, float* workspace, int n_rows,
+                     int n_seqs, int n_adapters, int max_rank, int in_features,
+                     hipStream_t stream = 0) {
+  llmk_shim::check(
+      llmk_lora_add(llmk_shim::h(x), ldx, llmk_shim::h(a), llmk_shim::h(b), ranks, scales, adapter_ids,
+                    row_starts, llmk_shim::h(y), ldy, part_ends, n_parts, workspace, n_rows, n_seqs,
+                    n_adapters, max_rank, in_features, stream),
+      "lora_add");
+}
+
+inline void rotary_apply(__half* q, int ldq, __half* k, int ldk, const int* positions,
+                         const float* inv_freq, const int* table_ids, const float* scales, int n_rows,
+                         int n_heads, int n_kv_heads, int head_dim, int rotary_dim, int n_tables,
+                         int layout, hipStream_t stream = 0) {
+  llmk_shim::check(
+      llmk_rotary_apply(llmk_shim::h(q), ldq, llmk_shim::h(k), ldk, positions, inv_freq, table_ids,
+                        scales, n_rows, n_heads, n_kv_heads, head_dim, rotary_dim, n_tables, layout,
+                        stream),
+      "rotary_apply");
+}
+
+inline void qkv_rotary_scatter(const __half* qkv, int ld, __half* q_out, __half* k_pool,
+                               __half* v_pool, const int* block_tables, const int* positions,
+                               const float* inv_freq, const int* table_ids, const float* scales, int n,
+                               int max_pages, int page_size, int n_heads, int n_kv_heads, int head_dim,
+                               int rotary_dim, int n_tables, int layout, hipStream_t stream = 0) {
+  llmk_shim::check(
+      llmk_qkv_rotary_scatter(llmk_shim::h(qkv), ld, llmk_shim::h(q_out), llmk_shim::h(k_pool),
+                              llmk_shim::h(v_pool), block_tables, positions, inv_freq, table_ids, scales,
+                              n, max_pages, page_size, n_heads, n_kv_heads, head_dim, rotary_dim,
+                              n_tables, layout, stream),
+      "qkv_rotary_scatter");
+}
+
+inline std::vector<float> compute_rotary_inv_freq(int scaling, int rotary_dim, double theta,
+                                                  double factor, double original_max_pos,
+                                                  double beta_fast, double beta_slow,
+                                                  float* scale = nullptr) {
+  std::vector<float> out(rotary_dim > 0 ? rotary_dim / 2 : 0);
+  llmk_shim::check(llmk_compute_rotary_inv_freq(scaling, rotary_dim, theta, factor, original_max_pos,
+                                                beta_fast, beta_slow, out.data(), scale),
+                   "compute_rotary_inv_freq");
+  return out;
+}
+
+inline void kv_copy_pages(void* const* pools, const size_t* page_bytes, int n_pools,
+                          const int* copies, const int* count, int n_copies, int num_pages,
+                          hipStream_t stream = 0) {
+  llmk_shim::check(llmk_kv_copy_pages(pools, page_bytes, n_pools, copies, count, n_copies, num_pages,
+                                      stream),
+                   "kv_copy_pages");
+}
+
+inline size_t kv_fork_workspace_ints(int n_old, int n_new, int max_pages, int num_pages) {
+  return llmk_kv_fork_workspace_ints(n_old, n_new, max_pages, num_pages);
+}
+
+inline void kv_fork(const int* block_tables, const int* seq_lens, const int* parents,
+                    const int* reserve, int* refs, int* new_tables, int* new_lens, int* copies,
+                    int* counts, int* workspace, int n_old, int n_new, int max_pages, int page_size,
+                    int num_pages, hipStream_t stream = 0) {
+  llmk_shim::check(llmk_kv_fork(block_tables, seq_lens, parents, reserve, refs, new_tables, new_lens,
+                                copies, counts, workspace, n_old, n_new, max_pages, page_size,
+                                num_pages, stream),
+                   "kv_fork");
+}
+
+inline size_t kv_compact_workspace_ints(int num_pages) {
+  return llmk_kv_compact_workspace_ints(num_pages);
+}
+
+inline void kv_compact(const int* block_tables, const int* refs, int* new_tables, int* new_refs,
+                       int* copies, int* counts, int* workspace, int n_seqs, int max_pages,
+                       int num_pages, hipStream_t stream = 0) {
+  llmk_shim::check(llmk_kv_compact(block_tables, refs, new_tables, new_refs, copies, counts, workspace,
+                                   n_seqs, max_pages, num_pages, stream),
+                   "kv_compact");
+}
