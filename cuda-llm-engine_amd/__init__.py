@@ -765,23 +765,17 @@ def verify_drafts(logits, draft_logits, drafts, row_starts, temperature, accept_
 # serving requests that are not alike: adapters, rotary layouts and scalings, shared cache pages
 # ---------------------------------------------------------------------------------------------
 def _rows(fn: str, t, n: int, ld: int, width: int, name: str) -> int:
-    """The address of n rows of `width` values, `ld` apart, that begin where t does. t may be a view of
-    a wider tensor's columns: its storage has to hold the rows, its last dimension to be unbroken."""
+    """The address of n rows of `width` values, ld apart: a matrix whose rows are that far apart (columns of
+    a wider one, too), or a contiguous tensor of another shape."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float16:
         _fail(fn, f"{name} must be a CUDA tensor of {torch.float16}")
-    if n == 0 or width == 0:
-        return t.data_ptr()
-    if t.dim() == 0 or (t.stride(-1) != 1 and t.shape[-1] > 1):
-        _fail(fn, f"{name}'s last dimension must be contiguous")
-    if t.dim() == 2 and t.shape[0] > 1 and t.stride(0) != ld:
-        _fail(fn, f"{name}'s rows are {t.stride(0)} apart, not {ld}")
-    if t.dim() != 2 and not t.is_contiguous():
-        _fail(fn, f"{name} must be contiguous or a matrix")
-    held = t.untyped_storage().nbytes() // 2 - t.storage_offset()
-    if t.numel() == 0 or held < (n - 1) * ld + width:
-        _fail(fn, f"{name} holds {held} elements, the call touches {(n - 1) * ld + width}")
-    if t.dim() == 2 and (t.shape[0] < n or t.shape[1] < width):
-        _fail(fn, f"{name} is {list(t.shape)}, the call touches [{n}, {width}]")
+    if n > 0 and width > 0 and t.dim() == 2:
+        if t.shape[0] < n or t.shape[1] < width:
+            _fail(fn, f"{name} is {list(t.shape)}, the call touches [{n}, {width}]")
+        if (t.shape[0] > 1 and t.stride(0) != ld) or (t.shape[1] > 1 and t.stride(1) != 1):
+            _fail(fn, f"{name}'s strides are {t.stride()}, not ({ld}, 1)")
+    elif n > 0 and width > 0:
+        _dev(fn, t, torch.float16, (n - 1) * ld + width, name)
     return t.data_ptr()
 
 
@@ -802,6 +796,11 @@ def lora_add(x, ldx: int, a, b, ranks, scales, adapter_ids, row_starts, y, ldy: 
     ``check_indices`` refuses row_starts that do not ascend from 0 to at most n_rows and ranks past
     max_rank."""
     fn = "lora_add"
+    if not _want_checks(check_indices):
+        st = _fast.lora_add(x, ldx, a, b, ranks, scales, adapter_ids, row_starts, y, ldy, part_ends,
+                            workspace, n_rows, n_seqs, n_adapters, max_rank, in_features, stream)
+        if st is not None:
+            return _check(fn, st)
     if min(n_rows, n_seqs, n_adapters) < 0 or min(max_rank, in_features) <= 0:
         _fail(fn, "n_rows, n_seqs and n_adapters must be >= 0 and the other sizes > 0")
     ends = (ctypes.c_int32 * max(1, len(part_ends)))(*part_ends)
@@ -859,6 +858,11 @@ def rotary_apply(q, ldq: int, k, ldk: int, positions, inv_freq, table_ids, scale
     inv_freq [tables, rotary_dim / 2], table_ids and scales may be None; ``layout``: ROTARY_HALVES or
     ROTARY_PAIRS. ``check_indices`` refuses table_ids that name no table."""
     fn = "rotary_apply"
+    if not _want_checks(check_indices):
+        st = _fast.rotary_apply(q, ldq, k, ldk, positions, inv_freq, table_ids, scales, n_rows, n_heads,
+                                n_kv_heads, head_dim, rotary_dim, layout, stream)
+        if st is not None:
+            return _check(fn, st)
     pq = _rows(fn, q, n_rows, ldq, n_heads * head_dim, "q") if n_heads else None
     pk = _rows(fn, k, n_rows, ldk, n_kv_heads * head_dim, "k") if n_kv_heads else None
     pp, pf, pt, ps, n_tables = _tables(fn, positions, inv_freq, table_ids, scales, n_rows, rotary_dim,
@@ -875,6 +879,12 @@ def qkv_rotary_scatter(qkv, ld: int, q_out, k_pool, v_pool, block_tables, positi
     """The rotation of rotary_apply on the way from a fused projection's rows into the paged fp16 cache
     (``llmk_qkv_rotary_scatter``). ``check_indices`` refuses rows that have no page of the pools."""
     fn = "qkv_rotary_scatter"
+    if not _want_checks(check_indices):
+        st = _fast.qkv_rotary_scatter(qkv, ld, q_out, k_pool, v_pool, block_tables, positions, inv_freq,
+                                      table_ids, scales, n, max_pages, page_size, n_heads, n_kv_heads,
+                                      head_dim, rotary_dim, layout, stream)
+        if st is not None:
+            return _check(fn, st)
     if min(max_pages, page_size, n_heads, n_kv_heads, head_dim) <= 0:
         _fail(fn, "max_pages, page_size, the head counts and head_dim must be > 0")
     check = _want_checks(check_indices)
@@ -914,6 +924,10 @@ def kv_copy_pages(pools, copies, count, n_copies: int, num_pages: int, stream=No
     count: None, or kv_compact's counts. ``check_indices`` refuses a page that two pairs write, and one
     that is written and read."""
     fn = "kv_copy_pages"
+    if not _want_checks(check_indices):
+        st = _fast.kv_copy_pages(pools, copies, count, n_copies, num_pages, stream)
+        if st is not None:
+            return _check(fn, st)
     if n_copies < 0 or num_pages <= 0:
         _fail(fn, "n_copies must be >= 0 and num_pages > 0")
     pc = _dev(fn, copies, torch.int32, 2 * n_copies, "copies")
@@ -958,6 +972,11 @@ def kv_fork(block_tables, seq_lens, parents, reserve, refs, new_tables, new_lens
     nobody holds any more are free (``llmk_kv_fork``; kv_copy_pages then makes the copies that it
     names). ``check_indices`` refuses counts in refs that are not the block tables' holders."""
     fn = "kv_fork"
+    if not _want_checks(check_indices):
+        st = _fast.kv_fork(block_tables, seq_lens, parents, reserve, refs, new_tables, new_lens, copies,
+                           counts, workspace, n_old, n_new, max_pages, page_size, num_pages, stream)
+        if st is not None:
+            return _check(fn, st)
     if min(n_old, n_new) < 0 or min(max_pages, page_size, num_pages) <= 0:
         _fail(fn, "n_old and n_new must be >= 0 and the other sizes > 0")
     i32 = torch.int32
@@ -993,6 +1012,10 @@ def kv_compact(block_tables, refs, new_tables, new_refs, copies, counts, workspa
     """Renumbers the pages that are held to the pool's front (``llmk_kv_compact``; kv_copy_pages with its
     copies and counts then moves them). In place where new_tables is block_tables, new_refs refs."""
     fn = "kv_compact"
+    st = _fast.kv_compact(block_tables, refs, new_tables, new_refs, copies, counts, workspace, n_seqs,
+                          max_pages, num_pages, stream)
+    if st is not None:
+        return _check(fn, st)
     if n_seqs < 0 or min(max_pages, num_pages) <= 0:
         _fail(fn, "n_seqs must be >= 0 and the other sizes > 0")
     i32 = torch.int32

@@ -15,7 +15,8 @@
 
 static PyObject *tensor_type, *half_dtype, *int_dtype, *float_dtype, *get_device, *get_stream,
     *e4m3_dtype;
-static PyObject *s_is_cuda, *s_dtype, *s_is_contiguous, *s_numel, *s_data_ptr, *s_get_device;
+static PyObject *s_is_cuda, *s_dtype, *s_is_contiguous, *s_numel, *s_data_ptr, *s_get_device, *s_shape, *s_stride,
+    *s_element_size;
 
 /* The device address of t when it is a contiguous CUDA torch.Tensor of this dtype with at least
  * `least` elements; 0 otherwise, with no exception set. (A tensor of no elements has no address
@@ -89,6 +90,55 @@ static void* address_on(PyObject* t, PyObject* dtype, long long least, long long
   }
   if (numel) *numel = n;
   return p;
+}
+
+/* What a call without arguments answers, as a number; -1 and no exception where it has none. */
+static long long number_of(PyObject* t, PyObject* method) {
+  long long n = -1;
+  PyObject* v = PyObject_CallMethodNoArgs(t, method);
+  if (v) {
+    n = PyLong_AsLongLong(v);
+    Py_DECREF(v);
+  }
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    n = -1;
+  }
+  return n;
+}
+
+/* A tuple's number i, -1 without an exception where there is none. */
+static long long item_of(PyObject* tuple, Py_ssize_t i) {
+  const long long n = PyLong_AsLongLong(PyTuple_GET_ITEM(tuple, i));
+  if (n == -1 && PyErr_Occurred()) PyErr_Clear();
+  return n;
+}
+
+/* address_on() of n >= 1 rows of `width` halves, ld apart: a matrix of at least so many rows and columns
+ * whose rows are ld apart (columns of a wider one, too), or a contiguous tensor of another shape. */
+static void* rows_on(PyObject* t, long long n, long long ld, long long width, long long device) {
+  if ((PyObject*)Py_TYPE(t) != tensor_type) return NULL;
+  PyObject* shape = PyObject_GetAttr(t, s_shape);
+  if (!shape || !PyTuple_Check(shape) || PyTuple_GET_SIZE(shape) != 2) {
+    if (!shape) PyErr_Clear();
+    Py_XDECREF(shape);
+    return address_on(t, half_dtype, (n - 1) * ld + width, device, NULL);
+  }
+  const long long rows = item_of(shape, 0), columns = item_of(shape, 1);
+  Py_DECREF(shape);
+  if (rows < n || columns < width || number_of(t, s_get_device) != device || device < 0) return NULL;
+  PyObject* v = PyObject_GetAttr(t, s_dtype);
+  const int half = v == half_dtype;
+  if (!v) PyErr_Clear();
+  Py_XDECREF(v);
+  if (!half) return NULL;
+  v = PyObject_CallMethodNoArgs(t, s_stride);
+  const int fits = v && PyTuple_Check(v) && PyTuple_GET_SIZE(v) == 2 &&
+                   (rows == 1 || item_of(v, 0) == ld) && (columns == 1 || item_of(v, 1) == 1);
+  if (!v) PyErr_Clear();
+  Py_XDECREF(v);
+  const long long at = fits ? number_of(t, s_data_ptr) : 0;
+  return at > 0 ? (void*)(uintptr_t)at : NULL;
 }
 
 /* torch's current stream for None, the number itself for a number. */
@@ -409,6 +459,169 @@ FUNCTION(verify_drafts, 14)
                             n_accepted, tokens, workspace, n_rows, n_seqs, vocab, stream));
 }
 
+#define ROWS_ON(name, at, n, ld, width)                                 \
+  uint16_t* name = (uint16_t*)rows_on(args[at], n, ld, width, here);     \
+  if (!name) Py_RETURN_NONE
+
+FUNCTION(lora_add, 18)
+  COUNT(ldx, 1);
+  COUNT(ldy, 9);
+  COUNT(n_rows, 12);
+  COUNT(n_seqs, 13);
+  COUNT(n_adapters, 14);
+  COUNT(max_rank, 15);
+  COUNT(in, 16);
+  PyObject* parts = args[10];
+  const int is_tuple = PyTuple_CheckExact(parts);
+  if (!is_tuple && !PyList_CheckExact(parts)) Py_RETURN_NONE;
+  const Py_ssize_t n_parts = is_tuple ? PyTuple_GET_SIZE(parts) : PyList_GET_SIZE(parts);
+  int32_t ends[8];
+  if (n_parts < 1 || n_parts > 8) Py_RETURN_NONE;
+  for (Py_ssize_t i = 0; i < n_parts; ++i)
+    if (!count_of(is_tuple ? PyTuple_GET_ITEM(parts, i) : PyList_GET_ITEM(parts, i), &ends[i]))
+      Py_RETURN_NONE;
+  const long long out = ends[n_parts - 1];
+  if (!n_rows || !n_seqs || !n_adapters || !max_rank || !in || !out || max_rank > 65535 || n_adapters > 1 << 20)
+    Py_RETURN_NONE;
+  const size_t floats = llmk_lora_add_workspace_floats(n_rows, n_seqs, n_adapters, max_rank, in, (int)n_parts);
+  if (floats > (size_t)LLONG_MAX || in > 1 << 24 || out > 1 << 24) Py_RETURN_NONE;
+  HERE(17);
+  ROWS_ON(x, 0, n_rows, ldx, in);
+  TENSOR_ON(uint16_t, a, 2, half_dtype, (long long)n_adapters * (int)n_parts * max_rank * in);
+  TENSOR_ON(uint16_t, b, 3, half_dtype, (long long)n_adapters * out * max_rank);
+  OPT_ON(int32_t, ranks, 4, int_dtype, n_adapters);
+  OPT_ON(float, scales, 5, float_dtype, n_adapters);
+  TENSOR_ON(int32_t, ids, 6, int_dtype, n_seqs);
+  OPT_ON(int32_t, starts, 7, int_dtype, n_seqs + 1LL);
+  ROWS_ON(y, 8, n_rows, ldy, out);
+  TENSOR_ON(float, workspace, 11, float_dtype, (long long)floats);
+  ANSWER(llmk_lora_add(x, ldx, a, b, ranks, scales, ids, starts, y, ldy, ends, (int)n_parts, workspace,
+                       n_rows, n_seqs, n_adapters, max_rank, in, stream));
+}
+
+/* The tensors of a rotation, at `at` and the three behind; n_tables is how many inv_freq holds. */
+#define TURNS(at, n)                                                                                  \
+  if (!rotary || rotary % 2) Py_RETURN_NONE;                                                          \
+  TENSOR_ON(int32_t, positions, at, int_dtype, n);                                                    \
+  long long frequencies = 0;                                                                          \
+  float* inv_freq = (float*)address_on(args[(at) + 1], float_dtype, rotary / 2, here, &frequencies);  \
+  if (!inv_freq || frequencies / (rotary / 2) > INT_MAX) Py_RETURN_NONE;                              \
+  const int n_tables = (int)(frequencies / (rotary / 2));                                             \
+  OPT_ON(int32_t, table_ids, (at) + 2, int_dtype, n);                                                 \
+  OPT_ON(float, scales, (at) + 3, float_dtype, n_tables)
+
+FUNCTION(rotary_apply, 15)
+  COUNT(ldq, 1);
+  COUNT(ldk, 3);
+  COUNT(n, 8);
+  COUNT(heads, 9);
+  COUNT(kv_heads, 10);
+  COUNT(head_dim, 11);
+  COUNT(rotary, 12);
+  COUNT(layout, 13);
+  if (!n || !heads || !kv_heads || !head_dim || heads > 65535 || kv_heads > 65535 || head_dim > 65535)
+    Py_RETURN_NONE;
+  HERE(14);
+  ROWS_ON(q, 0, n, ldq, (long long)heads * head_dim);
+  ROWS_ON(k, 2, n, ldk, (long long)kv_heads * head_dim);
+  TURNS(4, n);
+  ANSWER(llmk_rotary_apply(q, ldq, k, ldk, positions, inv_freq, table_ids, scales, n, heads, kv_heads,
+                           head_dim, rotary, n_tables, layout, stream));
+}
+
+FUNCTION(qkv_rotary_scatter, 19)
+  COUNT(ld, 1);
+  COUNT(n, 10);
+  COUNT(max_pages, 11);
+  COUNT(page_size, 12);
+  COUNT(heads, 13);
+  COUNT(kv_heads, 14);
+  COUNT(head_dim, 15);
+  COUNT(rotary, 16);
+  COUNT(layout, 17);
+  if (!n || !max_pages || !page_size || !heads || !kv_heads || !head_dim || heads > 65535 ||
+      kv_heads > 65535 || head_dim > 65535)
+    Py_RETURN_NONE;
+  HERE(18);
+  ROWS_ON(qkv, 0, n, ld, (heads + 2LL * kv_heads) * head_dim);
+  TENSOR_ON(uint16_t, q_out, 2, half_dtype, (long long)n * heads * head_dim);
+  TENSOR_ON(uint16_t, k_pool, 3, half_dtype, 0);
+  TENSOR_ON(uint16_t, v_pool, 4, half_dtype, 0);
+  TENSOR_ON(int32_t, tables, 5, int_dtype, (long long)n * max_pages);
+  TURNS(6, n);
+  ANSWER(llmk_qkv_rotary_scatter(qkv, ld, q_out, k_pool, v_pool, tables, positions, inv_freq, table_ids,
+                                 scales, n, max_pages, page_size, heads, kv_heads, head_dim, rotary,
+                                 n_tables, layout, stream));
+}
+
+/* args: pools, a list of tensors of any type. */
+FUNCTION(kv_copy_pages, 6)
+  COUNT(n_copies, 3);
+  COUNT(num_pages, 4);
+  if (!n_copies || !num_pages || !PyList_CheckExact(args[0])) Py_RETURN_NONE;
+  const Py_ssize_t n_pools = PyList_GET_SIZE(args[0]);
+  void* pools[256];
+  size_t bytes[256];
+  if (n_pools > 256) Py_RETURN_NONE;
+  HERE(5);
+  for (Py_ssize_t i = 0; i < n_pools; ++i) {
+    PyObject* t = PyList_GET_ITEM(args[0], i);
+    if ((PyObject*)Py_TYPE(t) != tensor_type || number_of(t, s_get_device) != here) Py_RETURN_NONE;
+    PyObject* v = PyObject_CallMethodNoArgs(t, s_is_contiguous);
+    const int contiguous = v == Py_True;
+    if (!v) PyErr_Clear();
+    Py_XDECREF(v);
+    const long long numel = number_of(t, s_numel), each = number_of(t, s_element_size);
+    const long long at = number_of(t, s_data_ptr);
+    if (!contiguous || numel <= 0 || each <= 0 || at <= 0 || numel * each % num_pages) Py_RETURN_NONE;
+    pools[i] = (void*)(uintptr_t)at;
+    bytes[i] = (size_t)(numel * each / num_pages);
+  }
+  TENSOR_ON(int32_t, copies, 1, int_dtype, 2LL * n_copies);
+  OPT_ON(int32_t, count, 2, int_dtype, 1);
+  ANSWER(llmk_kv_copy_pages(pools, bytes, (int)n_pools, copies, count, n_copies, num_pages, stream));
+}
+
+FUNCTION(kv_fork, 16)
+  COUNT(n_old, 10);
+  COUNT(n_new, 11);
+  COUNT(max_pages, 12);
+  COUNT(page_size, 13);
+  COUNT(num_pages, 14);
+  if (!n_old || !n_new || !max_pages || !num_pages) Py_RETURN_NONE;
+  HERE(15);
+  TENSOR_ON(int32_t, tables, 0, int_dtype, (long long)n_old * max_pages);
+  TENSOR_ON(int32_t, lens, 1, int_dtype, n_old);
+  TENSOR_ON(int32_t, parents, 2, int_dtype, n_new);
+  OPT_ON(int32_t, reserve, 3, int_dtype, n_new);
+  TENSOR_ON(int32_t, refs, 4, int_dtype, num_pages);
+  TENSOR_ON(int32_t, new_tables, 5, int_dtype, (long long)n_new * max_pages);
+  TENSOR_ON(int32_t, new_lens, 6, int_dtype, n_new);
+  TENSOR_ON(int32_t, copies, 7, int_dtype, 2LL * n_new);
+  TENSOR_ON(int32_t, counts, 8, int_dtype, 2);
+  TENSOR_ON(int32_t, workspace, 9, int_dtype,
+            (long long)llmk_kv_fork_workspace_ints(n_old, n_new, max_pages, num_pages));
+  ANSWER(llmk_kv_fork(tables, lens, parents, reserve, refs, new_tables, new_lens, copies, counts,
+                      workspace, n_old, n_new, max_pages, page_size, num_pages, stream));
+}
+
+FUNCTION(kv_compact, 11)
+  COUNT(n_seqs, 7);
+  COUNT(max_pages, 8);
+  COUNT(num_pages, 9);
+  if (!n_seqs || !max_pages || num_pages < 2) Py_RETURN_NONE;
+  HERE(10);
+  TENSOR_ON(int32_t, tables, 0, int_dtype, (long long)n_seqs * max_pages);
+  TENSOR_ON(int32_t, refs, 1, int_dtype, num_pages);
+  TENSOR_ON(int32_t, new_tables, 2, int_dtype, (long long)n_seqs * max_pages);
+  TENSOR_ON(int32_t, new_refs, 3, int_dtype, num_pages);
+  TENSOR_ON(int32_t, copies, 4, int_dtype, 2LL * (num_pages / 2));
+  TENSOR_ON(int32_t, counts, 5, int_dtype, 2);
+  TENSOR_ON(int32_t, workspace, 6, int_dtype, (long long)llmk_kv_compact_workspace_ints(num_pages));
+  ANSWER(llmk_kv_compact(tables, refs, new_tables, new_refs, copies, counts, workspace, n_seqs, max_pages,
+                         num_pages, stream));
+}
+
 /* setup(torch.Tensor, torch.float16, torch.int32, torch.float32, current device, current stream
  * of a device, torch.float8_e4m3fn) */
 static PyObject* setup(PyObject* self, PyObject* args) {
@@ -441,6 +654,12 @@ static PyMethodDef methods[] = {METHOD(rmsnorm),
                                 METHOD(kv8_gather),
                                 METHOD(kv8_attention),
                                 METHOD(verify_drafts),
+                                METHOD(lora_add),
+                                METHOD(rotary_apply),
+                                METHOD(qkv_rotary_scatter),
+                                METHOD(kv_copy_pages),
+                                METHOD(kv_fork),
+                                METHOD(kv_compact),
                                 {"setup", setup, METH_VARARGS, NULL},
                                 {NULL, NULL, 0, NULL}};
 
@@ -453,7 +672,10 @@ PyMODINIT_FUNC PyInit__fast_calls(void) {
       !(s_is_contiguous = PyUnicode_InternFromString("is_contiguous")) ||
       !(s_numel = PyUnicode_InternFromString("numel")) ||
       !(s_data_ptr = PyUnicode_InternFromString("data_ptr")) ||
-      !(s_get_device = PyUnicode_InternFromString("get_device")))
+      !(s_get_device = PyUnicode_InternFromString("get_device")) ||
+      !(s_shape = PyUnicode_InternFromString("shape")) ||
+      !(s_stride = PyUnicode_InternFromString("stride")) ||
+      !(s_element_size = PyUnicode_InternFromString("element_size")))
     return NULL;
   return PyModule_Create(&module);
 }
