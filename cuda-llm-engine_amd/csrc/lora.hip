@@ -27,9 +27,8 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kParts = 8, kMaxRank = 256;
 constexpr int kWindow = 256, kHash = 512;
 constexpr int kRows = 16;   // of a tile
-constexpr int kNote = 32;   // ints of a tile's note: adapter (-1: no tile), then its rows (-1: none)
+constexpr int kNote = 32;   // ints of a tile's note: adapter (-1: no tile), rank, scale; from 16 on its rows (-1: none)
 constexpr int kChunk = 256;  // of in_features that a wave takes at a time
-constexpr int kGroups = 4;  // of 16 ranks that it accumulates at a time
 
 struct LoraArgs {
   const f16 *x, *a, *b;
@@ -52,17 +51,13 @@ __device__ __forceinline__ int slot_of_window(const LoraArgs& g, int w) {
   return first_row(g, min(w * kWindow, g.n_seqs)) / kRows + w * (g.groups + 1);
 }
 
-__device__ __forceinline__ int rank_of(const LoraArgs& g, int a) {
-  return g.ranks ? min(g.ranks[a], g.max_rank) : g.max_rank;
-}
-
 __device__ __forceinline__ int wave_scan(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
   return v;
 }
 
@@ -70,12 +65,15 @@ __device__ __forceinline__ int wave_scan(int v) {  // inclusive
 __device__ __forceinline__ int block_scan(int v, int* part) {
   const int wave = threadIdx.x >> 6, in = wave_scan(v);
   if ((threadIdx.x & 63) == 63) part[wave] = in;
-  __syncthreads();
+  lds_barrier();
   int before = 0;
 #pragma unroll
   for (int w = 0; w < 3; ++w) before += w < wave ? part[w] : 0;
   return before + in - v;
 }
+
+// A value that all lanes have, in a scalar register.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 struct Plan {
   int key[kHash];            // the adapter of a slot of the table, -1: none
@@ -83,10 +81,12 @@ struct Plan {
   int first[kHash];          // its first member
   int part[2][4];
   int adapter, group, from;  // of the tile: its group's table slot, and its first row among the group's
+  int rank;
+  float scale;
   int row[kRows];
 };
 
-// Finds tile `slot` with 256 threads: its adapter (-1: there is none) and rows, in p.
+// Finds tile `slot` with 256 threads: its adapter (-1: there is none), what belongs to that, and rows, in p.
 __device__ __forceinline__ void find_tile(const LoraArgs& g, int slot, Plan& p) {
   const int tid = threadIdx.x;
   int w = 0;
@@ -111,9 +111,14 @@ __device__ __forceinline__ void find_tile(const LoraArgs& g, int slot, Plan& p) 
   }
   if (tid < kRows) p.row[tid] = -1;
   if (tid == 0) p.adapter = -1;
-  __syncthreads();
+  lds_barrier();
+  // what the first member will note is on its way while the table fills
+  int rank = g.max_rank;
+  float scale = 1.f;
   int at = -1;
   if (id >= 0) {  // at most kWindow adapters in kHash slots: the search ends
+    if (g.ranks) rank = g.ranks[id];
+    if (g.scales) scale = g.scales[id];
     at = (int)(((unsigned)id * 2654435761u) >> 23);
     for (;;) {
       const int was = atomicCAS(&p.key[at], -1, id);
@@ -123,7 +128,7 @@ __device__ __forceinline__ void find_tile(const LoraArgs& g, int slot, Plan& p) 
     atomicAdd(&p.rows[at], rows);
     atomicMin(&p.first[at], tid);
   }
-  __syncthreads();
+  lds_barrier();
   const bool leads = at >= 0 && p.first[at] == tid;
   const int tiles = leads ? (p.rows[at] + kRows - 1) / kRows : 0;
   const int begin = block_scan(tiles, p.part[0]);
@@ -131,219 +136,430 @@ __device__ __forceinline__ void find_tile(const LoraArgs& g, int slot, Plan& p) 
     p.adapter = id;
     p.group = at;
     p.from = (tile - begin) * kRows;
+    p.rank = min(rank, g.max_rank);
+    p.scale = scale;
   }
-  __syncthreads();
+  lds_barrier();
   if (p.adapter < 0) return;
   const bool mine = at == p.group;
   const int before = block_scan(mine ? rows : 0, p.part[1]) - p.from;
-  if (mine)
-    for (int i = max(-before, 0); i < rows && before + i < kRows; ++i) p.row[before + i] = r0 + i;
-  __syncthreads();
+  // the members that have rows of the tile, one behind the other, by a wave's first lanes
+  const int lane = tid & 63;
+  for (uint64_t m = __builtin_amdgcn_ballot_w64(mine && before < kRows && before + rows > 0); m; m &= m - 1) {
+    const int from = __builtin_ctzll(m);
+    const int i = lane - __builtin_amdgcn_readlane(before, from);
+    if (lane < kRows && i >= 0 && i < __builtin_amdgcn_readlane(rows, from))
+      p.row[lane] = __builtin_amdgcn_readlane(r0, from) + i;
+  }
+  lds_barrier();
+}
+
+// What a wave writes to its own part of LDS is there for all of its lanes.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// 16 rows of 512 bytes in LDS, in pieces of 16, which lie such that neither a row's 32 pieces nor a piece of
+// all rows share banks.
+typedef u32x4 Stage[kRows * 32];
+__device__ __forceinline__ int place_of(int row, int piece) { return row * 32 + (piece ^ row); }
+
+__device__ __forceinline__ void put_rows(u32x4* to, const u32x4 (&v)[8], int lane) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) to[place_of(2 * t + (lane >> 5), lane & 31)] = v[t];
+}
+__device__ __forceinline__ void get_rows(const u32x4* from, u32x4 (&v)[8], int n, int q) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) v[t] = from[place_of(n, 4 * t + q)];
+}
+
+// acc[i] += W_i x for the chunks of in_features that a wave takes: D[rank, row]. A chunk's rows are 512 bytes,
+// loaded two an instruction, in whole lines, all of them on their way before the first product waits for one, and
+// go through LDS to where the matrix instructions want them (row n, eight numbers from 8 q on in each step of
+// 32). Loaded as these want them, 64 bytes of 16 rows an instruction, they take three times as long: 8000
+// cycles for 32 instructions of four waves from the L2, not 2400. x: the lane's rows; w: of the lane's first row,
+// `rows` behind it clamped. Products `most` and behind are none.
+template <int NG>
+__device__ __forceinline__ void shrink_chunks(f32x4 (&acc)[NG], const LoraArgs& g, const int (&row)[8],
+                                              const f16* const (&w)[NG], const int (&left)[NG], int most,
+                                              int chunk, int step, u32x4* stage, int lane) {
+  const int n = lane & 15, q = lane >> 4, r = lane >> 5, at = 8 * (lane & 31), in = g.in;
+  for (int c = chunk; c * kChunk < in; c += step) {
+    const int k0 = c * kChunk + at, k = min(k0, in - 8);  // past in_features: loaded, and cleared below
+    u32x4 xr[8], wr[NG][8], xf[8], wf[8];
+#pragma unroll
+    for (int t = 0; t < 8; ++t) xr[t] = ld16(g.x + (size_t)row[t] * g.ldx + k);
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+      if (i < most)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) wr[i][t] = ld16(w[i] + (uint32_t)(min(2 * t + r, left[i]) * in + k));
+    if ((c + 1) * kChunk > in) {
+#pragma unroll
+      for (int t = 0; t < 8; ++t) xr[t] = k0 < in ? xr[t] : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < NG; ++i)
+#pragma unroll
+        for (int t = 0; t < 8; ++t) wr[i][t] = k0 < in ? wr[i][t] : u32x4{0, 0, 0, 0};
+    }
+    put_rows(stage, xr, lane);
+    wave_sync();
+    get_rows(stage, xf, n, q);
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < NG; ++i) {
+      if (i >= most) break;
+      put_rows(stage, wr[i], lane);
+      wave_sync();
+      get_rows(stage, wf, n, q);
+      __builtin_amdgcn_sched_barrier(0);  // all reads in front of the first product
+#pragma unroll
+      for (int t = 0; t < 8; ++t)
+        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(wf[t]), as_h8(xf[t]), acc[i], 0, 0, 0);
+      wave_sync();
+    }
+  }
+}
+
+// The rows of x that a lane loads; for one that is none, one that is: it gives what nobody reads.
+__device__ __forceinline__ void rows_of_x(const Plan& p, int (&row)[8], int lane) {
+#pragma unroll
+  for (int t = 0; t < 8; ++t) {
+    const int r = p.row[2 * t + (lane >> 5)];
+    row[t] = r >= 0 ? r : p.row[0];
+  }
 }
 
 // h of a tile: D[rank, row] = A[rank, k] x[row, k], by waves that take 256 of in_features at a time.
-__global__ void __launch_bounds__(256) k_lora_shrink(const LoraArgs g) {
+template <int NG>
+__global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const LoraArgs g) {
   __shared__ Plan p;
-  __shared__ f32x4 sum[3][kGroups][64];
-  const int slot = blockIdx.x, split = blockIdx.y;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+  __shared__ Stage stage[4];
+  const int slot = blockIdx.x / g.splits, split = blockIdx.x % g.splits;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
   find_tile(g, slot, p);
-  const int a = p.adapter;
+  const int a = uniform(p.adapter);
   if (split == 0) {
-    if (threadIdx.x == 0) g.notes[(size_t)slot * kNote] = a;
-    if (threadIdx.x < kRows) g.notes[(size_t)slot * kNote + 1 + threadIdx.x] = p.row[threadIdx.x];
+    int* note = g.notes + (size_t)slot * kNote;
+    if (threadIdx.x == 0) {
+      note[0] = a;
+      note[1] = p.rank;
+      note[2] = __builtin_bit_cast(int, p.scale);
+    }
+    if (threadIdx.x < kRows) note[kRows + threadIdx.x] = p.row[threadIdx.x];
   }
-  if (a < 0) return;
-  const int rank = rank_of(g, a);
-  if (rank <= 0) return;
+  const int rank = uniform(p.rank);
+  if (a < 0 || rank <= 0) return;
   const int per_part = (rank + 15) / 16, all = g.n_parts * per_part;
-  const int row = p.row[n] >= 0 ? p.row[n] : p.row[0];  // a row that is none gives what nobody reads
-  const f16* x = g.x + (size_t)row * g.ldx + 8 * q;
+  int xrow[8];
+  rows_of_x(p, xrow, lane);
   const size_t width = (size_t)g.n_parts * g.max_rank;
   float* out = g.h + ((size_t)split * g.slots + slot) * kRows * width + n * width + 4 * q;
-  for (int g0 = 0; g0 < all; g0 += kGroups) {
-    f32x4 acc[kGroups];
-    const f16* w[kGroups];
+  for (int g0 = 0; g0 < all; g0 += NG) {
+    f32x4 acc[NG];
+    const f16* w[NG];
+    int left[NG];
 #pragma unroll
-    for (int i = 0; i < kGroups; ++i) {
+    for (int i = 0; i < NG; ++i) {
       acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-      const int gi = min(g0 + i, all - 1), part = gi / per_part;
-      const int j = min((gi - part * per_part) * 16 + n, rank - 1);
-      w[i] = g.a + (((size_t)a * g.n_parts + part) * g.max_rank + j) * g.in + 8 * q;
+      const int gi = min(g0 + i, all - 1), part = gi / per_part, j = (gi - part * per_part) * 16;
+      w[i] = g.a + (((size_t)a * g.n_parts + part) * g.max_rank + j) * g.in;
+      left[i] = rank - 1 - j;
     }
-    for (int c = split * 4 + wave; c * kChunk < g.in; c += 4 * g.splits) {
-      const int k0 = c * kChunk;
-      u32x4 xf[8];
+    if (g0) lds_barrier();
+    shrink_chunks<NG>(acc, g, xrow, w, left, all - g0, split * 4 + wave, 4 * g.splits, stage[wave], lane);
+    // the four waves' sums
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        const int k = k0 + 32 * t;
-        xf[t] = k + 8 * q < g.in ? ld16(x + k) : u32x4{0, 0, 0, 0};
-      }
+    for (int i = 0; i < NG; ++i) stage[wave][i * 64 + lane] = __builtin_bit_cast(u32x4, acc[i]);
+    lds_barrier();
+    if (wave < NG && g0 + wave < all) {  // wave i adds product i's
+      f32x4 v[4];
 #pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        if (g0 + i >= all) break;
-        u32x4 wf[8];
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-          const int k = k0 + 32 * t;
-          wf[t] = k + 8 * q < g.in ? ld16(w[i] + k) : u32x4{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int t = 0; t < 8; ++t)
-          acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(wf[t]), as_h8(xf[t]), acc[i], 0, 0, 0);
-      }
+      for (int m = 0; m < 4; ++m) v[m] = __builtin_bit_cast(f32x4, stage[m][wave * 64 + lane]);
+      const int part = (g0 + wave) / per_part, j = (g0 + wave - part * per_part) * 16;
+      if (j + 4 * q < g.max_rank)
+        *reinterpret_cast<f32x4*>(out + (size_t)part * g.max_rank + j) = (v[0] + v[1]) + (v[2] + v[3]);
     }
-    // the four waves' sums, the first one's last
-    if (g0) __syncthreads();
-    if (wave > 0)
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) sum[wave - 1][i][lane] = acc[i];
-    __syncthreads();
-    if (wave == 0)
-#pragma unroll
-      for (int i = 0; i < kGroups; ++i) {
-        if (g0 + i >= all) break;
-        acc[i] = (acc[i] + sum[0][i][lane]) + (sum[1][i][lane] + sum[2][i][lane]);
-        const int part = (g0 + i) / per_part, j = (g0 + i - part * per_part) * 16;
-        if (j + 4 * q < g.max_rank)
-          *reinterpret_cast<f32x4*>(out + (size_t)part * g.max_rank + j) = acc[i];
-      }
   }
 }
 
-// y of a tile's rows and a block's columns: D[column, row] = B[column, j] h[row, j], in steps of 32 ranks (KS
-// at most). The columns of a wave are taken 32 at a time by two products, whose rows of B are chosen such
-// that a lane gets eight columns side by side.
-template <int KS>
-__global__ void __launch_bounds__(256) k_lora_expand(const LoraArgs g) {
-  constexpr int TILES = KS <= 2 ? 8 : 16 / KS, PAIRS = TILES / 2;  // products of a wave
-  constexpr int LD = 32 * KS + 8;                                  // of a row in LDS
-  __shared__ __attribute__((aligned(16))) f16 hi[kRows * LD], lo[kRows * LD];
-  __shared__ float power[kRows];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
-  int part = 0;
-  while ((int)blockIdx.y >= g.chunk_end[part]) ++part;
-  const int chunk = blockIdx.y - (part ? g.chunk_end[part - 1] : 0);
-  const int end = g.part_end[part], out = g.part_end[g.n_parts - 1];
-  const int c0 = (part ? g.part_end[part - 1] : 0) + (chunk * 4 + wave) * 16 * TILES;
-  const size_t width = (size_t)g.n_parts * g.max_rank;
-  u32x4 bf[TILES][KS];
-  int loaded = -1, rank = 0;
-  float scale = 0.f;
-  for (int i = 0; i < g.per_block; ++i) {
-    const int slot = blockIdx.x * g.per_block + i;
-    if (slot >= g.slots) break;
-    const int* note = g.notes + (size_t)slot * kNote;
-    const int a = note[0], row = note[1 + n];
-    if ((unsigned)a >= (unsigned)g.n_adapters) continue;
-    if (a != loaded) {
-      loaded = a;
-      rank = rank_of(g, a);
-      scale = g.scales ? g.scales[a] : 1.f;
-      if (rank > 0)
+// B's rows for the products of a wave, in steps of 32 ranks. The columns are taken 32 at a time by two products,
+// whose rows of B are chosen such that a lane gets eight columns side by side.
+template <int KS, int TILES>
+__device__ __forceinline__ void load_b(u32x4 (&bf)[TILES][KS], const f16* b, int c0, int end, int max_rank,
+                                       int rank, int n, int q) {
 #pragma unroll
-        for (int t = 0; t < TILES; ++t) {
-          const int c = min(c0 + 32 * (t / 2) + 8 * (n / 4) + 4 * (t & 1) + n % 4, end - 1);
-          const f16* b = g.b + ((size_t)a * out + c) * g.max_rank + 8 * q;
+  for (int t = 0; t < TILES; ++t) {
+    const int c = min(c0 + 32 * (t / 2) + 8 * (n / 4) + 4 * (t & 1) + n % 4, end - 1);
 #pragma unroll
-          for (int s = 0; s < KS; ++s) {
-            const int k = 32 * s + 8 * q;
-            f16x8 v = (f16x8)(f16)0;
-            if (k < rank) v = as_h8(ld16(b + 32 * s));
-            if (k + 8 > rank)
+    for (int s = 0; s < KS; ++s)
+      bf[t][s] = 32 * s + 8 * q < rank ? ld16(b + (size_t)c * max_rank + 32 * s + 8 * q) : u32x4{0, 0, 0, 0};
+  }
+}
+// What lies past the rank is not read as numbers.
+template <int KS, int TILES>
+__device__ __forceinline__ void cut_b(u32x4 (&bf)[TILES][KS], int rank, int q) {
+  if (rank % 8 == 0) return;
 #pragma unroll
-              for (int e = 0; e < 8; ++e) v[e] = k + e < rank ? v[e] : (f16)0;
-            bf[t][s] = as_u4(v);
-          }
-        }
-    }
-    if (rank <= 0) continue;
-    f16* y = g.y + (size_t)((unsigned)row < (unsigned)g.n_rows ? row : 0) * g.ldy + c0 + 8 * q;
-    u32x4 old[PAIRS];
-#pragma unroll
-    for (int t = 0; t < PAIRS; ++t)
-      if ((unsigned)row < (unsigned)g.n_rows && c0 + 32 * t + 8 * q < end) old[t] = ld16(y + 32 * t);
-    // h into LDS: 16 threads a row, eight ranks each
-    lds_barrier();
-    {
-      const int r = threadIdx.x >> 4, piece = threadIdx.x & 15;
-      constexpr int PIECES = (KS * 4 + 15) / 16;
-      float v[PIECES][8], most = 0.f;
-      const float* h = g.h + ((size_t)slot * kRows + r) * width + (size_t)part * g.max_rank;
-#pragma unroll
-      for (int m = 0; m < PIECES; ++m) {
-        const int k = 8 * (piece + 16 * m);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[m][e] = 0.f;
-        if (k < rank)
-          for (int s = 0; s < g.splits; ++s) {
-            const f32x4* from =
-                reinterpret_cast<const f32x4*>(h + (size_t)s * g.slots * kRows * width + k);
-            const f32x4 u = from[0], w = from[1];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[m][e] += u[e];
-              v[m][e + 4] += w[e];
-            }
-          }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[m][e] = k + e < rank ? v[m][e] : 0.f;
-          const float mag = __builtin_fabsf(v[m][e]);
-          most = mag < INFINITY ? __builtin_fmaxf(most, mag) : most;
-        }
-      }
-#pragma unroll
-      for (int d = 1; d < 16; d *= 2) most = __builtin_fmaxf(most, __shfl_xor(most, d));
-      // 2^e: the largest becomes 2^14 or more, below 2^15
-      int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14;
-      e = e < -100 ? -100 : e;
-      const float down = kv8::exp2_int(-e);
-      if (piece == 0) power[r] = kv8::exp2_int(e);
-#pragma unroll
-      for (int m = 0; m < PIECES; ++m) {
-        const int k = 8 * (piece + 16 * m);
-        f16x8 big, rest;
-#pragma unroll
-        for (int i2 = 0; i2 < 8; ++i2) {
-          const float u = v[m][i2] * down;
-          big[i2] = (f16)u;
-          rest[i2] = __builtin_fabsf(u) < INFINITY ? (f16)(u - (float)big[i2]) : (f16)0;
-        }
-        if (k < 32 * KS) {
-          *reinterpret_cast<f16x8*>(hi + r * LD + k) = big;
-          *reinterpret_cast<f16x8*>(lo + r * LD + k) = rest;
-        }
-      }
-    }
-    lds_barrier();
-    f16x8 hf[KS], lf[KS];
+  for (int t = 0; t < TILES; ++t)
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      hf[s] = *reinterpret_cast<const f16x8*>(hi + n * LD + 32 * s + 8 * q);
-      lf[s] = *reinterpret_cast<const f16x8*>(lo + n * LD + 32 * s + 8 * q);
+      f16x8 v = as_h8(bf[t][s]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = 32 * s + 8 * q + e < rank ? v[e] : (f16)0;
+      bf[t][s] = as_u4(v);
     }
-    const float by = scale * power[n];
+}
+
+// A lane's h (row n, ranks 32 s + 8 q on) as two fp16 each; returns the 2^e that they are to be multiplied by.
+template <int KS>
+__device__ __forceinline__ float split_h(const float (&v)[KS][8], f16x8 (&hi)[KS], f16x8 (&lo)[KS]) {
+  float most = 0.f;
 #pragma unroll
-    for (int t = 0; t < PAIRS; ++t) {
-      f32x4 d[2];
+  for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        d[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          d[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[2 * t + j][s]), hf[s], d[j], 0, 0, 0);
-          d[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[2 * t + j][s]), lf[s], d[j], 0, 0, 0);
-        }
-      }
-      if ((unsigned)row < (unsigned)g.n_rows && c0 + 32 * t + 8 * q < end) {
-        f16x8 v = as_h8(old[t]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (f16)((float)v[e] + by * d[e / 4][e % 4]);
-        st16(y + 32 * t, as_u4(v));
-      }
+    for (int e = 0; e < 8; ++e) {
+      const float mag = __builtin_fabsf(v[s][e]);
+      most = mag < INFINITY ? __builtin_fmaxf(most, mag) : most;
     }
+  most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+  most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+  int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14;
+  e = e < -100 ? -100 : e;
+  const float down = kv8::exp2_int(-e);
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float u = v[s][i] * down;
+      hi[s][i] = (f16)u;
+      lo[s][i] = __builtin_fabsf(u) < INFINITY ? (f16)(u - (float)hi[s][i]) : (f16)0;
+    }
+  return kv8::exp2_int(e);
+}
+
+// What is added to a wave's 16 rows and 16 * TILES columns: row n, columns 32 t + 8 q on of each pair of products,
+// times `by`, into LDS (in pieces of 16 bytes as above).
+template <int KS, int TILES>
+__device__ __forceinline__ void expand_columns(const u32x4 (&bf)[TILES][KS], const f16x8 (&hi)[KS],
+                                               const f16x8 (&lo)[KS], float by, u32x4* to, int n, int q) {
+#pragma unroll
+  for (int t = 0; t < TILES; ++t) {
+    f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[t][s]), hi[s], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[t][s]), lo[s], d, 0, 0, 0);
+    }
+    d = f32x4{by * d[0], by * d[1], by * d[2], by * d[3]};
+    to[n * 4 * TILES + ((8 * (t / 2) + 2 * q + (t & 1)) ^ (n & (4 * TILES - 1)))] =
+        __builtin_bit_cast(u32x4, d);
   }
+}
+
+// A wave's y: 2 * TILES lanes a row, eight columns each, so that accesses are of whole lines. row(t) is the
+// lane's t-th row among the 16; `inside`: whether its columns are the part's.
+template <int TILES>
+__device__ __forceinline__ int y_row(int t, int lane) { return t * (32 / TILES) + lane / (2 * TILES); }
+
+template <int TILES>
+__device__ __forceinline__ void load_y(u32x4 (&old)[TILES / 2], f16* const (&y)[TILES / 2]) {
+#pragma unroll
+  for (int t = 0; t < TILES / 2; ++t)
+    if (y[t]) old[t] = ld16_stream(y[t]);
+}
+
+template <int TILES>
+__device__ __forceinline__ void add_to_y(const u32x4 (&old)[TILES / 2], f16* const (&y)[TILES / 2], const u32x4* from,
+                                         int lane) {
+#pragma unroll
+  for (int t = 0; t < TILES / 2; ++t) {
+    const int r = y_row<TILES>(t, lane), piece = 2 * (lane % (2 * TILES)), flip = r & (4 * TILES - 1);
+    const f32x4 u = __builtin_bit_cast(f32x4, from[r * 4 * TILES + (piece ^ flip)]);
+    const f32x4 w = __builtin_bit_cast(f32x4, from[r * 4 * TILES + ((piece + 1) ^ flip)]);
+    f16x8 v = as_h8(old[t]);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[e] = (f16)((float)v[e] + u[e]);
+      v[e + 4] = (f16)((float)v[e + 4] + w[e]);
+    }
+    if (y[t]) st16_stream(y[t], as_u4(v));
+  }
+}
+
+// The part that a block's columns lie in, and the block's place in it.
+__device__ __forceinline__ int part_of(const LoraArgs& g, int chunk, int* place) {
+  int part = 0;
+  while (chunk >= g.chunk_end[part]) ++part;
+  *place = chunk - (part ? g.chunk_end[part - 1] : 0);
+  return part;
+}
+
+// y of a tile's rows: D[column, row] = B[column, j] h[row, j]. Waves work by themselves; those of a block take
+// columns side by side, so that h comes from the first-level cache but once. A wave keeps its columns of B while
+// its tiles, `per_block` in a row, have the same adapter.
+template <int KS, bool MANY>
+__global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_expand(const LoraArgs g) {
+  constexpr int TILES = KS <= 2 ? 8 : 16 / KS;
+  __shared__ u32x4 stage[4][kRows * 4 * TILES];
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+  int place;
+  const int chunks = g.chunk_end[g.n_parts - 1];
+  const int part = part_of(g, blockIdx.x % chunks, &place);
+  const int end = g.part_end[part], out = g.part_end[g.n_parts - 1];
+  const int c0 = (part ? g.part_end[part - 1] : 0) + (place * 4 + wave) * 16 * TILES;
+  if (!MANY && c0 >= end) return;
+  const int column = c0 + 8 * (lane % (2 * TILES));
+  const size_t width = (size_t)g.n_parts * g.max_rank;
+  __shared__ f32x4 shared_h[MANY ? 4 : 1][KS][2][64];
+  u32x4 bf[TILES][KS];
+  int loaded = -1;
+  const int first = blockIdx.x / chunks * g.per_block, behind = min(first + g.per_block, g.slots);
+  for (int slot = first; slot < behind; ++slot) {
+    const int* note = g.notes + (size_t)slot * kNote;
+    const int a = note[0], rank = note[1];
+    const float scale = __builtin_bit_cast(float, note[2]);
+    int row[TILES / 2];
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t) row[t] = note[kRows + y_row<TILES>(t, lane)];
+    // the splits' sums: up to two by the wave itself, more by the block's waves, two each, through LDS
+    float h[KS][8];
+    const float* from = g.h + ((size_t)slot * kRows + n) * width + (size_t)part * g.max_rank + 8 * q;
+    const auto add_split = [&](f32x4 (&v)[KS][2], int split) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int k = min(32 * s, g.max_rank - 8 - 8 * q);  // behind max_rank: not read as numbers
+        const f32x4* u = reinterpret_cast<const f32x4*>(from + (size_t)split * g.slots * kRows * width + k);
+        v[s][0] = u[0];
+        v[s][1] = u[1];
+      }
+    };
+    f32x4 u[KS][2], w[KS][2];
+    const int one = MANY ? wave : 0, two = MANY ? wave + 4 : 1;
+    if (one < g.splits) add_split(u, one);
+    if (two < g.splits) add_split(w, two);
+    if (one < g.splits && two < g.splits)
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) u[s][f] += w[s][f];
+    if (MANY) {
+      if (slot > first) lds_barrier();  // behind what the waves read of the last tile's
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) shared_h[wave][s][f][lane] = u[s][f];
+      lds_barrier();
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int f = 0; f < 2; ++f) {
+          f32x4 v[4];
+#pragma unroll
+          for (int m = 0; m < 4; ++m)
+            if (m < g.splits) v[m] = shared_h[m][s][f][lane];
+          u[s][f] = v[0];
+#pragma unroll
+          for (int m = 1; m < 4; ++m)
+            if (m < g.splits) u[s][f] += v[m];
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[s][e] = u[s][e / 4][e % 4];
+    if ((unsigned)a >= (unsigned)g.n_adapters || rank <= 0 || rank > g.max_rank) continue;
+    f16* y[TILES / 2];
+    u32x4 old[TILES / 2];
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t)
+      y[t] = (unsigned)row[t] < (unsigned)g.n_rows && column < end ? g.y + (size_t)row[t] * g.ldy + column
+                                                                   : nullptr;
+    load_y<TILES>(old, y);
+    if (a != loaded) {
+      loaded = a;
+      load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
+      cut_b<KS, TILES>(bf, rank, q);
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[s][e] = 32 * s + 8 * q + e < rank ? h[s][e] : 0.f;
+    f16x8 hi[KS], lo[KS];
+    const float by = scale * split_h<KS>(h, hi, lo);
+    wave_sync();
+    expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q);
+    wave_sync();
+    add_to_y<TILES>(old, y, stage[wave], lane);
+  }
+}
+
+// Both products of a tile and a block's columns in one launch: every block computes the h of its part again.
+template <int TILES>
+__global__ void __launch_bounds__(256, 2) k_lora_whole(const LoraArgs g) {
+  constexpr int KS = 1, NG = 2;
+  __shared__ Plan p;
+  __shared__ Stage stage[4];
+  // a tile's blocks share an XCD, whose L2 then reads its weights once
+  const int chunks = g.chunk_end[g.n_parts - 1], turn = blockIdx.x / 8;
+  const int slot = blockIdx.x % 8 + turn / chunks * 8;
+  if (slot >= g.slots) return;
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+  find_tile(g, slot, p);
+  const int a = uniform(p.adapter), rank = uniform(p.rank);
+  if (a < 0 || rank <= 0) return;
+  int place;
+  const int part = part_of(g, turn % chunks, &place);
+  const int end = g.part_end[part], out = g.part_end[g.n_parts - 1];
+  const int c0 = (part ? g.part_end[part - 1] : 0) + (place * 4 + wave) * 16 * TILES;
+  const int column = c0 + 8 * (lane % (2 * TILES));
+  int xrow[8];
+  rows_of_x(p, xrow, lane);
+  // what the second product needs is loaded in front of the first one
+  f16* y[TILES / 2];
+  u32x4 old[TILES / 2], bf[TILES][KS];
+#pragma unroll
+  for (int t = 0; t < TILES / 2; ++t) {
+    const int row = p.row[y_row<TILES>(t, lane)];
+    y[t] = row >= 0 && column < end ? g.y + (size_t)row * g.ldy + column : nullptr;
+  }
+  load_y<TILES>(old, y);
+  load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
+  f32x4 acc[NG];
+  const f16* w[NG];
+  int left[NG];
+#pragma unroll
+  for (int i = 0; i < NG; ++i) {
+    acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w[i] = g.a + (((size_t)a * g.n_parts + part) * g.max_rank + 16 * i) * g.in;
+    left[i] = rank - 1 - 16 * i;
+  }
+  shrink_chunks<NG>(acc, g, xrow, w, left, (rank + 15) / 16, wave, 4, stage[wave], lane);
+#pragma unroll
+  for (int i = 0; i < NG; ++i) stage[wave][i * 64 + lane] = __builtin_bit_cast(u32x4, acc[i]);
+  lds_barrier();
+  float h[KS][8];
+#pragma unroll
+  for (int s = 0; s < KS; ++s)
+#pragma unroll
+    for (int f = 0; f < 2; ++f) {
+      const int at = (2 * s + (q >> 1)) * 64 + (q & 1) * 32 + f * 16 + n;
+      f32x4 v[4];
+#pragma unroll
+      for (int m = 0; m < 4; ++m) v[m] = __builtin_bit_cast(f32x4, stage[m][at]);
+      v[0] = (v[0] + v[1]) + (v[2] + v[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[s][4 * f + e] = 32 * s + 8 * q + 4 * f + e < rank ? v[0][e] : 0.f;
+    }
+  cut_b<KS, TILES>(bf, rank, q);
+  f16x8 hi[KS], lo[KS];
+  const float by = p.scale * split_h<KS>(h, hi, lo);
+  lds_barrier();  // the other waves have read what this one puts its columns over
+  expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q);
+  wave_sync();
+  add_to_y<TILES>(old, y, stage[wave], lane);
 }
 
 // What a call takes of the chip and the workspace, by its sizes alone.
@@ -359,6 +575,8 @@ Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in) {
   const int most = (in + 4 * kChunk - 1) / (4 * kChunk);
   s.splits = (512 + s.slots - 1) / s.slots;
   if (s.splits > most) s.splits = most;
+  if (s.splits > 8) s.splits = 8;  // what k_lora_expand adds up
+  s.splits = (most + (most + s.splits - 1) / s.splits - 1) / ((most + s.splits - 1) / s.splits);  // none idle at the end
   return s;
 }
 
@@ -429,13 +647,39 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.groups = s.groups;
   g.windows = s.windows;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int status = launch(k_lora_shrink, dim3(s.slots, s.splits), dim3(256), 0, st, g);
-  if (status != LLMK_OK) return status;
   const int chunks = g.chunk_end[n_parts - 1];
+  const int per_part = (max_rank + 15) / 16;
+  // Both products in one launch, if a block's own h costs it little: 32 ranks, and few enough numbers of A and x (a
+  // wave's quarter is 2048 of 16 ranks or 1366 of 32), read by few enough blocks. At 16 ranks and 2048 columns, 4
+  // sequences: in_features 1024 5.8 us and not 8.3 of two launches, 2048 6.6 and 8.7, 4096 8.3 and 8.8, 8192 11.6 and
+  // 9.5. At 2048 and 16384 columns, 8 sequences (38 MB) 7.5 and 8.7, 128 (105 MB) 10.9 and 11.6; at 4096 and 16384,
+  // 8 sequences (75 MB) 9.3 and 9.0, 16 (151 MB) 11.9 and 10.1. A launch more is 2 us of the host's time, too.
+  const size_t whole = (size_t)s.slots * chunks * 16 * (per_part + 1) * 2 * in_features;
+  if (ks == 1 && (per_part + 1) * (size_t)in_features <= 8192 && whole <= 96000000) {
+    // 256 columns a block and not 512 while that is a block a CU: 5.8 us and not 6.2 for 20 of 512 columns, but 6.8
+    // and not 6.6 for 216
+    const bool narrow = (long long)s.slots * 2 * chunks <= 256;
+    int blocks = chunks;
+    if (narrow) {
+      for (int p = 0; p < n_parts; ++p)
+        g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
+                         (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), columns / 2);
+      blocks = g.chunk_end[n_parts - 1];
+    }
+    return launch(narrow ? k_lora_whole<4> : k_lora_whole<8>, dim3((s.slots + 7) / 8 * 8 * blocks), dim3(256),
+                  0, st, g);
+  }
+  const int all = n_parts * per_part;
+  const int status = launch(all == 1 ? k_lora_shrink<1> : all == 3 ? k_lora_shrink<3> : k_lora_shrink<2>,
+                            dim3(s.splits * s.slots), dim3(256), 0, st, g);
+  if (status != LLMK_OK) return status;
   g.per_block = 1;
-  while (g.per_block < 8 && (long long)s.slots * chunks / (2 * g.per_block) >= 2048) g.per_block *= 2;
-  const dim3 grid(ceil_div(s.slots, g.per_block), chunks);
-  return launch(ks == 1 ? k_lora_expand<1> : ks == 2 ? k_lora_expand<2>
-                : ks == 4 ? k_lora_expand<4> : k_lora_expand<8>,
+  while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= 2048) g.per_block *= 2;
+  const dim3 grid(chunks * ceil_div(s.slots, g.per_block));
+  const bool many = s.splits > 2;
+  return launch(ks == 1   ? (many ? k_lora_expand<1, true> : k_lora_expand<1, false>)
+                : ks == 2 ? (many ? k_lora_expand<2, true> : k_lora_expand<2, false>)
+                : ks == 4 ? (many ? k_lora_expand<4, true> : k_lora_expand<4, false>)
+                          : (many ? k_lora_expand<8, true> : k_lora_expand<8, false>),
                 grid, dim3(256), 0, st, g);
 }
