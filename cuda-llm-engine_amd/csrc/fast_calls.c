@@ -16,7 +16,7 @@
 static PyObject *tensor_type, *half_dtype, *int_dtype, *float_dtype, *get_device, *get_stream,
     *e4m3_dtype;
 static PyObject *s_is_cuda, *s_dtype, *s_is_contiguous, *s_numel, *s_data_ptr, *s_get_device, *s_shape, *s_stride,
-    *s_element_size;
+    *s_nbytes;
 
 /* The device address of t when it is a contiguous CUDA torch.Tensor of this dtype with at least
  * `least` elements; 0 otherwise, with no exception set. (A tensor of no elements has no address
@@ -571,11 +571,13 @@ FUNCTION(kv_copy_pages, 6)
     const int contiguous = v == Py_True;
     if (!v) PyErr_Clear();
     Py_XDECREF(v);
-    const long long numel = number_of(t, s_numel), each = number_of(t, s_element_size);
-    const long long at = number_of(t, s_data_ptr);
-    if (!contiguous || numel <= 0 || each <= 0 || at <= 0 || numel * each % num_pages) Py_RETURN_NONE;
+    v = PyObject_GetAttr(t, s_nbytes);
+    const long long size = v ? PyLong_AsLongLong(v) : -1, at = number_of(t, s_data_ptr);
+    if (!v || PyErr_Occurred()) PyErr_Clear();
+    Py_XDECREF(v);
+    if (!contiguous || size <= 0 || at <= 0 || size % num_pages) Py_RETURN_NONE;
     pools[i] = (void*)(uintptr_t)at;
-    bytes[i] = (size_t)(numel * each / num_pages);
+    bytes[i] = (size_t)(size / num_pages);
   }
   TENSOR_ON(int32_t, copies, 1, int_dtype, 2LL * n_copies);
   OPT_ON(int32_t, count, 2, int_dtype, 1);
@@ -675,7 +677,7 @@ PyMODINIT_FUNC PyInit__fast_calls(void) {
       !(s_get_device = PyUnicode_InternFromString("get_device")) ||
       !(s_shape = PyUnicode_InternFromString("shape")) ||
       !(s_stride = PyUnicode_InternFromString("stride")) ||
-      !(s_element_size = PyUnicode_InternFromString("element_size")))
+      !(s_nbytes = PyUnicode_InternFromString("nbytes")))
     return NULL;
   return PyModule_Create(&module);
 }

@@ -51,16 +51,6 @@ __device__ __forceinline__ int slot_of_window(const LoraArgs& g, int w) {
   return first_row(g, min(w * kWindow, g.n_seqs)) / kRows + w * (g.groups + 1);
 }
 
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr:1
-  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);  // row_shr:2
-  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);  // row_shr:4
-  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);  // row_shr:8
-  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1 and 3
-  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2 and 3
-  return v;
-}
-
 // The sum of v over the threads in front, of 256. part: four ints that no thread still reads.
 __device__ __forceinline__ int block_scan(int v, int* part) {
   const int wave = threadIdx.x >> 6, in = wave_scan(v);

@@ -1,7 +1,6 @@
 // The pages of a cache that sequences share: copies of pages, the fork from one batch to the next with
 // its counts of holders, and compaction. Integers but for the copies; nothing depends on the order in
 // which blocks run: counts are added up, and every page number comes from a count of what lies in front.
-#include <string.h>
 
 #include "common.hpp"
 
@@ -11,80 +10,87 @@ namespace {
 // ---------------------------------------------------------------------------------------------
 // copies
 // ---------------------------------------------------------------------------------------------
-constexpr int kPools = 64;        // of a launch
-constexpr int kPiece = 64 * 16 * 4;  // bytes that a wave copies at a time: 4 vectors a lane
+constexpr int kPools = 64;            // of a launch
+constexpr int kVectors = 4, kPiece = 64 * 16 * kVectors;  // of a lane, and the bytes that a wave copies
 
 struct CopyArgs {
-  unsigned char* pool[kPools];
+  unsigned char* pool[kPools];  // n_pools of any size, then n_small whose pages are `small` bytes
   size_t bytes[kPools];
   int first[kPools + 1];  // of each pool's pieces among a pair's
   const int *copies, *count;
-  int n_pools, n_copies, num_pages;
+  int n_pools, n_small, small, n_copies, num_pages, slices;
+  int each;  // pieces of every pool's page, 0 if they differ
 };
 
+// A block for each pair and four of its pieces; pairs that are none are behind one load. Pages of few
+// bytes (the scales of an 8-bit cache, 32 in each of 32 pools) are taken many pools a wave, 16 bytes a lane.
 template <bool VECTORS>
 __global__ void __launch_bounds__(256) k_copy_pages(const CopyArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int n = a.count ? min(max(*a.count, 0), a.n_copies) : a.n_copies;
-  const long long pieces = a.first[a.n_pools], total = n * pieces;
-  const long long step = (long long)gridDim.x * 4;
-  for (long long e = (long long)blockIdx.x * 4 + (threadIdx.x >> 6); e < total; e += step) {
-    const int pair = (int)(e / pieces), piece = (int)(e % pieces);
-    const int from = a.copies[2 * (size_t)pair], to = a.copies[2 * (size_t)pair + 1];
-    if ((unsigned)from >= (unsigned)a.num_pages || (unsigned)to >= (unsigned)a.num_pages || from == to)
-      continue;
-    int lo = 0, hi = a.n_pools;
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (a.first[mid] <= piece) lo = mid; else hi = mid;
-    }
-    const size_t bytes = a.bytes[lo], at = (size_t)(piece - a.first[lo]) * kPiece;
-    const unsigned char* src = a.pool[lo] + from * bytes;
-    unsigned char* dst = a.pool[lo] + to * bytes;
-    if (VECTORS) {
-      u32x4 x[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const size_t o = at + (i * 64 + lane) * 16;
-        if (o < bytes) x[i] = ld16_stream(src + o);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const size_t o = at + (i * 64 + lane) * 16;
-        if (o < bytes) st16_stream(dst + o, x[i]);
-      }
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int pair = blockIdx.x / a.slices;
+  if (a.count && pair >= *a.count) return;
+  const int from = a.copies[2 * (size_t)pair], to = a.copies[2 * (size_t)pair + 1];
+  int piece = (blockIdx.x - pair * a.slices) * 4 + wave;
+  const int pieces = a.first[a.n_pools];
+  if (piece < pieces) {
+    int lo = 0;
+    if (a.each) {
+      lo = piece / a.each;
+      piece -= lo * a.each;
     } else {
-      const size_t end = min(bytes, at + kPiece);
-      for (size_t o = at + 4 * lane; o < end; o += 256)
+      for (int hi = a.n_pools; hi - lo > 1;) {
+        const int mid = (lo + hi) / 2;
+        if (a.first[mid] <= piece) lo = mid; else hi = mid;
+      }
+      piece -= a.first[lo];
+    }
+    const size_t bytes = a.bytes[lo], at = (size_t)piece * kPiece;
+    unsigned char* pool = a.pool[lo] + at;
+    if ((unsigned)from >= (unsigned)a.num_pages || (unsigned)to >= (unsigned)a.num_pages || from == to)
+      return;
+    const unsigned char* src = pool + from * bytes;
+    unsigned char* dst = pool + to * bytes;
+    if (VECTORS && at + kPiece <= bytes) {
+      u32x4 x[kVectors];
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) x[i] = ld16_stream(src + (i * 64 + lane) * 16);
+#pragma unroll
+      for (int i = 0; i < kVectors; ++i) st16_stream(dst + (i * 64 + lane) * 16, x[i]);
+    } else if (VECTORS) {
+      for (size_t o = lane * 16; at + o < bytes; o += 1024) st16_stream(dst + o, ld16_stream(src + o));
+    } else {
+      const size_t end = min(bytes - at, (size_t)kPiece);
+      for (size_t o = 4 * lane; o < end; o += 256)
         *reinterpret_cast<uint32_t*>(dst + o) = *reinterpret_cast<const uint32_t*>(src + o);
     }
+    return;
+  }
+  if ((unsigned)from >= (unsigned)a.num_pages || (unsigned)to >= (unsigned)a.num_pages || from == to)
+    return;
+  piece -= pieces;
+  const int lanes = a.small / 16;  // of a small page; VECTORS alone has such pools
+  if (!VECTORS || lanes == 0) return;
+  const int mine = piece * (64 / lanes) + lane / lanes;
+  if (lane / lanes < 64 / lanes && mine < a.n_small) {
+    unsigned char* p = a.pool[a.n_pools + mine] + lane % lanes * 16;
+    st16(p + (size_t)to * a.small, ld16(p + (size_t)from * a.small));
   }
 }
 
 // ---------------------------------------------------------------------------------------------
-// block-wide sums, 256 or 1024 threads
+// block-wide sums
 // ---------------------------------------------------------------------------------------------
-__device__ __forceinline__ int wave_scan(int v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    const int o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
-
-// The sum of v over the threads in front, and *total over all. part: one int for each wave.
+// The sum of v over the threads in front, and *total over all. part: an int for each wave, two sets of which
+// take turns, so that one barrier is enough.
 __device__ __forceinline__ int block_scan(int v, int* part, int* total) {
-  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
-  const int in = wave_scan(v);
-  __syncthreads();
+  const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, in = wave_scan(v);
   if ((threadIdx.x & 63) == 63) part[wave] = in;
   __syncthreads();
   int before = 0, all = 0;
   for (int w = 0; w < waves; ++w) {
-    before += w < wave ? part[w] : 0;
-    all += part[w];
+    const int n = part[w];
+    before += w < wave ? n : 0;
+    all += n;
   }
   *total = all;
   return before + in - v;
@@ -96,27 +102,37 @@ __device__ __forceinline__ int block_scan(int v, int* part, int* total) {
 struct ForkArgs {
   const int *tables, *lens, *parents, *reserve;
   int *refs, *new_tables, *new_lens, *copies, *counts;
-  int *fresh, *list;  // workspace: wanted pages of each child, then of those in front; free pages
-  int n_old, n_new, max_pages, page_size, num_pages, most;
+  int* fresh;            // workspace: wanted pages of each child, then of those in front,
+  int2* columns;         // and their columns, with the page that is to be copied (-1: none)
+  int n_old, n_new, max_pages, page_size, num_pages;
 };
 
-constexpr int kWanted = -2;  // an entry of a new table that waits for a fresh page
+constexpr int kFound = 4096;  // children whose counts of wanted pages are kept in LDS
 
-// How many pages the old row holds; the same in every thread of the block.
-__device__ __forceinline__ int held_pages(const int* row, int max_pages, int num_pages, int* shared) {
-  if (threadIdx.x == 0) *shared = max_pages;
-  __syncthreads();
-  int end = max_pages;
-  for (int j = threadIdx.x; j < max_pages; j += blockDim.x)
-    if ((unsigned)row[j] >= (unsigned)num_pages) {
-      end = j;
-      break;
+// U entries a lane, 64 apart, on their way together; behind the end, `none`.
+template <int U>
+__device__ __forceinline__ void load_entries(const int* from, int at, int end, int none, int (&v)[U]) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = at + 64 * u + lane;
+    v[u] = i < end ? from[i] : none;
+  }
+}
+
+// How many pages the old row holds. A wave's work; all lanes get it.
+template <int U>
+__device__ __forceinline__ int held_pages(const int* row, int max_pages, int num_pages) {
+  for (int j = 0; j < max_pages; j += 64 * U) {
+    int v[U];
+    load_entries<U>(row, j, max_pages, -1, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64((unsigned)v[u] >= (unsigned)num_pages);
+      if (m) return min(j + 64 * u + __builtin_ctzll(m), max_pages);
     }
-  if (end < max_pages) atomicMin(shared, end);
-  __syncthreads();
-  const int held = *shared;
-  __syncthreads();
-  return held;
+  }
+  return max_pages;
 }
 
 __device__ __forceinline__ int length_of(const ForkArgs& a, int parent, int held) {
@@ -125,89 +141,139 @@ __device__ __forceinline__ int length_of(const ForkArgs& a, int parent, int held
   return len < 0 ? 0 : (int)(len < most ? len : most);
 }
 
-// The new rows, with what they keep, and how many fresh pages they want. Reads counts, changes none.
-__global__ void __launch_bounds__(256) k_fork_rows(const ForkArgs a) {
-  __shared__ int shared, part[4];
-  const int c = blockIdx.x, p = a.parents[c];
+// A child's row, with what it keeps, and which columns want fresh pages. Reads counts, changes none. A wave's work.
+template <int U>
+__device__ __forceinline__ void fork_row(const ForkArgs& a, int c) {
+  const int lane = threadIdx.x & 63, p = a.parents[c];
   const bool has = (unsigned)p < (unsigned)a.n_old;
+  uint64_t elder = 0;
+  for (int i = 0; i < c && !elder; i += 64 * U) {
+    int v[U];
+    load_entries<U>(a.parents, i, c, ~p, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) elder |= __builtin_amdgcn_ballot_w64(v[u] == p);
+  }
   const int* row = a.tables + (size_t)(has ? p : 0) * a.max_pages;
-  const int held = has ? held_pages(row, a.max_pages, a.num_pages, &shared) : 0;
+  const int held = has ? held_pages<U>(row, a.max_pages, a.num_pages) : 0;
   const int len = has ? length_of(a, p, held) : 0;
-  int elder = 0;
-  for (int i = threadIdx.x; i < c; i += 256) elder |= a.parents[i] == p;
-  const bool first = !__syncthreads_or(elder);
   const int room = a.reserve ? max(a.reserve[c], 0) : 0;
   const long long want = ((long long)len + room + a.page_size - 1) / a.page_size;
   const int need = (int)(want < a.max_pages ? want : a.max_pages);
   const int whole = len / a.page_size;
   int fresh = 0;
-  for (int j = threadIdx.x; j < a.max_pages; j += 256) {
-    int to = -1;
-    if (j < whole) to = row[j];
-    else if (j < need) {
-      to = kWanted;
-      if (first && j < held && a.refs[row[j]] == 1) to = row[j];
-      fresh += to == kWanted;
+  for (int j0 = 0; j0 < a.max_pages; j0 += 64 * U) {
+    int v[U], alone[U];
+    load_entries<U>(row, j0, held, -1, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + 64 * u + lane;
+      alone[u] = !elder && j >= whole && j < held && j < need ? a.refs[v[u]] : 0;
     }
-    a.new_tables[(size_t)c * a.max_pages + j] = to;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + 64 * u + lane;
+      const bool keeps = j < whole || alone[u] == 1, wants = !keeps && j < need;
+      if (j < a.max_pages) a.new_tables[(size_t)c * a.max_pages + j] = keeps ? v[u] : -1;
+      const uint64_t m = __builtin_amdgcn_ballot_w64(wants);
+      if (wants)
+        a.columns[(size_t)c * a.max_pages + fresh + __builtin_popcountll(m & ((1ull << lane) - 1))] =
+            make_int2(j, j == whole && len % a.page_size ? v[u] : -1);
+      fresh += __builtin_popcountll(m);
+    }
   }
-  int total;
-  block_scan(fresh, part, &total);
-  if (threadIdx.x == 0) {
-    a.fresh[c] = total;
+  if (lane == 0) {
+    a.fresh[c] = fresh;
     a.new_lens[c] = len;
+    a.copies[2 * c] = -1;
+    a.copies[2 * c + 1] = -1;
   }
 }
 
-// The holders of the old rows' pages: each lets go once, the children take.
-__global__ void __launch_bounds__(256) k_fork_refs(const ForkArgs a) {
-  __shared__ int shared, children, first;
-  const int p = blockIdx.x;
+// The holders of an old row's pages: it lets go once, its children take. A wave's work.
+template <int U>
+__device__ __forceinline__ void fork_refs(const ForkArgs& a, int p) {
+  const int lane = threadIdx.x & 63;
   const int* row = a.tables + (size_t)p * a.max_pages;
-  if (threadIdx.x == 0) {
-    children = 0;
-    first = a.n_new;
-  }
-  const int held = held_pages(row, a.max_pages, a.num_pages, &shared);
-  for (int c = threadIdx.x; c < a.n_new; c += 256)
-    if (a.parents[c] == p) {
-      atomicAdd(&children, 1);
-      atomicMin(&first, c);
+  const int held = held_pages<U>(row, a.max_pages, a.num_pages);
+  int children = 0, first = -1;
+  for (int i = 0; i < a.n_new; i += 64 * U) {
+    int v[U];
+    load_entries<U>(a.parents, i, a.n_new, -1, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t m = __builtin_amdgcn_ballot_w64(v[u] == p);
+      if (m && first < 0) first = i + 64 * u + __builtin_ctzll(m);
+      children += __builtin_popcountll(m);
     }
-  __syncthreads();
+  }
   const int whole = length_of(a, p, held) / a.page_size;
-  for (int j = threadIdx.x; j < held; j += 256) {
+  // whole pages of an only child stay as they are
+  for (int j = (children == 1 ? whole : 0) + lane; j < held; j += 64) {
     const int takes = j < whole ? children
                       : children ? a.new_tables[(size_t)first * a.max_pages + j] >= 0 : 0;
     if (takes != 1) atomicAdd(&a.refs[row[j]], takes - 1);
   }
 }
 
-// Finds the free pages that are wanted, in order, and makes them held. One block.
-__global__ void __launch_bounds__(1024) k_fork_find(const ForkArgs a) {
-  __shared__ int part[16];
+// The k-th wanted page: child c's, which is the last whose wanted ones begin at or before k.
+__device__ __forceinline__ void fork_give(const ForkArgs& a, const int* begin, int k, int page) {
+  int c = 0;
+  for (int hi = a.n_new; hi - c > 1;) {
+    const int mid = (c + hi) / 2;
+    if (begin[mid] <= k) c = mid; else hi = mid;
+  }
+  const int2 column = a.columns[(size_t)c * a.max_pages + (k - begin[c])];
+  a.new_tables[(size_t)c * a.max_pages + column.x] = page;
+  if (column.y >= 0) {
+    a.copies[2 * c] = column.y;
+    a.copies[2 * c + 1] = page;
+  }
+}
+
+// Which of a thread's four pages from p0 on are free, as bits; read past the first-level cache, which may hold the
+// counts from before other additions.
+__device__ __forceinline__ int free_bits(const ForkArgs& a, int p0) {
+  const int p = p0 + 4 * threadIdx.x;
+  int bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    bits |= (p + i < a.num_pages &&
+             __hip_atomic_load(&a.refs[p + i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0)
+            << i;
+  return bits;
+}
+
+// Gives the free pages that are wanted, in order. One block of 1024 threads.
+__device__ __forceinline__ void fork_find(const ForkArgs& a, int* found_begin, int (*part)[16]) {
+  const int* begin = a.n_new <= kFound ? found_begin : a.fresh;
+  int free = free_bits(a, 0);
   long long wanted = 0;
+  int turn = 0;
   for (int c0 = 0; c0 < a.n_new; c0 += 1024) {
     const int c = c0 + threadIdx.x, mine = c < a.n_new ? a.fresh[c] : 0;
     int total;
-    const int before = block_scan(mine, part, &total);
+    const int before = block_scan(mine, part[turn ^= 1], &total);
     if (c < a.n_new) {
       const long long at = wanted + before;
-      a.fresh[c] = (int)(at < a.num_pages ? at : a.num_pages);
+      const int b = (int)(at < a.num_pages ? at : a.num_pages);
+      if (a.n_new <= kFound) found_begin[c] = b; else a.fresh[c] = b;
     }
     wanted += total;
   }
+  __syncthreads();
   int found = 0;
-  for (int p0 = 0; p0 < a.num_pages && found < wanted; p0 += 1024) {
-    const int p = p0 + threadIdx.x;
-    const bool free = p < a.num_pages && a.refs[p] == 0;
+  for (int p0 = 0; p0 < a.num_pages && found < wanted;) {
+    const int next = free_bits(a, p0 + 4096);  // on its way in good time
     int total;
-    const int at = found + block_scan(free, part, &total);
-    if (free && at < wanted && at < a.most) {
-      a.list[at] = p;
-      a.refs[p] = 1;
+    int at = found + block_scan(__builtin_popcount(free), part[turn ^= 1], &total);
+    for (; free && at < wanted; free &= free - 1, ++at) {
+      const int page = p0 + 4 * threadIdx.x + __builtin_ctz(free);
+      a.refs[page] = 1;
+      fork_give(a, begin, at, page);
     }
     found += total;
+    p0 += 4096;
+    free = next;
   }
   if (threadIdx.x == 0) {
     const long long given = found < wanted ? found : wanted;
@@ -216,38 +282,37 @@ __global__ void __launch_bounds__(1024) k_fork_find(const ForkArgs a) {
   }
 }
 
-// Puts them into the rows.
-__global__ void __launch_bounds__(256) k_fork_fill(const ForkArgs a) {
-  __shared__ int part[4];
-  const int c = blockIdx.x, p = a.parents[c], len = a.new_lens[c], given = a.counts[0];
-  const int whole = len % a.page_size ? len / a.page_size : -1;  // the page that the length ends inside
-  int base = a.fresh[c], from = -1, to = -1;
-  for (int j0 = 0; j0 < a.max_pages; j0 += 256) {
-    const int j = j0 + threadIdx.x;
-    int* entry = a.new_tables + (size_t)c * a.max_pages + j;
-    const bool waits = j < a.max_pages && *entry == kWanted;
-    int total;
-    const int at = base + block_scan(waits, part, &total);
-    if (waits) {
-      const int page = at < given ? a.list[at] : -1;
-      *entry = page;
-      if (j == whole && page >= 0) {
-        from = a.tables[(size_t)p * a.max_pages + j];
-        to = page;
-      }
-    }
-    base += total;
-  }
-  if (whole < 0 ? threadIdx.x == 0 : threadIdx.x == whole % 256) {
-    a.copies[2 * c] = from;
-    a.copies[2 * c + 1] = to;
-  }
+// U: how many entries of a lane are on their way at a time.
+template <int U>
+__global__ void __launch_bounds__(256) k_fork_rows(const ForkArgs a) {
+  const int c = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (c < a.n_new) fork_row<U>(a, c);
+}
+template <int U>
+__global__ void __launch_bounds__(256) k_fork_refs(const ForkArgs a) {
+  const int p = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (p < a.n_old) fork_refs<U>(a, p);
+}
+__global__ void __launch_bounds__(1024) k_fork_find(const ForkArgs a) {
+  __shared__ int begin[kFound], part[2][16];
+  fork_find(a, begin, part);
+}
+// The three of them by one block. Its additions to counts are complete at the barrier and read where they were
+// made, so no fence of the device is needed, which takes 5 us.
+__global__ void __launch_bounds__(1024) k_fork(const ForkArgs a) {
+  __shared__ int begin[kFound], part[2][16];
+  const int wave = threadIdx.x >> 6;
+  for (int c = wave; c < a.n_new; c += 16) fork_row<1>(a, c);
+  __syncthreads();
+  for (int p = wave; p < a.n_old; p += 16) fork_refs<1>(a, p);
+  __syncthreads();
+  fork_find(a, begin, part);
 }
 
 // ---------------------------------------------------------------------------------------------
 // compaction
 // ---------------------------------------------------------------------------------------------
-constexpr int kChunk = 4096;  // pages that a block looks at
+constexpr int kChunk = 4096;  // pages that a block of 1024 threads looks at, four a thread
 
 struct CompactArgs {
   const int *tables, *refs;
@@ -259,65 +324,60 @@ struct CompactArgs {
   long long entries;
 };
 
-__global__ void __launch_bounds__(256) k_compact_count(const CompactArgs a) {
-  __shared__ int part[4];
-  int n = 0;
-  for (int i = threadIdx.x; i < kChunk; i += 256) {
-    const int p = blockIdx.x * kChunk + i;
-    n += p < a.num_pages && a.refs[p] > 0;
-  }
-  int total;
-  block_scan(n, part, &total);
-  if (threadIdx.x == 0) a.live[blockIdx.x] = total;
+// Which of a thread's four pages of a chunk are held, as bits.
+__device__ __forceinline__ int held_bits(const CompactArgs& a, int chunk) {
+  const int p = chunk * kChunk + 4 * threadIdx.x;
+  int bits = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) bits |= (p + i < a.num_pages && a.refs[p + i] > 0) << i;
+  return bits;
 }
 
-// Held pages in all, of chunks in front of `chunk`, and in front of page `n_live`.
-__device__ __forceinline__ void compact_sums(const CompactArgs& a, int chunk, int* part, int* n_live,
+// Held pages in all and in front of page n_live, of `before` in front of the chunk. 1024 threads.
+__device__ __forceinline__ void compact_sums(const CompactArgs& a, int chunk, int (*part)[16], int* n_live,
                                              int* before, int* low) {
   int all = 0, front = 0;
-  for (int i = threadIdx.x; i < a.chunks; i += blockDim.x) {
+  for (int i = threadIdx.x; i < a.chunks; i += 1024) {
     all += a.live[i];
     front += i < chunk ? a.live[i] : 0;
   }
-  block_scan(all, part, n_live);
-  block_scan(front, part, before);
+  block_scan(all, part[0], n_live);
+  block_scan(front, part[1], before);
   const int edge = *n_live / kChunk;  // the chunk that page n_live lies in
   int below = 0;
-  for (int i = threadIdx.x; i < edge && i < a.chunks; i += blockDim.x) below += a.live[i];
-  for (int p = edge * kChunk + threadIdx.x; p < *n_live; p += blockDim.x) below += a.refs[p] > 0;
-  block_scan(below, part, low);
+  for (int i = threadIdx.x; i < edge; i += 1024) below += a.live[i];
+  if (edge < a.chunks) {
+    const int left = *n_live - edge * kChunk - 4 * (int)threadIdx.x;  // of the thread's pages in front of it
+    below += __builtin_popcount(held_bits(a, edge) & ((1 << (left < 0 ? 0 : left > 4 ? 4 : left)) - 1));
+  }
+  block_scan(below, part[2], low);
 }
 
-__global__ void __launch_bounds__(256) k_compact_rank(const CompactArgs a) {
-  __shared__ int part[4];
-  int n_live, before, low;
-  compact_sums(a, blockIdx.x, part, &n_live, &before, &low);
-  const int most = a.num_pages / 2;
-  for (int i = 0; i < kChunk; i += 256) {
-    const int p = blockIdx.x * kChunk + i + threadIdx.x;
-    const bool held = p < a.num_pages && a.refs[p] > 0;
-    int total;
-    const int at = before + block_scan(held, part, &total);
-    before += total;
-    if (p >= a.num_pages) continue;
+__device__ __forceinline__ void compact_rank(const CompactArgs& a, int chunk, int (*part)[16], int n_live, int before,
+                                             int low) {
+  const int most = a.num_pages / 2, bits = held_bits(a, chunk), p0 = chunk * kChunk + 4 * threadIdx.x;
+  int total;
+  int at = before + block_scan(__builtin_popcount(bits), part[3], &total);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int p = p0 + i;
+    if (p >= a.num_pages) break;
+    const bool held = bits >> i & 1;
     int rank = -1;
     if (held && p >= n_live) rank = at - low;
     if (!held && p < n_live) rank = p - at;
     a.rank[p] = rank;
-    if (rank < 0 || rank >= most) continue;
-    a.moves[(held ? 0 : most) + rank] = p;
-    if (held) a.moves[2 * most + rank] = a.refs[p];
-  }
-  if (blockIdx.x == 0 && threadIdx.x == 0) {
-    a.counts[0] = n_live - low;
-    a.counts[1] = n_live;
+    if (rank >= 0 && rank < most) {
+      a.moves[(held ? 0 : most) + rank] = p;
+      if (held) a.moves[2 * most + rank] = a.refs[p];
+    }
+    at += held;
   }
 }
 
-__global__ void __launch_bounds__(256) k_compact_apply(const CompactArgs a) {
-  const int most = a.num_pages / 2, moved = a.counts[0], n_live = a.counts[1];
-  const long long step = (long long)gridDim.x * 256;
-  const long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+__device__ __forceinline__ void compact_apply(const CompactArgs& a, int moved, int n_live, long long at,
+                                              long long step) {
+  const int most = a.num_pages / 2;
   for (long long e = at; e < a.entries; e += step) {
     int p = a.tables[e];
     if (p >= n_live && p < a.num_pages) {
@@ -338,6 +398,55 @@ __global__ void __launch_bounds__(256) k_compact_apply(const CompactArgs a) {
   }
 }
 
+__global__ void __launch_bounds__(1024) k_compact_count(const CompactArgs a) {
+  __shared__ int part[16];
+  int total;
+  block_scan(__builtin_popcount(held_bits(a, blockIdx.x)), part, &total);
+  if (threadIdx.x == 0) a.live[blockIdx.x] = total;
+}
+
+__global__ void __launch_bounds__(1024) k_compact_rank(const CompactArgs a) {
+  __shared__ int part[4][16];
+  int n_live, before, low;
+  compact_sums(a, blockIdx.x, part, &n_live, &before, &low);
+  compact_rank(a, blockIdx.x, part, n_live, before, low);
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    a.counts[0] = n_live - low;
+    a.counts[1] = n_live;
+  }
+}
+
+__global__ void __launch_bounds__(256) k_compact_apply(const CompactArgs a) {
+  compact_apply(a, a.counts[0], a.counts[1], (long long)blockIdx.x * 256 + threadIdx.x,
+                (long long)gridDim.x * 256);
+}
+
+// The three of them by one block, for a pool of one chunk.
+__global__ void __launch_bounds__(1024) k_compact(const CompactArgs a) {
+  __shared__ int part[4][16];
+  int n_live, low;
+  const int bits = held_bits(a, 0);
+  block_scan(__builtin_popcount(bits), part[0], &n_live);
+  const int left = n_live - 4 * (int)threadIdx.x;
+  block_scan(__builtin_popcount(bits & ((1 << (left < 0 ? 0 : left > 4 ? 4 : left)) - 1)), part[1], &low);
+  compact_rank(a, 0, part, n_live, 0, low);
+  if (threadIdx.x == 0) {
+    a.counts[0] = n_live - low;
+    a.counts[1] = n_live;
+  }
+  __syncthreads();
+  compact_apply(a, n_live - low, n_live, threadIdx.x, 1024);
+}
+
+// Whether one block does it all: the launches cost more than the other CUs would give. A fork of 8 to 8 sequences
+// by tables of 20 pages takes 6.7 us and not 9.2, of 32 to 32 11.7 and 12.1, by 128 pages 12.9 and 11.9 (but two
+// launches less, 3 us, on the host), of 64 to 64 by 20 pages 16.9 and 11.5. A compaction of 1000 pages and 1920
+// entries 5.1 us and not 8.6, of 4096 and 8192 10.6 and 11.6, of 4096 and 32768 20.4 and 11.6.
+bool fork_by_one_block(int n_old, int n_new, int max_pages) {
+  return n_old + n_new <= 64 && (n_old + n_new) * max_pages <= 8192;
+}
+bool compact_by_one_block(int num_pages, long long entries) { return num_pages <= kChunk && entries <= 8192; }
+
 }  // namespace
 }  // namespace llmk
 
@@ -355,34 +464,51 @@ extern "C" int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, 
     if (reinterpret_cast<uintptr_t>(pools[i]) % 4) return LLMK_ERR_ALIGNMENT;
     if (page_bytes[i] > ((size_t)1 << 32)) return LLMK_ERR_UNSUPPORTED;
   }
-  for (int i = 0; i < n_pools;) {  // a launch takes kPools pools of one kind: whole vectors, or not
-    CopyArgs a{};
-    a.copies = copies;
-    a.count = count;
-    a.n_copies = n_copies;
-    a.num_pages = num_pages;
-    const auto whole = [&](int p) { return aligned16(pools[p]) && page_bytes[p] % 16 == 0; };
-    const bool vectors = whole(i);
-    for (; i < n_pools && a.n_pools < kPools && whole(i) == vectors; ++i) {
-      const int n = a.n_pools++;
-      a.pool[n] = static_cast<unsigned char*>(pools[i]);
-      a.bytes[n] = page_bytes[i];
-      a.first[n + 1] = a.first[n] + (int)((page_bytes[i] + kPiece - 1) / kPiece);
+  const auto whole = [&](int p) { return aligned16(pools[p]) && page_bytes[p] % 16 == 0; };
+  // small pages of whole vectors, all of one size, go together
+  size_t small = 0;
+  for (int p = 0; p < n_pools && !small; ++p)
+    if (whole(p) && page_bytes[p] <= 512) small = page_bytes[p];
+  for (int kind = 0; kind < 2; ++kind)  // whole vectors, then what is not
+    for (int i = 0; i < n_pools;) {
+      CopyArgs a{};
+      a.copies = copies;
+      a.count = count;
+      a.n_copies = n_copies;
+      a.num_pages = num_pages;
+      int taken = 0;
+      const int begin = i;
+      for (; i < n_pools && taken < kPools; ++i) taken += whole(i) == (kind == 0);
+      if (taken == 0) break;
+      const auto is_small = [&](int p) { return kind == 0 && small && page_bytes[p] == small; };
+      for (int p = begin; p < i; ++p) {
+        if (whole(p) != (kind == 0) || is_small(p)) continue;
+        const int n = a.n_pools++;
+        a.pool[n] = static_cast<unsigned char*>(pools[p]);
+        a.bytes[n] = page_bytes[p];
+        a.first[n + 1] = a.first[n] + (int)((page_bytes[p] + kPiece - 1) / kPiece);
+      }
+      for (int p = begin; p < i; ++p)
+        if (whole(p) && is_small(p)) a.pool[a.n_pools + a.n_small++] = static_cast<unsigned char*>(pools[p]);
+      a.small = a.n_small ? (int)small : 0;
+      size_t pieces = a.first[a.n_pools];
+      if (a.n_small) pieces += ceil_div(a.n_small, 64 / (a.small / 16));
+      a.slices = (int)((pieces + 3) / 4);
+      a.each = a.first[1];
+      for (int p = 0; p < a.n_pools; ++p)
+        if (a.first[p + 1] - a.first[p] != a.each) a.each = 0;
+      const size_t blocks = (size_t)n_copies * a.slices;
+      if (!grid_takes(blocks, 256)) return LLMK_ERR_UNSUPPORTED;
+      const int st = launch(kind == 0 ? k_copy_pages<true> : k_copy_pages<false>, dim3((unsigned)blocks), dim3(256),
+                            0, static_cast<hipStream_t>(stream), a);
+      if (st != LLMK_OK) return st;
     }
-    const size_t pieces = (size_t)n_copies * a.first[a.n_pools];
-    const size_t blocks = (pieces + 3) / 4;
-    const int st = launch(vectors ? k_copy_pages<true> : k_copy_pages<false>,
-                          dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0,
-                          static_cast<hipStream_t>(stream), a);
-    if (st != LLMK_OK) return st;
-  }
   return LLMK_OK;
 }
 
 extern "C" size_t llmk_kv_fork_workspace_ints(int n_old, int n_new, int max_pages, int num_pages) {
   if (n_old < 0 || n_new < 0 || max_pages <= 0 || num_pages <= 0) return 0;
-  const size_t wanted = (size_t)n_new * (size_t)max_pages;
-  return (size_t)n_new + (wanted < (size_t)num_pages ? wanted : (size_t)num_pages) + 1;
+  return 2 + (size_t)n_new * (2 * (size_t)max_pages + 1);
 }
 
 extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
@@ -395,6 +521,7 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   if (!refs || !counts || !workspace || (n_old > 0 && (!block_tables || !seq_lens)) ||
       (n_new > 0 && (!parents || !new_tables || !new_lens || !copies)))
     return LLMK_ERR_INVALID_VALUE;
+  if (reinterpret_cast<uintptr_t>(workspace) % 8) return LLMK_ERR_ALIGNMENT;
   if (n_old > 65535 || n_new > 65535 || max_pages > (1 << 24)) return LLMK_ERR_UNSUPPORTED;
   hipStream_t s = static_cast<hipStream_t>(stream);
   ForkArgs a{};
@@ -408,18 +535,21 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   a.copies = copies;
   a.counts = counts;
   a.fresh = workspace;
-  a.list = workspace + n_new;
+  a.columns = reinterpret_cast<int2*>(workspace + n_new + (n_new & 1));
   a.n_old = n_old;
   a.n_new = n_new;
   a.max_pages = max_pages;
   a.page_size = page_size;
   a.num_pages = num_pages;
-  a.most = (int)(llmk_kv_fork_workspace_ints(n_old, n_new, max_pages, num_pages) - n_new - 1);
+  if (fork_by_one_block(n_old, n_new, max_pages)) return launch(k_fork, dim3(1), dim3(1024), 0, s, a);
+  // tables of 1024 pages: 24 us with four entries a lane at a time and 26.6 with one; of 20 pages 12.0 and 11.5
+  const bool wide = max_pages > 256;
   int st = LLMK_OK;
-  if (n_new > 0) st = launch(k_fork_rows, dim3(n_new), dim3(256), 0, s, a);
-  if (st == LLMK_OK && n_old > 0) st = launch(k_fork_refs, dim3(n_old), dim3(256), 0, s, a);
+  if (n_new > 0)
+    st = launch(wide ? k_fork_rows<4> : k_fork_rows<1>, dim3(ceil_div(n_new, 4)), dim3(256), 0, s, a);
+  if (st == LLMK_OK && n_old > 0)
+    st = launch(wide ? k_fork_refs<4> : k_fork_refs<1>, dim3(ceil_div(n_old, 4)), dim3(256), 0, s, a);
   if (st == LLMK_OK) st = launch(k_fork_find, dim3(1), dim3(1024), 0, s, a);
-  if (st == LLMK_OK && n_new > 0) st = launch(k_fork_fill, dim3(n_new), dim3(256), 0, s, a);
   return st;
 }
 
@@ -451,8 +581,9 @@ extern "C" int llmk_kv_compact(const int32_t* block_tables, const int32_t* refs,
   a.moves = a.rank + num_pages;
   a.num_pages = num_pages;
   a.entries = (long long)n_seqs * max_pages;
-  int st = launch(k_compact_count, dim3(a.chunks), dim3(256), 0, s, a);
-  if (st == LLMK_OK) st = launch(k_compact_rank, dim3(a.chunks), dim3(256), 0, s, a);
+  if (compact_by_one_block(num_pages, a.entries)) return launch(k_compact, dim3(1), dim3(1024), 0, s, a);
+  int st = launch(k_compact_count, dim3(a.chunks), dim3(1024), 0, s, a);
+  if (st == LLMK_OK) st = launch(k_compact_rank, dim3(a.chunks), dim3(1024), 0, s, a);
   if (st != LLMK_OK) return st;
   const long long most = a.entries > num_pages ? a.entries : num_pages;
   const long long blocks = (most + 255) / 256;

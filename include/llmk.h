@@ -502,7 +502,7 @@ LLMK_API int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, in
  * [n_new, 2] is (-1, -1) where nothing is to be copied (llmk_kv_copy_pages does that); counts [2] = fresh pages
  * given, and lacking (the table's row of a child that lacks some is then too short for L + reserve). refs is
  * brought up to date. n_new == 0 frees the old batch. New and old arrays may not overlap.
- * workspace: llmk_kv_fork_workspace_ints(..) int32. Batches up to 65535 sequences. */
+ * workspace: llmk_kv_fork_workspace_ints(..) int32, 8-byte aligned. Batches up to 65535 sequences. */
 LLMK_API size_t llmk_kv_fork_workspace_ints(int n_old, int n_new, int max_pages, int num_pages);
 LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
                           const int32_t* parents, const int32_t* reserve, int32_t* refs,
