@@ -23,17 +23,27 @@ struct RotaryArgs {
   int ldq, ldk, ldq_out, ldk_out;  // ldk_out: of a row of the pool (in place: ldk)
   int n_rows, n_heads, n_kv_heads, head_dim, rotary_dim, n_tables;
   int max_pages, page_size;
-  int rows_per_block;
+  int rows, chunks, per_row;  // of a block; blocks of a row (where it is wide), units of a row
+  FastDiv by_row, by_unit, by_half;
 };
 
-// (scale cos, scale sin) of pair i of a row.
-__device__ __forceinline__ float2 turn_of(const RotaryArgs& a, int row, int i) {
+// What the turn of pair i of a row is made of, and the turn: (scale cos, scale sin).
+struct Angle {
+  int pos;
+  float freq, scale;
+};
+__device__ __forceinline__ Angle angle_of(const RotaryArgs& a, int row, int i) {
+  Angle x;
+  x.pos = a.positions[row];
   int t = a.table_ids ? a.table_ids[row] : 0;
   t = (unsigned)t < (unsigned)a.n_tables ? t : 0;
-  const double f = (double)a.inv_freq[(size_t)t * (a.rotary_dim / 2) + i];
-  const double2 cs = cos_sin((double)a.positions[row] * f);
-  const double s = a.scales ? (double)a.scales[t] : 1.0;
-  return make_float2((float)(cs.x * s), (float)(cs.y * s));
+  x.freq = a.inv_freq[(size_t)t * (a.rotary_dim / 2) + i];
+  x.scale = a.scales ? a.scales[t] : 1.f;
+  return x;
+}
+__device__ __forceinline__ float2 turn_of(Angle x) {
+  const double2 cs = cos_sin((double)x.pos * (double)x.freq);
+  return make_float2((float)(cs.x * (double)x.scale), (float)(cs.y * (double)x.scale));
 }
 
 // The pool row (page * page_size + token) of a row, -1 where it has none.
@@ -67,51 +77,57 @@ __device__ __forceinline__ void turn(f16x8& x, f16x8& y, const float2* lo, const
   }
 }
 
+// A unit a thread. What the turns are made of is loaded first, then the data: the turns are computed while that
+// is on its way, and it is turned and stored behind the barrier.
 template <bool PAIRS, bool SCATTER>
-__global__ void __launch_bounds__(256) k_rotary(const RotaryArgs a) {
+__global__ void __launch_bounds__(512) k_rotary(const RotaryArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float2* turns = reinterpret_cast<float2*>(smem);  // [row][pair]
-  const int half = a.rotary_dim / 2, R = a.rotary_dim / 16;
-  const int row0 = blockIdx.x * a.rows_per_block;
-  const int rows = min(a.rows_per_block, a.n_rows - row0);
-  long long* pool_row = reinterpret_cast<long long*>(turns + (size_t)a.rows_per_block * half);
-  for (int e = threadIdx.x; e < rows * half; e += 256)
-    turns[e] = turn_of(a, row0 + e / half, e % half);
-  if (SCATTER)
-    for (int e = threadIdx.x; e < rows; e += 256) pool_row[e] = pool_row_of(a, row0 + e);
-  __syncthreads();
-  // a head's units: R that turn and, where rows move, those behind them; v's heads move whole
-  const int units = SCATTER ? a.head_dim / 16 : R;
-  const int heads = a.n_heads + (SCATTER ? 2 : 1) * a.n_kv_heads;
-  const int per_row = heads * units;
-  for (int e = threadIdx.x; e < rows * per_row; e += 256) {
-    const int r = e / per_row, head = e % per_row / units, u = e % units;
-    const size_t row = row0 + r;
-    const int kv = head - a.n_heads, vv = kv - a.n_kv_heads;
-    const f16* src;
-    f16* dst;
-    if (kv < 0) {
-      src = a.q + row * a.ldq + (size_t)head * a.head_dim;
-      dst = a.q_out + row * a.ldq_out + (size_t)head * a.head_dim;
-    } else {
-      const long long to = SCATTER ? pool_row[r] : (long long)row;
-      if (to < 0) continue;
-      const bool is_v = SCATTER && vv >= 0;
-      const int h = is_v ? vv : kv;
-      src = (is_v ? a.v : a.k) + row * a.ldk + (size_t)h * a.head_dim;
-      dst = (is_v ? a.v_out : a.k_out) + to * a.ldk_out + (size_t)h * a.head_dim;
-    }
-    const bool moves = SCATTER && (u >= R || vv >= 0);
-    const int i = moves ? 2 * u : u, j = moves ? 2 * u + 1 : u + R;
-    f16x8 x = as_h8(ld16_stream(src + 8 * i)), y = as_h8(ld16_stream(src + 8 * j));
-    if (!moves) {
-      const float2* t = turns + (size_t)r * half;
-      if (PAIRS) turn<true>(x, y, t + 4 * i, t + 4 * j);
-      else turn<false>(x, y, t + 8 * i, nullptr);
-    }
-    st16_stream(dst + 8 * i, as_u4(x));
-    st16_stream(dst + 8 * j, as_u4(y));
+  const int tid = threadIdx.x, threads = blockDim.x, half = a.rotary_dim / 2, R = a.rotary_dim / 16;
+  const int group = blockIdx.x / a.chunks, row0 = group * a.rows, rows = min(a.rows, a.n_rows - row0);
+  const int unit = (blockIdx.x - group * a.chunks) * threads + tid;
+  long long* pool_row = reinterpret_cast<long long*>(turns + (size_t)a.rows * half);
+  const int n_turns = rows * half;
+  Angle angle;
+  if (tid < n_turns) {
+    const int r = (int)fdiv(tid, a.by_half);
+    angle = angle_of(a, row0 + r, tid - r * half);
   }
+  if (SCATTER && tid < rows) pool_row[tid] = pool_row_of(a, row0 + tid);
+  // a head's units: R that turn and, where rows move, those behind them; v's heads move whole
+  const int r = (int)fdiv(unit, a.by_row), rest = unit - r * a.per_row;
+  const int head = (int)fdiv(rest, a.by_unit), u = rest - head * (int)a.by_unit.d;
+  const int kv = head - a.n_heads, vv = kv - a.n_kv_heads;
+  const bool moves = SCATTER && (u >= R || vv >= 0);
+  const int i = moves ? 2 * u : u, j = moves ? 2 * u + 1 : u + R;
+  f16x8 x, y;
+  if (r < rows) {
+    const size_t row = row0 + r;
+    const f16* src = kv < 0               ? a.q + row * a.ldq + (size_t)head * a.head_dim
+                     : SCATTER && vv >= 0 ? a.v + row * a.ldk + (size_t)vv * a.head_dim
+                                          : a.k + row * a.ldk + (size_t)kv * a.head_dim;
+    x = as_h8(ld16_stream(src + 8 * i));
+    y = as_h8(ld16_stream(src + 8 * j));
+  }
+  if (tid < n_turns) turns[tid] = turn_of(angle);
+  for (int e = tid + threads; e < n_turns; e += threads) {
+    const int q = (int)fdiv(e, a.by_half);
+    turns[e] = turn_of(angle_of(a, row0 + q, e - q * half));
+  }
+  lds_barrier();
+  if (r >= rows) return;
+  const long long to = SCATTER && kv >= 0 ? pool_row[r] : (long long)(row0 + r);
+  if (to < 0) return;
+  f16* dst = kv < 0               ? a.q_out + to * a.ldq_out + (size_t)head * a.head_dim
+             : SCATTER && vv >= 0 ? a.v_out + to * a.ldk_out + (size_t)vv * a.head_dim
+                                  : a.k_out + to * a.ldk_out + (size_t)kv * a.head_dim;
+  if (!moves) {
+    const float2* t = turns + (size_t)r * half;
+    if (PAIRS) turn<true>(x, y, t + 4 * i, t + 4 * j);
+    else turn<false>(x, y, t + 8 * i, nullptr);
+  }
+  st16_stream(dst + 8 * i, as_u4(x));
+  st16_stream(dst + 8 * j, as_u4(y));
 }
 
 // Any sizes, strides and alignment, in place: a pair for each thread and step.
@@ -120,10 +136,10 @@ __global__ void __launch_bounds__(256) k_rotary_scalar(const RotaryArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float2* turns = reinterpret_cast<float2*>(smem);
   const int half = a.rotary_dim / 2;
-  const int row0 = blockIdx.x * a.rows_per_block;
-  const int rows = min(a.rows_per_block, a.n_rows - row0);
+  const int row0 = blockIdx.x * a.rows;
+  const int rows = min(a.rows, a.n_rows - row0);
   for (int e = threadIdx.x; e < rows * half; e += 256)
-    turns[e] = turn_of(a, row0 + e / half, e % half);
+    turns[e] = turn_of(angle_of(a, row0 + e / half, e % half));
   __syncthreads();
   const int per_row = (a.n_heads + a.n_kv_heads) * half;
   for (int e = threadIdx.x; e < rows * per_row; e += 256) {
@@ -139,11 +155,37 @@ __global__ void __launch_bounds__(256) k_rotary_scalar(const RotaryArgs a) {
   }
 }
 
-// Rows of a block: its cosines and sines fill at most 32 KiB.
+// Rows of a block of k_rotary_scalar: its cosines and sines fill at most 32 KiB.
 int rows_of_block(int n_rows, int half, int most) {
   int rows = 1;
   while (rows < most && (size_t)2 * rows * half * 8 <= 32768 && n_rows / (2 * rows) >= 512) rows *= 2;
   return rows;
+}
+
+// k_rotary's launch for rows of `heads` heads of `units` units each.
+template <bool SCATTER>
+int launch_rotary(RotaryArgs& a, int heads, int units, bool pairs, hipStream_t stream) {
+  const int half = a.rotary_dim / 2;
+  if ((long long)heads * units > 0x7FFFFFFF / 64) return LLMK_ERR_UNSUPPORTED;
+  a.per_row = heads * units;
+  // as many rows as 256 threads take (at most 8, whose page numbers and angles they load); a wide row by blocks
+  // of up to 512. Four units a thread, and rows to match, took 9.5 us and not 10.4 for 4000 rows of 40 heads of 64,
+  // but 20.4 and not 18.2 for 8000, 5.2 and not 4.4 for 1000, 4.2 and not 2.7 for 256.
+  a.rows = 256 / a.per_row;
+  a.rows = a.rows < 1 ? 1 : a.rows > 8 ? 8 : a.rows;
+  while (a.rows > 1 && (size_t)a.rows * half * 8 > 32768) --a.rows;
+  if (a.rows > a.n_rows) a.rows = a.n_rows;
+  const int units_all = a.rows * a.per_row;
+  a.chunks = (int)ceil_div(units_all, 512);
+  const int threads = (int)ceil_div(ceil_div(units_all, a.chunks), 64) * 64;
+  a.by_row = make_fastdiv((uint32_t)a.per_row);
+  a.by_unit = make_fastdiv((uint32_t)units);
+  a.by_half = make_fastdiv((uint32_t)half);
+  const size_t blocks = (size_t)ceil_div((size_t)a.n_rows, (size_t)a.rows) * a.chunks;
+  if (!grid_takes(blocks, 256)) return LLMK_ERR_UNSUPPORTED;
+  const size_t lds = (size_t)a.rows * (half * 8 + (SCATTER ? 8 : 0));
+  return launch(pairs ? k_rotary<true, SCATTER> : k_rotary<false, SCATTER>, dim3((unsigned)blocks),
+                dim3(threads), lds, stream, a);
 }
 
 int check_turn(const float* inv_freq, const int32_t* positions, int rotary_dim, int n_tables, int layout) {
@@ -187,19 +229,18 @@ extern "C" int llmk_rotary_apply(uint16_t* q, int ldq, uint16_t* k, int ldk, con
   a.head_dim = head_dim;
   a.rotary_dim = rotary_dim;
   a.n_tables = n_tables;
-  a.rows_per_block = rows_of_block(n_rows, rotary_dim / 2, 16);
-  const unsigned blocks = ceil_div((size_t)n_rows, (size_t)a.rows_per_block);
-  const size_t lds = (size_t)a.rows_per_block * (rotary_dim / 2) * 8;
-  if (!grid_takes(blocks, 256) ||
-      (long long)a.rows_per_block * (n_heads + n_kv_heads) * head_dim > 0x7FFFFFFF - 4096)
-    return LLMK_ERR_UNSUPPORTED;
   const bool vectors = head_dim % 8 == 0 && rotary_dim % 16 == 0 &&
                        (n_heads == 0 || (aligned16(q) && ldq % 8 == 0)) &&
                        (n_kv_heads == 0 || (aligned16(k) && ldk % 8 == 0));
   const bool pairs = layout == LLMK_ROTARY_PAIRS;
-  return launch(vectors ? (pairs ? k_rotary<true, false> : k_rotary<false, false>)
-                        : (pairs ? k_rotary_scalar<true> : k_rotary_scalar<false>),
-                dim3(blocks), dim3(256), lds, static_cast<hipStream_t>(stream), a);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (vectors) return launch_rotary<false>(a, n_heads + n_kv_heads, rotary_dim / 16, pairs, s);
+  a.rows = rows_of_block(n_rows, rotary_dim / 2, 16);
+  const unsigned blocks = ceil_div((size_t)n_rows, (size_t)a.rows);
+  if (!grid_takes(blocks, 256) || (long long)a.rows * (n_heads + n_kv_heads) * head_dim > 0x7FFFFFFF - 4096)
+    return LLMK_ERR_UNSUPPORTED;
+  return launch(pairs ? k_rotary_scalar<true> : k_rotary_scalar<false>, dim3(blocks), dim3(256),
+                (size_t)a.rows * (rotary_dim / 2) * 8, s, a);
 }
 
 extern "C" int llmk_qkv_rotary_scatter(const uint16_t* qkv, int ld, uint16_t* q_out, uint16_t* k_pool,
@@ -245,12 +286,6 @@ extern "C" int llmk_qkv_rotary_scatter(const uint16_t* qkv, int ld, uint16_t* q_
   a.n_tables = n_tables;
   a.max_pages = max_pages;
   a.page_size = page_size;
-  a.rows_per_block = rows_of_block(n, rotary_dim / 2, 16);
-  const unsigned blocks = ceil_div((size_t)n, (size_t)a.rows_per_block);
-  const size_t lds = (size_t)a.rows_per_block * ((rotary_dim / 2) * 8 + 8);
-  if (!grid_takes(blocks, 256) ||
-      (long long)a.rows_per_block * (n_heads + 2LL * n_kv_heads) * head_dim > 0x7FFFFFFF - 4096)
-    return LLMK_ERR_UNSUPPORTED;
-  return launch(layout == LLMK_ROTARY_PAIRS ? k_rotary<true, true> : k_rotary<false, true>,
-                dim3(blocks), dim3(256), lds, static_cast<hipStream_t>(stream), a);
+  return launch_rotary<true>(a, n_heads + 2 * n_kv_heads, head_dim / 16, layout == LLMK_ROTARY_PAIRS,
+                             static_cast<hipStream_t>(stream));
 }
