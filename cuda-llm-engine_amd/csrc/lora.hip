@@ -36,10 +36,10 @@ struct LoraArgs {
   const float* scales;
   f16* y;
   int* notes;   // workspace: [slots, kNote]
-  float* h;     // [splits, slots, kRows, n_parts * max_rank]
+  f32x4* h;     // [splits, slots, n_parts, steps of 32 ranks, 2, 64]: lane by lane as the second product wants it
   int part_end[kParts], chunk_end[kParts];  // columns, and blocks of k_lora_expand, up to each part's end
   int ldx, ldy, n_parts, n_rows, n_seqs, n_adapters, max_rank, in;
-  int slots, splits, groups, windows, per_block;
+  int slots, splits, groups, windows, per_block, steps;
 };
 
 __device__ __forceinline__ int first_row(const LoraArgs& g, int s) {
@@ -153,7 +153,7 @@ __device__ __forceinline__ void wave_sync() {
 
 // 16 rows of 512 bytes in LDS, in pieces of 16, which lie such that neither a row's 32 pieces nor a piece of
 // all rows share banks.
-typedef u32x4 Stage[kRows * 32];
+typedef u32x4 Stage[kRows * 32 + 4];  // and four more for 16 numbers behind them
 __device__ __forceinline__ int place_of(int row, int piece) { return row * 32 + (piece ^ row); }
 
 __device__ __forceinline__ void put_rows(u32x4* to, const u32x4 (&v)[8], int lane) {
@@ -245,8 +245,7 @@ __global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const Lora
   const int per_part = (rank + 15) / 16, all = g.n_parts * per_part;
   int xrow[8];
   rows_of_x(p, xrow, lane);
-  const size_t width = (size_t)g.n_parts * g.max_rank;
-  float* out = g.h + ((size_t)split * g.slots + slot) * kRows * width + n * width + 4 * q;
+  f32x4* out = g.h + ((size_t)split * g.slots + slot) * g.n_parts * g.steps * 128;
   for (int g0 = 0; g0 < all; g0 += NG) {
     f32x4 acc[NG];
     const f16* w[NG];
@@ -268,9 +267,10 @@ __global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const Lora
       f32x4 v[4];
 #pragma unroll
       for (int m = 0; m < 4; ++m) v[m] = __builtin_bit_cast(f32x4, stage[m][wave * 64 + lane]);
-      const int part = (g0 + wave) / per_part, j = (g0 + wave - part * per_part) * 16;
-      if (j + 4 * q < g.max_rank)
-        *reinterpret_cast<f32x4*>(out + (size_t)part * g.max_rank + j) = (v[0] + v[1]) + (v[2] + v[3]);
+      // ranks 4 q on of 16: numbers 4 (q & 1) on of the eight that lane (n, 2 (i & 1) + q / 2) has of step i / 2
+      const int part = (g0 + wave) / per_part, i = g0 + wave - part * per_part;
+      out[(((size_t)part * g.steps + i / 2) * 2 + (q & 1)) * 64 + (2 * (i & 1) + (q >> 1)) * 16 + n] =
+          (v[0] + v[1]) + (v[2] + v[3]);
     }
   }
 }
@@ -330,8 +330,8 @@ __device__ __forceinline__ float split_h(const float (&v)[KS][8], f16x8 (&hi)[KS
   return kv8::exp2_int(e);
 }
 
-// What is added to a wave's 16 rows and 16 * TILES columns: row n, columns 32 t + 8 q on of each pair of products,
-// times `by`, into LDS (in pieces of 16 bytes as above).
+// B h of a wave's 16 rows and 16 * TILES columns: row n, columns 32 t + 8 q on of each pair of products, into LDS
+// (in pieces of 16 bytes as above); and what the row's are to be multiplied by, behind them.
 template <int KS, int TILES>
 __device__ __forceinline__ void expand_columns(const u32x4 (&bf)[TILES][KS], const f16x8 (&hi)[KS],
                                                const f16x8 (&lo)[KS], float by, u32x4* to, int n, int q) {
@@ -343,10 +343,10 @@ __device__ __forceinline__ void expand_columns(const u32x4 (&bf)[TILES][KS], con
       d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[t][s]), hi[s], d, 0, 0, 0);
       d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[t][s]), lo[s], d, 0, 0, 0);
     }
-    d = f32x4{by * d[0], by * d[1], by * d[2], by * d[3]};
     to[n * 4 * TILES + ((8 * (t / 2) + 2 * q + (t & 1)) ^ (n & (4 * TILES - 1)))] =
         __builtin_bit_cast(u32x4, d);
   }
+  if (q == 0) reinterpret_cast<float*>(to + kRows * 4 * TILES)[n] = by;
 }
 
 // A wave's y: 2 * TILES lanes a row, eight columns each, so that accesses are of whole lines. row(t) is the
@@ -354,28 +354,51 @@ __device__ __forceinline__ void expand_columns(const u32x4 (&bf)[TILES][KS], con
 template <int TILES>
 __device__ __forceinline__ int y_row(int t, int lane) { return t * (32 / TILES) + lane / (2 * TILES); }
 
+// Whether all of the wave's accesses are: most tiles have 16 rows and most waves only columns of the part.
 template <int TILES>
-__device__ __forceinline__ void load_y(u32x4 (&old)[TILES / 2], f16* const (&y)[TILES / 2]) {
+__device__ __forceinline__ bool all_of(f16* const (&y)[TILES / 2]) {
+  bool all = true;
 #pragma unroll
-  for (int t = 0; t < TILES / 2; ++t)
-    if (y[t]) old[t] = ld16_stream(y[t]);
+  for (int t = 0; t < TILES / 2; ++t) all &= y[t] != nullptr;
+  return __builtin_amdgcn_ballot_w64(all) == ~0ull;
 }
 
 template <int TILES>
-__device__ __forceinline__ void add_to_y(const u32x4 (&old)[TILES / 2], f16* const (&y)[TILES / 2], const u32x4* from,
-                                         int lane) {
+__device__ __forceinline__ void load_y(u32x4 (&old)[TILES / 2], f16* const (&y)[TILES / 2], bool all) {
+  if (all) {
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t) old[t] = ld16_stream(y[t]);
+  } else {
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t)
+      if (y[t]) old[t] = ld16_stream(y[t]);
+  }
+}
+
+template <int TILES>
+__device__ __forceinline__ void add_to_y(u32x4 (&old)[TILES / 2], f16* const (&y)[TILES / 2], bool all,
+                                         const u32x4* from, int lane) {
 #pragma unroll
   for (int t = 0; t < TILES / 2; ++t) {
     const int r = y_row<TILES>(t, lane), piece = 2 * (lane % (2 * TILES)), flip = r & (4 * TILES - 1);
     const f32x4 u = __builtin_bit_cast(f32x4, from[r * 4 * TILES + (piece ^ flip)]);
     const f32x4 w = __builtin_bit_cast(f32x4, from[r * 4 * TILES + ((piece + 1) ^ flip)]);
+    const float by = reinterpret_cast<const float*>(from + kRows * 4 * TILES)[r];
     f16x8 v = as_h8(old[t]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[e] = (f16)((float)v[e] + u[e]);
-      v[e + 4] = (f16)((float)v[e + 4] + w[e]);
+    for (int e = 0; e < 4; ++e) {  // an instruction each: product and sum in fp32, one rounding
+      v[e] = (f16)__builtin_fmaf(u[e], by, (float)v[e]);
+      v[e + 4] = (f16)__builtin_fmaf(w[e], by, (float)v[e + 4]);
     }
-    if (y[t]) st16_stream(y[t], as_u4(v));
+    old[t] = as_u4(v);
+  }
+  if (all) {
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t) st16_stream(y[t], old[t]);
+  } else {
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t)
+      if (y[t]) st16_stream(y[t], old[t]);
   }
 }
 
@@ -393,7 +416,7 @@ __device__ __forceinline__ int part_of(const LoraArgs& g, int chunk, int* place)
 template <int KS, bool MANY>
 __global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_expand(const LoraArgs g) {
   constexpr int TILES = KS <= 2 ? 8 : 16 / KS;
-  __shared__ u32x4 stage[4][kRows * 4 * TILES];
+  __shared__ u32x4 stage[4][kRows * 4 * TILES + 4];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
   int place;
   const int chunks = g.chunk_end[g.n_parts - 1];
@@ -402,7 +425,6 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_exp
   const int c0 = (part ? g.part_end[part - 1] : 0) + (place * 4 + wave) * 16 * TILES;
   if (!MANY && c0 >= end) return;
   const int column = c0 + 8 * (lane % (2 * TILES));
-  const size_t width = (size_t)g.n_parts * g.max_rank;
   __shared__ f32x4 shared_h[MANY ? 4 : 1][KS][2][64];
   u32x4 bf[TILES][KS];
   int loaded = -1;
@@ -416,15 +438,13 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_exp
     for (int t = 0; t < TILES / 2; ++t) row[t] = note[kRows + y_row<TILES>(t, lane)];
     // the splits' sums: up to two by the wave itself, more by the block's waves, two each, through LDS
     float h[KS][8];
-    const float* from = g.h + ((size_t)slot * kRows + n) * width + (size_t)part * g.max_rank + 8 * q;
+    const f32x4* from = g.h + ((size_t)slot * g.n_parts + part) * g.steps * 128 + lane;
     const auto add_split = [&](f32x4 (&v)[KS][2], int split) {
+      const f32x4* u = from + (size_t)split * g.slots * g.n_parts * g.steps * 128;
 #pragma unroll
-      for (int s = 0; s < KS; ++s) {
-        const int k = min(32 * s, g.max_rank - 8 - 8 * q);  // behind max_rank: not read as numbers
-        const f32x4* u = reinterpret_cast<const f32x4*>(from + (size_t)split * g.slots * kRows * width + k);
-        v[s][0] = u[0];
-        v[s][1] = u[1];
-      }
+      for (int s = 0; s < KS; ++s)  // steps behind the last: its numbers, which rank cuts off
+#pragma unroll
+        for (int f = 0; f < 2; ++f) v[s][f] = u[(min(s, g.steps - 1) * 2 + f) * 64];
     };
     f32x4 u[KS][2], w[KS][2];
     const int one = MANY ? wave : 0, two = MANY ? wave + 4 : 1;
@@ -467,7 +487,8 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_exp
     for (int t = 0; t < TILES / 2; ++t)
       y[t] = (unsigned)row[t] < (unsigned)g.n_rows && column < end ? g.y + (size_t)row[t] * g.ldy + column
                                                                    : nullptr;
-    load_y<TILES>(old, y);
+    const bool all = all_of<TILES>(y);
+    load_y<TILES>(old, y, all);
     if (a != loaded) {
       loaded = a;
       load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
@@ -482,7 +503,7 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_exp
     wave_sync();
     expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q);
     wave_sync();
-    add_to_y<TILES>(old, y, stage[wave], lane);
+    add_to_y<TILES>(old, y, all, stage[wave], lane);
   }
 }
 
@@ -515,7 +536,8 @@ __global__ void __launch_bounds__(256, 2) k_lora_whole(const LoraArgs g) {
     const int row = p.row[y_row<TILES>(t, lane)];
     y[t] = row >= 0 && column < end ? g.y + (size_t)row * g.ldy + column : nullptr;
   }
-  load_y<TILES>(old, y);
+  const bool all = all_of<TILES>(y);
+  load_y<TILES>(old, y, all);
   load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
   f32x4 acc[NG];
   const f16* w[NG];
@@ -549,7 +571,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_whole(const LoraArgs g) {
   lds_barrier();  // the other waves have read what this one puts its columns over
   expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q);
   wave_sync();
-  add_to_y<TILES>(old, y, stage[wave], lane);
+  add_to_y<TILES>(old, y, all, stage[wave], lane);
 }
 
 // What a call takes of the chip and the workspace, by its sizes alone.
@@ -581,7 +603,7 @@ extern "C" size_t llmk_lora_add_workspace_floats(int n_rows, int n_seqs, int n_a
       n_parts <= 0)
     return 0;
   const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features);
-  return (size_t)s.slots * (kNote + (size_t)s.splits * kRows * n_parts * max_rank);
+  return (size_t)s.slots * (kNote + (size_t)s.splits * n_parts * ((max_rank + 31) / 32) * 512);
 }
 
 extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, const uint16_t* b,
@@ -623,7 +645,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.scales = scales;
   g.y = reinterpret_cast<f16*>(y);
   g.notes = reinterpret_cast<int*>(workspace);
-  g.h = workspace + (size_t)s.slots * kNote;
+  g.h = reinterpret_cast<f32x4*>(workspace + (size_t)s.slots * kNote);
   g.ldx = ldx;
   g.ldy = ldy;
   g.n_parts = n_parts;
@@ -633,6 +655,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.max_rank = max_rank;
   g.in = in_features;
   g.slots = s.slots;
+  g.steps = steps;
   g.splits = s.splits;
   g.groups = s.groups;
   g.windows = s.windows;
