@@ -682,13 +682,14 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
     return launch(narrow ? k_lora_whole<4> : k_lora_whole<8>, dim3((s.slots + 7) / 8 * 8 * blocks), dim3(256),
                   0, st, g);
   }
+  g.per_block = 1;
+  while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= 2048) g.per_block *= 2;
+  if (!grid_takes((size_t)chunks * ceil_div(s.slots, g.per_block), 256)) return LLMK_ERR_UNSUPPORTED;
   const int all = n_parts * per_part;
   const int status = launch(all == 1 ? k_lora_shrink<1> : all == 3 ? k_lora_shrink<3> : k_lora_shrink<2>,
                             dim3(s.splits * s.slots), dim3(256), 0, st, g);
   if (status != LLMK_OK) return status;
-  g.per_block = 1;
-  while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= 2048) g.per_block *= 2;
-  const dim3 grid(chunks * ceil_div(s.slots, g.per_block));
+  const dim3 grid(chunks * ceil_div(s.slots, g.per_block));  // fits: checked in front of the first launch
   const bool many = s.splits > 2;
   return launch(ks == 1   ? (many ? k_lora_expand<1, true> : k_lora_expand<1, false>)
                 : ks == 2 ? (many ? k_lora_expand<2, true> : k_lora_expand<2, false>)

@@ -2,6 +2,8 @@
 // its counts of holders, and compaction. Integers but for the copies; nothing depends on the order in
 // which blocks run: counts are added up, and every page number comes from a count of what lies in front.
 
+#include <limits.h>
+
 #include "common.hpp"
 
 namespace llmk {
@@ -278,7 +280,7 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, int* found_begin, i
   if (threadIdx.x == 0) {
     const long long given = found < wanted ? found : wanted;
     a.counts[0] = (int)given;
-    a.counts[1] = (int)(wanted - given);
+    a.counts[1] = (int)min(wanted - given, (long long)INT_MAX);
   }
 }
 

@@ -400,7 +400,8 @@ LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_lo
  * may be a fused one: its n_parts (1 to 8) parts end at columns part_ends[0] < part_ends[1] < .. (a
  * HOST array; q|k|v, gate|up; one part: its width), and an adapter has an A for each of them.
  * a [n_adapters, n_parts, max_rank, in_features], b [n_adapters, part_ends[n_parts - 1], max_rank];
- * ranks [n_adapters], or NULL for max_rank: what lies past an adapter's rank is not read as numbers.
+ * ranks [n_adapters], or NULL for max_rank (larger ones count as it): what lies past an adapter's rank is not read
+ * as numbers.
  * scales [n_adapters], or NULL for 1. Sequence s owns the rows row_starts[s] .. row_starts[s + 1] - 1
  * (NULL: one row each, n_rows == n_seqs), as the batches of the 8-bit cache do. Rows of no
  * sequence, of an adapter outside [0, n_adapters) and of one of rank <= 0 are left as they are, bit
@@ -409,8 +410,9 @@ LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_lo
  * x rows have stride ldx and y rows ldy (elements, multiples of 8); in_features, max_rank (at most
  * 256) and the part ends are multiples of 8; x, a, b and y are 16-byte aligned. x and y may not overlap.
  * workspace: llmk_lora_add_workspace_floats(..) floats, 16-byte aligned; calls that may overlap need
- * one each, graphs replayed one behind the other may share one. LLMK_ERR_UNSUPPORTED for more than
- * 2^20 rows or sequences. */
+ * one each, graphs replayed one behind the other may share one. LLMK_ERR_UNSUPPORTED, before any launch, for more
+ * than 2^20 rows or sequences, 2^24 in_features or 65535 * 512 columns (fewer for ranks past 64), or rows times
+ * columns past 2^38. */
 LLMK_API size_t llmk_lora_add_workspace_floats(int n_rows, int n_seqs, int n_adapters, int max_rank,
                                                int in_features, int n_parts);
 LLMK_API int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, const uint16_t* b,
