@@ -449,6 +449,12 @@ bool fork_by_one_block(int n_old, int n_new, int max_pages) {
 }
 bool compact_by_one_block(int num_pages, long long entries) { return num_pages <= kChunk && entries <= 8192; }
 
+// Whether two arrays of ints share memory.
+bool overlap(const int32_t* a, size_t n, const int32_t* b, size_t m) {
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+  return a && b && n && m && x < y + 4 * m && y < x + 4 * n;
+}
+
 }  // namespace
 }  // namespace llmk
 
@@ -523,8 +529,18 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   if (!refs || !counts || !workspace || (n_old > 0 && (!block_tables || !seq_lens)) ||
       (n_new > 0 && (!parents || !new_tables || !new_lens || !copies)))
     return LLMK_ERR_INVALID_VALUE;
-  if (reinterpret_cast<uintptr_t>(workspace) % 8) return LLMK_ERR_ALIGNMENT;
   if (n_old > 65535 || n_new > 65535 || max_pages > (1 << 24)) return LLMK_ERR_UNSUPPORTED;
+  {  // what is written, and what else there is
+    const size_t n = n_new, m = n_old, width = max_pages;
+    const int32_t* at[] = {refs,   new_tables, new_lens,     copies,   counts,
+                           workspace, block_tables, seq_lens, parents, reserve};
+    const size_t size[] = {(size_t)num_pages, n * width, n, 2 * n, 2,
+                           llmk_kv_fork_workspace_ints(n_old, n_new, max_pages, num_pages), m * width, m, n, n};
+    for (int i = 0; i < 6; ++i)
+      for (int j = i + 1; j < 10; ++j)
+        if (overlap(at[i], size[i], at[j], size[j])) return LLMK_ERR_INVALID_VALUE;
+  }
+  if (reinterpret_cast<uintptr_t>(workspace) % 8) return LLMK_ERR_ALIGNMENT;
   hipStream_t s = static_cast<hipStream_t>(stream);
   ForkArgs a{};
   a.tables = block_tables;
@@ -569,6 +585,17 @@ extern "C" int llmk_kv_compact(const int32_t* block_tables, const int32_t* refs,
       (n_seqs > 0 && (!block_tables || !new_tables)))
     return LLMK_ERR_INVALID_VALUE;
   if (num_pages > (1 << 24)) return LLMK_ERR_UNSUPPORTED;
+  {
+    const size_t pages = num_pages, entries = (size_t)n_seqs * max_pages;
+    const int32_t* at[] = {new_tables, new_refs, copies, counts, workspace, block_tables, refs};
+    const size_t size[] = {entries, pages, 2 * (pages / 2), 2, llmk_kv_compact_workspace_ints(num_pages),
+                           entries, pages};
+    for (int i = 0; i < 5; ++i)
+      for (int j = i + 1; j < 7; ++j) {
+        const bool same = at[i] == at[j] && ((i == 0 && j == 5) || (i == 1 && j == 6));
+        if (!same && overlap(at[i], size[i], at[j], size[j])) return LLMK_ERR_INVALID_VALUE;
+      }
+  }
   hipStream_t s = static_cast<hipStream_t>(stream);
   CompactArgs a{};
   a.tables = block_tables;

@@ -503,7 +503,8 @@ LLMK_API int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, in
  * taken over, in the order of (c, j); where they run out the entry is -1. new_lens [n_new] = L; copies
  * [n_new, 2] is (-1, -1) where nothing is to be copied (llmk_kv_copy_pages does that); counts [2] = fresh pages
  * given, and lacking (the table's row of a child that lacks some is then too short for L + reserve). refs is
- * brought up to date. n_new == 0 frees the old batch. New and old arrays may not overlap.
+ * brought up to date. n_new == 0 frees the old batch. No array that is written may overlap another
+ * (LLMK_ERR_INVALID_VALUE).
  * workspace: llmk_kv_fork_workspace_ints(..) int32, 8-byte aligned. Batches up to 65535 sequences. */
 LLMK_API size_t llmk_kv_fork_workspace_ints(int n_old, int n_new, int max_pages, int num_pages);
 LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
@@ -516,7 +517,7 @@ LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
  * goes to the k-th free page below n. new_tables [n_seqs, max_pages] names pages by their new numbers (entries
  * that are no held page stay as they are), new_refs [num_pages] counts their holders; copies [num_pages / 2, 2]
  * gets the pairs (from, to), whose number is counts[0] (counts[1] = n), for llmk_kv_copy_pages. new_tables may be
- * block_tables, new_refs may be refs. workspace: llmk_kv_compact_workspace_ints(num_pages) int32. num_pages up to
+ * block_tables, new_refs may be refs; other arrays may not overlap (LLMK_ERR_INVALID_VALUE). workspace: llmk_kv_compact_workspace_ints(num_pages) int32. num_pages up to
  * 2^24. */
 LLMK_API size_t llmk_kv_compact_workspace_ints(int num_pages);
 LLMK_API int llmk_kv_compact(const int32_t* block_tables, const int32_t* refs, int32_t* new_tables,

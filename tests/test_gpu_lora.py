@@ -267,6 +267,31 @@ def test_on_another_stream(llmk):
     assert (np.abs(y.cpu().numpy().astype(np.float64) - want) <= bound)[c.has()].all()
 
 
+def test_offsets_past_32_bits(llmk):
+    """Rows of x and y and an adapter's weights whose bytes lie past 2^32."""
+    rng = np.random.default_rng(16)
+    n, ldx, ldy, inner = 40000, 65536, 65536, 16384
+    x = torch.zeros(n, ldx, dtype=torch.float16, device=DEV)
+    y = torch.zeros(n, ldy, dtype=torch.float16, device=DEV)
+    a = torch.zeros(710, 1, 256, inner, dtype=torch.float16, device=DEV)  # 8 MiB each
+    b = torch.zeros(710, 64, 256, dtype=torch.float16, device=DEV)
+    row, rank = n - 3, 5
+    x[row, :inner], y[row, :64] = half(rng.standard_normal(inner)), half(rng.standard_normal(64))
+    a[709, 0, :rank] = half(rng.standard_normal((rank, inner)) * inner ** -0.5)
+    b[709, :, :rank] = half(rng.standard_normal((64, rank)))
+    ids = torch.full((n,), -1, dtype=torch.int32, device=DEV)
+    ids[row] = 709
+    ranks = torch.full((710,), rank, dtype=torch.int32, device=DEV)
+    want, bound = ref.lora_add(x[row:row + 1, :inner].cpu().numpy(), a[709:].cpu().numpy(), b[709:].cpu().numpy(),
+                               np.array([rank]), None, [0], None, y[row:row + 1, :64].cpu().numpy(), (64,))
+    ws = torch.empty(llmk.lora_add_workspace_floats(n, n, 710, 256, inner, 1), device=DEV)
+    llmk.lora_add(x, ldx, a, b, ranks, None, ids, None, y, ldy, (64,), ws, n, n, 710, 256, inner)
+    got = y[row, :64].cpu().numpy().astype(np.float64)
+    assert (np.abs(got - want[0]) <= bound[0]).all()
+    y[row, :64] = 0
+    assert not y.any()
+
+
 def test_columns_of_wider_tensors(llmk):
     """x and y as views of columns: what lies beside them stays."""
     rng = np.random.default_rng(15)

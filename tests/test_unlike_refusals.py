@@ -44,14 +44,17 @@ def copy_pages(L, **kw):
     return L.llmk_kv_copy_pages(*a.values(), None)
 
 
+AT = [FAKE + 0x1000 * i for i in range(12)]  # arrays apart from one another
+
+
 def fork(L, **kw):
-    a = dict(tables=FAKE, lens=FAKE, parents=FAKE, reserve=None, refs=FAKE, new=FAKE, new_lens=FAKE,
-             copies=FAKE, counts=FAKE, ws=FAKE, n_old=2, n_new=2, max_pages=4, page=16, pages=9) | kw
+    a = dict(tables=AT[0], lens=AT[1], parents=AT[2], reserve=None, refs=AT[3], new=AT[4], new_lens=AT[5],
+             copies=AT[6], counts=AT[7], ws=AT[8], n_old=2, n_new=2, max_pages=4, page=16, pages=9) | kw
     return L.llmk_kv_fork(*a.values(), None)
 
 
 def compact(L, **kw):
-    a = dict(tables=FAKE, refs=FAKE, new=FAKE, new_refs=FAKE, copies=FAKE, counts=FAKE, ws=FAKE, n=2,
+    a = dict(tables=AT[0], refs=AT[1], new=AT[2], new_refs=AT[3], copies=AT[4], counts=AT[5], ws=AT[6], n=2,
              max_pages=4, pages=9) | kw
     return L.llmk_kv_compact(*a.values(), None)
 
@@ -121,14 +124,23 @@ def test_pages(llmk):
                 dict(refs=None), dict(counts=None), dict(ws=None), dict(tables=None), dict(lens=None),
                 dict(parents=None), dict(new=None), dict(new_lens=None), dict(copies=None)):
         assert fork(L, **bad) == E.LLMK_ERR_INVALID_VALUE, bad
+    for bad in (dict(new=AT[0]), dict(new=AT[0] + 28), dict(new_lens=AT[1] + 4), dict(refs=AT[0]), dict(ws=AT[4]),
+                dict(copies=AT[2]), dict(counts=AT[3] + 32), dict(reserve=AT[5])):
+        assert fork(L, **bad) == E.LLMK_ERR_INVALID_VALUE, bad
+    apart = dict(new=1 << 36, ws=1 << 40, new_lens=1 << 44, copies=1 << 43, tables=1 << 45)
     for bad in (dict(n_old=65536), dict(n_new=65536), dict(max_pages=(1 << 24) + 1)):
-        assert fork(L, **bad) == E.LLMK_ERR_UNSUPPORTED, bad
+        assert fork(L, **(apart | bad)) == E.LLMK_ERR_UNSUPPORTED, bad
+    assert fork(L, ws=AT[8] + 4) == E.LLMK_ERR_ALIGNMENT
     assert llmk.kv_fork_workspace_ints(-1, 1, 1, 1) == llmk.kv_fork_workspace_ints(1, 1, 0, 1) == 0
 
     for bad in (dict(n=-1), dict(max_pages=0), dict(pages=0), dict(refs=None), dict(new_refs=None),
                 dict(copies=None), dict(counts=None), dict(ws=None), dict(tables=None), dict(new=None)):
         assert compact(L, **bad) == E.LLMK_ERR_INVALID_VALUE, bad
-    assert compact(L, pages=(1 << 24) + 1) == E.LLMK_ERR_UNSUPPORTED
+    for bad in (dict(new=AT[0] + 4), dict(new=AT[0] - 4), dict(new_refs=AT[1] + 32), dict(copies=AT[0]),
+                dict(counts=AT[1]), dict(ws=AT[4]), dict(new=AT[1]), dict(new_refs=AT[0])):
+        assert compact(L, **bad) == E.LLMK_ERR_INVALID_VALUE, bad
+    apart = dict(refs=1 << 36, new_refs=1 << 37, copies=1 << 38, ws=1 << 40)
+    assert compact(L, pages=(1 << 24) + 1, **apart) == E.LLMK_ERR_UNSUPPORTED
     assert llmk.kv_compact_workspace_ints(0) == 0
 
 
