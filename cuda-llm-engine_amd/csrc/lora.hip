@@ -29,6 +29,7 @@ constexpr int kWindow = 256, kHash = 512;
 constexpr int kRows = 16;   // of a tile
 constexpr int kNote = 32;   // ints of a tile's note: adapter (-1: no tile), rank, scale; from 16 on its rows (-1: none)
 constexpr int kChunk = 256;  // of in_features that a wave takes at a time
+constexpr int kWaves = 8;    // of a block of k_lora_whole
 
 struct LoraArgs {
   const f16 *x, *a, *b;
@@ -39,7 +40,8 @@ struct LoraArgs {
   f32x4* h;     // [splits, slots, n_parts, steps of 32 ranks, 2, 64]: lane by lane as the second product wants it
   int part_end[kParts], chunk_end[kParts];  // columns, and blocks of k_lora_expand, up to each part's end
   int ldx, ldy, n_parts, n_rows, n_seqs, n_adapters, max_rank, in;
-  int slots, splits, groups, windows, per_block, steps;
+  int slots, splits, groups, windows, steps;
+  int per_block;  // tiles of a block of k_lora_expand; for k_lora_whole, whether a tile's blocks share an XCD
 };
 
 __device__ __forceinline__ int first_row(const LoraArgs& g, int s) {
@@ -51,10 +53,10 @@ __device__ __forceinline__ int slot_of_window(const LoraArgs& g, int w) {
   return first_row(g, min(w * kWindow, g.n_seqs)) / kRows + w * (g.groups + 1);
 }
 
-// The sum of v over the threads in front, of 256. part: four ints that no thread still reads.
+// The sum of v over the threads in front, of the first 256. part: four ints that no thread still reads.
 __device__ __forceinline__ int block_scan(int v, int* part) {
   const int wave = threadIdx.x >> 6, in = wave_scan(v);
-  if ((threadIdx.x & 63) == 63) part[wave] = in;
+  if ((threadIdx.x & 63) == 63 && wave < 4) part[wave] = in;
   lds_barrier();
   int before = 0;
 #pragma unroll
@@ -140,7 +142,7 @@ __device__ __forceinline__ Tile find_tile_by_wave(const LoraArgs& g, int slot, P
   return {-1, 0, 0.f};
 }
 
-// Finds tile `slot` with 256 threads.
+// Finds tile `slot` with 256 threads or more.
 __device__ __forceinline__ Tile find_tile(const LoraArgs& g, int slot, Plan& p) {
   // one sequence's call takes 5.7 us so and 6.3 by the table, 48 sequences' of 16 adapters 12.6 and 12.1
   if (g.groups <= 4 && g.n_seqs <= 64) return find_tile_by_wave(g, slot, p);
@@ -152,7 +154,7 @@ __device__ __forceinline__ Tile find_tile(const LoraArgs& g, int slot, Plan& p) 
   }
   const int s = w * kWindow + tid;
   int id = -1, r0 = 0, rows = 0;
-  if (s < g.n_seqs) {
+  if (tid < kWindow && s < g.n_seqs) {
     id = g.ids[s];
     r0 = first_row(g, s);
     rows = g.starts ? max(first_row(g, s + 1) - r0, 0) : 1;
@@ -564,14 +566,15 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_exp
 }
 
 // Both products of a tile and a block's columns in one launch: every block computes the h of its part again.
-template <int TILES>
-__global__ void __launch_bounds__(256, 2) k_lora_whole(const LoraArgs g) {
-  constexpr int KS = 1, NG = 2;
+template <int TILES, int NG>
+__global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g) {
+  constexpr int KS = 1;
   __shared__ Plan p;
-  __shared__ Stage stage[4];
-  // a tile's blocks share an XCD, whose L2 then reads its weights once
-  const int chunks = g.chunk_end[g.n_parts - 1], turn = blockIdx.x / 8;
-  const int slot = blockIdx.x % 8 + turn / chunks * 8;
+  __shared__ Stage stage[kWaves];
+  // a tile's blocks share an XCD, whose L2 then reads its weights once, unless few tiles would leave most CUs idle
+  // (one tile's 64 blocks 8.7 us, and 4.9 for 4)
+  const int chunks = g.chunk_end[g.n_parts - 1], turn = g.per_block ? blockIdx.x / 8 : blockIdx.x;
+  const int slot = g.per_block ? blockIdx.x % 8 + turn / chunks * 8 : turn / chunks;
   if (slot >= g.slots) return;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
   const Tile tile = find_tile(g, slot, p);
@@ -580,7 +583,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_whole(const LoraArgs g) {
   int place;
   const int part = part_of(g, turn % chunks, &place);
   const int end = g.part_end[part], out = g.part_end[g.n_parts - 1];
-  const int c0 = (part ? g.part_end[part - 1] : 0) + (place * 4 + wave) * 16 * TILES;
+  const int c0 = (part ? g.part_end[part - 1] : 0) + (place * kWaves + wave) * 16 * TILES;
   const int column = c0 + 8 * (lane % (2 * TILES));
   int xrow[8];
   rows_of_x(p, xrow, lane);
@@ -604,7 +607,7 @@ __global__ void __launch_bounds__(256, 2) k_lora_whole(const LoraArgs g) {
     w[i] = g.a + (((size_t)a * g.n_parts + part) * g.max_rank + 16 * i) * g.in;
     left[i] = rank - 1 - 16 * i;
   }
-  shrink_chunks<NG>(acc, g, xrow, w, left, (rank + 15) / 16, wave, 4, stage[wave], lane);
+  shrink_chunks<NG>(acc, g, xrow, w, left, (rank + 15) / 16, wave, kWaves, stage[wave], lane);
 #pragma unroll
   for (int i = 0; i < NG; ++i) stage[wave][i * 64 + lane] = __builtin_bit_cast(u32x4, acc[i]);
   lds_barrier();
@@ -613,11 +616,14 @@ __global__ void __launch_bounds__(256, 2) k_lora_whole(const LoraArgs g) {
   for (int s = 0; s < KS; ++s)
 #pragma unroll
     for (int f = 0; f < 2; ++f) {
-      const int at = (2 * s + (q >> 1)) * 64 + (q & 1) * 32 + f * 16 + n;
-      f32x4 v[4];
+      const int at = (NG == 1 ? 0 : q >> 1) * 64 + (q & 1) * 32 + f * 16 + n;  // NG 1: the ranks past 16 are cut
+      f32x4 v[kWaves];
 #pragma unroll
-      for (int m = 0; m < 4; ++m) v[m] = __builtin_bit_cast(f32x4, stage[m][at]);
-      v[0] = (v[0] + v[1]) + (v[2] + v[3]);
+      for (int m = 0; m < kWaves; ++m) v[m] = __builtin_bit_cast(f32x4, stage[m][at]);
+#pragma unroll
+      for (int d = kWaves / 2; d > 0; d /= 2)
+#pragma unroll
+        for (int m = 0; m < d; ++m) v[m] += v[m + d];
 #pragma unroll
       for (int e = 0; e < 4; ++e) h[s][4 * f + e] = 32 * s + 8 * q + 4 * f + e < rank ? v[0][e] : 0.f;
     }
@@ -718,25 +724,33 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int chunks = g.chunk_end[n_parts - 1];
   const int per_part = (max_rank + 15) / 16;
-  // Both products in one launch, if a block's own h costs it little: 32 ranks, and few enough numbers of A and x (a
-  // wave's quarter is 2048 of 16 ranks or 1366 of 32), read by few enough blocks. At 16 ranks and 2048 columns, 4
-  // sequences: in_features 1024 5.8 us and not 8.3 of two launches, 2048 6.6 and 8.7, 4096 8.3 and 8.8, 8192 11.6 and
-  // 9.5. At 2048 and 16384 columns, 8 sequences (38 MB) 7.5 and 8.7, 128 (105 MB) 10.9 and 11.6; at 4096 and 16384,
-  // 8 sequences (75 MB) 9.3 and 9.0, 16 (151 MB) 11.9 and 10.1. A launch more is 2 us of the host's time, too.
-  const size_t whole = (size_t)s.slots * chunks * 16 * (per_part + 1) * 2 * in_features;
-  if (ks == 1 && (per_part + 1) * (size_t)in_features <= 8192 && whole <= 96000000) {
-    // 256 columns a block and not 512 while that is a block a CU: 5.8 us and not 6.2 for 20 of 512 columns, but 6.8
-    // and not 6.6 for 216
-    const bool narrow = (long long)s.slots * 2 * chunks <= 256;
-    int blocks = chunks;
-    if (narrow) {
-      for (int p = 0; p < n_parts; ++p)
-        g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
-                         (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), columns / 2);
-      blocks = g.chunk_end[n_parts - 1];
-    }
-    return launch(narrow ? k_lora_whole<4> : k_lora_whole<8>, dim3((s.slots + 7) / 8 * 8 * blocks), dim3(256),
-                  0, st, g);
+  // Both products in one launch, if a block's own h costs it little: 32 ranks at most, few enough numbers of A and x for
+  // a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. At 16
+  // ranks and 2048 columns, 4 sequences: in_features 1024 5.4 us and not 8.0 of two launches, 2048 5.8 and 8.1, 4096
+  // 7.2 and 8.5, 6144 8.5 and 8.5, 8192 9.8 and 8.7; at 32 ranks 4096 9.0 and 9.2, 6144 10.7 and 9.3. At 16 ranks
+  // and 16384 columns 2048 numbers of 128 sequences (52 MB) take 10.5 us and 11.5, 4096 of 16 (75 MB) 10.6 and 9.7, of
+  // 128 (105 MB) 14.0 and 12.2. A launch more is 2 us of the host's time, too.
+  int tiles = 2, blocks = 0;
+  for (;; tiles *= 2) {
+    blocks = 0;
+    for (int p = 0; p < n_parts; ++p)
+      blocks += (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
+    if (tiles == 8 || (long long)s.slots * blocks <= 256) break;
+  }
+  const size_t whole = (size_t)s.slots * blocks * 16 * (per_part + 1) * 2 * in_features;
+  if (ks == 1 && (per_part + 1) * (size_t)in_features <= 12288 && whole <= 70000000) {
+    for (int p = 0; p < n_parts; ++p)
+      g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
+                       (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
+    g.per_block = s.slots >= 8 || blocks <= 32;  // whether a tile's blocks share an XCD
+    const dim3 grid((g.per_block ? (s.slots + 7) / 8 * 8 : s.slots) * blocks), threads(64 * kWaves);
+    return launch(per_part == 1 ? (tiles == 2   ? k_lora_whole<2, 1>
+                                   : tiles == 4 ? k_lora_whole<4, 1>
+                                                : k_lora_whole<8, 1>)
+                                : (tiles == 2   ? k_lora_whole<2, 2>
+                                   : tiles == 4 ? k_lora_whole<4, 2>
+                                                : k_lora_whole<8, 2>),
+                  grid, threads, 0, st, g);
   }
   g.per_block = 1;
   while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= 2048) g.per_block *= 2;

@@ -130,6 +130,19 @@ def test_parts_and_ranks(llmk, ends, rank):
          ranks=rng.integers(1, rank + 1, 4)).check(llmk)
 
 
+@pytest.mark.parametrize("n,adapters,rank,ends", [
+    (1, 1, 16, (16384,)), (1, 2, 32, (11008, 22016)), (3, 3, 8, (16384,)), (9, 4, 24, (8192, 16384)),
+    (20, 16, 16, (6144,)), (40, 20, 16, (16384,)), (100, 3, 32, (4096, 5120, 6144)), (64, 1, 64, (16384,)),
+    (30, 7, 128, (8192,)), (17, 5, 256, (2504, 5000))])
+def test_wide_projections(llmk, n, adapters, rank, ends):
+    """Few columns a block and many, a tile's blocks together and spread, few and many tiles a block."""
+    rng = np.random.default_rng([n, ends[-1]])
+    Case(rng, ids_of(rng, n, adapters), None, adapters, rank, 264, ends).check(llmk)
+    rows = rng.integers(0, 60, n) if n <= 40 else rng.integers(0, 9, n)
+    Case(rng, ids_of(rng, n, adapters, 0.05), rows, adapters, rank, 2048 if n < 30 else 1032, ends,
+         ranks=rng.integers(1, rank + 1, adapters), behind=2).check(llmk)
+
+
 @pytest.mark.parametrize("rows", [1, 2, 7, 15, 16, 17, 31, 33, 64, 65, 130, 257, 700])
 def test_one_sequence(llmk, rows):
     rng = np.random.default_rng(rows)
