@@ -41,6 +41,7 @@ struct LoraArgs {
   int part_end[kParts], chunk_end[kParts];  // columns, and blocks of k_lora_expand, up to each part's end
   int ldx, ldy, n_parts, n_rows, n_seqs, n_adapters, max_rank, in;
   int slots, splits, groups, windows, steps;
+  int turns;      // blocks of k_lora_shrink that share out the products of a tile and split
   int per_block;  // tiles of a block of k_lora_expand; for k_lora_whole, whether a tile's blocks share an XCD
 };
 
@@ -286,11 +287,12 @@ template <int NG>
 __global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const LoraArgs g) {
   __shared__ Plan p;
   __shared__ Stage stage[4];
-  const int slot = blockIdx.x / g.splits, split = blockIdx.x % g.splits;
+  const int slot = blockIdx.x / (g.splits * g.turns), rest = blockIdx.x - slot * g.splits * g.turns;
+  const int split = rest / g.turns, turn = rest - split * g.turns;
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
   const Tile tile = find_tile(g, slot, p);
   const int a = tile.adapter, rank = tile.rank;
-  if (split == 0) {
+  if (rest == 0) {
     int* note = g.notes + (size_t)slot * kNote;
     if (threadIdx.x == 0) {
       note[0] = a;
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const Lora
   int xrow[8];
   rows_of_x(p, xrow, lane);
   f32x4* out = g.h + ((size_t)split * g.slots + slot) * g.n_parts * g.steps * 128;
-  for (int g0 = 0; g0 < all; g0 += NG) {
+  for (int g0 = turn * NG; g0 < all; g0 += g.turns * NG) {
     f32x4 acc[NG];
     const f16* w[NG];
     int left[NG];
@@ -315,7 +317,7 @@ __global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const Lora
       w[i] = g.a + (((size_t)a * g.n_parts + part) * g.max_rank + j) * g.in;
       left[i] = rank - 1 - j;
     }
-    if (g0) lds_barrier();
+    if (g0 >= g.turns * NG) lds_barrier();  // behind what is read of the last ones' sums
     shrink_chunks<NG>(acc, g, xrow, w, left, all - g0, split * 4 + wave, 4 * g.splits, stage[wave], lane);
     // the four waves' sums
 #pragma unroll
@@ -755,9 +757,12 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.per_block = 1;
   while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= 2048) g.per_block *= 2;
   if (!grid_takes((size_t)chunks * ceil_div(s.slots, g.per_block), 256)) return LLMK_ERR_UNSUPPORTED;
-  const int all = n_parts * per_part;
-  const int status = launch(all == 1 ? k_lora_shrink<1> : all == 3 ? k_lora_shrink<3> : k_lora_shrink<2>,
-                            dim3(s.splits * s.slots), dim3(256), 0, st, g);
+  // products of 16 ranks at a time, and blocks for them while there are few: one tile of 3 parts of 128 ranks
+  const int all = n_parts * per_part, at_once = all == 1 ? 1 : all == 3 ? 3 : 2, passes = (all + at_once - 1) / at_once;
+  const int room = 1024 / (s.slots * s.splits);
+  g.turns = room < 1 ? 1 : room < passes ? room : passes;
+  const int status = launch(at_once == 1 ? k_lora_shrink<1> : at_once == 3 ? k_lora_shrink<3> : k_lora_shrink<2>,
+                            dim3(s.splits * s.slots * g.turns), dim3(256), 0, st, g);
   if (status != LLMK_OK) return status;
   const dim3 grid(chunks * ceil_div(s.slots, g.per_block));  // fits: checked in front of the first launch
   const bool many = s.splits > 2;
