@@ -363,6 +363,23 @@ __device__ __forceinline__ void cut_b(u32x4 (&bf)[TILES][KS], int rank, int q) {
     }
 }
 
+// 2^e for a row whose largest magnitude is `most`: that times 2^-e (*down) is from 2^14 to 2^15.
+__device__ __forceinline__ float power_of(float most, float* down) {
+  int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14;
+  e = e < -100 ? -100 : e;
+  *down = kv8::exp2_int(-e);
+  return kv8::exp2_int(e);
+}
+// Eight numbers times 2^-e as two fp16 each.
+__device__ __forceinline__ void two_halves(const float (&v)[8], float down, f16x8& hi, f16x8& lo) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float u = v[i] * down;
+    hi[i] = (f16)u;
+    lo[i] = __builtin_fabsf(u) < INFINITY ? (f16)(u - (float)hi[i]) : (f16)0;
+  }
+}
+
 // A lane's h (row n, ranks 32 s + 8 q on) as two fp16 each; returns the 2^e that they are to be multiplied by.
 template <int KS>
 __device__ __forceinline__ float split_h(const float (&v)[KS][8], f16x8 (&hi)[KS], f16x8 (&lo)[KS]) {
@@ -376,18 +393,11 @@ __device__ __forceinline__ float split_h(const float (&v)[KS][8], f16x8 (&hi)[KS
     }
   most = __builtin_fmaxf(most, __shfl_xor(most, 16));
   most = __builtin_fmaxf(most, __shfl_xor(most, 32));
-  int e = (int)(__builtin_bit_cast(uint32_t, most) >> 23) - 127 - 14;
-  e = e < -100 ? -100 : e;
-  const float down = kv8::exp2_int(-e);
+  float down;
+  const float up = power_of(most, &down);
 #pragma unroll
-  for (int s = 0; s < KS; ++s)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float u = v[s][i] * down;
-      hi[s][i] = (f16)u;
-      lo[s][i] = __builtin_fabsf(u) < INFINITY ? (f16)(u - (float)hi[s][i]) : (f16)0;
-    }
-  return kv8::exp2_int(e);
+  for (int s = 0; s < KS; ++s) two_halves(v[s], down, hi[s], lo[s]);
+  return up;
 }
 
 // B h of a wave's 16 rows and 16 * TILES columns: row n, columns 32 t + 8 q on of each pair of products, into LDS
@@ -474,8 +484,8 @@ __device__ __forceinline__ int part_of(const LoraArgs& g, int chunk, int* place)
 // columns side by side, so that h comes from the first-level cache but once. A wave keeps its columns of B while
 // its tiles, `per_block` in a row, have the same adapter.
 template <int KS, bool MANY>
-__global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_expand(const LoraArgs g) {
-  constexpr int TILES = KS <= 2 ? 8 : 16 / KS;
+__global__ void __launch_bounds__(256, KS == 1 ? 3 : 2) k_lora_expand(const LoraArgs g) {
+  constexpr int TILES = 8;
   __shared__ u32x4 stage[4][kRows * 4 * TILES + 4];
   const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
   int place;
@@ -567,6 +577,98 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : KS <= 4 ? 2 : 1) k_lora_exp
   }
 }
 
+// The same for more than 64 ranks: a block's waves share out the steps of 32 ranks, add up their splits and make them
+// the two fp16 once for all.
+template <int KS>
+__global__ void __launch_bounds__(256, 2) k_lora_expand_high(const LoraArgs g) {
+  constexpr int TILES = 32 / KS, MINE = KS / 4;
+  __shared__ u32x4 stage[4][kRows * 4 * TILES + 4];
+  __shared__ u32x4 pair[KS][2][64];
+  __shared__ float top[KS][kRows];
+  const int wave = uniform(threadIdx.x >> 6), lane = threadIdx.x & 63, n = lane & 15, q = lane >> 4;
+  int place;
+  const int chunks = g.chunk_end[g.n_parts - 1];
+  const int part = part_of(g, blockIdx.x % chunks, &place);
+  const int end = g.part_end[part], out = g.part_end[g.n_parts - 1];
+  const int c0 = (part ? g.part_end[part - 1] : 0) + (place * 4 + wave) * 16 * TILES;
+  const int column = c0 + 8 * (lane % (2 * TILES));
+  u32x4 bf[TILES][KS];
+  int loaded = -1;
+  const int first = blockIdx.x / chunks * g.per_block, behind = min(first + g.per_block, g.slots);
+  for (int slot = first; slot < behind; ++slot) {
+    const int* note = g.notes + (size_t)slot * kNote;
+    const int a = note[0], rank = note[1];
+    const float scale = __builtin_bit_cast(float, note[2]);
+    if ((unsigned)a >= (unsigned)g.n_adapters || rank <= 0 || rank > g.max_rank) continue;
+    f16* y[TILES / 2];
+    u32x4 old[TILES / 2];
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t) {
+      const int row = note[kRows + y_row<TILES>(t, lane)];
+      y[t] = (unsigned)row < (unsigned)g.n_rows && column < end ? g.y + (size_t)row * g.ldy + column : nullptr;
+    }
+    float h[MINE][8];
+    const f32x4* from = g.h + ((size_t)slot * g.n_parts + part) * g.steps * 128 + lane;
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[m][e] = 0.f;
+      const int s = wave + 4 * m;
+      if (s < g.steps)
+        for (int d = 0; d < g.splits; ++d) {
+          const f32x4* u = from + (size_t)d * g.slots * g.n_parts * g.steps * 128 + s * 128;
+          const f32x4 v = u[0], w = u[64];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            h[m][e] += v[e];
+            h[m][e + 4] += w[e];
+          }
+        }
+      float most = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        h[m][e] = 32 * s + 8 * q + e < rank ? h[m][e] : 0.f;
+        const float mag = __builtin_fabsf(h[m][e]);
+        most = mag < INFINITY ? __builtin_fmaxf(most, mag) : most;
+      }
+      most = __builtin_fmaxf(most, __shfl_xor(most, 16));
+      most = __builtin_fmaxf(most, __shfl_xor(most, 32));
+      if (q == 0) top[s][n] = most;
+    }
+    const bool all = all_of<TILES>(y);
+    load_y<TILES>(old, y, all);
+    if (a != loaded) {
+      loaded = a;
+      load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
+      cut_b<KS, TILES>(bf, rank, q);
+    }
+    lds_barrier();
+    float most = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) most = __builtin_fmaxf(most, top[s][n]);
+    float down;
+    const float up = power_of(most, &down);
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+      f16x8 hi, lo;
+      two_halves(h[m], down, hi, lo);
+      pair[wave + 4 * m][0][lane] = as_u4(hi);
+      pair[wave + 4 * m][1][lane] = as_u4(lo);
+    }
+    lds_barrier();
+    f16x8 hi[KS], lo[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      hi[s] = as_h8(pair[s][0][lane]);
+      lo[s] = as_h8(pair[s][1][lane]);
+    }
+    wave_sync();
+    expand_columns<KS, TILES>(bf, hi, lo, scale * up, stage[wave], n, q);
+    wave_sync();
+    add_to_y<TILES>(old, y, all, stage[wave], lane);
+  }
+}
+
 // Both products of a tile and a block's columns in one launch: every block computes the h of its part again.
 template <int TILES, int NG>
 __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g) {
@@ -638,18 +740,26 @@ __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g)
   add_to_y<TILES>(old, y, all, stage[wave], lane);
 }
 
+constexpr int kFill = 1024;  // blocks that k_lora_shrink is given if it has as many
+
 // What a call takes of the chip and the workspace, by its sizes alone.
 struct Shape {
   int groups, windows, slots, splits;
+  int at_once, turns;  // products of 16 ranks that a block of k_lora_shrink computes at a time, blocks that take turns
 };
-Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in) {
+Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in, int products) {
   Shape s;
   s.groups = n_seqs < kWindow ? n_seqs : kWindow;
   if (n_adapters < s.groups) s.groups = n_adapters;
   s.windows = (n_seqs + kWindow - 1) / kWindow;
   s.slots = n_rows / kRows + s.windows * (s.groups + 1);
-  const int most = (in + 4 * kChunk - 1) / (4 * kChunk);
-  s.splits = (512 + s.slots - 1) / s.slots;
+  s.at_once = products == 1 ? 1 : products == 3 ? 3 : 2;
+  // blocks for the products first, as long as kFill are not there, then for parts of in_features, whose sums every
+  // block of k_lora_expand has to add up
+  const int passes = (products + s.at_once - 1) / s.at_once, most = (in + 4 * kChunk - 1) / (4 * kChunk);
+  const int want = (kFill + s.slots - 1) / s.slots;
+  s.turns = want < passes ? want : passes;
+  s.splits = (kFill + s.slots * s.turns - 1) / (s.slots * s.turns);
   if (s.splits > most) s.splits = most;
   if (s.splits > 8) s.splits = 8;  // what k_lora_expand adds up
   s.splits = (most + (most + s.splits - 1) / s.splits - 1) / ((most + s.splits - 1) / s.splits);  // none idle at the end
@@ -666,7 +776,7 @@ extern "C" size_t llmk_lora_add_workspace_floats(int n_rows, int n_seqs, int n_a
   if (n_rows <= 0 || n_seqs <= 0 || n_adapters <= 0 || max_rank <= 0 || in_features <= 0 ||
       n_parts <= 0)
     return 0;
-  const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features);
+  const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features, n_parts * ((max_rank + 15) / 16));
   return (size_t)s.slots * (kNote + (size_t)s.splits * n_parts * ((max_rank + 31) / 32) * 512);
 }
 
@@ -680,7 +790,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
       n_parts < 1 || n_parts > kParts || !part_ends || (!row_starts && n_rows != n_seqs))
     return LLMK_ERR_INVALID_VALUE;
   const int steps = (max_rank + 31) / 32, ks = steps <= 2 ? steps : steps <= 4 ? 4 : 8;
-  const int columns = ks <= 2 ? 512 : 1024 / ks;  // of a block
+  const int columns = ks <= 4 ? 512 : 256;  // of a block
   LoraArgs g{};
   for (int p = 0; p < n_parts; ++p) {
     const int begin = p ? part_ends[p - 1] : 0;
@@ -699,7 +809,8 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   if (!x || !a || !b || !adapter_ids || !y || !workspace) return LLMK_ERR_INVALID_VALUE;
   if (!aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(y) || !aligned16(workspace))
     return LLMK_ERR_ALIGNMENT;
-  const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features);
+  const int per_part = (max_rank + 15) / 16;
+  const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features, n_parts * per_part);
   g.x = reinterpret_cast<const f16*>(x);
   g.a = reinterpret_cast<const f16*>(a);
   g.b = reinterpret_cast<const f16*>(b);
@@ -725,7 +836,6 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.windows = s.windows;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int chunks = g.chunk_end[n_parts - 1];
-  const int per_part = (max_rank + 15) / 16;
   // Both products in one launch, if a block's own h costs it little: 32 ranks at most, few enough numbers of A and x for
   // a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. At 16
   // ranks and 2048 columns, 4 sequences: in_features 1024 5.4 us and not 8.0 of two launches, 2048 5.8 and 8.1, 4096
@@ -755,20 +865,20 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
                   grid, threads, 0, st, g);
   }
   g.per_block = 1;
-  while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= 2048) g.per_block *= 2;
+  while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= (ks == 1 ? 2048 : 512))
+    g.per_block *= 2;
   if (!grid_takes((size_t)chunks * ceil_div(s.slots, g.per_block), 256)) return LLMK_ERR_UNSUPPORTED;
-  // products of 16 ranks at a time, and blocks for them while there are few: one tile of 3 parts of 128 ranks
-  const int all = n_parts * per_part, at_once = all == 1 ? 1 : all == 3 ? 3 : 2, passes = (all + at_once - 1) / at_once;
-  const int room = 1024 / (s.slots * s.splits);
-  g.turns = room < 1 ? 1 : room < passes ? room : passes;
-  const int status = launch(at_once == 1 ? k_lora_shrink<1> : at_once == 3 ? k_lora_shrink<3> : k_lora_shrink<2>,
-                            dim3(s.splits * s.slots * g.turns), dim3(256), 0, st, g);
+  g.turns = s.turns;
+  const int status = launch(s.at_once == 1   ? k_lora_shrink<1>
+                            : s.at_once == 3 ? k_lora_shrink<3>
+                                             : k_lora_shrink<2>,
+                            dim3(s.splits * s.slots * s.turns), dim3(256), 0, st, g);
   if (status != LLMK_OK) return status;
   const dim3 grid(chunks * ceil_div(s.slots, g.per_block));  // fits: checked in front of the first launch
   const bool many = s.splits > 2;
   return launch(ks == 1   ? (many ? k_lora_expand<1, true> : k_lora_expand<1, false>)
                 : ks == 2 ? (many ? k_lora_expand<2, true> : k_lora_expand<2, false>)
-                : ks == 4 ? (many ? k_lora_expand<4, true> : k_lora_expand<4, false>)
-                          : (many ? k_lora_expand<8, true> : k_lora_expand<8, false>),
+                : ks == 4 ? k_lora_expand_high<4>
+                          : k_lora_expand_high<8>,
                 grid, dim3(256), 0, st, g);
 }

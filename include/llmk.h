@@ -411,7 +411,7 @@ LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_lo
  * 256) and the part ends are multiples of 8; x, a, b and y are 16-byte aligned. x and y may not overlap.
  * workspace: llmk_lora_add_workspace_floats(..) floats, 16-byte aligned; calls that may overlap need
  * one each, graphs replayed one behind the other may share one. LLMK_ERR_UNSUPPORTED, before any launch, for more
- * than 2^20 rows or sequences, 2^24 in_features or 65535 * 512 columns (fewer for ranks past 64), or rows times
+ * than 2^20 rows or sequences, 2^24 in_features or 65535 * 512 columns (half for ranks past 128), or rows times
  * columns past 2^38. */
 LLMK_API size_t llmk_lora_add_workspace_floats(int n_rows, int n_seqs, int n_adapters, int max_rank,
                                                int in_features, int n_parts);
