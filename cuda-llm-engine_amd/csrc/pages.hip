@@ -110,6 +110,9 @@ struct ForkArgs {
 };
 
 constexpr int kFound = 4096;  // children whose counts of wanted pages are kept in LDS
+// Beside a first child's count of wanted pages (2^24 at most): it copies a page that others held, who may all let go.
+constexpr int kCopiesShared = 1 << 30;
+constexpr int kCopied = INT_MIN;  // holders of a page that is copied from and free behind that, while pages are given
 
 // U entries a lane, 64 apart, on their way together; behind the end, `none`.
 template <int U>
@@ -163,6 +166,7 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, int c) {
   const int need = (int)(want < a.max_pages ? want : a.max_pages);
   const int whole = len / a.page_size;
   int fresh = 0;
+  bool shared = false;
   for (int j0 = 0; j0 < a.max_pages; j0 += 64 * U) {
     int v[U], alone[U];
     load_entries<U>(row, j0, held, -1, v);
@@ -177,6 +181,7 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, int c) {
       const bool keeps = j < whole || alone[u] == 1, wants = !keeps && j < need;
       if (j < a.max_pages) a.new_tables[(size_t)c * a.max_pages + j] = keeps ? v[u] : -1;
       const uint64_t m = __builtin_amdgcn_ballot_w64(wants);
+      shared |= !elder && __builtin_amdgcn_ballot_w64(wants && j == whole && len % a.page_size) != 0;
       if (wants)
         a.columns[(size_t)c * a.max_pages + fresh + __builtin_popcountll(m & ((1ull << lane) - 1))] =
             make_int2(j, j == whole && len % a.page_size ? v[u] : -1);
@@ -184,7 +189,7 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, int c) {
     }
   }
   if (lane == 0) {
-    a.fresh[c] = fresh;
+    a.fresh[c] = fresh + (shared ? kCopiesShared : 0);
     a.new_lens[c] = len;
     a.copies[2 * c] = -1;
     a.copies[2 * c + 1] = -1;
@@ -246,13 +251,14 @@ __device__ __forceinline__ int free_bits(const ForkArgs& a, int p0) {
 }
 
 // Gives the free pages that are wanted, in order. One block of 1024 threads.
-__device__ __forceinline__ void fork_find(const ForkArgs& a, int* found_begin, int (*part)[16]) {
+__device__ __forceinline__ void fork_find(const ForkArgs& a, int* found_begin, int (*part)[16], int* marked) {
   const int* begin = a.n_new <= kFound ? found_begin : a.fresh;
+  if (threadIdx.x == 0) *marked = 0;
   int free = free_bits(a, 0);
   long long wanted = 0;
   int turn = 0;
   for (int c0 = 0; c0 < a.n_new; c0 += 1024) {
-    const int c = c0 + threadIdx.x, mine = c < a.n_new ? a.fresh[c] : 0;
+    const int c = c0 + threadIdx.x, noted = c < a.n_new ? a.fresh[c] : 0, mine = noted & (kCopiesShared - 1);
     int total;
     const int before = block_scan(mine, part[turn ^= 1], &total);
     if (c < a.n_new) {
@@ -260,9 +266,16 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, int* found_begin, i
       const int b = (int)(at < a.num_pages ? at : a.num_pages);
       if (a.n_new <= kFound) found_begin[c] = b; else a.fresh[c] = b;
     }
+    // sequences that were cut inside a page that they share: copied from, it is nobody's fresh page
+    if (noted & kCopiesShared) {
+      const int was = atomicCAS(&a.refs[a.columns[(size_t)c * a.max_pages].y], 0, kCopied);
+      if (was == 0 || was == kCopied) *marked = 1;
+    }
     wanted += total;
   }
   __syncthreads();
+  const bool some = *marked;
+  if (some) free = free_bits(a, 0);
   int found = 0;
   for (int p0 = 0; p0 < a.num_pages && found < wanted;) {
     const int next = free_bits(a, p0 + 4096);  // on its way in good time
@@ -276,6 +289,10 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, int* found_begin, i
     found += total;
     p0 += 4096;
     free = next;
+  }
+  if (some) {
+    __syncthreads();
+    for (int p = threadIdx.x; p < a.num_pages; p += 1024) atomicCAS(&a.refs[p], kCopied, 0);
   }
   if (threadIdx.x == 0) {
     const long long given = found < wanted ? found : wanted;
@@ -296,19 +313,19 @@ __global__ void __launch_bounds__(256) k_fork_refs(const ForkArgs a) {
   if (p < a.n_old) fork_refs<U>(a, p);
 }
 __global__ void __launch_bounds__(1024) k_fork_find(const ForkArgs a) {
-  __shared__ int begin[kFound], part[2][16];
-  fork_find(a, begin, part);
+  __shared__ int begin[kFound], part[2][16], marked;
+  fork_find(a, begin, part, &marked);
 }
 // The three of them by one block. Its additions to counts are complete at the barrier and read where they were
 // made, so no fence of the device is needed, which takes 5 us.
 __global__ void __launch_bounds__(1024) k_fork(const ForkArgs a) {
-  __shared__ int begin[kFound], part[2][16];
+  __shared__ int begin[kFound], part[2][16], marked;
   const int wave = threadIdx.x >> 6;
   for (int c = wave; c < a.n_new; c += 16) fork_row<1>(a, c);
   __syncthreads();
   for (int p = wave; p < a.n_old; p += 16) fork_refs<1>(a, p);
   __syncthreads();
-  fork_find(a, begin, part);
+  fork_find(a, begin, part, &marked);
 }
 
 // ---------------------------------------------------------------------------------------------

@@ -477,7 +477,7 @@ LLMK_API int llmk_compute_rotary_inv_freq(int scaling, int rotary_dim, double th
 
 /* Cache pages that sequences share, on the GPU. refs [num_pages] counts the holders of each page (0: free). A
  * sequence holds the pages that its row of a block table names, up to the first entry that is no page (negative or
- * past the pool), and its tokens fill them in order, page_size a page. Only whole pages are shared. */
+ * past the pool), and its tokens fill them in order, page_size a page. A fork shares only whole pages. */
 
 /* Copies pages within pools: pair i of copies [n_copies, 2] is (from, to); the same pairs for all n_pools pools.
  * pools and page_bytes are HOST arrays: the pools' device pointers and the bytes of a page in each (K and V of
@@ -500,7 +500,8 @@ LLMK_API int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, in
  *     else a fresh one; if it replaces the page that L ends inside, copies[c] = (parent's page, fresh page);
  *   j >= need: -1.
  * Fresh pages are the lowest-numbered ones that nobody holds once the old batch has let go and the new one has
- * taken over, in the order of (c, j); where they run out the entry is -1. new_lens [n_new] = L; copies
+ * taken over and no child copies (sequences cut inside a page that they share may), in the order of (c, j);
+ * where they run out the entry is -1. new_lens [n_new] = L; copies
  * [n_new, 2] is (-1, -1) where nothing is to be copied (llmk_kv_copy_pages does that); counts [2] = fresh pages
  * given, and lacking (the table's row of a child that lacks some is then too short for L + reserve). refs is
  * brought up to date. n_new == 0 frees the old batch. No array that is written may overlap another
@@ -517,8 +518,8 @@ LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
  * goes to the k-th free page below n. new_tables [n_seqs, max_pages] names pages by their new numbers (entries
  * that are no held page stay as they are), new_refs [num_pages] counts their holders; copies [num_pages / 2, 2]
  * gets the pairs (from, to), whose number is counts[0] (counts[1] = n), for llmk_kv_copy_pages. new_tables may be
- * block_tables, new_refs may be refs; other arrays may not overlap (LLMK_ERR_INVALID_VALUE). workspace: llmk_kv_compact_workspace_ints(num_pages) int32. num_pages up to
- * 2^24. */
+ * block_tables, new_refs may be refs; other arrays may not overlap (LLMK_ERR_INVALID_VALUE). workspace:
+ * llmk_kv_compact_workspace_ints(num_pages) int32. num_pages up to 2^24. */
 LLMK_API size_t llmk_kv_compact_workspace_ints(int num_pages);
 LLMK_API int llmk_kv_compact(const int32_t* block_tables, const int32_t* refs, int32_t* new_tables,
                              int32_t* new_refs, int32_t* copies, int32_t* counts,

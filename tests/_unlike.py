@@ -104,7 +104,8 @@ def fork(tables, lens, parents, reserve, refs, n_new, max_pages, page, num_pages
             else:
                 wanted.append((c, j, mine if j == length // page and length % page else -1))
         seen.add(p)
-    free = [p for p in range(num_pages) if refs[p] == 0]
+    copied = {mine for _, _, mine in wanted}
+    free = [p for p in range(num_pages) if refs[p] == 0 and p not in copied]
     for (c, j, mine), to in zip(wanted, free):
         new[c, j], refs[to] = to, 1
         if mine >= 0:

@@ -182,6 +182,33 @@ def test_no_pages_left(llmk):
         assert want[4][0] == gives and want[4][1] > 0
 
 
+@pytest.mark.parametrize("n,spare", [(2, 0), (2, 9), (40, 0), (40, 300), (3000, 1), (3000, 9000)])
+def test_sequences_cut_inside_a_page_that_they_share(llmk, n, spare):
+    """All let go of the page that their children copy: it is free afterwards, and no copy's destination."""
+    rng = np.random.default_rng([n, spare])
+    page, num_pages = 4, 3 * (n // 2) + spare
+    order, tables, refs = rng.permutation(num_pages), np.full((n, 5), -1), np.zeros(num_pages, np.int64)
+    for s in range(n):  # pairs share three pages, and are cut behind the first, in the second or in the third
+        tables[s, :3] = order[3 * (s // 2):3 * (s // 2) + 3]
+        refs[tables[s, :3]] += 1
+    lens = np.repeat(rng.integers(3, 12, n // 2), 2)
+    parents = rng.integers(0, n, n)
+    want = check_fork(llmk, tables, lens, parents, np.full(n, 2), refs, page, num_pages)
+    pairs = want[3][want[3][:, 0] >= 0]
+    assert not np.isin(pairs[:, 1], pairs[:, 0]).any() and len(set(pairs[:, 1])) == len(pairs)
+    assert (want[2] >= 0).all()
+    assert spare < n or len(pairs) > n // 4
+    # what the children hold is what their parents held
+    pool = torch.randint(-99, 99, (num_pages, page), dtype=torch.int32, device=DEV)
+    before = pool.cpu().numpy()
+    llmk.kv_copy_pages([pool], i32(want[3].reshape(-1)), None, n, num_pages, check_indices=True)
+    after = pool.cpu().numpy()
+    for c in range(n):
+        held = ref.held(want[0][c], num_pages)
+        tokens = min(int(lens[parents[c]]), len(held) * page)
+        assert np.array_equal(after[held].reshape(-1)[:tokens], before[tables[parents[c], :3]].reshape(-1)[:tokens])
+
+
 def test_a_search_captured_and_replayed(llmk):
     """Two graphs (the batch goes to and fro between two sets of arrays) run a search of many steps, whose
     pages hold what each beam wrote: nobody's tokens are lost or changed by others."""
