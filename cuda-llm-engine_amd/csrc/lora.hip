@@ -1,8 +1,21 @@
 // Low-rank adapters of a batch's sequences beside a shared projection:
 //   y[r, :] += scale_a B_a h, h = A_a x[r, :], a the adapter of row r's sequence.
 //
-// Two launches of matrix products, tiles of 16 rows that have the same adapter, so that its weights are
-// read once for them: k_lora_shrink finds the tiles and computes h, k_lora_expand adds B_a h to y.
+// Matrix products over tiles of 16 rows that have the same adapter, so that its weights are read once for them.
+// Bound by bytes: A and B of the adapters present, x, and y both ways; a prompt's by y. In two launches:
+// k_lora_shrink finds the tiles and computes h, k_lora_expand adds B_a h to y; or in one, k_lora_whole, where a
+// block's columns are few enough blocks that each may compute its h again.
+//
+// Measured (one MI355X, fp16, inputs from HBM; the floor is each byte once at 6 TB/s), us:
+//   1 row, rank 16, 2048 -> 2048: 5.4 (< 0.1). One launch: its loads one behind the other.
+//   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 11.3 (2.2). One launch; every block
+//     reads its tile's A and x again, from the L2: 9.6 where all of it is in the last-level cache.
+//   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 29.2 (12.6), 18 and 11. 60 MB by the first launch at 3.3
+//     TB/s: a tile's rows are found (2 us), then two rounds of loads that wait for one another.
+//   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.8 (27.7), 9 and 35. y in place by 16 rows of
+//     256 bytes a wave, which alone take 30.
+//   3 prompts of 456 rows, rank 128, 8192 -> 11008|11008: 92 (30.6), 40 and 58. A and B from the L2 by every tile, 540
+//     MB for the first; two tiles a block halve that, but also the waves a SIMD, and take as long.
 //
 // Tiles. Sequences are taken 256 at a time (a window); those of a window with the same adapter are a
 // group, in the order of their first ones, and a group's rows, in order, are cut into tiles of 16. Every
@@ -282,7 +295,8 @@ __device__ __forceinline__ void rows_of_x(const Plan& p, int (&row)[8], int lane
   }
 }
 
-// h of a tile: D[rank, row] = A[rank, k] x[row, k], by waves that take 256 of in_features at a time.
+// h of a tile: D[rank, row] = A[rank, k] x[row, k], by waves that take 256 of in_features at a time, NG products of 16
+// ranks side by side. Blocks share out a tile's products (turns) and its in_features (splits), as shape_of says.
 template <int NG>
 __global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const LoraArgs g) {
   __shared__ Plan p;
@@ -482,7 +496,8 @@ __device__ __forceinline__ int part_of(const LoraArgs& g, int chunk, int* place)
 
 // y of a tile's rows: D[column, row] = B[column, j] h[row, j]. Waves work by themselves; those of a block take
 // columns side by side, so that h comes from the first-level cache but once. A wave keeps its columns of B while
-// its tiles, `per_block` in a row, have the same adapter.
+// its tiles, `per_block` in a row, have the same adapter. MANY: more than two splits, whose sums the block's waves
+// share out.
 template <int KS, bool MANY>
 __global__ void __launch_bounds__(256, KS == 1 ? 3 : 2) k_lora_expand(const LoraArgs g) {
   constexpr int TILES = 8;
@@ -578,7 +593,8 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : 2) k_lora_expand(const Lora
 }
 
 // The same for more than 64 ranks: a block's waves share out the steps of 32 ranks, add up their splits and make them
-// the two fp16 once for all.
+// the two fp16 once for all. 3 prompts of 456 rows and rank 128 on 11008|11008 columns take 58 us, and 112 with h made
+// by every wave for itself and half the columns.
 template <int KS>
 __global__ void __launch_bounds__(256, 2) k_lora_expand_high(const LoraArgs g) {
   constexpr int TILES = 32 / KS, MINE = KS / 4;
@@ -740,7 +756,9 @@ __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g)
   add_to_y<TILES>(old, y, all, stage[wave], lane);
 }
 
-constexpr int kFill = 1024;  // blocks that k_lora_shrink is given if it has as many
+// Blocks that k_lora_shrink is given if it has as many. 512: 3 prompts of 456 rows and rank 128 on 8192 -> 11008|11008
+// take 100 us and not 92, of rank 64 on 4096 -> 4096|1024|1024 42.7 and 41; the other cases as long.
+constexpr int kFill = 1024;
 
 // What a call takes of the chip and the workspace, by its sizes alone.
 struct Shape {
@@ -762,7 +780,8 @@ Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in, int products) {
   s.splits = (kFill + s.slots * s.turns - 1) / (s.slots * s.turns);
   if (s.splits > most) s.splits = most;
   if (s.splits > 8) s.splits = 8;  // what k_lora_expand adds up
-  s.splits = (most + (most + s.splits - 1) / s.splits - 1) / ((most + s.splits - 1) / s.splits);  // none idle at the end
+  const int each = (most + s.splits - 1) / s.splits;
+  s.splits = (most + each - 1) / each;  // none idle at the end
   return s;
 }
 
@@ -836,8 +855,8 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.windows = s.windows;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int chunks = g.chunk_end[n_parts - 1];
-  // Both products in one launch, if a block's own h costs it little: 32 ranks at most, few enough numbers of A and x for
-  // a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. At 16
+  // Both products in one launch, if a block's own h costs it little: 32 ranks at most, few enough numbers of A and x
+  // for a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. At 16
   // ranks and 2048 columns, 4 sequences: in_features 1024 5.4 us and not 8.0 of two launches, 2048 5.8 and 8.1, 4096
   // 7.2 and 8.5, 6144 8.5 and 8.5, 8192 9.8 and 8.7; at 32 ranks 4096 9.0 and 9.2, 6144 10.7 and 9.3. At 16 ranks
   // and 16384 columns 2048 numbers of 128 sequences (52 MB) take 10.5 us and 11.5, 4096 of 16 (75 MB) 10.6 and 9.7, of
@@ -864,6 +883,8 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
                                                 : k_lora_whole<8, 2>),
                   grid, threads, 0, st, g);
   }
+  // as many tiles a block as leave 2048 blocks, or 512 past 32 ranks, where B is more than y: 2 prompts of 900 rows and
+  // rank 64 on 8192|8192 columns take 32 us, and 40 with 2048
   g.per_block = 1;
   while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= (ks == 1 ? 2048 : 512))
     g.per_block *= 2;
