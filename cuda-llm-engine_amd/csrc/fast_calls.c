@@ -15,8 +15,7 @@
 
 static PyObject *tensor_type, *half_dtype, *int_dtype, *float_dtype, *get_device, *get_stream,
     *e4m3_dtype;
-static PyObject *s_is_cuda, *s_dtype, *s_is_contiguous, *s_numel, *s_data_ptr, *s_get_device, *s_shape, *s_stride,
-    *s_nbytes;
+static PyObject *s_is_cuda, *s_dtype, *s_is_contiguous, *s_numel, *s_data_ptr, *s_get_device;
 
 /* The device address of t when it is a contiguous CUDA torch.Tensor of this dtype with at least
  * `least` elements; 0 otherwise, with no exception set. (A tensor of no elements has no address
@@ -92,53 +91,73 @@ static void* address_on(PyObject* t, PyObject* dtype, long long least, long long
   return p;
 }
 
-/* What a call without arguments answers, as a number; -1 and no exception where it has none. */
-static long long number_of(PyObject* t, PyObject* method) {
-  long long n = -1;
-  PyObject* v = PyObject_CallMethodNoArgs(t, method);
-  if (v) {
-    n = PyLong_AsLongLong(v);
-    Py_DECREF(v);
-  }
-  if (PyErr_Occurred()) {
+/* A tensor as DLPack describes it, and what of its exchange interface (version 1) is used here: one call of C
+ * that fills in the description, which takes 20 ns and not the 250 of five attributes, and one that gives the
+ * current stream. NULL where torch has none: no answer then. */
+typedef struct {
+  void* data;
+  struct {
+    int32_t type, id;
+  } device;
+  int32_t ndim;
+  struct {
+    uint8_t code, bits;
+    uint16_t lanes;
+  } dtype;
+  int64_t *shape, *strides;
+  uint64_t byte_offset;
+} View;
+typedef struct {
+  struct {
+    uint32_t major, minor;
+  } version;
+  void *previous, *allocate, *managed_from_object, *managed_to_object;
+  int (*view_of_object)(void* object, View* out);
+  int (*work_stream)(int32_t device_type, int32_t device, void** stream);
+} Exchange;
+enum { ROCM = 10, SIGNED = 0, FLOATING = 2 };
+static const Exchange* exchange;
+
+/* Whether t is a torch.Tensor of this device, and the description of it. */
+static int view_on(PyObject* t, long long device, View* v) {
+  if ((PyObject*)Py_TYPE(t) != tensor_type || !exchange) return 0;
+  if (exchange->view_of_object(t, v)) {
     PyErr_Clear();
-    n = -1;
+    return 0;
   }
-  return n;
+  v->data = (char*)v->data + v->byte_offset;
+  return v->device.type == ROCM && v->device.id == device && v->dtype.lanes == 1;
 }
 
-/* A tuple's number i, -1 without an exception where there is none. */
-static long long item_of(PyObject* tuple, Py_ssize_t i) {
-  const long long n = PyLong_AsLongLong(PyTuple_GET_ITEM(tuple, i));
-  if (n == -1 && PyErr_Occurred()) PyErr_Clear();
-  return n;
+/* How many elements a contiguous tensor has, -1 for another one. */
+static long long numel_of(const View* v) {
+  long long n = 1;
+  int dense = 1;
+  for (int d = v->ndim - 1; d >= 0; --d) {
+    dense &= v->shape[d] == 1 || v->strides[d] == n;
+    n *= v->shape[d];
+  }
+  return n == 0 ? 0 : dense ? n : -1;
 }
 
-/* address_on() of n >= 1 rows of `width` halves, ld apart: a matrix of at least so many rows and columns
+/* address_on() by the description. */
+static void* view_address(PyObject* t, int code, int bits, long long least, long long device, long long* numel) {
+  View v;
+  if (!view_on(t, device, &v) || v.dtype.code != code || v.dtype.bits != bits) return NULL;
+  const long long n = numel_of(&v);
+  if (numel) *numel = n;
+  return n >= least && n > 0 ? v.data : NULL;
+}
+
+/* view_address() of n >= 1 rows of `width` halves, ld apart: a matrix of at least so many rows and columns
  * whose rows are ld apart (columns of a wider one, too), or a contiguous tensor of another shape. */
 static void* rows_on(PyObject* t, long long n, long long ld, long long width, long long device) {
-  if ((PyObject*)Py_TYPE(t) != tensor_type) return NULL;
-  PyObject* shape = PyObject_GetAttr(t, s_shape);
-  if (!shape || !PyTuple_Check(shape) || PyTuple_GET_SIZE(shape) != 2) {
-    if (!shape) PyErr_Clear();
-    Py_XDECREF(shape);
-    return address_on(t, half_dtype, (n - 1) * ld + width, device, NULL);
-  }
-  const long long rows = item_of(shape, 0), columns = item_of(shape, 1);
-  Py_DECREF(shape);
-  if (rows < n || columns < width || number_of(t, s_get_device) != device || device < 0) return NULL;
-  PyObject* v = PyObject_GetAttr(t, s_dtype);
-  const int half = v == half_dtype;
-  if (!v) PyErr_Clear();
-  Py_XDECREF(v);
-  if (!half) return NULL;
-  v = PyObject_CallMethodNoArgs(t, s_stride);
-  const int fits = v && PyTuple_Check(v) && PyTuple_GET_SIZE(v) == 2 &&
-                   (rows == 1 || item_of(v, 0) == ld) && (columns == 1 || item_of(v, 1) == 1);
-  if (!v) PyErr_Clear();
-  Py_XDECREF(v);
-  const long long at = fits ? number_of(t, s_data_ptr) : 0;
-  return at > 0 ? (void*)(uintptr_t)at : NULL;
+  View v;
+  if (!view_on(t, device, &v) || v.dtype.code != FLOATING || v.dtype.bits != 16) return NULL;
+  if (v.ndim != 2) return numel_of(&v) >= (n - 1) * ld + width ? v.data : NULL;
+  const int fits = v.shape[0] >= n && v.shape[1] >= width && (v.shape[0] == 1 || v.strides[0] == ld) &&
+                   (v.shape[1] == 1 || v.strides[1] == 1);
+  return fits ? v.data : NULL;
 }
 
 /* torch's current stream for None, the number itself for a number. */
@@ -176,6 +195,21 @@ static long long device_and_stream(PyObject* o, void** stream) {
   }
   const int ok = v && !PyErr_Occurred();
   if (!ok) PyErr_Clear();
+  return ok ? at : -1;
+}
+
+/* The same by the exchange interface. */
+static long long device_and_work_stream(PyObject* o, void** stream) {
+  PyObject* dev = exchange ? PyObject_CallNoArgs(get_device) : NULL;
+  const long long at = dev ? PyLong_AsLongLong(dev) : -1;
+  Py_XDECREF(dev);
+  int ok = at >= 0;
+  if (ok && o == Py_None) ok = exchange->work_stream(ROCM, (int32_t)at, stream) == 0;
+  else if (ok && (ok = PyLong_CheckExact(o))) *stream = PyLong_AsVoidPtr(o);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    ok = 0;
+  }
   return ok ? at : -1;
 }
 
@@ -459,6 +493,28 @@ FUNCTION(verify_drafts, 14)
                             n_accepted, tokens, workspace, n_rows, n_seqs, vocab, stream));
 }
 
+/* The same for the calls that take tensors by their descriptions. */
+#define WHERE(at)                                                          \
+  void* stream;                                                            \
+  const long long here = device_and_work_stream(args[at], &stream);        \
+  if (here < 0) Py_RETURN_NONE
+#define HALVES(name, at, least)                                                                 \
+  uint16_t* name = (uint16_t*)view_address(args[at], FLOATING, 16, least, here, NULL);          \
+  if (!name) Py_RETURN_NONE
+#define INTS(name, at, least)                                                                   \
+  int32_t* name = (int32_t*)view_address(args[at], SIGNED, 32, least, here, NULL);              \
+  if (!name) Py_RETURN_NONE
+#define FLOATS(name, at, least)                                                                 \
+  float* name = (float*)view_address(args[at], FLOATING, 32, least, here, NULL);                \
+  if (!name) Py_RETURN_NONE
+#define OPT(kind, type, name, at, least)                                                        \
+  type* name = NULL;                                                                            \
+  if (args[at] != Py_None) {                                                                    \
+    kind(given, at, least);                                                                     \
+    name = given;                                                                               \
+  }
+#define OPT_INTS(name, at, least) OPT(INTS, int32_t, name, at, least)
+#define OPT_FLOATS(name, at, least) OPT(FLOATS, float, name, at, least)
 #define ROWS_ON(name, at, n, ld, width)                                 \
   uint16_t* name = (uint16_t*)rows_on(args[at], n, ld, width, here);     \
   if (!name) Py_RETURN_NONE
@@ -485,16 +541,16 @@ FUNCTION(lora_add, 18)
     Py_RETURN_NONE;
   const size_t floats = llmk_lora_add_workspace_floats(n_rows, n_seqs, n_adapters, max_rank, in, (int)n_parts);
   if (floats > (size_t)LLONG_MAX || in > 1 << 24 || out > 1 << 24) Py_RETURN_NONE;
-  HERE(17);
+  WHERE(17);
   ROWS_ON(x, 0, n_rows, ldx, in);
-  TENSOR_ON(uint16_t, a, 2, half_dtype, (long long)n_adapters * (int)n_parts * max_rank * in);
-  TENSOR_ON(uint16_t, b, 3, half_dtype, (long long)n_adapters * out * max_rank);
-  OPT_ON(int32_t, ranks, 4, int_dtype, n_adapters);
-  OPT_ON(float, scales, 5, float_dtype, n_adapters);
-  TENSOR_ON(int32_t, ids, 6, int_dtype, n_seqs);
-  OPT_ON(int32_t, starts, 7, int_dtype, n_seqs + 1LL);
+  HALVES(a, 2, (long long)n_adapters * (int)n_parts * max_rank * in);
+  HALVES(b, 3, (long long)n_adapters * out * max_rank);
+  OPT_INTS(ranks, 4, n_adapters);
+  OPT_FLOATS(scales, 5, n_adapters);
+  INTS(ids, 6, n_seqs);
+  OPT_INTS(starts, 7, n_seqs + 1LL);
   ROWS_ON(y, 8, n_rows, ldy, out);
-  TENSOR_ON(float, workspace, 11, float_dtype, (long long)floats);
+  FLOATS(workspace, 11, (long long)floats);
   ANSWER(llmk_lora_add(x, ldx, a, b, ranks, scales, ids, starts, y, ldy, ends, (int)n_parts, workspace,
                        n_rows, n_seqs, n_adapters, max_rank, in, stream));
 }
@@ -502,13 +558,13 @@ FUNCTION(lora_add, 18)
 /* The tensors of a rotation, at `at` and the three behind; n_tables is how many inv_freq holds. */
 #define TURNS(at, n)                                                                                  \
   if (!rotary || rotary % 2) Py_RETURN_NONE;                                                          \
-  TENSOR_ON(int32_t, positions, at, int_dtype, n);                                                    \
+  INTS(positions, at, n);                                                    \
   long long frequencies = 0;                                                                          \
-  float* inv_freq = (float*)address_on(args[(at) + 1], float_dtype, rotary / 2, here, &frequencies);  \
+  float* inv_freq = (float*)view_address(args[(at) + 1], FLOATING, 32, rotary / 2, here, &frequencies); \
   if (!inv_freq || frequencies / (rotary / 2) > INT_MAX) Py_RETURN_NONE;                              \
   const int n_tables = (int)(frequencies / (rotary / 2));                                             \
-  OPT_ON(int32_t, table_ids, (at) + 2, int_dtype, n);                                                 \
-  OPT_ON(float, scales, (at) + 3, float_dtype, n_tables)
+  OPT_INTS(table_ids, (at) + 2, n);                                                 \
+  OPT_FLOATS(scales, (at) + 3, n_tables)
 
 FUNCTION(rotary_apply, 15)
   COUNT(ldq, 1);
@@ -521,7 +577,7 @@ FUNCTION(rotary_apply, 15)
   COUNT(layout, 13);
   if (!n || !heads || !kv_heads || !head_dim || heads > 65535 || kv_heads > 65535 || head_dim > 65535)
     Py_RETURN_NONE;
-  HERE(14);
+  WHERE(14);
   ROWS_ON(q, 0, n, ldq, (long long)heads * head_dim);
   ROWS_ON(k, 2, n, ldk, (long long)kv_heads * head_dim);
   TURNS(4, n);
@@ -542,12 +598,12 @@ FUNCTION(qkv_rotary_scatter, 19)
   if (!n || !max_pages || !page_size || !heads || !kv_heads || !head_dim || heads > 65535 ||
       kv_heads > 65535 || head_dim > 65535)
     Py_RETURN_NONE;
-  HERE(18);
+  WHERE(18);
   ROWS_ON(qkv, 0, n, ld, (heads + 2LL * kv_heads) * head_dim);
-  TENSOR_ON(uint16_t, q_out, 2, half_dtype, (long long)n * heads * head_dim);
-  TENSOR_ON(uint16_t, k_pool, 3, half_dtype, 0);
-  TENSOR_ON(uint16_t, v_pool, 4, half_dtype, 0);
-  TENSOR_ON(int32_t, tables, 5, int_dtype, (long long)n * max_pages);
+  HALVES(q_out, 2, (long long)n * heads * head_dim);
+  HALVES(k_pool, 3, 0);
+  HALVES(v_pool, 4, 0);
+  INTS(tables, 5, (long long)n * max_pages);
   TURNS(6, n);
   ANSWER(llmk_qkv_rotary_scatter(qkv, ld, q_out, k_pool, v_pool, tables, positions, inv_freq, table_ids,
                                  scales, n, max_pages, page_size, heads, kv_heads, head_dim, rotary,
@@ -563,24 +619,17 @@ FUNCTION(kv_copy_pages, 6)
   void* pools[256];
   size_t bytes[256];
   if (n_pools > 256) Py_RETURN_NONE;
-  HERE(5);
+  WHERE(5);
   for (Py_ssize_t i = 0; i < n_pools; ++i) {
-    PyObject* t = PyList_GET_ITEM(args[0], i);
-    if ((PyObject*)Py_TYPE(t) != tensor_type || number_of(t, s_get_device) != here) Py_RETURN_NONE;
-    PyObject* v = PyObject_CallMethodNoArgs(t, s_is_contiguous);
-    const int contiguous = v == Py_True;
-    if (!v) PyErr_Clear();
-    Py_XDECREF(v);
-    v = PyObject_GetAttr(t, s_nbytes);
-    const long long size = v ? PyLong_AsLongLong(v) : -1, at = number_of(t, s_data_ptr);
-    if (!v || PyErr_Occurred()) PyErr_Clear();
-    Py_XDECREF(v);
-    if (!contiguous || size <= 0 || at <= 0 || size % num_pages) Py_RETURN_NONE;
-    pools[i] = (void*)(uintptr_t)at;
+    View v;
+    if (!view_on(PyList_GET_ITEM(args[0], i), here, &v) || v.dtype.bits % 8) Py_RETURN_NONE;
+    const long long size = numel_of(&v) * (v.dtype.bits / 8);
+    if (size <= 0 || size % num_pages) Py_RETURN_NONE;
+    pools[i] = v.data;
     bytes[i] = (size_t)(size / num_pages);
   }
-  TENSOR_ON(int32_t, copies, 1, int_dtype, 2LL * n_copies);
-  OPT_ON(int32_t, count, 2, int_dtype, 1);
+  INTS(copies, 1, 2LL * n_copies);
+  OPT_INTS(count, 2, 1);
   ANSWER(llmk_kv_copy_pages(pools, bytes, (int)n_pools, copies, count, n_copies, num_pages, stream));
 }
 
@@ -591,17 +640,17 @@ FUNCTION(kv_fork, 16)
   COUNT(page_size, 13);
   COUNT(num_pages, 14);
   if (!n_old || !n_new || !max_pages || !num_pages) Py_RETURN_NONE;
-  HERE(15);
-  TENSOR_ON(int32_t, tables, 0, int_dtype, (long long)n_old * max_pages);
-  TENSOR_ON(int32_t, lens, 1, int_dtype, n_old);
-  TENSOR_ON(int32_t, parents, 2, int_dtype, n_new);
-  OPT_ON(int32_t, reserve, 3, int_dtype, n_new);
-  TENSOR_ON(int32_t, refs, 4, int_dtype, num_pages);
-  TENSOR_ON(int32_t, new_tables, 5, int_dtype, (long long)n_new * max_pages);
-  TENSOR_ON(int32_t, new_lens, 6, int_dtype, n_new);
-  TENSOR_ON(int32_t, copies, 7, int_dtype, 2LL * n_new);
-  TENSOR_ON(int32_t, counts, 8, int_dtype, 2);
-  TENSOR_ON(int32_t, workspace, 9, int_dtype,
+  WHERE(15);
+  INTS(tables, 0, (long long)n_old * max_pages);
+  INTS(lens, 1, n_old);
+  INTS(parents, 2, n_new);
+  OPT_INTS(reserve, 3, n_new);
+  INTS(refs, 4, num_pages);
+  INTS(new_tables, 5, (long long)n_new * max_pages);
+  INTS(new_lens, 6, n_new);
+  INTS(copies, 7, 2LL * n_new);
+  INTS(counts, 8, 2);
+  INTS(workspace, 9,
             (long long)llmk_kv_fork_workspace_ints(n_old, n_new, max_pages, num_pages));
   ANSWER(llmk_kv_fork(tables, lens, parents, reserve, refs, new_tables, new_lens, copies, counts,
                       workspace, n_old, n_new, max_pages, page_size, num_pages, stream));
@@ -612,14 +661,14 @@ FUNCTION(kv_compact, 11)
   COUNT(max_pages, 8);
   COUNT(num_pages, 9);
   if (!n_seqs || !max_pages || num_pages < 2) Py_RETURN_NONE;
-  HERE(10);
-  TENSOR_ON(int32_t, tables, 0, int_dtype, (long long)n_seqs * max_pages);
-  TENSOR_ON(int32_t, refs, 1, int_dtype, num_pages);
-  TENSOR_ON(int32_t, new_tables, 2, int_dtype, (long long)n_seqs * max_pages);
-  TENSOR_ON(int32_t, new_refs, 3, int_dtype, num_pages);
-  TENSOR_ON(int32_t, copies, 4, int_dtype, 2LL * (num_pages / 2));
-  TENSOR_ON(int32_t, counts, 5, int_dtype, 2);
-  TENSOR_ON(int32_t, workspace, 6, int_dtype, (long long)llmk_kv_compact_workspace_ints(num_pages));
+  WHERE(10);
+  INTS(tables, 0, (long long)n_seqs * max_pages);
+  INTS(refs, 1, num_pages);
+  INTS(new_tables, 2, (long long)n_seqs * max_pages);
+  INTS(new_refs, 3, num_pages);
+  INTS(copies, 4, 2LL * (num_pages / 2));
+  INTS(counts, 5, 2);
+  INTS(workspace, 6, (long long)llmk_kv_compact_workspace_ints(num_pages));
   ANSWER(llmk_kv_compact(tables, refs, new_tables, new_refs, copies, counts, workspace, n_seqs, max_pages,
                          num_pages, stream));
 }
@@ -639,6 +688,11 @@ static PyObject* setup(PyObject* self, PyObject* args) {
     *to[i] = Py_NewRef(from[i]);
     Py_XDECREF(old);
   }
+  PyObject* api = PyObject_GetAttrString(tensor_type, "__dlpack_c_exchange_api__");
+  exchange = api ? (const Exchange*)PyCapsule_GetPointer(api, "dlpack_exchange_api") : NULL;
+  Py_XDECREF(api);  /* what it points to stays as long as the process */
+  if (PyErr_Occurred()) PyErr_Clear();
+  if (exchange && exchange->version.major != 1) exchange = NULL;
   Py_RETURN_NONE;
 }
 
@@ -674,10 +728,7 @@ PyMODINIT_FUNC PyInit__fast_calls(void) {
       !(s_is_contiguous = PyUnicode_InternFromString("is_contiguous")) ||
       !(s_numel = PyUnicode_InternFromString("numel")) ||
       !(s_data_ptr = PyUnicode_InternFromString("data_ptr")) ||
-      !(s_get_device = PyUnicode_InternFromString("get_device")) ||
-      !(s_shape = PyUnicode_InternFromString("shape")) ||
-      !(s_stride = PyUnicode_InternFromString("stride")) ||
-      !(s_nbytes = PyUnicode_InternFromString("nbytes")))
+      !(s_get_device = PyUnicode_InternFromString("get_device")))
     return NULL;
   return PyModule_Create(&module);
 }
