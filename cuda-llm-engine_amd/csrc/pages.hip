@@ -118,23 +118,27 @@ constexpr int kFound = 4096;  // children whose counts of wanted pages are kept 
 constexpr int kCopiesShared = 1 << 30;
 constexpr int kCopied = INT_MIN;  // holders of a page that is copied from and free behind that, while pages are given
 
-// U entries a lane, 64 apart, on their way together; behind the end, `none`.
+// U entries a lane, 64 apart, on their way together; behind the end, which is past `at`, `none`.
 template <int U>
 __device__ __forceinline__ void load_entries(const int* from, int at, int end, int none, int (&v)[U]) {
   const int lane = threadIdx.x & 63;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int i = at + 64 * u + lane;
-    v[u] = i < end ? from[i] : none;
-  }
+  for (int u = 0; u < U; ++u) v[u] = from[min(at + 64 * u + lane, end - 1)];
+#pragma unroll
+  for (int u = 0; u < U; ++u) v[u] = at + 64 * u + lane < end ? v[u] : none;
 }
 
-// How many pages the old row holds. A wave's work; all lanes get it.
+// How many pages the old row holds, whose first entries are v. A wave's work; all lanes get it.
 template <int U>
-__device__ __forceinline__ int held_pages(const int* row, int max_pages, int num_pages) {
+__device__ __forceinline__ int held_pages(const int* row, int max_pages, int num_pages, const int (&first)[U]) {
   for (int j = 0; j < max_pages; j += 64 * U) {
     int v[U];
-    load_entries<U>(row, j, max_pages, -1, v);
+    if (j == 0) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[u] = first[u];
+    } else {
+      load_entries<U>(row, j, max_pages, -1, v);
+    }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const uint64_t m = __builtin_amdgcn_ballot_w64((unsigned)v[u] >= (unsigned)num_pages);
@@ -144,28 +148,38 @@ __device__ __forceinline__ int held_pages(const int* row, int max_pages, int num
   return max_pages;
 }
 
-__device__ __forceinline__ int length_of(const ForkArgs& a, int parent, int held) {
+// A sequence's length, of which its pages hold at most so much.
+__device__ __forceinline__ int length_of(const ForkArgs& a, int len, int held) {
   const long long most = (long long)held * a.page_size;
-  const int len = a.lens[parent];
   return len < 0 ? 0 : (int)(len < most ? len : most);
 }
 
+constexpr int kParents = 4;  // entries of `parents` that a lane has on their way: 256 a wave
+
 // A child's row, with what it keeps, and which columns want fresh pages. Reads counts, changes none. A wave's work.
+// What is known where to find is loaded first: the parent, then its row, its length and the other parents.
 template <int U>
 __device__ __forceinline__ void fork_row(const ForkArgs& a, int c) {
   const int lane = threadIdx.x & 63, p = a.parents[c];
-  const bool has = (unsigned)p < (unsigned)a.n_old;
-  uint64_t elder = 0;
-  for (int i = 0; i < c && !elder; i += 64 * U) {
-    int v[U];
-    load_entries<U>(a.parents, i, c, ~p, v);
-#pragma unroll
-    for (int u = 0; u < U; ++u) elder |= __builtin_amdgcn_ballot_w64(v[u] == p);
-  }
-  const int* row = a.tables + (size_t)(has ? p : 0) * a.max_pages;
-  const int held = has ? held_pages<U>(row, a.max_pages, a.num_pages) : 0;
-  const int len = has ? length_of(a, p, held) : 0;
   const int room = a.reserve ? max(a.reserve[c], 0) : 0;
+  const bool has = (unsigned)p < (unsigned)a.n_old;
+  const int* row = a.tables + (size_t)(has ? p : 0) * a.max_pages;
+  int first[U], raw = 0;
+#pragma unroll
+  for (int u = 0; u < U; ++u) first[u] = -1;
+  if (has) {
+    raw = a.lens[p];
+    load_entries<U>(row, 0, a.max_pages, -1, first);
+  }
+  uint64_t elder = 0;
+  for (int i = 0; i < c && !elder; i += 64 * kParents) {
+    int v[kParents];
+    load_entries<kParents>(a.parents, i, c, ~p, v);
+#pragma unroll
+    for (int u = 0; u < kParents; ++u) elder |= __builtin_amdgcn_ballot_w64(v[u] == p);
+  }
+  const int held = has ? held_pages<U>(row, a.max_pages, a.num_pages, first) : 0;
+  const int len = length_of(a, raw, held);
   const long long want = ((long long)len + room + a.page_size - 1) / a.page_size;
   const int need = (int)(want < a.max_pages ? want : a.max_pages);
   const int whole = len / a.page_size;
@@ -173,10 +187,13 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, int c) {
   bool shared = false;
   for (int j0 = 0; j0 < a.max_pages; j0 += 64 * U) {
     int v[U], alone[U];
-    load_entries<U>(row, j0, held, -1, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = first[u];
+    if (j0 > 0 && j0 < held) load_entries<U>(row, j0, held, -1, v);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int j = j0 + 64 * u + lane;
+      v[u] = j < held ? v[u] : -1;
       alone[u] = !elder && j >= whole && j < held && j < need ? a.refs[v[u]] : 0;
     }
 #pragma unroll
@@ -205,19 +222,22 @@ template <int U>
 __device__ __forceinline__ void fork_refs(const ForkArgs& a, int p) {
   const int lane = threadIdx.x & 63;
   const int* row = a.tables + (size_t)p * a.max_pages;
-  const int held = held_pages<U>(row, a.max_pages, a.num_pages);
+  int start[U];
+  load_entries<U>(row, 0, a.max_pages, -1, start);
+  const int raw = a.lens[p];
   int children = 0, first = -1;
-  for (int i = 0; i < a.n_new; i += 64 * U) {
-    int v[U];
-    load_entries<U>(a.parents, i, a.n_new, -1, v);
+  for (int i = 0; i < a.n_new; i += 64 * kParents) {
+    int v[kParents];
+    load_entries<kParents>(a.parents, i, a.n_new, -1, v);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
+    for (int u = 0; u < kParents; ++u) {
       const uint64_t m = __builtin_amdgcn_ballot_w64(v[u] == p);
       if (m && first < 0) first = i + 64 * u + __builtin_ctzll(m);
       children += __builtin_popcountll(m);
     }
   }
-  const int whole = length_of(a, p, held) / a.page_size;
+  const int held = held_pages<U>(row, a.max_pages, a.num_pages, start);
+  const int whole = length_of(a, raw, held) / a.page_size;
   // whole pages of an only child stay as they are
   for (int j = (children == 1 ? whole : 0) + lane; j < held; j += 64) {
     const int takes = j < whole ? children
@@ -226,14 +246,29 @@ __device__ __forceinline__ void fork_refs(const ForkArgs& a, int p) {
   }
 }
 
+struct Find {  // in LDS
+  int begin[kFound];   // of each child's wanted pages among all,
+  int child[kFound];   // and, where no child wants two, whose the k-th is, and its column
+  int2 column[kFound];
+  int part[2][16];
+  int marked, listed;
+};
+
 // The k-th wanted page: child c's, which is the last whose wanted ones begin at or before k.
-__device__ __forceinline__ void fork_give(const ForkArgs& a, const int* begin, int k, int page) {
+__device__ __forceinline__ void fork_give(const ForkArgs& a, const Find& f, bool listed, const int* begin, int k,
+                                          int page) {
   int c = 0;
-  for (int hi = a.n_new; hi - c > 1;) {
-    const int mid = (c + hi) / 2;
-    if (begin[mid] <= k) c = mid; else hi = mid;
+  int2 column;
+  if (listed) {
+    c = f.child[k];
+    column = f.column[k];
+  } else {
+    for (int hi = a.n_new; hi - c > 1;) {
+      const int mid = (c + hi) / 2;
+      if (begin[mid] <= k) c = mid; else hi = mid;
+    }
+    column = a.columns[(size_t)c * a.max_pages + (k - begin[c])];
   }
-  const int2 column = a.columns[(size_t)c * a.max_pages + (k - begin[c])];
   a.new_tables[(size_t)c * a.max_pages + column.x] = page;
   if (column.y >= 0) {
     a.copies[2 * c] = column.y;
@@ -255,40 +290,49 @@ __device__ __forceinline__ int free_bits(const ForkArgs& a, int p0) {
 }
 
 // Gives the free pages that are wanted, in order. One block of 1024 threads.
-__device__ __forceinline__ void fork_find(const ForkArgs& a, int* found_begin, int (*part)[16], int* marked) {
-  const int* begin = a.n_new <= kFound ? found_begin : a.fresh;
-  if (threadIdx.x == 0) *marked = 0;
+__device__ __forceinline__ void fork_find(const ForkArgs& a, Find& f) {
+  const int* begin = a.n_new <= kFound ? f.begin : a.fresh;
+  if (threadIdx.x == 0) {
+    f.marked = 0;
+    f.listed = a.n_new <= kFound;
+  }
   int free = free_bits(a, 0);
   long long wanted = 0;
   int turn = 0;
   for (int c0 = 0; c0 < a.n_new; c0 += 1024) {
     const int c = c0 + threadIdx.x, noted = c < a.n_new ? a.fresh[c] : 0, mine = noted & (kCopiesShared - 1);
+    const int2 column = c < a.n_new ? a.columns[(size_t)c * a.max_pages] : make_int2(0, 0);  // if there is one
     int total;
-    const int before = block_scan(mine, part[turn ^= 1], &total);
+    const int before = block_scan(mine, f.part[turn ^= 1], &total);
     if (c < a.n_new) {
       const long long at = wanted + before;
       const int b = (int)(at < a.num_pages ? at : a.num_pages);
-      if (a.n_new <= kFound) found_begin[c] = b; else a.fresh[c] = b;
+      if (a.n_new <= kFound) f.begin[c] = b; else a.fresh[c] = b;
+      if (mine == 1 && at < kFound) {  // it is if no child wants two
+        f.child[at] = c;
+        f.column[at] = column;
+      }
+      if (mine > 1) f.listed = 0;
     }
     // sequences that were cut inside a page that they share: copied from, it is nobody's fresh page
     if (noted & kCopiesShared) {
-      const int was = atomicCAS(&a.refs[a.columns[(size_t)c * a.max_pages].y], 0, kCopied);
-      if (was == 0 || was == kCopied) *marked = 1;
+      const int was = atomicCAS(&a.refs[column.y], 0, kCopied);
+      if (was == 0 || was == kCopied) f.marked = 1;
     }
     wanted += total;
   }
   __syncthreads();
-  const bool some = *marked;
+  const bool some = f.marked, listed = f.listed;
   if (some) free = free_bits(a, 0);
   int found = 0;
   for (int p0 = 0; p0 < a.num_pages && found < wanted;) {
     const int next = free_bits(a, p0 + 4096);  // on its way in good time
     int total;
-    int at = found + block_scan(__builtin_popcount(free), part[turn ^= 1], &total);
+    int at = found + block_scan(__builtin_popcount(free), f.part[turn ^= 1], &total);
     for (; free && at < wanted; free &= free - 1, ++at) {
       const int page = p0 + 4 * threadIdx.x + __builtin_ctz(free);
       a.refs[page] = 1;
-      fork_give(a, begin, at, page);
+      fork_give(a, f, listed, begin, at, page);
     }
     found += total;
     p0 += 4096;
@@ -317,19 +361,19 @@ __global__ void __launch_bounds__(256) k_fork_refs(const ForkArgs a) {
   if (p < a.n_old) fork_refs<U>(a, p);
 }
 __global__ void __launch_bounds__(1024) k_fork_find(const ForkArgs a) {
-  __shared__ int begin[kFound], part[2][16], marked;
-  fork_find(a, begin, part, &marked);
+  __shared__ Find f;
+  fork_find(a, f);
 }
 // The three of them by one block. Its additions to counts are complete at the barrier and read where they were
 // made, so no fence of the device is needed, which takes 5 us.
 __global__ void __launch_bounds__(1024) k_fork(const ForkArgs a) {
-  __shared__ int begin[kFound], part[2][16], marked;
+  __shared__ Find f;
   const int wave = threadIdx.x >> 6;
   for (int c = wave; c < a.n_new; c += 16) fork_row<1>(a, c);
   __syncthreads();
   for (int p = wave; p < a.n_old; p += 16) fork_refs<1>(a, p);
   __syncthreads();
-  fork_find(a, begin, part, &marked);
+  fork_find(a, f);
 }
 
 // ---------------------------------------------------------------------------------------------
