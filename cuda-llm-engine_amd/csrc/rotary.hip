@@ -83,15 +83,15 @@ __device__ __forceinline__ void turn(f16x8& x, f16x8& y, const float2* lo, const
   }
 }
 
-// A unit a thread. What the turns are made of is loaded first, then the data: the turns are computed while that
+// U units a thread. What the turns are made of is loaded first, then the data: the turns are computed while that
 // is on its way, and it is turned and stored behind the barrier.
-template <bool PAIRS, bool SCATTER>
+template <bool PAIRS, bool SCATTER, int U>
 __global__ void __launch_bounds__(512) k_rotary(const RotaryArgs a) {
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   float2* turns = reinterpret_cast<float2*>(smem);  // [row][pair]
   const int tid = threadIdx.x, threads = blockDim.x, half = a.rotary_dim / 2, R = a.rotary_dim / 16;
   const int group = blockIdx.x / a.chunks, row0 = group * a.rows, rows = min(a.rows, a.n_rows - row0);
-  const int unit = (blockIdx.x - group * a.chunks) * threads + tid;
+  const int unit0 = (blockIdx.x - group * a.chunks) * threads * U + tid;
   long long* pool_row = reinterpret_cast<long long*>(turns + (size_t)a.rows * half);
   const int n_turns = rows * half;
   Angle angle;
@@ -101,19 +101,27 @@ __global__ void __launch_bounds__(512) k_rotary(const RotaryArgs a) {
   }
   if (SCATTER && tid < rows) pool_row[tid] = pool_row_of(a, row0 + tid);
   // a head's units: R that turn and, where rows move, those behind them; v's heads move whole
-  const int r = (int)fdiv(unit, a.by_row), rest = unit - r * a.per_row;
-  const int head = (int)fdiv(rest, a.by_unit), u = rest - head * (int)a.by_unit.d;
-  const int kv = head - a.n_heads, vv = kv - a.n_kv_heads;
-  const bool moves = SCATTER && (u >= R || vv >= 0);
-  const int i = moves ? 2 * u : u, j = moves ? 2 * u + 1 : u + R;
-  f16x8 x, y;
-  if (r < rows) {
-    const size_t row = row0 + r;
-    const f16* src = kv < 0               ? a.q + row * a.ldq + (size_t)head * a.head_dim
-                     : SCATTER && vv >= 0 ? a.v + row * a.ldk + (size_t)vv * a.head_dim
-                                          : a.k + row * a.ldk + (size_t)kv * a.head_dim;
-    x = as_h8(ld16_stream(src + 8 * i));
-    y = as_h8(ld16_stream(src + 8 * j));
+  int r[U], head[U], i[U], j[U];
+  bool moves[U];
+  f16x8 x[U], y[U];
+#pragma unroll
+  for (int m = 0; m < U; ++m) {
+    const int unit = unit0 + m * threads;
+    r[m] = (int)fdiv(unit, a.by_row);
+    const int rest = unit - r[m] * a.per_row;
+    head[m] = (int)fdiv(rest, a.by_unit);
+    const int u = rest - head[m] * (int)a.by_unit.d, kv = head[m] - a.n_heads, vv = kv - a.n_kv_heads;
+    moves[m] = SCATTER && (u >= R || vv >= 0);
+    i[m] = moves[m] ? 2 * u : u;
+    j[m] = moves[m] ? 2 * u + 1 : u + R;
+    if (r[m] < rows) {
+      const size_t row = row0 + r[m];
+      const f16* src = kv < 0               ? a.q + row * a.ldq + (size_t)head[m] * a.head_dim
+                       : SCATTER && vv >= 0 ? a.v + row * a.ldk + (size_t)vv * a.head_dim
+                                            : a.k + row * a.ldk + (size_t)kv * a.head_dim;
+      x[m] = as_h8(ld16_stream(src + 8 * i[m]));
+      y[m] = as_h8(ld16_stream(src + 8 * j[m]));
+    }
   }
   if (tid < n_turns) turns[tid] = turn_of(angle);
   for (int e = tid + threads; e < n_turns; e += threads) {
@@ -121,19 +129,23 @@ __global__ void __launch_bounds__(512) k_rotary(const RotaryArgs a) {
     turns[e] = turn_of(angle_of(a, row0 + q, e - q * half));
   }
   lds_barrier();
-  if (r >= rows) return;
-  const long long to = SCATTER && kv >= 0 ? pool_row[r] : (long long)(row0 + r);
-  if (to < 0) return;
-  f16* dst = kv < 0               ? a.q_out + to * a.ldq_out + (size_t)head * a.head_dim
-             : SCATTER && vv >= 0 ? a.v_out + to * a.ldk_out + (size_t)vv * a.head_dim
-                                  : a.k_out + to * a.ldk_out + (size_t)kv * a.head_dim;
-  if (!moves) {
-    const float2* t = turns + (size_t)r * half;
-    if (PAIRS) turn<true>(x, y, t + 4 * i, t + 4 * j);
-    else turn<false>(x, y, t + 8 * i, nullptr);
+#pragma unroll
+  for (int m = 0; m < U; ++m) {
+    if (r[m] >= rows) return;
+    const int kv = head[m] - a.n_heads, vv = kv - a.n_kv_heads;
+    const long long to = SCATTER && kv >= 0 ? pool_row[r[m]] : (long long)(row0 + r[m]);
+    if (to < 0) continue;
+    f16* dst = kv < 0               ? a.q_out + to * a.ldq_out + (size_t)head[m] * a.head_dim
+               : SCATTER && vv >= 0 ? a.v_out + to * a.ldk_out + (size_t)vv * a.head_dim
+                                    : a.k_out + to * a.ldk_out + (size_t)kv * a.head_dim;
+    if (!moves[m]) {
+      const float2* t = turns + (size_t)r[m] * half;
+      if (PAIRS) turn<true>(x[m], y[m], t + 4 * i[m], t + 4 * j[m]);
+      else turn<false>(x[m], y[m], t + 8 * i[m], nullptr);
+    }
+    st16_stream(dst + 8 * i[m], as_u4(x[m]));
+    st16_stream(dst + 8 * j[m], as_u4(y[m]));
   }
-  st16_stream(dst + 8 * i, as_u4(x));
-  st16_stream(dst + 8 * j, as_u4(y));
 }
 
 // Any sizes, strides and alignment, in place: a pair for each thread and step.
@@ -177,21 +189,31 @@ int launch_rotary(RotaryArgs& a, int heads, int units, bool pairs, hipStream_t s
   // as many rows as 256 threads take (at most 8, whose page numbers and angles they load); a wide row by blocks
   // of up to 512. Four units a thread, and rows to match, took 9.5 us and not 10.4 for 4000 rows of 40 heads of 64,
   // but 20.4 and not 18.2 for 8000, 5.2 and not 4.4 for 1000, 4.2 and not 2.7 for 256.
-  a.rows = 256 / a.per_row;
-  a.rows = a.rows < 1 ? 1 : a.rows > 8 ? 8 : a.rows;
-  while (a.rows > 1 && (size_t)a.rows * half * 8 > 32768) --a.rows;
-  if (a.rows > a.n_rows) a.rows = a.n_rows;
+  const auto rows_of = [&](int units_of_block) {
+    int rows = units_of_block / a.per_row;
+    rows = rows < 1 ? 1 : rows > 8 ? 8 : rows;
+    while (rows > 1 && (size_t)rows * half * 8 > 32768) --rows;
+    return rows > a.n_rows ? a.n_rows : rows;
+  };
+  // Three units a thread on the way into the cache where one would be 1.2 to 3 rounds of all the card's waves: 2000
+  // rows of 36 heads of 128 take 10.2 us and not 11.1, 3000 13.6 and not 15.3, 3000 rows of 48 heads of 64 10.3 and
+  // 11.1; but 1500 of these 7.4 and not 6.8, 8000 rows of 10 heads of 256 20.9 and 18.8, 1000 rows in place 4.2 and 3.6.
+  const long long all = (long long)a.n_rows * a.per_row;
+  const int many = SCATTER && all >= 400000 && all < 1000000 ? 3 : 1;
+  a.rows = rows_of(256 * many);
   const int units_all = a.rows * a.per_row;
-  a.chunks = (int)ceil_div(units_all, 512);
-  const int threads = (int)ceil_div(ceil_div(units_all, a.chunks), 64) * 64;
+  a.chunks = (int)ceil_div(units_all, 512 * many);
+  const int threads = (int)ceil_div(ceil_div(ceil_div(units_all, a.chunks), many), 64) * 64;
   a.by_row = make_fastdiv((uint32_t)a.per_row);
   a.by_unit = make_fastdiv((uint32_t)units);
   a.by_half = make_fastdiv((uint32_t)half);
   const size_t blocks = (size_t)ceil_div((size_t)a.n_rows, (size_t)a.rows) * a.chunks;
   if (!grid_takes(blocks, 256)) return LLMK_ERR_UNSUPPORTED;
   const size_t lds = (size_t)a.rows * (half * 8 + (SCATTER ? 8 : 0));
-  return launch(pairs ? k_rotary<true, SCATTER> : k_rotary<false, SCATTER>, dim3((unsigned)blocks),
-                dim3(threads), lds, stream, a);
+  const dim3 grid((unsigned)blocks), block(threads);
+  if (SCATTER && many == 3)
+    return launch(pairs ? k_rotary<true, true, 3> : k_rotary<false, true, 3>, grid, block, lds, stream, a);
+  return launch(pairs ? k_rotary<true, SCATTER, 1> : k_rotary<false, SCATTER, 1>, grid, block, lds, stream, a);
 }
 
 int check_turn(const float* inv_freq, const int32_t* positions, int rotary_dim, int n_tables, int layout) {

@@ -136,6 +136,14 @@ def test_scatter(llmk, pairs, n, heads, kv, dim, rotary, page, max_pages):
             assert (pool.view(np.uint16)[left] == 0x7F7F).all(), "another row of the pool was written"
 
 
+@pytest.mark.parametrize("pairs", [False, True])
+@pytest.mark.parametrize("n,heads,kv,dim,rotary", [
+    (1601, 28, 4, 128, 64), (2600, 8, 1, 256, 256), (401, 60, 2, 256, 96), (221, 118, 1, 256, 16),
+    (22300, 1, 1, 96, 96), (7001, 2, 1, 240, 16)])
+def test_scatter_of_long_prompts(llmk, pairs, n, heads, kv, dim, rotary):
+    test_scatter(llmk, pairs, n, heads, kv, dim, rotary, 16, 1)
+
+
 def test_numbers_that_are_none(llmk):
     """Infinities and NaN reach their partner and nothing else."""
     rng = np.random.default_rng(5)
