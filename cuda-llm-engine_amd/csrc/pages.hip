@@ -25,7 +25,8 @@ struct CopyArgs {
   int first[kPools + 1];  // of each pool's pieces among a pair's
   const int *copies, *count;
   int n_pools, n_small, small, n_copies, num_pages, slices;
-  int each;  // pieces of every pool's page, 0 if they differ
+  int each;    // pieces of every pool's page, 0 if they differ
+  int across;  // whether blocks side by side are of other pairs, and not of other pieces
 };
 
 // A block for each pair and four of its pieces; pairs that are none are behind one load. Pages of few
@@ -33,10 +34,11 @@ struct CopyArgs {
 template <bool VECTORS>
 __global__ void __launch_bounds__(256) k_copy_pages(const CopyArgs a) {
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int pair = blockIdx.x / a.slices;
+  const int group = a.across ? a.n_copies : a.slices, far = blockIdx.x / group, near = blockIdx.x - far * group;
+  const int pair = a.across ? near : far, slice = a.across ? far : near;
   if (a.count && pair >= *a.count) return;
   const int from = a.copies[2 * (size_t)pair], to = a.copies[2 * (size_t)pair + 1];
-  int piece = (blockIdx.x - pair * a.slices) * 4 + wave;
+  int piece = slice * 4 + wave;
   const int pieces = a.first[a.n_pools];
   if (piece < pieces) {
     int lo = 0;
@@ -538,6 +540,10 @@ extern "C" int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, 
     if (page_bytes[i] > ((size_t)1 << 32)) return LLMK_ERR_UNSUPPORTED;
   }
   const auto whole = [&](int p) { return aligned16(pools[p]) && page_bytes[p] % 16 == 0; };
+  // Many pairs are walked pool by pool, in whose order a compaction's lie in memory: 1024 pairs of 16 KB in 32 pools take
+  // 178 us and not 195 in order, 202 and not 214 at random; but 128 pairs in 4 pools 4.9 and not 4.5, 32 pairs of 8 KB
+  // in 32 pools 5.5 and not 3.4.
+  const bool across = n_copies >= 512;
   // small pages of whole vectors, all of one size, go together
   size_t small = 0;
   for (int p = 0; p < n_pools && !small; ++p)
@@ -549,6 +555,7 @@ extern "C" int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, 
       a.count = count;
       a.n_copies = n_copies;
       a.num_pages = num_pages;
+      a.across = across;
       int taken = 0;
       const int begin = i;
       for (; i < n_pools && taken < kPools; ++i) taken += whole(i) == (kind == 0);

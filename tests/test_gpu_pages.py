@@ -56,6 +56,12 @@ def test_copies(llmk, sizes, n):
             assert torch.equal(p, want)
 
 
+@pytest.mark.parametrize("sizes", [(16384,), (32, 4100, 4096, 32, 16), (20,) * 3])
+@pytest.mark.parametrize("n", [511, 512, 1300])
+def test_many_copies(llmk, sizes, n):
+    test_copies(llmk, sizes, n)
+
+
 def test_copies_of_any_type_and_address(llmk):
     """Pools of other types, and one that begins between 16-byte addresses."""
     flat = torch.arange(4096, device=DEV, dtype=torch.int32)
