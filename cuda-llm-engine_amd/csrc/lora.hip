@@ -7,9 +7,9 @@
 // block's columns are few enough blocks that each may compute its h again.
 //
 // Measured (one MI355X, fp16, inputs from HBM; the floor is each byte once at 6 TB/s), us:
-//   1 row, rank 16, 2048 -> 2048: 5.4 (< 0.1). One launch: its loads one behind the other.
-//   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 11.3 (2.2). One launch; every block
-//     reads its tile's A and x again, from the L2: 9.6 where all of it is in the last-level cache.
+//   1 row, rank 16, 2048 -> 2048: 5.1 (< 0.1). One launch: its loads one behind the other.
+//   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 11.2 (2.2). One launch; every block
+//     reads its tile's A and x again, from the L2: 9.5 where all of it is in the last-level cache.
 //   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 29.2 (12.6), 18 and 11. 60 MB by the first launch at 3.3
 //     TB/s: a tile's rows are found (2 us), then two rounds of loads that wait for one another.
 //   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.8 (27.7), 9 and 35. y in place by 16 rows of
@@ -244,16 +244,20 @@ __device__ __forceinline__ void get_rows(const u32x4* from, u32x4 (&v)[8], int n
 // 32). Loaded as these want them, 64 bytes of 16 rows an instruction, they take three times as long: 8000
 // cycles for 32 instructions of four waves from the L2, not 2400. x: the lane's rows; w: of the lane's first row,
 // `rows` behind it clamped. Products `most` and behind are none.
-template <int NG>
+// SOME: of x only the rows that there are, n_x instructions' worth or up to as many again; the others' numbers are what
+// LDS holds, and give what nobody reads.
+template <int NG, bool SOME>
 __device__ __forceinline__ void shrink_chunks(f32x4 (&acc)[NG], const LoraArgs& g, const int (&row)[8],
                                               const f16* const (&w)[NG], const int (&left)[NG], int most,
-                                              int chunk, int step, u32x4* stage, int lane) {
+                                              int chunk, int step, u32x4* stage, int lane, int n_x = 8) {
   const int n = lane & 15, q = lane >> 4, r = lane >> 5, at = 8 * (lane & 31), in = g.in;
+  const auto there = [&](int t) { return !SOME || t == 0 || n_x > (t == 1 ? 1 : t < 4 ? 2 : 4); };
   for (int c = chunk; c * kChunk < in; c += step) {
     const int k0 = c * kChunk + at, k = min(k0, in - 8);  // past in_features: loaded, and cleared below
     u32x4 xr[8], wr[NG][8], xf[8], wf[8];
 #pragma unroll
-    for (int t = 0; t < 8; ++t) xr[t] = ld16(g.x + (size_t)row[t] * g.ldx + k);
+    for (int t = 0; t < 8; ++t)
+      if (there(t)) xr[t] = ld16(g.x + (size_t)row[t] * g.ldx + k);
 #pragma unroll
     for (int i = 0; i < NG; ++i)
       if (i < most)
@@ -267,7 +271,9 @@ __device__ __forceinline__ void shrink_chunks(f32x4 (&acc)[NG], const LoraArgs& 
 #pragma unroll
         for (int t = 0; t < 8; ++t) wr[i][t] = k0 < in ? wr[i][t] : u32x4{0, 0, 0, 0};
     }
-    put_rows(stage, xr, lane);
+#pragma unroll
+    for (int t = 0; t < 8; ++t)
+      if (there(t)) stage[place_of(2 * t + r, lane & 31)] = xr[t];
     wave_sync();
     get_rows(stage, xf, n, q);
     wave_sync();
@@ -332,7 +338,7 @@ __global__ void __launch_bounds__(256, NG == 3 ? 2 : 3) k_lora_shrink(const Lora
       left[i] = rank - 1 - j;
     }
     if (g0 >= g.turns * NG) lds_barrier();  // behind what is read of the last ones' sums
-    shrink_chunks<NG>(acc, g, xrow, w, left, all - g0, split * 4 + wave, 4 * g.splits, stage[wave], lane);
+    shrink_chunks<NG, false>(acc, g, xrow, w, left, all - g0, split * 4 + wave, 4 * g.splits, stage[wave], lane);
     // the four waves' sums
 #pragma unroll
     for (int i = 0; i < NG; ++i) stage[wave][i * 64 + lane] = __builtin_bit_cast(u32x4, acc[i]);
@@ -727,7 +733,11 @@ __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g)
     w[i] = g.a + (((size_t)a * g.n_parts + part) * g.max_rank + 16 * i) * g.in;
     left[i] = rank - 1 - 16 * i;
   }
-  shrink_chunks<NG>(acc, g, xrow, w, left, (rank + 15) / 16, wave, kWaves, stage[wave], lane);
+  // Tiles of single tokens have few rows: with one product of 16 ranks they take 5.1 us and not 5.4 on 2048
+  // in_features, 5.9 and 6.7 on 4096, tiles of 16 rows as long as before; with two, which leave fewer registers, 12.3
+  // and 11.4.
+  const int n_x = (__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < kRows && p.row[lane % kRows] >= 0)) + 1) / 2;
+  shrink_chunks<NG, NG == 1>(acc, g, xrow, w, left, (rank + 15) / 16, wave, kWaves, stage[wave], lane, n_x);
 #pragma unroll
   for (int i = 0; i < NG; ++i) stage[wave][i * 64 + lane] = __builtin_bit_cast(u32x4, acc[i]);
   lds_barrier();
@@ -856,11 +866,13 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int chunks = g.chunk_end[n_parts - 1];
   // Both products in one launch, if a block's own h costs it little: 32 ranks at most, few enough numbers of A and x
-  // for a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. At 16
-  // ranks and 2048 columns, 4 sequences: in_features 1024 5.4 us and not 8.0 of two launches, 2048 5.8 and 8.1, 4096
-  // 7.2 and 8.5, 6144 8.5 and 8.5, 8192 9.8 and 8.7; at 32 ranks 4096 9.0 and 9.2, 6144 10.7 and 9.3. At 16 ranks
-  // and 16384 columns 2048 numbers of 128 sequences (52 MB) take 10.5 us and 11.5, 4096 of 16 (75 MB) 10.6 and 9.7, of
-  // 128 (105 MB) 14.0 and 12.2. A launch more is 2 us of the host's time, too.
+  // for a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. 16 ranks and
+  // 2048 columns of one sequence take 5.9 us with 4096 in_features and 7.8 with 8192, where two launches take 8.1; 16
+  // sequences' on 1000 columns 9.4 and 10.8, but one sequence of 16 rows 9.9 and 8.9, and 32 sequences of 4 adapters
+  // 11.0 and 9.9: there x counts as much as A. At 32 ranks and 4 sequences 4096 take 9.0 and 9.2, 6144 10.7 and 9.3. At 16
+  // ranks and 16384 columns 2048 numbers of 128 sequences (52 MB) take 10.5 us and 11.5, 4096 of 16 (75 MB) 10.6 and
+  // 9.7, of 128 (105 MB) 14.0 and 12.2. A launch more is 2 us of the host's time, too.
+  const size_t most = per_part == 1 && n_rows < 8 * s.groups ? 16384 : 12288;
   int tiles = 2, blocks = 0;
   for (;; tiles *= 2) {
     blocks = 0;
@@ -869,7 +881,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
     if (tiles == 8 || (long long)s.slots * blocks <= 256) break;
   }
   const size_t whole = (size_t)s.slots * blocks * 16 * (per_part + 1) * 2 * in_features;
-  if (ks == 1 && (per_part + 1) * (size_t)in_features <= 12288 && whole <= 70000000) {
+  if (ks == 1 && (per_part + 1) * (size_t)in_features <= most && whole <= 70000000) {
     for (int p = 0; p < n_parts; ++p)
       g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
                        (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
