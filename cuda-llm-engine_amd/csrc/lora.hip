@@ -10,7 +10,7 @@
 //   1 row, rank 16, 2048 -> 2048: 5.1 (< 0.1). One launch: its loads one behind the other.
 //   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 11.2 (2.2). One launch; every block
 //     reads its tile's A and x again, from the L2: 9.5 where all of it is in the last-level cache.
-//   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 29.2 (12.6), 18 and 11. 60 MB by the first launch at 3.3
+//   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 29.2 (12.6), 18 and 11. 61 MB by the first launch at 3.3
 //     TB/s: a tile's rows are found (2 us), then two rounds of loads that wait for one another.
 //   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.8 (27.7), 9 and 35. y in place by 16 rows of
 //     256 bytes a wave, which alone take 30.
@@ -869,9 +869,9 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   // for a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. 16 ranks and
   // 2048 columns of one sequence take 5.9 us with 4096 in_features and 7.8 with 8192, where two launches take 8.1; 16
   // sequences' on 1000 columns 9.4 and 10.8, but one sequence of 16 rows 9.9 and 8.9, and 32 sequences of 4 adapters
-  // 11.0 and 9.9: there x counts as much as A. At 32 ranks and 4 sequences 4096 take 9.0 and 9.2, 6144 10.7 and 9.3. At 16
-  // ranks and 16384 columns 2048 numbers of 128 sequences (52 MB) take 10.5 us and 11.5, 4096 of 16 (75 MB) 10.6 and
-  // 9.7, of 128 (105 MB) 14.0 and 12.2. A launch more is 2 us of the host's time, too.
+  // 11.0 and 9.9: there x counts as much as A. At 32 ranks and 4 sequences 4096 take 9.0 and 9.2, 6144 10.7 and 9.3.
+  // At 16 ranks and 16384 columns 2048 numbers of 128 sequences (52 MB) take 10.5 us and 11.5, 4096 of 16 (75 MB) 10.6
+  // and 9.7, of 128 (105 MB) 14.0 and 12.2. A launch more is 2 us of the host's time, too.
   const size_t most = per_part == 1 && n_rows < 8 * s.groups ? 16384 : 12288;
   int tiles = 2, blocks = 0;
   for (;; tiles *= 2) {

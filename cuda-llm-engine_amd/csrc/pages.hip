@@ -3,9 +3,9 @@
 // which blocks run: counts are added up, and every page number comes from a count of what lies in front.
 //
 // Copies are bound by bytes, tables by loads that wait for one another. Measured (one MI355X, inputs from HBM; the
-// floor is each byte once at 6 TB/s), us: the fork of 8 beams and its copies in 16 layers 9.3 (0.5), k_fork 7.1 and the
-// copies 3.1; of 256 beams over an 8-bit cache 27.4 (7.2), rows 4.8, holders 4.6, pages 7.4, copies 12.4 (43 MB); the
-// compaction of 64 sequences, half the pool free, 49.6 (37.5), 5.6 and the copies 43.7 (231 MB at 5.3 TB/s).
+// floor is each byte once at 6 TB/s), us: the fork of 8 beams and its copies in 16 layers 9.3 (0.5), k_fork 6.6 and the
+// copies 3.2; of 256 beams over an 8-bit cache 25.0 (7.2), rows 4.0, holders 4.0, pages 5.6, copies 12.8 (43 MB); the
+// compaction of 64 sequences, half the pool free, 47.6 (37.5), 5.8 and the copies 41.6 (231 MB at 5.5 TB/s).
 #include <limits.h>
 
 #include "common.hpp"
@@ -508,8 +508,8 @@ __global__ void __launch_bounds__(1024) k_compact(const CompactArgs a) {
 }
 
 // Whether one block does it all: the launches cost more than the other CUs would give. A fork of 8 to 8 sequences
-// by tables of 20 pages takes 6.7 us and not 9.2, of 32 to 32 11.7 and 12.1, by 128 pages 12.9 and 11.9 (but two
-// launches less, 3 us, on the host), of 64 to 64 by 20 pages 16.9 and 11.5. A compaction of 1000 pages and 1920
+// by tables of 20 pages takes 6.7 us and not 9.2, of 32 to 32 10.2 and some 10, by 128 pages 11.9 and 11 (but two
+// launches less, 3 us, on the host), of 64 to 64 by 20 pages 16.9 and 10.0. A compaction of 1000 pages and 1920
 // entries 5.1 us and not 8.6, of 4096 and 8192 10.6 and 11.6, of 4096 and 32768 20.4 and 11.6.
 bool fork_by_one_block(int n_old, int n_new, int max_pages) {
   return n_old + n_new <= 64 && (n_old + n_new) * max_pages <= 8192;
@@ -632,7 +632,7 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   a.page_size = page_size;
   a.num_pages = num_pages;
   if (fork_by_one_block(n_old, n_new, max_pages)) return launch(k_fork, dim3(1), dim3(1024), 0, s, a);
-  // tables of 1024 pages: 24 us with four entries a lane at a time and 26.6 with one; of 20 pages 12.0 and 11.5
+  // tables of 1024 pages: 24 us with four entries a lane at a time and 26.6 with one; of 20 pages half a us more
   const bool wide = max_pages > 256;
   int st = LLMK_OK;
   if (n_new > 0)

@@ -12,9 +12,9 @@
 //
 // Bound by bytes, each once each way; a 64-bit cosine and sine take some 60 instructions a pair of a row, which is why
 // they are computed once a row for all its heads and while the data is on its way. Measured (one MI355X, inputs from
-// HBM, the floor at 6 TB/s), us: 1 row 2.1 (one launch); 4001 rows of 40 heads of 64 in place 10.3 (6.8: 41 MB at 4.0
-// TB/s, a launch and a table's load, an angle and a barrier in front of the first store); 256 rows into the cache 3.6
-// (0.5); 2001 rows of 28 + 2 x 4 heads of 128 into the cache 11.1 (6.2: 37 MB).
+// HBM, the floor at 6 TB/s), us: 1 row 2.1 (one launch); 4001 rows of 40 heads of 64 in place 10.4 (6.8: 41 MB at 3.9
+// TB/s, as an addition in place to as many bytes takes 9.9); 256 rows into the cache 3.6 (0.5); 2001 rows of 28 + 2 x 4
+// heads of 128 into the cache 10.2 (6.2: 37 MB, of which a plain copy takes 7).
 #include "angles.hpp"
 #include "layer_ops.hpp"
 
