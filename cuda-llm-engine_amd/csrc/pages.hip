@@ -240,11 +240,20 @@ __device__ __forceinline__ void fork_refs(const ForkArgs& a, int p) {
   }
   const int held = held_pages<U>(row, a.max_pages, a.num_pages, start);
   const int whole = length_of(a, raw, held) / a.page_size;
-  // whole pages of an only child stay as they are
-  for (int j = (children == 1 ? whole : 0) + lane; j < held; j += 64) {
-    const int takes = j < whole ? children
-                      : children ? a.new_tables[(size_t)first * a.max_pages + j] >= 0 : 0;
-    if (takes != 1) atomicAdd(&a.refs[row[j]], takes - 1);
+  const int from = children == 1 ? whole : 0;  // whole pages of an only child stay as they are
+  for (int j0 = from / (64 * U) * (64 * U); j0 < held; j0 += 64 * U) {
+    int v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = start[u];
+    if (j0 > 0) load_entries<U>(row, j0, held, -1, v);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int j = j0 + 64 * u + lane;
+      if (j < from || j >= held) continue;
+      const int takes = j < whole ? children
+                        : children ? a.new_tables[(size_t)first * a.max_pages + j] >= 0 : 0;
+      if (takes != 1) atomicAdd(&a.refs[v[u]], takes - 1);
+    }
   }
 }
 
@@ -508,8 +517,8 @@ __global__ void __launch_bounds__(1024) k_compact(const CompactArgs a) {
 }
 
 // Whether one block does it all: the launches cost more than the other CUs would give. A fork of 8 to 8 sequences
-// by tables of 20 pages takes 6.7 us and not 9.2, of 32 to 32 10.2 and some 10, by 128 pages 11.9 and 11 (but two
-// launches less, 3 us, on the host), of 64 to 64 by 20 pages 16.9 and 10.0. A compaction of 1000 pages and 1920
+// by tables of 20 pages takes 6.7 us and not 8.8, of 32 to 32 10.6 and 9.9, by 128 pages 11.8 and 10.4 (but two
+// launches less, 3 us, on the host), of 64 to 64 by 20 pages 16.4 and 9.8. A compaction of 1000 pages and 1920
 // entries 5.1 us and not 8.6, of 4096 and 8192 10.6 and 11.6, of 4096 and 32768 20.4 and 11.6.
 bool fork_by_one_block(int n_old, int n_new, int max_pages) {
   return n_old + n_new <= 64 && (n_old + n_new) * max_pages <= 8192;
@@ -540,9 +549,9 @@ extern "C" int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, 
     if (page_bytes[i] > ((size_t)1 << 32)) return LLMK_ERR_UNSUPPORTED;
   }
   const auto whole = [&](int p) { return aligned16(pools[p]) && page_bytes[p] % 16 == 0; };
-  // Many pairs are walked pool by pool, in whose order a compaction's lie in memory: 1024 pairs of 16 KB in 32 pools take
-  // 178 us and not 195 in order, 202 and not 214 at random; but 128 pairs in 4 pools 4.9 and not 4.5, 32 pairs of 8 KB
-  // in 32 pools 5.5 and not 3.4.
+  // Many pairs are walked pool by pool, in whose order a compaction's lie in memory: 1024 pairs of 16 KB in 32 pools
+  // take 178 us and not 195 in order, 202 and not 214 at random; but 128 pairs in 4 pools 4.9 and not 4.5, 32 pairs of
+  // 8 KB in 32 pools 5.5 and not 3.4.
   const bool across = n_copies >= 512;
   // small pages of whole vectors, all of one size, go together
   size_t small = 0;
@@ -632,13 +641,16 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   a.page_size = page_size;
   a.num_pages = num_pages;
   if (fork_by_one_block(n_old, n_new, max_pages)) return launch(k_fork, dim3(1), dim3(1024), 0, s, a);
-  // tables of 1024 pages: 24 us with four entries a lane at a time and 26.6 with one; of 20 pages half a us more
-  const bool wide = max_pages > 256;
+  // Entries a lane has on their way, 1, 4 and 16: 32 to 32 sequences by tables of 20 pages take 9.9, 10.4 and 13.0 us,
+  // 256 by 130 14.0, 13.3 and 15.7, 32 by 257 13.5, 12.4 and 13.8, by 1024 25.9, 21.9 and 18.5.
+  const int entries = max_pages <= 128 ? 1 : max_pages <= 512 ? 4 : 16;
   int st = LLMK_OK;
   if (n_new > 0)
-    st = launch(wide ? k_fork_rows<4> : k_fork_rows<1>, dim3(ceil_div(n_new, 4)), dim3(256), 0, s, a);
+    st = launch(entries == 1 ? k_fork_rows<1> : entries == 4 ? k_fork_rows<4> : k_fork_rows<16>,
+                dim3(ceil_div(n_new, 4)), dim3(256), 0, s, a);
   if (st == LLMK_OK && n_old > 0)
-    st = launch(wide ? k_fork_refs<4> : k_fork_refs<1>, dim3(ceil_div(n_old, 4)), dim3(256), 0, s, a);
+    st = launch(entries == 1 ? k_fork_refs<1> : entries == 4 ? k_fork_refs<4> : k_fork_refs<16>,
+                dim3(ceil_div(n_old, 4)), dim3(256), 0, s, a);
   if (st == LLMK_OK) st = launch(k_fork_find, dim3(1), dim3(1024), 0, s, a);
   return st;
 }

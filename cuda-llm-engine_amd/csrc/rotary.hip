@@ -197,7 +197,8 @@ int launch_rotary(RotaryArgs& a, int heads, int units, bool pairs, hipStream_t s
   };
   // Three units a thread on the way into the cache where one would be 1.2 to 3 rounds of all the card's waves: 2000
   // rows of 36 heads of 128 take 10.2 us and not 11.1, 3000 13.6 and not 15.3, 3000 rows of 48 heads of 64 10.3 and
-  // 11.1; but 1500 of these 7.4 and not 6.8, 8000 rows of 10 heads of 256 20.9 and 18.8, 1000 rows in place 4.2 and 3.6.
+  // 11.1; but 1500 of these 7.4 and not 6.8, 8000 rows of 10 heads of 256 20.9 and 18.8, 1000 rows in place 4.2 and
+  // 3.6.
   const long long all = (long long)a.n_rows * a.per_row;
   const int many = SCATTER && all >= 400000 && all < 1000000 ? 3 : 1;
   a.rows = rows_of(256 * many);

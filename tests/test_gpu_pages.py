@@ -164,6 +164,16 @@ def test_wide_tables(llmk, max_pages):
                refs, 16, num_pages)
 
 
+@pytest.mark.parametrize("max_pages", [63, 64, 65, 128, 129, 300, 512, 513, 1025])
+def test_wide_tables_of_many(llmk, max_pages):
+    rng = np.random.default_rng(max_pages)
+    tables, lens, refs, num_pages = ref.batch(rng, 70, 3, 16 * max_pages, 16, max_pages, spare=600)
+    reserve = np.where(rng.random(70) < 0.1, rng.integers(0, 16 * max_pages, 70), 1)
+    check_fork(llmk, tables, lens, rng.integers(-1, 70, 70), reserve, refs, 16, num_pages)
+    lens = (lens * rng.random(70)).astype(np.int64)  # cut back into pages that others hold
+    check_fork(llmk, tables, lens, rng.integers(-1, 70, 70), np.full(70, 20), refs, 16, num_pages)
+
+
 def test_free_pages_far_behind(llmk):
     """A nearly full cache: the free pages lie at its end, some are freed by the call itself."""
     num_pages, n = 70000, 8
