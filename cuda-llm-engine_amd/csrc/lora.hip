@@ -795,6 +795,19 @@ Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in, int products) {
   return s;
 }
 
+bool within_limits(int n_rows, int n_seqs, int max_rank, int in) {
+  return max_rank <= kMaxRank && n_rows <= (1 << 20) && n_seqs <= (1 << 20) && in <= (1 << 24);
+}
+
+// Whether n rows of `width` halves, ld apart, share some with n of `width2`, ld2 apart; columns of one matrix do not.
+bool rows_overlap(const uint16_t* a, int ld, int width, const uint16_t* b, int ld2, int width2, int n) {
+  const long long d = ((long long)reinterpret_cast<uintptr_t>(b) - (long long)reinterpret_cast<uintptr_t>(a)) / 2;
+  if (d >= (long long)(n - 1) * ld + width || -d >= (long long)(n - 1) * ld2 + width2) return false;
+  if (ld != ld2) return true;
+  const long long at = (d % ld + ld) % ld;  // of b's columns among a's
+  return at < width || at + width2 > ld;
+}
+
 }  // namespace
 }  // namespace llmk
 
@@ -805,6 +818,7 @@ extern "C" size_t llmk_lora_add_workspace_floats(int n_rows, int n_seqs, int n_a
   if (n_rows <= 0 || n_seqs <= 0 || n_adapters <= 0 || max_rank <= 0 || in_features <= 0 ||
       n_parts <= 0)
     return 0;
+  if (!within_limits(n_rows, n_seqs, max_rank, in_features) || n_parts > kParts) return 0;  // nor is a call
   const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features, n_parts * ((max_rank + 15) / 16));
   return (size_t)s.slots * (kNote + (size_t)s.splits * n_parts * ((max_rank + 31) / 32) * 512);
 }
@@ -818,7 +832,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   if (n_rows < 0 || n_seqs < 0 || n_adapters < 0 || max_rank <= 0 || in_features <= 0 ||
       n_parts < 1 || n_parts > kParts || !part_ends || (!row_starts && n_rows != n_seqs))
     return LLMK_ERR_INVALID_VALUE;
-  const int steps = (max_rank + 31) / 32, ks = steps <= 2 ? steps : steps <= 4 ? 4 : 8;
+  const int ks = max_rank <= 32 ? 1 : max_rank <= 64 ? 2 : max_rank <= 128 ? 4 : 8;
   const int columns = ks <= 4 ? 512 : 256;  // of a block
   LoraArgs g{};
   for (int p = 0; p < n_parts; ++p) {
@@ -831,13 +845,13 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   if (in_features % 8 || max_rank % 8 || ldx % 8 || ldy % 8 || ldx < in_features ||
       ldy < part_ends[n_parts - 1])
     return LLMK_ERR_SHAPE;
-  if (max_rank > kMaxRank || n_rows > (1 << 20) || n_seqs > (1 << 20) || in_features > (1 << 24) ||
-      g.chunk_end[n_parts - 1] > 65535)
+  if (!within_limits(n_rows, n_seqs, max_rank, in_features) || g.chunk_end[n_parts - 1] > 65535)
     return LLMK_ERR_UNSUPPORTED;
   if (n_rows == 0 || n_seqs == 0 || n_adapters == 0) return LLMK_OK;
   if (!x || !a || !b || !adapter_ids || !y || !workspace) return LLMK_ERR_INVALID_VALUE;
   if (!aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(y) || !aligned16(workspace))
     return LLMK_ERR_ALIGNMENT;
+  if (rows_overlap(x, ldx, in_features, y, ldy, part_ends[n_parts - 1], n_rows)) return LLMK_ERR_INVALID_VALUE;
   const int per_part = (max_rank + 15) / 16;
   const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features, n_parts * per_part);
   g.x = reinterpret_cast<const f16*>(x);
@@ -859,7 +873,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.max_rank = max_rank;
   g.in = in_features;
   g.slots = s.slots;
-  g.steps = steps;
+  g.steps = (max_rank + 31) / 32;
   g.splits = s.splits;
   g.groups = s.groups;
   g.windows = s.windows;

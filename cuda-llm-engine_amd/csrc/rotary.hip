@@ -292,6 +292,8 @@ extern "C" int llmk_qkv_rotary_scatter(const uint16_t* qkv, int ld, uint16_t* q_
   if (!aligned16(qkv) || !aligned16(q_out) || !aligned16(k_pool) || !aligned16(v_pool))
     return LLMK_ERR_ALIGNMENT;
   if (head_dim > 512) return LLMK_ERR_UNSUPPORTED;
+  const size_t read = (size_t)(n - 1) * ld + ((size_t)n_heads + 2 * (size_t)n_kv_heads) * head_dim;
+  if (qkv < q_out + (size_t)n * n_heads * head_dim && q_out < qkv + read) return LLMK_ERR_INVALID_VALUE;
   RotaryArgs a{};
   a.q = reinterpret_cast<const f16*>(qkv);
   a.k = a.q + (size_t)n_heads * head_dim;

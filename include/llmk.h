@@ -408,7 +408,8 @@ LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_lo
  * for bit; a row depends on its own x, y and adapter alone. Sums in fp32; between the two products 22
  * bits of a row's values relative to its largest one of the part; one rounding.
  * x rows have stride ldx and y rows ldy (elements, multiples of 8); in_features, max_rank (at most
- * 256) and the part ends are multiples of 8; x, a, b and y are 16-byte aligned. x and y may not overlap.
+ * 256) and the part ends are multiples of 8; x, a, b and y are 16-byte aligned. Rows of x and y may not
+ * overlap (LLMK_ERR_INVALID_VALUE); they may be columns of one matrix.
  * workspace: llmk_lora_add_workspace_floats(..) floats, 16-byte aligned; calls that may overlap need
  * one each, graphs replayed one behind the other may share one. LLMK_ERR_UNSUPPORTED, before any launch, for more
  * than 2^20 rows or sequences, 2^24 in_features or 65535 * 512 columns (half for ranks past 128), or rows times
@@ -447,7 +448,7 @@ LLMK_API int llmk_rotary_apply(uint16_t* q, int ldq, uint16_t* k, int ldk, const
  * pools [num_pages, page_size, n_kv_heads, head_dim] at positions[r] by block_tables[r, :] [n, max_pages].
  * Rows whose position is below 0 or past the table, or whose table entry is negative, write no k and v.
  * head_dim % 16 == 0, up to 512; rotary_dim % 16 == 0; ld % 8 == 0; qkv, q_out and the pools 16-byte aligned and
- * not overlapping. */
+ * not overlapping (q_out and qkv: LLMK_ERR_INVALID_VALUE). */
 LLMK_API int llmk_qkv_rotary_scatter(const uint16_t* qkv, int ld, uint16_t* q_out, uint16_t* k_pool,
                                      uint16_t* v_pool, const int32_t* block_tables,
                                      const int32_t* positions, const float* inv_freq,

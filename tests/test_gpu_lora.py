@@ -121,6 +121,25 @@ def test_widths_and_ranks(llmk, inner, rank):
     Case(rng, ids_of(rng, 5, 2), rng.integers(0, 30, 5), 2, rank, inner, (40,), behind=3).check(llmk)
 
 
+def test_columns_of_one_matrix(llmk):
+    rng = np.random.default_rng(11)
+    c = Case(rng, ids_of(rng, 6, 3), rng.integers(0, 9, 6), 3, 16, 136, (24, 72))
+    y = c.upload(llmk)
+    for first in (True, False):  # x in front of y, and behind it
+        m = torch.full((c.n_rows, 136 + 72 + 24), 5.0, dtype=torch.float16, device=DEV)
+        x, out = (m[:, :136], m[:, 144:216]) if first else (m[:, 88:224], m[:, 8:80])
+        x.copy_(c.t["x"][:, :136])
+        out.copy_(y[:, :72])
+        llmk.lora_add(x, m.shape[1], c.t["a"], c.t["b"], c.t["ranks"], c.t["scales"], c.t["ids"], c.t["starts"], out,
+                      m.shape[1], (24, 72), c.ws, c.n_rows, 6, 3, 16, 136)
+        want = y.clone()
+        c.call(llmk, want)
+        assert torch.equal(out, want[:, :72]) and torch.equal(x, c.t["x"][:, :136])
+        with pytest.raises(llmk.LlmkError):
+            llmk.lora_add(x, m.shape[1], c.t["a"], c.t["b"], c.t["ranks"], c.t["scales"], c.t["ids"], c.t["starts"],
+                          x[:, :72], m.shape[1], (24, 72), c.ws, c.n_rows, 6, 3, 16, 136)
+
+
 @pytest.mark.parametrize("ends", [(8,), (16,), (24,), (64,), (72,), (264,), (1000,), (2048,), (8, 16), (16, 24, 32),
                                   (520, 584, 648), (32, 64, 96, 128, 160, 168, 176, 184), (8, 2056)])
 @pytest.mark.parametrize("rank", [8, 16, 32, 136, 256])

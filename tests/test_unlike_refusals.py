@@ -59,6 +59,34 @@ def compact(L, **kw):
     return L.llmk_kv_compact(*a.values(), None)
 
 
+def test_lora_add_refuses_rows_that_overlap(llmk):
+    """x at a megabyte; what does not overlap is refused for its workspace, which is checked in front."""
+    L, E, at = llmk.lib(), llmk, 1 << 20
+    wide = dict(x=at, ldx=128, ldy=128)  # rows of 64 and of 48, 128 apart
+    for y in (at, at + 16, at + 2 * 48, at - 2 * 32, at + 2 * 128, at + 2 * (128 + 48), at - 2 * 128 * 3,
+              at + 2 * 88):  # the last: its 48 columns end in x's next row
+        assert lora(L, **wide, y=y) == E.LLMK_ERR_INVALID_VALUE, y - at
+    assert lora(L, **wide | dict(ldx=64), y=at + 2 * 128) == E.LLMK_ERR_INVALID_VALUE
+    assert lora(L, **wide | dict(ldy=48), y=at + 2 * 64) == E.LLMK_ERR_INVALID_VALUE  # other strides, one stretch
+
+
+def test_qkv_rotary_scatter_refuses_q_over_qkv(llmk):
+    at, rows, q = 1 << 20, 2 * (2 * 512 + 512), 2 * 3 * 256
+    for to in (at, at + 16, at + rows - 16, at - q + 16):
+        assert scatter(llmk.lib(), qkv=at, q=to) == llmk.LLMK_ERR_INVALID_VALUE, to - at
+
+
+def test_lora_add_sizes_past_the_limits(llmk):
+    """The call is refused, and its workspace is none."""
+    L, E, most = llmk.lib(), llmk, 2 ** 31 - 8
+    for bad in (dict(rank=264), dict(rank=most), dict(n_rows=(1 << 20) + 1), dict(n_seqs=2 ** 31 - 1),
+                dict(inner=(1 << 24) + 8, ldx=(1 << 24) + 8), dict(inner=most, ldx=most)):
+        assert lora(L, **bad) == E.LLMK_ERR_UNSUPPORTED, bad
+        a = dict(n_rows=4, n_seqs=2, n_adapters=3, rank=16, inner=64) | {k: v for k, v in bad.items() if k != "ldx"}
+        assert llmk.lora_add_workspace_floats(*a.values(), 2) == 0
+    assert llmk.lora_add_workspace_floats(4, 2, 3, 16, 64, 9) == 0
+
+
 def test_lora_add(llmk):
     L, E = llmk.lib(), llmk
     for nothing in (dict(n_rows=0), dict(n_seqs=0), dict(n_adapters=0),
