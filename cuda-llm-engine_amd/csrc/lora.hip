@@ -30,6 +30,8 @@
 // each) and given to the matrix instructions as two fp16: h * 2^-e, with 2^e such that the row's largest
 // is from 2^14 to 2^15, rounded, and what that lost. That keeps 22 bits relative to the row's largest, and the sum
 // is multiplied by scale * 2^e in fp32. So neither large nor small values of h leave fp16's range.
+#include <math.h>
+
 #include "kv8.hpp"
 
 namespace llmk {
@@ -795,6 +797,13 @@ Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in, int products) {
   return s;
 }
 
+// How many tiles there will be about, if sequences choose among the adapters evenly.
+int tiles_expected(int n_rows, int n_seqs, int n_adapters, int windows) {
+  const double n = n_seqs < kWindow ? n_seqs : kWindow;
+  const double groups = windows * n_adapters * (1.0 - pow(1.0 - 1.0 / n_adapters, n));
+  return (int)fmax(groups, n_rows / (double)kRows + (groups - 1) / 2);
+}
+
 bool within_limits(int n_rows, int n_seqs, int max_rank, int in) {
   return max_rank <= kMaxRank && n_rows <= (1 << 20) && n_seqs <= (1 << 20) && in <= (1 << 24);
 }
@@ -879,27 +888,30 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.windows = s.windows;
   hipStream_t st = static_cast<hipStream_t>(stream);
   const int chunks = g.chunk_end[n_parts - 1];
-  // Both products in one launch, if a block's own h costs it little: 32 ranks at most, few enough numbers of A and x
-  // for a block, and for all of them. Columns a block: 256, 512 or 1024, the fewest that are a block a CU. 16 ranks and
-  // 2048 columns of one sequence take 5.9 us with 4096 in_features and 7.8 with 8192, where two launches take 8.1; 16
+  // Both products in one launch, if a block's own h costs it little, 32 ranks at most and few enough numbers of A and
+  // x, and if its blocks are expected to run at once: one a CU, 32 an XCD. Columns a block: 256, 512 or 1024, the
+  // fewest with which they do. 300 rows of one adapter of rank 16 on 1024 -> 6144 take 7.9 us and 9.0 in two launches
+  // (12.0 if a third of an XCD's blocks waits for the others), on 11008|11008 20.0 so and 15.9. 16 ranks and 2048
+  // columns of one sequence take 5.9 us with 4096 in_features and 7.8 with 8192, where two launches take 8.1; 16
   // sequences' on 1000 columns 9.4 and 10.8, but one sequence of 16 rows 9.9 and 8.9, and 32 sequences of 4 adapters
-  // 11.0 and 9.9: there x counts as much as A. At 32 ranks and 4 sequences 4096 take 9.0 and 9.2, 6144 10.7 and 9.3.
-  // At 16 ranks and 16384 columns 2048 numbers of 128 sequences (52 MB) take 10.5 us and 11.5, 4096 of 16 (75 MB) 10.6
-  // and 9.7, of 128 (105 MB) 14.0 and 12.2. A launch more is 2 us of the host's time, too.
+  // 11.0 and 9.9: there x counts as much as A. At 32 ranks and 8 sequences 4096 -> 4096|1024|1024 takes 10.4 and
+  // 11.4, 4 sequences of 6144 in_features 10.7 and 9.3. A launch more is 2 us of the host's time, too.
   const size_t most = per_part == 1 && n_rows < 8 * s.groups ? 16384 : 12288;
+  const int used = tiles_expected(n_rows, n_seqs, n_adapters, s.windows);
   int tiles = 2, blocks = 0;
+  bool fits = false;
   for (;; tiles *= 2) {
     blocks = 0;
     for (int p = 0; p < n_parts; ++p)
       blocks += (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
-    if (tiles == 8 || (long long)s.slots * blocks <= 256) break;
+    g.per_block = s.slots >= 8 || blocks <= 32;  // whether a tile's blocks share an XCD
+    fits = g.per_block ? (used + 7) / 8 * blocks <= 32 : used * blocks <= 256;
+    if (tiles == 8 || fits) break;
   }
-  const size_t whole = (size_t)s.slots * blocks * 16 * (per_part + 1) * 2 * in_features;
-  if (ks == 1 && (per_part + 1) * (size_t)in_features <= most && whole <= 70000000) {
+  if (fits && ks == 1 && (per_part + 1) * (size_t)in_features <= most) {
     for (int p = 0; p < n_parts; ++p)
       g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
                        (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
-    g.per_block = s.slots >= 8 || blocks <= 32;  // whether a tile's blocks share an XCD
     const dim3 grid((g.per_block ? (s.slots + 7) / 8 * 8 : s.slots) * blocks), threads(64 * kWaves);
     return launch(per_part == 1 ? (tiles == 2   ? k_lora_whole<2, 1>
                                    : tiles == 4 ? k_lora_whole<4, 1>
