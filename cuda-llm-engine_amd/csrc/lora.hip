@@ -797,11 +797,14 @@ Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in, int products) {
   return s;
 }
 
-// How many tiles there will be about, if sequences choose among the adapters evenly.
-int tiles_expected(int n_rows, int n_seqs, int n_adapters, int windows) {
-  const double n = n_seqs < kWindow ? n_seqs : kWindow;
-  const double groups = windows * n_adapters * (1.0 - pow(1.0 - 1.0 / n_adapters, n));
-  return (int)fmax(groups, n_rows / (double)kRows + (groups - 1) / 2);
+// How many tiles there will be about if sequences choose among the adapters evenly, and if all choose another.
+struct Tiles {
+  int likely, many;
+};
+Tiles tiles_of(int n_rows, int n_seqs, int n_adapters, int windows, int groups) {
+  const double n = n_seqs < kWindow ? n_seqs : kWindow, rows = n_rows / (double)kRows, most = (double)windows * groups;
+  const double some = windows * n_adapters * (1.0 - pow(1.0 - 1.0 / n_adapters, n));
+  return {(int)fmax(some, rows + 0.5 * (some - 1)), (int)ceil(fmax(most, rows + 0.75 * (most - 1)))};
 }
 
 bool within_limits(int n_rows, int n_seqs, int max_rank, int in) {
@@ -897,18 +900,19 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   // 11.0 and 9.9: there x counts as much as A. At 32 ranks and 8 sequences 4096 -> 4096|1024|1024 takes 10.4 and
   // 11.4, 4 sequences of 6144 in_features 10.7 and 9.3. A launch more is 2 us of the host's time, too.
   const size_t most = per_part == 1 && n_rows < 8 * s.groups ? 16384 : 12288;
-  const int used = tiles_expected(n_rows, n_seqs, n_adapters, s.windows);
+  // The columns are chosen for many tiles, as too few of them cost more: 48 sequences of up to 5 rows, 16 adapters,
+  // 4096 -> 4096|1024|1024, 11.2 us with 1024 and 14.6 with 512, of which a third has to wait on some XCDs.
+  const Tiles used = tiles_of(n_rows, n_seqs, n_adapters, s.windows, s.groups);
   int tiles = 2, blocks = 0;
-  bool fits = false;
+  const auto fits = [&](int n) { return g.per_block ? (n + 7) / 8 * blocks <= 32 : (long long)n * blocks <= 256; };
   for (;; tiles *= 2) {
     blocks = 0;
     for (int p = 0; p < n_parts; ++p)
       blocks += (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
     g.per_block = s.slots >= 8 || blocks <= 32;  // whether a tile's blocks share an XCD
-    fits = g.per_block ? (used + 7) / 8 * blocks <= 32 : used * blocks <= 256;
-    if (tiles == 8 || fits) break;
+    if (tiles == 8 || fits(used.many)) break;
   }
-  if (fits && ks == 1 && (per_part + 1) * (size_t)in_features <= most) {
+  if (fits(used.likely) && ks == 1 && (per_part + 1) * (size_t)in_features <= most) {
     for (int p = 0; p < n_parts; ++p)
       g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
                        (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
