@@ -10,11 +10,11 @@
 //   1 row, rank 16, 2048 -> 2048: 5.1 (< 0.1). One launch: its loads one behind the other.
 //   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 11.2 (2.2). One launch; every block
 //     reads its tile's A and x again, from the L2: 9.5 where all of it is in the last-level cache.
-//   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 29.2 (12.6), 18 and 11. 61 MB by the first launch at 3.3
+//   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 28.6 (12.6), 18 and 10. 61 MB by the first launch at 3.3
 //     TB/s: a tile's rows are found (2 us), then two rounds of loads that wait for one another.
-//   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.8 (27.7), 9 and 35. y in place by 16 rows of
+//   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.0 (27.7), 9 and 35. y in place by 16 rows of
 //     256 bytes a wave, which alone take 30.
-//   3 prompts of 456 rows, rank 128, 8192 -> 11008|11008: 92 (30.6), 40 and 58. A and B from the L2 by every tile, 540
+//   3 prompts of 456 rows, rank 128, 8192 -> 11008|11008: 89 (30.6), 40 and 57. A and B from the L2 by every tile, 540
 //     MB for the first; two tiles a block halve that, but also the waves a SIMD, and take as long.
 //
 // Tiles. Sequences are taken 256 at a time (a window); those of a window with the same adapter are a
@@ -529,20 +529,34 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : 2) k_lora_expand(const Lora
     int row[TILES / 2];
 #pragma unroll
     for (int t = 0; t < TILES / 2; ++t) row[t] = note[kRows + y_row<TILES>(t, lane)];
-    // the splits' sums: up to two by the wave itself, more by the block's waves, two each, through LDS
-    float h[KS][8];
+    if ((unsigned)a >= (unsigned)g.n_adapters || rank <= 0 || rank > g.max_rank) continue;
+    // all that the note leads to is on its way before the first of it is waited for: h, then y and B
     const f32x4* from = g.h + ((size_t)slot * g.n_parts + part) * g.steps * 128 + lane;
-    const auto add_split = [&](f32x4 (&v)[KS][2], int split) {
+    const auto load_split = [&](f32x4 (&v)[KS][2], int split) {
       const f32x4* u = from + (size_t)split * g.slots * g.n_parts * g.steps * 128;
 #pragma unroll
       for (int s = 0; s < KS; ++s)  // steps behind the last: its numbers, which rank cuts off
 #pragma unroll
         for (int f = 0; f < 2; ++f) v[s][f] = u[(min(s, g.steps - 1) * 2 + f) * 64];
     };
+    // the splits' sums: up to two by the wave itself, more by the block's waves, two each, through LDS
     f32x4 u[KS][2], w[KS][2];
     const int one = MANY ? wave : 0, two = MANY ? wave + 4 : 1;
-    if (one < g.splits) add_split(u, one);
-    if (two < g.splits) add_split(w, two);
+    if (one < g.splits) load_split(u, one);
+    if (two < g.splits) load_split(w, two);
+    f16* y[TILES / 2];
+    u32x4 old[TILES / 2];
+#pragma unroll
+    for (int t = 0; t < TILES / 2; ++t)
+      y[t] = (unsigned)row[t] < (unsigned)g.n_rows && column < end ? g.y + (size_t)row[t] * g.ldy + column
+                                                                   : nullptr;
+    const bool all = all_of<TILES>(y);
+    load_y<TILES>(old, y, all);
+    const bool fresh = a != loaded;
+    if (fresh) {
+      loaded = a;
+      load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
+    }
     if (one < g.splits && two < g.splits)
 #pragma unroll
       for (int s = 0; s < KS; ++s)
@@ -569,28 +583,12 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : 2) k_lora_expand(const Lora
             if (m < g.splits) u[s][f] += v[m];
         }
     }
+    float h[KS][8];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) h[s][e] = u[s][e / 4][e % 4];
-    if ((unsigned)a >= (unsigned)g.n_adapters || rank <= 0 || rank > g.max_rank) continue;
-    f16* y[TILES / 2];
-    u32x4 old[TILES / 2];
-#pragma unroll
-    for (int t = 0; t < TILES / 2; ++t)
-      y[t] = (unsigned)row[t] < (unsigned)g.n_rows && column < end ? g.y + (size_t)row[t] * g.ldy + column
-                                                                   : nullptr;
-    const bool all = all_of<TILES>(y);
-    load_y<TILES>(old, y, all);
-    if (a != loaded) {
-      loaded = a;
-      load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
-      cut_b<KS, TILES>(bf, rank, q);
-    }
-#pragma unroll
-    for (int s = 0; s < KS; ++s)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) h[s][e] = 32 * s + 8 * q + e < rank ? h[s][e] : 0.f;
+      for (int e = 0; e < 8; ++e) h[s][e] = 32 * s + 8 * q + e < rank ? u[s][e / 4][e % 4] : 0.f;
+    if (fresh) cut_b<KS, TILES>(bf, rank, q);
     f16x8 hi[KS], lo[KS];
     const float by = scale * split_h<KS>(h, hi, lo);
     wave_sync();
@@ -601,11 +599,11 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : 2) k_lora_expand(const Lora
 }
 
 // The same for more than 64 ranks: a block's waves share out the steps of 32 ranks, add up their splits and make them
-// the two fp16 once for all. 3 prompts of 456 rows and rank 128 on 11008|11008 columns take 58 us, and 112 with h made
+// the two fp16 once for all. 3 prompts of 456 rows and rank 128 on 11008|11008 columns take 57 us, and 112 with h made
 // by every wave for itself and half the columns.
 template <int KS>
 __global__ void __launch_bounds__(256, 2) k_lora_expand_high(const LoraArgs g) {
-  constexpr int TILES = 32 / KS, MINE = KS / 4;
+  constexpr int TILES = 32 / KS, MINE = KS / 4, AT = KS == 4 ? 4 : 1;  // AT: splits at a time, as registers allow
   __shared__ u32x4 stage[4][kRows * 4 * TILES + 4];
   __shared__ u32x4 pair[KS][2][64];
   __shared__ float top[KS][kRows];
@@ -631,23 +629,45 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand_high(const LoraArgs g) {
       const int row = note[kRows + y_row<TILES>(t, lane)];
       y[t] = (unsigned)row < (unsigned)g.n_rows && column < end ? g.y + (size_t)row * g.ldy + column : nullptr;
     }
-    float h[MINE][8];
+    // as above: h of the wave's steps, then y and B; with 256 ranks' B, h is out of the registers first
     const f32x4* from = g.h + ((size_t)slot * g.n_parts + part) * g.steps * 128 + lane;
+    f32x4 sum[MINE][AT][2];
+    const auto load_splits = [&](int d0) {
 #pragma unroll
-    for (int m = 0; m < MINE; ++m) {
+      for (int m = 0; m < MINE; ++m)
+#pragma unroll
+        for (int k = 0; k < AT; ++k) {
+          const f32x4* u = from + (size_t)min(d0 + k, g.splits - 1) * g.slots * g.n_parts * g.steps * 128 +
+                           min(wave + 4 * m, g.steps - 1) * 128;
+          sum[m][k][0] = u[0];
+          sum[m][k][1] = u[64];
+        }
+    };
+    const bool all = all_of<TILES>(y), fresh = a != loaded;
+    const auto load_y_and_b = [&] {
+      load_y<TILES>(old, y, all);
+      if (fresh) load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
+      loaded = a;
+    };
+    load_splits(0);
+    if (KS == 4) load_y_and_b();
+    float h[MINE][8];
+#pragma unroll
+    for (int m = 0; m < MINE; ++m)
 #pragma unroll
       for (int e = 0; e < 8; ++e) h[m][e] = 0.f;
-      const int s = wave + 4 * m;
-      if (s < g.steps)
-        for (int d = 0; d < g.splits; ++d) {
-          const f32x4* u = from + (size_t)d * g.slots * g.n_parts * g.steps * 128 + s * 128;
-          const f32x4 v = u[0], w = u[64];
+    for (int d0 = 0; d0 < g.splits; d0 += AT) {
+      if (d0 > 0) load_splits(d0);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            h[m][e] += v[e];
-            h[m][e + 4] += w[e];
-          }
-        }
+      for (int m = 0; m < MINE; ++m)
+#pragma unroll
+        for (int k = 0; k < AT; ++k)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) h[m][e] += d0 + k < g.splits ? sum[m][k][e / 4][e % 4] : 0.f;
+    }
+#pragma unroll
+    for (int m = 0; m < MINE; ++m) {
+      const int s = wave + 4 * m;
       float most = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -659,13 +679,8 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand_high(const LoraArgs g) {
       most = __builtin_fmaxf(most, __shfl_xor(most, 32));
       if (q == 0) top[s][n] = most;
     }
-    const bool all = all_of<TILES>(y);
-    load_y<TILES>(old, y, all);
-    if (a != loaded) {
-      loaded = a;
-      load_b<KS, TILES>(bf, g.b + (size_t)a * out * g.max_rank, c0, end, g.max_rank, rank, n, q);
-      cut_b<KS, TILES>(bf, rank, q);
-    }
+    if (KS == 8) load_y_and_b();
+    if (fresh) cut_b<KS, TILES>(bf, rank, q);
     lds_barrier();
     float most = 0.f;
 #pragma unroll
