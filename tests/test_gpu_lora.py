@@ -121,6 +121,20 @@ def test_widths_and_ranks(llmk, inner, rank):
     Case(rng, ids_of(rng, 5, 2), rng.integers(0, 30, 5), 2, rank, inner, (40,), behind=3).check(llmk)
 
 
+@pytest.mark.parametrize("n,rows,adapters,rank,inner,ends", [
+    (2, 64, 1, 16, 264, (4096, 5120, 6144)), (2, 150, 1, 16, 72, (4096, 5120, 6144)), (2, 100, 1, 32, 72, (11008, 22016)),
+    (1, 500, 3, 8, 264, (2048,)), (2, 400, 1, 24, 72, (2560, 5120, 7680)), (12, 10, 48, 16, 72, (8192, 16384)),
+    (24, 6, 96, 16, 72, (2048,)), (48, 5, 16, 16, 520, (4096, 5120, 6144)), (80, 2, 300, 8, 72, (4096, 5120, 6144)),
+    (8, 1, 16, 16, 8192, (4096, 5120, 6144)), (16, 1, 32, 16, 6152, (1000,)), (1, 16, 8, 16, 8192, (2048,)),
+    (700, 1, 40, 16, 136, (1024,)), (30, 3, 30, 32, 2056, (4096,))])
+def test_batches_around_one_launch(llmk, n, rows, adapters, rank, inner, ends):
+    """By the sizes some go in one launch and some in two, with 256, 512 or 1024 columns a block."""
+    rng = np.random.default_rng([n, rows, adapters, rank])
+    for same in (False, True):  # adapters as they fall, and the same for all: more tiles, and fewer, than expected
+        ids = np.full(n, adapters - 1) if same else rng.permutation(max(n, adapters))[:n] % adapters
+        Case(rng, ids, rng.integers(1, rows + 1, n) if rows > 1 else None, adapters, rank, inner, ends).check(llmk)
+
+
 def test_columns_of_one_matrix(llmk):
     rng = np.random.default_rng(11)
     c = Case(rng, ids_of(rng, 6, 3), rng.integers(0, 9, 6), 3, 16, 136, (24, 72))
