@@ -8,8 +8,8 @@
 //
 // Measured (one MI355X, fp16, inputs from HBM; the floor is each byte once at 6 TB/s), us:
 //   1 row, rank 16, 2048 -> 2048: 5.1 (< 0.1). One launch: its loads one behind the other.
-//   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 11.2 (2.2). One launch; every block
-//     reads its tile's A and x again, from the L2: 9.5 where all of it is in the last-level cache.
+//   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 10.4 (2.2). One launch; every block
+//     reads its tile's A and x again, from the L2: 8.9 where all of it is in the last-level cache.
 //   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 28.6 (12.6), 18 and 10. 61 MB by the first launch at 3.3
 //     TB/s: a tile's rows are found (2 us), then two rounds of loads that wait for one another.
 //   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.0 (27.7), 9 and 35. y in place by 16 rows of
@@ -17,14 +17,14 @@
 //   3 prompts of 456 rows, rank 128, 8192 -> 11008|11008: 89 (30.6), 40 and 57. A and B from the L2 by every tile, 540
 //     MB for the first; two tiles a block halve that, but also the waves a SIMD, and take as long.
 //
-// Tiles. Sequences are taken 256 at a time (a window); those of a window with the same adapter are a
-// group, in the order of their first ones, and a group's rows, in order, are cut into tiles of 16. Every
-// block of k_lora_shrink finds its tile by itself: adapters into a hash table in LDS, whose slots collect
-// the rows and the first member; counts of tiles summed up by those. That takes about a
-// microsecond beside the loads of ids and starts, which a launch of its own would have to wait for too.
-// What a block finds does not depend on the order in which threads reach the table. Window w's tiles
-// begin at slot starts[256 w] / 16 + w * (groups + 1), which leaves room for all of them: slots without a
-// tile are noted as such.
+// Tiles. Sequences are taken 256 at a time (a window); those of a window with the same adapter are a group, in the
+// order of their first ones, and a group's rows, in order, are cut into tiles of 16. Every block of the first
+// product finds its tile by itself: up to 64 sequences by a wave, whose lanes compare adapters bit by bit; more by
+// adapters in a hash table in LDS, whose slots collect the rows and the first member, and counts of tiles summed up
+// by those. That takes half a microsecond, or one and a half, beside the loads of ids and starts, which a launch of
+// its own would have to wait for too. What a block finds does not depend on the order in which threads reach the
+// table. Window w's tiles begin at slot starts[256 w] / 16 + w * (groups + 1), which leaves room for all of them:
+// slots without a tile are noted as such.
 //
 // Between the products h is held in fp32 (the blocks of a tile that share out in_features leave a sum
 // each) and given to the matrix instructions as two fp16: h * 2^-e, with 2^e such that the row's largest
@@ -118,8 +118,8 @@ __device__ __forceinline__ int row_of_tile(uint64_t members, int before, int row
   return row;
 }
 
-// Finds tile `slot` of few groups among 64 sequences at most: every wave by itself, group by group, without a barrier.
-// All write the same rows.
+// Finds tile `slot` among 64 sequences at most: every wave by itself, a sequence a lane, without a barrier. All write
+// the same rows.
 __device__ __forceinline__ Tile find_tile_by_wave(const LoraArgs& g, int slot, Plan& p) {
   const int lane = threadIdx.x & 63;
   int id = -1, r0 = 0, rows = 0, rank = g.max_rank;
@@ -134,34 +134,48 @@ __device__ __forceinline__ Tile find_tile_by_wave(const LoraArgs& g, int slot, P
     if (g.ranks) rank = g.ranks[id];
     if (g.scales) scale = g.scales[id];
   }
-  int tile = slot - uniform(first_row(g, 0)) / kRows;
-  for (uint64_t left = __builtin_amdgcn_ballot_w64(id >= 0); left;) {
-    const int first = __builtin_ctzll(left), a = __builtin_amdgcn_readlane(id, first);
-    const bool mine = id == a;
-    const uint64_t members = __builtin_amdgcn_ballot_w64(mine);
-    const int upto = wave_scan(mine ? rows : 0);
-    const int tiles = (__builtin_amdgcn_readlane(upto, 63) + kRows - 1) / kRows;
-    if (tile >= 0 && tile < tiles) {
-      const int before = upto - rows - tile * kRows;
-      const int row = row_of_tile(
-          __builtin_amdgcn_ballot_w64(mine && before < kRows && before + rows > 0), before, rows, r0, -1);
-      if (lane < kRows) p.row[lane] = row;
-      wave_sync();
-      return {a, min(__builtin_amdgcn_readlane(rank, first), g.max_rank),
-              __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), first))};
-    }
-    tile -= tiles;
-    left &= ~members;
+  uint64_t group = __builtin_amdgcn_ballot_w64(id >= 0);  // the lanes of the same adapter, bit by bit of its number
+  const int numbers = g.n_seqs > 1 ? g.n_adapters - 1 : 0;
+  for (int bit = 0; numbers >> bit; ++bit) {
+    const bool set = id >> bit & 1;
+    const uint64_t all = __builtin_amdgcn_ballot_w64(set);
+    group &= set ? all : ~all;
   }
-  if (lane < kRows) p.row[lane] = -1;  // the note's
+  const int leader = id >= 0 ? __builtin_ctzll(group) : lane;
+  int total = __builtin_popcountll(group);
+  if (g.starts) {
+    int* sums = p.rows + (threadIdx.x & ~63);
+    sums[lane] = 0;
+    wave_sync();
+    if (id >= 0) atomicAdd(&sums[leader], rows);
+    wave_sync();
+    total = sums[lane];
+  }
+  const bool leads = id >= 0 && leader == lane;
+  const int tiles = leads ? (total + kRows - 1) / kRows : 0, upto = wave_scan(tiles);
+  const int tile = slot - uniform(first_row(g, 0)) / kRows;
+  const uint64_t here = __builtin_amdgcn_ballot_w64(leads && tile >= upto - tiles && tile < upto);
+  if (here == 0) {
+    if (lane < kRows) p.row[lane] = -1;  // the note's
+    wave_sync();
+    return {-1, 0, 0.f};
+  }
+  const int first = __builtin_ctzll(here);
+  const bool mine = id >= 0 && leader == first;
+  const int from = (tile - __builtin_amdgcn_readlane(upto - tiles, first)) * kRows;
+  const int before = wave_scan(mine ? rows : 0) - rows - from;
+  const int row = row_of_tile(
+      __builtin_amdgcn_ballot_w64(mine && before < kRows && before + rows > 0), before, rows, r0, -1);
+  if (lane < kRows) p.row[lane] = row;
   wave_sync();
-  return {-1, 0, 0.f};
+  return {__builtin_amdgcn_readlane(id, first), min(__builtin_amdgcn_readlane(rank, first), g.max_rank),
+          __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), first))};
 }
 
 // Finds tile `slot` with 256 threads or more.
 __device__ __forceinline__ Tile find_tile(const LoraArgs& g, int slot, Plan& p) {
-  // one sequence's call takes 5.7 us so and 6.3 by the table, 48 sequences' of 16 adapters 12.6 and 12.1
-  if (g.groups <= 4 && g.n_seqs <= 64) return find_tile_by_wave(g, slot, p);
+  // 48 sequences of 16 adapters take 10.4 us so and 11.2 by the table, 8 of 8 9.5 and 10.5 (rank 32)
+  if (g.n_seqs <= 64) return find_tile_by_wave(g, slot, p);
   const int tid = threadIdx.x;
   int w = 0;
   for (int hi = g.windows; hi - w > 1;) {  // the last window that begins at or before the slot
