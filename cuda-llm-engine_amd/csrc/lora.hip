@@ -929,14 +929,13 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   // (12.0 if a third of an XCD's blocks waits for the others), on 11008|11008 20.0 so and 15.9. 16 ranks and 2048
   // columns of one sequence take 5.9 us with 4096 in_features and 7.8 with 8192, where two launches take 8.1; 16
   // sequences' on 1000 columns 9.4 and 10.8, but one sequence of 16 rows 9.9 and 8.9, and 32 sequences of 4 adapters
-  // 11.0 and 9.9: there x counts as much as A. At 32 ranks and 8 sequences 4096 -> 4096|1024|1024 takes 10.4 and
-  // 11.4, 4 sequences of 6144 in_features 10.7 and 9.3. A launch more is 2 us of the host's time, too.
-  const size_t most = per_part == 1 && n_rows < 8 * s.groups ? 16384 : 12288;
+  // 11.0 and 9.9: there x counts as much as A. At 32 ranks 8 sequences on 4096 -> 4096|1024|1024 take 9.5 and 11.3, 4
+  // of 16 rows on 8192|8192, 1024 columns a block, 12.4 and 10.6. A launch more is 2 us of the host's time, too.
   // The columns are chosen for many tiles, as too few of them cost more: 48 sequences of up to 5 rows, 16 adapters,
   // 4096 -> 4096|1024|1024, 11.2 us with 1024 and 14.6 with 512, of which a third has to wait on some XCDs.
   const Tiles used = tiles_of(n_rows, n_seqs, n_adapters, s.windows, s.groups);
   int tiles = 2, blocks = 0;
-  const auto fits = [&](int n) { return g.per_block ? (n + 7) / 8 * blocks <= 32 : (long long)n * blocks <= 256; };
+  const auto fits = [&](long long n) { return g.per_block ? (n + 7) / 8 * blocks <= 32 : n * blocks <= 256; };
   for (;; tiles *= 2) {
     blocks = 0;
     for (int p = 0; p < n_parts; ++p)
@@ -944,6 +943,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
     g.per_block = s.slots >= 8 || blocks <= 32;  // whether a tile's blocks share an XCD
     if (tiles == 8 || fits(used.many)) break;
   }
+  const size_t most = per_part == 1 && n_rows < 8 * s.groups ? 16384 : tiles == 8 ? 10240 : 12288;
   if (fits(used.likely) && ks == 1 && (per_part + 1) * (size_t)in_features <= most) {
     for (int p = 0; p < n_parts; ++p)
       g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
