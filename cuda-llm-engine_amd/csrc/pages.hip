@@ -9,6 +9,7 @@
 #include <limits.h>
 
 #include "common.hpp"
+#include "fork_notes.hpp"
 
 namespace llmk {
 namespace {
@@ -89,19 +90,15 @@ __global__ void __launch_bounds__(256) k_copy_pages(const CopyArgs a) {
 // block-wide sums
 // ---------------------------------------------------------------------------------------------
 // The sum of v over the threads in front, and *total over all. part: an int for each wave, two sets of which
-// take turns, so that one barrier is enough.
-__device__ __forceinline__ int block_scan(int v, int* part, int* total) {
+// take turns, so that one barrier is enough. Over a wave in 32 bits, over the block in T's.
+template <typename T>
+__device__ __forceinline__ T block_scan(int v, int* part, T* total) {
   const int wave = threadIdx.x >> 6, waves = blockDim.x >> 6, in = wave_scan(v);
   if ((threadIdx.x & 63) == 63) part[wave] = in;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < waves; ++w) {
-    const int n = part[w];
-    before += w < wave ? n : 0;
-    all += n;
-  }
-  *total = all;
-  return before + in - v;
+  const pages::Sums<T> s = pages::sums_of<T>(part, waves, wave);
+  *total = s.all;
+  return s.before + in - v;
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -116,7 +113,7 @@ struct ForkArgs {
 };
 
 constexpr int kFound = 4096;  // children whose counts of wanted pages are kept in LDS
-// Beside a first child's count of wanted pages (2^24 at most): it copies a page that others held, who may all let go.
+// Beside a first child's count of wanted pages (kMostWanted at most): it copies a page that others held, who may all let go.
 constexpr int kCopiesShared = 1 << 30;
 constexpr int kCopied = INT_MIN;  // holders of a page that is copied from and free behind that, while pages are given
 
@@ -313,8 +310,8 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, Find& f) {
   for (int c0 = 0; c0 < a.n_new; c0 += 1024) {
     const int c = c0 + threadIdx.x, noted = c < a.n_new ? a.fresh[c] : 0, mine = noted & (kCopiesShared - 1);
     const int2 column = c < a.n_new ? a.columns[(size_t)c * a.max_pages] : make_int2(0, 0);  // if there is one
-    int total;
-    const int before = block_scan(mine, f.part[turn ^= 1], &total);
+    long long total;
+    const long long before = block_scan(mine, f.part[turn ^= 1], &total);
     if (c < a.n_new) {
       const long long at = wanted + before;
       const int b = (int)(at < a.num_pages ? at : a.num_pages);
@@ -610,7 +607,7 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   if (!refs || !counts || !workspace || (n_old > 0 && (!block_tables || !seq_lens)) ||
       (n_new > 0 && (!parents || !new_tables || !new_lens || !copies)))
     return LLMK_ERR_INVALID_VALUE;
-  if (n_old > 65535 || n_new > 65535 || max_pages > (1 << 24)) return LLMK_ERR_UNSUPPORTED;
+  if (n_old > 65535 || n_new > 65535 || max_pages > pages::kMostWanted) return LLMK_ERR_UNSUPPORTED;
   {  // what is written, and what else there is
     const size_t n = n_new, m = n_old, width = max_pages;
     const int32_t* at[] = {refs,   new_tables, new_lens,     copies,   counts,
