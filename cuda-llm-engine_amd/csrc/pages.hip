@@ -108,13 +108,11 @@ struct ForkArgs {
   const int *tables, *lens, *parents, *reserve;
   int *refs, *new_tables, *new_lens, *copies, *counts;
   int* fresh;            // workspace: wanted pages of each child, then of those in front,
-  int2* columns;         // and their columns, with the page that is to be copied (-1: none)
+  pages::Column* columns;  // and their columns
   int n_old, n_new, max_pages, page_size, num_pages;
 };
 
 constexpr int kFound = 4096;  // children whose counts of wanted pages are kept in LDS
-// Beside a first child's count of wanted pages (kMostWanted at most): it copies a page that others held, who may all let go.
-constexpr int kCopiesShared = 1 << 30;
 constexpr int kCopied = INT_MIN;  // holders of a page that is copied from and free behind that, while pages are given
 
 // U entries a lane, 64 apart, on their way together; behind the end, which is past `at`, `none`.
@@ -204,12 +202,12 @@ __device__ __forceinline__ void fork_row(const ForkArgs& a, int c) {
       shared |= !elder && __builtin_amdgcn_ballot_w64(wants && j == whole && len % a.page_size) != 0;
       if (wants)
         a.columns[(size_t)c * a.max_pages + fresh + __builtin_popcountll(m & ((1ull << lane) - 1))] =
-            make_int2(j, j == whole && len % a.page_size ? v[u] : -1);
+            pages::Column{j, j == whole && len % a.page_size ? v[u] : -1};
       fresh += __builtin_popcountll(m);
     }
   }
   if (lane == 0) {
-    a.fresh[c] = fresh + (shared ? kCopiesShared : 0);
+    a.fresh[c] = fresh + (shared ? pages::kCopiesShared : 0);
     a.new_lens[c] = len;
     a.copies[2 * c] = -1;
     a.copies[2 * c + 1] = -1;
@@ -257,7 +255,7 @@ __device__ __forceinline__ void fork_refs(const ForkArgs& a, int p) {
 struct Find {  // in LDS
   int begin[kFound];   // of each child's wanted pages among all,
   int child[kFound];   // and, where no child wants two, whose the k-th is, and its column
-  int2 column[kFound];
+  pages::Column column[kFound];
   int part[2][16];
   int marked, listed;
 };
@@ -266,7 +264,7 @@ struct Find {  // in LDS
 __device__ __forceinline__ void fork_give(const ForkArgs& a, const Find& f, bool listed, const int* begin, int k,
                                           int page) {
   int c = 0;
-  int2 column;
+  pages::Column column;
   if (listed) {
     c = f.child[k];
     column = f.column[k];
@@ -275,11 +273,12 @@ __device__ __forceinline__ void fork_give(const ForkArgs& a, const Find& f, bool
       const int mid = (c + hi) / 2;
       if (begin[mid] <= k) c = mid; else hi = mid;
     }
-    column = a.columns[(size_t)c * a.max_pages + (k - begin[c])];
+    column = a.columns[(size_t)c * a.max_pages + pages::place_of(k, begin[c], a.max_pages)];
   }
-  a.new_tables[(size_t)c * a.max_pages + column.x] = page;
-  if (column.y >= 0) {
-    a.copies[2 * c] = column.y;
+  column = pages::checked(column, a.max_pages, a.num_pages);
+  if (column.at >= 0) a.new_tables[(size_t)c * a.max_pages + column.at] = page;
+  if (column.from >= 0) {
+    a.copies[2 * c] = column.from;
     a.copies[2 * c + 1] = page;
   }
 }
@@ -308,8 +307,10 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, Find& f) {
   long long wanted = 0;
   int turn = 0;
   for (int c0 = 0; c0 < a.n_new; c0 += 1024) {
-    const int c = c0 + threadIdx.x, noted = c < a.n_new ? a.fresh[c] : 0, mine = noted & (kCopiesShared - 1);
-    const int2 column = c < a.n_new ? a.columns[(size_t)c * a.max_pages] : make_int2(0, 0);  // if there is one
+    const int c = c0 + threadIdx.x, noted = c < a.n_new ? a.fresh[c] : 0;
+    const int mine = pages::wanted_of(noted, a.max_pages);
+    const pages::Column column =  // if there is one
+        c < a.n_new ? a.columns[(size_t)c * a.max_pages] : pages::Column{-1, -1};
     long long total;
     const long long before = block_scan(mine, f.part[turn ^= 1], &total);
     if (c < a.n_new) {
@@ -323,8 +324,9 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, Find& f) {
       if (mine > 1) f.listed = 0;
     }
     // sequences that were cut inside a page that they share: copied from, it is nobody's fresh page
-    if (noted & kCopiesShared) {
-      const int was = atomicCAS(&a.refs[column.y], 0, kCopied);
+    if (noted & pages::kCopiesShared) {
+      const int copied = pages::checked(column, a.max_pages, a.num_pages).from;
+      const int was = copied < 0 ? 1 : atomicCAS(&a.refs[copied], 0, kCopied);
       if (was == 0 || was == kCopied) f.marked = 1;
     }
     wanted += total;
@@ -631,7 +633,7 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   a.copies = copies;
   a.counts = counts;
   a.fresh = workspace;
-  a.columns = reinterpret_cast<int2*>(workspace + n_new + (n_new & 1));
+  a.columns = reinterpret_cast<pages::Column*>(workspace + n_new + (n_new & 1));
   a.n_old = n_old;
   a.n_new = n_new;
   a.max_pages = max_pages;

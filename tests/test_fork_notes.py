@@ -36,6 +36,48 @@ int main() {  // in: children and the pages that each wants; out: pages wanted i
 }
 """
 
+NOTES = r"""
+#include <cstdio>
+#include <random>
+#include "fork_notes.hpp"
+using namespace llmk::pages;
+int main() {  // whatever the workspace holds, what is read and written is the call's
+  std::mt19937 rng(5);
+  auto any = [&](long long lo, long long hi) { return (int)std::uniform_int_distribution<long long>(lo, hi)(rng); };
+  auto odd = [&](int a) {
+    switch (any(0, 3)) {
+      case 0: return any(a - 2LL, a + 2LL);
+      case 1: return any(-2, a);
+      case 2: return any(0, 1) == 0 ? (int)0x80000000 : 0x7FFFFFFF;
+      default: return any(-2147483648LL, 2147483647LL);
+    }
+  };
+  for (int turn = 0; turn < 2000000; ++turn) {
+    const int max_pages = any(0, 1) ? any(1, 9) : kMostWanted, num_pages = any(1, 30);
+    const int noted = odd(max_pages), wanted = wanted_of(noted, max_pages);
+    if (wanted < 0 || wanted > max_pages) return 1;
+    const Column c = checked({odd(max_pages), odd(num_pages)}, max_pages, num_pages);
+    if (c.at < -1 || c.at >= max_pages || c.from < -1 || c.from >= num_pages) return 2;
+    if (c.at < 0 && c.from >= 0) return 3;
+    const int at = place_of(any(0, num_pages - 1), odd(num_pages), max_pages);
+    if (at < 0 || at >= max_pages) return 4;
+  }
+  // what the steps themselves note stays as it is
+  for (int n : {0, 1, 5, kMostWanted})
+    for (int beside : {0, kCopiesShared})
+      if (wanted_of(n + beside, kMostWanted) != n) return 5;
+  for (int j = 0; j < 6; ++j)
+    for (int page = -1; page < 9; ++page) {
+      const Column c = checked({j, page}, 6, 9);
+      if (c.at != j || c.from != page) return 6;
+    }
+  for (int begin = 0; begin < 5; ++begin)
+    for (int k = begin; k < begin + 6; ++k)
+      if (place_of(k, begin, 6) != k - begin) return 7;
+  return 0;
+}
+"""
+
 
 def program(tmp_path, source):
     (tmp_path / "main.cpp").write_text(source)
@@ -53,3 +95,8 @@ def test_sums_past_32_bits(tmp_path):
         out = subprocess.run([run], input=" ".join(map(str, [len(wants), *wants])), capture_output=True, text=True,
                              check=True).stdout
         assert [int(x) for x in out.split()] == [sum(wants[:c]) for c in range(len(wants) + 1)]
+
+
+def test_notes_of_any_content_are_places_of_the_call(tmp_path):
+    r = subprocess.run([program(tmp_path, NOTES)])
+    assert r.returncode == 0
