@@ -296,7 +296,8 @@ __device__ __forceinline__ int free_bits(const ForkArgs& a, int p0) {
   return bits;
 }
 
-// Gives the free pages that are wanted, in order. One block of 1024 threads.
+// Gives the free pages that are wanted, in order. One block of 1024 threads. T: for sums of wanted pages.
+template <typename T>
 __device__ __forceinline__ void fork_find(const ForkArgs& a, Find& f) {
   const int* begin = a.n_new <= kFound ? f.begin : a.fresh;
   if (threadIdx.x == 0) {
@@ -304,17 +305,17 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, Find& f) {
     f.listed = a.n_new <= kFound;
   }
   int free = free_bits(a, 0);
-  long long wanted = 0;
+  T wanted = 0;
   int turn = 0;
   for (int c0 = 0; c0 < a.n_new; c0 += 1024) {
     const int c = c0 + threadIdx.x, noted = c < a.n_new ? a.fresh[c] : 0;
     const int mine = pages::wanted_of(noted, a.max_pages);
     const pages::Column column =  // if there is one
         c < a.n_new ? a.columns[(size_t)c * a.max_pages] : pages::Column{-1, -1};
-    long long total;
-    const long long before = block_scan(mine, f.part[turn ^= 1], &total);
+    T total;
+    const T before = block_scan(mine, f.part[turn ^= 1], &total);
     if (c < a.n_new) {
-      const long long at = wanted + before;
+      const T at = wanted + before;
       const int b = (int)(at < a.num_pages ? at : a.num_pages);
       if (a.n_new <= kFound) f.begin[c] = b; else a.fresh[c] = b;
       if (mine == 1 && at < kFound) {  // it is if no child wants two
@@ -353,9 +354,9 @@ __device__ __forceinline__ void fork_find(const ForkArgs& a, Find& f) {
     for (int p = threadIdx.x; p < a.num_pages; p += 1024) atomicCAS(&a.refs[p], kCopied, 0);
   }
   if (threadIdx.x == 0) {
-    const long long given = found < wanted ? found : wanted;
+    const T given = found < wanted ? found : wanted;
     a.counts[0] = (int)given;
-    a.counts[1] = (int)min(wanted - given, (long long)INT_MAX);
+    a.counts[1] = (int)min(wanted - given, (T)INT_MAX);
   }
 }
 
@@ -372,9 +373,9 @@ __global__ void __launch_bounds__(256) k_fork_refs(const ForkArgs a) {
 }
 __global__ void __launch_bounds__(1024) k_fork_find(const ForkArgs a) {
   __shared__ Find f;
-  fork_find(a, f);
+  fork_find<long long>(a, f);
 }
-// The three of them by one block. Its additions to counts are complete at the barrier and read where they were
+// The three of them by one block, whose batches want at most 8192 pages. Its additions to counts are complete at the barrier and read where they were
 // made, so no fence of the device is needed, which takes 5 us.
 __global__ void __launch_bounds__(1024) k_fork(const ForkArgs a) {
   __shared__ Find f;
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(1024) k_fork(const ForkArgs a) {
   __syncthreads();
   for (int p = wave; p < a.n_old; p += 16) fork_refs<1>(a, p);
   __syncthreads();
-  fork_find(a, f);
+  fork_find<int>(a, f);
 }
 
 // ---------------------------------------------------------------------------------------------
