@@ -1,4 +1,4 @@
-// What the steps of llmk_kv_fork count and leave one another. No device code: a program on the host may
+// What the steps of llmk_kv_fork and llmk_kv_compact count and leave one another. No device code: a program on the host may
 // include it.
 #pragma once
 
@@ -49,6 +49,10 @@ constexpr int place_of(int k, int begin, int max_pages) {
   const long long at = (long long)k - begin;
   return at < 0 ? 0 : at < max_pages ? (int)at : max_pages - 1;
 }
+
+// The same for llmk_kv_compact: its counts are added up from the workspace and pass through `counts`, ranks are
+// compared with them where they are used.
+constexpr int within(int n, int most) { return n < 0 ? 0 : n < most ? n : most; }
 
 }  // namespace pages
 }  // namespace llmk

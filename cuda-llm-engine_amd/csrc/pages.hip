@@ -421,6 +421,7 @@ __device__ __forceinline__ void compact_sums(const CompactArgs& a, int chunk, in
   }
   block_scan(all, part[0], n_live);
   block_scan(front, part[1], before);
+  *n_live = pages::within(*n_live, a.num_pages);
   const int edge = *n_live / kChunk;  // the chunk that page n_live lies in
   int below = 0;
   for (int i = threadIdx.x; i < edge; i += 1024) below += a.live[i];
@@ -456,6 +457,8 @@ __device__ __forceinline__ void compact_rank(const CompactArgs& a, int chunk, in
 __device__ __forceinline__ void compact_apply(const CompactArgs& a, int moved, int n_live, long long at,
                                               long long step) {
   const int most = a.num_pages / 2;
+  moved = pages::within(moved, most);
+  n_live = pages::within(n_live, a.num_pages);
   for (long long e = at; e < a.entries; e += step) {
     int p = a.tables[e];
     if (p >= n_live && p < a.num_pages) {

@@ -507,7 +507,8 @@ LLMK_API int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, in
  * given, and lacking (the table's row of a child that lacks some is then too short for L + reserve). refs is
  * brought up to date. n_new == 0 frees the old batch. No array that is written may overlap another
  * (LLMK_ERR_INVALID_VALUE).
- * workspace: llmk_kv_fork_workspace_ints(..) int32, 8-byte aligned. Batches up to 65535 sequences. */
+ * workspace: llmk_kv_fork_workspace_ints(..) int32, 8-byte aligned; calls that may overlap need one each, graphs
+ * replayed one behind the other may share one. Batches up to 65535 sequences. */
 LLMK_API size_t llmk_kv_fork_workspace_ints(int n_old, int n_new, int max_pages, int num_pages);
 LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
                           const int32_t* parents, const int32_t* reserve, int32_t* refs,
@@ -520,7 +521,7 @@ LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
  * that are no held page stay as they are), new_refs [num_pages] counts their holders; copies [num_pages / 2, 2]
  * gets the pairs (from, to), whose number is counts[0] (counts[1] = n), for llmk_kv_copy_pages. new_tables may be
  * block_tables, new_refs may be refs; other arrays may not overlap (LLMK_ERR_INVALID_VALUE). workspace:
- * llmk_kv_compact_workspace_ints(num_pages) int32. num_pages up to 2^24. */
+ * llmk_kv_compact_workspace_ints(num_pages) int32, as for llmk_kv_fork. num_pages up to 2^24. */
 LLMK_API size_t llmk_kv_compact_workspace_ints(int num_pages);
 LLMK_API int llmk_kv_compact(const int32_t* block_tables, const int32_t* refs, int32_t* new_tables,
                              int32_t* new_refs, int32_t* copies, int32_t* counts,

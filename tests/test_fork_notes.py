@@ -1,5 +1,5 @@
-"""What the steps of llmk_kv_fork count and leave one another (csrc/fork_notes.hpp): host code, compiled for the
-CPU; the kernels' uses of it are restated here."""
+"""What the steps of llmk_kv_fork and llmk_kv_compact count and leave one another (csrc/fork_notes.hpp): host code,
+compiled for the CPU; the kernels' uses of it are restated here."""
 import os
 import random
 import subprocess
@@ -78,6 +78,38 @@ int main() {  // whatever the workspace holds, what is read and written is the c
 }
 """
 
+COMPACT = r"""
+#include <cstdio>
+#include <random>
+#include "fork_notes.hpp"
+using namespace llmk::pages;
+int main() {  // the places that the steps read and write, whatever the workspace and the counts hold
+  std::mt19937 rng(6);
+  auto any = [&](long long lo, long long hi) { return (int)std::uniform_int_distribution<long long>(lo, hi)(rng); };
+  auto odd = [&](int a) {
+    switch (any(0, 3)) {
+      case 0: return any(a - 2LL, a + 2LL);
+      case 1: return any(-2, a);
+      case 2: return any(0, 1) == 0 ? (int)0x80000000 : 0x7FFFFFFF;
+      default: return any(-2147483648LL, 2147483647LL);
+    }
+  };
+  for (int turn = 0; turn < 2000000; ++turn) {
+    const int num_pages = any(0, 1) ? any(1, 20000) : any(1, 1 << 24), most = num_pages / 2;
+    const int chunks = (num_pages + 4095) / 4096;
+    const int edge = within(odd(num_pages), num_pages) / 4096;
+    if (edge < 0 || edge > chunks) return 1;  // sums of chunks below it; its own counts if it is below `chunks`
+    const int moved = within(odd(most), most), n_live = within(odd(num_pages), num_pages);
+    const int p = odd(num_pages), rank = odd(most);
+    if (p >= n_live && p < num_pages && p < 0) return 2;  // a table's entry becomes an address
+    if ((unsigned)rank < (unsigned)moved && (rank < 0 || rank >= most)) return 3;
+  }
+  for (int n = 0; n <= 9; ++n)
+    if (within(n, 9) != n) return 4;
+  return 0;
+}
+"""
+
 
 def program(tmp_path, source):
     (tmp_path / "main.cpp").write_text(source)
@@ -99,4 +131,9 @@ def test_sums_past_32_bits(tmp_path):
 
 def test_notes_of_any_content_are_places_of_the_call(tmp_path):
     r = subprocess.run([program(tmp_path, NOTES)])
+    assert r.returncode == 0
+
+
+def test_counts_of_any_content_are_places_of_the_call(tmp_path):
+    r = subprocess.run([program(tmp_path, COMPACT)])
     assert r.returncode == 0
