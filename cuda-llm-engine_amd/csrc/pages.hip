@@ -112,6 +112,7 @@ struct ForkArgs {
   int n_old, n_new, max_pages, page_size, num_pages;
 };
 
+constexpr int kMostPages = 1 << 30;  // k_fork_find looks at up to 8192 page numbers past the last
 constexpr int kFound = 4096;  // children whose counts of wanted pages are kept in LDS
 constexpr int kCopied = INT_MIN;  // holders of a page that is copied from and free behind that, while pages are given
 
@@ -613,7 +614,8 @@ extern "C" int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens
   if (!refs || !counts || !workspace || (n_old > 0 && (!block_tables || !seq_lens)) ||
       (n_new > 0 && (!parents || !new_tables || !new_lens || !copies)))
     return LLMK_ERR_INVALID_VALUE;
-  if (n_old > 65535 || n_new > 65535 || max_pages > pages::kMostWanted) return LLMK_ERR_UNSUPPORTED;
+  if (n_old > 65535 || n_new > 65535 || max_pages > pages::kMostWanted || num_pages > kMostPages)
+    return LLMK_ERR_UNSUPPORTED;
   {  // what is written, and what else there is
     const size_t n = n_new, m = n_old, width = max_pages;
     const int32_t* at[] = {refs,   new_tables, new_lens,     copies,   counts,

@@ -508,7 +508,8 @@ LLMK_API int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, in
  * brought up to date. n_new == 0 frees the old batch. No array that is written may overlap another
  * (LLMK_ERR_INVALID_VALUE).
  * workspace: llmk_kv_fork_workspace_ints(..) int32, 8-byte aligned; calls that may overlap need one each, graphs
- * replayed one behind the other may share one. Batches up to 65535 sequences. */
+ * replayed one behind the other may share one. Batches up to 65535 sequences, tables up to 2^24 pages
+ * wide, num_pages up to 2^30. */
 LLMK_API size_t llmk_kv_fork_workspace_ints(int n_old, int n_new, int max_pages, int num_pages);
 LLMK_API int llmk_kv_fork(const int32_t* block_tables, const int32_t* seq_lens,
                           const int32_t* parents, const int32_t* reserve, int32_t* refs,
