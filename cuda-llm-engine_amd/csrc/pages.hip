@@ -546,11 +546,13 @@ extern "C" int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, 
   if (n_pools < 0 || n_copies < 0 || num_pages <= 0) return LLMK_ERR_INVALID_VALUE;
   if (n_pools == 0 || n_copies == 0) return LLMK_OK;
   if (!pools || !page_bytes || !copies) return LLMK_ERR_INVALID_VALUE;
+  size_t all = 0;  // pieces of a pair in all pools
   for (int i = 0; i < n_pools; ++i) {
     if (!pools[i] || page_bytes[i] == 0) return LLMK_ERR_INVALID_VALUE;
     if (page_bytes[i] % 4) return LLMK_ERR_SHAPE;
     if (reinterpret_cast<uintptr_t>(pools[i]) % 4) return LLMK_ERR_ALIGNMENT;
     if (page_bytes[i] > ((size_t)1 << 32)) return LLMK_ERR_UNSUPPORTED;
+    all += (page_bytes[i] + kPiece - 1) / kPiece;
   }
   const auto whole = [&](int p) { return aligned16(pools[p]) && page_bytes[p] % 16 == 0; };
   // Many pairs are walked pool by pool, in whose order a compaction's lie in memory: 1024 pairs of 16 KB in 32 pools
@@ -561,41 +563,44 @@ extern "C" int llmk_kv_copy_pages(void* const* pools, const size_t* page_bytes, 
   size_t small = 0;
   for (int p = 0; p < n_pools && !small; ++p)
     if (whole(p) && page_bytes[p] <= 512) small = page_bytes[p];
-  for (int kind = 0; kind < 2; ++kind)  // whole vectors, then what is not
-    for (int i = 0; i < n_pools;) {
-      CopyArgs a{};
-      a.copies = copies;
-      a.count = count;
-      a.n_copies = n_copies;
-      a.num_pages = num_pages;
-      a.across = across;
-      int taken = 0;
-      const int begin = i;
-      for (; i < n_pools && taken < kPools; ++i) taken += whole(i) == (kind == 0);
-      if (taken == 0) break;
-      const auto is_small = [&](int p) { return kind == 0 && small && page_bytes[p] == small; };
-      for (int p = begin; p < i; ++p) {
-        if (whole(p) != (kind == 0) || is_small(p)) continue;
-        const int n = a.n_pools++;
-        a.pool[n] = static_cast<unsigned char*>(pools[p]);
-        a.bytes[n] = page_bytes[p];
-        a.first[n + 1] = a.first[n] + (int)((page_bytes[p] + kPiece - 1) / kPiece);
+  // where a launch might not take its blocks, all are counted before the first one
+  for (int pass = grid_takes((size_t)n_copies * ((all + 3) / 4), 256) ? 1 : 0; pass < 2; ++pass)
+    for (int kind = 0; kind < 2; ++kind)  // whole vectors, then what is not
+      for (int i = 0; i < n_pools;) {
+        CopyArgs a{};
+        a.copies = copies;
+        a.count = count;
+        a.n_copies = n_copies;
+        a.num_pages = num_pages;
+        a.across = across;
+        int taken = 0;
+        const int begin = i;
+        for (; i < n_pools && taken < kPools; ++i) taken += whole(i) == (kind == 0);
+        if (taken == 0) break;
+        const auto is_small = [&](int p) { return kind == 0 && small && page_bytes[p] == small; };
+        for (int p = begin; p < i; ++p) {
+          if (whole(p) != (kind == 0) || is_small(p)) continue;
+          const int n = a.n_pools++;
+          a.pool[n] = static_cast<unsigned char*>(pools[p]);
+          a.bytes[n] = page_bytes[p];
+          a.first[n + 1] = a.first[n] + (int)((page_bytes[p] + kPiece - 1) / kPiece);
+        }
+        for (int p = begin; p < i; ++p)
+          if (whole(p) && is_small(p)) a.pool[a.n_pools + a.n_small++] = static_cast<unsigned char*>(pools[p]);
+        a.small = a.n_small ? (int)small : 0;
+        size_t pieces = a.first[a.n_pools];
+        if (a.n_small) pieces += ceil_div(a.n_small, 64 / (a.small / 16));
+        a.slices = (int)((pieces + 3) / 4);
+        a.each = a.first[1];
+        for (int p = 0; p < a.n_pools; ++p)
+          if (a.first[p + 1] - a.first[p] != a.each) a.each = 0;
+        const size_t blocks = (size_t)n_copies * a.slices;
+        if (!grid_takes(blocks, 256)) return LLMK_ERR_UNSUPPORTED;
+        if (pass == 0) continue;
+        const int st = launch(kind == 0 ? k_copy_pages<true> : k_copy_pages<false>, dim3((unsigned)blocks),
+                              dim3(256), 0, static_cast<hipStream_t>(stream), a);
+        if (st != LLMK_OK) return st;
       }
-      for (int p = begin; p < i; ++p)
-        if (whole(p) && is_small(p)) a.pool[a.n_pools + a.n_small++] = static_cast<unsigned char*>(pools[p]);
-      a.small = a.n_small ? (int)small : 0;
-      size_t pieces = a.first[a.n_pools];
-      if (a.n_small) pieces += ceil_div(a.n_small, 64 / (a.small / 16));
-      a.slices = (int)((pieces + 3) / 4);
-      a.each = a.first[1];
-      for (int p = 0; p < a.n_pools; ++p)
-        if (a.first[p + 1] - a.first[p] != a.each) a.each = 0;
-      const size_t blocks = (size_t)n_copies * a.slices;
-      if (!grid_takes(blocks, 256)) return LLMK_ERR_UNSUPPORTED;
-      const int st = launch(kind == 0 ? k_copy_pages<true> : k_copy_pages<false>, dim3((unsigned)blocks), dim3(256),
-                            0, static_cast<hipStream_t>(stream), a);
-      if (st != LLMK_OK) return st;
-    }
   return LLMK_OK;
 }
 

@@ -1,8 +1,10 @@
 """Sizes past what the entry points for adapters, rotary layouts and shared pages take are refused as such, before any
 launch: at the C-ABI, on the CPU."""
+import ctypes
+
 import pytest
 
-from test_unlike_refusals import fork
+from test_unlike_refusals import FAKE, copy_pages, fork
 
 APART = dict(refs=1 << 42, new=1 << 36, ws=1 << 40, new_lens=1 << 44, copies=1 << 43, tables=1 << 45)
 
@@ -12,3 +14,13 @@ def test_kv_fork_pages(llmk, pages):
     """Page numbers are looked at some thousands past the last one: they have to stay below 2^31."""
     for n in (2, 300):
         assert fork(llmk.lib(), **APART, pages=pages, n_new=n) == llmk.LLMK_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("first,last", [(64, 1 << 32), (20, 1 << 32), (20, (1 << 32) - 4), (64, 1 << 31)])
+def test_kv_copy_pages_of_more_blocks_than_a_launch_takes(llmk, first, last):
+    """64 pools of small pages go in a launch of their own, those that are no whole vectors too: the call is refused
+    before the first one, and not behind it."""
+    pools = (ctypes.c_void_p * 65)(*[FAKE] * 65)
+    sizes = (ctypes.c_size_t * 65)(*[first] * 64, last)
+    for n in (256, 2 ** 31 - 1):
+        assert copy_pages(llmk.lib(), pools=pools, sizes=sizes, n=65, n_copies=n) == llmk.LLMK_ERR_UNSUPPORTED
