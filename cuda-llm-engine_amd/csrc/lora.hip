@@ -33,18 +33,17 @@
 #include <math.h>
 
 #include "kv8.hpp"
+#include "lora_plan.hpp"
 
 namespace llmk {
 namespace {
 
+using namespace lora;
+
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-constexpr int kParts = 8, kMaxRank = 256;
-constexpr int kWindow = 256, kHash = 512;
-constexpr int kRows = 16;   // of a tile
-constexpr int kNote = 32;   // ints of a tile's note: adapter (-1: no tile), rank, scale; from 16 on its rows (-1: none)
-constexpr int kChunk = 256;  // of in_features that a wave takes at a time
-constexpr int kWaves = 8;    // of a block of k_lora_whole
+constexpr int kHash = 512;
+constexpr int kNote = 32;  // ints of a tile's note: adapter (-1: no tile), rank, scale; from 16 on its rows (-1: none)
 
 struct LoraArgs {
   const f16 *x, *a, *b;
@@ -797,52 +796,6 @@ __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g)
   add_to_y<TILES>(old, y, all, stage[wave], lane);
 }
 
-// Blocks that k_lora_shrink is given if it has as many. 512: 3 prompts of 456 rows and rank 128 on 8192 -> 11008|11008
-// take 100 us and not 92, of rank 64 on 4096 -> 4096|1024|1024 42.7 and 41; the other cases as long.
-constexpr int kFill = 1024;
-
-// What a call takes of the chip and the workspace, by its sizes alone.
-struct Shape {
-  int groups, windows, slots, splits;
-  int at_once, turns;  // products of 16 ranks that a block of k_lora_shrink computes at a time, blocks that take turns
-};
-Shape shape_of(int n_rows, int n_seqs, int n_adapters, int in, int products) {
-  Shape s;
-  s.groups = n_seqs < kWindow ? n_seqs : kWindow;
-  if (n_adapters < s.groups) s.groups = n_adapters;
-  s.windows = (n_seqs + kWindow - 1) / kWindow;
-  s.slots = n_rows / kRows + s.windows * (s.groups + 1);
-  // one at a time where tiles are few: one row of rank 128 on 4096 -> 11008|11008 takes 13.5 us and not 14.2 with
-  // two, 32 rows of rank 16 on 8192 -> 4096|1024|1024 10.6 and not 11.9 with three; but 256 rows of 100 adapters of
-  // up to 64 29.2 and not 28.7, 3 prompts of 456 rows and rank 128 110 and not 89
-  s.at_once = products == 1 || s.slots * products <= 256 ? 1 : products == 3 ? 3 : 2;
-  // blocks for the products first, as long as kFill are not there, then for parts of in_features, whose sums every
-  // block of k_lora_expand has to add up
-  const int passes = (products + s.at_once - 1) / s.at_once, most = (in + 4 * kChunk - 1) / (4 * kChunk);
-  const int want = (kFill + s.slots - 1) / s.slots;
-  s.turns = want < passes ? want : passes;
-  s.splits = (kFill + s.slots * s.turns - 1) / (s.slots * s.turns);
-  if (s.splits > most) s.splits = most;
-  if (s.splits > 8) s.splits = 8;  // what k_lora_expand adds up
-  const int each = (most + s.splits - 1) / s.splits;
-  s.splits = (most + each - 1) / each;  // none idle at the end
-  return s;
-}
-
-// How many tiles there will be about if sequences choose among the adapters evenly, and if all choose another.
-struct Tiles {
-  int likely, many;
-};
-Tiles tiles_of(int n_rows, int n_seqs, int n_adapters, int windows, int groups) {
-  const double n = n_seqs < kWindow ? n_seqs : kWindow, rows = n_rows / (double)kRows, most = (double)windows * groups;
-  const double some = windows * n_adapters * (1.0 - pow(1.0 - 1.0 / n_adapters, n));
-  return {(int)fmax(some, rows + 0.5 * (some - 1)), (int)ceil(fmax(most, rows + 0.75 * (most - 1)))};
-}
-
-bool within_limits(int n_rows, int n_seqs, int max_rank, int in) {
-  return max_rank <= kMaxRank && n_rows <= (1 << 20) && n_seqs <= (1 << 20) && in <= (1 << 24);
-}
-
 // Whether n rows of `width` halves, ld apart, share some with n of `width2`, ld2 apart; columns of one matrix do not.
 bool rows_overlap(const uint16_t* a, int ld, int width, const uint16_t* b, int ld2, int width2, int n) {
   const long long d = ((long long)reinterpret_cast<uintptr_t>(b) - (long long)reinterpret_cast<uintptr_t>(a)) / 2;
@@ -876,20 +829,22 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   if (n_rows < 0 || n_seqs < 0 || n_adapters < 0 || max_rank <= 0 || in_features <= 0 ||
       n_parts < 1 || n_parts > kParts || !part_ends || (!row_starts && n_rows != n_seqs))
     return LLMK_ERR_INVALID_VALUE;
-  const int ks = max_rank <= 32 ? 1 : max_rank <= 64 ? 2 : max_rank <= 128 ? 4 : 8;
-  const int columns = ks <= 4 ? 512 : 256;  // of a block
   LoraArgs g{};
   for (int p = 0; p < n_parts; ++p) {
     const int begin = p ? part_ends[p - 1] : 0;
     if (part_ends[p] <= begin) return LLMK_ERR_INVALID_VALUE;
     if (part_ends[p] % 8) return LLMK_ERR_SHAPE;
     g.part_end[p] = part_ends[p];
-    g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) + (int)ceil_div(part_ends[p] - begin, columns);
   }
   if (in_features % 8 || max_rank % 8 || ldx % 8 || ldy % 8 || ldx < in_features ||
       ldy < part_ends[n_parts - 1])
     return LLMK_ERR_SHAPE;
-  if (!within_limits(n_rows, n_seqs, max_rank, in_features) || g.chunk_end[n_parts - 1] > 65535)
+  const auto chunks_of = [&](int columns) {  // blocks up to each part's end
+    for (int p = 0; p < n_parts; ++p)
+      g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) + over(part_ends[p] - (p ? part_ends[p - 1] : 0), columns);
+    return g.chunk_end[n_parts - 1];
+  };
+  if (!within_limits(n_rows, n_seqs, max_rank, in_features) || chunks_of(max_rank <= 128 ? 512 : 256) > 65535)
     return LLMK_ERR_UNSUPPORTED;
   if (n_rows == 0 || n_seqs == 0 || n_adapters == 0) return LLMK_OK;
   if (!x || !a || !b || !adapter_ids || !y || !workspace) return LLMK_ERR_INVALID_VALUE;
@@ -898,6 +853,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   if (rows_overlap(x, ldx, in_features, y, ldy, part_ends[n_parts - 1], n_rows)) return LLMK_ERR_INVALID_VALUE;
   const int per_part = (max_rank + 15) / 16;
   const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features, n_parts * per_part);
+  const Launches l = launches_of(s, n_rows, n_seqs, n_adapters, max_rank, in_features, part_ends, n_parts);
   g.x = reinterpret_cast<const f16*>(x);
   g.a = reinterpret_cast<const f16*>(a);
   g.b = reinterpret_cast<const f16*>(b);
@@ -922,58 +878,30 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   g.groups = s.groups;
   g.windows = s.windows;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  const int chunks = g.chunk_end[n_parts - 1];
-  // Both products in one launch, if a block's own h costs it little, 32 ranks at most and few enough numbers of A and
-  // x, and if its blocks are expected to run at once: one a CU, 32 an XCD. Columns a block: 256, 512 or 1024, the
-  // fewest with which they do. 300 rows of one adapter of rank 16 on 1024 -> 6144 take 7.9 us and 9.0 in two launches
-  // (12.0 if a third of an XCD's blocks waits for the others), on 11008|11008 20.0 so and 15.9. 16 ranks and 2048
-  // columns of one sequence take 5.9 us with 4096 in_features and 7.8 with 8192, where two launches take 8.1; 16
-  // sequences' on 1000 columns 9.4 and 10.8, but one sequence of 16 rows 9.9 and 8.9, and 32 sequences of 4 adapters
-  // 11.0 and 9.9: there x counts as much as A. At 32 ranks 8 sequences on 4096 -> 4096|1024|1024 take 9.5 and 11.3, 4
-  // of 16 rows on 8192|8192, 1024 columns a block, 12.4 and 10.6. A launch more is 2 us of the host's time, too.
-  // The columns are chosen for many tiles, as too few of them cost more: 48 sequences of up to 5 rows, 16 adapters,
-  // 4096 -> 4096|1024|1024, 11.2 us with 1024 and 14.6 with 512, of which a third has to wait on some XCDs.
-  const Tiles used = tiles_of(n_rows, n_seqs, n_adapters, s.windows, s.groups);
-  int tiles = 2, blocks = 0;
-  const auto fits = [&](long long n) { return g.per_block ? (n + 7) / 8 * blocks <= 32 : n * blocks <= 256; };
-  for (;; tiles *= 2) {
-    blocks = 0;
-    for (int p = 0; p < n_parts; ++p)
-      blocks += (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
-    g.per_block = s.slots >= 8 || blocks <= 32;  // whether a tile's blocks share an XCD
-    if (tiles == 8 || fits(used.many)) break;
+  if (l.one) {
+    g.per_block = l.together;
+    chunks_of(16 * kWaves * l.tiles);
+    return launch(per_part == 1 ? (l.tiles == 2   ? k_lora_whole<2, 1>
+                                   : l.tiles == 4 ? k_lora_whole<4, 1>
+                                                  : k_lora_whole<8, 1>)
+                                : (l.tiles == 2   ? k_lora_whole<2, 2>
+                                   : l.tiles == 4 ? k_lora_whole<4, 2>
+                                                  : k_lora_whole<8, 2>),
+                  dim3((unsigned)l.grid), dim3(64 * kWaves), 0, st, g);
   }
-  const size_t most = per_part == 1 && n_rows < 8 * s.groups ? 16384 : tiles == 8 ? 10240 : 12288;
-  if (fits(used.likely) && ks == 1 && (per_part + 1) * (size_t)in_features <= most) {
-    for (int p = 0; p < n_parts; ++p)
-      g.chunk_end[p] = (p ? g.chunk_end[p - 1] : 0) +
-                       (int)ceil_div(part_ends[p] - (p ? part_ends[p - 1] : 0), 16 * kWaves * tiles);
-    const dim3 grid((g.per_block ? (s.slots + 7) / 8 * 8 : s.slots) * blocks), threads(64 * kWaves);
-    return launch(per_part == 1 ? (tiles == 2   ? k_lora_whole<2, 1>
-                                   : tiles == 4 ? k_lora_whole<4, 1>
-                                                : k_lora_whole<8, 1>)
-                                : (tiles == 2   ? k_lora_whole<2, 2>
-                                   : tiles == 4 ? k_lora_whole<4, 2>
-                                                : k_lora_whole<8, 2>),
-                  grid, threads, 0, st, g);
-  }
-  // as many tiles a block as leave 2048 blocks, or 512 past 32 ranks, where B is more than y: 2 prompts of 900 rows and
-  // rank 64 on 8192|8192 columns take 32 us, and 40 with 2048
-  g.per_block = 1;
-  while (g.per_block < 16 && (long long)s.slots * chunks / (2 * g.per_block) >= (ks == 1 ? 2048 : 512))
-    g.per_block *= 2;
-  if (!grid_takes((size_t)chunks * ceil_div(s.slots, g.per_block), 256)) return LLMK_ERR_UNSUPPORTED;
+  if (!grid_takes(l.grid2, 256)) return LLMK_ERR_UNSUPPORTED;
+  g.per_block = l.per_block;
   g.turns = s.turns;
   const int status = launch(s.at_once == 1   ? k_lora_shrink<1>
                             : s.at_once == 3 ? k_lora_shrink<3>
                                              : k_lora_shrink<2>,
-                            dim3(s.splits * s.slots * s.turns), dim3(256), 0, st, g);
+                            dim3((unsigned)l.grid), dim3(256), 0, st, g);
   if (status != LLMK_OK) return status;
-  const dim3 grid(chunks * ceil_div(s.slots, g.per_block));  // fits: checked in front of the first launch
+  const dim3 grid((unsigned)l.grid2);  // fits: checked in front of the first launch
   const bool many = s.splits > 2;
-  return launch(ks == 1   ? (many ? k_lora_expand<1, true> : k_lora_expand<1, false>)
-                : ks == 2 ? (many ? k_lora_expand<2, true> : k_lora_expand<2, false>)
-                : ks == 4 ? k_lora_expand_high<4>
-                          : k_lora_expand_high<8>,
+  return launch(l.steps == 1   ? (many ? k_lora_expand<1, true> : k_lora_expand<1, false>)
+                : l.steps == 2 ? (many ? k_lora_expand<2, true> : k_lora_expand<2, false>)
+                : l.steps == 4 ? k_lora_expand_high<4>
+                               : k_lora_expand_high<8>,
                 grid, dim3(256), 0, st, g);
 }
