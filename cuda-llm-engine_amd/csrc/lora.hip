@@ -889,7 +889,6 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
                                                   : k_lora_whole<8, 2>),
                   dim3((unsigned)l.grid), dim3(64 * kWaves), 0, st, g);
   }
-  if (!grid_takes(l.grid2, 256)) return LLMK_ERR_UNSUPPORTED;
   g.per_block = l.per_block;
   g.turns = s.turns;
   const int status = launch(s.at_once == 1   ? k_lora_shrink<1>
@@ -897,7 +896,7 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
                                              : k_lora_shrink<2>,
                             dim3((unsigned)l.grid), dim3(256), 0, st, g);
   if (status != LLMK_OK) return status;
-  const dim3 grid((unsigned)l.grid2);  // fits: checked in front of the first launch
+  const dim3 grid((unsigned)l.grid2);
   const bool many = s.splits > 2;
   return launch(l.steps == 1   ? (many ? k_lora_expand<1, true> : k_lora_expand<1, false>)
                 : l.steps == 2 ? (many ? k_lora_expand<2, true> : k_lora_expand<2, false>)

@@ -17,6 +17,8 @@ constexpr int kWaves = 8;     // of a block of k_lora_whole
 // take 100 us and not 92, of rank 64 on 4096 -> 4096|1024|1024 42.7 and 41; the other cases as long.
 constexpr int kFill = 1024;
 
+constexpr int kMostBlocks = (1 << 24) - 1;  // of 256 threads, which a launch counts in 32 bits
+
 inline int over(long long a, long long b) { return (int)((a + b - 1) / b); }
 
 inline bool within_limits(int n_rows, int n_seqs, int max_rank, int in) {
@@ -113,6 +115,7 @@ inline Launches launches_of(const Shape& s, int n_rows, int n_seqs, int n_adapte
   l.per_block = 1;
   while (l.per_block < 16 && (long long)s.slots * chunks / (2 * l.per_block) >= (l.steps == 1 ? 2048 : 512))
     l.per_block *= 2;
+  while ((size_t)chunks * over(s.slots, l.per_block) > kMostBlocks) l.per_block *= 2;  // ends: chunks are 65535 at most
   l.grid2 = (size_t)chunks * over(s.slots, l.per_block);
   return l;
 }

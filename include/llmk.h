@@ -412,8 +412,8 @@ LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_lo
  * overlap (LLMK_ERR_INVALID_VALUE); they may be columns of one matrix.
  * workspace: llmk_lora_add_workspace_floats(..) floats, 16-byte aligned; calls that may overlap need
  * one each, graphs replayed one behind the other may share one. LLMK_ERR_UNSUPPORTED, before any launch, for more
- * than 2^20 rows or sequences, 2^24 in_features or 65535 * 512 columns (half for ranks past 128), or rows times
- * columns past 2^38. */
+ * than 2^20 rows or sequences, 2^24 in_features, or 65535 blocks of 512 columns (256 for ranks past 128), of which
+ * a part's last one counts as whole. */
 LLMK_API size_t llmk_lora_add_workspace_floats(int n_rows, int n_seqs, int n_adapters, int max_rank,
                                                int in_features, int n_parts);
 LLMK_API int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, const uint16_t* b,

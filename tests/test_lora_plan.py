@@ -30,7 +30,9 @@ LARGEST = [(MOST, MOST, 1 << 19, 16, 64, (8192,)), (MOST, MOST, 1 << 19, 16, 64,
            (MOST, MOST, (1 << 31) - 1, 8, 8, (131072,)), (MOST, MOST, 1 << 20, 256, 1 << 24, (8, 16)),
            (1, MOST, 1 << 30, 32, 64, (4096, 8192)), (MOST, 1, 1, 8, 8, (8,)), (1, 1, 1, 8, 8, (8,)),
            (MOST, MOST, 256, 8, 64, (1024,)), (300000, 300000, 12000000, 16, 512, (2048,)),
-           (1, 1, 49, 16, 64, (1 << 20,)), (1, 1, 2 ** 31 - 1, 16, 64, (1 << 20,))]
+           (1, 1, 49, 16, 64, (1 << 20,)), (1, 1, 2 ** 31 - 1, 16, 64, (1 << 20,)),
+           (MOST, MOST, 256, 16, 64, (1 << 17,)), (MOST, MOST, 256, 256, 64, (1 << 16,)),
+           (MOST, MOST, 256, 128, 64, (65535 * 512,)), (MOST, MOST, 256, 136, 64, (65535 * 256,))]
 
 
 @pytest.mark.parametrize("calls", [LARGEST, drawn(1, 4000)], ids=["largest", "drawn"])
@@ -52,4 +54,4 @@ def test_estimates_and_grids(tmp_path, calls):
         else:
             assert p["grid"] == p["slots"] * p["splits"] * p["turns"] < 2 ** 32 // 256
             chunks = sum(-(-w // (512 if rank <= 128 else 256)) for w in widths)
-            assert p["grid2"] == chunks * -(-p["slots"] // p["per_block"])
+            assert p["grid2"] == chunks * -(-p["slots"] // p["per_block"]) < 2 ** 32 // 256

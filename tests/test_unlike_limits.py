@@ -4,7 +4,7 @@ import ctypes
 
 import pytest
 
-from test_unlike_refusals import FAKE, copy_pages, fork
+from test_unlike_refusals import FAKE, MIS, copy_pages, fork, ints, lora
 
 APART = dict(refs=1 << 42, new=1 << 36, ws=1 << 40, new_lens=1 << 44, copies=1 << 43, tables=1 << 45)
 
@@ -24,3 +24,12 @@ def test_kv_copy_pages_of_more_blocks_than_a_launch_takes(llmk, first, last):
     sizes = (ctypes.c_size_t * 65)(*[first] * 64, last)
     for n in (256, 2 ** 31 - 1):
         assert copy_pages(llmk.lib(), pools=pools, sizes=sizes, n=65, n_copies=n) == llmk.LLMK_ERR_UNSUPPORTED
+
+
+@pytest.mark.parametrize("rank,most", [(16, 65535 * 512), (128, 65535 * 512), (136, 65535 * 256), (256, 65535 * 256)])
+def test_lora_add_columns(llmk, rank, most):
+    """Refused by the columns alone: a misaligned x of a call that is not shows that these are not refused for it."""
+    for n in (4, 1 << 20):
+        sizes = dict(rank=rank, n_rows=n, n_seqs=n, parts=1, x=MIS)
+        for columns, status in ((most, llmk.LLMK_ERR_ALIGNMENT), (most + 8, llmk.LLMK_ERR_UNSUPPORTED)):
+            assert lora(llmk.lib(), **sizes, ends=ints(columns), ldy=columns) == status
