@@ -435,11 +435,23 @@ __device__ __forceinline__ float split_h(const float (&v)[KS][8], f16x8 (&hi)[KS
   return up;
 }
 
+// v with its infinities and NaN as 0.
+__device__ __forceinline__ u32x4 finite_of(u32x4 v) {
+  f16x8 x = as_h8(v);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = __builtin_fabsf((float)x[e]) < INFINITY ? x[e] : (f16)0;
+  return as_u4(x);
+}
+
 // B h of a wave's 16 rows and 16 * TILES columns: row n, columns 32 t + 8 q on of each pair of products, into LDS
-// (in pieces of 16 bytes as above); and what the row's are to be multiplied by, behind them.
-template <int KS, int TILES>
+// (in pieces of 16 bytes as above); and what the row's are to be multiplied by, behind them. Where a sum is no number
+// it is made again, the lower halves of h by B's finite numbers alone: an infinity of B times a lower half, which may be
+// 0 or of the other sign, is NaN, and the product's is an infinity. h_of: the halves of h once more.
+template <int KS, int TILES, typename H>
 __device__ __forceinline__ void expand_columns(const u32x4 (&bf)[TILES][KS], const f16x8 (&hi)[KS],
-                                               const f16x8 (&lo)[KS], float by, u32x4* to, int n, int q) {
+                                               const f16x8 (&lo)[KS], float by, u32x4* to, int n, int q, H h_of) {
+  const auto place = [&](int t) { return n * 4 * TILES + ((8 * (t / 2) + 2 * q + (t & 1)) ^ (n & (4 * TILES - 1))); };
+  bool none = false;
 #pragma unroll
   for (int t = 0; t < TILES; ++t) {
     f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -448,8 +460,25 @@ __device__ __forceinline__ void expand_columns(const u32x4 (&bf)[TILES][KS], con
       d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[t][s]), hi[s], d, 0, 0, 0);
       d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[t][s]), lo[s], d, 0, 0, 0);
     }
-    to[n * 4 * TILES + ((8 * (t / 2) + 2 * q + (t & 1)) ^ (n & (4 * TILES - 1)))] =
-        __builtin_bit_cast(u32x4, d);
+    to[place(t)] = __builtin_bit_cast(u32x4, d);
+    const float sum = (d[0] + d[1]) + (d[2] + d[3]);
+    none |= sum != sum;
+  }
+  if (__builtin_amdgcn_ballot_w64(none)) {
+    wave_sync();
+#pragma unroll
+    for (int t = 0; t < TILES; ++t) {
+      f32x4 d = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        f16x8 high, low;
+        __builtin_amdgcn_sched_barrier(0);  // one step's at a time
+        h_of(s, high, low);
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(bf[t][s]), high, d, 0, 0, 0);
+        d = __builtin_amdgcn_mfma_f32_16x16x32_f16(as_h8(finite_of(bf[t][s])), low, d, 0, 0, 0);
+      }
+      to[place(t)] = __builtin_bit_cast(u32x4, d);
+    }
   }
   if (q == 0) reinterpret_cast<float*>(to + kRows * 4 * TILES)[n] = by;
 }
@@ -604,8 +633,9 @@ __global__ void __launch_bounds__(256, KS == 1 ? 3 : 2) k_lora_expand(const Lora
     if (fresh) cut_b<KS, TILES>(bf, rank, q);
     f16x8 hi[KS], lo[KS];
     const float by = scale * split_h<KS>(h, hi, lo);
+    const auto of_registers = [&](int s, f16x8& high, f16x8& low) { high = hi[s], low = lo[s]; };
     wave_sync();
-    expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q);
+    expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q, of_registers);
     wave_sync();
     add_to_y<TILES>(old, y, all, stage[wave], lane);
   }
@@ -715,7 +745,10 @@ __global__ void __launch_bounds__(256, 2) k_lora_expand_high(const LoraArgs g) {
       lo[s] = as_h8(pair[s][1][lane]);
     }
     wave_sync();
-    expand_columns<KS, TILES>(bf, hi, lo, scale * up, stage[wave], n, q);
+    expand_columns<KS, TILES>(bf, hi, lo, scale * up, stage[wave], n, q, [&](int s, f16x8& high, f16x8& low) {
+      high = as_h8(pair[s][0][lane]);  // held in registers since the first time, they would not fit
+      low = as_h8(pair[s][1][lane]);
+    });
     wave_sync();
     add_to_y<TILES>(old, y, all, stage[wave], lane);
   }
@@ -767,6 +800,7 @@ __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g)
   // in_features, 5.9 and 6.7 on 4096, tiles of 16 rows as long as before; with two, which leave fewer registers, 12.3
   // and 11.4.
   const int n_x = (__builtin_popcountll(__builtin_amdgcn_ballot_w64(lane < kRows && p.row[lane % kRows] >= 0)) + 1) / 2;
+  const int has = p.row[n] >= 0 ? rank : 0;  // the values of a row that is none may be anything
   shrink_chunks<NG, NG == 1>(acc, g, xrow, w, left, (rank + 15) / 16, wave, kWaves, stage[wave], lane, n_x);
 #pragma unroll
   for (int i = 0; i < NG; ++i) stage[wave][i * 64 + lane] = __builtin_bit_cast(u32x4, acc[i]);
@@ -785,13 +819,14 @@ __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g)
 #pragma unroll
         for (int m = 0; m < d; ++m) v[m] += v[m + d];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) h[s][4 * f + e] = 32 * s + 8 * q + 4 * f + e < rank ? v[0][e] : 0.f;
+      for (int e = 0; e < 4; ++e) h[s][4 * f + e] = 32 * s + 8 * q + 4 * f + e < has ? v[0][e] : 0.f;
     }
   cut_b<KS, TILES>(bf, rank, q);
   f16x8 hi[KS], lo[KS];
   const float by = tile.scale * split_h<KS>(h, hi, lo);
+  const auto of_registers = [&](int s, f16x8& high, f16x8& low) { high = hi[s], low = lo[s]; };
   lds_barrier();  // the other waves have read what this one puts its columns over
-  expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q);
+  expand_columns<KS, TILES>(bf, hi, lo, by, stage[wave], n, q, of_registers);
   wave_sync();
   add_to_y<TILES>(old, y, all, stage[wave], lane);
 }
