@@ -447,7 +447,8 @@ LLMK_API int llmk_rotary_apply(uint16_t* q, int ldq, uint16_t* k, int ldk, const
  * q, k and v as for llmk_qkv_rope_scatter; q goes to q_out [n, n_heads, head_dim], k (rotated) and v to the
  * pools [num_pages, page_size, n_kv_heads, head_dim] at positions[r] by block_tables[r, :] [n, max_pages].
  * Rows whose position is below 0 or past the table, or whose table entry is negative, write no k and v.
- * head_dim % 16 == 0, up to 512; rotary_dim % 16 == 0; ld % 8 == 0; qkv, q_out and the pools 16-byte aligned and
+ * head_dim % 16 == 0, up to 512; rotary_dim % 16 == 0, or even and a whole fraction of head_dim (20 or 40 of heads of
+ * 80); ld % 8 == 0; qkv, q_out and the pools 16-byte aligned and
  * not overlapping (q_out and qkv: LLMK_ERR_INVALID_VALUE). */
 LLMK_API int llmk_qkv_rotary_scatter(const uint16_t* qkv, int ld, uint16_t* q_out, uint16_t* k_pool,
                                      uint16_t* v_pool, const int32_t* block_tables,

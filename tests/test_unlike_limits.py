@@ -4,7 +4,7 @@ import ctypes
 
 import pytest
 
-from test_unlike_refusals import FAKE, MIS, copy_pages, fork, ints, lora
+from test_unlike_refusals import FAKE, MIS, copy_pages, fork, ints, lora, scatter
 
 APART = dict(refs=1 << 42, new=1 << 36, ws=1 << 40, new_lens=1 << 44, copies=1 << 43, tables=1 << 45)
 
@@ -33,3 +33,12 @@ def test_lora_add_columns(llmk, rank, most):
         sizes = dict(rank=rank, n_rows=n, n_seqs=n, parts=1, x=MIS)
         for columns, status in ((most, llmk.LLMK_ERR_ALIGNMENT), (most + 8, llmk.LLMK_ERR_UNSUPPORTED)):
             assert lora(llmk.lib(), **sizes, ends=ints(columns), ldy=columns) == status
+
+
+def test_qkv_rotary_scatter_parts_of_a_head(llmk):
+    """Multiples of 16, and even whole fractions of the head; a misaligned q shows that they are not refused as shapes."""
+    for dim, rot, status in ((80, 20, 0), (80, 40, 0), (80, 16, 0), (64, 2, 0), (64, 24, 1), (80, 60, 1), (80, 5, 1), (16, 1, 1),
+                             (80, 160, 1), (64, 6, 1)):
+        want = llmk.LLMK_ERR_SHAPE if status else llmk.LLMK_ERR_ALIGNMENT
+        assert scatter(llmk.lib(), dim=dim, rot=rot, ld=8 * dim, q=MIS) == want, (dim, rot)
+        assert scatter(llmk.lib(), dim=dim, rot=rot, ld=8 * dim, n=0) == (llmk.LLMK_ERR_SHAPE if status else 0), (dim, rot)
