@@ -34,6 +34,7 @@
 
 #include "kv8.hpp"
 #include "lora_plan.hpp"
+#include "overlap.hpp"
 
 namespace llmk {
 namespace {
@@ -831,14 +832,8 @@ __global__ void __launch_bounds__(64 * kWaves, 1) k_lora_whole(const LoraArgs g)
   add_to_y<TILES>(old, y, all, stage[wave], lane);
 }
 
-// Whether n rows of `width` halves, ld apart, share some with n of `width2`, ld2 apart; columns of one matrix do not.
-bool rows_overlap(const uint16_t* a, int ld, int width, const uint16_t* b, int ld2, int width2, int n) {
-  const long long d = ((long long)reinterpret_cast<uintptr_t>(b) - (long long)reinterpret_cast<uintptr_t>(a)) / 2;
-  if (d >= (long long)(n - 1) * ld + width || -d >= (long long)(n - 1) * ld2 + width2) return false;
-  if (ld != ld2) return true;
-  const long long at = (d % ld + ld) % ld;  // of b's columns among a's
-  return at < width || at + width2 > ld;
-}
+// Elements of an array of so many by so many by .., which a call may name more of than any memory holds.
+long long elements(double a, double b, double c = 1, double d = 1) { return (long long)fmin(a * b * c * d, 1e18); }
 
 }  // namespace
 }  // namespace llmk
@@ -885,7 +880,24 @@ extern "C" int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, cons
   if (!x || !a || !b || !adapter_ids || !y || !workspace) return LLMK_ERR_INVALID_VALUE;
   if (!aligned16(x) || !aligned16(a) || !aligned16(b) || !aligned16(y) || !aligned16(workspace))
     return LLMK_ERR_ALIGNMENT;
-  if (rows_overlap(x, ldx, in_features, y, ldy, part_ends[n_parts - 1], n_rows)) return LLMK_ERR_INVALID_VALUE;
+  {  // what is written, and what else there is
+    const long long out = part_ends[n_parts - 1];
+    const Rows written[] = {
+        rows_of(y, n_rows, ldy, out),
+        bytes_of(workspace, 4 * llmk_lora_add_workspace_floats(n_rows, n_seqs, n_adapters, max_rank, in_features, n_parts))};
+    const auto array = [](const void* p, long long n) { return rows_of(p, 1, 0, n); };  // n elements of 2 bytes
+    const Rows others[] = {rows_of(x, n_rows, ldx, in_features),
+                           array(a, elements(n_adapters, n_parts, max_rank, in_features)),
+                           array(b, elements(n_adapters, out, max_rank)),
+                           array(ranks, 2LL * n_adapters),
+                           array(scales, 2LL * n_adapters),
+                           array(adapter_ids, 2LL * n_seqs),
+                           array(row_starts, 2LL * n_seqs + 2)};
+    if (overlap(written[0], written[1])) return LLMK_ERR_INVALID_VALUE;
+    for (const Rows& w : written)
+      for (const Rows& o : others)
+        if (overlap(w, o)) return LLMK_ERR_INVALID_VALUE;
+  }
   const int per_part = (max_rank + 15) / 16;
   const Shape s = shape_of(n_rows, n_seqs, n_adapters, in_features, n_parts * per_part);
   const Launches l = launches_of(s, n_rows, n_seqs, n_adapters, max_rank, in_features, part_ends, n_parts);

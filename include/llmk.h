@@ -408,8 +408,9 @@ LLMK_API int llmk_verify_drafts(const uint16_t* logits, const uint16_t* draft_lo
  * for bit; a row depends on its own x, y and adapter alone. Sums in fp32; between the two products 22
  * bits of a row's values relative to its largest one of the part; one rounding.
  * x rows have stride ldx and y rows ldy (elements, multiples of 8); in_features, max_rank (at most
- * 256) and the part ends are multiples of 8; x, a, b and y are 16-byte aligned. Rows of x and y may not
- * overlap (LLMK_ERR_INVALID_VALUE); they may be columns of one matrix.
+ * 256) and the part ends are multiples of 8; x, a, b and y are 16-byte aligned. What is written, y's
+ * rows and the workspace, may not overlap each other nor another array (LLMK_ERR_INVALID_VALUE); x and y may be columns
+ * of one matrix.
  * workspace: llmk_lora_add_workspace_floats(..) floats, 16-byte aligned; calls that may overlap need
  * one each, graphs replayed one behind the other may share one. LLMK_ERR_UNSUPPORTED, before any launch, for more
  * than 2^20 rows or sequences, 2^24 in_features, or 65535 blocks of 512 columns (256 for ranks past 128), of which
