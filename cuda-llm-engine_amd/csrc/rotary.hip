@@ -17,6 +17,7 @@
 // heads of 128 into the cache 10.2 (6.2: 37 MB, of which a plain copy takes 7).
 #include "angles.hpp"
 #include "layer_ops.hpp"
+#include "overlap.hpp"
 
 namespace llmk {
 namespace {
@@ -307,6 +308,9 @@ extern "C" int llmk_rotary_apply(uint16_t* q, int ldq, uint16_t* k, int ldk, con
   const int st = check_turn(inv_freq, positions, rotary_dim, n_tables, layout);
   if (st != LLMK_OK) return st;
   if (head_dim > 4096) return LLMK_ERR_UNSUPPORTED;
+  const Rows turned_q{reinterpret_cast<uintptr_t>(q), n_rows, ldq, n_heads, head_dim, rotary_dim};
+  const Rows turned_k{reinterpret_cast<uintptr_t>(k), n_rows, ldk, n_kv_heads, head_dim, rotary_dim};
+  if (n_heads > 0 && n_kv_heads > 0 && overlap(turned_q, turned_k)) return LLMK_ERR_INVALID_VALUE;
   RotaryArgs a{};
   a.q = a.q_out = reinterpret_cast<f16*>(q);
   a.k = a.k_out = reinterpret_cast<f16*>(k);

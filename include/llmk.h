@@ -431,7 +431,8 @@ LLMK_API int llmk_lora_add(const uint16_t* x, int ldx, const uint16_t* a, const 
 
 /* Rotates the first rotary_dim elements of every head of q and k where they lie; the rest of a head is
  * neither read nor written. Row r of q (stride ldq elements) holds n_heads heads of head_dim, row r of k
- * (stride ldk) n_kv_heads; they may be columns of one fused projection. With t = table_ids[r], the angle
+ * (stride ldk) n_kv_heads; they may be columns of one fused projection, and what is rotated of q and k may not overlap
+ * (LLMK_ERR_INVALID_VALUE). With t = table_ids[r], the angle
  * of pair i is positions[r] * inv_freq[t, i] and
  *   x1' = fp16(scales[t] (x1 cos - x2 sin)), x2' = fp16(scales[t] (x2 cos + x1 sin)):
  * angles, cosines and sines in 64 bits, products in 32, one rounding. inv_freq [n_tables, rotary_dim / 2],

@@ -2,7 +2,7 @@
 the C-ABI, on the CPU: no call gets as far as a launch."""
 import pytest
 
-from test_unlike_refusals import ints, lora
+from test_unlike_refusals import ints, lora, rotary
 
 AT = 1 << 24
 
@@ -40,3 +40,13 @@ def test_lora_add_over_a_row_of_y(llmk, behind):
     """B of 64 numbers at a row's last columns, and reaching into the next row."""
     wide = dict(ldy=4096, n_adapters=1, rank=8, ends=ints(8), parts=1)
     assert lora(llmk.lib(), **APART | wide | dict(b=APART["y"] + 2 * behind)) == llmk.LLMK_ERR_INVALID_VALUE
+
+
+@pytest.mark.parametrize("behind,sizes", [
+    (0, {}), (2 * 31, {}), (2 * 4 * 256 - 2 * 128, {}), (-2 * 64, {}), (-2 * 95, {}),  # heads of 64, of which 32 turn
+    (2 * (3 * 256 + 3 * 64 + 31), dict(n=5)), (2 * 200, dict(ldk=136)), (2 * 3 * 256, dict(heads=1, kv=1, ldk=64)),
+    (2 * (512 - 64), dict(ldq=512, ldk=512)), (2 * 40, dict(rot=64)), (-2 * 3 * 256, dict(ldk=256))])
+def test_rotary_apply_q_over_k(llmk, behind, sizes):
+    """What one head's turned part shares with another's, in the same row, in the next, or across strides."""
+    a = dict(n=4, ldq=256, ldk=256, q=AT, k=AT + behind) | sizes
+    assert rotary(llmk.lib(), **a) == llmk.LLMK_ERR_INVALID_VALUE
