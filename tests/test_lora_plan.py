@@ -5,6 +5,7 @@ import random
 import pytest
 
 from _lora_plan import plans
+from _lora_variants import SIZES, Sizes
 
 MOST = 1 << 20
 
@@ -55,3 +56,27 @@ def test_estimates_and_grids(tmp_path, calls):
             assert p["grid"] == p["slots"] * p["splits"] * p["turns"] < 2 ** 32 // 256
             chunks = sum(-(-w // (512 if rank <= 128 else 256)) for w in widths)
             assert p["grid2"] == chunks * -(-p["slots"] // p["per_block"]) < 2 ** 32 // 256
+
+
+def test_the_gpu_tests_take_every_way(tmp_path):
+    """The cases of _lora_variants.py between them run every kernel of lora_add in every manner that the sizes choose."""
+    calls = [Sizes(i).call() for i in range(len(SIZES))]
+    one, two = set(), set()
+    for (rows, seqs, adapters, rank, inner, ends), p in zip(calls, plans(tmp_path, calls), strict=True):
+        if p["one"]:
+            one |= {(p["tiles"], (rank + 15) // 16), ("together", p["together"]), ("wave", seqs <= 64)}
+            one |= {("together", p["tiles"], p["together"])}
+        else:
+            some, run = p["splits"], p["per_block"] > 1
+            two |= {("at once", p["at_once"]), ("turns", p["turns"] > 1), ("wave", seqs <= 64), ("windows", p["windows"] > 1)}
+            if p["steps"] <= 2:
+                two.add((p["steps"], some > 2, run))
+                two.add((p["steps"], some > 1))
+            else:
+                two.add((p["steps"], some > 4 if p["steps"] == 4 else some > 1, run))
+    both = (False, True)
+    assert one >= {(t, ng) for t in (2, 4, 8) for ng in (1, 2)} | {("wave", w) for w in both}
+    assert one >= {("together", t, w) for t in (2, 4, 8) for w in (0, 1)}
+    assert two >= {("at once", n) for n in (1, 2, 3)} | {(w, b) for w in ("turns", "wave", "windows") for b in both}
+    assert two >= {(steps, some, run) for steps in (1, 2, 4, 8) for some in both for run in both}
+    assert two >= {(steps, some) for steps in (1, 2) for some in both}
