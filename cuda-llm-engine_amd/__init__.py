@@ -934,7 +934,7 @@ def kv_copy_pages(pools, copies, count, n_copies: int, num_pages: int, stream=No
     pn = _opt(fn, count, torch.int32, 1, "count")
     ptrs, sizes = (_vp * max(1, len(pools)))(), (_sz * max(1, len(pools)))()
     for i, pool in enumerate(pools):
-        ptrs[i] = _dev(fn, pool, pool.dtype, 1, f"pools[{i}]")
+        ptrs[i] = _dev(fn, pool, getattr(pool, "dtype", None), 1, f"pools[{i}]")
         nbytes = pool.numel() * pool.element_size()
         if nbytes % num_pages:
             _fail(fn, f"pools[{i}] is not {num_pages} equal pages")
