@@ -2,6 +2,7 @@
 pages that run out."""
 import numpy as np
 import pytest
+import torch
 
 import _unlike as ref
 from test_gpu_pages import check_fork
@@ -64,3 +65,18 @@ def test_pages_run_out_in_a_large_cache(llmk, n, free):
     parents = np.sort(rng.integers(0, n, n + 40))
     want = check_fork(llmk, tables, lens, parents, np.full(n + 40, 200), refs, 16, num_pages)
     assert want[4][1] > 0 or free == 200
+
+
+@pytest.mark.parametrize("bytes_of_a_page", [16, 20])
+def test_many_pairs_in_many_pools(llmk, bytes_of_a_page):
+    """Pairs and pools whose blocks are counted before the first launch, as one might not take its own."""
+    n, num_pages, n_pools = 900000, 2000, 130
+    pools = [torch.randint(-9, 9, (num_pages, bytes_of_a_page // 4), dtype=torch.int32, device="cuda") for _ in range(n_pools)]
+    before = [p.clone() for p in pools]
+    pairs = torch.full((n, 2), -1, dtype=torch.int32, device="cuda")
+    for i, pair in ((0, (3, 7)), (n // 2, (1999, 0)), (n - 1, (5, 1200))):
+        pairs[i] = torch.tensor(pair)
+    llmk.kv_copy_pages(pools, pairs, None, n, num_pages)
+    for p, b in zip(pools, before):
+        b[7], b[0], b[1200] = b[3].clone(), b[1999].clone(), b[5].clone()
+        assert torch.equal(p, b)
