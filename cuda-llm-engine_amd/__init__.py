@@ -877,7 +877,8 @@ def qkv_rotary_scatter(qkv, ld: int, q_out, k_pool, v_pool, block_tables, positi
                        n_kv_heads: int, head_dim: int, rotary_dim: int, layout: int = 0, stream=None,
                        check_indices: bool | None = None) -> None:
     """The rotation of rotary_apply on the way from a fused projection's rows into the paged fp16 cache
-    (``llmk_qkv_rotary_scatter``). ``check_indices`` refuses rows that have no page of the pools."""
+    (``llmk_qkv_rotary_scatter``): rotary_dim a multiple of 16, or an even whole fraction of head_dim.
+    ``check_indices`` refuses rows that have no page of the pools."""
     fn = "qkv_rotary_scatter"
     if not _want_checks(check_indices):
         st = _fast.qkv_rotary_scatter(qkv, ld, q_out, k_pool, v_pool, block_tables, positions, inv_freq,
@@ -970,7 +971,7 @@ def kv_fork(block_tables, seq_lens, parents, reserve, refs, new_tables, new_lens
             stream=None, check_indices: bool | None = None) -> None:
     """The step from one batch to the next: children share their parents' whole pages, and pages that
     nobody holds any more are free (``llmk_kv_fork``; kv_copy_pages then makes the copies that it
-    names). ``check_indices`` refuses counts in refs that are not the block tables' holders."""
+    names). ``check_indices`` refuses refs that count fewer holders of a page than the block tables have."""
     fn = "kv_fork"
     if not _want_checks(check_indices):
         st = _fast.kv_fork(block_tables, seq_lens, parents, reserve, refs, new_tables, new_lens, copies,

@@ -8,11 +8,11 @@
 //
 // Measured (one MI355X, fp16, inputs from HBM; the floor is each byte once at 6 TB/s), us:
 //   1 row, rank 16, 2048 -> 2048: 5.1 (< 0.1). One launch: its loads one behind the other.
-//   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 10.4 (2.2). One launch; every block
+//   48 sequences of up to 5 rows, 16 adapters of rank 16, 4096 -> 4096|1024|1024: 10.5 (2.2). One launch; every block
 //     reads its tile's A and x again, from the L2: 8.9 where all of it is in the last-level cache.
-//   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 28.6 (12.6), 18 and 10. 61 MB by the first launch at 3.3
+//   256 rows of 100 adapters of ranks up to 64, 8192 -> 2048: 28.7 (12.6), 18 and 10. 61 MB by the first launch at 3.3
 //     TB/s: a tile's rows are found (2 us), then two rounds of loads that wait for one another.
-//   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.0 (27.7), 9 and 35. y in place by 16 rows of
+//   4 prompts of up to 1001 rows, ranks up to 32, 2048 -> 8192|8192: 42.1 (27.7), 9 and 35. y in place by 16 rows of
 //     256 bytes a wave, which alone take 30.
 //   3 prompts of 456 rows, rank 128, 8192 -> 11008|11008: 89 (30.6), 40 and 57. A and B from the L2 by every tile, 540
 //     MB for the first; two tiles a block halve that, but also the waves a SIMD, and take as long.
@@ -29,7 +29,8 @@
 // Between the products h is held in fp32 (the blocks of a tile that share out in_features leave a sum
 // each) and given to the matrix instructions as two fp16: h * 2^-e, with 2^e such that the row's largest
 // is from 2^14 to 2^15, rounded, and what that lost. That keeps 22 bits relative to the row's largest, and the sum
-// is multiplied by scale * 2^e in fp32. So neither large nor small values of h leave fp16's range.
+// is multiplied by scale * 2^e in fp32. So neither large nor small values of h leave fp16's range. Infinities of A and
+// B come out as the formula has them (expand_columns).
 #include <math.h>
 
 #include "kv8.hpp"

@@ -3,9 +3,13 @@
 // which blocks run: counts are added up, and every page number comes from a count of what lies in front.
 //
 // Copies are bound by bytes, tables by loads that wait for one another. Measured (one MI355X, inputs from HBM; the
-// floor is each byte once at 6 TB/s), us: the fork of 8 beams and its copies in 16 layers 9.3 (0.5), k_fork 6.6 and the
-// copies 3.2; of 256 beams over an 8-bit cache 25.0 (7.2), rows 4.0, holders 4.0, pages 5.6, copies 12.8 (43 MB); the
-// compaction of 64 sequences, half the pool free, 47.6 (37.5), 5.8 and the copies 41.6 (231 MB at 5.5 TB/s).
+// floor is each byte once at 6 TB/s), us: the fork of 8 beams and its copies in 16 layers 9.3 (0.5), k_fork 6.4 and the
+// copies 3.1; of 256 beams over an 8-bit cache 25.4 (7.2), rows 4.0, holders 3.6, pages 5.8, copies 13 (43 MB); the
+// compaction of 64 sequences, half the pool free, 47.6 (37.5), 5.8 and the copies 42 (231 MB at 5.5 TB/s). Larger pools:
+// a fork of 256 beams by tables of 129 pages 11.5 without its copies in 2200 pages and 12.4 in 16000, by 256 pages 14.1
+// in 64000; a compaction's tables in three launches, 16000 pages of 128 sequences 12.8, 250000 of 256 15.4.
+//
+// Between their launches forks and compactions trust the workspace with numbers and with no address (fork_notes.hpp).
 #include <limits.h>
 
 #include "common.hpp"

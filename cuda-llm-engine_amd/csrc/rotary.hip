@@ -12,9 +12,11 @@
 //
 // Bound by bytes, each once each way; a 64-bit cosine and sine take some 60 instructions a pair of a row, which is why
 // they are computed once a row for all its heads and while the data is on its way. Measured (one MI355X, inputs from
-// HBM, the floor at 6 TB/s), us: 1 row 2.1 (one launch); 4001 rows of 40 heads of 64 in place 10.4 (6.8: 41 MB at 3.9
-// TB/s, as an addition in place to as many bytes takes 9.9); 256 rows into the cache 3.6 (0.5); 2001 rows of 28 + 2 x 4
-// heads of 128 into the cache 10.2 (6.2: 37 MB, of which a plain copy takes 7).
+// HBM, the floor at 6 TB/s), us: 1 row 2.1 (one launch); 4001 rows of 40 heads of 64 in place 10.2 (6.8: 41 MB at 4
+// TB/s; not the memory's bound, as more units a thread take 9.5); 256 rows into the cache 3.6 (0.5); 2001 rows of 28 +
+// 2 x 4 heads of 128 into the cache 10.2 (6.2: 37 MB, of which a plain copy takes 7). What is no whole vectors is turned
+// pair by pair: 4001 rows of 40 heads of 64 with 24 elements turned take 11.9 (2.6), with all of them at odd addresses
+// 22.3 (6.8), one row 2.5.
 #include "angles.hpp"
 #include "layer_ops.hpp"
 #include "overlap.hpp"
@@ -236,8 +238,9 @@ int launch_rotary(RotaryArgs& a, int heads, int units, bool pairs, hipStream_t s
   if ((long long)heads * units > 0x7FFFFFFF / 64) return LLMK_ERR_UNSUPPORTED;
   a.per_row = heads * units;
   // as many rows as 256 threads take (at most 8, whose page numbers and angles they load); a wide row by blocks
-  // of up to 512. Four units a thread, and rows to match, took 9.5 us and not 10.4 for 4000 rows of 40 heads of 64,
-  // but 20.4 and not 18.2 for 8000, 5.2 and not 4.4 for 1000, 4.2 and not 2.7 for 256.
+  // of up to 512. In place one unit a thread: four, and rows to match, took 9.5 us and not 10.4 for 4000 rows of 40
+  // heads of 64, but 20.4 and not 18.2 for 8000, 5.2 and not 4.4 for 1000, 4.2 and not 2.7 for 256; between 1000 and
+  // 8000 rows it is not known where they begin and cease to win.
   const auto rows_of = [&](int units_of_block) {
     int rows = units_of_block / a.per_row;
     rows = rows < 1 ? 1 : rows > 8 ? 8 : rows;
