@@ -380,8 +380,8 @@ __global__ void __launch_bounds__(1024) k_fork_find(const ForkArgs a) {
   __shared__ Find f;
   fork_find<long long>(a, f);
 }
-// The three of them by one block, whose batches want at most 8192 pages. Its additions to counts are complete at the barrier and read where they were
-// made, so no fence of the device is needed, which takes 5 us.
+// The three of them by one block, whose batches want at most 8192 pages. Its additions to counts are complete at the
+// barrier and read where they were made, so no fence of the device is needed, which takes 5 us.
 __global__ void __launch_bounds__(1024) k_fork(const ForkArgs a) {
   __shared__ Find f;
   const int wave = threadIdx.x >> 6;
